@@ -522,6 +522,66 @@ int llmq_seed_step(const int64_t* token_src_or_null, int64_t* token_or_null, int
                    const void* embed_or_null, void* hidden_out_or_null, int row_bytes, int64_t vocab,
                    llmq_stream_t stream);
 
+/* The norm of every query and key head and the position rotation behind it, in one pass: for models that norm their
+ * heads (no counterpart in the reference, which leaves both to transformers). For each head x of head_dim elements
+ *   y = x * rsqrt(mean(x^2) + eps) * weight
+ *   z[i] = y[i] cos[i] - y[i + R/2] sin[i], z[i + R/2] = y[i + R/2] cos[i + R/2] + y[i] sin[i + R/2]   (i < R/2)
+ *   z[i] = y[i]                                                                                          (i >= R)
+ * in fp32, rounded to `dtype` once. R = rotary_dim: the width of cos_table and sin_table [table_rows, rotary_dim], which
+ * hold `dtype` or fp32 (table_dtype); token t takes their row positions[t] (int32 or int64 by position_bytes; NULL: row
+ * t). A position outside [0, table_rows) makes rows of NaN. q [tokens, q_heads * head_dim] and k [tokens, kv_heads *
+ * head_dim] with row strides in elements, q_out and k_out contiguous (they may not overlap q or k). head_dim and
+ * rotary_dim: multiples of 16 (8 for fp32), head_dim up to 256. All tensors 16-byte aligned. */
+int llmq_qk_norm_rope(const void* q, const void* k, const void* q_weight, const void* k_weight, const void* cos_table,
+                      const void* sin_table, const void* positions_or_null, int position_bytes, void* q_out, void* k_out,
+                      int tokens, int q_heads, int kv_heads, int head_dim, int rotary_dim, int table_rows,
+                      int64_t q_row_stride, int64_t k_row_stride, float eps, int dtype, int table_dtype,
+                      llmq_stream_t stream);
+
+/* A cache in blocks, one layer, for a batch of sequences. A block holds `block` (16, 32, 64 or 128) consecutive tokens of
+ * one sequence for every head, int8 codes under one fp32 scale for a block and head:
+ *   k_codes [n_blocks, kv_heads, block, head_dim]          v_codes [n_blocks, kv_heads, block / 16, head_dim, 16]
+ *   k_scale, v_scale [n_blocks, kv_heads]
+ * (value codes have 16 tokens innermost). block_table [sequences, table_width] int32, rows table_stride elements apart,
+ * names the blocks of each sequence in order; an entry outside [0, n_blocks) is no block. cached [sequences] int32: tokens
+ * a sequence holds before the call; negative: the sequence takes no part. The call's tokens are rows query_start[b] ..
+ * query_start[b + 1] - 1 of sequence b (int32 [sequences + 1], not decreasing; NULL: one row each, tokens == sequences), at
+ * positions cached[b] on. head_dim 64, 128 or 256; codes 16-byte aligned. The reference holds its quantized cache
+ * for one sequence at a time (llmquant/quantizers/fake.py:39-55).
+ *
+ * llmq_kv_block_append quantizes the call's rows (key, value [tokens, kv_heads, head_dim], row strides in elements) into
+ * the blocks, which no other sequence of the call may share. a = max |x| over the call's tokens in a block and head:
+ *   scale = max(a / 127, 1e-8) where the call writes the block's first token, else max(scale, that)
+ *   code = clamp(rint(x / scale), -128, 127); codes the block held before: clamp(rint((code * old scale) / scale))
+ * Tokens whose position has no block are left out; places behind a sequence's last token keep what they hold.
+ *
+ * llmq_kv_block_dequant reads tokens first[b] .. of sequence b (first NULL: 0) into columns starts[b] .. starts[b + 1] - 1
+ * of k_out and v_out [kv_heads, n_tokens, head_dim]: (dtype)(code * scale), zeros for a token without a block. Columns
+ * that no sequence has are not written. */
+int llmq_kv_block_append(const void* key, const void* value, int64_t key_row_stride, int64_t value_row_stride, void* k_codes,
+                         void* v_codes, float* k_scale, float* v_scale, const int32_t* block_table, int64_t table_stride,
+                         const int32_t* cached, const int32_t* query_start_or_null, int tokens, int sequences, int kv_heads,
+                         int head_dim, int block, int n_blocks, int table_width, int dtype, llmq_stream_t stream);
+int llmq_kv_block_dequant(const void* k_codes, const void* v_codes, const float* k_scale, const float* v_scale,
+                          const int32_t* block_table, int64_t table_stride, const int32_t* starts,
+                          const int32_t* first_or_null, void* k_out, void* v_out, int n_tokens, int sequences, int kv_heads,
+                          int head_dim, int block, int n_blocks, int table_width, int dtype, llmq_stream_t stream);
+
+/* Causal grouped-query attention of the call's rows over the cache in blocks, theirs included (call it behind
+ * llmq_kv_block_append with the same `cached` and query_start): row i of sequence b sees tokens 0 .. cached[b] + i,
+ *   out[row, h, :] = softmax(sm_scale * q[row, h, :] . k[j, h / (q_heads / kv_heads), :]) v
+ * q [tokens, q_heads, head_dim] (row stride in elements), out [tokens, q_heads * head_dim]. Tokens without a block are left
+ * out; a row that sees nothing (a sequence that takes no part among them) is zero; rows that no sequence has are not
+ * written. workspace: llmq_kv_block_attention_workspace_bytes(...) bytes, 16-byte aligned (NULL where that is 0), needs no
+ * clearing; calls that overlap in time need one each. */
+size_t llmq_kv_block_attention_workspace_bytes(int tokens, int sequences, int q_heads, int kv_heads, int head_dim, int block,
+                                               int table_width);
+int llmq_kv_block_attention(const void* query, int64_t q_row_stride, const void* k_codes, const void* v_codes,
+                            const float* k_scale, const float* v_scale, const int32_t* block_table, int64_t table_stride,
+                            const int32_t* cached, const int32_t* query_start_or_null, void* out, void* workspace,
+                            size_t workspace_bytes, float sm_scale, int tokens, int sequences, int q_heads, int kv_heads,
+                            int head_dim, int block, int n_blocks, int table_width, int dtype, llmq_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -377,6 +377,9 @@ int rope_kv_append_packets(const void* q, const void* k, const void* v, int64_t 
                            void* v_codes, float* k_scale, float* v_scale, void* dq_k_or_null, void* dq_v_or_null,
                            const int32_t* pos_dev, int tokens, int q_heads, int kv_heads, int head_dim, int t_max, int bits,
                            int dtype, hipStream_t s);
+// What the calls on a cache in blocks ask of their sizes (kv_blocks.hip); 0 or the error.
+int check_block_shape(int rows, int sequences, int kv_heads, int head_dim, int block, int blocks, int table_width,
+                      int64_t table_stride, int dtype);
 int gemv_batched_mfma_launch(const void* x, const void* qw, const float* ws, void* out, const int32_t* block_expert,
                              const int32_t* block_row0, const int32_t* block_rows, int n_blocks, int n_rows,
                              int n_experts, int N, int G, int out_group, int wformat, int dtype,

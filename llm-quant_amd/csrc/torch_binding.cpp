@@ -13,6 +13,7 @@
 #include <c10/hip/HIPStream.h>
 #include <hipblaslt/hipblaslt.h>
 
+#include <algorithm>
 #include <map>
 #include <mutex>
 #include <tuple>
@@ -1457,6 +1458,215 @@ at::Tensor prefill_attention(const at::Tensor& q, const at::Tensor& k, const at:
   return out;
 }
 
+// ---- a batch of sequences over a cache in blocks -------------------------------------------------------------------
+// A tensor's rows as the kernels take them: contiguous within a row, rows and base on 16-byte packets (else a copy).
+at::Tensor packet_rows(const at::Tensor& t) {
+  const int64_t packet = 16 / t.element_size();
+  int64_t inner = 1;
+  bool dense = reinterpret_cast<uintptr_t>(t.const_data_ptr()) % 16 == 0;
+  for (int64_t d = t.dim() - 1; d > 0; --d) {
+    dense = dense && (t.size(d) == 1 || t.stride(d) == inner);
+    inner *= t.size(d);
+  }
+  if (dense && (t.size(0) == 1 || (t.stride(0) % packet == 0 && t.stride(0) >= 0))) return t;
+  auto copy = t.contiguous();
+  return reinterpret_cast<uintptr_t>(copy.const_data_ptr()) % 16 == 0 ? copy : copy.clone();
+}
+int64_t row_stride(const at::Tensor& t) { return t.size(0) == 1 ? t.numel() : t.stride(0); }
+
+void check_int(int64_t value, const char* name) {
+  TORCH_CHECK(value >= 0 && value <= INT32_MAX, name, " is out of range: ", value);
+}
+
+struct BlockCache {
+  int blocks, heads, block, dim;
+};
+BlockCache block_cache(const at::Tensor& k_codes, const at::Tensor& v_codes, const at::Tensor& k_scale, const at::Tensor& v_scale) {
+  TORCH_CHECK(k_codes.is_cuda() && v_codes.is_cuda() && k_scale.is_cuda() && v_scale.is_cuda(), "the cache must be CUDA tensors");
+  for (const at::Tensor* t : {&v_codes, &k_scale, &v_scale})
+    TORCH_CHECK(t->device() == k_codes.device(), "the cache must lie on one device");
+  TORCH_CHECK(k_codes.dim() == 4 && k_codes.is_contiguous() && k_codes.scalar_type() == at::kChar,
+              "k_codes must be contiguous int8 [blocks, kv_heads, block, head_dim]");
+  const int64_t n = k_codes.size(0), heads = k_codes.size(1), block = k_codes.size(2), dim = k_codes.size(3);
+  TORCH_CHECK(v_codes.dim() == 5 && v_codes.is_contiguous() && v_codes.scalar_type() == at::kChar && v_codes.size(0) == n &&
+                  v_codes.size(1) == heads && v_codes.size(2) * 16 == block && v_codes.size(3) == dim && v_codes.size(4) == 16,
+              "v_codes must be contiguous int8 [blocks, kv_heads, block / 16, head_dim, 16] with the blocks, heads and head_dim of k_codes");
+  for (const at::Tensor* t : {&k_scale, &v_scale})
+    TORCH_CHECK(t->dim() == 2 && t->is_contiguous() && t->scalar_type() == at::kFloat && t->size(0) == n && t->size(1) == heads,
+                "the scales must be contiguous float32 [blocks, kv_heads]");
+  check_int(n, "the number of blocks");
+  check_int(heads, "kv_heads");
+  return {static_cast<int>(n), static_cast<int>(heads), static_cast<int>(block), static_cast<int>(dim)};
+}
+
+// int32 vector of a batch on the device of `like`
+at::Tensor batch_vector(const at::Tensor& t, int64_t n, const at::Tensor& like, const char* name) {
+  TORCH_CHECK(t.device() == like.device() && t.scalar_type() == at::kInt && t.dim() == 1 && t.size(0) == n, name,
+              " must be int32 [", n, "] on the cache's device");
+  return t.contiguous();
+}
+
+struct Batch {
+  at::Tensor table, cached, start;   // start: undefined for one row a sequence
+  int sequences, width;
+  int64_t table_stride;
+  const int32_t* start_or_null() const { return start.defined() ? start.const_data_ptr<int32_t>() : nullptr; }
+};
+at::Tensor check_table(const at::Tensor& block_table, const at::Tensor& like) {
+  TORCH_CHECK(block_table.device() == like.device() && block_table.scalar_type() == at::kInt && block_table.dim() == 2,
+              "block_table must be int32 [sequences, width] on the cache's device");
+  check_int(block_table.size(0), "the number of sequences");
+  check_int(block_table.size(1), "the width of block_table");
+  const bool rows = (block_table.size(1) <= 1 || block_table.stride(1) == 1) && block_table.stride(0) >= 0;
+  return rows ? block_table : block_table.contiguous();
+}
+Batch batch_of(const at::Tensor& block_table, const at::Tensor& cached, const c10::optional<at::Tensor>& query_start,
+               int64_t tokens, const at::Tensor& like) {
+  Batch b;
+  b.table = check_table(block_table, like);
+  const int64_t sequences = b.table.size(0);
+  b.cached = batch_vector(cached, sequences, like, "cached");
+  if (query_start.has_value()) b.start = batch_vector(*query_start, sequences + 1, like, "query_start");
+  else TORCH_CHECK(tokens == sequences, "without query_start a sequence has one row: ", tokens, " rows, ", sequences, " sequences");
+  b.sequences = static_cast<int>(sequences);
+  b.width = static_cast<int>(b.table.size(1));
+  b.table_stride = b.table.stride(0);
+  return b;
+}
+
+// q [tokens, q_heads * head_dim], k [tokens, kv_heads * head_dim], weights [head_dim], tables [rows, rotary_dim].
+std::tuple<at::Tensor, at::Tensor> qk_norm_rope(const at::Tensor& q, const at::Tensor& k, const at::Tensor& q_weight,
+                                                const at::Tensor& k_weight, const at::Tensor& cos, const at::Tensor& sin,
+                                                double eps, const c10::optional<at::Tensor>& positions) {
+  TORCH_CHECK(q.is_cuda() && k.is_cuda() && q_weight.is_cuda() && k_weight.is_cuda() && cos.is_cuda() && sin.is_cuda(),
+              "all tensors must be CUDA tensors");
+  for (const at::Tensor* t : {&k, &q_weight, &k_weight, &cos, &sin})
+    TORCH_CHECK(t->device() == q.device(), "all tensors must lie on one device");
+  const int dtype = dtype_code(q, "q");
+  TORCH_CHECK(k.scalar_type() == q.scalar_type() && q_weight.scalar_type() == q.scalar_type() && k_weight.scalar_type() == q.scalar_type(),
+              "k and the weights must have q's dtype");
+  TORCH_CHECK(q_weight.dim() == 1 && k_weight.sizes() == q_weight.sizes(), "the weights must be [head_dim]");
+  TORCH_CHECK(cos.dim() == 2 && cos.sizes() == sin.sizes() && cos.scalar_type() == sin.scalar_type() &&
+                  (cos.scalar_type() == q.scalar_type() || cos.scalar_type() == at::kFloat),
+              "cos and sin must be [rows, rotary_dim] of q's dtype or float32");
+  const int64_t dim = q_weight.size(0);
+  TORCH_CHECK(q.dim() == 2 && k.dim() == 2 && k.size(0) == q.size(0), "q and k must be [tokens, heads * head_dim]");
+  TORCH_CHECK(dim > 0 && q.size(1) % dim == 0 && k.size(1) % dim == 0, "the widths of q and k must be whole heads of ", dim);
+  const int64_t tokens = q.size(0), q_heads = q.size(1) / dim, kv_heads = k.size(1) / dim;
+  check_int(tokens, "the number of tokens");
+  check_int(std::max(q.size(1), k.size(1)), "the width of q or k");
+  check_int(cos.size(0), "the number of table rows");
+  at::Tensor at;
+  if (positions.has_value()) {
+    TORCH_CHECK(positions->device() == q.device() && positions->dim() == 1 && positions->size(0) == tokens &&
+                    (positions->scalar_type() == at::kInt || positions->scalar_type() == at::kLong),
+                "positions must be int32 or int64 [", tokens, "] on q's device");
+    at = positions->contiguous();
+  }
+  auto q_out = at::empty({tokens, q_heads, dim}, q.options());
+  auto k_out = at::empty({tokens, kv_heads, dim}, q.options());
+  const c10::OptionalDeviceGuard guard(at::device_of(q));
+  const auto qr = packet_rows(q), kr = packet_rows(k), qw = packet_rows(q_weight.reshape({1, dim})),
+             kw = packet_rows(k_weight.reshape({1, dim}));
+  const auto ct = packet_rows(cos.contiguous()), st = packet_rows(sin.contiguous());
+  check_rc(llmq_qk_norm_rope(qr.const_data_ptr(), kr.const_data_ptr(), qw.const_data_ptr(), kw.const_data_ptr(),
+                             ct.const_data_ptr(), st.const_data_ptr(), at.defined() ? at.const_data_ptr() : nullptr,
+                             at.defined() ? static_cast<int>(at.element_size()) : 0, q_out.mutable_data_ptr(),
+                             k_out.mutable_data_ptr(), static_cast<int>(tokens), static_cast<int>(q_heads),
+                             static_cast<int>(kv_heads), static_cast<int>(dim), static_cast<int>(ct.size(1)),
+                             static_cast<int>(ct.size(0)), row_stride(qr), row_stride(kr), static_cast<float>(eps), dtype,
+                             dtype_code(ct, "cos"), current_stream(q)),
+           "qk_norm_rope");
+  return {q_out, k_out};
+}
+
+// key, value [tokens, kv_heads, head_dim] into the blocks of their sequences.
+void kv_block_append(const at::Tensor& key, const at::Tensor& value, at::Tensor& k_codes, at::Tensor& v_codes,
+                     at::Tensor& k_scale, at::Tensor& v_scale, const at::Tensor& block_table, const at::Tensor& cached,
+                     const c10::optional<at::Tensor>& query_start) {
+  const BlockCache c = block_cache(k_codes, v_codes, k_scale, v_scale);
+  TORCH_CHECK(key.device() == k_codes.device() && value.device() == k_codes.device(), "key and value must lie on the cache's device");
+  const int dtype = dtype_code(key, "key");
+  TORCH_CHECK(key.dim() == 3 && value.sizes() == key.sizes() && value.scalar_type() == key.scalar_type() &&
+                  key.size(1) == c.heads && key.size(2) == c.dim,
+              "key and value must be [tokens, ", c.heads, ", ", c.dim, "] of one dtype");
+  check_int(key.size(0), "the number of tokens");
+  const Batch b = batch_of(block_table, cached, query_start, key.size(0), k_codes);
+  const c10::OptionalDeviceGuard guard(at::device_of(key));
+  const auto kr = packet_rows(key), vr = packet_rows(value);
+  check_rc(llmq_kv_block_append(kr.const_data_ptr(), vr.const_data_ptr(), row_stride(kr), row_stride(vr),
+                                k_codes.mutable_data_ptr(), v_codes.mutable_data_ptr(), k_scale.mutable_data_ptr<float>(),
+                                v_scale.mutable_data_ptr<float>(), b.table.const_data_ptr<int32_t>(), b.table_stride,
+                                b.cached.const_data_ptr<int32_t>(), b.start_or_null(), static_cast<int>(key.size(0)),
+                                b.sequences, c.heads, c.dim, c.block, c.blocks, b.width, dtype, current_stream(key)),
+           "kv_block_append");
+}
+
+// (keys, values) [kv_heads, n_tokens, head_dim]: tokens first[b] .. of sequence b in columns starts[b] .. starts[b + 1] - 1.
+std::tuple<at::Tensor, at::Tensor> kv_block_dequant(const at::Tensor& k_codes, const at::Tensor& v_codes,
+                                                    const at::Tensor& k_scale, const at::Tensor& v_scale,
+                                                    const at::Tensor& block_table, const at::Tensor& starts, int64_t n_tokens,
+                                                    at::ScalarType out_dtype, const c10::optional<at::Tensor>& first) {
+  const BlockCache c = block_cache(k_codes, v_codes, k_scale, v_scale);
+  check_int(n_tokens, "n_tokens");
+  const auto table = check_table(block_table, k_codes);
+  const int64_t sequences = table.size(0);
+  const auto from = batch_vector(starts, sequences + 1, k_codes, "starts");
+  at::Tensor begin;
+  if (first.has_value()) begin = batch_vector(*first, sequences, k_codes, "first");
+  const c10::OptionalDeviceGuard guard(at::device_of(k_codes));
+  auto k_out = at::empty({c.heads, n_tokens, c.dim}, k_codes.options().dtype(out_dtype));
+  auto v_out = at::empty({c.heads, n_tokens, c.dim}, k_codes.options().dtype(out_dtype));
+  check_rc(llmq_kv_block_dequant(k_codes.const_data_ptr(), v_codes.const_data_ptr(), k_scale.const_data_ptr<float>(),
+                                 v_scale.const_data_ptr<float>(), table.const_data_ptr<int32_t>(), table.stride(0),
+                                 from.const_data_ptr<int32_t>(), begin.defined() ? begin.const_data_ptr<int32_t>() : nullptr,
+                                 k_out.mutable_data_ptr(), v_out.mutable_data_ptr(), static_cast<int>(n_tokens),
+                                 static_cast<int>(sequences), c.heads, c.dim, c.block, c.blocks,
+                                 static_cast<int>(table.size(1)), dtype_code(k_out, "output dtype"), current_stream(k_codes)),
+           "kv_block_dequant");
+  return {k_out, v_out};
+}
+
+// query [tokens, q_heads, head_dim] -> [tokens, q_heads * head_dim].
+at::Tensor kv_block_attention(const at::Tensor& query, const at::Tensor& k_codes, const at::Tensor& v_codes,
+                              const at::Tensor& k_scale, const at::Tensor& v_scale, const at::Tensor& block_table,
+                              const at::Tensor& cached, double sm_scale, const c10::optional<at::Tensor>& query_start,
+                              const c10::optional<at::Tensor>& out) {
+  const BlockCache c = block_cache(k_codes, v_codes, k_scale, v_scale);
+  TORCH_CHECK(query.device() == k_codes.device(), "query must lie on the cache's device");
+  const int dtype = dtype_code(query, "query");
+  TORCH_CHECK(query.dim() == 3 && query.size(2) == c.dim, "query must be [tokens, q_heads, ", c.dim, "]");
+  const int64_t tokens = query.size(0), q_heads = query.size(1);
+  check_int(tokens, "the number of tokens");
+  check_int(q_heads * c.dim, "the width of query");
+  const Batch b = batch_of(block_table, cached, query_start, tokens, k_codes);
+  const c10::OptionalDeviceGuard guard(at::device_of(query));
+  at::Tensor result;
+  if (out.has_value()) {
+    TORCH_CHECK(out->device() == query.device() && out->scalar_type() == query.scalar_type() && out->is_contiguous() &&
+                    out->dim() == 2 && out->size(0) == tokens && out->size(1) == q_heads * c.dim &&
+                    reinterpret_cast<uintptr_t>(out->const_data_ptr()) % 16 == 0,
+                "out must be contiguous [", tokens, ", ", q_heads * c.dim, "] of query's dtype, 16-byte aligned");
+    result = *out;
+  } else {
+    result = at::empty({tokens, q_heads * c.dim}, query.options());
+  }
+  const auto qr = packet_rows(query);
+  const size_t need = llmq_kv_block_attention_workspace_bytes(static_cast<int>(tokens), b.sequences, static_cast<int>(q_heads),
+                                                              c.heads, c.dim, c.block, b.width);
+  at::Tensor workspace;
+  if (need) workspace = at::empty({static_cast<int64_t>(need)}, query.options().dtype(at::kByte));
+  check_rc(llmq_kv_block_attention(qr.const_data_ptr(), row_stride(qr), k_codes.const_data_ptr(), v_codes.const_data_ptr(),
+                                   k_scale.const_data_ptr<float>(), v_scale.const_data_ptr<float>(),
+                                   b.table.const_data_ptr<int32_t>(), b.table_stride, b.cached.const_data_ptr<int32_t>(),
+                                   b.start_or_null(), result.mutable_data_ptr(), need ? workspace.mutable_data_ptr() : nullptr,
+                                   need, static_cast<float>(sm_scale), static_cast<int>(tokens), b.sequences,
+                                   static_cast<int>(q_heads), c.heads, c.dim, c.block, c.blocks, b.width, dtype,
+                                   current_stream(query)),
+           "kv_block_attention");
+  return result;
+}
+
 // argmax_advance over 32 workgroups, and the winner's row of the embedding table copied to hidden_out (both or
 // neither of embed / hidden_out). workspace: int32 zeros of argmax_workspace_ints() elements, kept by the caller.
 at::Tensor argmax_advance_embed(const at::Tensor& x, at::Tensor& token, at::Tensor& step64, at::Tensor& step32,
@@ -1706,6 +1916,22 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         py::arg("out_dtype") = at::kBFloat16);
   m.def("prefill_attention", &prefill_attention, "causal grouped-query attention of a prompt on the matrix core",
         py::arg("q"), py::arg("k"), py::arg("v"), py::arg("scale"));
+  m.def("qk_norm_rope", &qk_norm_rope,
+        "RMS norm of every query and key head and the position rotation behind it, one launch, rounded once",
+        py::arg("q"), py::arg("k"), py::arg("q_weight"), py::arg("k_weight"), py::arg("cos"), py::arg("sin"), py::arg("eps"),
+        py::arg("positions") = py::none());
+  m.def("kv_block_append", &kv_block_append,
+        "Quantize a batch's new K/V rows into the blocks of their sequences, one scale for a block and head",
+        py::arg("key"), py::arg("value"), py::arg("k_codes"), py::arg("v_codes"), py::arg("k_scale"), py::arg("v_scale"),
+        py::arg("block_table"), py::arg("cached"), py::arg("query_start") = py::none());
+  m.def("kv_block_dequant", &kv_block_dequant, "Dequantize tokens of a batch's sequences from their blocks",
+        py::arg("k_codes"), py::arg("v_codes"), py::arg("k_scale"), py::arg("v_scale"), py::arg("block_table"),
+        py::arg("starts"), py::arg("n_tokens"), py::arg("out_dtype"), py::arg("first") = py::none());
+  m.def("kv_block_attention", &kv_block_attention,
+        "Causal GQA attention of a batch's rows over the cache in blocks, theirs included",
+        py::arg("query"), py::arg("k_codes"), py::arg("v_codes"), py::arg("k_scale"), py::arg("v_scale"),
+        py::arg("block_table"), py::arg("cached"), py::arg("sm_scale"), py::arg("query_start") = py::none(),
+        py::arg("out") = py::none());
   m.def("argmax_advance_embed", &argmax_advance_embed,
         "argmax_advance over 32 workgroups; with embed / hidden_out also hidden_out <- embed[index]", py::arg("x"),
         py::arg("token"), py::arg("step64"), py::arg("step32"), py::arg("embed") = py::none(),

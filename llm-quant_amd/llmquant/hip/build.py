@@ -190,6 +190,17 @@ def load_capi() -> ctypes.CDLL:
     lib.llmq_wq_gemv_batched_max_rows.restype = c_int
     lib.llmq_dequant_weight.argtypes = [c_p, c_p, c_p] + [c_int] * 7 + [c_p]
     lib.llmq_dequant_weight.restype = c_int
+    lib.llmq_qk_norm_rope.argtypes = [c_p] * 7 + [c_int] + [c_p] * 2 + [c_int] * 6 + [c_i64] * 2 + [c_f] + [c_int] * 2 + [c_p]
+    lib.llmq_qk_norm_rope.restype = c_int
+    lib.llmq_kv_block_append.argtypes = ([c_p] * 2 + [c_i64] * 2 + [c_p] * 5 + [c_i64] + [c_p] * 2 + [c_int] * 8 + [c_p])
+    lib.llmq_kv_block_append.restype = c_int
+    lib.llmq_kv_block_dequant.argtypes = [c_p] * 5 + [c_i64] + [c_p] * 4 + [c_int] * 8 + [c_p]
+    lib.llmq_kv_block_dequant.restype = c_int
+    lib.llmq_kv_block_attention_workspace_bytes.argtypes = [c_int] * 7
+    lib.llmq_kv_block_attention_workspace_bytes.restype = ctypes.c_size_t
+    lib.llmq_kv_block_attention.argtypes = ([c_p, c_i64] + [c_p] * 5 + [c_i64] + [c_p] * 4 + [ctypes.c_size_t, c_f]
+                                            + [c_int] * 9 + [c_p])
+    lib.llmq_kv_block_attention.restype = c_int
     for name in ("llmq_fake_quant_group", "llmq_quant_group_codes", "llmq_wq_gemv", "llmq_kv_append",
                  "llmq_kv_dequant", "llmq_kv_decode_attention"):
         getattr(lib, name).restype = c_int

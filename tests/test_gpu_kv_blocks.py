@@ -1,0 +1,478 @@
+"""The batch's operators over a cache in blocks (qk_norm_rope, kv_block_append, kv_block_dequant, kv_block_attention)
+against their formulas in 64 bits, or, where every rounding is fixed, bit for bit.
+
+Tolerances are bounds by arithmetic: half a step of the output's type, and what the kernels' roundings on the way can
+add up to (given at each test)."""
+
+import numpy as np
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+DTYPES = [torch.bfloat16, torch.float16, torch.float32]
+TAGS = {torch.bfloat16: "bf16", torch.float16: "f16", torch.float32: "f32"}
+U32 = 2.0 ** -24   # half a step of fp32
+
+
+@pytest.fixture(scope="module")
+def ext():
+    from llmquant.hip import load_extension
+
+    return load_extension()
+
+
+def half_step(dtype, want):
+    """Half a step of `dtype` at the values `want` (its smallest subnormals included)."""
+    info = torch.finfo(dtype)
+    return torch.clamp(want.abs() * (info.eps / 2), min=info.tiny * info.eps / 2)
+
+
+# ---- the norm of heads and the rotation ------------------------------------------------------------------------------
+def norm_rope64(x, weight, cos, sin, eps):
+    """x [tokens, heads, D] and cos, sin [tokens, R] in 64 bits -> (result, sum of the magnitudes that make an element)."""
+    y = x * torch.rsqrt(x.square().mean(-1, keepdim=True) + eps) * weight
+    half = cos.shape[-1] // 2
+    cos, sin = cos[:, None], sin[:, None]
+    turned = torch.cat([-y[..., half:2 * half], y[..., :half]], -1)
+    out, size = y.clone(), y.abs()
+    out[..., :2 * half] = y[..., :2 * half] * cos + turned * sin
+    size[..., :2 * half] = (y[..., :2 * half] * cos).abs() + (turned * sin).abs()
+    return out, size
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=TAGS.get)
+@pytest.mark.parametrize("tokens,q_heads,kv_heads,dim,rotary,wide,kind", [
+    (1, 32, 8, 128, 128, False, "int32"), (1, 4, 4, 64, 64, True, "none"), (7, 6, 2, 128, 64, True, "int64"),
+    (33, 5, 1, 256, 256, False, "int32"), (3, 7, 0, 96, 96, True, "int32"), (65, 3, 3, 80, 32, False, "int64"),
+    (5, 0, 2, 16, 16, True, "none"), (257, 28, 4, 128, 128, True, "int32"), (2, 1, 1, 240, 48, False, "int32")])
+def test_norm_and_rotation(ext, dtype, tokens, q_heads, kv_heads, dim, rotary, wide, kind):
+    g = torch.Generator().manual_seed(tokens * dim)
+    rows, eps = 300, 1e-6
+    # queries and keys as column blocks of wider rows; a head of zeros, a very small and a very large one among them
+    flat = torch.randn(tokens, (q_heads + kv_heads + 2) * dim, generator=g) * 2
+    flat[0, :dim] = 0.0
+    flat[-1, dim:2 * dim] *= 1e-4
+    flat[-1, -dim * 2:] *= 100.0
+    flat = flat.to(dtype).cuda()
+    q, k = flat[:, dim:(1 + q_heads) * dim], flat[:, (1 + q_heads) * dim:(1 + q_heads + kv_heads) * dim]
+    qw, kw = ((1 + torch.randn(dim, generator=g)).to(dtype).cuda() for _ in range(2))
+    angle = torch.arange(rows, dtype=torch.float64)[:, None] * (100.0 ** (-torch.arange(0, rotary, 2, dtype=torch.float64) / rotary))
+    # (the two halves of a row need not be alike: the formula takes each element's own)
+    table = torch.float32 if wide else dtype
+    cos, sin = torch.cat([angle.cos(), angle.cos() * 0.5], -1).to(table).cuda(), torch.cat([angle.sin(), angle.sin() + 0.1], -1).to(table).cuda()
+    position = None if kind == "none" else torch.randint(0, rows, (tokens,), generator=g).to(getattr(torch, kind)).cuda()
+    got = ext.qk_norm_rope(q, k, qw, kw, cos, sin, eps, position)
+    at = torch.arange(tokens, device="cuda") if position is None else position.long()
+    for out, x, w, heads in zip(got, (q, k), (qw, kw), (q_heads, kv_heads)):
+        assert out.shape == (tokens, heads, dim) and out.dtype == dtype and out.is_contiguous()
+        want, size = norm_rope64(x.double().reshape(tokens, heads, dim), w.double(), cos[at].double(), sin[at].double(), eps)
+        # fp32 on the way: a sum of squares (at most 16 + 5 roundings in a row, halved by the root), the mean, the root, the
+        # reciprocal, two products (5), a product and a multiply-add (2): below 20 half steps of what is added up
+        assert torch.all((out.double() - want).abs() <= half_step(dtype, want) + 20 * U32 * size)
+
+
+def test_norm_of_positions_outside_the_tables(ext):
+    q, w = torch.randn(5, 128, device="cuda"), torch.ones(64, device="cuda")
+    table = torch.ones(4, 32, device="cuda")
+    position = torch.tensor([0, -1, 3, 4, 2 ** 31 - 1], dtype=torch.int32, device="cuda")
+    for where in (position, position.long() * 2 ** 20):
+        known = ((where >= 0) & (where < 4)).cpu()
+        for out in ext.qk_norm_rope(q, q, w, w, table, table, 1e-5, where):
+            nan = out.isnan().cpu()
+            assert torch.equal(nan.all(-1).all(-1), ~known) and torch.equal(nan.any(-1).any(-1), ~known)
+
+
+def test_norm_takes_odd_layouts(ext):
+    """Rows that are not 16-byte aligned, transposed and expanded tensors: copied, same bits."""
+    g = torch.Generator(device="cuda").manual_seed(3)
+    base = torch.randn(6, 4 * 64 + 1, generator=g, device="cuda", dtype=torch.float16)
+    w, table = torch.ones(64, device="cuda", dtype=torch.float16), torch.rand(6, 64, generator=g, device="cuda")
+    plain = ext.qk_norm_rope(base[:, 1:].contiguous(), base[:, 1:129].contiguous(), w, w, table, table, 1e-5)
+    odd = ext.qk_norm_rope(base[:, 1:], base[:, 1:129], w, w, table, table, 1e-5)
+    turned = ext.qk_norm_rope(base[:, 1:].t().contiguous().t(), base[:, 1:129], w[:1].expand(64), w, table.t().contiguous().t(), table, 1e-5)
+    same = ext.qk_norm_rope(base[:1, 1:].expand(6, -1), base[:, 1:129], w, w, table[:1].expand(6, -1), table[:1].expand(6, -1), 1e-5)
+    assert all(torch.equal(a, b) for a, b in zip(plain * 2, odd + turned))
+    assert torch.equal(same[0], same[0][:1].expand(6, -1, -1))
+
+
+# ---- a batch's cache ---------------------------------------------------------------------------------------------------
+def make_cache(g, blocks, heads, block, dim, outliers=True):
+    """Codes and scales of any values, on the CPU; scales far from each other from block to block."""
+    k = torch.randint(-127, 128, (blocks, heads, block, dim), generator=g, dtype=torch.int8)
+    v = torch.randint(-127, 128, (blocks, heads, block // 16, dim, 16), generator=g, dtype=torch.int8)
+    ks, vs = (torch.exp(0.5 * torch.randn(blocks, heads, generator=g)) / 60 for _ in range(2))
+    if outliers and blocks > 2:
+        vs[1] *= 1e4   # one block's values are far above the others', another's far below
+        vs[2] *= 1e-5
+    return [k, v, ks, vs]
+
+
+def make_table(g, counts, blocks, spare=1):
+    """Blocks for sequences of `counts` blocks each, in any order; entries behind them name no block."""
+    order = torch.randperm(blocks, generator=g, dtype=torch.int64).tolist()
+    table = torch.full((len(counts), max(counts) + spare), -1, dtype=torch.int32)
+    for b, n in enumerate(counts):
+        table[b, :n] = torch.tensor(order[:n], dtype=torch.int32)
+        order = order[n:]
+    return table
+
+
+def starts_of(new):
+    return torch.tensor(np.concatenate([[0], np.cumsum(new)]), dtype=torch.int32)
+
+
+def rows_first(v):
+    """Value codes [.., block / 16, D, 16] as [.., block, D]."""
+    return np.ascontiguousarray(np.swapaxes(v, -1, -2)).reshape(*v.shape[:-3], -1, v.shape[-2])
+
+
+def append_oracle(x, codes, scale, table, cached, start, block):
+    """fp32 with every rounding in its place; x [tokens, heads, D], codes [blocks, heads, block, D] (changed)."""
+    f = np.float32
+    for b in range(len(cached)):
+        n, c = int(start[b + 1] - start[b]), int(cached[b])
+        if c < 0:
+            continue
+        for logical in range(c // block, (c + n - 1) // block + 1 if n else 0):
+            id = table[b, logical] if logical < table.shape[1] else -1
+            if not 0 <= id < len(codes):
+                continue
+            lo, hi = max(c, logical * block), min(c + n, (logical + 1) * block)
+            rows = x[start[b] + lo - c:start[b] + hi - c].astype(f)       # [new, heads, D]
+            s = np.maximum(np.abs(rows).max((0, 2)) / f(127), f(1e-8))
+            old = lo - logical * block
+            if old:
+                before = scale[id].copy()
+                s = np.maximum(s, before)
+                moved = np.clip(np.rint(codes[id, :, :old].astype(f) * before[:, None, None] / s[:, None, None]), -128, 127)
+                codes[id, :, :old] = np.where((s > before)[:, None, None], moved, codes[id, :, :old]).astype(np.int8)
+            scale[id] = s
+            codes[id, :, old:hi - logical * block] = np.clip(np.rint(rows.transpose(1, 0, 2) / s[:, None, None]), -128, 127).astype(np.int8)
+
+
+APPENDS = [  # block, D, heads, cached, new (None: a row each)
+    (64, 64, 2, [0], None), (64, 128, 1, [0, 1, 63, 64, 65, -1, 640], None), (16, 64, 8, [15, 16, 17, 31, 0], None),
+    (128, 256, 3, [127, 128, 5], None), (32, 128, 4, [0, 31, 40, -1, 7], [100, 1, 0, 9, 33]), (64, 64, 1, [0], [64]),
+    (16, 256, 2, [3, 0, 16], [200, 16, 15]), (128, 64, 5, [100, 0], [27, 300]), (64, 128, 2, [10] * 70, [3] * 70),
+    (64, 128, 1, [70] * 130, None), (32, 64, 3, [0, 0, 0], [0, 0, 5]), (128, 128, 2, [130], [1]), (16, 128, 1, [0, -1], [1, 0])]
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=TAGS.get)
+@pytest.mark.parametrize("block,dim,heads,cached,new", APPENDS)
+def test_append_bit_for_bit(ext, dtype, block, dim, heads, cached, new):
+    """Every code and scale of the cache, those that the call must leave alone too."""
+    counts = [(max(c, 0) + n - 1) // block + 1 for c, n in zip(cached, new or [1] * len(cached))]
+    g = torch.Generator().manual_seed(sum(counts) + dim)
+    blocks = sum(counts) + 3
+    cache, table = make_cache(g, blocks, heads, block, dim, outliers=False), make_table(g, counts, blocks)
+    start = starts_of(new or [1] * len(cached))
+    rows = torch.randn(int(start[-1]), 2, heads, dim, generator=g) * torch.exp(torch.randn(int(start[-1]), 2, heads, 1, generator=g))
+    if len(rows) > 1:
+        rows[1, :, 0] = 0.0     # a token of zeros
+    rows = rows.to(dtype)
+    cache[2][table[0, 0], 0] = float("nan") if cached[0] == 0 else 1e-3   # (a new block's old scale does not count)
+    want_k, want_ks = cache[0].numpy().copy(), cache[2].numpy().copy()
+    want_v, want_vs = rows_first(cache[1].numpy()), cache[3].numpy().copy()
+    append_oracle(rows[:, 0].float().numpy(), want_k, want_ks, table.numpy(), cached, start.numpy(), block)
+    append_oracle(rows[:, 1].float().numpy(), want_v, want_vs, table.numpy(), cached, start.numpy(), block)
+    on_gpu = [t.cuda() for t in cache]
+    side = rows.cuda()   # keys and values as slices of one tensor
+    args = (side[:, 0], side[:, 1], *on_gpu, table.cuda(), torch.tensor(cached, dtype=torch.int32, device="cuda"),
+            None if new is None else start.cuda())
+    ext.kv_block_append(*args)
+    for _ in range(2):
+        k, v, ks, vs = (t.cpu().numpy() for t in on_gpu)
+        np.testing.assert_array_equal(ks, want_ks)
+        np.testing.assert_array_equal(vs, want_vs)
+        np.testing.assert_array_equal(k, want_k)
+        np.testing.assert_array_equal(rows_first(v), want_v)
+        ext.kv_block_append(*args)   # the same rows at the same places again change nothing
+
+
+def test_append_token_by_token_stays_within_its_steps(ext):
+    """A block that is filled one token at a time: half a step of the last scale for each time that it grew, and half."""
+    g = torch.Generator().manual_seed(5)
+    block, dim, heads = 64, 128, 2
+    cache, table = [t.cuda() for t in make_cache(g, 2, heads, block, dim)], torch.tensor([[1]], dtype=torch.int32, device="cuda")
+    rows = (torch.randn(block, heads, dim, generator=g) * torch.exp(torch.randn(block, heads, 1, generator=g))).cuda()
+    grew = torch.zeros(heads, dtype=torch.int64)
+    for t in range(block):
+        before = cache[2][1].cpu()
+        ext.kv_block_append(rows[t:t + 1], rows[t:t + 1], *cache, table, torch.tensor([t], dtype=torch.int32, device="cuda"))
+        grew += cache[2][1].cpu() > before if t else 1
+    largest = rows.abs().amax((0, 2)).cpu()
+    assert torch.equal(cache[2][1].cpu(), largest / 127)
+    for codes in (cache[0][1].cpu().double(), torch.from_numpy(rows_first(cache[1][1].cpu().numpy())).double()):
+        off = (codes * cache[2][1].cpu()[:, None, None].double() - rows.cpu().double().transpose(0, 1)).abs().amax((1, 2))
+        assert torch.all(off <= 0.5 * grew * cache[2][1].cpu().double() * (1 + 1e-5)) and int(grew.max()) < 12
+
+
+def test_append_leaves_out_tokens_without_a_block(ext):
+    g = torch.Generator().manual_seed(9)
+    block, dim, heads = 16, 64, 2
+    cache = make_cache(g, 3, heads, block, dim)
+    # beyond the table, no block, an id above the cache's, in the first and in the middle sequence
+    table = torch.tensor([[0, -1], [3, 1], [2, 2 ** 31 - 1]], dtype=torch.int32)
+    cached, start = [10, 0, 20], starts_of([30, 20, 20])
+    rows = torch.randn(70, heads, dim, generator=g)
+    want_k, want_ks = cache[0].numpy().copy(), cache[2].numpy().copy()
+    append_oracle(rows.numpy(), want_k, want_ks, table.numpy(), cached, start.numpy(), block)
+    on_gpu = [t.cuda() for t in cache]
+    ext.kv_block_append(rows.cuda(), rows.cuda(), *on_gpu, table.cuda(), torch.tensor(cached, dtype=torch.int32, device="cuda"), start.cuda())
+    np.testing.assert_array_equal(on_gpu[0].cpu().numpy(), want_k)
+    np.testing.assert_array_equal(on_gpu[2].cpu().numpy(), want_ks)
+    # positions near the end of 32 bits, more rows than the starts name, fewer sequences than a table's
+    far = torch.tensor([2 ** 31 - 1, 2 ** 31 - 8, -2 ** 31], dtype=torch.int32, device="cuda")
+    held = [t.clone() for t in on_gpu]
+    ext.kv_block_append(rows.cuda(), rows.cuda(), *on_gpu, table.cuda(), far, start.cuda())
+    assert all(torch.equal(a, b) for a, b in zip(held, on_gpu))
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=TAGS.get)
+@pytest.mark.parametrize("block,dim,heads,first,count", [
+    (64, 64, 2, None, [1]), (64, 128, 1, None, [64, 0, 65, 200]), (16, 64, 3, [5, 16, 0], [1, 40, 16]),
+    (32, 256, 2, [31, 0], [2, 33]), (128, 128, 4, [100, 128, 7], [29, 127, 300]), (128, 64, 1, None, [3] * 70)])
+def test_dequant_is_the_product_rounded(ext, dtype, block, dim, heads, first, count):
+    g = torch.Generator().manual_seed(dim + sum(count))
+    begin = first or [0] * len(count)
+    counts = [max((f + n - 1) // block + 1, 1) for f, n in zip(begin, count)]
+    blocks = sum(counts) + 1
+    cache, table = make_cache(g, blocks, heads, block, dim), make_table(g, counts, blocks)
+    table[-1, 0] = blocks   # no block: zeros
+    tokens = sum(count)
+    on_gpu = [t.cuda() for t in cache]
+    got = ext.kv_block_dequant(*on_gpu, table.cuda(), starts_of(count).cuda(), tokens, dtype,
+                               None if first is None else torch.tensor(first, dtype=torch.int32, device="cuda"))
+    flat = [cache[0], torch.from_numpy(rows_first(cache[1].numpy()))]
+    for out, codes, scale in zip(got, flat, cache[2:]):
+        want = torch.zeros(heads, tokens, dim)
+        at = 0
+        for b, n in enumerate(count):
+            for p in range(begin[b], begin[b] + n):
+                id = int(table[b, p // block])
+                if 0 <= id < blocks:
+                    want[:, at] = codes[id, :, p % block].float() * scale[id][:, None]
+                at += 1
+        assert out.shape == want.shape and torch.equal(out.cpu(), want.to(dtype))
+
+
+# ---- attention -----------------------------------------------------------------------------------------------------------
+def attention64(q, cache, table, cached, start, block, scale, bias, weight_step):
+    """(result, bound of what the kernel's roundings on the way can add), both [tokens, q_heads, D] in 64 bits, NaN in
+    rows of no sequence. Roundings: the scores' sums of D products of a query and a code (the code may enter with `bias`, which
+    is taken out again); queries as 11-bit pieces below their row's largest; softmax weights as numbers of `weight_step`,
+    at the least 2^-25 of the row's largest; and a handful of fp32 operations on each weight and sum."""
+    tokens, q_heads, dim = q.shape
+    keys, values = cache[0].double() * cache[2].double()[..., None, None], torch.from_numpy(rows_first(cache[1].numpy())).double() * cache[3].double()[..., None, None]
+    heads = keys.shape[1]
+    out, bound = torch.full(q.shape, float("nan"), dtype=torch.float64), torch.zeros(q.shape, dtype=torch.float64)
+    for b in range(len(cached)):
+        for i in range(int(start[b + 1] - start[b])):
+            row, limit = int(start[b]) + i, int(cached[b]) + i + 1 if cached[b] >= 0 else 0
+            at = [(int(table[b, p // block]), p % block) for p in range(min(limit, table.shape[1] * block)) if 0 <= int(table[b, p // block]) < len(keys)]
+            out[row] = 0.0
+            if not at:
+                continue
+            ids, slots = (torch.tensor(t) for t in zip(*at))
+            for h in range(q_heads):
+                k, v, x = keys[ids, h * heads // q_heads, slots], values[ids, h * heads // q_heads, slots], q[row, h].double()
+                step = cache[2][ids, h * heads // q_heads].double()
+                t = scale * (k @ x)
+                p = torch.softmax(t, 0)
+                out[row, h] = p @ v
+                x_off = (2.0 ** -22 * x.abs() if weight_step < 2.0 ** -12 else 0.0) + 2.0 ** -25 * x.abs().max()
+                off = abs(scale) * (k.abs() @ (x_off + torch.zeros(dim, dtype=torch.float64)) + U32 * (dim + 8) * ((k.abs() + bias * step[:, None]) @ x.abs()))
+                off = off + 4 * U32 * (t.abs() + (t.abs().max()) + 24)       # the exponent's own roundings
+                rel = weight_step + 2 * float(off.max()) + 40 * U32 + len(at) * U32
+                weighted = p * cache[3][ids, h * heads // q_heads].double()
+                bound[row, h] = rel * (p @ v.abs()) + len(at) * 2.0 ** -25 * (1 if weight_step > 2.0 ** -12 else 2.0 ** -11) * 127 * weighted.max()
+    return out, bound
+
+
+def check_attention(ext, dtype, block, dim, heads, group, cached, new, seed=0, table=None, out=None, rows=None, scale=None, adjust=None):
+    g = torch.Generator().manual_seed(seed + dim * block + sum(cached))
+    count = new or [1] * len(cached)
+    counts = [max((max(c, 0) + n - 1) // block + 1, 1) for c, n in zip(cached, count)]
+    blocks = sum(counts) + 2 if table is None else 9
+    cache = make_cache(g, blocks, heads, block, dim)
+    table = make_table(g, counts, blocks) if table is None else table
+    start = starts_of(count)
+    q = (torch.randn(rows or int(start[-1]), heads * group, dim, generator=g) * 1.5).to(dtype)
+    if adjust:
+        adjust(q, cache, table)
+    scale = dim ** -0.5 if scale is None else scale
+    on_gpu = [t.cuda() for t in cache]
+    args = (q.cuda(), *on_gpu, table.cuda(), torch.tensor(cached, dtype=torch.int32, device="cuda"), scale,
+            None if new is None else start.cuda())
+    got = ext.kv_block_attention(*args) if out is None else ext.kv_block_attention(*args, out)
+    assert got.shape == (len(q), heads * group * dim) and got.dtype == dtype
+    narrow = dtype != torch.float32
+    want, bound = attention64(q, cache, table, cached, start, block, scale, 1152.0 if narrow else 0.0, 2.0 ** -11 if narrow else 2.0 ** -22)
+    covered = int(start[-1])
+    off = (got.cpu().double().reshape(want.shape) - want)[:covered].abs()
+    tolerance = (half_step(dtype, want) + bound)[:covered]
+    assert torch.all(off <= tolerance), f"worst {float((off / tolerance).max()):.3f} of what may be"
+    assert torch.equal(got, ext.kv_block_attention(*args) if out is None else ext.kv_block_attention(*args, out))   # the same bits again
+    return got, args
+
+
+STEPS = [  # block, D, kv heads, group, cached, new
+    (64, 64, 1, 1, [0], None), (64, 64, 2, 4, [0, 1, 14, 15, 16, 62, 63, 64, 65], None), (16, 128, 2, 4, [300, 0, -1, 15, 31], None),
+    (32, 64, 1, 7, [33, 31, 95, 257], None), (128, 128, 1, 8, [127, 128, 500], None), (64, 256, 2, 2, [70, 3], None),
+    (128, 256, 1, 3, [200], None), (16, 64, 1, 16, [47, 200], None), (64, 128, 1, 24, [90], None), (16, 256, 1, 1, [17], None),
+    (64, 128, 1, 40, [65, 130], None), (64, 64, 1, 100, [66], None), (32, 128, 3, 5, [-1, -1, 40], None)]
+DRAFTS = [
+    (64, 64, 1, 4, [60, 0, 200], [5, 3, 4]), (16, 128, 1, 7, [100, 31, -1, 0], [4, 5, 2, 1]), (32, 64, 2, 1, [10, 40], [17, 0]),
+    (64, 128, 1, 8, [3], [9]), (128, 64, 1, 2, [0, 130], [33, 8]), (64, 256, 1, 4, [20], [6]), (16, 64, 1, 4, [5] * 67, [2] * 67)]
+PROMPTS = [
+    (64, 64, 1, 4, [0], [130]), (16, 128, 1, 2, [37, 0], [70, 150]), (64, 128, 1, 1, [200], [100]), (32, 256, 1, 2, [0, 9], [75, 40]),
+    (128, 64, 1, 3, [0, 3, 100], [1, 200, 40]), (64, 64, 1, 1, [64], [64]), (64, 128, 2, 4, [0], [65])]
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=TAGS.get)
+@pytest.mark.parametrize("block,dim,heads,group,cached,new", STEPS + DRAFTS + PROMPTS)
+def test_attention(ext, dtype, block, dim, heads, group, cached, new):
+    check_attention(ext, dtype, block, dim, heads, group, cached, new)
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=TAGS.get)
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_attention_of_long_sequences(ext, dtype, dim):
+    """Long enough for the work to be split over the tokens, short sequences and one of nothing beside them."""
+    check_attention(ext, dtype, 64, dim, 1, 4, [5000, 3, -1, 0, 1500], None)
+    check_attention(ext, dtype, 16, dim, 2, 2, [2600], [3])
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=TAGS.get)
+def test_attention_without_some_blocks(ext, dtype):
+    """Blocks that are none, in the middle, at the end and throughout; a sequence longer than its table."""
+    table = torch.tensor([[0, -1, 2, 99], [-1, -1, -1, -1], [3, 4, 5, 6], [2 ** 31 - 1, 7, -2 ** 31, 1]], dtype=torch.int32)
+    check_attention(ext, dtype, 16, 64, 2, 2, [60, 60, 300, 40], None, table=table)
+    check_attention(ext, dtype, 32, 128, 1, 4, [100, 5, 126, 70], [3, 2, 9, 40], table=table)
+    check_attention(ext, dtype, 64, 64, 1, 1, [2 ** 31 - 1, -2 ** 31, 2 ** 31 - 2, 200], None, table=table)
+
+
+def test_attention_leaves_rows_of_no_sequence(ext):
+    for new, cached in (([3, 0, 2], [70, 5, 9]), ([40, 1, 30], [2, 0, 100])):
+        out = torch.full((sum(new) + 7, 4 * 64), 7.5, device="cuda", dtype=torch.float16)
+        check_attention(ext, torch.float16, 16, 64, 1, 4, cached, new, out=out, rows=sum(new) + 7)
+        assert torch.all(out[sum(new):] == 7.5)
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=TAGS.get)
+def test_attention_of_far_apart_values(ext, dtype):
+    """Queries whose elements lie far apart, scores that leave one token, scales of zero, negative and large factors."""
+    def wide(q, cache, table):
+        q[..., 0] *= 300.0
+        q[..., 1] *= 1e-4
+        q[0, 0] = 0.0
+        q[0, 1] *= 1e-3 if dtype == torch.float16 else 1e-30
+
+    def nothing(q, cache, table):
+        cache[2][table[0, 0]] = 0.0
+        cache[3][table[0, 1]] = 0.0
+        cache[3][table[1, 0]] = 1e-8
+
+    check_attention(ext, dtype, 16, 64, 1, 4, [90, 40], None, adjust=wide)
+    check_attention(ext, dtype, 16, 64, 1, 4, [90, 40], None, adjust=nothing)
+    check_attention(ext, dtype, 64, 128, 1, 2, [90, 200], [2, 3], scale=-0.05)
+    check_attention(ext, dtype, 64, 64, 1, 2, [130], None, scale=0.0)
+
+
+def test_values_behind_the_last_token_do_not_count(ext):
+    """Places behind a sequence's last token, and blocks of other sequences, may hold anything."""
+    g = torch.Generator().manual_seed(1)
+    cache = make_cache(g, 4, 2, 32, 64)
+    table = torch.tensor([[2, 0], [1, 3]], dtype=torch.int32, device="cuda")
+    q = torch.randn(2, 4, 64, generator=g).half().cuda()
+    cached = torch.tensor([40, 3], dtype=torch.int32, device="cuda")
+    plain = ext.kv_block_attention(q, *[t.cuda() for t in cache], table, cached, 0.125)
+    cache[0][0, :, 9:] = -128
+    cache[1][0, :, 1, :, :] = -128          # tokens 16 .. 31 of that block: behind the last one
+    cache[1][0, :, 0, :, 9:] = -128
+    cache[0][3], cache[1][3] = 127, 127
+    cache[2][3], cache[3][3] = float("nan"), float("inf")
+    assert torch.equal(plain, ext.kv_block_attention(q, *[t.cuda() for t in cache], table, cached, 0.125))
+
+
+def test_a_query_that_is_not_a_number_stays_in_its_rows(ext):
+    g = torch.Generator().manual_seed(2)
+    cache = [t.cuda() for t in make_cache(g, 4, 1, 64, 64)]
+    table = torch.tensor([[2, 0], [1, 3]], dtype=torch.int32, device="cuda")
+    q = torch.randn(2, 3, 64, generator=g).cuda()
+    cached = torch.tensor([70, 90], dtype=torch.int32, device="cuda")
+    for dtype in DTYPES:
+        clean = ext.kv_block_attention(q.to(dtype), *cache, table, cached, 0.125).reshape(2, 3, 64)
+        for bad in (float("nan"), float("inf")):
+            x = q.clone()
+            x[0, 1, 5] = bad
+            got = ext.kv_block_attention(x.to(dtype), *cache, table, cached, 0.125).reshape(2, 3, 64)
+            assert got[0, 1].isnan().all()
+            got[0, 1] = clean[0, 1]
+            assert torch.equal(got, clean)
+
+
+# ---- together ----------------------------------------------------------------------------------------------------------
+def test_refusals(ext):
+    cache = [t.cuda() for t in make_cache(torch.Generator().manual_seed(0), 2, 2, 16, 64)]
+    table, cached = torch.zeros(1, 1, dtype=torch.int32, device="cuda"), torch.zeros(1, dtype=torch.int32, device="cuda")
+    row, q = torch.zeros(1, 2, 64, device="cuda"), torch.zeros(1, 4, 64, device="cuda")
+
+    def refused(what, call, *args):
+        with pytest.raises(RuntimeError, match=what):
+            call(*args)
+
+    append, attend, back = ext.kv_block_append, ext.kv_block_attention, ext.kv_block_dequant
+    refused("one row", append, row.expand(2, -1, -1), row.expand(2, -1, -1), *cache, table, cached)
+    refused("of one dtype", append, row, row.half(), *cache, table, cached)
+    refused("of one dtype", append, row[..., :32], row[..., :32], *cache, table, cached)
+    refused("float32, float16 or bfloat16", append, row.double(), row.double(), *cache, table, cached)
+    refused("cached must be int32", append, row, row, *cache, table, cached.long())
+    refused("block_table must be int32", append, row, row, *cache, table.long(), cached)
+    refused("query_start must be int32", append, row, row, *cache, table, cached, cached)
+    refused("v_codes must be", append, row, row, cache[0], cache[0], *cache[2:], table, cached)
+    refused("k_codes must be", append, row, row, cache[0].transpose(0, 1), *cache[1:], table, cached)
+    refused("scales must be", append, row, row, *cache[:2], cache[2].half(), cache[3], table, cached)
+    refused("cache's device", append, row.cpu(), row, *cache, table, cached)
+    refused("CUDA", append, row, row, *[t.cpu() for t in cache], table, cached)
+    refused("not a multiple of kv_heads", attend, torch.zeros(1, 3, 64, device="cuda"), *cache, table, cached, 1.0)
+    refused("query must be", attend, torch.zeros(1, 4, 32, device="cuda"), *cache, table, cached, 1.0)
+    refused("finite", attend, q, *cache, table, cached, float("inf"))
+    refused("finite", attend, q, *cache, table, cached, float("nan"))
+    refused("out must be", attend, q, *cache, table, cached, 1.0, None, torch.zeros(1, 4, 64, device="cuda"))
+    refused("n_tokens is out of range", back, *cache, table, torch.zeros(2, dtype=torch.int32, device="cuda"), -1, torch.float16)
+    refused("starts must be int32", back, *cache, table, cached, 1, torch.float16)
+    narrow = [cache[0][..., :32].contiguous(), cache[1][..., :32, :].contiguous(), *cache[2:]]
+    refused("head_dim must be 64", attend, torch.zeros(1, 2, 32, device="cuda"), *narrow, table, cached, 1.0)
+    odd = [cache[0][:, :, :8].contiguous(), cache[1][:, :, :0].contiguous(), *cache[2:]]
+    refused("v_codes must be", attend, q, *odd, table, cached, 1.0)
+    w, t = torch.ones(64, device="cuda"), torch.ones(1, 64, device="cuda")
+    flat = torch.zeros(1, 128, device="cuda")
+    refused("whole heads", ext.qk_norm_rope, flat[:, :96], flat, w, w, t, t, 1e-5)
+    refused("without positions", ext.qk_norm_rope, flat.expand(2, -1), flat.expand(2, -1), w, w, t, t, 1e-5)
+    refused("q's dtype", ext.qk_norm_rope, flat, flat, w.half(), w, t, t, 1e-5)
+    refused("rotated part", ext.qk_norm_rope, flat, flat, w, w, t[:, :36], t[:, :36], 1e-5)
+    refused("rotated part", ext.qk_norm_rope, flat, flat, w, w, flat, flat, 1e-5)
+    refused("eps", ext.qk_norm_rope, flat, flat, w, w, t, t, -1.0)
+    refused("positions must be", ext.qk_norm_rope, flat, flat, w, w, t, t, 1e-5, torch.zeros(1, device="cuda"))
+
+
+def test_nothing_to_do(ext):
+    for blocks, sequences, width in ((0, 0, 0), (2, 0, 0), (0, 2, 3), (2, 2, 0)):
+        cache = [torch.zeros(blocks, 2, 16, 64, dtype=torch.int8, device="cuda"), torch.zeros(blocks, 2, 1, 64, 16, dtype=torch.int8, device="cuda"),
+                 torch.zeros(blocks, 2, device="cuda"), torch.zeros(blocks, 2, device="cuda")]
+        table = torch.zeros(sequences, width, dtype=torch.int32, device="cuda")
+        cached, row = torch.zeros(sequences, dtype=torch.int32, device="cuda"), torch.ones(sequences, 2, 64, device="cuda")
+        ext.kv_block_append(row, row, *cache, table, cached)
+        got = ext.kv_block_attention(row, *cache, table, cached, 1.0)
+        assert got.shape == (sequences, 128) and torch.all(got == 0)
+        starts = torch.arange(sequences + 1, dtype=torch.int32, device="cuda")
+        for out in ext.kv_block_dequant(*cache, table, starts, sequences, torch.float16):
+            assert out.shape == (2, sequences, 64) and torch.all(out == 0)
+    w, t = torch.ones(64, device="cuda"), torch.ones(0, 64, device="cuda")
+    q, k = ext.qk_norm_rope(torch.zeros(0, 128, device="cuda"), torch.zeros(0, 64, device="cuda"), w, w, t, t, 1e-5)
+    assert q.shape == (0, 2, 64) and k.shape == (0, 1, 64)
+    q, k = ext.qk_norm_rope(torch.ones(1, 128, device="cuda"), torch.zeros(1, 0, device="cuda"), w, w, t, t, 1e-5,
+                            torch.zeros(1, dtype=torch.int32, device="cuda"))
+    assert q.isnan().all() and k.shape == (1, 0, 64)   # (a table of no rows knows no position)

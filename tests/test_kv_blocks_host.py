@@ -1,0 +1,118 @@
+"""The entry points over a cache in blocks refuse what their kernels do not take, before any device is asked for."""
+
+import pytest
+
+F32, F16, BF16 = 0, 1, 2
+
+
+@pytest.fixture(scope="module")
+def lib():
+    from llmquant.hip.build import CAPI_PATH, build_extension, load_capi
+
+    if not CAPI_PATH.exists():
+        build_extension()
+    return load_capi()
+
+
+def text(lib):
+    return lib.llmq_last_error().decode()
+
+
+def norm(lib, **change):
+    a = dict(tokens=4, q_heads=8, kv_heads=2, dim=128, rotary=128, rows=64, q_stride=1280, k_stride=1280, eps=1e-6, dtype=BF16, table=BF16,
+             position_bytes=4, positions=16) | change
+    return lib.llmq_qk_norm_rope(*[a.get("pointer")] * 6, a["positions"], a["position_bytes"], *[a.get("pointer")] * 2, a["tokens"], a["q_heads"],
+                                 a["kv_heads"], a["dim"], a["rotary"], a["rows"], a["q_stride"], a["k_stride"], a["eps"], a["dtype"],
+                                 a["table"], None)
+
+
+@pytest.mark.parametrize("change,what", [
+    (dict(tokens=-1), "bad dimension"), (dict(dtype=7), "float32, float16 or bfloat16"), (dict(table=F16), "the tables hold"),
+    (dict(dim=72), "head_dim must be a multiple of 16"), (dict(dim=512, rotary=64), "up to 256"), (dict(dim=0), "head_dim"),
+    (dict(rotary=8), "rotated part"), (dict(rotary=256), "rotated part"), (dict(rotary=0), "rotated part"),
+    (dict(q_stride=1281), "row strides"), (dict(k_stride=1284), "row strides"), (dict(position_bytes=2), "4 or 8 bytes"),
+    (dict(positions=None, rows=3), "a row for each"), (dict(eps=-1e-6), "eps"), (dict(eps=float("nan")), "eps"),
+    (dict(eps=float("inf")), "eps"), (dict(), "null tensor pointer"), (dict(pointer=24), "16-byte aligned"),
+    (dict(pointer=16, tokens=2 ** 31 - 1, rows=1), "too many heads")])
+def test_norm_and_rotation_refuses(lib, change, what):
+    assert norm(lib, **change) == 1 and what in text(lib)
+
+
+def test_norm_and_rotation_of_nothing(lib):
+    assert norm(lib, tokens=0) == 0 and norm(lib, q_heads=0, kv_heads=0) == 0
+    assert norm(lib, dtype=F32, table=F32, dim=72, rotary=8) == 1 and "null tensor pointer" in text(lib)   # packets of four
+
+
+SHAPE = dict(tokens=4, sequences=4, kv_heads=2, dim=64, block=64, blocks=8, width=3, stride=3, dtype=BF16)
+SHAPES = [
+    (dict(tokens=-1), "bad dimension"), (dict(sequences=-1), "bad dimension"), (dict(kv_heads=0), "bad dimension"),
+    (dict(blocks=-1), "bad dimension"), (dict(width=-1), "bad dimension"), (dict(dim=96), "head_dim must be 64, 128 or 256"),
+    (dict(block=48), "block must be"), (dict(block=8), "block must be"), (dict(block=256), "block must be"), (dict(dtype=3), "dtype code 3"),
+    (dict(stride=-3), "negative stride"), (dict(tokens=2 ** 31 - 1, sequences=2 ** 31 - 1, kv_heads=64), "too many rows")]
+
+
+def append(lib, **change):
+    a = SHAPE | dict(key_stride=128, value_stride=128) | change
+    p = a.get("pointer")
+    return lib.llmq_kv_block_append(p, p, a["key_stride"], a["value_stride"], a.get("codes", p), p, p, p, p, a["stride"], p, a.get("start"),
+                                    a["tokens"], a["sequences"], a["kv_heads"], a["dim"], a["block"], a["blocks"], a["width"], a["dtype"], None)
+
+
+@pytest.mark.parametrize("change,what", SHAPES + [
+    (dict(sequences=3), "one row"), (dict(key_stride=130), "row strides"), (dict(value_stride=130), "row strides"),
+    (dict(dtype=F32, key_stride=130), "row strides"), (dict(), "null tensor pointer"), (dict(pointer=16, codes=None), "null tensor pointer"),
+    (dict(pointer=16, codes=24), "codes must be 16-byte aligned"), (dict(pointer=8, codes=16), "16-byte aligned")])
+def test_append_refuses(lib, change, what):
+    assert append(lib, **change) == 1 and what in text(lib)
+
+
+def test_append_of_nothing(lib):
+    assert append(lib, tokens=0, sequences=0) == 0 and append(lib, blocks=0) == 0 and append(lib, width=0) == 0
+
+
+def dequant(lib, **change):
+    a = SHAPE | change
+    p = a.get("pointer")
+    return lib.llmq_kv_block_dequant(a.get("codes", p), p, p, p, p, a["stride"], p, None, p, p, a["tokens"], a["sequences"], a["kv_heads"],
+                                     a["dim"], a["block"], a["blocks"], a["width"], a["dtype"], None)
+
+
+@pytest.mark.parametrize("change,what", SHAPES + [
+    (dict(), "null tensor pointer"), (dict(pointer=16, codes=24), "codes must be 16-byte aligned"), (dict(pointer=8, codes=16), "16-byte aligned")])
+def test_dequant_refuses(lib, change, what):
+    assert dequant(lib, **change) == 1 and what in text(lib)
+
+
+def test_dequant_of_nothing(lib):
+    assert dequant(lib, tokens=0) == 0 and dequant(lib, sequences=0) == 0
+
+
+def attention(lib, **change):
+    a = SHAPE | dict(q_stride=512, q_heads=8, scale=0.125, space=2 ** 40) | change
+    p = a.get("pointer")
+    return lib.llmq_kv_block_attention(p, a["q_stride"], a.get("codes", p), p, p, p, p, a["stride"], p, a.get("start"), p, a.get("workspace", p), a["space"],
+                                       a["scale"], a["tokens"], a["sequences"], a["q_heads"], a["kv_heads"], a["dim"], a["block"], a["blocks"],
+                                       a["width"], a["dtype"], None)
+
+
+@pytest.mark.parametrize("change,what", SHAPES + [
+    (dict(q_heads=7), "not a multiple"), (dict(q_heads=0), "not a multiple"), (dict(scale=float("nan")), "finite"),
+    (dict(scale=float("inf")), "finite"), (dict(sequences=3), "one row"), (dict(q_stride=513), "row strides"), (dict(), "null tensor pointer"),
+    (dict(pointer=16, codes=24), "16-byte aligned"), (dict(pointer=8, codes=16), "16-byte aligned"),
+    (dict(tokens=2 ** 27, sequences=2 ** 20, start=16, pointer=16, q_heads=64), "too many rows")])
+def test_attention_refuses(lib, change, what):
+    assert attention(lib, **change) == 1 and what in text(lib)
+
+
+def test_attention_of_nothing(lib):
+    assert attention(lib, tokens=0, sequences=0) == 0 and attention(lib, sequences=0, tokens=0, start=16) == 0
+
+
+def test_attention_workspace(lib):
+    """(tokens, sequences, q_heads, kv_heads, head_dim, block, table width)"""
+    size = lib.llmq_kv_block_attention_workspace_bytes
+    assert size(0, 0, 8, 2, 64, 64, 100) == 0 and size(1, 1, 8, 0, 64, 64, 100) == 0 and size(1, 1, 8, 2, 64, 64, 0) == 0
+    need = size(1, 1, 32, 8, 128, 128, 1024)
+    if need:   # a long sequence of few rows is split, and a workspace that is too small refused
+        assert attention(lib, tokens=1, sequences=1, q_heads=32, kv_heads=8, dim=128, block=128, width=1024, q_stride=4096, pointer=16, space=need - 1) == 1
+        assert "workspace" in text(lib)
