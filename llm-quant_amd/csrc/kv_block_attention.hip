@@ -1,6 +1,24 @@
-// Attention of a batch over a cache in blocks (layout: kv_blocks.h), gfx950: row i of sequence b sees the tokens
-// 0 .. cached[b] + i,
-//   t_j = (q . k_j) s_k scale,   out = sum 2^t_j s_v c_j / sum 2^t_j
+// Attention of a batch over a cache in blocks (layout: kv_blocks.h), on the matrix core, gfx950: row i of sequence b sees
+// the tokens 0 .. cached[b] + i,
+//   t_j = (q . k_j) s_k(j) scale log2 e,   out = sum_j 2^t_j s_v(j) c_j / sum_j 2^t_j      (k, c: the bare codes)
+//
+// Mathematics. The value scale goes into the exponent: u_j = t_j + log2 s_v(j), w_j = 2^(u_j - max u), so that
+//   out = sum w_j c_j / sum (w_j / s_v(j))
+// and the second product meets bare codes with weights of at most 1, however far the blocks' scales lie apart; the division in
+// the sum of the softmax is one product for 16 scores, all of one block. Codes become fp16 by placing them, sign flipped, in
+// the mantissa of 1024 (one byte permute for two codes, exact); the 1152 too many are taken from the value codes (one packed
+// add for two), and from the scores through sum q, in fp32. A query row is brought to [1, 2) by a power of two and enters as
+// fp16: exact for 16-bit types but for elements 2^-14 below the row's largest (off by 2^-25 of that), the weights as fp16 (off by
+// 2^-11, below what a 16-bit output is rounded by). For fp32 both enter as two such pieces, the second 2^11 times as high, and the
+// keys without the 1152 too many: 22 bits. Running maximum and sum, and everything that is added up, are fp32.
+//
+// Layout. A wave takes 64 tokens at a time: four strips of 16. Both products are transposed: S^T = K Q^T leaves lane
+// (row, g) with the 16 scores of strip g for its row, so scales and the block of a strip are the lane's own, and its
+// weights are, as they lie, the second product's operand: O^T = V^T P^T, whose other operand, 16 tokens of one column, is
+// one 16-byte load of the value codes. Keys and values go from memory to registers, with no LDS in between and no barrier in
+// the walk. A workgroup has four waves and 64 NR rows (rows of a sequence x query heads of one key head): waves
+// take row tiles of 16 NR each, or, where there are fewer, share a row tile's tokens and meet in LDS at the end.
+#include <algorithm>
 #include <cmath>
 
 #include "kv_blocks.h"
@@ -9,64 +27,491 @@ namespace {
 
 using namespace llmq;
 
-constexpr int kMaxDim = 256;
+typedef _Float16 v8h __attribute__((ext_vector_type(8)));
+typedef _Float16 v2h __attribute__((ext_vector_type(2)));
+typedef float v4f __attribute__((ext_vector_type(4)));
+typedef float v2f __attribute__((ext_vector_type(2)));
 
-// a wave per row and query head
-template <typename T>
-__global__ __launch_bounds__(kWave) void attention_kernel(
-    const T* __restrict__ query, const int64_t q_stride, const int8_t* __restrict__ k_codes, const int8_t* __restrict__ v_codes,
-    const float* __restrict__ k_scale, const float* __restrict__ v_scale, const BlockTable table,
-    const int32_t* __restrict__ cached, const Ragged rows, T* __restrict__ out, const int q_heads, const int heads, const int D,
-    const int block, const float scale_log2e) {
-  __shared__ float s_q[kMaxDim], s_w[kWave];
-  const int lane = threadIdx.x, qh = blockIdx.x % q_heads, row = blockIdx.x / q_heads, h = qh / (q_heads / heads);
-  int found = 0;
-  for (int b0 = 0; b0 < rows.sequences; b0 += kWave) {
-    const int b = b0 + lane;
-    found += __popcll(__ballot(b < rows.sequences && rows.first(b) <= row));
+constexpr int kWaves = 4, kThreads = kWaves * kWave, kTile = 64;
+constexpr int kHeader = 4;            // floats in front of a partial result: maximum, sum, two of nothing
+constexpr int kMaxSplits = 64;
+constexpr float kBias = 1152.0f;      // what a code is too high as an operand: 1024, and 128 of the flipped sign
+constexpr float kNoScale = 0x1p-100f; // value scales below count as zero
+constexpr float kPiece = 2048.0f;     // the second piece of an fp32 number is this much too high
+
+struct Problem {
+  const void* query;
+  int64_t q_stride;
+  const int8_t *k_codes, *v_codes;
+  const float *k_scale, *v_scale;
+  BlockTable table;
+  const int32_t* cached;
+  Ragged rows;
+  void* out;
+  float* partials;
+  int splits, q_heads, heads, group, block_shift;
+  float scale_log2e;
+};
+
+template <typename T> struct Pieces { static constexpr int N = 1; };
+template <> struct Pieces<float> { static constexpr int N = 2; };
+
+// The two values that a lane and the one 32 (16) lanes away have, in either of them.
+template <int STEP> __device__ __forceinline__ v2f both(float v) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  const uint32_t x = __builtin_bit_cast(uint32_t, v);
+  uint32_t lo, hi;   // (the cast of a vector's element reads its first one: taken out ahead of it)
+  if constexpr (STEP == 32) {
+    const auto r = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+    lo = r[0];
+    hi = r[1];
+  } else {
+    const auto r = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+    lo = r[0];
+    hi = r[1];
   }
-  const int b = found - 1;
-  if (b < 0 || row - rows.first(b) >= rows.count(b)) return;
-  T* o = out + (static_cast<int64_t>(row) * q_heads + qh) * D;
-  const int64_t limit = cached[b] < 0 ? 0 : min(static_cast<int64_t>(cached[b]) + row - rows.first(b) + 1, static_cast<int64_t>(table.width) * block);
-  for (int d = lane; d < D; d += kWave) s_q[d] = to_float(query[row * q_stride + static_cast<int64_t>(qh) * D + d]);
-  float m = -INFINITY, l = 0.0f, acc[kMaxDim / kWave] = {};
-  for (int64_t j0 = 0; j0 < limit; j0 += kWave) {
-    __syncthreads();
-    const int64_t j = j0 + lane;
-    const int id = j < limit ? table.at(b, static_cast<int>(j / block)) : -1;
-    const int64_t at = (static_cast<int64_t>(max(id, 0)) * heads + h) * block * D;
-    float t = -INFINITY;
-    if (id >= 0) {
-      float dot = 0.0f;
-      for (int d = 0; d < D; ++d) dot = fmaf(s_q[d], static_cast<float>(k_codes[at + (j % block) * D + d]), dot);
-      t = dot * k_scale[static_cast<int64_t>(id) * heads + h] * scale_log2e;
+  return v2f{__builtin_bit_cast(float, lo), __builtin_bit_cast(float, hi)};
+#else
+  return v2f{v, v};
+#endif
+}
+// over the four lanes (row, 0 .. 3)
+__device__ __forceinline__ float max_of_rows(float v) {
+  v2f x = both<32>(v);
+  x = both<16>(fmaxf(x[0], x[1]));
+  return fmaxf(x[0], x[1]);
+}
+__device__ __forceinline__ float sum_of_rows(float v) {
+  v2f x = both<32>(v);
+  x = both<16>(x[0] + x[1]);
+  return x[0] + x[1];
+}
+
+__device__ __forceinline__ v4f product(u32x4 a, u32x4 b, v4f c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8h, a), __builtin_bit_cast(v8h, b), c, 0, 0, 0);
+}
+__device__ __forceinline__ uint32_t pack_half(float lo, float hi) {
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector(v2f{lo, hi}, v2h));
+}
+// four codes as fp16, EXACT or 1152 too high
+template <bool EXACT> __device__ __forceinline__ u32x2 codes_to_half(uint32_t word) {
+  const uint32_t w = word ^ 0x80808080u;
+  u32x2 r{__builtin_amdgcn_perm(0x64646464u, w, 0x04010400u), __builtin_amdgcn_perm(0x64646464u, w, 0x04030402u)};
+  if constexpr (EXACT) {
+    const v2h bias = {static_cast<_Float16>(-kBias), static_cast<_Float16>(-kBias)};
+    r.x = __builtin_bit_cast(uint32_t, __builtin_bit_cast(v2h, r.x) + bias);
+    r.y = __builtin_bit_cast(uint32_t, __builtin_bit_cast(v2h, r.y) + bias);
+  }
+  return r;
+}
+template <bool EXACT> __device__ __forceinline__ u32x4 operand(uint32_t lo, uint32_t hi) {
+  const u32x2 a = codes_to_half<EXACT>(lo), b = codes_to_half<EXACT>(hi);
+  return u32x4{a.x, a.y, b.x, b.y};
+}
+
+template <typename T> __device__ __forceinline__ void load8(const T* p, float* f) {
+#pragma unroll
+  for (int i = 0; i < 8; i += Pack<T>::N) Pack<T>::unpack(load16(p + i), f + i);
+}
+template <typename T> __device__ __forceinline__ void store8(T* p, const float* f) {
+#pragma unroll
+  for (int i = 0; i < 8; i += Pack<T>::N) store16(p + i, Pack<T>::pack(f + i));
+}
+
+template <typename T, int D, int NR>
+__global__ __launch_bounds__(kThreads, 2) void attention_kernel(const Problem a) {
+  constexpr int kPieces = Pieces<T>::N;
+  constexpr bool kExactKeys = kPieces > 1;
+  constexpr int kChunks = D / 64, kSteps = D / 32, kColumns = D / 16;   // 64-element pieces, k-steps of S^T, row tiles of O^T
+  constexpr int kRows = 16 * NR, kGroupRows = kWaves * kRows, kRow = D + 4;
+  __shared__ __attribute__((aligned(16))) float s_part[kWaves * kRows * kRow];
+  __shared__ float s_max[kGroupRows], s_sum[kGroupRows];
+
+  const int tid = threadIdx.x, lane = tid & (kWave - 1), r16 = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
+  // key heads fastest: with eight of them each XCD's cache holds one. Late rows, which see most, first.
+  const int h = blockIdx.x % a.heads, rest = blockIdx.x / a.heads, split = rest % a.splits;
+  int64_t piece = gridDim.x / a.heads / a.splits - 1 - rest / a.splits;
+  int b;
+  if (a.rows.start == nullptr) {
+    const int per = (a.group + kGroupRows - 1) / kGroupRows;
+    b = static_cast<int>(piece / per);
+    piece %= per;
+  } else {
+    b = a.rows.find(a.group, kGroupRows, 1, piece);
+  }
+  const int n_rows = a.rows.count(b) * a.group, row0 = static_cast<int>(min(piece * kGroupRows, static_cast<int64_t>(INT32_MAX)));
+  if (row0 >= n_rows) return;
+  const int first_row = a.rows.first(b), cached = a.cached[b];
+  const int here = min(n_rows - row0, kGroupRows), tiles_of_rows = (here + kRows - 1) / kRows;
+  const int sharing = tiles_of_rows == 1 ? 4 : tiles_of_rows == 2 ? 2 : 1;   // waves that share a row tile
+  const int my_tile = wave / sharing, my_share = wave % sharing;
+  const int wave_row = row0 + my_tile * kRows;
+  const int64_t held = static_cast<int64_t>(a.table.width) << a.block_shift;
+
+  // this lane's rows
+  u32x4 q[NR][kSteps][kPieces];
+  float q_scale[NR], q_bias[NR];
+  int last[NR];   // the last token that the row sees; -1: none
+#pragma unroll
+  for (int n = 0; n < NR; ++n) {
+    const int row = min(wave_row + 16 * n + r16, n_rows - 1), token = row / a.group;
+    last[n] = cached < 0 ? -1 : static_cast<int>(min(min(static_cast<int64_t>(cached) + token, held - 1), static_cast<int64_t>(INT32_MAX - 2 * kTile)));
+    const T* x = static_cast<const T*>(a.query) + (first_row + token) * a.q_stride +
+                 static_cast<int64_t>(h * a.group + row % a.group) * D + 16 * g;
+    float f[kSteps][8], largest = 0.0f;
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s) {
+      load8(x + 64 * (s / 2) + 8 * (s % 2), f[s]);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) largest = fmaxf(largest, fabsf(f[s][e]));
     }
-    const float m_new = fmaxf(m, group_max<64>(t)), base = m_new == -INFINITY ? 0.0f : m_new;
-    const float alpha = exp2f(m - base), p = exp2f(t - base);
-    m = m_new;
-    l = l * alpha + wave_sum(p);
-    s_w[lane] = id >= 0 ? p * v_scale[static_cast<int64_t>(id) * heads + h] : 0.0f;
-    __syncthreads();
-    for (int e = 0; e < D / kWave; ++e) {
-      float sum = 0.0f;
-      for (int i = 0; i < kWave; ++i) {
-        const int64_t ji = j0 + i;
-        const int idi = ji < limit ? table.at(b, static_cast<int>(ji / block)) : -1;
-        if (idi < 0) continue;
-        const int64_t ati = (static_cast<int64_t>(idi) * heads + h) * block * D;
-        const int slot = static_cast<int>(ji % block);
-        sum = fmaf(s_w[i], static_cast<float>(v_codes[ati + (static_cast<int64_t>(slot / kStrip) * D + e * kWave + lane) * kStrip + slot % kStrip]), sum);
+    largest = max_of_rows(largest);
+    const int exponent = __builtin_amdgcn_frexp_expf(largest) - 1;
+    float total = 0.0f;
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s) {
+      uint32_t hi[4], lo[4];
+#pragma unroll
+      for (int e = 0; e < 8; e += 2) {
+        const float x0 = ldexpf(f[s][e], -exponent), x1 = ldexpf(f[s][e + 1], -exponent);
+        hi[e / 2] = pack_half(x0, x1);
+        const v2h top = __builtin_bit_cast(v2h, hi[e / 2]);
+        if constexpr (kPieces > 1) lo[e / 2] = pack_half((x0 - static_cast<float>(top[0])) * kPiece, (x1 - static_cast<float>(top[1])) * kPiece);
+        else total += static_cast<float>(top[0]) + static_cast<float>(top[1]);
       }
-      acc[e] = acc[e] * alpha + sum;
+      q[n][s][0] = u32x4{hi[0], hi[1], hi[2], hi[3]};
+      if constexpr (kPieces > 1) q[n][s][kPieces - 1] = u32x4{lo[0], lo[1], lo[2], lo[3]};
+    }
+    q_bias[n] = kExactKeys ? 0.0f : -kBias * sum_of_rows(total);
+    q_scale[n] = ldexpf(a.scale_log2e, exponent);
+  }
+
+  // the walk: tiles of 64 tokens, from the split's first one on
+  const int seen_first = __builtin_amdgcn_readfirstlane(last[0]);   // (rows of a wave see more and more)
+  int seen_last = -1;
+  if (wave_row < n_rows) {
+    const int64_t newest = cached < 0 ? -1 : static_cast<int64_t>(cached) + (min(row0 + (my_tile + 1) * kRows, n_rows) - 1) / a.group;
+    seen_last = static_cast<int>(min(min(newest, held - 1), static_cast<int64_t>(INT32_MAX - 2 * kTile)));
+  }
+  const int tiles = (seen_last + kTile) / kTile, per_split = (tiles + a.splits - 1) / a.splits;
+  const int begin = split * per_split, end = min(begin + per_split, tiles);
+
+  // the blocks of a tile's strips: for its keys a lane reads strip r16 / 4, for its values and scales strip g
+  const int k_strip = r16 >> 2;
+  int k_id, v_id;
+  auto find_blocks = [&](int tile) {
+    k_id = v_id = -1;
+    const int at = tile * kTile;
+    if (tile < end) {
+      if (at + kStrip * k_strip <= seen_last) k_id = a.table.at(b, (at + kStrip * k_strip) >> a.block_shift);
+      if (at + kStrip * g <= seen_last) v_id = a.table.at(b, (at + kStrip * g) >> a.block_shift);
+    }
+  };
+  const int in_block = (1 << a.block_shift) - 1;
+  u32x4 k_raw[4][kChunks], v_raw[kColumns];
+  auto load_keys = [&](int tile) {
+    const int slot = (tile * kTile + kStrip * k_strip) & in_block;
+    const int8_t* p = a.k_codes + ((static_cast<int64_t>(max(k_id, 0)) * a.heads + h) * (in_block + 1) + slot + (r16 & 3)) * D + 16 * g;
+#pragma unroll
+    for (int t = 0; t < 4; ++t)
+#pragma unroll
+      for (int c = 0; c < kChunks; ++c) k_raw[t][c] = load16(p + 4 * t * D + 64 * c);
+  };
+  auto load_values = [&](int tile) {
+    const int slot = (tile * kTile + kStrip * g) & in_block;
+    const int8_t* p = a.v_codes + ((static_cast<int64_t>(max(v_id, 0)) * a.heads + h) * (in_block + 1) + slot) * D + kStrip * r16;
+#pragma unroll
+    for (int c = 0; c < kColumns; ++c) v_raw[c] = load16(p + 16 * kStrip * c);
+  };
+  float k_scale = 0.0f, v_scale = 0.0f;
+  auto load_scales = [&]() {
+    const int64_t at = static_cast<int64_t>(max(v_id, 0)) * a.heads + h;
+    k_scale = a.k_scale[at];
+    v_scale = a.v_scale[at];
+  };
+
+  v4f o[NR][kColumns];
+  float m_run[NR], l_run[NR];
+#pragma unroll
+  for (int n = 0; n < NR; ++n) {
+    m_run[n] = -INFINITY;
+    l_run[n] = 0.0f;
+#pragma unroll
+    for (int c = 0; c < kColumns; ++c) o[n][c] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+  }
+
+  int tile = begin + my_share;
+  find_blocks(tile);
+  bool with_block = v_id >= 0;
+  if (tile < end) {
+    load_keys(tile);
+    load_scales();
+    load_values(tile);
+  }
+  for (; tile < end; tile += sharing) {
+    const int next = tile + sharing;
+    const float ks = k_scale, vs = v_scale;
+    const bool strip = with_block;
+    find_blocks(next);
+    with_block = v_id >= 0;
+    // scores: lane (row, g) gets token 16 g + 4 t + i in s[.][t][i]
+    v4f s[NR][4];
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+#pragma unroll
+      for (int n = 0; n < NR; ++n) s[n][t] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+      u32x4 k[kSteps];
+#pragma unroll
+      for (int c = 0; c < kChunks; ++c) {
+        k[2 * c] = operand<kExactKeys>(k_raw[t][c].x, k_raw[t][c].y);
+        k[2 * c + 1] = operand<kExactKeys>(k_raw[t][c].z, k_raw[t][c].w);
+      }
+      if constexpr (kPieces > 1) {
+#pragma unroll
+        for (int n = 0; n < NR; ++n) {
+#pragma unroll
+          for (int x = 0; x < kSteps; ++x) s[n][t] = product(k[x], q[n][x][kPieces - 1], s[n][t]);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) s[n][t][i] *= 1.0f / kPiece;
+        }
+      }
+#pragma unroll
+      for (int x = 0; x < kSteps; ++x)
+#pragma unroll
+        for (int n = 0; n < NR; ++n) s[n][t] = product(k[x], q[n][x][0], s[n][t]);
+    }
+    if (next < end) {
+      load_keys(next);
+      load_scales();
+    }
+    // weights
+    const bool no_values = vs < kNoScale;   // (not a number: stays so)
+    const float log_vs = strip ? __builtin_amdgcn_logf(no_values ? kNoScale : vs) : -INFINITY;
+    const float inv_vs = 1.0f / (no_values ? kNoScale : vs);
+    const int at = tile * kTile + kStrip * g;
+    const bool whole = tile * kTile + kTile - 1 <= seen_first;
+    u32x4 p[NR][2][kPieces];
+    float alpha[NR];
+#pragma unroll
+    for (int n = 0; n < NR; ++n) {
+      const float factor = strip ? q_scale[n] * ks : 0.0f, offset = fmaf(q_bias[n], factor, log_vs);
+      float top = -INFINITY;
+#pragma unroll
+      for (int t = 0; t < 4; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          float u = fmaf(s[n][t][i], factor, offset);
+          if (!whole && at + 4 * t + i > last[n]) u = -INFINITY;
+          s[n][t][i] = u;
+          top = fmaxf(top, u);
+        }
+      const float m_new = fmaxf(m_run[n], max_of_rows(top)), base = m_new == -INFINITY ? 0.0f : m_new;
+      alpha[n] = __builtin_amdgcn_exp2f(m_run[n] - base);
+      m_run[n] = m_new;
+      float total = 0.0f;
+#pragma unroll
+      for (int t = 0; t < 4; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; i += 2) {
+          const float w0 = __builtin_amdgcn_exp2f(s[n][t][i] - base), w1 = __builtin_amdgcn_exp2f(s[n][t][i + 1] - base);
+          total += w0 + w1;
+          const uint32_t hi = pack_half(w0, w1);
+          (&p[n][t / 2][0].x)[2 * (t % 2) + i / 2] = hi;
+          if constexpr (kPieces > 1) {
+            const v2h h2 = __builtin_bit_cast(v2h, hi);
+            (&p[n][t / 2][kPieces - 1].x)[2 * (t % 2) + i / 2] =
+                pack_half((w0 - static_cast<float>(h2[0])) * kPiece, (w1 - static_cast<float>(h2[1])) * kPiece);
+          }
+        }
+      // (a strip that this row does not see adds nothing, whatever its scale holds)
+      l_run[n] = fmaf(l_run[n], alpha[n], total == 0.0f ? 0.0f : total * inv_vs);
+    }
+    if (__any(strip && no_values)) {   // values of nothing: their tokens count in the sum alone
+#pragma unroll
+      for (int n = 0; n < NR; ++n)
+#pragma unroll
+        for (int y = 0; y < 2; ++y)
+#pragma unroll
+          for (int e = 0; e < kPieces; ++e)
+            if (no_values) p[n][y][e] = u32x4{0u, 0u, 0u, 0u};
+    }
+    // weighted codes
+    bool moved = false;
+#pragma unroll
+    for (int n = 0; n < NR; ++n) moved = moved || alpha[n] != 1.0f;
+    if (__any(moved)) {
+#pragma unroll
+      for (int n = 0; n < NR; ++n)
+#pragma unroll
+        for (int c = 0; c < kColumns; ++c)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) o[n][c][i] *= alpha[n];
+    }
+#pragma unroll
+    for (int c = 0; c < kColumns; ++c) {
+      const u32x4 v0 = operand<true>(v_raw[c].x, v_raw[c].y), v1 = operand<true>(v_raw[c].z, v_raw[c].w);
+#pragma unroll
+      for (int n = 0; n < NR; ++n) {
+        if constexpr (kPieces > 1) {
+          v4f low = {0.0f, 0.0f, 0.0f, 0.0f};
+          low = product(v0, p[n][0][kPieces - 1], low);
+          low = product(v1, p[n][1][kPieces - 1], low);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) o[n][c][i] = fmaf(low[i], 1.0f / kPiece, o[n][c][i]);
+        }
+        o[n][c] = product(v0, p[n][0][0], o[n][c]);
+        o[n][c] = product(v1, p[n][1][0], o[n][c]);
+      }
+    }
+    if (next < end) load_values(next);
+  }
+
+  // the waves that share a row tile: max m_w, sum l_w 2^(m_w - m), sum O_w 2^(m_w - m), in wave order
+#pragma unroll
+  for (int n = 0; n < NR; ++n) {
+    l_run[n] = sum_of_rows(l_run[n]);
+    if (g == 0) {
+      s_max[wave * kRows + 16 * n + r16] = m_run[n];
+      s_sum[wave * kRows + 16 * n + r16] = l_run[n];
+    }
+    float* part = s_part + (wave * kRows + 16 * n + r16) * kRow + 4 * g;
+#pragma unroll
+    for (int c = 0; c < kColumns; ++c) *reinterpret_cast<v4f*>(part + 16 * c) = o[n][c];
+  }
+  __syncthreads();
+  constexpr int kPackets = D / 8;
+  for (int item = tid; item < here * kPackets; item += kThreads) {
+    const int row = item / kPackets, d = item % kPackets * 8, wave0 = row / kRows * sharing, in_tile = row % kRows;
+    float m = s_max[wave0 * kRows + in_tile];
+    for (int w = 1; w < sharing; ++w) m = fmaxf(m, s_max[(wave0 + w) * kRows + in_tile]);
+    const float base = m == -INFINITY ? 0.0f : m;
+    float l = 0.0f, f[8] = {};
+    for (int w = 0; w < sharing; ++w) {
+      const int at = (wave0 + w) * kRows + in_tile;
+      const float weight = __builtin_amdgcn_exp2f(s_max[at] - base);
+      l = fmaf(s_sum[at], weight, l);
+      const v4f lo = *reinterpret_cast<const v4f*>(s_part + at * kRow + d), hi = *reinterpret_cast<const v4f*>(s_part + at * kRow + d + 4);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        f[e] = fmaf(lo[e], weight, f[e]);
+        f[e + 4] = fmaf(hi[e], weight, f[e + 4]);
+      }
+    }
+    const int token = (row0 + row) / a.group, head = h * a.group + (row0 + row) % a.group;
+    const int64_t vector = static_cast<int64_t>(first_row + token) * a.q_heads + head;
+    if (a.splits == 1) {
+      const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) f[e] *= inv;
+      store8(static_cast<T*>(a.out) + vector * D + d, f);
+    } else {
+      float* record = a.partials + (vector * a.splits + split) * (D + kHeader);
+      if (d == 0) *reinterpret_cast<v2f*>(record) = v2f{m, l};
+      if (m != -INFINITY || l != 0.0f) store8(record + kHeader + d, f);   // (else nobody reads it)
     }
   }
-  for (int e = 0; e < D / kWave; ++e) o[e * kWave + lane] = from_float<T>(l == 0.0f ? 0.0f : acc[e] / l);
+}
+
+// The splits' records of a row and head, by a wave: a lane holds a split's maximum and sum, then four columns of every
+// 64 / (D / 4)-th record.
+template <typename T, int D>
+__global__ __launch_bounds__(kThreads) void merge_kernel(const float* __restrict__ partials, T* __restrict__ out, const Ragged rows,
+                                                         const int q_heads, const int splits) {
+  constexpr int kQuads = D / 4, kAtOnce = kWave / kQuads, kRecord = D + kHeader;
+  const int lane = threadIdx.x & (kWave - 1);
+  const int64_t vector = static_cast<int64_t>(blockIdx.x) * kWaves + __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  if (vector >= static_cast<int64_t>(rows.rows) * q_heads) return;
+  if (rows.start != nullptr) {   // rows of no sequence have no records
+    const int row = static_cast<int>(vector / q_heads);
+    int found = 0;
+    for (int b0 = 0; b0 < rows.sequences; b0 += kWave) {
+      const int b = b0 + lane;
+      const int n = __popcll(__ballot(b < rows.sequences && rows.first(b) <= row));
+      found += n;
+      if (n < kWave) break;
+    }
+    if (found == 0 || row - rows.first(found - 1) >= rows.count(found - 1)) return;
+  }
+  const float* record = partials + vector * splits * kRecord;
+  const v2f mine = lane < splits ? *reinterpret_cast<const v2f*>(record + lane * kRecord) : v2f{-INFINITY, 0.0f};
+  const float m = group_max<64>(mine[0]), base = m == -INFINITY ? 0.0f : m;
+  const float weight = __builtin_amdgcn_exp2f(mine[0] - base);
+  const float l = wave_sum(mine[1] * weight);
+  const bool empty = mine[0] == -INFINITY && mine[1] == 0.0f;   // (its columns were not written)
+  const int quad = lane % kQuads, at = lane / kQuads;
+  v4f total = {0.0f, 0.0f, 0.0f, 0.0f};
+  for (int s0 = 0; s0 < splits; s0 += kAtOnce) {
+    const int s = s0 + at;
+    const float w = __shfl(weight, min(s, splits - 1), kWave);
+    const bool none = __shfl(static_cast<int>(empty), min(s, splits - 1), kWave) != 0 || s >= splits;
+    if (!none) total += *reinterpret_cast<const v4f*>(record + s * kRecord + kHeader + 4 * quad) * w;
+  }
+#pragma unroll
+  for (int step = kQuads; step < kWave; step *= 2)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) total[e] += __shfl_xor(total[e], step, kWave);
+  if (at != 0) return;
+  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+  T* o = out + vector * D + 4 * quad;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) o[e] = from_float<T>(total[e] * inv);
+}
+
+// rows that a wave takes, in 16ths: what an average sequence has
+int row_tiles(int64_t rows, int sequences, int group, int head_dim) {
+  const int64_t average = rows * group / sequences;
+  const int most = head_dim == 64 ? 4 : head_dim == 128 ? 2 : 1;   // (registers)
+  return average <= 16 || most == 1 ? 1 : average <= 32 || most == 2 ? 2 : 4;
+}
+
+// row groups of the batch (an upper bound: Ragged::find with spare 1)
+int64_t row_groups(int64_t rows, int sequences, int group, int tiles) {
+  return rows * group / (kWaves * 16 * tiles) + sequences;
+}
+
+int split_count(int64_t groups, int kv_heads, int block, int table_width) {
+  const int64_t workgroups = groups * kv_heads, tiles = (static_cast<int64_t>(table_width) * block + kTile - 1) / kTile;
+  const int64_t wanted = 768 / workgroups, most = tiles / 16;
+  return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({wanted, most, kMaxSplits})));
+}
+
+template <typename T> int launch(const Problem& a, int D, int tiles, int64_t groups, hipStream_t s) {
+  const dim3 grid(static_cast<unsigned>(groups * a.splits * a.heads)), block(kThreads);
+#define LLMQ_ATTEND(DIM, NR) hipLaunchKernelGGL((attention_kernel<T, DIM, NR>), grid, block, 0, s, a)
+  if (D == 64) {
+    if (tiles == 1) LLMQ_ATTEND(64, 1);
+    else if (tiles == 2) LLMQ_ATTEND(64, 2);
+    else LLMQ_ATTEND(64, 4);
+  } else if (D == 128) {
+    if (tiles == 1) LLMQ_ATTEND(128, 1);
+    else LLMQ_ATTEND(128, 2);
+  } else {
+    LLMQ_ATTEND(256, 1);
+  }
+#undef LLMQ_ATTEND
+  if (int rc = llmq_host::check_launch("attention_kernel")) return rc;
+  if (a.splits == 1) return 0;
+  const dim3 merge_grid(static_cast<unsigned>((static_cast<int64_t>(a.rows.rows) * a.q_heads + kWaves - 1) / kWaves));
+#define LLMQ_MERGE(DIM) \
+  hipLaunchKernelGGL((merge_kernel<T, DIM>), merge_grid, block, 0, s, a.partials, static_cast<T*>(a.out), a.rows, a.q_heads, a.splits)
+  if (D == 64) LLMQ_MERGE(64);
+  else if (D == 128) LLMQ_MERGE(128);
+  else LLMQ_MERGE(256);
+#undef LLMQ_MERGE
+  return llmq_host::check_launch("merge_kernel");
 }
 
 }  // namespace
 
-extern "C" size_t llmq_kv_block_attention_workspace_bytes(int, int, int, int, int, int, int) { return 0; }
+extern "C" size_t llmq_kv_block_attention_workspace_bytes(int tokens, int sequences, int q_heads, int kv_heads, int head_dim,
+                                                          int block, int table_width) {
+  if (tokens <= 0 || sequences <= 0 || q_heads <= 0 || kv_heads <= 0 || head_dim <= 0 || block <= 0 || table_width <= 0) return 0;
+  const int group = q_heads / kv_heads;
+  if (group == 0) return 0;
+  const int splits = split_count(row_groups(tokens, sequences, group, row_tiles(tokens, sequences, group, head_dim)), kv_heads, block, table_width);
+  return splits == 1 ? 0 : sizeof(float) * static_cast<size_t>(tokens) * q_heads * splits * (head_dim + kHeader);
+}
 
 extern "C" int llmq_kv_block_attention(const void* query, int64_t q_row_stride, const void* k_codes, const void* v_codes,
                                        const float* k_scale, const float* v_scale, const int32_t* block_table,
@@ -82,27 +527,32 @@ extern "C" int llmq_kv_block_attention(const void* query, int64_t q_row_stride, 
   const int v = dtype == LLMQ_F32 ? 4 : 8;
   if (q_row_stride % v) return llmq_host::fail_invalid("row strides must be multiples of %d elements", v);
   if (tokens == 0 || sequences == 0) return 0;
-  if (static_cast<int64_t>(tokens) * q_heads > INT32_MAX / 2)
+  if (n_blocks == 0) table_width = 0;   // no token has a block
+  const int group = q_heads / kv_heads, tiles = row_tiles(tokens, sequences, group, head_dim);
+  // (row numbers, and the launch's workgroups, are counted in 32 bits)
+  const int64_t groups = query_start_or_null ? row_groups(tokens, sequences, group, tiles)
+                                             : static_cast<int64_t>(sequences) * ((group + kWaves * 16 * tiles - 1) / (kWaves * 16 * tiles));
+  const int splits = split_count(row_groups(tokens, sequences, group, tiles), kv_heads, block, table_width);
+  if (static_cast<int64_t>(tokens) * q_heads > INT32_MAX / 2 || groups * splits * kv_heads > INT32_MAX)
     return llmq_host::fail_invalid("too many rows and heads for one launch: %d, %d", tokens, q_heads);
-  const bool empty = n_blocks == 0 || table_width == 0;   // (tensors of no elements have no address)
-  if (!query || !cached || !out || (!empty && (!k_codes || !v_codes || !k_scale || !v_scale || !block_table)))
+  if (!query || !cached || !out || (table_width != 0 && (!k_codes || !v_codes || !k_scale || !v_scale || !block_table)))
     return llmq_host::fail_invalid("null tensor pointer");
+  const size_t need = llmq_kv_block_attention_workspace_bytes(tokens, sequences, q_heads, kv_heads, head_dim, block, table_width);
+  if (workspace_bytes < need || (need && !workspace))
+    return llmq_host::fail_invalid("the workspace has %zu bytes, llmq_kv_block_attention_workspace_bytes() asks for %zu", workspace_bytes, need);
   uintptr_t all = 0;
-  for (const void* t : {query, k_codes, v_codes, static_cast<const void*>(out)}) all |= reinterpret_cast<uintptr_t>(t);
-  if (all & 15u) return llmq_host::fail_invalid("query, codes and out must be 16-byte aligned");
-  const BlockTable table{block_table, table_stride, table_width, n_blocks};
-  const Ragged rows{query_start_or_null, sequences, tokens};
-  const dim3 grid(static_cast<unsigned>(tokens) * q_heads);
+  for (const void* t : {query, k_codes, v_codes, static_cast<const void*>(out), static_cast<const void*>(workspace)})
+    all |= reinterpret_cast<uintptr_t>(t);
+  if (all & 15u) return llmq_host::fail_invalid("query, codes, out and workspace must be 16-byte aligned");
+  int shift = 4;
+  while ((1 << shift) < block) ++shift;
+  const Problem a{query, q_row_stride, static_cast<const int8_t*>(k_codes), static_cast<const int8_t*>(v_codes), k_scale, v_scale,
+                  {block_table, table_stride, table_width, n_blocks}, cached, {query_start_or_null, sequences, tokens}, out,
+                  static_cast<float*>(workspace), splits, q_heads, kv_heads, group, shift, sm_scale * 1.4426950408889634f};
   hipStream_t s = static_cast<hipStream_t>(stream);
-#define LLMQ_ATTEND(T)                                                                                                      \
-  hipLaunchKernelGGL(attention_kernel<T>, grid, dim3(kWave), 0, s, static_cast<const T*>(query), q_row_stride,              \
-                     static_cast<const int8_t*>(k_codes), static_cast<const int8_t*>(v_codes), k_scale, v_scale, table,     \
-                     cached, rows, static_cast<T*>(out), q_heads, kv_heads, head_dim, block, sm_scale * 1.4426950408889634f)
   switch (dtype) {
-    case LLMQ_F32: LLMQ_ATTEND(float); break;
-    case LLMQ_F16: LLMQ_ATTEND(f16_t); break;
-    default: LLMQ_ATTEND(bf16_t); break;
+    case LLMQ_F32: return launch<float>(a, head_dim, tiles, groups, s);
+    case LLMQ_F16: return launch<f16_t>(a, head_dim, tiles, groups, s);
+    default: return launch<bf16_t>(a, head_dim, tiles, groups, s);
   }
-#undef LLMQ_ATTEND
-  return llmq_host::check_launch("attention_kernel");
 }
