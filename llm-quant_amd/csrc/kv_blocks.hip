@@ -4,90 +4,244 @@
 //            s = max(a / 127, 1e-8) where the call writes the block's first token, else max(s_old, that)
 //            codes of the call's tokens: clamp(rint(x / s)); of the block's earlier tokens: clamp(rint((c s_old) / s))
 //   dequant  T(c s)
+//
+// Both take a strip of 16 tokens by eight columns a lane: a packet of 16-bit values for each token, eight bytes of each
+// token's key codes, 16 bytes of each column's value codes (16 tokens innermost), so that the transposition of the
+// values is a choice of bytes within a lane. Bound: HBM, each tensor read once and written once; at a step's few tokens the
+// chain starts -> cached -> table -> block.
 #include "kv_blocks.h"
 
 namespace {
 
 using namespace llmq;
 
-constexpr int kThreads = 256;
+constexpr int kColumns = 8;   // of a lane's strip
 
-__device__ __forceinline__ int64_t code_at(bool value, int64_t id, int h, int heads, int block, int D, int slot, int d) {
-  const int64_t base = (id * heads + h) * block * D;
-  return base + (value ? (static_cast<int64_t>(slot / kStrip) * D + d) * kStrip + slot % kStrip : static_cast<int64_t>(slot) * D + d);
+template <typename T> __device__ __forceinline__ void load8(const T* p, float* f) {
+#pragma unroll
+  for (int i = 0; i < kColumns; i += Pack<T>::N) Pack<T>::unpack(load16(p + i), f + i);
+}
+template <typename T> __device__ __forceinline__ void store8(T* p, const float* f) {
+#pragma unroll
+  for (int i = 0; i < kColumns; i += Pack<T>::N) store16(p + i, Pack<T>::pack(f + i));
+}
+__device__ __forceinline__ float code_of(uint32_t word, int byte) { return static_cast<float>(static_cast<int8_t>(word >> (8 * byte))); }
+__device__ __forceinline__ uint32_t byte_of(float code, int byte) { return (static_cast<uint32_t>(static_cast<int>(code)) & 0xffu) << (8 * byte); }
+
+// The tokens of the call that lie in one block of a sequence.
+struct Touched {
+  int id;          // the block, -1: none
+  int lo, hi;      // its slots lo .. hi - 1
+  int64_t row;     // the row of slot lo
+};
+// `from`: the position of the sequence's first row; piece: which of the blocks from there on. False: no row in that block.
+__device__ __forceinline__ bool touched_block(const BlockTable& table, int b, int64_t first_row, int n, int64_t from, int64_t piece,
+                                              int block_shift, Touched& t) {
+  const int64_t logical = (from >> block_shift) + piece, at = logical << block_shift;
+  if (n == 0 || at > from + n - 1) return false;
+  t.id = logical < table.width ? table.at(b, static_cast<int>(logical)) : -1;
+  t.lo = static_cast<int>(max(from - at, static_cast<int64_t>(0)));
+  t.hi = static_cast<int>(min(from + n - at, static_cast<int64_t>(1) << block_shift));
+  t.row = first_row + (at + t.lo - from);
+  return true;
 }
 
-template <typename T>
-__global__ __launch_bounds__(kThreads) void append_kernel(
+// A head's lanes: (BLOCK / 16) (D / 8), the strips of a block; a workgroup has as many whole heads as 64 lanes hold, or one.
+template <int D, int BLOCK> struct AppendShape {
+  static constexpr int kLanes = BLOCK / kStrip * (D / kColumns);
+  static constexpr int kThreads = kLanes > kWave ? kLanes : kWave, kHeads = kThreads / kLanes;
+};
+
+template <typename T, int D, int BLOCK>
+__global__ __launch_bounds__((AppendShape<D, BLOCK>::kThreads)) void append_kernel(
     const T* __restrict__ key, const T* __restrict__ value, const int64_t key_stride, const int64_t value_stride,
     int8_t* __restrict__ k_codes, int8_t* __restrict__ v_codes, float* __restrict__ k_scale, float* __restrict__ v_scale,
-    const BlockTable table, const int32_t* __restrict__ cached, const Ragged rows, const int heads, const int D, const int block) {
-  __shared__ float red[kThreads / kWave];
+    const BlockTable table, const int32_t* __restrict__ cached, const Ragged rows, const int heads) {
+  using Shape = AppendShape<D, BLOCK>;
+  constexpr int kShift = BLOCK == 16 ? 4 : BLOCK == 32 ? 5 : BLOCK == 64 ? 6 : 7;
+  __shared__ float s_max[Shape::kThreads / kWave];
+  const int sets = (heads + Shape::kHeads - 1) / Shape::kHeads;   // of heads
   const bool is_value = blockIdx.x & 1;
-  const int h = static_cast<int>(blockIdx.x / 2) % heads;
-  int64_t piece = blockIdx.x / 2 / heads;
-  const int b = rows.find(1, block, 2, piece);
-  const int64_t from = cached[b];
-  const int n = rows.count(b);
-  if (from < 0 || n == 0) return;
-  const int64_t logical = from / block + piece;
-  if (logical > (from + n - 1) / block) return;
-  const int id = table.at(b, static_cast<int>(min(logical, static_cast<int64_t>(INT32_MAX))));
-  if (id < 0) return;
-  const int64_t at = logical * block;   // the block's first position
-  const int lo = static_cast<int>(max(from - at, static_cast<int64_t>(0))), hi = static_cast<int>(min(from + n - at, static_cast<int64_t>(block)));
-  const int64_t row0 = rows.first(b) + (at + lo - from);   // the row of slot lo
-  const T* x = (is_value ? value + row0 * value_stride : key + row0 * key_stride) + static_cast<int64_t>(h) * D;
-  const int64_t stride = is_value ? value_stride : key_stride;
-  int8_t* codes = is_value ? v_codes : k_codes;
-  float* scale = (is_value ? v_scale : k_scale) + static_cast<int64_t>(id) * heads + h;
-
-  float amax = 0.0f;
-  for (int i = threadIdx.x; i < (hi - lo) * D; i += kThreads) amax = fmaxf(amax, fabsf(to_float(x[(i / D) * stride + i % D])));
-  amax = group_max<64>(amax);
-  if ((threadIdx.x & (kWave - 1)) == 0) red[threadIdx.x / kWave] = amax;
+  const int set = static_cast<int>(blockIdx.x / 2) % sets;
+  int64_t piece = blockIdx.x / 2 / sets;
+  int b;
+  if (rows.start == nullptr) {
+    b = static_cast<int>(piece);
+    piece = 0;
+  } else {
+    b = rows.find(1, BLOCK, 2, piece);
+  }
+  const int from = cached[b];
+  Touched here;
+  if (from < 0 || !touched_block(table, b, rows.first(b), rows.count(b), from, piece, kShift, here) || here.id < 0) return;
+  const int h = set * Shape::kHeads + static_cast<int>(threadIdx.x) / Shape::kLanes, in_head = threadIdx.x % Shape::kLanes;
+  const int strip = in_head / (D / kColumns), d = in_head % (D / kColumns) * kColumns;
+  const bool active = h < heads;   // (the others stay for the barrier)
+  const int64_t unit = static_cast<int64_t>(here.id) * heads + min(h, heads - 1);
+  float* scale = (is_value ? v_scale : k_scale) + unit;
   const float before = *scale;
-  __syncthreads();
+  // the strip's tokens of the call: lo .. hi - 1 of its 16; the block's earlier ones: below lo
+  const int lo = min(max(here.lo - kStrip * strip, 0), kStrip), hi = active ? min(max(here.hi - kStrip * strip, 0), kStrip) : 0;
+  const int64_t stride = is_value ? value_stride : key_stride;
+  const T* x = (is_value ? value : key) + (here.row + kStrip * strip - here.lo) * stride + static_cast<int64_t>(h) * D + d;
+  constexpr int kPackets = kColumns / Pack<T>::N;
+  u32x4 raw[kStrip][kPackets];
 #pragma unroll
-  for (int w = 0; w < kThreads / kWave; ++w) amax = fmaxf(amax, red[w]);
+  for (int i = 0; i < kStrip; ++i)
+    if (i >= lo && i < hi) {
+#pragma unroll
+      for (int e = 0; e < kPackets; ++e) raw[i][e] = load16(x + i * stride + e * Pack<T>::N);
+    } else {
+#pragma unroll
+      for (int e = 0; e < kPackets; ++e) raw[i][e] = u32x4{0u, 0u, 0u, 0u};
+    }
+  float amax = 0.0f;
+#pragma unroll
+  for (int i = 0; i < kStrip; ++i) {
+    float f[kColumns];
+#pragma unroll
+    for (int e = 0; e < kPackets; ++e) Pack<T>::unpack(raw[i][e], f + e * Pack<T>::N);
+#pragma unroll
+    for (int e = 0; e < kColumns; ++e) amax = fmaxf(amax, fabsf(f[e]));
+  }
+  amax = group_max<(Shape::kLanes < kWave ? Shape::kLanes : kWave)>(amax);
+  if constexpr (Shape::kThreads > kWave) {
+    if (threadIdx.x % kWave == 0) s_max[threadIdx.x / kWave] = amax;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < Shape::kThreads / kWave; ++w) amax = fmaxf(amax, s_max[w]);
+  }
+  if (!active) return;
   float s = scale_from_amax(amax, 127.0f);
-  if (lo > 0) s = fmaxf(s, before);
-  if (threadIdx.x == 0) *scale = s;
-  if (s > before) {
-    for (int i = threadIdx.x; i < lo * D; i += kThreads) {
-      int8_t* c = codes + code_at(is_value, id, h, heads, block, D, i / D, i % D);
-      *c = static_cast<int8_t>(quant_code(static_cast<float>(*c) * before, s, -128.0f, 127.0f));
+  if (here.lo > 0) s = fmaxf(s, before);
+  const bool grown = here.lo > 0 && s > before;
+  if (in_head == 0) *scale = s;
+  if (hi <= lo && !(grown && lo > 0)) return;   // nothing of this strip changes
+
+  const auto moved = [&](uint32_t word, int byte) { return byte_of(quant_code(code_of(word, byte) * before, s, -128.0f, 127.0f), byte); };
+  const auto codes_of = [&](int i, float* f) {
+#pragma unroll
+    for (int e = 0; e < kPackets; ++e) Pack<T>::unpack(raw[i][e], f + e * Pack<T>::N);
+#pragma unroll
+    for (int e = 0; e < kColumns; ++e) f[e] = quant_code(f[e], s, -128.0f, 127.0f);
+  };
+  if (!is_value) {
+    int8_t* codes = k_codes + (unit * BLOCK + kStrip * strip) * D + d;
+#pragma unroll
+    for (int i = 0; i < kStrip; ++i) {
+      u32x2* at = reinterpret_cast<u32x2*>(codes + i * D);
+      if (i >= lo && i < hi) {
+        float f[kColumns];
+        codes_of(i, f);
+        *at = u32x2{byte_of(f[0], 0) | byte_of(f[1], 1) | byte_of(f[2], 2) | byte_of(f[3], 3),
+                    byte_of(f[4], 0) | byte_of(f[5], 1) | byte_of(f[6], 2) | byte_of(f[7], 3)};
+      } else if (grown && i < lo) {
+        const u32x2 w = *at;
+        *at = u32x2{moved(w.x, 0) | moved(w.x, 1) | moved(w.x, 2) | moved(w.x, 3),
+                    moved(w.y, 0) | moved(w.y, 1) | moved(w.y, 2) | moved(w.y, 3)};
+      }
+    }
+    return;
+  }
+  int8_t* codes = v_codes + ((unit * (BLOCK / kStrip) + strip) * D + d) * kStrip;
+  if (hi - lo == 1 && !(grown && lo > 0)) {   // a token: its bytes alone (a step's; nothing is read)
+#pragma unroll
+    for (int i = 0; i < kStrip; ++i)
+      if (i == lo) {
+        float f[kColumns];
+        codes_of(i, f);
+#pragma unroll
+        for (int e = 0; e < kColumns; ++e) codes[e * kStrip + i] = static_cast<int8_t>(f[e]);
+      }
+    return;
+  }
+  uint32_t words[kColumns][kStrip / 4] = {};
+  if (hi > lo) {
+#pragma unroll
+    for (int i = 0; i < kStrip; ++i) {
+      float f[kColumns];
+      codes_of(i, f);
+#pragma unroll
+      for (int e = 0; e < kColumns; ++e) words[e][i / 4] |= byte_of(f[e], i % 4);
     }
   }
-  for (int i = threadIdx.x; i < (hi - lo) * D; i += kThreads) {
-    const float f = to_float(x[(i / D) * stride + i % D]);
-    codes[code_at(is_value, id, h, heads, block, D, lo + i / D, i % D)] = static_cast<int8_t>(quant_code(f, s, -128.0f, 127.0f));
+  if (lo > 0 || hi < kStrip) {   // bytes of other tokens lie among them
+    uint32_t fresh[kStrip / 4] = {}, old[kStrip / 4] = {};
+#pragma unroll
+    for (int i = 0; i < kStrip; ++i) {
+      fresh[i / 4] |= i >= lo && i < hi ? 0xffu << (8 * (i % 4)) : 0u;
+      old[i / 4] |= grown && i < lo ? 0xffu << (8 * (i % 4)) : 0u;
+    }
+#pragma unroll
+    for (int e = 0; e < kColumns; ++e) {
+      const u32x4 r = load16(codes + e * kStrip);
+      const uint32_t held[kStrip / 4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+      for (int w = 0; w < kStrip / 4; ++w) {
+        uint32_t kept = held[w];
+        if (old[w] != 0u) kept = (kept & ~old[w]) | ((moved(kept, 0) | moved(kept, 1) | moved(kept, 2) | moved(kept, 3)) & old[w]);
+        words[e][w] = (kept & ~fresh[w]) | (words[e][w] & fresh[w]);
+      }
+    }
   }
+#pragma unroll
+  for (int e = 0; e < kColumns; ++e) store16(codes + e * kStrip, u32x4{words[e][0], words[e][1], words[e][2], words[e][3]});
 }
 
-template <typename T>
-__global__ __launch_bounds__(kThreads) void dequant_kernel(
+constexpr int kDequantThreads = 256;
+
+// The lanes of a block: strips of all its heads, keys and values in workgroups of their own.
+template <typename T, int D>
+__global__ __launch_bounds__(kDequantThreads) void dequant_kernel(
     const int8_t* __restrict__ k_codes, const int8_t* __restrict__ v_codes, const float* __restrict__ k_scale,
     const float* __restrict__ v_scale, const BlockTable table, const Ragged rows, const int32_t* __restrict__ first_or_null,
-    T* __restrict__ k_out, T* __restrict__ v_out, const int heads, const int D, const int block) {
+    T* __restrict__ k_out, T* __restrict__ v_out, const int heads, const int block_shift) {
+  const int strips = 1 << (block_shift - 4), lanes = heads * strips * (D / kColumns), sets = (lanes + kDequantThreads - 1) / kDequantThreads;
   const bool is_value = blockIdx.x & 1;
-  const int h = static_cast<int>(blockIdx.x / 2) % heads;
-  int64_t piece = blockIdx.x / 2 / heads;
-  const int b = rows.find(1, block, 2, piece);
-  const int64_t from = first_or_null == nullptr ? 0 : max(first_or_null[b], 0);
-  const int n = rows.count(b);
-  const int64_t logical = from / block + piece;
-  if (n == 0 || logical > (from + n - 1) / block) return;
-  const int id = table.at(b, static_cast<int>(min(logical, static_cast<int64_t>(INT32_MAX))));
-  const int64_t at = logical * block;
-  const int lo = static_cast<int>(max(from - at, static_cast<int64_t>(0))), hi = static_cast<int>(min(from + n - at, static_cast<int64_t>(block)));
-  const int64_t row0 = rows.first(b) + (at + lo - from);
-  T* out = (is_value ? v_out : k_out) + (static_cast<int64_t>(h) * rows.rows + row0) * D;
-  const int8_t* codes = is_value ? v_codes : k_codes;
-  const float s = id < 0 ? 0.0f : (is_value ? v_scale : k_scale)[static_cast<int64_t>(id) * heads + h];
-  for (int i = threadIdx.x; i < (hi - lo) * D; i += kThreads) {
-    const float c = id < 0 ? 0.0f : static_cast<float>(codes[code_at(is_value, id, h, heads, block, D, lo + i / D, i % D)]);
-    out[i] = from_float<T>(c * s);
+  const int set = static_cast<int>(blockIdx.x / 2) % sets;
+  int64_t piece = blockIdx.x / 2 / sets;
+  const int b = rows.find(1, strips * kStrip, 2, piece);
+  Touched here;
+  if (!touched_block(table, b, rows.first(b), rows.count(b), first_or_null == nullptr ? 0 : max(first_or_null[b], 0), piece, block_shift, here)) return;
+  const int item = set * kDequantThreads + static_cast<int>(threadIdx.x);
+  if (item >= lanes) return;
+  const int d = item % (D / kColumns) * kColumns, strip = item / (D / kColumns) % strips, h = item / (D / kColumns) / strips;
+  const int lo = max(here.lo - kStrip * strip, 0), hi = min(here.hi - kStrip * strip, kStrip);
+  if (hi <= lo) return;
+  const int64_t unit = static_cast<int64_t>(max(here.id, 0)) * heads + h;
+  T* out = (is_value ? v_out : k_out) + (static_cast<int64_t>(h) * rows.rows + here.row + kStrip * strip - here.lo) * D + d;
+  uint32_t words[kStrip][2] = {};   // keys: a token's eight codes; values: [column][half the strip]
+  float s = 0.0f;
+  if (here.id >= 0) {
+    s = (is_value ? v_scale : k_scale)[unit];
+    if (is_value) {
+      const int8_t* codes = v_codes + ((unit * strips + strip) * D + d) * kStrip;
+#pragma unroll
+      for (int e = 0; e < kColumns; ++e) {
+        const u32x4 r = load16(codes + e * kStrip);
+        words[2 * e][0] = r.x;
+        words[2 * e][1] = r.y;
+        words[2 * e + 1][0] = r.z;
+        words[2 * e + 1][1] = r.w;
+      }
+    } else {
+      const int8_t* codes = k_codes + ((unit * strips + strip) * kStrip) * D + d;
+#pragma unroll
+      for (int i = 0; i < kStrip; ++i) {
+        const u32x2 r = *reinterpret_cast<const u32x2*>(codes + i * D);
+        words[i][0] = r.x;
+        words[i][1] = r.y;
+      }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < kStrip; ++i) {
+    if (i < lo || i >= hi) continue;
+    float f[kColumns];
+#pragma unroll
+    for (int e = 0; e < kColumns; ++e)
+      f[e] = (is_value ? code_of(words[2 * e + i / 8][i / 4 % 2], i % 4) : code_of(words[i][e / 4], e % 4)) * s;
+    store8(out + static_cast<int64_t>(i) * D, f);
   }
 }
 
@@ -134,17 +288,34 @@ extern "C" int llmq_kv_block_append(const void* key, const void* value, int64_t 
     return llmq_host::fail_invalid("key and value must be 16-byte aligned");
   const BlockTable table{block_table, table_stride, table_width, n_blocks};
   const Ragged rows{query_start_or_null, sequences, tokens};
-  const dim3 grid(static_cast<unsigned>(pieces(tokens, sequences, block) * 2 * kv_heads));
+  const int64_t n_pieces = query_start_or_null ? pieces(tokens, sequences, block) : sequences;
   hipStream_t s = static_cast<hipStream_t>(stream);
-#define LLMQ_APPEND(T)                                                                                                       \
-  hipLaunchKernelGGL(append_kernel<T>, grid, dim3(kThreads), 0, s, static_cast<const T*>(key), static_cast<const T*>(value), \
+#define LLMQ_APPEND(T, D, BLOCK)                                                                                             \
+  hipLaunchKernelGGL((append_kernel<T, D, BLOCK>),                                                                           \
+                     dim3(static_cast<unsigned>(n_pieces * 2 * ((kv_heads + AppendShape<D, BLOCK>::kHeads - 1) / AppendShape<D, BLOCK>::kHeads))), \
+                     dim3(AppendShape<D, BLOCK>::kThreads), 0, s, static_cast<const T*>(key), static_cast<const T*>(value),  \
                      key_row_stride, value_row_stride, static_cast<int8_t*>(k_codes), static_cast<int8_t*>(v_codes),         \
-                     k_scale, v_scale, table, cached, rows, kv_heads, head_dim, block)
-  switch (dtype) {
-    case LLMQ_F32: LLMQ_APPEND(float); break;
-    case LLMQ_F16: LLMQ_APPEND(f16_t); break;
-    default: LLMQ_APPEND(bf16_t); break;
+                     k_scale, v_scale, table, cached, rows, kv_heads)
+#define LLMQ_APPEND_D(T, D)                        \
+  switch (block) {                                 \
+    case 16: LLMQ_APPEND(T, D, 16); break;         \
+    case 32: LLMQ_APPEND(T, D, 32); break;         \
+    case 64: LLMQ_APPEND(T, D, 64); break;         \
+    default: LLMQ_APPEND(T, D, 128); break;        \
   }
+#define LLMQ_APPEND_T(T)                           \
+  switch (head_dim) {                              \
+    case 64: LLMQ_APPEND_D(T, 64); break;          \
+    case 128: LLMQ_APPEND_D(T, 128); break;        \
+    default: LLMQ_APPEND_D(T, 256); break;         \
+  }
+  switch (dtype) {
+    case LLMQ_F32: LLMQ_APPEND_T(float); break;
+    case LLMQ_F16: LLMQ_APPEND_T(f16_t); break;
+    default: LLMQ_APPEND_T(bf16_t); break;
+  }
+#undef LLMQ_APPEND_T
+#undef LLMQ_APPEND_D
 #undef LLMQ_APPEND
   return llmq_host::check_launch("append_kernel");
 }
@@ -163,17 +334,30 @@ extern "C" int llmq_kv_block_dequant(const void* k_codes, const void* v_codes, c
     return llmq_host::fail_invalid("the outputs must be 16-byte aligned");
   const BlockTable table{block_table, table_stride, table_width, n_blocks};
   const Ragged rows{starts, sequences, n_tokens};
-  const dim3 grid(static_cast<unsigned>(pieces(n_tokens, sequences, block) * 2 * kv_heads));
+  int shift = 4;
+  while ((1 << shift) < block) ++shift;
+  const int64_t lanes = static_cast<int64_t>(kv_heads) * (block / kStrip) * (head_dim / kColumns);
+  const int64_t workgroups = pieces(n_tokens, sequences, block) * 2 * ((lanes + kDequantThreads - 1) / kDequantThreads);
+  if (lanes > INT32_MAX - kDequantThreads || workgroups > INT32_MAX)
+    return llmq_host::fail_invalid("too many rows, sequences and heads for one launch: %d, %d, %d", n_tokens, sequences, kv_heads);
+  const dim3 grid(static_cast<unsigned>(workgroups));
   hipStream_t s = static_cast<hipStream_t>(stream);
-#define LLMQ_DEQUANT(T)                                                                                                  \
-  hipLaunchKernelGGL(dequant_kernel<T>, grid, dim3(kThreads), 0, s, static_cast<const int8_t*>(k_codes),                 \
+#define LLMQ_DEQUANT(T, D)                                                                                               \
+  hipLaunchKernelGGL((dequant_kernel<T, D>), grid, dim3(kDequantThreads), 0, s, static_cast<const int8_t*>(k_codes),     \
                      static_cast<const int8_t*>(v_codes), k_scale, v_scale, table, rows, first_or_null,                  \
-                     static_cast<T*>(k_out), static_cast<T*>(v_out), kv_heads, head_dim, block)
-  switch (dtype) {
-    case LLMQ_F32: LLMQ_DEQUANT(float); break;
-    case LLMQ_F16: LLMQ_DEQUANT(f16_t); break;
-    default: LLMQ_DEQUANT(bf16_t); break;
+                     static_cast<T*>(k_out), static_cast<T*>(v_out), kv_heads, shift)
+#define LLMQ_DEQUANT_T(T)                       \
+  switch (head_dim) {                           \
+    case 64: LLMQ_DEQUANT(T, 64); break;        \
+    case 128: LLMQ_DEQUANT(T, 128); break;      \
+    default: LLMQ_DEQUANT(T, 256); break;       \
   }
+  switch (dtype) {
+    case LLMQ_F32: LLMQ_DEQUANT_T(float); break;
+    case LLMQ_F16: LLMQ_DEQUANT_T(f16_t); break;
+    default: LLMQ_DEQUANT_T(bf16_t); break;
+  }
+#undef LLMQ_DEQUANT_T
 #undef LLMQ_DEQUANT
   return llmq_host::check_launch("dequant_kernel");
 }
