@@ -34,7 +34,10 @@ typedef float v2f __attribute__((ext_vector_type(2)));
 
 constexpr int kWaves = 4, kThreads = kWaves * kWave, kTile = 64;
 constexpr int kHeader = 4;            // floats in front of a partial result: maximum, sum, two of nothing
-constexpr int kMaxSplits = 64;
+constexpr int kMaxSplits = 64;        // of a row: what a wave's lanes hold
+constexpr int kUnits = 1024;          // workgroups that the work is cut for: two rounds of those resident with heads of 128
+constexpr int kLeastTiles = 8;        // of a split: two for each wave
+constexpr int kMostRecords = 1 << 16; // partial results of a launch (more would cost more than they save)
 constexpr float kBias = 1152.0f;      // what a code is too high as an operand: 1024, and 128 of the flipped sign
 constexpr float kNoScale = 0x1p-100f; // value scales below count as zero
 constexpr float kPiece = 2048.0f;     // the second piece of an fp32 number is this much too high
@@ -48,10 +51,72 @@ struct Problem {
   const int32_t* cached;
   Ragged rows;
   void* out;
-  float* partials;
+  int32_t* split_counts;   // [rows, q_heads]: how many partial results there are
+  float* partials;         // [rows, q_heads, splits]
   int splits, q_heads, heads, group, block_shift;
   float scale_log2e;
 };
+
+__device__ __forceinline__ int wave_total(int v) {
+  v = row16_sum(v);
+  return (__builtin_amdgcn_readlane(v, 0) + __builtin_amdgcn_readlane(v, 16)) + (__builtin_amdgcn_readlane(v, 32) + __builtin_amdgcn_readlane(v, 48));
+}
+// sum over the lanes up to and with this one
+__device__ __forceinline__ int wave_prefix(int v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, true);   // from 1, 2, 4 and 8 lanes below within a row of 16
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, true);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, true);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, true);
+  const int row = (threadIdx.x & (kWave - 1)) >> 4, a = __builtin_amdgcn_readlane(v, 15), b = __builtin_amdgcn_readlane(v, 31),
+            c = __builtin_amdgcn_readlane(v, 47);
+  return v + (row > 0 ? a : 0) + (row > 1 ? b : 0) + (row > 2 ? c : 0);
+}
+
+// Where a sequence's work lies: `groups` row groups of `tiles` tiles of 64 tokens (its last row's).
+struct Work {
+  int groups, tiles;
+};
+__device__ __forceinline__ Work work_of(const Problem& a, int b, int group_rows) {
+  const int n = a.rows.count(b), cached = a.cached[b];
+  const int64_t held = min(static_cast<int64_t>(a.table.width) << a.block_shift, static_cast<int64_t>(INT32_MAX - 2 * kTile));
+  const int seen = cached < 0 ? 0 : static_cast<int>(min(static_cast<int64_t>(cached) + n, held));
+  return Work{(n * a.group + group_rows - 1) / group_rows, (seen + kTile - 1) / kTile};
+}
+// The piece of work of a workgroup, found by each of its waves.
+struct Unit {
+  int b, row_group, split, splits;   // splits of this sequence
+};
+// Lengths lie on the device: how the tokens are cut is decided here, the same way by everyone. All units are of about as many
+// tiles, C = max(kLeastTiles, all tiles / (kUnits / heads)), a sequence is cut into ceil(tiles / C) equal splits, at most
+// a.splits; so there are at most sum(groups (tiles / C + 1)) <= kUnits / heads + groups of them, the launch's size.
+__device__ __forceinline__ bool find_unit(const Problem& a, int group_rows, int64_t index, Unit& u) {
+  const int lane = threadIdx.x & (kWave - 1), sequences = a.rows.sequences;
+  int64_t all = 0;
+  Work w{0, 0};
+  for (int b0 = 0; b0 < sequences; b0 += kWave) {
+    w = b0 + lane < sequences ? work_of(a, b0 + lane, group_rows) : Work{0, 0};
+    const int64_t product = static_cast<int64_t>(w.groups) * w.tiles;
+    all += wave_total(static_cast<int>(product & 0xffff)) + (static_cast<int64_t>(wave_total(static_cast<int>(product >> 16))) << 16);
+  }
+  const int64_t wanted = (kUnits + a.heads - 1) / a.heads;
+  const int size = static_cast<int>(max((all + wanted - 1) / wanted, static_cast<int64_t>(kLeastTiles)));
+  for (int b0 = 0; b0 < sequences; b0 += kWave) {
+    if (sequences > kWave) w = b0 + lane < sequences ? work_of(a, b0 + lane, group_rows) : Work{0, 0};   // (else the one above)
+    const int splits = max(min((w.tiles + size - 1) / size, a.splits), 1), units = w.groups * splits, up_to = wave_prefix(units);
+    const int total = __builtin_amdgcn_readlane(up_to, kWave - 1);
+    if (index < total) {
+      const int at = __popcll(__ballot(up_to <= index));   // (the first lane whose units reach beyond the index)
+      u.b = b0 + at;
+      u.splits = __builtin_amdgcn_readlane(splits, at);
+      const int within = static_cast<int>(index) - (__builtin_amdgcn_readlane(up_to, at) - __builtin_amdgcn_readlane(units, at));
+      u.row_group = within / u.splits;
+      u.split = within % u.splits;
+      return true;
+    }
+    index -= total;
+  }
+  return false;
+}
 
 template <typename T> struct Pieces { static constexpr int N = 1; };
 template <> struct Pieces<float> { static constexpr int N = 2; };
@@ -130,17 +195,21 @@ __global__ __launch_bounds__(kThreads, 2) void attention_kernel(const Problem a)
   const int tid = threadIdx.x, lane = tid & (kWave - 1), r16 = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
   // key heads fastest: with eight of them each XCD's cache holds one. Late rows, which see most, first.
-  const int h = blockIdx.x % a.heads, rest = blockIdx.x / a.heads, split = rest % a.splits;
-  int64_t piece = gridDim.x / a.heads / a.splits - 1 - rest / a.splits;
-  int b;
-  if (a.rows.start == nullptr) {
+  const int h = blockIdx.x % a.heads;
+  int64_t piece = gridDim.x / a.heads - 1 - blockIdx.x / a.heads;
+  Unit unit{0, 0, 0, 1};
+  if (a.splits > 1) {
+    if (!find_unit(a, kGroupRows, piece, unit)) return;
+  } else if (a.rows.start == nullptr) {
     const int per = (a.group + kGroupRows - 1) / kGroupRows;
-    b = static_cast<int>(piece / per);
-    piece %= per;
+    unit.b = static_cast<int>(piece / per);
+    unit.row_group = static_cast<int>(piece % per);
   } else {
-    b = a.rows.find(a.group, kGroupRows, 1, piece);
+    unit.b = a.rows.find(a.group, kGroupRows, 1, piece);
+    unit.row_group = static_cast<int>(min(piece, static_cast<int64_t>(INT32_MAX / kGroupRows)));
   }
-  const int n_rows = a.rows.count(b) * a.group, row0 = static_cast<int>(min(piece * kGroupRows, static_cast<int64_t>(INT32_MAX)));
+  const int b = unit.b, split = unit.split;
+  const int n_rows = a.rows.count(b) * a.group, row0 = unit.row_group * kGroupRows;
   if (row0 >= n_rows) return;
   const int first_row = a.rows.first(b), cached = a.cached[b];
   const int here = min(n_rows - row0, kGroupRows), tiles_of_rows = (here + kRows - 1) / kRows;
@@ -194,7 +263,7 @@ __global__ __launch_bounds__(kThreads, 2) void attention_kernel(const Problem a)
     const int64_t newest = cached < 0 ? -1 : static_cast<int64_t>(cached) + (min(row0 + (my_tile + 1) * kRows, n_rows) - 1) / a.group;
     seen_last = static_cast<int>(min(min(newest, held - 1), static_cast<int64_t>(INT32_MAX - 2 * kTile)));
   }
-  const int tiles = (seen_last + kTile) / kTile, per_split = (tiles + a.splits - 1) / a.splits;
+  const int tiles = (seen_last + kTile) / kTile, per_split = (tiles + unit.splits - 1) / unit.splits;
   const int begin = split * per_split, end = min(begin + per_split, tiles);
 
   // the blocks of a tile's strips: for its keys a lane reads strip r16 / 4, for its values and scales strip g
@@ -400,7 +469,8 @@ __global__ __launch_bounds__(kThreads, 2) void attention_kernel(const Problem a)
     }
     const int token = (row0 + row) / a.group, head = h * a.group + (row0 + row) % a.group;
     const int64_t vector = static_cast<int64_t>(first_row + token) * a.q_heads + head;
-    if (a.splits == 1) {
+    if (a.splits > 1 && split == 0 && d == 0) a.split_counts[vector] = unit.splits;
+    if (unit.splits == 1) {
       const float inv = l == 0.0f ? 0.0f : 1.0f / l;
 #pragma unroll
       for (int e = 0; e < 8; ++e) f[e] *= inv;
@@ -413,49 +483,46 @@ __global__ __launch_bounds__(kThreads, 2) void attention_kernel(const Problem a)
   }
 }
 
-// The splits' records of a row and head, by a wave: a lane holds a split's maximum and sum, then four columns of every
-// 64 / (D / 4)-th record.
+// The partial results of a row and head, by a workgroup: four columns of every kAtOnce-th of them a thread, all asked for at once.
 template <typename T, int D>
-__global__ __launch_bounds__(kThreads) void merge_kernel(const float* __restrict__ partials, T* __restrict__ out, const Ragged rows,
-                                                         const int q_heads, const int splits) {
-  constexpr int kQuads = D / 4, kAtOnce = kWave / kQuads, kRecord = D + kHeader;
-  const int lane = threadIdx.x & (kWave - 1);
-  const int64_t vector = static_cast<int64_t>(blockIdx.x) * kWaves + __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-  if (vector >= static_cast<int64_t>(rows.rows) * q_heads) return;
-  if (rows.start != nullptr) {   // rows of no sequence have no records
-    const int row = static_cast<int>(vector / q_heads);
-    int found = 0;
-    for (int b0 = 0; b0 < rows.sequences; b0 += kWave) {
-      const int b = b0 + lane;
-      const int n = __popcll(__ballot(b < rows.sequences && rows.first(b) <= row));
-      found += n;
-      if (n < kWave) break;
-    }
-    if (found == 0 || row - rows.first(found - 1) >= rows.count(found - 1)) return;
+__global__ __launch_bounds__(kThreads) void merge_kernel(const Problem a) {
+  constexpr int kQuads = D / 4, kAtOnce = kThreads / kQuads, kEach = kMaxSplits / kAtOnce, kRecord = D + kHeader;
+  __shared__ __attribute__((aligned(16))) float s_part[kAtOnce][D];
+  const int tid = threadIdx.x, lane = tid & (kWave - 1), quad = tid % kQuads, at = tid / kQuads;
+  const int64_t vector = blockIdx.x;
+  if (a.rows.start != nullptr) {   // rows of no sequence have none
+    const int row = static_cast<int>(vector / a.q_heads);
+    if (row < a.rows.first(0) || row >= a.rows.first(a.rows.sequences)) return;
   }
-  const float* record = partials + vector * splits * kRecord;
+  const int splits = min(a.split_counts[vector], a.splits);
+  if (splits <= 1) return;   // (written by its only one)
+  const float* record = a.partials + vector * a.splits * kRecord;
+  v4f part[kEach];
+#pragma unroll
+  for (int i = 0; i < kEach; ++i)
+    part[i] = at + i * kAtOnce < splits ? *reinterpret_cast<const v4f*>(record + (at + i * kAtOnce) * kRecord + kHeader + 4 * quad) : v4f{0.0f, 0.0f, 0.0f, 0.0f};
   const v2f mine = lane < splits ? *reinterpret_cast<const v2f*>(record + lane * kRecord) : v2f{-INFINITY, 0.0f};
   const float m = group_max<64>(mine[0]), base = m == -INFINITY ? 0.0f : m;
   const float weight = __builtin_amdgcn_exp2f(mine[0] - base);
   const float l = wave_sum(mine[1] * weight);
-  const bool empty = mine[0] == -INFINITY && mine[1] == 0.0f;   // (its columns were not written)
-  const int quad = lane % kQuads, at = lane / kQuads;
   v4f total = {0.0f, 0.0f, 0.0f, 0.0f};
-  for (int s0 = 0; s0 < splits; s0 += kAtOnce) {
-    const int s = s0 + at;
-    const float w = __shfl(weight, min(s, splits - 1), kWave);
-    const bool none = __shfl(static_cast<int>(empty), min(s, splits - 1), kWave) != 0 || s >= splits;
-    if (!none) total += *reinterpret_cast<const v4f*>(record + s * kRecord + kHeader + 4 * quad) * w;
+#pragma unroll
+  for (int i = 0; i < kEach; ++i) {
+    const float w = __shfl(weight, (at + i * kAtOnce) & (kWave - 1), kWave);
+    if (w != 0.0f) total += part[i] * w;   // (a split that saw nothing has written no columns)
   }
+  *reinterpret_cast<v4f*>(&s_part[at][4 * quad]) = total;
+  __syncthreads();
+  if (tid >= D / 8) return;
+  float f[8] = {};
 #pragma unroll
-  for (int step = kQuads; step < kWave; step *= 2)
+  for (int i = 0; i < kAtOnce; ++i)
 #pragma unroll
-    for (int e = 0; e < 4; ++e) total[e] += __shfl_xor(total[e], step, kWave);
-  if (at != 0) return;
+    for (int e = 0; e < 8; ++e) f[e] += s_part[i][8 * tid + e];
   const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-  T* o = out + vector * D + 4 * quad;
 #pragma unroll
-  for (int e = 0; e < 4; ++e) o[e] = from_float<T>(total[e] * inv);
+  for (int e = 0; e < 8; ++e) f[e] *= inv;
+  store8(static_cast<T*>(a.out) + vector * D + 8 * tid, f);
 }
 
 // rows that a wave takes, in 16ths: what an average sequence has
@@ -470,14 +537,16 @@ int64_t row_groups(int64_t rows, int sequences, int group, int tiles) {
   return rows * group / (kWaves * 16 * tiles) + sequences;
 }
 
-int split_count(int64_t groups, int kv_heads, int block, int table_width) {
-  const int64_t workgroups = groups * kv_heads, tiles = (static_cast<int64_t>(table_width) * block + kTile - 1) / kTile;
-  const int64_t wanted = 768 / workgroups, most = tiles / 16;
-  return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({wanted, most, kMaxSplits})));
+// Partial results that a row can have, 1: none. By the table's width, the longest that a sequence can be.
+int most_splits(int64_t vectors, int block, int table_width) {
+  const int64_t tiles = (static_cast<int64_t>(table_width) * block + kTile - 1) / kTile;
+  if (tiles < 2 * kLeastTiles) return 1;   // (a second launch costs more than half of so short a walk)
+  return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({(tiles + kLeastTiles - 1) / kLeastTiles, kMostRecords / vectors, kMaxSplits})));
 }
+size_t counts_bytes(int64_t vectors) { return (static_cast<size_t>(vectors) * sizeof(int32_t) + 15) / 16 * 16; }
 
 template <typename T> int launch(const Problem& a, int D, int tiles, int64_t groups, hipStream_t s) {
-  const dim3 grid(static_cast<unsigned>(groups * a.splits * a.heads)), block(kThreads);
+  const dim3 grid(static_cast<unsigned>(groups * a.heads)), block(kThreads);
 #define LLMQ_ATTEND(DIM, NR) hipLaunchKernelGGL((attention_kernel<T, DIM, NR>), grid, block, 0, s, a)
   if (D == 64) {
     if (tiles == 1) LLMQ_ATTEND(64, 1);
@@ -492,9 +561,8 @@ template <typename T> int launch(const Problem& a, int D, int tiles, int64_t gro
 #undef LLMQ_ATTEND
   if (int rc = llmq_host::check_launch("attention_kernel")) return rc;
   if (a.splits == 1) return 0;
-  const dim3 merge_grid(static_cast<unsigned>((static_cast<int64_t>(a.rows.rows) * a.q_heads + kWaves - 1) / kWaves));
-#define LLMQ_MERGE(DIM) \
-  hipLaunchKernelGGL((merge_kernel<T, DIM>), merge_grid, block, 0, s, a.partials, static_cast<T*>(a.out), a.rows, a.q_heads, a.splits)
+  const dim3 merge_grid(static_cast<unsigned>(a.rows.rows) * a.q_heads);
+#define LLMQ_MERGE(DIM) hipLaunchKernelGGL((merge_kernel<T, DIM>), merge_grid, block, 0, s, a)
   if (D == 64) LLMQ_MERGE(64);
   else if (D == 128) LLMQ_MERGE(128);
   else LLMQ_MERGE(256);
@@ -507,10 +575,9 @@ template <typename T> int launch(const Problem& a, int D, int tiles, int64_t gro
 extern "C" size_t llmq_kv_block_attention_workspace_bytes(int tokens, int sequences, int q_heads, int kv_heads, int head_dim,
                                                           int block, int table_width) {
   if (tokens <= 0 || sequences <= 0 || q_heads <= 0 || kv_heads <= 0 || head_dim <= 0 || block <= 0 || table_width <= 0) return 0;
-  const int group = q_heads / kv_heads;
-  if (group == 0) return 0;
-  const int splits = split_count(row_groups(tokens, sequences, group, row_tiles(tokens, sequences, group, head_dim)), kv_heads, block, table_width);
-  return splits == 1 ? 0 : sizeof(float) * static_cast<size_t>(tokens) * q_heads * splits * (head_dim + kHeader);
+  const int64_t vectors = static_cast<int64_t>(tokens) * q_heads;
+  const int splits = most_splits(vectors, block, table_width);
+  return splits == 1 ? 0 : counts_bytes(vectors) + sizeof(float) * static_cast<size_t>(vectors) * splits * (head_dim + kHeader);
 }
 
 extern "C" int llmq_kv_block_attention(const void* query, int64_t q_row_stride, const void* k_codes, const void* v_codes,
@@ -530,10 +597,12 @@ extern "C" int llmq_kv_block_attention(const void* query, int64_t q_row_stride, 
   if (n_blocks == 0) table_width = 0;   // no token has a block
   const int group = q_heads / kv_heads, tiles = row_tiles(tokens, sequences, group, head_dim);
   // (row numbers, and the launch's workgroups, are counted in 32 bits)
-  const int64_t groups = query_start_or_null ? row_groups(tokens, sequences, group, tiles)
-                                             : static_cast<int64_t>(sequences) * ((group + kWaves * 16 * tiles - 1) / (kWaves * 16 * tiles));
-  const int splits = split_count(row_groups(tokens, sequences, group, tiles), kv_heads, block, table_width);
-  if (static_cast<int64_t>(tokens) * q_heads > INT32_MAX / 2 || groups * splits * kv_heads > INT32_MAX)
+  const int64_t vectors = static_cast<int64_t>(tokens) * q_heads;
+  const int splits = most_splits(vectors, block, table_width);
+  const int64_t groups = splits > 1            ? row_groups(tokens, sequences, group, tiles) + (kUnits + kv_heads - 1) / kv_heads
+                         : query_start_or_null ? row_groups(tokens, sequences, group, tiles)
+                                               : static_cast<int64_t>(sequences) * ((group + kWaves * 16 * tiles - 1) / (kWaves * 16 * tiles));
+  if (vectors > INT32_MAX / 2 || groups * kv_heads > INT32_MAX)
     return llmq_host::fail_invalid("too many rows and heads for one launch: %d, %d", tokens, q_heads);
   if (!query || !cached || !out || (table_width != 0 && (!k_codes || !v_codes || !k_scale || !v_scale || !block_table)))
     return llmq_host::fail_invalid("null tensor pointer");
@@ -548,7 +617,8 @@ extern "C" int llmq_kv_block_attention(const void* query, int64_t q_row_stride, 
   while ((1 << shift) < block) ++shift;
   const Problem a{query, q_row_stride, static_cast<const int8_t*>(k_codes), static_cast<const int8_t*>(v_codes), k_scale, v_scale,
                   {block_table, table_stride, table_width, n_blocks}, cached, {query_start_or_null, sequences, tokens}, out,
-                  static_cast<float*>(workspace), splits, q_heads, kv_heads, group, shift, sm_scale * 1.4426950408889634f};
+                  static_cast<int32_t*>(workspace),
+                  workspace ? reinterpret_cast<float*>(static_cast<char*>(workspace) + counts_bytes(vectors)) : nullptr, splits, q_heads, kv_heads, group, shift, sm_scale * 1.4426950408889634f};
   hipStream_t s = static_cast<hipStream_t>(stream);
   switch (dtype) {
     case LLMQ_F32: return launch<float>(a, head_dim, tiles, groups, s);
