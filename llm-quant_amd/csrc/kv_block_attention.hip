@@ -183,6 +183,19 @@ template <typename T> __device__ __forceinline__ void store8(T* p, const float* 
   for (int i = 0; i < 8; i += Pack<T>::N) store16(p + i, Pack<T>::pack(f + i));
 }
 
+// Loads of codes in front of the walk and within it. Of two loads whose results meet at the head of a loop the compiler makes one
+// behind it, which is where they are needed; being of different kinds, these stay where they are asked for.
+struct InWalk {
+  static __device__ __forceinline__ u32x4 load(const void* p) { return load16(p); }
+};
+struct Ahead {
+  static __device__ __forceinline__ u32x4 load(const void* p) {
+    typedef uint32_t v4u __attribute__((ext_vector_type(4)));
+    const v4u r = *static_cast<const v4u*>(p);
+    return u32x4{r[0], r[1], r[2], r[3]};
+  }
+};
+
 template <typename T, int D, int NR>
 __global__ __launch_bounds__(kThreads, 2) void attention_kernel(const Problem a) {
   constexpr int kPieces = Pieces<T>::N;
@@ -218,7 +231,8 @@ __global__ __launch_bounds__(kThreads, 2) void attention_kernel(const Problem a)
   const int wave_row = row0 + my_tile * kRows;
   const int64_t held = static_cast<int64_t>(a.table.width) << a.block_shift;
 
-  // this lane's rows
+  // this lane's rows, with the scale's sign: the largest score is the largest sum of products
+  const float sign = a.scale_log2e < 0.0f ? -1.0f : 1.0f;
   u32x4 q[NR][kSteps][kPieces];
   float q_scale[NR], q_bias[NR];
   int last[NR];   // the last token that the row sees; -1: none
@@ -243,7 +257,7 @@ __global__ __launch_bounds__(kThreads, 2) void attention_kernel(const Problem a)
       uint32_t hi[4], lo[4];
 #pragma unroll
       for (int e = 0; e < 8; e += 2) {
-        const float x0 = ldexpf(f[s][e], -exponent), x1 = ldexpf(f[s][e + 1], -exponent);
+        const float x0 = ldexpf(f[s][e] * sign, -exponent), x1 = ldexpf(f[s][e + 1] * sign, -exponent);
         hi[e / 2] = pack_half(x0, x1);
         const v2h top = __builtin_bit_cast(v2h, hi[e / 2]);
         if constexpr (kPieces > 1) lo[e / 2] = pack_half((x0 - static_cast<float>(top[0])) * kPiece, (x1 - static_cast<float>(top[1])) * kPiece);
@@ -253,7 +267,7 @@ __global__ __launch_bounds__(kThreads, 2) void attention_kernel(const Problem a)
       if constexpr (kPieces > 1) q[n][s][kPieces - 1] = u32x4{lo[0], lo[1], lo[2], lo[3]};
     }
     q_bias[n] = kExactKeys ? 0.0f : -kBias * sum_of_rows(total);
-    q_scale[n] = ldexpf(a.scale_log2e, exponent);
+    q_scale[n] = ldexpf(fabsf(a.scale_log2e), exponent);
   }
 
   // the walk: tiles of 64 tokens, from the split's first one on
@@ -268,34 +282,35 @@ __global__ __launch_bounds__(kThreads, 2) void attention_kernel(const Problem a)
 
   // the blocks of a tile's strips: for its keys a lane reads strip r16 / 4, for its values and scales strip g
   const int k_strip = r16 >> 2;
-  int k_id, v_id;
-  auto find_blocks = [&](int tile) {
-    k_id = v_id = -1;
-    const int at = tile * kTile;
-    if (tile < end) {
-      if (at + kStrip * k_strip <= seen_last) k_id = a.table.at(b, (at + kStrip * k_strip) >> a.block_shift);
-      if (at + kStrip * g <= seen_last) v_id = a.table.at(b, (at + kStrip * g) >> a.block_shift);
-    }
+  const int32_t* table = a.table.entries + b * a.table.row_stride;
+  struct Entries {
+    int k, v;   // of the table, as they are
   };
+  const auto entries_of = [&](int tile) {
+    const int at = tile * kTile, most = a.table.width - 1;
+    return Entries{table[min((at + kStrip * k_strip) >> a.block_shift, most)], table[min((at + kStrip * g) >> a.block_shift, most)]};
+  };
+  // the block of a strip, -1: none, or none that is seen
+  const auto block_of = [&](int entry, int at) { return ((at > seen_last) | (entry >= a.table.blocks)) ? -1 : entry; };
   const int in_block = (1 << a.block_shift) - 1;
   u32x4 k_raw[4][kChunks], v_raw[kColumns];
-  auto load_keys = [&](int tile) {
+  const auto load_keys = [&](int tile, int id, auto when) {
     const int slot = (tile * kTile + kStrip * k_strip) & in_block;
-    const int8_t* p = a.k_codes + ((static_cast<int64_t>(max(k_id, 0)) * a.heads + h) * (in_block + 1) + slot + (r16 & 3)) * D + 16 * g;
+    const int8_t* p = a.k_codes + ((static_cast<int64_t>(max(id, 0)) * a.heads + h) * (in_block + 1) + slot + (r16 & 3)) * D + 16 * g;
 #pragma unroll
     for (int t = 0; t < 4; ++t)
 #pragma unroll
-      for (int c = 0; c < kChunks; ++c) k_raw[t][c] = load16(p + 4 * t * D + 64 * c);
+      for (int c = 0; c < kChunks; ++c) k_raw[t][c] = when.load(p + 4 * t * D + 64 * c);
   };
-  auto load_values = [&](int tile) {
+  const auto load_values = [&](int tile, int id, auto when) {
     const int slot = (tile * kTile + kStrip * g) & in_block;
-    const int8_t* p = a.v_codes + ((static_cast<int64_t>(max(v_id, 0)) * a.heads + h) * (in_block + 1) + slot) * D + kStrip * r16;
+    const int8_t* p = a.v_codes + ((static_cast<int64_t>(max(id, 0)) * a.heads + h) * (in_block + 1) + slot) * D + kStrip * r16;
 #pragma unroll
-    for (int c = 0; c < kColumns; ++c) v_raw[c] = load16(p + 16 * kStrip * c);
+    for (int c = 0; c < kColumns; ++c) v_raw[c] = when.load(p + 16 * kStrip * c);
   };
   float k_scale = 0.0f, v_scale = 0.0f;
-  auto load_scales = [&]() {
-    const int64_t at = static_cast<int64_t>(max(v_id, 0)) * a.heads + h;
+  const auto load_scales = [&](int id) {
+    const int64_t at = static_cast<int64_t>(max(id, 0)) * a.heads + h;
     k_scale = a.k_scale[at];
     v_scale = a.v_scale[at];
   };
@@ -310,20 +325,25 @@ __global__ __launch_bounds__(kThreads, 2) void attention_kernel(const Problem a)
     for (int c = 0; c < kColumns; ++c) o[n][c] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
   }
 
+  // A tile: scores, weights, weighted codes. The next one's keys are asked for as soon as this one's are in operands, its values
+  // likewise. A wave's loads come back in order, so what is waited for stands in front of what is not (the blocks of
+  // the tile after next are looked up between the next tile's keys and its values), and no load depends on a branch, behind
+  // which the compiler would have to wait as if it had not been issued: the last tile asks for itself once more.
   int tile = begin + my_share;
-  find_blocks(tile);
-  bool with_block = v_id >= 0;
+  Entries next{0, 0};
+  int v_id = -1;
   if (tile < end) {
-    load_keys(tile);
-    load_scales();
-    load_values(tile);
+    const Entries now = entries_of(tile);
+    next = entries_of(min(tile + sharing, end - 1));
+    v_id = block_of(now.v, tile * kTile + kStrip * g);
+    load_keys(tile, block_of(now.k, tile * kTile + kStrip * k_strip), Ahead());
+    load_scales(v_id);
+    load_values(tile, v_id, Ahead());
   }
   for (; tile < end; tile += sharing) {
-    const int next = tile + sharing;
+    const int next_tile = min(tile + sharing, end - 1);
     const float ks = k_scale, vs = v_scale;
-    const bool strip = with_block;
-    find_blocks(next);
-    with_block = v_id >= 0;
+    const bool strip = v_id >= 0;
     // scores: lane (row, g) gets token 16 g + 4 t + i in s[.][t][i]
     v4f s[NR][4];
 #pragma unroll
@@ -350,10 +370,12 @@ __global__ __launch_bounds__(kThreads, 2) void attention_kernel(const Problem a)
 #pragma unroll
         for (int n = 0; n < NR; ++n) s[n][t] = product(k[x], q[n][x][0], s[n][t]);
     }
-    if (next < end) {
-      load_keys(next);
-      load_scales();
-    }
+    __builtin_amdgcn_sched_barrier(0);   // (the phases as they stand: mixed, they take more registers than there are)
+    v_id = block_of(next.v, next_tile * kTile + kStrip * g);
+    load_keys(next_tile, block_of(next.k, next_tile * kTile + kStrip * k_strip), InWalk());
+    load_scales(v_id);
+    next = entries_of(min(tile + 2 * sharing, end - 1));
+    __builtin_amdgcn_sched_barrier(0);
     // weights
     const bool no_values = vs < kNoScale;   // (not a number: stays so)
     const float log_vs = strip ? __builtin_amdgcn_logf(no_values ? kNoScale : vs) : -INFINITY;
@@ -366,16 +388,18 @@ __global__ __launch_bounds__(kThreads, 2) void attention_kernel(const Problem a)
     for (int n = 0; n < NR; ++n) {
       const float factor = strip ? q_scale[n] * ks : 0.0f, offset = fmaf(q_bias[n], factor, log_vs);
       float top = -INFINITY;
+      if (!whole) {   // the scores in full, with those that are not seen left out
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) s[n][t][i] = at + 4 * t + i > last[n] ? -INFINITY : fmaf(s[n][t][i], factor, offset);
+      }
 #pragma unroll
       for (int t = 0; t < 4; ++t)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          float u = fmaf(s[n][t][i], factor, offset);
-          if (!whole && at + 4 * t + i > last[n]) u = -INFINITY;
-          s[n][t][i] = u;
-          top = fmaxf(top, u);
-        }
-      const float m_new = fmaxf(m_run[n], max_of_rows(top)), base = m_new == -INFINITY ? 0.0f : m_new;
+        for (int i = 0; i < 4; ++i) top = fmaxf(top, s[n][t][i]);
+      const float by = whole ? factor : 1.0f, plus = whole ? offset : 0.0f;   // (factor is not negative)
+      const float m_new = fmaxf(m_run[n], max_of_rows(fmaf(top, by, plus))), base = m_new == -INFINITY ? 0.0f : m_new;
       alpha[n] = __builtin_amdgcn_exp2f(m_run[n] - base);
       m_run[n] = m_new;
       float total = 0.0f;
@@ -383,7 +407,7 @@ __global__ __launch_bounds__(kThreads, 2) void attention_kernel(const Problem a)
       for (int t = 0; t < 4; ++t)
 #pragma unroll
         for (int i = 0; i < 4; i += 2) {
-          const float w0 = __builtin_amdgcn_exp2f(s[n][t][i] - base), w1 = __builtin_amdgcn_exp2f(s[n][t][i + 1] - base);
+          const float w0 = __builtin_amdgcn_exp2f(fmaf(s[n][t][i], by, plus - base)), w1 = __builtin_amdgcn_exp2f(fmaf(s[n][t][i + 1], by, plus - base));
           total += w0 + w1;
           const uint32_t hi = pack_half(w0, w1);
           (&p[n][t / 2][0].x)[2 * (t % 2) + i / 2] = hi;
@@ -405,6 +429,7 @@ __global__ __launch_bounds__(kThreads, 2) void attention_kernel(const Problem a)
           for (int e = 0; e < kPieces; ++e)
             if (no_values) p[n][y][e] = u32x4{0u, 0u, 0u, 0u};
     }
+    __builtin_amdgcn_sched_barrier(0);
     // weighted codes
     bool moved = false;
 #pragma unroll
@@ -433,7 +458,8 @@ __global__ __launch_bounds__(kThreads, 2) void attention_kernel(const Problem a)
         o[n][c] = product(v1, p[n][1][0], o[n][c]);
       }
     }
-    if (next < end) load_values(next);
+    __builtin_amdgcn_sched_barrier(0);
+    load_values(next_tile, v_id, InWalk());
   }
 
   // the waves that share a row tile: max m_w, sum l_w 2^(m_w - m), sum O_w 2^(m_w - m), in wave order
