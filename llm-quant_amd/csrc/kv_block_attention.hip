@@ -20,6 +20,7 @@
 // take row tiles of 16 NR each, or, where there are fewer, share a row tile's tokens and meet in LDS at the end.
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 #include "kv_blocks.h"
 
@@ -42,6 +43,16 @@ constexpr float kBias = 1152.0f;      // what a code is too high as an operand: 
 constexpr float kNoScale = 0x1p-100f; // value scales below count as zero
 constexpr float kPiece = 2048.0f;     // the second piece of an fp32 number is this much too high
 
+// Division by a number that the host knows: the estimate is the quotient or one more.
+struct Divisor {
+  uint32_t by, inverse;   // 2^32 / by, rounded up (by > 1)
+  __device__ __forceinline__ uint32_t quotient(uint32_t x) const {
+    if (by == 1) return x;
+    const uint32_t q = __umulhi(x, inverse);
+    return q * by > x ? q - 1 : q;
+  }
+};
+
 struct Problem {
   const void* query;
   int64_t q_stride;
@@ -55,6 +66,7 @@ struct Problem {
   float* partials;         // [rows, q_heads, splits]
   int splits, q_heads, heads, group, block_shift;
   float scale_log2e;
+  Divisor by_group;
 };
 
 __device__ __forceinline__ int wave_total(int v) {
@@ -72,43 +84,59 @@ __device__ __forceinline__ int wave_prefix(int v) {
   return v + (row > 0 ? a : 0) + (row > 1 ? b : 0) + (row > 2 ? c : 0);
 }
 
-// Where a sequence's work lies: `groups` row groups of `tiles` tiles of 64 tokens (its last row's).
-struct Work {
-  int groups, tiles;
+// A sequence of the batch, and its work: `groups` row groups of at most `tiles` tiles of 64 tokens.
+struct Sequence {
+  int first, n, cached, groups, tiles;
 };
-__device__ __forceinline__ Work work_of(const Problem& a, int b, int group_rows) {
-  const int n = a.rows.count(b), cached = a.cached[b];
+__device__ __forceinline__ Sequence sequence_of(const Problem& a, int b, int group_rows) {
+  if (b >= a.rows.sequences) return Sequence{0, 0, -1, 0, 0};
+  const int first = a.rows.first(b), n = a.rows.count(b), cached = a.cached[b];
   const int64_t held = min(static_cast<int64_t>(a.table.width) << a.block_shift, static_cast<int64_t>(INT32_MAX - 2 * kTile));
   const int seen = cached < 0 ? 0 : static_cast<int>(min(static_cast<int64_t>(cached) + n, held));
-  return Work{(n * a.group + group_rows - 1) / group_rows, (seen + kTile - 1) / kTile};
+  return Sequence{first, n, cached, (n * a.group + group_rows - 1) / group_rows, (seen + kTile - 1) / kTile};
 }
 // The piece of work of a workgroup, found by each of its waves.
 struct Unit {
-  int b, row_group, split, splits;   // splits of this sequence
+  int b, first, n, cached;          // its sequence
+  int row_group, split, splits;     // splits of this sequence
 };
 // Lengths lie on the device: how the tokens are cut is decided here, the same way by everyone. All units are of about as many
 // tiles, C = max(kLeastTiles, all tiles / (kUnits / heads)), a sequence is cut into ceil(tiles / C) equal splits, at most
 // a.splits; so there are at most sum(groups (tiles / C + 1)) <= kUnits / heads + groups of them, the launch's size.
-__device__ __forceinline__ bool find_unit(const Problem& a, int group_rows, int64_t index, Unit& u) {
+__device__ __forceinline__ bool find_unit(const Problem& a, int group_rows, int index, Unit& u) {
   const int lane = threadIdx.x & (kWave - 1), sequences = a.rows.sequences;
-  int64_t all = 0;
-  Work w{0, 0};
-  for (int b0 = 0; b0 < sequences; b0 += kWave) {
-    w = b0 + lane < sequences ? work_of(a, b0 + lane, group_rows) : Work{0, 0};
-    const int64_t product = static_cast<int64_t>(w.groups) * w.tiles;
-    all += wave_total(static_cast<int>(product & 0xffff)) + (static_cast<int64_t>(wave_total(static_cast<int>(product >> 16))) << 16);
+  constexpr int kBatches = 4;   // of 64 sequences, asked for together
+  Sequence s = sequence_of(a, lane, group_rows);
+  int size = INT32_MAX / 2;
+  if (a.splits > 1) {
+    int64_t all = 0;
+    const auto add = [&](const Sequence& x) {
+      const int64_t product = static_cast<int64_t>(x.groups) * x.tiles;
+      all += wave_total(static_cast<int>(product & 0xffff)) + (static_cast<int64_t>(wave_total(static_cast<int>(product >> 16))) << 16);
+    };
+    add(s);
+    for (int b0 = kWave; b0 < sequences; b0 += kBatches * kWave) {
+      Sequence more[kBatches];
+#pragma unroll
+      for (int i = 0; i < kBatches; ++i) more[i] = sequence_of(a, b0 + i * kWave + lane, group_rows);
+#pragma unroll
+      for (int i = 0; i < kBatches; ++i) add(more[i]);
+    }
+    const int64_t wanted = (kUnits + a.heads - 1) / a.heads;
+    size = static_cast<int>(max((all + wanted - 1) / wanted, static_cast<int64_t>(kLeastTiles)));
   }
-  const int64_t wanted = (kUnits + a.heads - 1) / a.heads;
-  const int size = static_cast<int>(max((all + wanted - 1) / wanted, static_cast<int64_t>(kLeastTiles)));
   for (int b0 = 0; b0 < sequences; b0 += kWave) {
-    if (sequences > kWave) w = b0 + lane < sequences ? work_of(a, b0 + lane, group_rows) : Work{0, 0};   // (else the one above)
-    const int splits = max(min((w.tiles + size - 1) / size, a.splits), 1), units = w.groups * splits, up_to = wave_prefix(units);
+    if (b0 != 0) s = sequence_of(a, b0 + lane, group_rows);
+    const int splits = max(min((s.tiles + size - 1) / size, a.splits), 1), units = s.groups * splits, up_to = wave_prefix(units);
     const int total = __builtin_amdgcn_readlane(up_to, kWave - 1);
     if (index < total) {
       const int at = __popcll(__ballot(up_to <= index));   // (the first lane whose units reach beyond the index)
       u.b = b0 + at;
+      u.first = __builtin_amdgcn_readlane(s.first, at);
+      u.n = __builtin_amdgcn_readlane(s.n, at);
+      u.cached = __builtin_amdgcn_readlane(s.cached, at);
       u.splits = __builtin_amdgcn_readlane(splits, at);
-      const int within = static_cast<int>(index) - (__builtin_amdgcn_readlane(up_to, at) - __builtin_amdgcn_readlane(units, at));
+      const int within = index - (__builtin_amdgcn_readlane(up_to, at) - __builtin_amdgcn_readlane(units, at));
       u.row_group = within / u.splits;
       u.split = within % u.splits;
       return true;
@@ -207,82 +235,35 @@ __global__ __launch_bounds__(kThreads, 2) void attention_kernel(const Problem a)
 
   const int tid = threadIdx.x, lane = tid & (kWave - 1), r16 = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
-  // key heads fastest: with eight of them each XCD's cache holds one. Late rows, which see most, first.
-  const int h = blockIdx.x % a.heads;
-  int64_t piece = gridDim.x / a.heads - 1 - blockIdx.x / a.heads;
-  Unit unit{0, 0, 0, 1};
-  if (a.splits > 1) {
-    if (!find_unit(a, kGroupRows, piece, unit)) return;
-  } else if (a.rows.start == nullptr) {
+  // Key heads fastest: with eight of them each XCD's cache holds one. Rows that see most first where nothing is split; where it is,
+  // all units are alike, and the launch's spare workgroups stand behind them.
+  const int h = blockIdx.x % a.heads, index = blockIdx.x / a.heads;
+  Unit unit{0, 0, 1, 0, 0, 0, 1};
+  if (a.splits == 1 && a.rows.start == nullptr) {
     const int per = (a.group + kGroupRows - 1) / kGroupRows;
-    unit.b = static_cast<int>(piece / per);
-    unit.row_group = static_cast<int>(piece % per);
-  } else {
-    unit.b = a.rows.find(a.group, kGroupRows, 1, piece);
-    unit.row_group = static_cast<int>(min(piece, static_cast<int64_t>(INT32_MAX / kGroupRows)));
+    unit.b = unit.first = index / per;
+    unit.row_group = index % per;
+    unit.cached = a.cached[unit.b];
+  } else if (!find_unit(a, kGroupRows, a.splits > 1 ? index : static_cast<int>(gridDim.x / a.heads) - 1 - index, unit)) {
+    return;
   }
-  const int b = unit.b, split = unit.split;
-  const int n_rows = a.rows.count(b) * a.group, row0 = unit.row_group * kGroupRows;
-  if (row0 >= n_rows) return;
-  const int first_row = a.rows.first(b), cached = a.cached[b];
+  const int n_rows = unit.n * a.group, row0 = unit.row_group * kGroupRows, cached = unit.cached;
   const int here = min(n_rows - row0, kGroupRows), tiles_of_rows = (here + kRows - 1) / kRows;
   const int sharing = tiles_of_rows == 1 ? 4 : tiles_of_rows == 2 ? 2 : 1;   // waves that share a row tile
   const int my_tile = wave / sharing, my_share = wave % sharing;
   const int wave_row = row0 + my_tile * kRows;
+
+  // the walk: tiles of 64 tokens, from the split's first one on. `seen`: the last token of a row of the sequence, -1: none
   const int64_t held = static_cast<int64_t>(a.table.width) << a.block_shift;
-
-  // this lane's rows, with the scale's sign: the largest score is the largest sum of products
-  const float sign = a.scale_log2e < 0.0f ? -1.0f : 1.0f;
-  u32x4 q[NR][kSteps][kPieces];
-  float q_scale[NR], q_bias[NR];
-  int last[NR];   // the last token that the row sees; -1: none
-#pragma unroll
-  for (int n = 0; n < NR; ++n) {
-    const int row = min(wave_row + 16 * n + r16, n_rows - 1), token = row / a.group;
-    last[n] = cached < 0 ? -1 : static_cast<int>(min(min(static_cast<int64_t>(cached) + token, held - 1), static_cast<int64_t>(INT32_MAX - 2 * kTile)));
-    const T* x = static_cast<const T*>(a.query) + (first_row + token) * a.q_stride +
-                 static_cast<int64_t>(h * a.group + row % a.group) * D + 16 * g;
-    float f[kSteps][8], largest = 0.0f;
-#pragma unroll
-    for (int s = 0; s < kSteps; ++s) {
-      load8(x + 64 * (s / 2) + 8 * (s % 2), f[s]);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) largest = fmaxf(largest, fabsf(f[s][e]));
-    }
-    largest = max_of_rows(largest);
-    const int exponent = __builtin_amdgcn_frexp_expf(largest) - 1;
-    float total = 0.0f;
-#pragma unroll
-    for (int s = 0; s < kSteps; ++s) {
-      uint32_t hi[4], lo[4];
-#pragma unroll
-      for (int e = 0; e < 8; e += 2) {
-        const float x0 = ldexpf(f[s][e] * sign, -exponent), x1 = ldexpf(f[s][e + 1] * sign, -exponent);
-        hi[e / 2] = pack_half(x0, x1);
-        const v2h top = __builtin_bit_cast(v2h, hi[e / 2]);
-        if constexpr (kPieces > 1) lo[e / 2] = pack_half((x0 - static_cast<float>(top[0])) * kPiece, (x1 - static_cast<float>(top[1])) * kPiece);
-        else total += static_cast<float>(top[0]) + static_cast<float>(top[1]);
-      }
-      q[n][s][0] = u32x4{hi[0], hi[1], hi[2], hi[3]};
-      if constexpr (kPieces > 1) q[n][s][kPieces - 1] = u32x4{lo[0], lo[1], lo[2], lo[3]};
-    }
-    q_bias[n] = kExactKeys ? 0.0f : -kBias * sum_of_rows(total);
-    q_scale[n] = ldexpf(fabsf(a.scale_log2e), exponent);
-  }
-
-  // the walk: tiles of 64 tokens, from the split's first one on
-  const int seen_first = __builtin_amdgcn_readfirstlane(last[0]);   // (rows of a wave see more and more)
-  int seen_last = -1;
-  if (wave_row < n_rows) {
-    const int64_t newest = cached < 0 ? -1 : static_cast<int64_t>(cached) + (min(row0 + (my_tile + 1) * kRows, n_rows) - 1) / a.group;
-    seen_last = static_cast<int>(min(min(newest, held - 1), static_cast<int64_t>(INT32_MAX - 2 * kTile)));
-  }
-  const int tiles = (seen_last + kTile) / kTile, per_split = (tiles + unit.splits - 1) / unit.splits;
-  const int begin = split * per_split, end = min(begin + per_split, tiles);
+  const int most_seen = static_cast<int>(min(held - 1, static_cast<int64_t>(INT32_MAX - 2 * kTile)));
+  const auto seen = [&](int token) { return cached < 0 ? -1 : static_cast<int>(min(static_cast<int64_t>(cached) + token, static_cast<int64_t>(most_seen))); };
+  const int seen_last = wave_row < n_rows ? seen(static_cast<int>(a.by_group.quotient(min(row0 + (my_tile + 1) * kRows, n_rows) - 1))) : -1;
+  const int tiles = (seen_last + kTile) / kTile, per_split = unit.splits == 1 ? tiles : (tiles + unit.splits - 1) / unit.splits;
+  const int begin = unit.split * per_split, end = min(begin + per_split, tiles);
 
   // the blocks of a tile's strips: for its keys a lane reads strip r16 / 4, for its values and scales strip g
   const int k_strip = r16 >> 2;
-  const int32_t* table = a.table.entries + b * a.table.row_stride;
+  const int32_t* table = a.table.entries + unit.b * a.table.row_stride;
   struct Entries {
     int k, v;   // of the table, as they are
   };
@@ -315,6 +296,71 @@ __global__ __launch_bounds__(kThreads, 2) void attention_kernel(const Problem a)
     v_scale = a.v_scale[at];
   };
 
+  // what the first tile needs is asked for in the order of its use: table, queries, keys, values
+  int tile = begin + my_share;
+  Entries now{0, 0}, next{0, 0};
+  if (tile < end) {
+    now = entries_of(tile);
+    next = entries_of(min(tile + sharing, end - 1));
+  }
+  constexpr int kPackets = 8 / Pack<T>::N;
+  u32x4 q_raw[NR][kSteps][kPackets];
+  int last[NR];   // the last token that the row sees
+#pragma unroll
+  for (int n = 0; n < NR; ++n) {
+    const uint32_t row = min(wave_row + 16 * n + r16, n_rows - 1), token = a.by_group.quotient(row);
+    last[n] = seen(static_cast<int>(token));
+    const T* x = static_cast<const T*>(a.query) + (unit.first + static_cast<int64_t>(token)) * a.q_stride +
+                 static_cast<int64_t>(h * a.group + (row - token * a.group)) * D + 16 * g;
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s)
+#pragma unroll
+      for (int e = 0; e < kPackets; ++e) q_raw[n][s][e] = load16(x + 64 * (s / 2) + 8 * (s % 2) + e * Pack<T>::N);
+  }
+  const int seen_first = __builtin_amdgcn_readfirstlane(last[0]);   // (rows of a wave see more and more)
+  int v_id = -1;
+  if (tile < end) {
+    v_id = block_of(now.v, tile * kTile + kStrip * g);
+    load_keys(tile, block_of(now.k, tile * kTile + kStrip * k_strip), Ahead());
+    load_scales(v_id);
+    load_values(tile, v_id, Ahead());
+  }
+
+  // this lane's rows, with the scale's sign: the largest score is the largest sum of products
+  const float sign = a.scale_log2e < 0.0f ? -1.0f : 1.0f;
+  u32x4 q[NR][kSteps][kPieces];
+  float q_scale[NR], q_bias[NR];
+#pragma unroll
+  for (int n = 0; n < NR; ++n) {
+    float f[kSteps][8], largest = 0.0f;
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s) {
+#pragma unroll
+      for (int e = 0; e < kPackets; ++e) Pack<T>::unpack(q_raw[n][s][e], f[s] + e * Pack<T>::N);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) largest = fmaxf(largest, fabsf(f[s][e]));
+    }
+    largest = max_of_rows(largest);
+    const int exponent = __builtin_amdgcn_frexp_expf(largest) - 1;
+    float total = 0.0f;
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s) {
+      uint32_t hi[4], lo[4];
+#pragma unroll
+      for (int e = 0; e < 8; e += 2) {
+        const float x0 = ldexpf(f[s][e] * sign, -exponent), x1 = ldexpf(f[s][e + 1] * sign, -exponent);
+        hi[e / 2] = pack_half(x0, x1);
+        const v2h top = __builtin_bit_cast(v2h, hi[e / 2]);
+        if constexpr (kPieces > 1) lo[e / 2] = pack_half((x0 - static_cast<float>(top[0])) * kPiece, (x1 - static_cast<float>(top[1])) * kPiece);
+        else total += static_cast<float>(top[0]) + static_cast<float>(top[1]);
+      }
+      q[n][s][0] = u32x4{hi[0], hi[1], hi[2], hi[3]};
+      if constexpr (kPieces > 1) q[n][s][kPieces - 1] = u32x4{lo[0], lo[1], lo[2], lo[3]};
+    }
+    q_bias[n] = kExactKeys ? 0.0f : -kBias * sum_of_rows(total);
+    q_scale[n] = ldexpf(fabsf(a.scale_log2e), exponent);
+  }
+
   v4f o[NR][kColumns];
   float m_run[NR], l_run[NR];
 #pragma unroll
@@ -329,17 +375,6 @@ __global__ __launch_bounds__(kThreads, 2) void attention_kernel(const Problem a)
   // likewise. A wave's loads come back in order, so what is waited for stands in front of what is not (the blocks of
   // the tile after next are looked up between the next tile's keys and its values), and no load depends on a branch, behind
   // which the compiler would have to wait as if it had not been issued: the last tile asks for itself once more.
-  int tile = begin + my_share;
-  Entries next{0, 0};
-  int v_id = -1;
-  if (tile < end) {
-    const Entries now = entries_of(tile);
-    next = entries_of(min(tile + sharing, end - 1));
-    v_id = block_of(now.v, tile * kTile + kStrip * g);
-    load_keys(tile, block_of(now.k, tile * kTile + kStrip * k_strip), Ahead());
-    load_scales(v_id);
-    load_values(tile, v_id, Ahead());
-  }
   for (; tile < end; tile += sharing) {
     const int next_tile = min(tile + sharing, end - 1);
     const float ks = k_scale, vs = v_scale;
@@ -475,38 +510,49 @@ __global__ __launch_bounds__(kThreads, 2) void attention_kernel(const Problem a)
     for (int c = 0; c < kColumns; ++c) *reinterpret_cast<v4f*>(part + 16 * c) = o[n][c];
   }
   __syncthreads();
-  constexpr int kPackets = D / 8;
-  for (int item = tid; item < here * kPackets; item += kThreads) {
-    const int row = item / kPackets, d = item % kPackets * 8, wave0 = row / kRows * sharing, in_tile = row % kRows;
-    float m = s_max[wave0 * kRows + in_tile];
-    for (int w = 1; w < sharing; ++w) m = fmaxf(m, s_max[(wave0 + w) * kRows + in_tile]);
-    const float base = m == -INFINITY ? 0.0f : m;
-    float l = 0.0f, f[8] = {};
-    for (int w = 0; w < sharing; ++w) {
-      const int at = (wave0 + w) * kRows + in_tile;
-      const float weight = __builtin_amdgcn_exp2f(s_max[at] - base);
-      l = fmaf(s_sum[at], weight, l);
-      const v4f lo = *reinterpret_cast<const v4f*>(s_part + at * kRow + d), hi = *reinterpret_cast<const v4f*>(s_part + at * kRow + d + 4);
+  constexpr int kPacketsOut = D / 8;
+  const auto finish = [&](auto sharing_tag) {
+    constexpr int kSharing = decltype(sharing_tag)::value;
+    for (int item = tid; item < here * kPacketsOut; item += kThreads) {
+      const int row = item / kPacketsOut, d = item % kPacketsOut * 8, at = row / kRows * kSharing * kRows + row % kRows;
+      float m[kSharing], l = 0.0f, f[8] = {}, top = -INFINITY;
+      v4f lo[kSharing], hi[kSharing];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        f[e] = fmaf(lo[e], weight, f[e]);
-        f[e + 4] = fmaf(hi[e], weight, f[e + 4]);
+      for (int w = 0; w < kSharing; ++w) {
+        m[w] = s_max[at + w * kRows];
+        lo[w] = *reinterpret_cast<const v4f*>(s_part + (at + w * kRows) * kRow + d);
+        hi[w] = *reinterpret_cast<const v4f*>(s_part + (at + w * kRows) * kRow + d + 4);
+        top = fmaxf(top, m[w]);
+      }
+      const float base = top == -INFINITY ? 0.0f : top;
+#pragma unroll
+      for (int w = 0; w < kSharing; ++w) {
+        const float weight = __builtin_amdgcn_exp2f(m[w] - base);
+        l = fmaf(s_sum[at + w * kRows], weight, l);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          f[e] = fmaf(lo[w][e], weight, f[e]);
+          f[e + 4] = fmaf(hi[w][e], weight, f[e + 4]);
+        }
+      }
+      const uint32_t token = a.by_group.quotient(row0 + row);
+      const int64_t vector = (unit.first + static_cast<int64_t>(token)) * a.q_heads + h * a.group + (row0 + row - token * a.group);
+      if (a.splits > 1 && unit.split == 0 && d == 0) a.split_counts[vector] = unit.splits;
+      if (unit.splits == 1) {
+        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) f[e] *= inv;
+        store8(static_cast<T*>(a.out) + vector * D + d, f);
+      } else {
+        float* record = a.partials + (vector * a.splits + unit.split) * (D + kHeader);
+        if (d == 0) *reinterpret_cast<v2f*>(record) = v2f{top, l};
+        if (top != -INFINITY || l != 0.0f) store8(record + kHeader + d, f);   // (else nobody reads it)
       }
     }
-    const int token = (row0 + row) / a.group, head = h * a.group + (row0 + row) % a.group;
-    const int64_t vector = static_cast<int64_t>(first_row + token) * a.q_heads + head;
-    if (a.splits > 1 && split == 0 && d == 0) a.split_counts[vector] = unit.splits;
-    if (unit.splits == 1) {
-      const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) f[e] *= inv;
-      store8(static_cast<T*>(a.out) + vector * D + d, f);
-    } else {
-      float* record = a.partials + (vector * a.splits + split) * (D + kHeader);
-      if (d == 0) *reinterpret_cast<v2f*>(record) = v2f{m, l};
-      if (m != -INFINITY || l != 0.0f) store8(record + kHeader + d, f);   // (else nobody reads it)
-    }
-  }
+  };
+  if (sharing == 4) finish(std::integral_constant<int, 4>());
+  else if (sharing == 2) finish(std::integral_constant<int, 2>());
+  else finish(std::integral_constant<int, 1>());
 }
 
 // The partial results of a row and head, by a workgroup: four columns of every kAtOnce-th of them a thread, all asked for at once.
@@ -644,7 +690,8 @@ extern "C" int llmq_kv_block_attention(const void* query, int64_t q_row_stride, 
   const Problem a{query, q_row_stride, static_cast<const int8_t*>(k_codes), static_cast<const int8_t*>(v_codes), k_scale, v_scale,
                   {block_table, table_stride, table_width, n_blocks}, cached, {query_start_or_null, sequences, tokens}, out,
                   static_cast<int32_t*>(workspace),
-                  workspace ? reinterpret_cast<float*>(static_cast<char*>(workspace) + counts_bytes(vectors)) : nullptr, splits, q_heads, kv_heads, group, shift, sm_scale * 1.4426950408889634f};
+                  workspace ? reinterpret_cast<float*>(static_cast<char*>(workspace) + counts_bytes(vectors)) : nullptr, splits, q_heads, kv_heads, group, shift, sm_scale * 1.4426950408889634f,
+                  {static_cast<uint32_t>(group), static_cast<uint32_t>(((uint64_t{1} << 32) + group - 1) / group)}};
   hipStream_t s = static_cast<hipStream_t>(stream);
   switch (dtype) {
     case LLMQ_F32: return launch<float>(a, head_dim, tiles, groups, s);
