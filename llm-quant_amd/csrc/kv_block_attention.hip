@@ -89,8 +89,15 @@ struct Sequence {
   int first, n, cached, groups, tiles;
 };
 __device__ __forceinline__ Sequence sequence_of(const Problem& a, int b, int group_rows) {
-  if (b >= a.rows.sequences) return Sequence{0, 0, -1, 0, 0};
-  const int first = a.rows.first(b), n = a.rows.count(b), cached = a.cached[b];
+  // (its three numbers are asked for together: one trip to memory)
+  const int at = min(b, a.rows.sequences - 1);
+  int from = at, to = at + 1;
+  if (a.rows.start != nullptr) {
+    from = a.rows.start[at];
+    to = a.rows.start[at + 1];
+  }
+  const int cached = a.cached[at];
+  const int first = min(max(from, 0), a.rows.rows), n = b < a.rows.sequences ? max(min(max(to, 0), a.rows.rows) - first, 0) : 0;
   const int64_t held = min(static_cast<int64_t>(a.table.width) << a.block_shift, static_cast<int64_t>(INT32_MAX - 2 * kTile));
   const int seen = cached < 0 ? 0 : static_cast<int>(min(static_cast<int64_t>(cached) + n, held));
   return Sequence{first, n, cached, (n * a.group + group_rows - 1) / group_rows, (seen + kTile - 1) / kTile};
@@ -224,13 +231,19 @@ struct Ahead {
   }
 };
 
+// waves a SIMD: heads of 256, and fp32 with several row tiles, need more than half of its registers
+template <typename T, int D, int NR> constexpr int kOccupancy = D == 256 || (Pieces<T>::N > 1 && NR * D >= 256) ? 1 : 2;
+
 template <typename T, int D, int NR>
-__global__ __launch_bounds__(kThreads, 2) void attention_kernel(const Problem a) {
+__global__ __launch_bounds__(kThreads, (kOccupancy<T, D, NR>)) void attention_kernel(const Problem a) {
   constexpr int kPieces = Pieces<T>::N;
   constexpr bool kExactKeys = kPieces > 1;
   constexpr int kChunks = D / 64, kSteps = D / 32, kColumns = D / 16;   // 64-element pieces, k-steps of S^T, row tiles of O^T
   constexpr int kRows = 16 * NR, kGroupRows = kWaves * kRows, kRow = D + 4;
-  __shared__ __attribute__((aligned(16))) float s_part[kWaves * kRows * kRow];
+  constexpr bool kTogether = NR > 1;   // whether waves with a row tile each share the conversion of the codes
+  constexpr int kOperands = 4 * kSteps + 2 * kColumns, kParts = kColumns / kWaves;   // of a tile, 1 KB each; value columns that a wave converts
+  constexpr int kResults = kWaves * kRows * kRow * 4, kBuffers = kTogether ? 2 * kOperands * 1024 : 0;
+  __shared__ __attribute__((aligned(16))) unsigned char s_mem[kResults > kBuffers ? kResults : kBuffers];
   __shared__ float s_max[kGroupRows], s_sum[kGroupRows];
 
   const int tid = threadIdx.x, lane = tid & (kWave - 1), r16 = lane & 15, g = lane >> 4;
@@ -258,7 +271,9 @@ __global__ __launch_bounds__(kThreads, 2) void attention_kernel(const Problem a)
   const int most_seen = static_cast<int>(min(held - 1, static_cast<int64_t>(INT32_MAX - 2 * kTile)));
   const auto seen = [&](int token) { return cached < 0 ? -1 : static_cast<int>(min(static_cast<int64_t>(cached) + token, static_cast<int64_t>(most_seen))); };
   const int seen_last = wave_row < n_rows ? seen(static_cast<int>(a.by_group.quotient(min(row0 + (my_tile + 1) * kRows, n_rows) - 1))) : -1;
-  const int tiles = (seen_last + kTile) / kTile, per_split = unit.splits == 1 ? tiles : (tiles + unit.splits - 1) / unit.splits;
+  const bool together = kTogether && sharing == 1;
+  const int seen_here = together ? seen(static_cast<int>(a.by_group.quotient(row0 + here - 1))) : seen_last;   // by what walks as one
+  const int tiles = (seen_here + kTile) / kTile, per_split = unit.splits == 1 ? tiles : (tiles + unit.splits - 1) / unit.splits;
   const int begin = unit.split * per_split, end = min(begin + per_split, tiles);
 
   // the blocks of a tile's strips: for its keys a lane reads strip r16 / 4, for its values and scales strip g
@@ -272,20 +287,27 @@ __global__ __launch_bounds__(kThreads, 2) void attention_kernel(const Problem a)
     return Entries{table[min((at + kStrip * k_strip) >> a.block_shift, most)], table[min((at + kStrip * g) >> a.block_shift, most)]};
   };
   // the block of a strip, -1: none, or none that is seen
-  const auto block_of = [&](int entry, int at) { return ((at > seen_last) | (entry >= a.table.blocks)) ? -1 : entry; };
+  const auto block_of = [&](int entry, int at) { return ((at > seen_here) | (entry >= a.table.blocks)) ? -1 : entry; };
   const int in_block = (1 << a.block_shift) - 1;
+  // this lane's first bytes of a tile: key codes of token 16 k_strip + r16 % 4 from element 16 g on, value codes of strip g and column r16
+  const auto key_address = [&](int tile, int id) {
+    const int slot = (tile * kTile + kStrip * k_strip) & in_block;
+    return a.k_codes + ((static_cast<int64_t>(max(id, 0)) * a.heads + h) * (in_block + 1) + slot + (r16 & 3)) * D + 16 * g;
+  };
+  const auto value_address = [&](int tile, int id) {
+    const int slot = (tile * kTile + kStrip * g) & in_block;
+    return a.v_codes + ((static_cast<int64_t>(max(id, 0)) * a.heads + h) * (in_block + 1) + slot) * D + kStrip * r16;
+  };
   u32x4 k_raw[4][kChunks], v_raw[kColumns];
   const auto load_keys = [&](int tile, int id, auto when) {
-    const int slot = (tile * kTile + kStrip * k_strip) & in_block;
-    const int8_t* p = a.k_codes + ((static_cast<int64_t>(max(id, 0)) * a.heads + h) * (in_block + 1) + slot + (r16 & 3)) * D + 16 * g;
+    const int8_t* p = key_address(tile, id);
 #pragma unroll
     for (int t = 0; t < 4; ++t)
 #pragma unroll
       for (int c = 0; c < kChunks; ++c) k_raw[t][c] = when.load(p + 4 * t * D + 64 * c);
   };
   const auto load_values = [&](int tile, int id, auto when) {
-    const int slot = (tile * kTile + kStrip * g) & in_block;
-    const int8_t* p = a.v_codes + ((static_cast<int64_t>(max(id, 0)) * a.heads + h) * (in_block + 1) + slot) * D + kStrip * r16;
+    const int8_t* p = value_address(tile, id);
 #pragma unroll
     for (int c = 0; c < kColumns; ++c) v_raw[c] = when.load(p + 16 * kStrip * c);
   };
@@ -318,18 +340,12 @@ __global__ __launch_bounds__(kThreads, 2) void attention_kernel(const Problem a)
       for (int e = 0; e < kPackets; ++e) q_raw[n][s][e] = load16(x + 64 * (s / 2) + 8 * (s % 2) + e * Pack<T>::N);
   }
   const int seen_first = __builtin_amdgcn_readfirstlane(last[0]);   // (rows of a wave see more and more)
-  int v_id = -1;
-  if (tile < end) {
-    v_id = block_of(now.v, tile * kTile + kStrip * g);
-    load_keys(tile, block_of(now.k, tile * kTile + kStrip * k_strip), Ahead());
-    load_scales(v_id);
-    load_values(tile, v_id, Ahead());
-  }
 
   // this lane's rows, with the scale's sign: the largest score is the largest sum of products
   const float sign = a.scale_log2e < 0.0f ? -1.0f : 1.0f;
   u32x4 q[NR][kSteps][kPieces];
   float q_scale[NR], q_bias[NR];
+  const auto take_queries = [&]() {
 #pragma unroll
   for (int n = 0; n < NR; ++n) {
     float f[kSteps][8], largest = 0.0f;
@@ -360,9 +376,11 @@ __global__ __launch_bounds__(kThreads, 2) void attention_kernel(const Problem a)
     q_bias[n] = kExactKeys ? 0.0f : -kBias * sum_of_rows(total);
     q_scale[n] = ldexpf(fabsf(a.scale_log2e), exponent);
   }
+  };
 
-  v4f o[NR][kColumns];
-  float m_run[NR], l_run[NR];
+  v4f o[NR][kColumns], s[NR][4];
+  uint32_t p[NR][2][kPieces][4];
+  float m_run[NR], l_run[NR], alpha[NR];
 #pragma unroll
   for (int n = 0; n < NR; ++n) {
     m_run[n] = -INFINITY;
@@ -370,55 +388,31 @@ __global__ __launch_bounds__(kThreads, 2) void attention_kernel(const Problem a)
 #pragma unroll
     for (int c = 0; c < kColumns; ++c) o[n][c] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
   }
-
-  // A tile: scores, weights, weighted codes. The next one's keys are asked for as soon as this one's are in operands, its values
-  // likewise. A wave's loads come back in order, so what is waited for stands in front of what is not (the blocks of
-  // the tile after next are looked up between the next tile's keys and its values), and no load depends on a branch, behind
-  // which the compiler would have to wait as if it had not been issued: the last tile asks for itself once more.
-  for (; tile < end; tile += sharing) {
-    const int next_tile = min(tile + sharing, end - 1);
-    const float ks = k_scale, vs = v_scale;
-    const bool strip = v_id >= 0;
-    // scores: lane (row, g) gets token 16 g + 4 t + i in s[.][t][i]
-    v4f s[NR][4];
+  // scores of tokens 16 g + 4 t + i, in s[.][t][i] of lane (row, g): the products of sub-tile t
+  const auto scores = [&](int t, const u32x4* k) {
 #pragma unroll
-    for (int t = 0; t < 4; ++t) {
+    for (int n = 0; n < NR; ++n) s[n][t] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+    if constexpr (kPieces > 1) {
 #pragma unroll
-      for (int n = 0; n < NR; ++n) s[n][t] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
-      u32x4 k[kSteps];
+      for (int n = 0; n < NR; ++n) {
 #pragma unroll
-      for (int c = 0; c < kChunks; ++c) {
-        k[2 * c] = operand<kExactKeys>(k_raw[t][c].x, k_raw[t][c].y);
-        k[2 * c + 1] = operand<kExactKeys>(k_raw[t][c].z, k_raw[t][c].w);
+        for (int x = 0; x < kSteps; ++x) s[n][t] = product(k[x], q[n][x][kPieces - 1], s[n][t]);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[n][t][i] *= 1.0f / kPiece;
       }
-      if constexpr (kPieces > 1) {
-#pragma unroll
-        for (int n = 0; n < NR; ++n) {
-#pragma unroll
-          for (int x = 0; x < kSteps; ++x) s[n][t] = product(k[x], q[n][x][kPieces - 1], s[n][t]);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) s[n][t][i] *= 1.0f / kPiece;
-        }
-      }
-#pragma unroll
-      for (int x = 0; x < kSteps; ++x)
-#pragma unroll
-        for (int n = 0; n < NR; ++n) s[n][t] = product(k[x], q[n][x][0], s[n][t]);
     }
-    __builtin_amdgcn_sched_barrier(0);   // (the phases as they stand: mixed, they take more registers than there are)
-    v_id = block_of(next.v, next_tile * kTile + kStrip * g);
-    load_keys(next_tile, block_of(next.k, next_tile * kTile + kStrip * k_strip), InWalk());
-    load_scales(v_id);
-    next = entries_of(min(tile + 2 * sharing, end - 1));
-    __builtin_amdgcn_sched_barrier(0);
-    // weights
+#pragma unroll
+    for (int x = 0; x < kSteps; ++x)
+#pragma unroll
+      for (int n = 0; n < NR; ++n) s[n][t] = product(k[x], q[n][x][0], s[n][t]);
+  };
+  // their weights in operands p, and the running maximum and sum
+  const auto weights = [&](int at_tile, float ks, float vs, bool strip) {
     const bool no_values = vs < kNoScale;   // (not a number: stays so)
     const float log_vs = strip ? __builtin_amdgcn_logf(no_values ? kNoScale : vs) : -INFINITY;
     const float inv_vs = 1.0f / (no_values ? kNoScale : vs);
-    const int at = tile * kTile + kStrip * g;
-    const bool whole = tile * kTile + kTile - 1 <= seen_first;
-    u32x4 p[NR][2][kPieces];
-    float alpha[NR];
+    const int at = at_tile * kTile + kStrip * g;
+    const bool whole = at_tile * kTile + kTile - 1 <= seen_first;
 #pragma unroll
     for (int n = 0; n < NR; ++n) {
       const float factor = strip ? q_scale[n] * ks : 0.0f, offset = fmaf(q_bias[n], factor, log_vs);
@@ -445,10 +439,10 @@ __global__ __launch_bounds__(kThreads, 2) void attention_kernel(const Problem a)
           const float w0 = __builtin_amdgcn_exp2f(fmaf(s[n][t][i], by, plus - base)), w1 = __builtin_amdgcn_exp2f(fmaf(s[n][t][i + 1], by, plus - base));
           total += w0 + w1;
           const uint32_t hi = pack_half(w0, w1);
-          (&p[n][t / 2][0].x)[2 * (t % 2) + i / 2] = hi;
+          p[n][t / 2][0][2 * (t % 2) + i / 2] = hi;
           if constexpr (kPieces > 1) {
             const v2h h2 = __builtin_bit_cast(v2h, hi);
-            (&p[n][t / 2][kPieces - 1].x)[2 * (t % 2) + i / 2] =
+            p[n][t / 2][kPieces - 1][2 * (t % 2) + i / 2] =
                 pack_half((w0 - static_cast<float>(h2[0])) * kPiece, (w1 - static_cast<float>(h2[1])) * kPiece);
           }
         }
@@ -462,10 +456,10 @@ __global__ __launch_bounds__(kThreads, 2) void attention_kernel(const Problem a)
         for (int y = 0; y < 2; ++y)
 #pragma unroll
           for (int e = 0; e < kPieces; ++e)
-            if (no_values) p[n][y][e] = u32x4{0u, 0u, 0u, 0u};
+#pragma unroll
+            for (int w = 0; w < 4; ++w) p[n][y][e][w] = no_values ? 0u : p[n][y][e][w];
     }
     __builtin_amdgcn_sched_barrier(0);
-    // weighted codes
     bool moved = false;
 #pragma unroll
     for (int n = 0; n < NR; ++n) moved = moved || alpha[n] != 1.0f;
@@ -477,26 +471,135 @@ __global__ __launch_bounds__(kThreads, 2) void attention_kernel(const Problem a)
 #pragma unroll
           for (int i = 0; i < 4; ++i) o[n][c][i] *= alpha[n];
     }
+  };
+  // the weighted codes of 16 columns
+  const auto add_values = [&](int c, const u32x4& v0, const u32x4& v1) {
+    const auto weight = [&](int n, int y, int e) { return u32x4{p[n][y][e][0], p[n][y][e][1], p[n][y][e][2], p[n][y][e][3]}; };
 #pragma unroll
-    for (int c = 0; c < kColumns; ++c) {
-      const u32x4 v0 = operand<true>(v_raw[c].x, v_raw[c].y), v1 = operand<true>(v_raw[c].z, v_raw[c].w);
+    for (int n = 0; n < NR; ++n) {
+      if constexpr (kPieces > 1) {
+        v4f low = {0.0f, 0.0f, 0.0f, 0.0f};
+        low = product(v0, weight(n, 0, kPieces - 1), low);
+        low = product(v1, weight(n, 1, kPieces - 1), low);
 #pragma unroll
-      for (int n = 0; n < NR; ++n) {
-        if constexpr (kPieces > 1) {
-          v4f low = {0.0f, 0.0f, 0.0f, 0.0f};
-          low = product(v0, p[n][0][kPieces - 1], low);
-          low = product(v1, p[n][1][kPieces - 1], low);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) o[n][c][i] = fmaf(low[i], 1.0f / kPiece, o[n][c][i]);
-        }
-        o[n][c] = product(v0, p[n][0][0], o[n][c]);
-        o[n][c] = product(v1, p[n][1][0], o[n][c]);
+        for (int i = 0; i < 4; ++i) o[n][c][i] = fmaf(low[i], 1.0f / kPiece, o[n][c][i]);
       }
+      o[n][c] = product(v0, weight(n, 0, 0), o[n][c]);
+      o[n][c] = product(v1, weight(n, 1, 0), o[n][c]);
     }
-    __builtin_amdgcn_sched_barrier(0);
-    load_values(next_tile, v_id, InWalk());
+  };
+
+  if (!together) {
+    // Each wave its own tiles: scores, weights, weighted codes. The next tile's keys are asked for as soon as this one's are in
+    // operands, its values likewise. A wave's loads come back in order, so what is waited for stands in front of what is
+    // not (the table's entries of the tile after next are read between the next tile's keys and its values), and no load
+    // depends on a branch, behind which the compiler would have to wait as if it had not been issued: the last tile asks for
+    // itself once more.
+    int v_id = -1;
+    if (tile < end) {
+      v_id = block_of(now.v, tile * kTile + kStrip * g);
+      load_keys(tile, block_of(now.k, tile * kTile + kStrip * k_strip), Ahead());
+      load_scales(v_id);
+      load_values(tile, v_id, Ahead());
+    }
+    take_queries();
+    for (; tile < end; tile += sharing) {
+      const int next_tile = min(tile + sharing, end - 1);
+      const float ks = k_scale, vs = v_scale;
+      const bool strip = v_id >= 0;
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        u32x4 k[kSteps];
+#pragma unroll
+        for (int c = 0; c < kChunks; ++c) {
+          k[2 * c] = operand<kExactKeys>(k_raw[t][c].x, k_raw[t][c].y);
+          k[2 * c + 1] = operand<kExactKeys>(k_raw[t][c].z, k_raw[t][c].w);
+        }
+        scores(t, k);
+      }
+      __builtin_amdgcn_sched_barrier(0);   // (the phases as they stand: mixed, they take more registers than there are)
+      v_id = block_of(next.v, next_tile * kTile + kStrip * g);
+      load_keys(next_tile, block_of(next.k, next_tile * kTile + kStrip * k_strip), InWalk());
+      load_scales(v_id);
+      next = entries_of(min(tile + 2 * sharing, end - 1));
+      __builtin_amdgcn_sched_barrier(0);
+      weights(tile, ks, vs, strip);
+#pragma unroll
+      for (int c = 0; c < kColumns; ++c) add_values(c, operand<true>(v_raw[c].x, v_raw[c].y), operand<true>(v_raw[c].z, v_raw[c].w));
+      __builtin_amdgcn_sched_barrier(0);
+      load_values(next_tile, v_id, InWalk());
+    }
+  } else if constexpr (kTogether) {
+    // All waves the same tiles, each with rows of its own: a wave converts a quarter of a tile's codes (keys of sub-tile `wave`,
+    // some columns of the values) and hands the operands on through LDS, in the order in which they are read, 16 bytes a lane.
+    // Two buffers: while one is read the next tile is written into the other, one barrier a tile.
+    u32x4* buffer = reinterpret_cast<u32x4*>(s_mem);
+    u32x4 k_part[kChunks], v_part[kParts];
+    const auto load_part = [&](int at_tile, const Entries& e, auto when, bool& strip) {
+      const int k_id = block_of(e.k, at_tile * kTile + kStrip * k_strip), v_id = block_of(e.v, at_tile * kTile + kStrip * g);
+      strip = v_id >= 0;
+      const int8_t* k = key_address(at_tile, k_id) + 4 * wave * D;
+#pragma unroll
+      for (int c = 0; c < kChunks; ++c) k_part[c] = when.load(k + 64 * c);
+      load_scales(v_id);
+      const int8_t* v = value_address(at_tile, v_id) + 16 * kStrip * kParts * wave;
+#pragma unroll
+      for (int c = 0; c < kParts; ++c) v_part[c] = when.load(v + 16 * kStrip * c);
+    };
+    const auto hand_on = [&](int which) {
+      u32x4* to = buffer + which * kOperands * kWave + lane;
+#pragma unroll
+      for (int c = 0; c < kChunks; ++c) {
+        to[(wave * kSteps + 2 * c) * kWave] = operand<kExactKeys>(k_part[c].x, k_part[c].y);
+        to[(wave * kSteps + 2 * c + 1) * kWave] = operand<kExactKeys>(k_part[c].z, k_part[c].w);
+      }
+#pragma unroll
+      for (int c = 0; c < kParts; ++c) {
+        to[(4 * kSteps + 2 * (kParts * wave + c)) * kWave] = operand<true>(v_part[c].x, v_part[c].y);
+        to[(4 * kSteps + 2 * (kParts * wave + c) + 1) * kWave] = operand<true>(v_part[c].z, v_part[c].w);
+      }
+    };
+    bool strip = false, next_strip = false;
+    float ks = 0.0f, vs = 0.0f;
+    int which = 0;
+    if (tile < end) {
+      load_part(tile, now, Ahead(), strip);
+      take_queries();
+      hand_on(0);
+      ks = k_scale;
+      vs = v_scale;
+      load_part(min(tile + 1, end - 1), next, Ahead(), next_strip);
+      next = entries_of(min(tile + 2, end - 1));
+      __syncthreads();
+    }
+    for (; tile < end; ++tile) {
+      if (tile * kTile <= seen_last) {   // (of this wave)
+        const u32x4* from = buffer + which * kOperands * kWave + lane;
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+          u32x4 k[kSteps];
+#pragma unroll
+          for (int x = 0; x < kSteps; ++x) k[x] = from[(t * kSteps + x) * kWave];
+          scores(t, k);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        weights(tile, ks, vs, strip);
+#pragma unroll
+        for (int c = 0; c < kColumns; ++c) add_values(c, from[(4 * kSteps + 2 * c) * kWave], from[(4 * kSteps + 2 * c + 1) * kWave]);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      which ^= 1;
+      hand_on(which);
+      ks = k_scale;
+      vs = v_scale;
+      strip = next_strip;
+      load_part(min(tile + 2, end - 1), next, InWalk(), next_strip);
+      next = entries_of(min(tile + 3, end - 1));
+      __syncthreads();
+    }
   }
 
+  float* s_part = reinterpret_cast<float*>(s_mem);   // (behind the walk's last barrier, where it has one)
   // the waves that share a row tile: max m_w, sum l_w 2^(m_w - m), sum O_w 2^(m_w - m), in wave order
 #pragma unroll
   for (int n = 0; n < NR; ++n) {
@@ -600,8 +703,8 @@ __global__ __launch_bounds__(kThreads) void merge_kernel(const Problem a) {
 // rows that a wave takes, in 16ths: what an average sequence has
 int row_tiles(int64_t rows, int sequences, int group, int head_dim) {
   const int64_t average = rows * group / sequences;
-  const int most = head_dim == 64 ? 4 : head_dim == 128 ? 2 : 1;   // (registers)
-  return average <= 16 || most == 1 ? 1 : average <= 32 || most == 2 ? 2 : 4;
+  const int most = head_dim == 64 ? 4 : 2;   // (registers)
+  return average <= 16 ? 1 : average <= 32 || most == 2 ? 2 : 4;
 }
 
 // row groups of the batch (an upper bound: Ragged::find with spare 1)
@@ -628,7 +731,8 @@ template <typename T> int launch(const Problem& a, int D, int tiles, int64_t gro
     if (tiles == 1) LLMQ_ATTEND(128, 1);
     else LLMQ_ATTEND(128, 2);
   } else {
-    LLMQ_ATTEND(256, 1);
+    if (tiles == 1) LLMQ_ATTEND(256, 1);
+    else LLMQ_ATTEND(256, 2);
   }
 #undef LLMQ_ATTEND
   if (int rc = llmq_host::check_launch("attention_kernel")) return rc;
