@@ -38,6 +38,7 @@ constexpr int kHeader = 4;            // floats in front of a partial result: ma
 constexpr int kMaxSplits = 64;        // of a row: what a wave's lanes hold
 constexpr int kUnits = 1024;          // workgroups that the work is cut for: two rounds of those resident with heads of 128
 constexpr int kLeastTiles = 8;        // of a split: two for each wave
+constexpr int kFewSplits = 8;         // .. that a row's wave merges
 constexpr int kMostRecords = 1 << 16; // partial results of a launch (more would cost more than they save)
 constexpr float kBias = 1152.0f;      // what a code is too high as an operand: 1024, and 128 of the flipped sign
 constexpr float kNoScale = 0x1p-100f; // value scales below count as zero
@@ -421,7 +422,7 @@ __global__ __launch_bounds__(kThreads, (kOccupancy<T, D, NR>)) void attention_ke
 #pragma unroll
         for (int t = 0; t < 4; ++t)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) s[n][t][i] = at + 4 * t + i > last[n] ? -INFINITY : fmaf(s[n][t][i], factor, offset);
+          for (int i = 0; i < 4; ++i) s[n][t][i] = 4 * t + i > last[n] - at ? -INFINITY : fmaf(s[n][t][i], factor, offset);
       }
 #pragma unroll
       for (int t = 0; t < 4; ++t)
@@ -658,13 +659,15 @@ __global__ __launch_bounds__(kThreads, (kOccupancy<T, D, NR>)) void attention_ke
   else finish(std::integral_constant<int, 1>());
 }
 
-// The partial results of a row and head, by a workgroup: four columns of every kAtOnce-th of them a thread, all asked for at once.
-template <typename T, int D>
+// The partial results of a row and head, by WAVES waves: four columns of every kAtOnce-th of at most SPLITS a thread, all asked for
+// at once. One wave a row where there are many rows, which then have few splits (most_splits); else a workgroup.
+template <typename T, int D, int WAVES, int SPLITS>
 __global__ __launch_bounds__(kThreads) void merge_kernel(const Problem a) {
-  constexpr int kQuads = D / 4, kAtOnce = kThreads / kQuads, kEach = kMaxSplits / kAtOnce, kRecord = D + kHeader;
-  __shared__ __attribute__((aligned(16))) float s_part[kAtOnce][D];
-  const int tid = threadIdx.x, lane = tid & (kWave - 1), quad = tid % kQuads, at = tid / kQuads;
-  const int64_t vector = blockIdx.x;
+  constexpr int kQuads = D / 4, kAtOnce = WAVES * kWave / kQuads, kEach = (SPLITS + kAtOnce - 1) / kAtOnce, kRecord = D + kHeader;
+  __shared__ __attribute__((aligned(16))) float s_part[WAVES > 1 ? kAtOnce : 1][D];
+  const int tid = threadIdx.x % (WAVES * kWave), lane = tid & (kWave - 1), quad = tid % kQuads, at = tid / kQuads;
+  const int64_t vector = static_cast<int64_t>(blockIdx.x) * (kWaves / WAVES) + __builtin_amdgcn_readfirstlane(threadIdx.x / (WAVES * kWave));
+  if (vector >= static_cast<int64_t>(a.rows.rows) * a.q_heads) return;
   if (a.rows.start != nullptr) {   // rows of no sequence have none
     const int row = static_cast<int>(vector / a.q_heads);
     if (row < a.rows.first(0) || row >= a.rows.first(a.rows.sequences)) return;
@@ -686,25 +689,35 @@ __global__ __launch_bounds__(kThreads) void merge_kernel(const Problem a) {
     const float w = __shfl(weight, (at + i * kAtOnce) & (kWave - 1), kWave);
     if (w != 0.0f) total += part[i] * w;   // (a split that saw nothing has written no columns)
   }
-  *reinterpret_cast<v4f*>(&s_part[at][4 * quad]) = total;
-  __syncthreads();
-  if (tid >= D / 8) return;
-  float f[8] = {};
-#pragma unroll
-  for (int i = 0; i < kAtOnce; ++i)
-#pragma unroll
-    for (int e = 0; e < 8; ++e) f[e] += s_part[i][8 * tid + e];
   const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+  if constexpr (WAVES == 1) {
 #pragma unroll
-  for (int e = 0; e < 8; ++e) f[e] *= inv;
-  store8(static_cast<T*>(a.out) + vector * D + 8 * tid, f);
+    for (int step = kQuads; step < kWave; step *= 2)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) total[e] += __shfl_xor(total[e], step, kWave);
+    if (at != 0) return;
+    T* out = static_cast<T*>(a.out) + vector * D + 4 * quad;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) out[e] = from_float<T>(total[e] * inv);
+  } else {
+    *reinterpret_cast<v4f*>(&s_part[at][4 * quad]) = total;
+    __syncthreads();
+    if (tid >= D / 8) return;
+    float f[8] = {};
+#pragma unroll
+    for (int i = 0; i < kAtOnce; ++i)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) f[e] += s_part[i][8 * tid + e];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) f[e] *= inv;
+    store8(static_cast<T*>(a.out) + vector * D + 8 * tid, f);
+  }
 }
 
 // rows that a wave takes, in 16ths: what an average sequence has
-int row_tiles(int64_t rows, int sequences, int group, int head_dim) {
+int row_tiles(int64_t rows, int sequences, int group) {
   const int64_t average = rows * group / sequences;
-  const int most = head_dim == 64 ? 4 : 2;   // (registers)
-  return average <= 16 ? 1 : average <= 32 || most == 2 ? 2 : 4;
+  return average <= 16 ? 1 : 2;
 }
 
 // row groups of the batch (an upper bound: Ragged::find with spare 1)
@@ -725,8 +738,7 @@ template <typename T> int launch(const Problem& a, int D, int tiles, int64_t gro
 #define LLMQ_ATTEND(DIM, NR) hipLaunchKernelGGL((attention_kernel<T, DIM, NR>), grid, block, 0, s, a)
   if (D == 64) {
     if (tiles == 1) LLMQ_ATTEND(64, 1);
-    else if (tiles == 2) LLMQ_ATTEND(64, 2);
-    else LLMQ_ATTEND(64, 4);
+    else LLMQ_ATTEND(64, 2);
   } else if (D == 128) {
     if (tiles == 1) LLMQ_ATTEND(128, 1);
     else LLMQ_ATTEND(128, 2);
@@ -737,8 +749,14 @@ template <typename T> int launch(const Problem& a, int D, int tiles, int64_t gro
 #undef LLMQ_ATTEND
   if (int rc = llmq_host::check_launch("attention_kernel")) return rc;
   if (a.splits == 1) return 0;
-  const dim3 merge_grid(static_cast<unsigned>(a.rows.rows) * a.q_heads);
-#define LLMQ_MERGE(DIM) hipLaunchKernelGGL((merge_kernel<T, DIM>), merge_grid, block, 0, s, a)
+  const bool few = a.splits <= kFewSplits;
+  const int64_t vectors = static_cast<int64_t>(a.rows.rows) * a.q_heads;
+  const dim3 merge_grid(static_cast<unsigned>(few ? (vectors + kWaves - 1) / kWaves : vectors));
+#define LLMQ_MERGE(DIM)                                                                                          \
+  do {                                                                                                           \
+    if (few) hipLaunchKernelGGL((merge_kernel<T, DIM, 1, kFewSplits>), merge_grid, block, 0, s, a);              \
+    else hipLaunchKernelGGL((merge_kernel<T, DIM, kWaves, kMaxSplits>), merge_grid, block, 0, s, a);             \
+  } while (0)
   if (D == 64) LLMQ_MERGE(64);
   else if (D == 128) LLMQ_MERGE(128);
   else LLMQ_MERGE(256);
@@ -771,7 +789,7 @@ extern "C" int llmq_kv_block_attention(const void* query, int64_t q_row_stride, 
   if (q_row_stride % v) return llmq_host::fail_invalid("row strides must be multiples of %d elements", v);
   if (tokens == 0 || sequences == 0) return 0;
   if (n_blocks == 0) table_width = 0;   // no token has a block
-  const int group = q_heads / kv_heads, tiles = row_tiles(tokens, sequences, group, head_dim);
+  const int group = q_heads / kv_heads, tiles = row_tiles(tokens, sequences, group);
   // (row numbers, and the launch's workgroups, are counted in 32 bits)
   const int64_t vectors = static_cast<int64_t>(tokens) * q_heads;
   const int splits = most_splits(vectors, block, table_width);
