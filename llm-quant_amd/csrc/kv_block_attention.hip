@@ -98,7 +98,7 @@ __device__ __forceinline__ Sequence sequence_of(const Problem& a, int b, int gro
     to = a.rows.start[at + 1];
   }
   const int cached = a.cached[at];
-  const int first = min(max(from, 0), a.rows.rows), n = b < a.rows.sequences ? max(min(max(to, 0), a.rows.rows) - first, 0) : 0;
+  const int first = min(max(from, 0), a.rows.rows), n = b < a.rows.sequences ? max(min(max(to, 0), a.rows.rows) - first, 0) : 0;   // (as in Ragged)
   const int64_t held = min(static_cast<int64_t>(a.table.width) << a.block_shift, static_cast<int64_t>(INT32_MAX - 2 * kTile));
   const int seen = cached < 0 ? 0 : static_cast<int>(min(static_cast<int64_t>(cached) + n, held));
   return Sequence{first, n, cached, (n * a.group + group_rows - 1) / group_rows, (seen + kTile - 1) / kTile};
@@ -720,7 +720,7 @@ int row_tiles(int64_t rows, int sequences, int group) {
   return average <= 16 ? 1 : 2;
 }
 
-// row groups of the batch (an upper bound: Ragged::find with spare 1)
+// row groups of the batch (an upper bound)
 int64_t row_groups(int64_t rows, int sequences, int group, int tiles) {
   return rows * group / (kWaves * 16 * tiles) + sequences;
 }

@@ -27,6 +27,10 @@ struct BlockTable {
   }
 };
 
+// The rows of a sequence.
+struct Span {
+  int first, n;
+};
 // The rows of a batch. Everything read from `start` is clamped, so that no content of it leads out of the tensors.
 struct Ragged {
   const int32_t* start;   // [sequences + 1], or null: one row each
@@ -34,26 +38,34 @@ struct Ragged {
   __device__ __forceinline__ int first(int b) const {
     return start == nullptr ? b : min(max(start[b], 0), rows);
   }
-  __device__ __forceinline__ int count(int b) const {
-    return start == nullptr ? 1 : max(min(max(start[b + 1], 0), rows) - first(b), 0);
-  }
-  // A launch cannot know on the host how many pieces of `tile` units each sequence's rows make (the starts lie on the
-  // device), but it can bound their sum: sequence b's pieces are numbered from floor(first(b) * units / tile) + spare * b,
-  // and between two sequences' numbers there is room for floor(rows * units / tile) + spare pieces. Finds the sequence
-  // of piece `slot`, 64 starts at a time (they grow with b, so the last one at or below the slot is counted), and leaves in
-  // `slot` the piece's index within the sequence. Called by whole waves. sequences > 0.
-  __device__ __forceinline__ int find(int64_t units, int tile, int spare, int64_t& slot) const {
+  // A launch cannot know on the host how many blocks each sequence's rows touch (the starts lie on the device), but it can bound
+  // their sum: sequence b's pieces are numbered from floor(first(b) / block) + 2 b on, and up to the next sequence's number
+  // there is room for floor(n / block) + 2, which is as many as n rows can touch. Finds the sequence of piece `slot`, 64
+  // at a time (the numbers grow with b, so the last one at or below the slot is counted); leaves in `slot` the piece's index
+  // within the sequence, its rows in `span` and its entry of `more` (may be null: 0) in `other`, all read in one trip to
+  // memory. Called by whole waves. sequences > 0.
+  __device__ __forceinline__ int find(int block_shift, const int32_t* more, int& slot, Span& span, int& other) const {
     const int lane = threadIdx.x & (kWave - 1);
-    int found = 0;
+    int b = 0, number = 0;
     for (int b0 = 0; b0 < sequences; b0 += kWave) {
-      const int b = b0 + lane;
-      const bool below = b < sequences && first(b) * units / tile + static_cast<int64_t>(spare) * b <= slot;
-      const int n = __popcll(__ballot(below));
-      found += n;
-      if (n < kWave) break;
+      const int at = min(b0 + lane, sequences - 1);
+      int from = at, to = at + 1;
+      if (start != nullptr) {
+        from = start[at];
+        to = start[at + 1];
+      }
+      const int value = more != nullptr ? more[at] : 0;
+      from = min(max(from, 0), rows);
+      const int n = max(min(max(to, 0), rows) - from, 0), mine = (from >> block_shift) + 2 * (b0 + lane);
+      const int below = __popcll(__ballot(b0 + lane < sequences && mine <= slot));
+      if (below == 0) break;
+      b = b0 + below - 1;
+      number = __builtin_amdgcn_readlane(mine, below - 1);
+      span = Span{__builtin_amdgcn_readlane(from, below - 1), __builtin_amdgcn_readlane(n, below - 1)};
+      other = __builtin_amdgcn_readlane(value, below - 1);
+      if (below < kWave) break;
     }
-    const int b = max(found - 1, 0);
-    slot -= first(b) * units / tile + static_cast<int64_t>(spare) * b;
+    slot -= number;
     return b;
   }
 };

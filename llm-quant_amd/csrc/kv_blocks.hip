@@ -5,9 +5,9 @@
 //            codes of the call's tokens: clamp(rint(x / s)); of the block's earlier tokens: clamp(rint((c s_old) / s))
 //   dequant  T(c s)
 //
-// Both take a strip of 16 tokens by eight columns a lane: a packet of 16-bit values for each token, eight bytes of each
-// token's key codes, 16 bytes of each column's value codes (16 tokens innermost), so that the transposition of the
-// values is a choice of bytes within a lane. Bound: HBM, each tensor read once and written once; at a step's few tokens the
+// A lane takes eight columns of eight tokens (append) or of a strip of 16 (dequant): a packet of 16-bit values for each token,
+// eight bytes of each token's key codes, eight or 16 bytes of each column's value codes (16 tokens innermost), so that the
+// transposition of the values is a choice of bytes within a lane. Bound: HBM, each tensor read once and written once; at a step's few tokens the
 // chain starts -> cached -> table -> block.
 #include "kv_blocks.h"
 
@@ -25,8 +25,43 @@ template <typename T> __device__ __forceinline__ void store8(T* p, const float* 
 #pragma unroll
   for (int i = 0; i < kColumns; i += Pack<T>::N) store16(p + i, Pack<T>::pack(f + i));
 }
+// (past the caches)
+template <typename T> __device__ __forceinline__ void stream8(T* p, const float* f) {
+#pragma unroll
+  for (int i = 0; i < kColumns; i += Pack<T>::N) stream16(p + i, Pack<T>::pack(f + i));
+}
 __device__ __forceinline__ float code_of(uint32_t word, int byte) { return static_cast<float>(static_cast<int8_t>(word >> (8 * byte))); }
+// rint(x / s), clamped, for eight values: the quotient by way of the reciprocal, which is off by less than 2.4e-5 (codes are at most
+// 127.5), and divided where that could make another integer. Eight divisions are some eighty instructions, this is thirty.
+__device__ __forceinline__ void codes_of8(float* f, float s, float inv) {
+  float q[kColumns], far = 0.0f;
+#pragma unroll
+  for (int e = 0; e < kColumns; ++e) {
+    const float r = f[e] * inv;
+    q[e] = rintf(r);
+    far = fmaxf(far, fabsf(r - q[e]));
+  }
+  if (far > 0.49995f) {
+#pragma unroll
+    for (int e = 0; e < kColumns; ++e) q[e] = rintf(f[e] / s);
+  }
+#pragma unroll
+  for (int e = 0; e < kColumns; ++e) f[e] = fminf(fmaxf(q[e], -128.0f), 127.0f);
+}
 __device__ __forceinline__ uint32_t byte_of(float code, int byte) { return (static_cast<uint32_t>(static_cast<int>(code)) & 0xffu) << (8 * byte); }
+
+__device__ __forceinline__ u32x2 bytes_of(const float* f) {
+  return u32x2{byte_of(f[0], 0) | byte_of(f[1], 1) | byte_of(f[2], 2) | byte_of(f[3], 3),
+               byte_of(f[4], 0) | byte_of(f[5], 1) | byte_of(f[6], 2) | byte_of(f[7], 3)};
+}
+// eight codes brought to another scale
+__device__ __forceinline__ u32x2 moved8(u32x2 w, float before, float s, float inv) {
+  float f[kColumns];
+#pragma unroll
+  for (int e = 0; e < kColumns; ++e) f[e] = code_of(e < 4 ? w.x : w.y, e % 4) * before;
+  codes_of8(f, s, inv);
+  return bytes_of(f);
+}
 
 // The tokens of the call that lie in one block of a sequence.
 struct Touched {
@@ -35,20 +70,22 @@ struct Touched {
   int64_t row;     // the row of slot lo
 };
 // `from`: the position of the sequence's first row; piece: which of the blocks from there on. False: no row in that block.
-__device__ __forceinline__ bool touched_block(const BlockTable& table, int b, int64_t first_row, int n, int64_t from, int64_t piece,
-                                              int block_shift, Touched& t) {
+__device__ __forceinline__ bool touched_block(const BlockTable& table, int b, const Span& rows, int64_t from, int piece, int block_shift,
+                                              Touched& t) {
   const int64_t logical = (from >> block_shift) + piece, at = logical << block_shift;
-  if (n == 0 || at > from + n - 1) return false;
+  if (rows.n == 0 || at > from + rows.n - 1) return false;
   t.id = logical < table.width ? table.at(b, static_cast<int>(logical)) : -1;
   t.lo = static_cast<int>(max(from - at, static_cast<int64_t>(0)));
-  t.hi = static_cast<int>(min(from + n - at, static_cast<int64_t>(1) << block_shift));
-  t.row = first_row + (at + t.lo - from);
+  t.hi = static_cast<int>(min(from + rows.n - at, static_cast<int64_t>(1) << block_shift));
+  t.row = rows.first + (at + t.lo - from);
   return true;
 }
 
-// A head's lanes: (BLOCK / 16) (D / 8), the strips of a block; a workgroup has as many whole heads as 64 lanes hold, or one.
+constexpr int kTokens = 8;   // of a lane of append
+
+// A head's lanes: (BLOCK / 8) (D / 8); a workgroup has as many whole heads as 64 lanes hold, or one.
 template <int D, int BLOCK> struct AppendShape {
-  static constexpr int kLanes = BLOCK / kStrip * (D / kColumns);
+  static constexpr int kLanes = BLOCK / kTokens * (D / kColumns);
   static constexpr int kThreads = kLanes > kWave ? kLanes : kWave, kHeads = kThreads / kLanes;
 };
 
@@ -63,41 +100,35 @@ __global__ __launch_bounds__((AppendShape<D, BLOCK>::kThreads)) void append_kern
   const int sets = (heads + Shape::kHeads - 1) / Shape::kHeads;   // of heads
   const bool is_value = blockIdx.x & 1;
   const int set = static_cast<int>(blockIdx.x / 2) % sets;
-  int64_t piece = blockIdx.x / 2 / sets;
-  int b;
+  int piece = blockIdx.x / 2 / sets, b = piece, from;
+  Span span{b, 1};
   if (rows.start == nullptr) {
-    b = static_cast<int>(piece);
+    from = cached[b];
     piece = 0;
   } else {
-    b = rows.find(1, BLOCK, 2, piece);
+    b = rows.find(kShift, cached, piece, span, from);
   }
-  const int from = cached[b];
   Touched here;
-  if (from < 0 || !touched_block(table, b, rows.first(b), rows.count(b), from, piece, kShift, here) || here.id < 0) return;
+  if (from < 0 || !touched_block(table, b, span, from, piece, kShift, here) || here.id < 0) return;
   const int h = set * Shape::kHeads + static_cast<int>(threadIdx.x) / Shape::kLanes, in_head = threadIdx.x % Shape::kLanes;
-  const int strip = in_head / (D / kColumns), d = in_head % (D / kColumns) * kColumns;
+  const int slot0 = in_head / (D / kColumns) * kTokens, d = in_head % (D / kColumns) * kColumns;
   const bool active = h < heads;   // (the others stay for the barrier)
   const int64_t unit = static_cast<int64_t>(here.id) * heads + min(h, heads - 1);
   float* scale = (is_value ? v_scale : k_scale) + unit;
   const float before = *scale;
-  // the strip's tokens of the call: lo .. hi - 1 of its 16; the block's earlier ones: below lo
-  const int lo = min(max(here.lo - kStrip * strip, 0), kStrip), hi = active ? min(max(here.hi - kStrip * strip, 0), kStrip) : 0;
+  // the lane's tokens of the call: lo .. hi - 1 of its eight; the block's earlier ones: below lo
+  const int lo = min(max(here.lo - slot0, 0), kTokens), hi = active ? min(max(here.hi - slot0, 0), kTokens) : 0;
   const int64_t stride = is_value ? value_stride : key_stride;
-  const T* x = (is_value ? value : key) + (here.row + kStrip * strip - here.lo) * stride + static_cast<int64_t>(h) * D + d;
+  const T* x = (is_value ? value : key) + (here.row + slot0 - here.lo) * stride + static_cast<int64_t>(h) * D + d;
   constexpr int kPackets = kColumns / Pack<T>::N;
-  u32x4 raw[kStrip][kPackets];
+  u32x4 raw[kTokens][kPackets];
 #pragma unroll
-  for (int i = 0; i < kStrip; ++i)
-    if (i >= lo && i < hi) {
+  for (int i = 0; i < kTokens; ++i)
 #pragma unroll
-      for (int e = 0; e < kPackets; ++e) raw[i][e] = load16(x + i * stride + e * Pack<T>::N);
-    } else {
-#pragma unroll
-      for (int e = 0; e < kPackets; ++e) raw[i][e] = u32x4{0u, 0u, 0u, 0u};
-    }
+    for (int e = 0; e < kPackets; ++e) raw[i][e] = i >= lo && i < hi ? load16(x + i * stride + e * Pack<T>::N) : u32x4{0u, 0u, 0u, 0u};
   float amax = 0.0f;
 #pragma unroll
-  for (int i = 0; i < kStrip; ++i) {
+  for (int i = 0; i < kTokens; ++i) {
     float f[kColumns];
 #pragma unroll
     for (int e = 0; e < kPackets; ++e) Pack<T>::unpack(raw[i][e], f + e * Pack<T>::N);
@@ -114,78 +145,69 @@ __global__ __launch_bounds__((AppendShape<D, BLOCK>::kThreads)) void append_kern
   if (!active) return;
   float s = scale_from_amax(amax, 127.0f);
   if (here.lo > 0) s = fmaxf(s, before);
-  const bool grown = here.lo > 0 && s > before;
+  const bool grown = here.lo > 0 && s > before && lo > 0;   // and this lane has earlier tokens
   if (in_head == 0) *scale = s;
-  if (hi <= lo && !(grown && lo > 0)) return;   // nothing of this strip changes
+  if (hi <= lo && !grown) return;   // nothing of this lane's changes
 
-  const auto moved = [&](uint32_t word, int byte) { return byte_of(quant_code(code_of(word, byte) * before, s, -128.0f, 127.0f), byte); };
-  const auto codes_of = [&](int i, float* f) {
+  const float inv = 1.0f / s;
+  const auto codes_of = [&](int i) {   // the eight codes of token i
+    float f[kColumns];
 #pragma unroll
     for (int e = 0; e < kPackets; ++e) Pack<T>::unpack(raw[i][e], f + e * Pack<T>::N);
-#pragma unroll
-    for (int e = 0; e < kColumns; ++e) f[e] = quant_code(f[e], s, -128.0f, 127.0f);
+    codes_of8(f, s, inv);
+    return bytes_of(f);
   };
   if (!is_value) {
-    int8_t* codes = k_codes + (unit * BLOCK + kStrip * strip) * D + d;
+    int8_t* codes = k_codes + (unit * BLOCK + slot0) * D + d;
 #pragma unroll
-    for (int i = 0; i < kStrip; ++i) {
+    for (int i = 0; i < kTokens; ++i) {
       u32x2* at = reinterpret_cast<u32x2*>(codes + i * D);
-      if (i >= lo && i < hi) {
-        float f[kColumns];
-        codes_of(i, f);
-        *at = u32x2{byte_of(f[0], 0) | byte_of(f[1], 1) | byte_of(f[2], 2) | byte_of(f[3], 3),
-                    byte_of(f[4], 0) | byte_of(f[5], 1) | byte_of(f[6], 2) | byte_of(f[7], 3)};
-      } else if (grown && i < lo) {
-        const u32x2 w = *at;
-        *at = u32x2{moved(w.x, 0) | moved(w.x, 1) | moved(w.x, 2) | moved(w.x, 3),
-                    moved(w.y, 0) | moved(w.y, 1) | moved(w.y, 2) | moved(w.y, 3)};
-      }
+      if (i >= lo && i < hi) *at = codes_of(i);
+      else if (grown && i < lo) *at = moved8(*at, before, s, inv);
     }
     return;
   }
-  int8_t* codes = v_codes + ((unit * (BLOCK / kStrip) + strip) * D + d) * kStrip;
-  if (hi - lo == 1 && !(grown && lo > 0)) {   // a token: its bytes alone (a step's; nothing is read)
+  int8_t* codes = v_codes + ((unit * (BLOCK / kStrip) + slot0 / kStrip) * D + d) * kStrip + slot0 % kStrip;
+  if (hi - lo == 1 && !grown) {   // a token: its bytes alone (a step's; nothing is read)
 #pragma unroll
-    for (int i = 0; i < kStrip; ++i)
+    for (int i = 0; i < kTokens; ++i)
       if (i == lo) {
-        float f[kColumns];
-        codes_of(i, f);
+        const u32x2 c = codes_of(i);
 #pragma unroll
-        for (int e = 0; e < kColumns; ++e) codes[e * kStrip + i] = static_cast<int8_t>(f[e]);
+        for (int e = 0; e < kColumns; ++e) codes[e * kStrip + i] = static_cast<int8_t>((e < 4 ? c.x : c.y) >> (8 * (e % 4)));
       }
     return;
   }
-  uint32_t words[kColumns][kStrip / 4] = {};
-  if (hi > lo) {
+  // columns of eight tokens, out of tokens of eight columns
+  u32x2 tokens[kTokens];
 #pragma unroll
-    for (int i = 0; i < kStrip; ++i) {
-      float f[kColumns];
-      codes_of(i, f);
+  for (int i = 0; i < kTokens; ++i) tokens[i] = codes_of(i);
+  // bytes of other tokens among them stay, or move to the new scale
+  uint32_t fresh[2] = {}, old[2] = {};
 #pragma unroll
-      for (int e = 0; e < kColumns; ++e) words[e][i / 4] |= byte_of(f[e], i % 4);
-    }
+  for (int i = 0; i < kTokens; ++i) {
+    fresh[i / 4] |= i >= lo && i < hi ? 0xffu << (8 * (i % 4)) : 0u;
+    old[i / 4] |= grown && i < lo ? 0xffu << (8 * (i % 4)) : 0u;
   }
-  if (lo > 0 || hi < kStrip) {   // bytes of other tokens lie among them
-    uint32_t fresh[kStrip / 4] = {}, old[kStrip / 4] = {};
 #pragma unroll
-    for (int i = 0; i < kStrip; ++i) {
-      fresh[i / 4] |= i >= lo && i < hi ? 0xffu << (8 * (i % 4)) : 0u;
-      old[i / 4] |= grown && i < lo ? 0xffu << (8 * (i % 4)) : 0u;
+  for (int e = 0; e < kColumns; ++e) {
+    u32x2 column{0u, 0u};
+#pragma unroll
+    for (int i = 0; i < kTokens; ++i) {
+      const uint32_t code = ((e < 4 ? tokens[i].x : tokens[i].y) >> (8 * (e % 4)) & 0xffu) << (8 * (i % 4));
+      (i < 4 ? column.x : column.y) |= code;
     }
-#pragma unroll
-    for (int e = 0; e < kColumns; ++e) {
-      const u32x4 r = load16(codes + e * kStrip);
-      const uint32_t held[kStrip / 4] = {r.x, r.y, r.z, r.w};
-#pragma unroll
-      for (int w = 0; w < kStrip / 4; ++w) {
-        uint32_t kept = held[w];
-        if (old[w] != 0u) kept = (kept & ~old[w]) | ((moved(kept, 0) | moved(kept, 1) | moved(kept, 2) | moved(kept, 3)) & old[w]);
-        words[e][w] = (kept & ~fresh[w]) | (words[e][w] & fresh[w]);
+    u32x2* at = reinterpret_cast<u32x2*>(codes + e * kStrip);
+    if (lo > 0 || hi < kTokens) {
+      u32x2 held = *at;
+      if (grown) {
+        const u32x2 m = moved8(held, before, s, inv);
+        held = u32x2{(held.x & ~old[0]) | (m.x & old[0]), (held.y & ~old[1]) | (m.y & old[1])};
       }
+      column = u32x2{(held.x & ~fresh[0]) | (column.x & fresh[0]), (held.y & ~fresh[1]) | (column.y & fresh[1])};
     }
+    *at = column;
   }
-#pragma unroll
-  for (int e = 0; e < kColumns; ++e) store16(codes + e * kStrip, u32x4{words[e][0], words[e][1], words[e][2], words[e][3]});
 }
 
 constexpr int kDequantThreads = 256;
@@ -195,14 +217,15 @@ template <typename T, int D>
 __global__ __launch_bounds__(kDequantThreads) void dequant_kernel(
     const int8_t* __restrict__ k_codes, const int8_t* __restrict__ v_codes, const float* __restrict__ k_scale,
     const float* __restrict__ v_scale, const BlockTable table, const Ragged rows, const int32_t* __restrict__ first_or_null,
-    T* __restrict__ k_out, T* __restrict__ v_out, const int heads, const int block_shift) {
+    T* __restrict__ k_out, T* __restrict__ v_out, const int heads, const int block_shift, const bool past_caches) {
   const int strips = 1 << (block_shift - 4), lanes = heads * strips * (D / kColumns), sets = (lanes + kDequantThreads - 1) / kDequantThreads;
   const bool is_value = blockIdx.x & 1;
   const int set = static_cast<int>(blockIdx.x / 2) % sets;
-  int64_t piece = blockIdx.x / 2 / sets;
-  const int b = rows.find(1, strips * kStrip, 2, piece);
+  int piece = blockIdx.x / 2 / sets, from;
+  Span span{0, 0};
+  const int b = rows.find(block_shift, first_or_null, piece, span, from);
   Touched here;
-  if (!touched_block(table, b, rows.first(b), rows.count(b), first_or_null == nullptr ? 0 : max(first_or_null[b], 0), piece, block_shift, here)) return;
+  if (!touched_block(table, b, span, max(from, 0), piece, block_shift, here)) return;
   const int item = set * kDequantThreads + static_cast<int>(threadIdx.x);
   if (item >= lanes) return;
   const int d = item % (D / kColumns) * kColumns, strip = item / (D / kColumns) % strips, h = item / (D / kColumns) / strips;
@@ -241,7 +264,9 @@ __global__ __launch_bounds__(kDequantThreads) void dequant_kernel(
 #pragma unroll
     for (int e = 0; e < kColumns; ++e)
       f[e] = (is_value ? code_of(words[2 * e + i / 8][i / 4 % 2], i % 4) : code_of(words[i][e / 4], e % 4)) * s;
-    store8(out + static_cast<int64_t>(i) * D, f);
+    T* to = out + static_cast<int64_t>(i) * D;
+    if (past_caches) stream8(to, f);
+    else store8(to, f);
   }
 }
 
@@ -252,7 +277,7 @@ int check_cache(const void* k_codes, const void* v_codes, const void* k_scale, c
   return 0;
 }
 
-// pieces of a ragged batch (Ragged::find with spare 2): an upper bound of the blocks that its rows touch
+// pieces of a ragged batch (Ragged::find): an upper bound of the blocks that its rows touch
 int64_t pieces(int rows, int sequences, int block) { return rows / block + 2LL * sequences; }
 
 }  // namespace
@@ -340,12 +365,15 @@ extern "C" int llmq_kv_block_dequant(const void* k_codes, const void* v_codes, c
   const int64_t workgroups = pieces(n_tokens, sequences, block) * 2 * ((lanes + kDequantThreads - 1) / kDequantThreads);
   if (lanes > INT32_MAX - kDequantThreads || workgroups > INT32_MAX)
     return llmq_host::fail_invalid("too many rows, sequences and heads for one launch: %d, %d, %d", n_tokens, sequences, kv_heads);
+  // What is larger than the L2 caches (eight of 4 MB) leaves them before it is read: written past them it does not push the codes
+  // out either. 40000 tokens of eight heads of 128, bf16: 54.8 -> 39.7 us (6.2 TB/s).
+  const bool past_caches = 2.0 * n_tokens * kv_heads * head_dim * (dtype == LLMQ_F32 ? 4 : 2) > 32e6;
   const dim3 grid(static_cast<unsigned>(workgroups));
   hipStream_t s = static_cast<hipStream_t>(stream);
 #define LLMQ_DEQUANT(T, D)                                                                                               \
   hipLaunchKernelGGL((dequant_kernel<T, D>), grid, dim3(kDequantThreads), 0, s, static_cast<const int8_t*>(k_codes),     \
                      static_cast<const int8_t*>(v_codes), k_scale, v_scale, table, rows, first_or_null,                  \
-                     static_cast<T*>(k_out), static_cast<T*>(v_out), kv_heads, shift)
+                     static_cast<T*>(k_out), static_cast<T*>(v_out), kv_heads, shift, past_caches)
 #define LLMQ_DEQUANT_T(T)                       \
   switch (head_dim) {                           \
     case 64: LLMQ_DEQUANT(T, 64); break;        \
