@@ -1,7 +1,7 @@
 // Writing a cache in blocks (layout: kv_blocks.h), quantized, and reading it back, gfx950.
 //
 //   append   a = max |x| over the call's tokens in a block, for each head
-//            s = max(a / 127, 1e-8) where the call writes the block's first token, else max(s_old, that)
+//            s = max(a (1 / 127), 1e-8) where the call writes the block's first token, else max(s_old, that)
 //            codes of the call's tokens: clamp(rint(x / s)); of the block's earlier tokens: clamp(rint((c s_old) / s))
 //   dequant  T(c s)
 //
@@ -143,7 +143,7 @@ __global__ __launch_bounds__((AppendShape<D, BLOCK>::kThreads)) void append_kern
     for (int w = 0; w < Shape::kThreads / kWave; ++w) amax = fmaxf(amax, s_max[w]);
   }
   if (!active) return;
-  float s = scale_from_amax(amax, 127.0f);
+  float s = fmaxf(amax * (1.0f / 127.0f), kScaleEps);
   if (here.lo > 0) s = fmaxf(s, before);
   const bool grown = here.lo > 0 && s > before && lo > 0;   // and this lane has earlier tokens
   if (in_head == 0) *scale = s;

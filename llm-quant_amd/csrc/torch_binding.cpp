@@ -1472,6 +1472,11 @@ at::Tensor packet_rows(const at::Tensor& t) {
   auto copy = t.contiguous();
   return reinterpret_cast<uintptr_t>(copy.const_data_ptr()) % 16 == 0 ? copy : copy.clone();
 }
+// ... and a vector
+at::Tensor packet_vector(const at::Tensor& t) {
+  const bool dense = (t.size(0) <= 1 || t.stride(0) == 1) && reinterpret_cast<uintptr_t>(t.const_data_ptr()) % 16 == 0;
+  return dense ? t : packet_rows(t.reshape({1, t.size(0)}));
+}
 int64_t row_stride(const at::Tensor& t) { return t.size(0) == 1 ? t.numel() : t.stride(0); }
 
 void check_int(int64_t value, const char* name) {
@@ -1566,8 +1571,7 @@ std::tuple<at::Tensor, at::Tensor> qk_norm_rope(const at::Tensor& q, const at::T
   auto q_out = at::empty({tokens, q_heads, dim}, q.options());
   auto k_out = at::empty({tokens, kv_heads, dim}, q.options());
   const c10::OptionalDeviceGuard guard(at::device_of(q));
-  const auto qr = packet_rows(q), kr = packet_rows(k), qw = packet_rows(q_weight.reshape({1, dim})),
-             kw = packet_rows(k_weight.reshape({1, dim}));
+  const auto qr = packet_rows(q), kr = packet_rows(k), qw = packet_vector(q_weight), kw = packet_vector(k_weight);
   const auto ct = packet_rows(cos.contiguous()), st = packet_rows(sin.contiguous());
   check_rc(llmq_qk_norm_rope(qr.const_data_ptr(), kr.const_data_ptr(), qw.const_data_ptr(), kw.const_data_ptr(),
                              ct.const_data_ptr(), st.const_data_ptr(), at.defined() ? at.const_data_ptr() : nullptr,

@@ -8,6 +8,9 @@ written by the append kernel at a position that lives on the device and read bac
 decode-attention kernel. Nothing about it changes shape or address from step to step, so a
 decode step that uses it can be captured in a HIP graph -- which the reference's
 quantized cache cannot (llmquant/runtime/graph_decode.py:40-43).
+
+BlockQuantCache is the same for a batch of sequences, whose tokens lie in blocks (no counterpart in the reference, which
+runs one sequence at a time).
 """
 
 from __future__ import annotations
@@ -106,6 +109,154 @@ class KernelQuantCache:
         k = self._ext.kv_dequant(self.k_codes[layer], self.k_scale[layer], n_tokens, dtype)
         v = self._ext.kv_dequant(self.v_codes[layer], self.v_scale[layer], n_tokens, dtype)
         return k, v
+
+
+class BlockQuantCache:
+    """K/V codes and scales for every layer of a batch of sequences that come and go, in blocks.
+
+    A block holds `block` consecutive tokens of one sequence under one scale per head (8 bytes a block and head, where
+    KernelQuantCache keeps 8 a token); sequences take blocks as they grow and give them back when they end, so that memory
+    goes by what is cached and not by the longest sequence that might come. The batch has `max_sequences` places. What the
+    kernels read of it lies on the device and keeps its address (a step can be captured in a HIP graph):
+
+    block_table  int32 [max_sequences, blocks of max_len]: a place's blocks in order, -1 where there is none
+    cached       int32 [max_sequences]: tokens a place holds; -1: nobody is in it, and it takes no part
+
+    A step: reserve() the blocks for its tokens, append() and attend() in every layer, advance(). The rows of a call are one
+    for each place, or, with `query_start` (int32 [max_sequences + 1]), rows query_start[b] .. query_start[b + 1] - 1 for
+    place b: drafted tokens, prompts, a prompt's next chunk, single tokens, mixed as they come.
+    """
+
+    def __init__(self, num_layers: int, kv_heads: int, head_dim: int, num_blocks: int, max_sequences: int, max_len: int,
+                 block: int = 64, device="cuda"):
+        if block not in (16, 32, 64, 128):
+            raise ValueError(f"a block holds 16, 32, 64 or 128 tokens, got {block}")
+        if head_dim not in (64, 128, 256):
+            raise ValueError(f"head_dim must be 64, 128 or 256, got {head_dim}")
+        if min(num_layers, kv_heads, num_blocks, max_sequences, max_len) < 1:
+            raise ValueError("layers, heads, blocks, sequences and max_len must be positive")
+        self.num_layers, self.kv_heads, self.head_dim, self.block = num_layers, kv_heads, head_dim, block
+        self.num_blocks, self.max_sequences, self.max_len = num_blocks, max_sequences, max_len
+        width = -(-max_len // block)
+        self.k_codes = torch.zeros(num_layers, num_blocks, kv_heads, block, head_dim, dtype=torch.int8, device=device)
+        self.v_codes = torch.zeros(num_layers, num_blocks, kv_heads, block // 16, head_dim, 16, dtype=torch.int8, device=device)
+        self.k_scale = torch.zeros(num_layers, num_blocks, kv_heads, dtype=torch.float32, device=device)
+        self.v_scale = torch.zeros(num_layers, num_blocks, kv_heads, dtype=torch.float32, device=device)
+        self.block_table = torch.full((max_sequences, width), -1, dtype=torch.int32, device=device)
+        self.cached = torch.full((max_sequences,), -1, dtype=torch.int32, device=device)
+        self._ext = load_extension() if self.cached.is_cuda else None
+        self._free = list(range(num_blocks - 1, -1, -1))
+        self._blocks: list[list[int]] = [[] for _ in range(max_sequences)]
+        self._lengths = [-1] * max_sequences   # as `cached`, on the host
+
+    # ---- bookkeeping (host calls, outside of a captured step) ------------------------------------------
+    def get_seq_length(self, place: int) -> int:
+        """Tokens cached for the sequence in a place."""
+        self._taken(place)
+        return self._lengths[place]
+
+    def free_blocks(self) -> int:
+        return len(self._free)
+
+    def add(self) -> int:
+        """A place for a new sequence, which holds nothing yet."""
+        place = next((i for i, n in enumerate(self._lengths) if n < 0), None)
+        if place is None:
+            raise RuntimeError(f"all {self.max_sequences} places of the batch are taken")
+        self._set_length(place, 0)
+        return place
+
+    def release(self, place: int) -> None:
+        """The sequence in a place ends; its blocks are free again."""
+        self._taken(place)
+        self._free.extend(reversed(self._blocks[place]))
+        self._blocks[place] = []
+        self.block_table[place].fill_(-1)
+        self._set_length(place, -1)
+
+    def truncate(self, place: int, length: int) -> None:
+        """Take back what was cached behind the first `length` tokens (drafted tokens that were not accepted). Blocks stay
+        reserved; a partly kept block keeps its scale."""
+        self._taken(place)
+        if not 0 <= length <= self._lengths[place]:
+            raise ValueError(f"place {place} holds {self._lengths[place]} tokens, cannot be cut to {length}")
+        self._set_length(place, length)
+
+    def reserve(self, new) -> None:
+        """Blocks for `new` more tokens of every sequence: a number, or one for each place (0 for an empty one). Nothing
+        changes if there are not enough."""
+        new = self._per_place(new)
+        wanted = [0 if n < 0 else max(0, -(-(n + more) // self.block) - len(have))
+                  for n, more, have in zip(self._lengths, new, self._blocks)]
+        for place, (n, more) in enumerate(zip(self._lengths, new)):
+            if n >= 0 and n + more > self.max_len:
+                raise ValueError(f"place {place} would hold {n + more} tokens, at most {self.max_len} fit")
+        if sum(wanted) > len(self._free):
+            raise RuntimeError(f"{sum(wanted)} more blocks are needed, {len(self._free)} are free")
+        at: list[tuple[int, int]] = []
+        ids: list[int] = []
+        for place, count in enumerate(wanted):
+            for _ in range(count):
+                at.append((place, len(self._blocks[place])))
+                ids.append(self._free.pop())
+                self._blocks[place].append(ids[-1])
+        if ids:
+            rows, columns = (torch.tensor(i, device=self.block_table.device) for i in zip(*at))
+            self.block_table[rows, columns] = torch.tensor(ids, dtype=torch.int32, device=self.block_table.device)
+
+    def advance(self, new, device: bool = True) -> None:
+        """Count `new` tokens (as for reserve) as cached, behind the last layer of a step. device=False: the host's counts
+        alone, for a step whose captured graph has advanced `cached` itself (advance_device)."""
+        new = self._per_place(new)
+        self._lengths = [n if n < 0 else n + more for n, more in zip(self._lengths, new)]
+        if device:
+            self.cached.copy_(torch.tensor(self._lengths, dtype=torch.int32))
+
+    def advance_device(self, new) -> None:
+        """The device's counts alone, by a number or an int32 tensor [max_sequences]; empty places stay (capturable)."""
+        torch.where(self.cached >= 0, self.cached + new, self.cached, out=self.cached)
+
+    def bytes_per_token(self) -> float:
+        """Codes and scales stored per cached token of full blocks over all layers, K and V."""
+        return 2 * self.num_layers * self.kv_heads * (self.head_dim + 4 / self.block)
+
+    def _taken(self, place: int) -> None:
+        if not 0 <= place < self.max_sequences or self._lengths[place] < 0:
+            raise ValueError(f"nobody is in place {place}")
+
+    def _set_length(self, place: int, length: int) -> None:
+        self._lengths[place] = length
+        self.cached[place] = length
+
+    def _per_place(self, new) -> list[int]:
+        if isinstance(new, int):
+            new = [new if n >= 0 else 0 for n in self._lengths]
+        new = [int(n) for n in new]
+        if len(new) != self.max_sequences or min(new) < 0:
+            raise ValueError(f"one number for each of {self.max_sequences} places, none negative, got {new}")
+        if any(more and n < 0 for n, more in zip(self._lengths, new)):
+            raise ValueError("tokens for a place that nobody is in")
+        return new
+
+    # ---- per-layer operations -----------------------------------------------------------------------
+    def _layer(self, layer: int):
+        return self.k_codes[layer], self.v_codes[layer], self.k_scale[layer], self.v_scale[layer], self.block_table
+
+    def append(self, layer: int, key: torch.Tensor, value: torch.Tensor, query_start: torch.Tensor | None = None) -> None:
+        """key / value: [tokens, kv_heads, head_dim] (rows may be slices of wider ones), written behind what is cached."""
+        self._ext.kv_block_append(key, value, *self._layer(layer), self.cached, query_start)
+
+    def attend(self, layer: int, query: torch.Tensor, scaling: float, query_start: torch.Tensor | None = None) -> torch.Tensor:
+        """query [tokens, q_heads, head_dim] -> [tokens, q_heads * head_dim], causal, over what is cached and the call's own
+        tokens, which append() has written. Rows of empty places are zero."""
+        return self._ext.kv_block_attention(query, *self._layer(layer), self.cached, scaling, query_start)
+
+    def dequantized(self, layer: int, place: int, dtype=torch.bfloat16):
+        """(keys, values) [kv_heads, tokens, head_dim] of the sequence in a place."""
+        tokens = self.get_seq_length(place)
+        starts = torch.zeros(self.max_sequences + 1, dtype=torch.int32, device=self.cached.device)
+        starts[place + 1:] = tokens
+        return self._ext.kv_block_dequant(*self._layer(layer), starts, tokens, dtype)
 
 
 def make_kernel_cache_factory(num_bits, model, max_len: int):

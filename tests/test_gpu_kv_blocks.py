@@ -140,7 +140,7 @@ def append_oracle(x, codes, scale, table, cached, start, block):
                 continue
             lo, hi = max(c, logical * block), min(c + n, (logical + 1) * block)
             rows = x[start[b] + lo - c:start[b] + hi - c].astype(f)       # [new, heads, D]
-            s = np.maximum(np.abs(rows).max((0, 2)) / f(127), f(1e-8))
+            s = np.maximum(np.abs(rows).max((0, 2)) * (f(1) / f(127)), f(1e-8))
             old = lo - logical * block
             if old:
                 before = scale[id].copy()
@@ -202,7 +202,7 @@ def test_append_token_by_token_stays_within_its_steps(ext):
         ext.kv_block_append(rows[t:t + 1], rows[t:t + 1], *cache, table, torch.tensor([t], dtype=torch.int32, device="cuda"))
         grew += cache[2][1].cpu() > before if t else 1
     largest = rows.abs().amax((0, 2)).cpu()
-    assert torch.equal(cache[2][1].cpu(), largest / 127)
+    assert torch.equal(cache[2][1].cpu(), largest * torch.tensor(np.float32(1) / np.float32(127)))
     for codes in (cache[0][1].cpu().double(), torch.from_numpy(rows_first(cache[1][1].cpu().numpy())).double()):
         off = (codes * cache[2][1].cpu()[:, None, None].double() - rows.cpu().double().transpose(0, 1)).abs().amax((1, 2))
         assert torch.all(off <= 0.5 * grew * cache[2][1].cpu().double() * (1 + 1e-5)) and int(grew.max()) < 12
@@ -476,3 +476,185 @@ def test_nothing_to_do(ext):
     q, k = ext.qk_norm_rope(torch.ones(1, 128, device="cuda"), torch.zeros(1, 0, device="cuda"), w, w, t, t, 1e-5,
                             torch.zeros(1, dtype=torch.int32, device="cuda"))
     assert q.isnan().all() and k.shape == (1, 0, 64)   # (a table of no rows knows no position)
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=TAGS.get)
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_attention_of_many_rows_over_long_sequences(ext, dtype, dim):
+    """Rows enough for waves with a row tile each (three and four of them, the last part of one), over tokens enough to be split."""
+    check_attention(ext, dtype, 64, dim, 1, 4, [1990], [29])
+    check_attention(ext, dtype, 16, dim, 1, 3, [1200, -1, 40], [33, 2, 35])
+
+
+def test_attention_of_a_large_batch(ext):
+    """More sequences than the places of several waves, most of them short, some long."""
+    cached = [700 if b % 97 == 5 else -1 if b % 50 == 3 else b % 40 for b in range(450)]
+    check_attention(ext, torch.bfloat16, 16, 64, 1, 2, cached, None)
+    check_attention(ext, torch.float32, 32, 64, 1, 1, cached[:330], [b % 3 for b in range(330)])
+
+
+def test_blocks_far_into_a_large_cache(ext):
+    """Codes beyond 2^31 bytes: the same bits as at the front."""
+    blocks, heads, block, dim = 17000, 8, 128, 128
+    cache = [torch.zeros(blocks, heads, block, dim, dtype=torch.int8, device="cuda"),
+             torch.zeros(blocks, heads, block // 16, dim, 16, dtype=torch.int8, device="cuda"),
+             torch.zeros(blocks, heads, device="cuda"), torch.zeros(blocks, heads, device="cuda")]
+    g = torch.Generator(device="cuda").manual_seed(4)
+    rows = torch.randn(300, heads, dim, generator=g, device="cuda", dtype=torch.bfloat16)
+    q = torch.randn(300, 2 * heads, dim, generator=g, device="cuda", dtype=torch.bfloat16)
+    start = torch.tensor([0, 300], dtype=torch.int32, device="cuda")
+    none = torch.zeros(1, dtype=torch.int32, device="cuda")
+    got = []
+    for table in ([[0, 1, 2]], [[16999, 16500, 16998]]):
+        table = torch.tensor(table, dtype=torch.int32, device="cuda")
+        ext.kv_block_append(rows, rows, *cache, table, none, start)
+        got.append((ext.kv_block_attention(q, *cache, table, none, 0.1, start),
+                    ext.kv_block_attention(q[:1], *cache, table, none + 299, 0.1),
+                    *ext.kv_block_dequant(*cache, table, start, 300, torch.float16)))
+    assert all(torch.equal(a, b) for a, b in zip(*got)) and got[0][0].abs().sum() > 0 and got[0][2].abs().sum() > 0
+
+
+def fresh(cls, **change):
+    return cls(**(dict(num_layers=2, kv_heads=2, head_dim=64, num_blocks=40, max_sequences=3, max_len=400, block=16) | change))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=TAGS.get)
+def test_a_batch_as_it_is_served(ext, dtype):
+    """Prompts, a prompt's second chunk, single tokens, drafts some of which are taken back, a sequence that ends and one that takes
+    its place: norm and rotation, append, attention, reading back, each against its formula on what the others gave."""
+    from llmquant.runtime import BlockQuantCache
+
+    cache, heads, group, dim = fresh(BlockQuantCache), 2, 3, 64
+    g = torch.Generator().manual_seed(11)
+    qw, kw = ((1 + 0.2 * torch.randn(dim, generator=g)).to(dtype).cuda() for _ in range(2))
+    angle = torch.arange(400, dtype=torch.float64)[:, None] * (1000.0 ** (-torch.arange(0, dim, 2, dtype=torch.float64) / dim))
+    cos, sin = (torch.cat([t, t], -1).float().cuda() for t in (angle.cos(), angle.sin()))
+    narrow = dtype != torch.float32
+    codes = [[np.zeros((40, heads, 16, dim), np.int8) for _ in range(2)] for _ in range(2)]
+    scales = [[np.zeros((40, heads), np.float32) for _ in range(2)] for _ in range(2)]
+
+    def step(new):
+        cache.reserve(new)
+        held = [max(cache._lengths[p], 0) if cache._lengths[p] >= 0 else -1 for p in range(3)]
+        start = None if all(n == 1 for n in new) else starts_of(new)
+        offsets = starts_of(new)
+        tokens = int(offsets[-1])
+        position = torch.cat([torch.arange(max(h, 0), max(h, 0) + n) for h, n in zip(held, new)]).to(torch.int32)
+        table = cache.block_table.cpu()
+        for layer in range(2):
+            qkv = torch.randn(tokens, (heads * group + 2 * heads) * dim, generator=g).to(dtype).cuda()
+            k_at, v_at = heads * group * dim, (heads * group + heads) * dim
+            q, k = ext.qk_norm_rope(qkv[:, :k_at], qkv[:, k_at:v_at], qw, kw, cos, sin, 1e-6, position.cuda())
+            want_q, size = norm_rope64(qkv[:, :k_at].double().reshape(tokens, -1, dim), qw.double(), cos[position.long().cuda()].double(),
+                                       sin[position.long().cuda()].double(), 1e-6)
+            assert torch.all((q.double() - want_q).abs() <= half_step(dtype, want_q) + 20 * U32 * size)
+            value = qkv[:, v_at:].unflatten(1, (heads, dim))
+            cache.append(layer, k, value, None if start is None else start.cuda())
+            for x, which in ((k, 0), (value, 1)):
+                append_oracle(x.float().cpu().numpy(), codes[layer][which], scales[layer][which], table.numpy(), held, offsets.numpy(), 16)
+            np.testing.assert_array_equal(cache.k_codes[layer].cpu().numpy(), codes[layer][0])
+            np.testing.assert_array_equal(rows_first(cache.v_codes[layer].cpu().numpy()), codes[layer][1])
+            np.testing.assert_array_equal(cache.k_scale[layer].cpu().numpy(), scales[layer][0])
+            got = cache.attend(layer, q, 0.125, None if start is None else start.cuda())
+            on_cpu = [cache.k_codes[layer].cpu(), cache.v_codes[layer].cpu(), cache.k_scale[layer].cpu(), cache.v_scale[layer].cpu()]
+            want, bound = attention64(q.cpu(), on_cpu, table, held, offsets, 16, 0.125, 1152.0 if narrow else 0.0, 2.0 ** -11 if narrow else 2.0 ** -22)
+            assert torch.all((got.cpu().double().reshape(want.shape) - want).abs() <= half_step(dtype, want) + bound)
+        cache.advance(new)
+
+    cache.add(), cache.add()
+    step([50, 17, 0])
+    step([70, 1, 0])             # the first prompt's second chunk, the second sequence's next token
+    assert cache.add() == 2
+    step([1, 1, 33])
+    step([1, 1, 1])
+    step([5, 4, 1])              # drafts
+    cache.truncate(0, cache.get_seq_length(0) - 3)
+    cache.truncate(1, cache.get_seq_length(1) - 4)
+    step([1, 1, 1])
+    cache.release(1)
+    step([1, 0, 1])
+    assert cache.add() == 1
+    step([1, 40, 1])
+    for place in range(3):
+        k, v = cache.dequantized(1, place, torch.float32)
+        for out, which in ((k, 0), (v, 1)):
+            ids = cache._blocks[place]
+            want = (codes[1][which][ids] * scales[1][which][ids][..., None, None]).transpose(1, 0, 2, 3).reshape(heads, -1, dim)
+            np.testing.assert_array_equal(out.cpu().numpy(), want[:, :cache.get_seq_length(place)])
+
+
+def test_a_captured_step_replays(ext):
+    """A step of two layers in a graph, replayed with eager work of the same program in between: outputs and the whole cache are
+    the eager step's, bit for bit, while sequences grow through blocks and one place is empty."""
+    from llmquant.runtime import BlockQuantCache
+
+    # (max_len: long enough that the tokens are split and merged)
+    eager, graphed = (fresh(BlockQuantCache, max_len=2048, num_blocks=300) for _ in range(2))
+    g = torch.Generator(device="cuda").manual_seed(2)
+    w = torch.ones(64, device="cuda", dtype=torch.float16)
+    angle = torch.arange(2048, device="cuda")[:, None] * (1000.0 ** (-torch.arange(0, 64, 2, device="cuda") / 64))
+    cos, sin = (torch.cat([t, t], -1) for t in (angle.cos(), angle.sin()))
+    static = torch.zeros(3, 8 * 64, device="cuda", dtype=torch.float16)
+
+    def step(cache, rows):
+        outs = []
+        for layer in range(2):
+            q, k = ext.qk_norm_rope(rows[:, :256], rows[:, 256:384], w, w, cos, sin, 1e-6, cache.cached)
+            cache.append(layer, k, rows[:, 384:].unflatten(1, (2, 64)))
+            outs.append(cache.attend(layer, q, 0.125))
+        cache.advance_device(1)
+        return outs
+
+    start = torch.tensor([0, 900, 0 + 900, 1000], dtype=torch.int32, device="cuda")
+    prompt = torch.randn(1000, 2, 64, generator=g, device="cuda", dtype=torch.float16)
+    for cache in (eager, graphed):
+        cache.add(), cache.add(), cache.add(), cache.release(1)
+        cache.reserve([900, 0, 100])
+        for layer in range(2):
+            cache.append(layer, prompt, prompt, start)
+        cache.advance([900, 0, 100])
+        cache.reserve([40, 0, 40])
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):   # (a warm-up, taken back)
+        step(graphed, static)
+    torch.cuda.current_stream().wait_stream(side)
+    for place in (0, 2):
+        graphed.truncate(place, graphed.get_seq_length(place))
+    for a, b in zip((eager.k_codes, eager.v_codes, eager.k_scale, eager.v_scale), (graphed.k_codes, graphed.v_codes, graphed.k_scale, graphed.v_scale)):
+        b.copy_(a)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = step(graphed, static)
+    for turn in range(37):
+        rows = torch.randn(3, 8 * 64, generator=g, device="cuda", dtype=torch.float16) * (1 + 0.1 * turn)
+        want = step(eager, rows)
+        static.copy_(rows)
+        graph.replay()
+        if turn % 3 == 0:
+            torch.cuda.synchronize()
+        for a, b in zip(want, captured):
+            assert torch.equal(a, b) and torch.all(a[1] == 0) and a[0].abs().sum() > 0
+        assert torch.equal(eager.cached, graphed.cached)
+    for a, b in ((eager.k_codes, graphed.k_codes), (eager.v_codes, graphed.v_codes), (eager.k_scale, graphed.k_scale), (eager.v_scale, graphed.v_scale)):
+        assert torch.equal(a, b)
+
+
+def test_two_streams_at_once(ext):
+    """Calls on two streams, each with its workspace, beside each other: the bits of one after the other."""
+    g = torch.Generator().manual_seed(6)
+    sets = []
+    for seed in range(2):
+        cache, table = make_cache(g, 60, 2, 64, 128, outliers=False), make_table(g, [50, 3, 1], 60)
+        sets.append((torch.randn(3, 8, 128, generator=g).bfloat16().cuda(), *[t.cuda() for t in cache], table.cuda(),
+                     torch.tensor([3150, 150, 9 + seed], dtype=torch.int32, device="cuda"), 0.09))
+    want = [ext.kv_block_attention(*s) for s in sets]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in sets]
+    got = [[], []]
+    for _ in range(20):
+        for i, stream in enumerate(streams):
+            with torch.cuda.stream(stream):
+                got[i].append(ext.kv_block_attention(*sets[i]))
+    torch.cuda.synchronize()
+    assert all(torch.equal(w, x) for w, xs in zip(want, got) for x in xs)

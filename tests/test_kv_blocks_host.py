@@ -116,3 +116,64 @@ def test_attention_workspace(lib):
     if need:   # a long sequence of few rows is split, and a workspace that is too small refused
         assert attention(lib, tokens=1, sequences=1, q_heads=32, kv_heads=8, dim=128, block=128, width=1024, q_stride=4096, pointer=16, space=need - 1) == 1
         assert "workspace" in text(lib)
+
+
+# ---- the batch's bookkeeping ------------------------------------------------------------------------------------------
+def make(**change):
+    from llmquant.runtime import BlockQuantCache
+
+    return BlockQuantCache(**(dict(num_layers=2, kv_heads=2, head_dim=64, num_blocks=10, max_sequences=3, max_len=100, block=16, device="cpu") | change))
+
+
+def test_cache_shapes_and_refusals():
+    cache = make(block=64, num_blocks=5)
+    assert cache.k_codes.shape == (2, 5, 2, 64, 64) and cache.v_codes.shape == (2, 5, 2, 4, 64, 16) and cache.k_scale.shape == (2, 5, 2)
+    assert cache.block_table.tolist() == [[-1, -1]] * 3 and cache.cached.tolist() == [-1] * 3
+    assert cache.bytes_per_token() == 2 * 2 * 2 * (64 + 4 / 64)
+    for bad in (dict(block=48), dict(head_dim=96), dict(num_blocks=0), dict(max_len=0)):
+        with pytest.raises(ValueError):
+            make(**bad)
+
+
+def test_sequences_come_grow_and_go():
+    cache = make()
+    a, b = cache.add(), cache.add()
+    assert (a, b) == (0, 1) and cache.cached.tolist() == [0, 0, -1]
+    cache.reserve([33, 16, 0])
+    assert cache.free_blocks() == 6 and [(r >= 0).sum().item() for r in cache.block_table] == [3, 1, 0]
+    cache.advance([33, 16, 0])
+    assert cache.cached.tolist() == [33, 16, -1] and cache.get_seq_length(a) == 33
+    cache.reserve(1)                      # a token each: only the full block's owner needs another
+    assert cache.free_blocks() == 5 and (cache.block_table[1] >= 0).sum() == 2
+    cache.advance(1)
+    c = cache.add()
+    assert c == 2 and cache.cached.tolist() == [34, 17, 0]
+    with pytest.raises(RuntimeError, match="places"):
+        cache.add()
+    used = cache.block_table[cache.block_table >= 0].tolist()
+    assert len(set(used)) == len(used) == 5
+    cache.truncate(a, 20)
+    assert cache.get_seq_length(a) == 20 and cache.cached.tolist() == [20, 17, 0] and cache.free_blocks() == 5
+    cache.reserve([20, 0, 0])             # within what it still has
+    assert cache.free_blocks() == 5
+    cache.release(b)
+    assert cache.cached.tolist() == [20, -1, 0] and cache.free_blocks() == 7 and cache.block_table[1].tolist() == [-1] * 7
+    cache.advance_device(2)
+    assert cache.cached.tolist() == [22, -1, 2]
+    cache.advance(2, device=False)
+    assert cache.get_seq_length(a) == 22 and cache.get_seq_length(c) == 2
+
+
+def test_bookkeeping_refuses_and_changes_nothing():
+    cache = make()
+    a = cache.add()
+    for call, error in ((lambda: cache.reserve([101, 0, 0]), ValueError), (lambda: cache.reserve([1, 1, 0]), ValueError),
+                        (lambda: cache.reserve([-1, 0, 0]), ValueError), (lambda: cache.reserve([1, 0]), ValueError),
+                        (lambda: cache.release(1), ValueError), (lambda: cache.release(3), ValueError), (lambda: cache.truncate(a, 1), ValueError),
+                        (lambda: cache.get_seq_length(2), ValueError), (lambda: cache.advance([0, 0, 1]), ValueError)):
+        with pytest.raises(error):
+            call()
+    b = cache.add()
+    with pytest.raises(RuntimeError, match="11 more blocks are needed, 10 are free"):
+        cache.reserve([100, 50, 0])
+    assert cache.free_blocks() == 10 and cache.block_table.eq(-1).all() and cache.get_seq_length(b) == 0
