@@ -36,7 +36,7 @@ typedef float v2f __attribute__((ext_vector_type(2)));
 constexpr int kWaves = 4, kThreads = kWaves * kWave, kTile = 64;
 constexpr int kHeader = 4;            // floats in front of a partial result: maximum, sum, two of nothing
 constexpr int kMaxSplits = 64;        // of a row: what a wave's lanes hold
-constexpr int kUnits = 1024;          // workgroups that the work is cut for: two rounds of those resident with heads of 128
+constexpr int kUnits = 768;           // workgroups that the work is cut for: a round and a half of those resident with heads of 128
 constexpr int kLeastTiles = 8;        // of a split: two for each wave
 constexpr int kFewSplits = 8;         // .. that a row's wave merges
 constexpr int kMostRecords = 1 << 16; // partial results of a launch (more would cost more than they save)
@@ -220,12 +220,19 @@ template <typename T> __device__ __forceinline__ void store8(T* p, const float* 
 }
 
 // Loads of codes in front of the walk and within it. Of two loads whose results meet at the head of a loop the compiler makes one
-// behind it, which is where they are needed; being of different kinds, these stay where they are asked for.
-struct InWalk {
-  static __device__ __forceinline__ u32x4 load(const void* p) { return load16(p); }
-};
-struct Ahead {
+// behind it, which is where they are needed; being of different kinds, these stay where they are asked for. ONCE: past the caches,
+// where a launch may read more than they hold and a wave what no other one does (streams, the rule below).
+template <bool ONCE> struct InWalk {
   static __device__ __forceinline__ u32x4 load(const void* p) {
+    if constexpr (!ONCE) return load16(p);
+    typedef uint32_t v4u __attribute__((ext_vector_type(4)));
+    const v4u r = __builtin_nontemporal_load(static_cast<const v4u*>(p));
+    return u32x4{r[0], r[1], r[2], r[3]};
+  }
+};
+template <bool ONCE> struct Ahead {
+  static __device__ __forceinline__ u32x4 load(const void* p) {
+    if constexpr (ONCE) return load16(p);
     typedef uint32_t v4u __attribute__((ext_vector_type(4)));
     const v4u r = *static_cast<const v4u*>(p);
     return u32x4{r[0], r[1], r[2], r[3]};
@@ -235,7 +242,7 @@ struct Ahead {
 // waves a SIMD: heads of 256, and fp32 with several row tiles, need more than half of its registers
 template <typename T, int D, int NR> constexpr int kOccupancy = D == 256 || (Pieces<T>::N > 1 && NR * D >= 256) ? 1 : 2;
 
-template <typename T, int D, int NR>
+template <typename T, int D, int NR, bool ONCE>
 __global__ __launch_bounds__(kThreads, (kOccupancy<T, D, NR>)) void attention_kernel(const Problem a) {
   constexpr int kPieces = Pieces<T>::N;
   constexpr bool kExactKeys = kPieces > 1;
@@ -499,9 +506,9 @@ __global__ __launch_bounds__(kThreads, (kOccupancy<T, D, NR>)) void attention_ke
     int v_id = -1;
     if (tile < end) {
       v_id = block_of(now.v, tile * kTile + kStrip * g);
-      load_keys(tile, block_of(now.k, tile * kTile + kStrip * k_strip), Ahead());
+      load_keys(tile, block_of(now.k, tile * kTile + kStrip * k_strip), Ahead<ONCE>());
       load_scales(v_id);
-      load_values(tile, v_id, Ahead());
+      load_values(tile, v_id, Ahead<ONCE>());
     }
     take_queries();
     for (; tile < end; tile += sharing) {
@@ -520,7 +527,7 @@ __global__ __launch_bounds__(kThreads, (kOccupancy<T, D, NR>)) void attention_ke
       }
       __builtin_amdgcn_sched_barrier(0);   // (the phases as they stand: mixed, they take more registers than there are)
       v_id = block_of(next.v, next_tile * kTile + kStrip * g);
-      load_keys(next_tile, block_of(next.k, next_tile * kTile + kStrip * k_strip), InWalk());
+      load_keys(next_tile, block_of(next.k, next_tile * kTile + kStrip * k_strip), InWalk<ONCE>());
       load_scales(v_id);
       next = entries_of(min(tile + 2 * sharing, end - 1));
       __builtin_amdgcn_sched_barrier(0);
@@ -528,7 +535,7 @@ __global__ __launch_bounds__(kThreads, (kOccupancy<T, D, NR>)) void attention_ke
 #pragma unroll
       for (int c = 0; c < kColumns; ++c) add_values(c, operand<true>(v_raw[c].x, v_raw[c].y), operand<true>(v_raw[c].z, v_raw[c].w));
       __builtin_amdgcn_sched_barrier(0);
-      load_values(next_tile, v_id, InWalk());
+      load_values(next_tile, v_id, InWalk<ONCE>());
     }
   } else if constexpr (kTogether) {
     // All waves the same tiles, each with rows of its own: a wave converts a quarter of a tile's codes (keys of sub-tile `wave`,
@@ -564,12 +571,12 @@ __global__ __launch_bounds__(kThreads, (kOccupancy<T, D, NR>)) void attention_ke
     float ks = 0.0f, vs = 0.0f;
     int which = 0;
     if (tile < end) {
-      load_part(tile, now, Ahead(), strip);
+      load_part(tile, now, Ahead<ONCE>(), strip);
       take_queries();
       hand_on(0);
       ks = k_scale;
       vs = v_scale;
-      load_part(min(tile + 1, end - 1), next, Ahead(), next_strip);
+      load_part(min(tile + 1, end - 1), next, Ahead<ONCE>(), next_strip);
       next = entries_of(min(tile + 2, end - 1));
       __syncthreads();
     }
@@ -594,7 +601,7 @@ __global__ __launch_bounds__(kThreads, (kOccupancy<T, D, NR>)) void attention_ke
       ks = k_scale;
       vs = v_scale;
       strip = next_strip;
-      load_part(min(tile + 2, end - 1), next, InWalk(), next_strip);
+      load_part(min(tile + 2, end - 1), next, InWalk<ONCE>(), next_strip);
       next = entries_of(min(tile + 3, end - 1));
       __syncthreads();
     }
@@ -733,19 +740,26 @@ int most_splits(int64_t vectors, int block, int table_width) {
 }
 size_t counts_bytes(int64_t vectors) { return (static_cast<size_t>(vectors) * sizeof(int32_t) + 15) / 16 * 16; }
 
+// Whether codes are read past the caches: more than half of what the 256 MB Infinity Cache holds, by the longest that the
+// sequences can be (their table's width). One row tile a sequence, 131000 tokens of eight heads of 128 (268 MB): 52.6 -> 49.2 us,
+// 48 ragged sequences (308 MB) 68.2 -> 64.0; 16 sequences of 30 MB together 13.4 -> 14.9, one of 4000 tokens 8.9 -> 9.8. Two row
+// tiles, which other waves may read again: 20.4 -> 22.9.
+bool streams(const Problem& a, int D) {
+  return 2.0 * a.rows.sequences * a.table.width * (1 << a.block_shift) * a.heads * D > 128e6;
+}
+
 template <typename T> int launch(const Problem& a, int D, int tiles, int64_t groups, hipStream_t s) {
   const dim3 grid(static_cast<unsigned>(groups * a.heads)), block(kThreads);
-#define LLMQ_ATTEND(DIM, NR) hipLaunchKernelGGL((attention_kernel<T, DIM, NR>), grid, block, 0, s, a)
-  if (D == 64) {
-    if (tiles == 1) LLMQ_ATTEND(64, 1);
-    else LLMQ_ATTEND(64, 2);
-  } else if (D == 128) {
-    if (tiles == 1) LLMQ_ATTEND(128, 1);
-    else LLMQ_ATTEND(128, 2);
-  } else {
-    if (tiles == 1) LLMQ_ATTEND(256, 1);
-    else LLMQ_ATTEND(256, 2);
-  }
+#define LLMQ_ATTEND(DIM)                                                                                           \
+  do {                                                                                                             \
+    if (tiles > 1) hipLaunchKernelGGL((attention_kernel<T, DIM, 2, false>), grid, block, 0, s, a);                  \
+    else if (once) hipLaunchKernelGGL((attention_kernel<T, DIM, 1, true>), grid, block, 0, s, a);                   \
+    else hipLaunchKernelGGL((attention_kernel<T, DIM, 1, false>), grid, block, 0, s, a);                            \
+  } while (0)
+  const bool once = streams(a, D);
+  if (D == 64) LLMQ_ATTEND(64);
+  else if (D == 128) LLMQ_ATTEND(128);
+  else LLMQ_ATTEND(256);
 #undef LLMQ_ATTEND
   if (int rc = llmq_host::check_launch("attention_kernel")) return rc;
   if (a.splits == 1) return 0;

@@ -212,13 +212,13 @@ __global__ __launch_bounds__((AppendShape<D, BLOCK>::kThreads)) void append_kern
 
 constexpr int kDequantThreads = 256;
 
-// The lanes of a block: strips of all its heads, keys and values in workgroups of their own.
+// The lanes of a block: eight tokens each of all its heads, keys and values in workgroups of their own.
 template <typename T, int D>
 __global__ __launch_bounds__(kDequantThreads) void dequant_kernel(
     const int8_t* __restrict__ k_codes, const int8_t* __restrict__ v_codes, const float* __restrict__ k_scale,
     const float* __restrict__ v_scale, const BlockTable table, const Ragged rows, const int32_t* __restrict__ first_or_null,
     T* __restrict__ k_out, T* __restrict__ v_out, const int heads, const int block_shift, const bool past_caches) {
-  const int strips = 1 << (block_shift - 4), lanes = heads * strips * (D / kColumns), sets = (lanes + kDequantThreads - 1) / kDequantThreads;
+  const int strips = 1 << (block_shift - 4), lanes = heads * strips * (kStrip / kTokens) * (D / kColumns), sets = (lanes + kDequantThreads - 1) / kDequantThreads;
   const bool is_value = blockIdx.x & 1;
   const int set = static_cast<int>(blockIdx.x / 2) % sets;
   int piece = blockIdx.x / 2 / sets, from;
@@ -228,42 +228,31 @@ __global__ __launch_bounds__(kDequantThreads) void dequant_kernel(
   if (!touched_block(table, b, span, max(from, 0), piece, block_shift, here)) return;
   const int item = set * kDequantThreads + static_cast<int>(threadIdx.x);
   if (item >= lanes) return;
-  const int d = item % (D / kColumns) * kColumns, strip = item / (D / kColumns) % strips, h = item / (D / kColumns) / strips;
-  const int lo = max(here.lo - kStrip * strip, 0), hi = min(here.hi - kStrip * strip, kStrip);
+  const int groups = strips * (kStrip / kTokens);   // of eight tokens
+  const int d = item % (D / kColumns) * kColumns, slot0 = item / (D / kColumns) % groups * kTokens, h = item / (D / kColumns) / groups;
+  const int lo = max(here.lo - slot0, 0), hi = min(here.hi - slot0, kTokens);
   if (hi <= lo) return;
   const int64_t unit = static_cast<int64_t>(max(here.id, 0)) * heads + h;
-  T* out = (is_value ? v_out : k_out) + (static_cast<int64_t>(h) * rows.rows + here.row + kStrip * strip - here.lo) * D + d;
-  uint32_t words[kStrip][2] = {};   // keys: a token's eight codes; values: [column][half the strip]
+  T* out = (is_value ? v_out : k_out) + (static_cast<int64_t>(h) * rows.rows + here.row + slot0 - here.lo) * D + d;
+  u32x2 words[kTokens] = {};   // keys: a token's eight codes; values: a column's eight
   float s = 0.0f;
   if (here.id >= 0) {
     s = (is_value ? v_scale : k_scale)[unit];
-    if (is_value) {
-      const int8_t* codes = v_codes + ((unit * strips + strip) * D + d) * kStrip;
+    const int8_t* codes = is_value ? v_codes + ((unit * strips + slot0 / kStrip) * D + d) * kStrip + slot0 % kStrip
+                                   : k_codes + ((unit << block_shift) + slot0) * D + d;
+    const int step = is_value ? kStrip : D;
 #pragma unroll
-      for (int e = 0; e < kColumns; ++e) {
-        const u32x4 r = load16(codes + e * kStrip);
-        words[2 * e][0] = r.x;
-        words[2 * e][1] = r.y;
-        words[2 * e + 1][0] = r.z;
-        words[2 * e + 1][1] = r.w;
-      }
-    } else {
-      const int8_t* codes = k_codes + ((unit * strips + strip) * kStrip) * D + d;
-#pragma unroll
-      for (int i = 0; i < kStrip; ++i) {
-        const u32x2 r = *reinterpret_cast<const u32x2*>(codes + i * D);
-        words[i][0] = r.x;
-        words[i][1] = r.y;
-      }
-    }
+    for (int i = 0; i < kTokens; ++i) words[i] = *reinterpret_cast<const u32x2*>(codes + i * step);
   }
 #pragma unroll
-  for (int i = 0; i < kStrip; ++i) {
+  for (int i = 0; i < kTokens; ++i) {
     if (i < lo || i >= hi) continue;
     float f[kColumns];
 #pragma unroll
-    for (int e = 0; e < kColumns; ++e)
-      f[e] = (is_value ? code_of(words[2 * e + i / 8][i / 4 % 2], i % 4) : code_of(words[i][e / 4], e % 4)) * s;
+    for (int e = 0; e < kColumns; ++e) {
+      const uint32_t of_key = e < 4 ? words[i].x : words[i].y, of_value = i < 4 ? words[e].x : words[e].y;
+      f[e] = (is_value ? code_of(of_value, i % 4) : code_of(of_key, e % 4)) * s;
+    }
     T* to = out + static_cast<int64_t>(i) * D;
     if (past_caches) stream8(to, f);
     else store8(to, f);
@@ -361,7 +350,7 @@ extern "C" int llmq_kv_block_dequant(const void* k_codes, const void* v_codes, c
   const Ragged rows{starts, sequences, n_tokens};
   int shift = 4;
   while ((1 << shift) < block) ++shift;
-  const int64_t lanes = static_cast<int64_t>(kv_heads) * (block / kStrip) * (head_dim / kColumns);
+  const int64_t lanes = static_cast<int64_t>(kv_heads) * (block / kTokens) * (head_dim / kColumns);
   const int64_t workgroups = pieces(n_tokens, sequences, block) * 2 * ((lanes + kDequantThreads - 1) / kDequantThreads);
   if (lanes > INT32_MAX - kDequantThreads || workgroups > INT32_MAX)
     return llmq_host::fail_invalid("too many rows, sequences and heads for one launch: %d, %d, %d", n_tokens, sequences, kv_heads);
