@@ -19,12 +19,6 @@ struct BlockTable {
   const int32_t* entries;
   int64_t row_stride;
   int width, blocks;
-  // the block that holds tokens `logical` * block on of sequence b, -1 where there is none
-  __device__ __forceinline__ int at(int b, int logical) const {
-    if (logical < 0 || logical >= width) return -1;
-    const int id = entries[b * row_stride + logical];
-    return id >= 0 && id < blocks ? id : -1;
-  }
 };
 
 // The rows of a sequence.

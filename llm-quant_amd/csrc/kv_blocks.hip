@@ -31,22 +31,23 @@ template <typename T> __device__ __forceinline__ void stream8(T* p, const float*
   for (int i = 0; i < kColumns; i += Pack<T>::N) stream16(p + i, Pack<T>::pack(f + i));
 }
 __device__ __forceinline__ float code_of(uint32_t word, int byte) { return static_cast<float>(static_cast<int8_t>(word >> (8 * byte))); }
-// rint(x / s), clamped, for eight values: the quotient by way of the reciprocal, which is off by less than 2.4e-5 (codes are at most
-// 127.5), and divided where that could make another integer. Eight divisions are some eighty instructions, this is thirty.
-__device__ __forceinline__ void codes_of8(float* f, float s, float inv) {
-  float q[kColumns], far = 0.0f;
-#pragma unroll
-  for (int e = 0; e < kColumns; ++e) {
-    const float r = f[e] * inv;
-    q[e] = rintf(r);
-    far = fmaxf(far, fabsf(r - q[e]));
+// A divisor with its correctly rounded reciprocal: the quotient to the last bit in five instructions. x inv is within an ulp and a half,
+// one correction by its remainder (a multiply-add, exact but for the last rounding) leaves it within an ulp, and a second
+// one is then the rounded quotient (Markstein's theorem). The compiler's division is a dozen instructions and more, in a hundred places. By
+// an infinite scale: 0, or not a number for an infinite x, as divided.
+struct Scale {
+  float by, inv;
+  explicit __device__ __forceinline__ Scale(float s) : by(s < INFINITY ? s : 1.0f), inv(1.0f / s) {}
+  __device__ __forceinline__ float quotient(float x) const {
+    float r = x * inv;
+    r = fmaf(fmaf(-r, by, x), inv, r);
+    return fmaf(fmaf(-r, by, x), inv, r);
   }
-  if (far > 0.49995f) {
+};
+// rint(x / s), clamped, for eight values
+__device__ __forceinline__ void codes_of8(float* f, const Scale& s) {
 #pragma unroll
-    for (int e = 0; e < kColumns; ++e) q[e] = rintf(f[e] / s);
-  }
-#pragma unroll
-  for (int e = 0; e < kColumns; ++e) f[e] = fminf(fmaxf(q[e], -128.0f), 127.0f);
+  for (int e = 0; e < kColumns; ++e) f[e] = fminf(fmaxf(rintf(s.quotient(f[e])), -128.0f), 127.0f);
 }
 __device__ __forceinline__ uint32_t byte_of(float code, int byte) { return (static_cast<uint32_t>(static_cast<int>(code)) & 0xffu) << (8 * byte); }
 
@@ -55,18 +56,18 @@ __device__ __forceinline__ u32x2 bytes_of(const float* f) {
                byte_of(f[4], 0) | byte_of(f[5], 1) | byte_of(f[6], 2) | byte_of(f[7], 3)};
 }
 // eight codes brought to another scale
-__device__ __forceinline__ u32x2 moved8(u32x2 w, float before, float s, float inv) {
+__device__ __forceinline__ u32x2 moved8(u32x2 w, float before, const Scale& s) {
   float f[kColumns];
 #pragma unroll
   for (int e = 0; e < kColumns; ++e) f[e] = code_of(e < 4 ? w.x : w.y, e % 4) * before;
-  codes_of8(f, s, inv);
+  codes_of8(f, s);
   return bytes_of(f);
 }
 
 // The tokens of the call that lie in one block of a sequence.
 struct Touched {
-  int id;          // the block, -1: none
-  int lo, hi;      // its slots lo .. hi - 1
+  int entry;       // of the block table, as it is; -1 beyond it
+  int lo, hi;      // the block's slots lo .. hi - 1
   int64_t row;     // the row of slot lo
 };
 // `from`: the position of the sequence's first row; piece: which of the blocks from there on. False: no row in that block.
@@ -74,7 +75,7 @@ __device__ __forceinline__ bool touched_block(const BlockTable& table, int b, co
                                               Touched& t) {
   const int64_t logical = (from >> block_shift) + piece, at = logical << block_shift;
   if (rows.n == 0 || at > from + rows.n - 1) return false;
-  t.id = logical < table.width ? table.at(b, static_cast<int>(logical)) : -1;
+  t.entry = logical < table.width ? table.entries[b * table.row_stride + logical] : -1;
   t.lo = static_cast<int>(max(from - at, static_cast<int64_t>(0)));
   t.hi = static_cast<int>(min(from + rows.n - at, static_cast<int64_t>(1) << block_shift));
   t.row = rows.first + (at + t.lo - from);
@@ -109,23 +110,27 @@ __global__ __launch_bounds__((AppendShape<D, BLOCK>::kThreads)) void append_kern
     b = rows.find(kShift, cached, piece, span, from);
   }
   Touched here;
-  if (from < 0 || !touched_block(table, b, span, from, piece, kShift, here) || here.id < 0) return;
+  if (from < 0 || !touched_block(table, b, span, from, piece, kShift, here)) return;
   const int h = set * Shape::kHeads + static_cast<int>(threadIdx.x) / Shape::kLanes, in_head = threadIdx.x % Shape::kLanes;
   const int slot0 = in_head / (D / kColumns) * kTokens, d = in_head % (D / kColumns) * kColumns;
   const bool active = h < heads;   // (the others stay for the barrier)
-  const int64_t unit = static_cast<int64_t>(here.id) * heads + min(h, heads - 1);
-  float* scale = (is_value ? v_scale : k_scale) + unit;
-  const float before = *scale;
   // the lane's tokens of the call: lo .. hi - 1 of its eight; the block's earlier ones: below lo
   const int lo = min(max(here.lo - slot0, 0), kTokens), hi = active ? min(max(here.hi - slot0, 0), kTokens) : 0;
   const int64_t stride = is_value ? value_stride : key_stride;
-  const T* x = (is_value ? value : key) + (here.row + slot0 - here.lo) * stride + static_cast<int64_t>(h) * D + d;
+  const T* x = (is_value ? value : key) + here.row * stride + static_cast<int64_t>(min(h, heads - 1)) * D + d;
   constexpr int kPackets = kColumns / Pack<T>::N;
   u32x4 raw[kTokens][kPackets];
 #pragma unroll
-  for (int i = 0; i < kTokens; ++i)
+  for (int i = 0; i < kTokens; ++i) {   // (a slot without a row of the call reads the nearest one that has: no branch around a load)
+    const int64_t at = min(max(slot0 + i, here.lo), here.hi - 1) - here.lo;
 #pragma unroll
-    for (int e = 0; e < kPackets; ++e) raw[i][e] = i >= lo && i < hi ? load16(x + i * stride + e * Pack<T>::N) : u32x4{0u, 0u, 0u, 0u};
+    for (int e = 0; e < kPackets; ++e) raw[i][e] = load16(x + at * stride + e * Pack<T>::N);
+  }
+  // (the rows are asked for beside the block, whose scale is a trip to memory behind the table's)
+  if (here.entry < 0 || here.entry >= table.blocks) return;   // (the workgroup's: one block)
+  const int64_t unit = static_cast<int64_t>(here.entry) * heads + min(h, heads - 1);
+  float* scale = (is_value ? v_scale : k_scale) + unit;
+  const float before = *scale;
   float amax = 0.0f;
 #pragma unroll
   for (int i = 0; i < kTokens; ++i) {
@@ -133,7 +138,7 @@ __global__ __launch_bounds__((AppendShape<D, BLOCK>::kThreads)) void append_kern
 #pragma unroll
     for (int e = 0; e < kPackets; ++e) Pack<T>::unpack(raw[i][e], f + e * Pack<T>::N);
 #pragma unroll
-    for (int e = 0; e < kColumns; ++e) amax = fmaxf(amax, fabsf(f[e]));
+    for (int e = 0; e < kColumns; ++e) amax = fmaxf(amax, fabsf(f[e]));   // (rows that are read twice change no maximum)
   }
   amax = group_max<(Shape::kLanes < kWave ? Shape::kLanes : kWave)>(amax);
   if constexpr (Shape::kThreads > kWave) {
@@ -149,21 +154,25 @@ __global__ __launch_bounds__((AppendShape<D, BLOCK>::kThreads)) void append_kern
   if (in_head == 0) *scale = s;
   if (hi <= lo && !grown) return;   // nothing of this lane's changes
 
-  const float inv = 1.0f / s;
+  const Scale by(s);
   const auto codes_of = [&](int i) {   // the eight codes of token i
     float f[kColumns];
 #pragma unroll
     for (int e = 0; e < kPackets; ++e) Pack<T>::unpack(raw[i][e], f + e * Pack<T>::N);
-    codes_of8(f, s, inv);
+    codes_of8(f, by);
     return bytes_of(f);
   };
   if (!is_value) {
     int8_t* codes = k_codes + (unit * BLOCK + slot0) * D + d;
 #pragma unroll
-    for (int i = 0; i < kTokens; ++i) {
-      u32x2* at = reinterpret_cast<u32x2*>(codes + i * D);
-      if (i >= lo && i < hi) *at = codes_of(i);
-      else if (grown && i < lo) *at = moved8(*at, before, s, inv);
+    for (int i = 0; i < kTokens; ++i)
+      if (i >= lo && i < hi) *reinterpret_cast<u32x2*>(codes + i * D) = codes_of(i);
+    if (grown) {
+#pragma unroll 1   // (rare: short code, since a launch reads it from memory before it runs)
+      for (int i = 0; i < lo; ++i) {
+        u32x2* at = reinterpret_cast<u32x2*>(codes + i * D);
+        *at = moved8(*at, before, by);
+      }
     }
     return;
   }
@@ -178,17 +187,26 @@ __global__ __launch_bounds__((AppendShape<D, BLOCK>::kThreads)) void append_kern
       }
     return;
   }
+  if (grown) {   // the columns' earlier tokens first, the others as they are
+    uint32_t old[2] = {};
+#pragma unroll
+    for (int i = 0; i < kTokens; ++i) old[i / 4] |= i < lo ? 0xffu << (8 * (i % 4)) : 0u;
+#pragma unroll 1
+    for (int e = 0; e < kColumns; ++e) {
+      u32x2* at = reinterpret_cast<u32x2*>(codes + e * kStrip);
+      const u32x2 held = *at, m = moved8(held, before, by);
+      *at = u32x2{(held.x & ~old[0]) | (m.x & old[0]), (held.y & ~old[1]) | (m.y & old[1])};
+    }
+    if (hi <= lo) return;
+  }
   // columns of eight tokens, out of tokens of eight columns
   u32x2 tokens[kTokens];
 #pragma unroll
   for (int i = 0; i < kTokens; ++i) tokens[i] = codes_of(i);
-  // bytes of other tokens among them stay, or move to the new scale
-  uint32_t fresh[2] = {}, old[2] = {};
+  // bytes of other tokens among them stay
+  uint32_t fresh[2] = {};
 #pragma unroll
-  for (int i = 0; i < kTokens; ++i) {
-    fresh[i / 4] |= i >= lo && i < hi ? 0xffu << (8 * (i % 4)) : 0u;
-    old[i / 4] |= grown && i < lo ? 0xffu << (8 * (i % 4)) : 0u;
-  }
+  for (int i = 0; i < kTokens; ++i) fresh[i / 4] |= i >= lo && i < hi ? 0xffu << (8 * (i % 4)) : 0u;
 #pragma unroll
   for (int e = 0; e < kColumns; ++e) {
     u32x2 column{0u, 0u};
@@ -199,11 +217,7 @@ __global__ __launch_bounds__((AppendShape<D, BLOCK>::kThreads)) void append_kern
     }
     u32x2* at = reinterpret_cast<u32x2*>(codes + e * kStrip);
     if (lo > 0 || hi < kTokens) {
-      u32x2 held = *at;
-      if (grown) {
-        const u32x2 m = moved8(held, before, s, inv);
-        held = u32x2{(held.x & ~old[0]) | (m.x & old[0]), (held.y & ~old[1]) | (m.y & old[1])};
-      }
+      const u32x2 held = *at;
       column = u32x2{(held.x & ~fresh[0]) | (column.x & fresh[0]), (held.y & ~fresh[1]) | (column.y & fresh[1])};
     }
     *at = column;
@@ -232,11 +246,12 @@ __global__ __launch_bounds__(kDequantThreads) void dequant_kernel(
   const int d = item % (D / kColumns) * kColumns, slot0 = item / (D / kColumns) % groups * kTokens, h = item / (D / kColumns) / groups;
   const int lo = max(here.lo - slot0, 0), hi = min(here.hi - slot0, kTokens);
   if (hi <= lo) return;
-  const int64_t unit = static_cast<int64_t>(max(here.id, 0)) * heads + h;
+  const bool held = here.entry >= 0 && here.entry < table.blocks;
+  const int64_t unit = static_cast<int64_t>(held ? here.entry : 0) * heads + h;
   T* out = (is_value ? v_out : k_out) + (static_cast<int64_t>(h) * rows.rows + here.row + slot0 - here.lo) * D + d;
   u32x2 words[kTokens] = {};   // keys: a token's eight codes; values: a column's eight
   float s = 0.0f;
-  if (here.id >= 0) {
+  if (held) {
     s = (is_value ? v_scale : k_scale)[unit];
     const int8_t* codes = is_value ? v_codes + ((unit * strips + slot0 / kStrip) * D + d) * kStrip + slot0 % kStrip
                                    : k_codes + ((unit << block_shift) + slot0) * D + d;
