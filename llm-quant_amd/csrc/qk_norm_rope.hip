@@ -5,6 +5,9 @@
 //   z_i = y_i                                                       for i >= R
 //
 // in fp32, rounded once, where it is stored. cos and sin are row positions[t] of the tables (row t without positions).
+//
+// Bound: HBM, each element read and written once; for a few tokens one trip to memory and the launch. By trace, heads of 128: 4100
+// tokens of 40 heads, bf16 15.9 us (5.6 TB/s), 77 tokens of 32 heads 4.0, one token 2.8.
 #include <cmath>
 
 #include "llmq_device.h"
