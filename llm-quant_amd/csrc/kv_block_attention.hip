@@ -727,7 +727,7 @@ __global__ __launch_bounds__(kThreads) void merge_kernel(const Problem a) {
   }
 }
 
-// rows that a wave takes, in 16ths: what an average sequence has
+// Row tiles of 16 that a wave takes: one where an average sequence has no more (its waves then share tokens), else two.
 int row_tiles(int64_t rows, int sequences, int group) {
   const int64_t average = rows * group / sequences;
   return average <= 16 ? 1 : 2;
