@@ -41,6 +41,8 @@ struct Ragged {
   __device__ __forceinline__ int find(int block_shift, const int32_t* more, int& slot, Span& span, int& other) const {
     const int lane = threadIdx.x & (kWave - 1);
     int b = 0, number = 0;
+    span = Span{0, 0};   // (a piece in front of the first sequence's rows is nobody's)
+    other = 0;
     for (int b0 = 0; b0 < sequences; b0 += kWave) {
       const int at = min(b0 + lane, sequences - 1);
       int from = at, to = at + 1;
@@ -60,6 +62,7 @@ struct Ragged {
       if (below < kWave) break;
     }
     slot -= number;
+    if (slot < 0) span.n = 0;   // (starts that decrease, against the contract: no piece in front of the sequence's first)
     return b;
   }
 };

@@ -103,7 +103,7 @@ __global__ __launch_bounds__((AppendShape<D, BLOCK>::kThreads)) void append_kern
   const int sets = (heads + Shape::kHeads - 1) / Shape::kHeads;   // of heads
   const bool is_value = blockIdx.x & 1;
   const int set = static_cast<int>(blockIdx.x / 2) % sets;
-  int piece = blockIdx.x / 2 / sets, b = piece, from;
+  int piece = blockIdx.x / 2 / sets, b = piece, from = 0;
   Span span{b, 1};
   if (rows.start == nullptr) {
     from = cached[b];
@@ -237,7 +237,7 @@ __global__ __launch_bounds__(kDequantThreads) void dequant_kernel(
   const int strips = 1 << (block_shift - 4), lanes = heads * strips * (kStrip / kTokens) * (D / kColumns), sets = (lanes + kDequantThreads - 1) / kDequantThreads;
   const bool is_value = blockIdx.x & 1;
   const int set = static_cast<int>(blockIdx.x / 2) % sets;
-  int piece = blockIdx.x / 2 / sets, from;
+  int piece = blockIdx.x / 2 / sets, from = 0;
   Span span{0, 0};
   const int b = rows.find(block_shift, first_or_null, piece, span, from);
   Touched here;

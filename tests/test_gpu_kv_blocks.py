@@ -658,3 +658,35 @@ def test_two_streams_at_once(ext):
                 got[i].append(ext.kv_block_attention(*sets[i]))
     torch.cuda.synchronize()
     assert all(torch.equal(w, x) for w, xs in zip(want, got) for x in xs)
+
+
+@pytest.mark.parametrize("block,in_front", [(16, 15), (16, 16), (16, 100), (64, 300), (128, 128)])
+def test_rows_in_front_of_the_first_sequence_are_nobodys(ext, block, in_front):
+    g = torch.Generator().manual_seed(17)
+    dim, heads, cached, new = 64, 2, [3, 40, -1, 0], [20, 1, 5, 33]
+    counts = [-(-max(c + n, 1) // block) for c, n in zip(cached, new)]
+    cache = make_cache(g, sum(counts) + 2, heads, block, dim, outliers=False)
+    table, start = make_table(g, counts, sum(counts) + 2), in_front + starts_of(new)
+    rows = torch.randn(in_front + sum(new) + 9, heads, dim, generator=g)
+    rows[:in_front] = rows[in_front + sum(new):] = 1e4   # (would raise every scale)
+    want, want_scale = cache[0].numpy().copy(), cache[2].numpy().copy()
+    append_oracle(rows.numpy(), want, want_scale, table.numpy(), cached, start.numpy(), block)
+    want_v, want_v_scale = rows_first(cache[1].numpy()).copy(), cache[3].numpy().copy()
+    append_oracle(rows.numpy(), want_v, want_v_scale, table.numpy(), cached, start.numpy(), block)
+    on_gpu = [t.cuda() for t in cache]
+    lengths = torch.tensor(cached, dtype=torch.int32, device="cuda")
+    ext.kv_block_append(rows.cuda(), rows.cuda(), *on_gpu, table.cuda(), lengths, start.cuda())
+    np.testing.assert_array_equal(on_gpu[0].cpu().numpy(), want)
+    np.testing.assert_array_equal(rows_first(on_gpu[1].cpu().numpy()), want_v)
+    np.testing.assert_array_equal(on_gpu[2].cpu().numpy(), want_scale)
+    np.testing.assert_array_equal(on_gpu[3].cpu().numpy(), want_v_scale)
+    # read back, and attended to: as with the rows from 0 on
+    shifted, plain = start.cuda(), starts_of(new).cuda()
+    total = in_front + sum(new)
+    for a, b in zip(ext.kv_block_dequant(*on_gpu, table.cuda(), shifted, total, torch.float32), ext.kv_block_dequant(*on_gpu, table.cuda(), plain, sum(new), torch.float32)):
+        assert torch.equal(a[:, in_front:], b)
+    query = torch.randn(total, 4, dim, generator=g).cuda()
+    out = torch.full((total, 4 * dim), 7.5, device="cuda")
+    ext.kv_block_attention(query, *on_gpu, table.cuda(), lengths, dim ** -0.5, shifted, out)
+    assert torch.all(out[:in_front] == 7.5)
+    assert torch.equal(out[in_front:], ext.kv_block_attention(query[in_front:], *on_gpu, table.cuda(), lengths, dim ** -0.5, plain))
