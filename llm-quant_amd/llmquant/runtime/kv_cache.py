@@ -208,6 +208,9 @@ class BlockQuantCache:
         """Count `new` tokens (as for reserve) as cached, behind the last layer of a step. device=False: the host's counts
         alone, for a step whose captured graph has advanced `cached` itself (advance_device)."""
         new = self._per_place(new)
+        for place, (n, more, have) in enumerate(zip(self._lengths, new, self._blocks)):
+            if device and n + more > len(have) * self.block:   # (else the device has counted them already)
+                raise ValueError(f"place {place} would hold {n + more} tokens, blocks for {len(have) * self.block} are reserved")
         self._lengths = [n if n < 0 else n + more for n, more in zip(self._lengths, new)]
         if device:
             self.cached.copy_(torch.tensor(self._lengths, dtype=torch.int32))

@@ -177,3 +177,14 @@ def test_bookkeeping_refuses_and_changes_nothing():
     with pytest.raises(RuntimeError, match="11 more blocks are needed, 10 are free"):
         cache.reserve([100, 50, 0])
     assert cache.free_blocks() == 10 and cache.block_table.eq(-1).all() and cache.get_seq_length(b) == 0
+
+
+def test_advance_refuses_tokens_without_blocks():
+    cache = make()
+    a = cache.add()
+    cache.reserve([17, 0, 0])             # two blocks
+    with pytest.raises(ValueError, match="would hold 33 tokens, blocks for 32 are reserved"):
+        cache.advance([33, 0, 0])
+    assert cache.get_seq_length(a) == 0 and cache.cached.tolist() == [0, -1, -1]
+    cache.advance(32)
+    assert cache.get_seq_length(a) == 32
