@@ -574,7 +574,7 @@ int llmq_kv_block_dequant(const void* k_codes, const void* v_codes, const float*
  * q [tokens, q_heads, head_dim] (row stride in elements), out [tokens, q_heads * head_dim]. Tokens without a block are left
  * out; a row that sees nothing (a sequence that takes no part among them) is zero; rows that no sequence has are not
  * written. workspace: llmq_kv_block_attention_workspace_bytes(...) bytes, 16-byte aligned (NULL where that is 0), needs no
- * clearing; calls that overlap in time need one each. */
+ * clearing; calls that overlap in time need one each. out shares no memory with the inputs. */
 size_t llmq_kv_block_attention_workspace_bytes(int tokens, int sequences, int q_heads, int kv_heads, int head_dim, int block,
                                                int table_width);
 int llmq_kv_block_attention(const void* query, int64_t q_row_stride, const void* k_codes, const void* v_codes,

@@ -9,6 +9,7 @@
 // No kernel lives here and nothing here synchronises, so every op stays graph-capturable.
 #include <torch/extension.h>
 
+#include <ATen/MemoryOverlap.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <hipblaslt/hipblaslt.h>
@@ -1651,6 +1652,11 @@ at::Tensor kv_block_attention(const at::Tensor& query, const at::Tensor& k_codes
                     out->dim() == 2 && out->size(0) == tokens && out->size(1) == q_heads * c.dim &&
                     reinterpret_cast<uintptr_t>(out->const_data_ptr()) % 16 == 0,
                 "out must be contiguous [", tokens, ", ", q_heads * c.dim, "] of query's dtype, 16-byte aligned");
+    const auto overlaps = [&](const at::Tensor& t) {
+      const auto status = at::get_overlap_status(*out, t);
+      return status == at::MemOverlapStatus::Full || status == at::MemOverlapStatus::Partial;
+    };
+    TORCH_CHECK(!overlaps(query) && !overlaps(k_codes) && !overlaps(v_codes), "out must not share memory with query or the cache");
     result = *out;
   } else {
     result = at::empty({tokens, q_heads * c.dim}, query.options());

@@ -690,3 +690,36 @@ def test_rows_in_front_of_the_first_sequence_are_nobodys(ext, block, in_front):
     ext.kv_block_attention(query, *on_gpu, table.cuda(), lengths, dim ** -0.5, shifted, out)
     assert torch.all(out[:in_front] == 7.5)
     assert torch.equal(out[in_front:], ext.kv_block_attention(query[in_front:], *on_gpu, table.cuda(), lengths, dim ** -0.5, plain))
+
+
+def test_out_may_not_share_memory(ext):
+    cache = [t.cuda() for t in make_cache(torch.Generator().manual_seed(0), 2, 2, 16, 64)]
+    table, cached = torch.zeros(2, 1, dtype=torch.int32, device="cuda"), torch.zeros(2, dtype=torch.int32, device="cuda")
+    room = torch.zeros(4, 4, 64, device="cuda")
+    for out in (room[:2].view(2, 256), room[1:3].view(2, 256)):   # the query's memory, and one row of it
+        with pytest.raises(RuntimeError, match="out must not share memory"):
+            ext.kv_block_attention(room[:2], *cache, table, cached, 1.0, None, out)
+    beside = room[2:].view(2, 256)
+    assert ext.kv_block_attention(room[:2], *cache, table, cached, 1.0, None, beside).data_ptr() == beside.data_ptr()
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=TAGS.get)
+def test_blocks_shared_for_reading(ext, dtype):
+    g = torch.Generator().manual_seed(23)
+    block, dim, heads, n = 32, 128, 2, 40
+    cache = [t.cuda() for t in make_cache(g, n, heads, block, dim, outliers=False)]
+    query = torch.randn(3, 8, dim, generator=g).to(dtype).cuda()
+    lengths = torch.tensor([32 * 36 - 1, 700, 32 * 20], dtype=torch.int32, device="cuda")
+    prefix = torch.randperm(n, generator=g)[:36].to(torch.int32)
+    prefix[5] = prefix[9]   # the same block twice in a sequence
+    one = prefix[None].cuda()
+    attend = lambda q, t, c: ext.kv_block_attention(q, *cache, t, c, dim ** -0.5)
+    got = attend(query, one.expand(3, -1), lengths)                     # one row of a table for all
+    assert torch.equal(got, attend(query, one.repeat(3, 1), lengths))
+    # .. and as from copies of the blocks, each sequence its own
+    copies = [t[one.repeat(3, 1).flatten().long()].contiguous() for t in cache]
+    own = torch.arange(3 * 36, dtype=torch.int32, device="cuda").view(3, 36)
+    assert torch.equal(got, ext.kv_block_attention(query, *copies, own, lengths, dim ** -0.5))
+    starts = torch.tensor([0, 100, 150, 151], dtype=torch.int32, device="cuda")
+    for a, b in zip(ext.kv_block_dequant(*cache, one.expand(3, -1), starts, 151, dtype), ext.kv_block_dequant(*copies, own, starts, 151, dtype)):
+        assert torch.equal(a, b)
