@@ -746,12 +746,15 @@ int most_splits(int64_t vectors, int block, int table_width) {
 }
 size_t counts_bytes(int64_t vectors) { return (static_cast<size_t>(vectors) * sizeof(int32_t) + 15) / 16 * 16; }
 
-// Whether codes are read past the caches: more than half of what the 256 MB Infinity Cache holds, by the longest that the
-// sequences can be (their table's width). One row tile a sequence, 131000 tokens of eight heads of 128 (268 MB): 52.6 -> 49.2 us,
-// 48 ragged sequences (308 MB) 68.2 -> 64.0; 16 sequences of 30 MB together 13.4 -> 14.9, one of 4000 tokens 8.9 -> 9.8. Two row
-// tiles, which other waves may read again: 20.4 -> 22.9.
+// Whether codes are read past the caches, by the bytes of the longest that the sequences can be (their table's width), against the
+// 256 MB Infinity Cache; one row tile a wave. Long sequences: 131000 tokens of eight heads of 128 51.8 -> 49.9 us, 400000
+// 143 -> 133, two of 200000 together 78.5 -> 73.8, but one of 65000 30.6 -> 30.9. A batch's lengths differ and it holds about half of its bound: 48 sequences of 308 MB
+// together 65.8 -> 64.0, 614 MB 115 -> 113, but 205 MB 46.8 -> 50.1, 102 MB 31.5 -> 34.2. Heads of 64, whose requests are the
+// smallest, gain earlier: 64 sequences of 154 MB 37.1 -> 34.2. Heads of 256 do not: 48 sequences of 307 MB 78.6 -> 85.0, 205 MB 61 -> 67.
+// Two row tiles, which other waves may read again: 20.4 -> 22.9.
 bool streams(const Problem& a, int D) {
-  return 2.0 * a.rows.sequences * a.table.width * (1 << a.block_shift) * a.heads * D > 128e6;
+  const double bytes = 2.0 * a.rows.sequences * a.table.width * (1 << a.block_shift) * a.heads * D;
+  return D != 256 && bytes > (D == 64 ? 128e6 : std::min(128e6 * a.rows.sequences, 512e6));
 }
 
 template <typename T> int launch(const Problem& a, int D, int tiles, int64_t groups, hipStream_t s) {
@@ -759,7 +762,7 @@ template <typename T> int launch(const Problem& a, int D, int tiles, int64_t gro
 #define LLMQ_ATTEND(DIM)                                                                                           \
   do {                                                                                                             \
     if (tiles > 1) hipLaunchKernelGGL((attention_kernel<T, DIM, 2, false>), grid, block, 0, s, a);                  \
-    else if (once) hipLaunchKernelGGL((attention_kernel<T, DIM, 1, true>), grid, block, 0, s, a);                   \
+    else if (once) hipLaunchKernelGGL((attention_kernel<T, DIM, 1, (DIM < 256)>), grid, block, 0, s, a);            \
     else hipLaunchKernelGGL((attention_kernel<T, DIM, 1, false>), grid, block, 0, s, a);                            \
   } while (0)
   const bool once = streams(a, D);
