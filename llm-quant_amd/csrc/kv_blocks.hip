@@ -8,7 +8,7 @@
 // A lane takes eight columns of eight tokens: a packet of 16-bit values for each token, eight bytes of each token's key codes,
 // eight bytes of each column's value codes (16 tokens innermost), so that the transposition of the values is a choice of bytes within a
 // lane. Bound: HBM, each tensor read once and written once (40000 tokens
-// of eight heads of 128 read back, bf16: 38.5 us by trace, 6.4 TB/s); at few tokens the chain starts and lengths -> table -> scales and
+// of eight heads of 128 read back, bf16: 46.6 us by trace, 5.3 TB/s); at few tokens the chain starts and lengths -> table -> scales and
 // codes, a trip to memory each (600 tokens read 4.6 us, a step of 64 rows written 4.7), and for prompts the length of append's
 // program besides, which few waves run (6011 tokens of eight heads of 64: 9.6).
 #include "kv_blocks.h"
@@ -26,11 +26,6 @@ template <typename T> __device__ __forceinline__ void load8(const T* p, float* f
 template <typename T> __device__ __forceinline__ void store8(T* p, const float* f) {
 #pragma unroll
   for (int i = 0; i < kColumns; i += Pack<T>::N) store16(p + i, Pack<T>::pack(f + i));
-}
-// (past the caches)
-template <typename T> __device__ __forceinline__ void stream8(T* p, const float* f) {
-#pragma unroll
-  for (int i = 0; i < kColumns; i += Pack<T>::N) stream16(p + i, Pack<T>::pack(f + i));
 }
 __device__ __forceinline__ float code_of(uint32_t word, int byte) { return static_cast<float>(static_cast<int8_t>(word >> (8 * byte))); }
 // A divisor with its correctly rounded reciprocal: the quotient to the last bit in five instructions. x inv is within an ulp and a half,
@@ -233,7 +228,7 @@ template <typename T, int D>
 __global__ __launch_bounds__(kDequantThreads) void dequant_kernel(
     const int8_t* __restrict__ k_codes, const int8_t* __restrict__ v_codes, const float* __restrict__ k_scale,
     const float* __restrict__ v_scale, const BlockTable table, const Ragged rows, const int32_t* __restrict__ first_or_null,
-    T* __restrict__ k_out, T* __restrict__ v_out, const int heads, const int block_shift, const bool past_caches) {
+    T* __restrict__ k_out, T* __restrict__ v_out, const int heads, const int block_shift) {
   const int strips = 1 << (block_shift - 4), lanes = heads * strips * (kStrip / kTokens) * (D / kColumns), sets = (lanes + kDequantThreads - 1) / kDequantThreads;
   const bool is_value = blockIdx.x & 1;
   const int set = static_cast<int>(blockIdx.x / 2) % sets;
@@ -271,8 +266,7 @@ __global__ __launch_bounds__(kDequantThreads) void dequant_kernel(
       f[e] = (is_value ? code_of(of_value, i % 4) : code_of(of_key, e % 4)) * s;
     }
     T* to = out + static_cast<int64_t>(i) * D;
-    if (past_caches) stream8(to, f);
-    else store8(to, f);
+    store8(to, f);
   }
 }
 
@@ -371,15 +365,14 @@ extern "C" int llmq_kv_block_dequant(const void* k_codes, const void* v_codes, c
   const int64_t workgroups = pieces(n_tokens, sequences, block) * 2 * ((lanes + kDequantThreads - 1) / kDequantThreads);
   if (lanes > INT32_MAX - kDequantThreads || workgroups > INT32_MAX)
     return llmq_host::fail_invalid("too many rows, sequences and heads for one launch: %d, %d, %d", n_tokens, sequences, kv_heads);
-  // What is larger than the L2 caches (eight of 4 MB) leaves them before it is read: written past them it does not push the codes
-  // out either. 40000 tokens of eight heads of 128, bf16: 54.8 -> 39.7 us (6.2 TB/s).
-  const bool past_caches = 2.0 * n_tokens * kv_heads * head_dim * (dtype == LLMQ_F32 ? 4 : 2) > 32e6;
+  // (the output through the caches: past them 40000 tokens of eight heads of 128 alone take 38 us instead of 56, but with an operator that
+  // reads it behind 94 instead of 84, 20000 tokens 53 instead of 48)
   const dim3 grid(static_cast<unsigned>(workgroups));
   hipStream_t s = static_cast<hipStream_t>(stream);
 #define LLMQ_DEQUANT(T, D)                                                                                               \
   hipLaunchKernelGGL((dequant_kernel<T, D>), grid, dim3(kDequantThreads), 0, s, static_cast<const int8_t*>(k_codes),     \
                      static_cast<const int8_t*>(v_codes), k_scale, v_scale, table, rows, first_or_null,                  \
-                     static_cast<T*>(k_out), static_cast<T*>(v_out), kv_heads, shift, past_caches)
+                     static_cast<T*>(k_out), static_cast<T*>(v_out), kv_heads, shift)
 #define LLMQ_DEQUANT_T(T)                       \
   switch (head_dim) {                           \
     case 64: LLMQ_DEQUANT(T, 64); break;        \

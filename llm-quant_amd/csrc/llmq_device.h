@@ -66,11 +66,6 @@ __device__ __forceinline__ u32x4 load16(const void* p) {
   return *reinterpret_cast<const u32x4*>(p);
 }
 __device__ __forceinline__ void store16(void* p, u32x4 v) { *reinterpret_cast<u32x4*>(p) = v; }
-// store16 past the caches: for what is larger than they are, and not read again soon
-__device__ __forceinline__ void stream16(void* p, u32x4 v) {
-  typedef uint32_t v4u __attribute__((ext_vector_type(4)));
-  __builtin_nontemporal_store(v4u{v.x, v.y, v.z, v.w}, static_cast<v4u*>(p));
-}
 
 // A 16-byte packet of T, unpacked to fp32 and back.
 template <typename T> struct Pack;

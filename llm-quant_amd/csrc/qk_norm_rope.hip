@@ -7,7 +7,7 @@
 // in fp32, rounded once, where it is stored. cos and sin are row positions[t] of the tables (row t without positions).
 //
 // Bound: HBM, each element read and written once; for a few tokens one trip to memory and the launch. By trace, heads of 128: 4100
-// tokens of 40 heads, bf16 15.9 us (5.6 TB/s), 77 tokens of 32 heads 4.0, one token 2.8.
+// tokens of 40 heads, bf16 17.9 us (4.9 TB/s; back to back 17.2), 77 tokens of 32 heads 4.0, one token 2.8.
 #include <cmath>
 
 #include "llmq_device.h"
@@ -47,7 +47,7 @@ __global__ __launch_bounds__(kThreads) void qk_norm_rope_kernel(
     const T* __restrict__ q_weight, const T* __restrict__ k_weight, const TABLE* __restrict__ cos_table,
     const TABLE* __restrict__ sin_table, const void* __restrict__ positions, const bool wide_positions,
     T* __restrict__ q_out, T* __restrict__ k_out, const uint32_t vectors, const uint32_t q_heads, const uint32_t kv_heads,
-    const uint32_t step, const int D, const int R, const int table_rows, const float eps, const bool past_caches) {
+    const uint32_t step, const int D, const int R, const int table_rows, const float eps) {
   constexpr int V = Pack<T>::N;
   const uint32_t item = blockIdx.x * kThreads + threadIdx.x, vector = item / LANES;   // (below 2^31: the host's rule)
   if (vector >= vectors) return;   // a head's lanes leave together
@@ -115,13 +115,8 @@ __global__ __launch_bounds__(kThreads) void qk_norm_rope_kernel(
       b[e] = rotated ? fmaf(y1, c1[e], y0 * s1[e]) : y1;
     }
     T* out = is_k ? k_out + (static_cast<int64_t>(t) * kv_heads + (h - q_heads)) * D : q_out + (static_cast<int64_t>(t) * q_heads + h) * D;
-    if (past_caches) {
-      stream16(out + at0, Pack<T>::pack(a));
-      stream16(out + at1, Pack<T>::pack(b));
-    } else {
-      store16(out + at0, Pack<T>::pack(a));
-      store16(out + at1, Pack<T>::pack(b));
-    }
+    store16(out + at0, Pack<T>::pack(a));
+    store16(out + at1, Pack<T>::pack(b));
   }
 }
 
@@ -163,8 +158,8 @@ extern "C" int llmq_qk_norm_rope(const void* q, const void* k, const void* q_wei
   const int step = many ? (heads + kPasses - 1) / kPasses : heads;
   const int64_t vectors = static_cast<int64_t>(tokens) * step, items = vectors * lanes;
   if (items > INT32_MAX - kThreads) return llmq_host::fail_invalid("too many heads for one launch: %lld", static_cast<long long>(vectors));
-  // what is larger than the L2 caches (eight of 4 MB) is written past them: 4100 tokens of 40 heads of 128 17.8 -> 16.6 us
-  const bool past_caches = 2.0 * vectors / step * heads * head_dim * (dtype == LLMQ_F32 ? 2 : 1) > 32e6;
+  // (the outputs through the caches: past them 16000 tokens of 40 heads alone take 61 us instead of 65, but with an operator that reads the
+  // queries behind 111 instead of 105)
   const dim3 grid(static_cast<unsigned>((items + kThreads - 1) / kThreads));
   hipStream_t s = static_cast<hipStream_t>(stream);
 #define LLMQ_NORM_P(T, TABLE, L, P)                                                                                          \
@@ -173,7 +168,7 @@ extern "C" int llmq_qk_norm_rope(const void* q, const void* k, const void* q_wei
                      static_cast<const T*>(k_weight), static_cast<const TABLE*>(cos_table),                                  \
                      static_cast<const TABLE*>(sin_table), positions_or_null, position_bytes == 8, static_cast<T*>(q_out),   \
                      static_cast<T*>(k_out), static_cast<uint32_t>(vectors), static_cast<uint32_t>(q_heads),                 \
-                     static_cast<uint32_t>(kv_heads), static_cast<uint32_t>(step), head_dim, rotary_dim, table_rows, eps, past_caches)
+                     static_cast<uint32_t>(kv_heads), static_cast<uint32_t>(step), head_dim, rotary_dim, table_rows, eps)
 #define LLMQ_NORM(T, TABLE, L)                     \
   do {                                             \
     if (many) LLMQ_NORM_P(T, TABLE, L, kPasses);   \
