@@ -554,6 +554,8 @@ int llmq_qk_norm_rope(const void* q, const void* k, const void* q_weight, const 
  *   scale = max(a * (1 / 127), 1e-8) (the reciprocal rounded to fp32) where the call writes the block's first token,
  *           else max(scale, that)
  *   code = clamp(rint(x / scale), -128, 127); codes the block held before: clamp(rint((code * old scale) / scale))
+ * A NaN or an infinity among the values makes their block's scale NaN in that head: all of its tokens read as NaN there (what they
+ * held is lost) until a call writes the block's first token again.
  * Tokens whose position has no block are left out; places behind a sequence's last token keep what they hold.
  *
  * llmq_kv_block_dequant reads tokens first[b] .. of sequence b (first NULL: 0) into columns starts[b] .. starts[b + 1] - 1

@@ -1,7 +1,8 @@
 // Writing a cache in blocks (layout: kv_blocks.h), quantized, and reading it back, gfx950.
 //
 //   append   a = max |x| over the call's tokens in a block, for each head
-//            s = max(a (1 / 127), 1e-8) where the call writes the block's first token, else max(s_old, that)
+//            s = max(a (1 / 127), 1e-8) where the call writes the block's first token, else max(s_old, that);
+//                not a number where an x is not finite, so that c s is not a number for any token of the block
 //            codes of the call's tokens: clamp(rint(x / s)); of the block's earlier tokens: clamp(rint((c s_old) / s))
 //   dequant  T(c s)
 //
@@ -30,11 +31,10 @@ template <typename T> __device__ __forceinline__ void store8(T* p, const float* 
 __device__ __forceinline__ float code_of(uint32_t word, int byte) { return static_cast<float>(static_cast<int8_t>(word >> (8 * byte))); }
 // A divisor with its correctly rounded reciprocal: the quotient to the last bit in five instructions. x inv is within an ulp and a half,
 // one correction by its remainder (a multiply-add, exact but for the last rounding) leaves it within an ulp, and a second
-// one is then the rounded quotient (Markstein's theorem). The compiler's division is a dozen instructions and more, in a hundred places. By
-// an infinite scale: 0, or not a number for an infinite x, as divided.
+// one is then the rounded quotient (Markstein's theorem). The compiler's division is a dozen instructions and more, in a hundred places.
 struct Scale {
   float by, inv;
-  explicit __device__ __forceinline__ Scale(float s) : by(s < INFINITY ? s : 1.0f), inv(1.0f / s) {}
+  explicit __device__ __forceinline__ Scale(float s) : by(s), inv(1.0f / s) {}
   __device__ __forceinline__ float quotient(float x) const {
     float r = x * inv;
     r = fmaf(fmaf(-r, by, x), inv, r);
@@ -51,6 +51,21 @@ __device__ __forceinline__ uint32_t byte_of(float code, int byte) { return (stat
 __device__ __forceinline__ u32x2 bytes_of(const float* f) {
   return u32x2{byte_of(f[0], 0) | byte_of(f[1], 1) | byte_of(f[2], 2) | byte_of(f[3], 3),
                byte_of(f[4], 0) | byte_of(f[5], 1) | byte_of(f[6], 2) | byte_of(f[7], 3)};
+}
+// The largest magnitude of a head, where what is not a number counts as above infinity. Lanes gather it with the instruction that keeps
+// what is not a number (fmaxf passes over it). Over each aligned group of WIDTH lanes, 16, 32 or 64: as bits of magnitudes, which have this order.
+template <int WIDTH> __device__ __forceinline__ int largest_bits(float magnitude) {
+  static_assert(WIDTH == 16 || WIDTH == 32 || WIDTH == kWave, "a head's lanes");
+  int v = __builtin_bit_cast(int, magnitude) & 0x7fffffff;
+  v = max(v, dpp<kDppXor1>(v));
+  v = max(v, dpp<kDppXor2>(v));
+  v = max(v, dpp<kDppHalfMirror>(v));
+  v = max(v, dpp<kDppMirror>(v));
+  if constexpr (WIDTH == 16) return v;
+  const int lo = max(__builtin_amdgcn_readlane(v, 0), __builtin_amdgcn_readlane(v, 16)),
+            hi = max(__builtin_amdgcn_readlane(v, 32), __builtin_amdgcn_readlane(v, 48));
+  if constexpr (WIDTH == 32) return (threadIdx.x & 32) ? hi : lo;
+  return max(lo, hi);
 }
 // eight codes brought to another scale
 __device__ __forceinline__ u32x2 moved8(u32x2 w, float before, const Scale& s) {
@@ -94,7 +109,7 @@ __global__ __launch_bounds__((AppendShape<D, BLOCK>::kThreads)) void append_kern
     const BlockTable table, const int32_t* __restrict__ cached, const Ragged rows, const int heads) {
   using Shape = AppendShape<D, BLOCK>;
   constexpr int kShift = BLOCK == 16 ? 4 : BLOCK == 32 ? 5 : BLOCK == 64 ? 6 : 7;
-  __shared__ float s_max[Shape::kThreads / kWave];
+  __shared__ int s_max[Shape::kThreads / kWave];
   const int sets = (heads + Shape::kHeads - 1) / Shape::kHeads;   // of heads
   const bool is_value = blockIdx.x & 1;
   const int set = static_cast<int>(blockIdx.x / 2) % sets;
@@ -128,25 +143,27 @@ __global__ __launch_bounds__((AppendShape<D, BLOCK>::kThreads)) void append_kern
   const int64_t unit = static_cast<int64_t>(here.entry) * heads + min(h, heads - 1);
   float* scale = (is_value ? v_scale : k_scale) + unit;
   const float before = *scale;
-  float amax = 0.0f;
+  float largest = 0.0f;
 #pragma unroll
   for (int i = 0; i < kTokens; ++i) {
     float f[kColumns];
 #pragma unroll
     for (int e = 0; e < kPackets; ++e) Pack<T>::unpack(raw[i][e], f + e * Pack<T>::N);
 #pragma unroll
-    for (int e = 0; e < kColumns; ++e) amax = fmaxf(amax, fabsf(f[e]));   // (rows that are read twice change no maximum)
+    for (int e = 0; e < kColumns; ++e) largest = __builtin_elementwise_maximum(largest, fabsf(f[e]));   // (rows that are read twice change no maximum)
   }
-  amax = group_max<(Shape::kLanes < kWave ? Shape::kLanes : kWave)>(amax);
+  int bits = largest_bits<(Shape::kLanes < kWave ? Shape::kLanes : kWave)>(largest);
   if constexpr (Shape::kThreads > kWave) {
-    if (threadIdx.x % kWave == 0) s_max[threadIdx.x / kWave] = amax;
+    if (threadIdx.x % kWave == 0) s_max[threadIdx.x / kWave] = bits;
     __syncthreads();
 #pragma unroll
-    for (int w = 0; w < Shape::kThreads / kWave; ++w) amax = fmaxf(amax, s_max[w]);
+    for (int w = 0; w < Shape::kThreads / kWave; ++w) bits = max(bits, s_max[w]);
   }
   if (!active) return;
+  const float amax = __builtin_bit_cast(float, bits);
   float s = fmaxf(amax * (1.0f / 127.0f), kScaleEps);
   if (here.lo > 0) s = fmaxf(s, before);
+  if (!(amax < INFINITY) || (here.lo > 0 && before != before)) s = NAN;
   const bool grown = here.lo > 0 && s > before && lo > 0;   // and this lane has earlier tokens
   if (in_head == 0) *scale = s;
   if (hi <= lo && !grown) return;   // nothing of this lane's changes

@@ -723,3 +723,56 @@ def test_blocks_shared_for_reading(ext, dtype):
     starts = torch.tensor([0, 100, 150, 151], dtype=torch.int32, device="cuda")
     for a, b in zip(ext.kv_block_dequant(*cache, one.expand(3, -1), starts, 151, dtype), ext.kv_block_dequant(*copies, own, starts, 151, dtype)):
         assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=TAGS.get)
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf")])
+@pytest.mark.parametrize("cached,new,at", [(0, 30, 7), (0, 30, 25), (5, 30, 3), (5, 30, 29), (5, 1, 0), (0, 1, 0), (15, 2, 1)])
+def test_append_of_values_that_are_not_finite(ext, dtype, bad, cached, new, at):
+    """They show: the block's scale is not a number, and neither are its tokens in that head, when they are read back and in the
+    attention rows that see them. Other blocks and heads do not change, and the block's next first token makes it whole."""
+    g = torch.Generator().manual_seed(31 + cached + new)
+    block, dim, heads, head = 16, 64, 2, 1
+    total, spot = cached + new, (cached + at) // block
+    start = torch.tensor([0, new, new + 2], dtype=torch.int32, device="cuda")
+    lengths = torch.tensor([cached, 4], dtype=torch.int32, device="cuda")
+    table = torch.tensor([[2, 0, 3], [1, -1, -1]], dtype=torch.int32, device="cuda")
+    first = make_cache(g, 4, heads, block, dim, outliers=False)
+    rows = torch.randn(new + 2, 2, heads, dim, generator=g)
+    query = torch.randn(new + 2, 4, dim, generator=g).to(dtype).cuda()
+    ends = torch.tensor([0, total, total], dtype=torch.int32, device="cuda")
+
+    def outcome(rows):
+        cache = [t.cuda() for t in first]
+        on_gpu = rows.to(dtype).cuda()
+        ext.kv_block_append(on_gpu[:, 0], on_gpu[:, 1], *cache, table, lengths, start)
+        back = ext.kv_block_dequant(*cache, table, ends, total, torch.float32)
+        return cache, back, ext.kv_block_attention(query, *cache, table, lengths, 0.125, start).reshape(new + 2, 4, dim)
+
+    clean = outcome(rows)
+    for which in range(2):   # a key, a value
+        spoilt = rows.clone()
+        spoilt[at, which, head, 33] = bad
+        cache, back, out = outcome(spoilt)
+        unit = (int(table[0, spot]), head)
+        assert cache[2 + which][unit].isnan()
+        lo, hi = spot * block, min((spot + 1) * block, total)
+        assert back[which][head, lo:hi].isnan().all()
+        back[which][head, lo:hi] = clean[1][which][head, lo:hi]
+        assert all(torch.equal(a, b) for a, b in zip(back, clean[1]))
+        for got, want in zip(cache, clean[0]):
+            got[unit] = want[unit]
+            assert torch.equal(got, want)
+        see = torch.arange(new + 2, device="cuda").lt(new) & (cached + torch.arange(new + 2, device="cuda") >= lo)   # the block's first token
+        assert out[see][:, 2 * head:2 * head + 2].isnan().all()
+        out[see, 2 * head:2 * head + 2] = clean[2][see, 2 * head:2 * head + 2]
+        assert torch.equal(out, clean[2])
+    # a block whose scale is not a number, from its first token on again
+    cache = [t.cuda() for t in first]
+    for values in (rows.clone().fill_(bad), rows):
+        on_gpu = values[:1].to(dtype).cuda()
+        ext.kv_block_append(on_gpu[:, 0], on_gpu[:, 1], *cache, table[:1], torch.zeros(1, dtype=torch.int32, device="cuda"))
+    want = [t.numpy().copy() for t in first]
+    append_oracle(rows[:1, 0].to(dtype).float().numpy(), want[0], want[2], table[:1].cpu().numpy(), [0], np.array([0, 1]), block)
+    np.testing.assert_array_equal(cache[2].cpu().numpy(), want[2])
+    np.testing.assert_array_equal(cache[0][:, :, 0].cpu().numpy(), want[0][:, :, 0])
