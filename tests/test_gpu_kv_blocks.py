@@ -776,3 +776,99 @@ def test_append_of_values_that_are_not_finite(ext, dtype, bad, cached, new, at):
     append_oracle(rows[:1, 0].to(dtype).float().numpy(), want[0], want[2], table[:1].cpu().numpy(), [0], np.array([0, 1]), block)
     np.testing.assert_array_equal(cache[2].cpu().numpy(), want[2])
     np.testing.assert_array_equal(cache[0][:, :, 0].cpu().numpy(), want[0][:, :, 0])
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=TAGS.get)
+@pytest.mark.parametrize("tokens,q_heads,kv_heads,dim,rotary,wide", [
+    (2049, 28, 4, 128, 128, True), (13200, 7, 3, 64, 32, False), (3300, 4, 1, 256, 256, False), (9500, 5, 2, 96, 96, True),
+    (33000, 3, 1, 64, 64, False), (33000, 0, 4, 64, 64, True), (9000, 1, 7, 80, 48, False), (4200, 32, 8, 128, 128, False)])
+def test_norm_of_many_heads(ext, dtype, tokens, q_heads, kv_heads, dim, rotary, wide):
+    """Calls of more lanes than the chip holds, where a lane takes several heads of a token (heads that are no multiple of four, lanes with
+    query and key heads among them): the formula, and the bits of calls of a few tokens."""
+    g = torch.Generator(device="cuda").manual_seed(tokens + dim)
+    flat = (torch.randn(tokens, (q_heads + kv_heads) * dim, generator=g, device="cuda") * 2).to(dtype)
+    q, k = flat[:, :q_heads * dim], flat[:, q_heads * dim:]
+    qw, kw = ((1 + 0.5 * torch.randn(dim, generator=g, device="cuda")).to(dtype) for _ in range(2))
+    angle = torch.rand(500, rotary, generator=g, device="cuda") * 6.28
+    cos, sin = (t.to(torch.float32 if wide else dtype) for t in (angle.cos(), angle.sin()))
+    position = torch.randint(0, 500, (tokens,), generator=g, device="cuda")
+    got = ext.qk_norm_rope(q, k, qw, kw, cos, sin, 1e-6, position)
+    for out, x, w, heads in zip(got, (q, k), (qw, kw), (q_heads, kv_heads)):
+        want, size = norm_rope64(x.double().reshape(tokens, heads, dim), w.double(), cos[position].double(), sin[position].double(), 1e-6)
+        # (as in test_norm_and_rotation)
+        assert torch.all((out.double() - want).abs() <= half_step(dtype, want) + 20 * U32 * size)
+    few = [ext.qk_norm_rope(q[at:at + 600], k[at:at + 600], qw, kw, cos, sin, 1e-6, position[at:at + 600]) for at in range(0, tokens, 600)]
+    assert all(torch.equal(a, torch.cat(parts)) for a, parts in zip(got, zip(*few)))
+
+
+PAST = [  # block, D, kv heads, group, cached, new, rows of the table (-1, 99: no block)
+    (128, 64, 1, 4, [700, 90, -1, 0, 200], None, [[0, 1, 2, 3, 4, 5], [6], [7], [8], [3, 0]]),
+    (128, 128, 2, 4, [1100], None, [[8, 7, 6, 5, 4, 3, 2, 1, 0]]),
+    (16, 64, 2, 2, [100, 140], None, [[0, -1, 2, 99, 4, 5, 6], [8, 7, 1, 3, 5, 0, 2, -1, 6]]),
+    (64, 128, 1, 8, [300, -1, 5, 63], None, [[4, 3, 99, 1, 0], [2], [8], [7]]),
+    (32, 128, 1, 4, [200, 7], [4, 3], [[0, 1, 2, 3, 4, 5, 6], [7]]),
+    (64, 64, 1, 7, [0, 250, 64], [1, 2, 3], [[7], [0, 2, 4, 6], [1, 3]]),
+    (16, 128, 4, 1, [127], [16], [[0, 1, 2, 3, 4, 5, 6, 7, 8]])]
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=TAGS.get)
+@pytest.mark.parametrize("block,dim,heads,group,cached,new,entries", PAST)
+def test_attention_past_the_caches(ext, dtype, block, dim, heads, group, cached, new, entries):
+    """Tables so wide that codes are read past the caches (as long as their bound says 512 MB and more, or 128 MB a sequence; heads of 64:
+    128 MB together): the formula, and the bits of a table one entry narrower, whose codes are read through them."""
+    limit = 128e6 if dim == 64 else min(128e6 * len(cached), 512e6)
+    width = int(limit // (2 * len(cached) * block * heads * dim)) + 1
+    table = torch.full((len(cached), width), -1, dtype=torch.int32)
+    for b, row in enumerate(entries):
+        table[b, :len(row)] = torch.tensor(row, dtype=torch.int32)
+    got, args = check_attention(ext, dtype, block, dim, heads, group, cached, new, table=table)
+    assert torch.equal(got, ext.kv_block_attention(*args[:5], args[5][:, :-1], *args[6:]))
+
+
+def test_a_captured_step_past_the_caches(ext):
+    """A graph of append and attention under a table of a long max_len, replayed with eager work in between: the eager step's bits."""
+    from llmquant.runtime import BlockQuantCache
+
+    eager, graphed = (fresh(BlockQuantCache, max_len=400000, block=128, num_blocks=30, kv_heads=2) for _ in range(2))
+    g = torch.Generator(device="cuda").manual_seed(8)
+    static = torch.zeros(3, 8 * 64, device="cuda", dtype=torch.bfloat16)
+
+    def step(cache, rows):
+        outs = []
+        for layer in range(2):
+            cache.append(layer, rows[:, 256:384].unflatten(1, (2, 64)), rows[:, 384:].unflatten(1, (2, 64)))
+            outs.append(cache.attend(layer, rows[:, :256].unflatten(1, (4, 64)), 0.125))
+        cache.advance_device(1)
+        return outs
+
+    start = torch.tensor([0, 1500, 1500, 1600], dtype=torch.int32, device="cuda")
+    prompt = torch.randn(1600, 2, 64, generator=g, device="cuda", dtype=torch.bfloat16)
+    for cache in (eager, graphed):
+        cache.add(), cache.add(), cache.add(), cache.release(1)
+        cache.reserve([1600, 0, 200])
+        for layer in range(2):
+            cache.append(layer, prompt, prompt, start)
+        cache.advance([1500, 0, 100])
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):   # (a warm-up, taken back)
+        step(graphed, static)
+    torch.cuda.current_stream().wait_stream(side)
+    for place in (0, 2):
+        graphed.truncate(place, graphed.get_seq_length(place))
+    for a, b in zip((eager.k_codes, eager.v_codes, eager.k_scale, eager.v_scale), (graphed.k_codes, graphed.v_codes, graphed.k_scale, graphed.v_scale)):
+        b.copy_(a)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = step(graphed, static)
+    for turn in range(12):
+        rows = torch.randn(3, 8 * 64, generator=g, device="cuda", dtype=torch.bfloat16)
+        want = step(eager, rows)
+        static.copy_(rows)
+        graph.replay()
+        if turn % 3 == 0:
+            torch.cuda.synchronize()
+        for a, b in zip(want, captured):
+            assert torch.equal(a, b) and torch.all(a[1] == 0) and a[0].abs().sum() > 0
+    for a, b in ((eager.k_codes, graphed.k_codes), (eager.v_codes, graphed.v_codes), (eager.cached, graphed.cached)):
+        assert torch.equal(a, b)
