@@ -550,7 +550,7 @@ int llmq_qk_norm_rope(const void* q, const void* k, const void* q_weight, const 
  * for one sequence at a time (llmquant/quantizers/fake.py:39-55).
  *
  * llmq_kv_block_append quantizes the call's rows (key, value [tokens, kv_heads, head_dim], row strides in elements) into
- * the blocks, which no other sequence of the call may share. a = max |x| over the call's tokens in a block and head:
+ * the blocks, which no other sequence of the call may share. Its tensors share no memory. a = max |x| over the call's tokens in a block and head:
  *   scale = max(a * (1 / 127), 1e-8) (the reciprocal rounded to fp32) where the call writes the block's first token,
  *           else max(scale, that)
  *   code = clamp(rint(x / scale), -128, 127); codes the block held before: clamp(rint((code * old scale) / scale))

@@ -9,7 +9,6 @@
 // No kernel lives here and nothing here synchronises, so every op stays graph-capturable.
 #include <torch/extension.h>
 
-#include <ATen/MemoryOverlap.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <hipblaslt/hipblaslt.h>
@@ -1480,6 +1479,17 @@ at::Tensor packet_vector(const at::Tensor& t) {
 }
 int64_t row_stride(const at::Tensor& t) { return t.size(0) == 1 ? t.numel() : t.stride(0); }
 
+// Whether `out`, contiguous, has bytes of `t`, whose rows are contiguous and may stand apart (torch's own test knows of dense tensors only).
+bool shares_memory(const at::Tensor& out, const at::Tensor& t) {
+  if (out.numel() == 0 || t.numel() == 0) return false;
+  const auto address = [](const at::Tensor& x) { return static_cast<int64_t>(reinterpret_cast<uintptr_t>(x.const_data_ptr())); };
+  const int64_t begin = address(out), end = begin + static_cast<int64_t>(out.nbytes()), rows = t.size(0), first = address(t);
+  const int64_t row = t.numel() / rows * t.element_size(), step = t.stride(0) * t.element_size();
+  // the first row that ends behind `begin`
+  const int64_t at = rows == 1 || step == 0 || first + row > begin ? 0 : (begin - first - row) / step + 1;
+  return at < rows && first + at * step + row > begin && first + at * step < end;
+}
+
 void check_int(int64_t value, const char* name) {
   TORCH_CHECK(value >= 0 && value <= INT32_MAX, name, " is out of range: ", value);
 }
@@ -1646,22 +1656,19 @@ at::Tensor kv_block_attention(const at::Tensor& query, const at::Tensor& k_codes
   check_int(q_heads * c.dim, "the width of query");
   const Batch b = batch_of(block_table, cached, query_start, tokens, k_codes);
   const c10::OptionalDeviceGuard guard(at::device_of(query));
+  const auto qr = packet_rows(query);
   at::Tensor result;
   if (out.has_value()) {
     TORCH_CHECK(out->device() == query.device() && out->scalar_type() == query.scalar_type() && out->is_contiguous() &&
                     out->dim() == 2 && out->size(0) == tokens && out->size(1) == q_heads * c.dim &&
                     reinterpret_cast<uintptr_t>(out->const_data_ptr()) % 16 == 0,
                 "out must be contiguous [", tokens, ", ", q_heads * c.dim, "] of query's dtype, 16-byte aligned");
-    const auto overlaps = [&](const at::Tensor& t) {
-      const auto status = at::get_overlap_status(*out, t);
-      return status == at::MemOverlapStatus::Full || status == at::MemOverlapStatus::Partial;
-    };
-    TORCH_CHECK(!overlaps(query) && !overlaps(k_codes) && !overlaps(v_codes), "out must not share memory with query or the cache");
+    for (const at::Tensor* t : {&qr, &k_codes, &v_codes, &k_scale, &v_scale, &b.table, &b.cached, &b.start})
+      TORCH_CHECK(!t->defined() || !shares_memory(*out, *t), "out must not share memory with query, the cache, block_table, cached or query_start");
     result = *out;
   } else {
     result = at::empty({tokens, q_heads * c.dim}, query.options());
   }
-  const auto qr = packet_rows(query);
   const size_t need = llmq_kv_block_attention_workspace_bytes(static_cast<int>(tokens), b.sequences, static_cast<int>(q_heads),
                                                               c.heads, c.dim, c.block, b.width);
   at::Tensor workspace;

@@ -872,3 +872,38 @@ def test_a_captured_step_past_the_caches(ext):
             assert torch.equal(a, b) and torch.all(a[1] == 0) and a[0].abs().sum() > 0
     for a, b in ((eager.k_codes, graphed.k_codes), (eager.v_codes, graphed.v_codes), (eager.cached, graphed.cached)):
         assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=TAGS.get)
+def test_out_may_not_share_memory_with_rows_that_stand_apart(ext, dtype):
+    """Queries as slices of q|k|v rows: refused where out has a byte of one, of the scales or of the batch's vectors; taken between and behind them."""
+    g = torch.Generator().manual_seed(41)
+    cache = [t.cuda() for t in make_cache(g, 2, 2, 16, 64)]
+    table, cached = torch.zeros(3, 1, dtype=torch.int32, device="cuda"), torch.tensor([3, 9, 15], dtype=torch.int32, device="cuda")
+    heads, wide, tokens, row = 2, 2048, 3, 128
+    room = torch.randn(6, wide, generator=g).to(dtype).cuda()
+    query = room[:tokens, 512:512 + row].unflatten(1, (heads, 64))
+    want, flat, size = ext.kv_block_attention(query, *cache, table, cached, 1.0), room.view(-1), tokens * row
+
+    def attend(at):
+        return ext.kv_block_attention(query, *cache, table, cached, 1.0, None, flat[at:at + size].view(tokens, row))
+
+    # rows 0, 1 and 2: from the start, the last packet, the first one
+    for at in (512, 512 + row - 8, 512 - size + 8, wide + 512 + row - 8, wide + 512 - size + 8, 2 * wide + 512 - size + 8, 2 * wide + 512 + row - 8):
+        with pytest.raises(RuntimeError, match="out must not share memory"):
+            attend(at)
+    for at in (0, 512 - size, 512 + row, wide + 512 - size, wide + 512 + row, 2 * wide + 512 - size, 2 * wide + 512 + row, 3 * wide):
+        kept = room.clone()
+        assert torch.equal(attend(at), want)
+        room.copy_(kept)
+    # the codes, the scales, a table whose rows stand apart and the vectors
+    out = torch.zeros(tokens, row, device="cuda")
+    q, words, inside = query.float(), out.view(-1).view(torch.int32), out.view(-1)[8:12].view(2, 2)
+    apart = words.as_strided((tokens, 1), (row, 1), 3)
+    for args in ((q, *cache[:2], inside, cache[3], table, cached, 1.0, None), (q, *cache[:3], inside, table, cached, 1.0, None),
+                 (q, *cache, apart, cached, 1.0, None), (q, *cache, table, words[9:12], 1.0, None), (q, *cache, table, cached, 1.0, words[9:13])):
+        with pytest.raises(RuntimeError, match="out must not share memory"):
+            ext.kv_block_attention(*args, out)
+    for codes in cache[:2]:
+        with pytest.raises(RuntimeError, match="out must not share memory"):
+            ext.kv_block_attention(q, *cache, table, cached, 1.0, None, codes.view(-1)[:4 * size].view(torch.float32).view(tokens, row))
