@@ -15,6 +15,8 @@ runs one sequence at a time).
 
 from __future__ import annotations
 
+import warnings
+
 import torch
 
 from llmquant.hip.build import load_extension
@@ -184,8 +186,12 @@ class BlockQuantCache:
 
     def reserve(self, new) -> None:
         """Blocks for `new` more tokens of every sequence: a number, or one for each place (0 for an empty one). Nothing
-        changes if there are not enough."""
+        changes if there are not enough. A sequence that counts more tokens than its blocks hold is refused: a new block would
+        pass for tokens that were never stored."""
         new = self._per_place(new)
+        for place, (n, have) in enumerate(zip(self._lengths, self._blocks)):
+            if n > len(have) * self.block:
+                raise ValueError(f"place {place} counts {n} tokens, its blocks hold {len(have) * self.block}: truncate() it first")
         wanted = [0 if n < 0 else max(0, -(-(n + more) // self.block) - len(have))
                   for n, more, have in zip(self._lengths, new, self._blocks)]
         for place, (n, more) in enumerate(zip(self._lengths, new)):
@@ -206,11 +212,16 @@ class BlockQuantCache:
 
     def advance(self, new, device: bool = True) -> None:
         """Count `new` tokens (as for reserve) as cached, behind the last layer of a step. device=False: the host's counts
-        alone, for a step whose captured graph has advanced `cached` itself (advance_device)."""
+        alone, for a step whose captured graph has advanced `cached` itself (advance_device). Tokens that no block was reserved
+        for are refused, or, where the device has counted them already, warned of: append() has left them out."""
         new = self._per_place(new)
         for place, (n, more, have) in enumerate(zip(self._lengths, new, self._blocks)):
-            if device and n + more > len(have) * self.block:   # (else the device has counted them already)
+            if n + more <= len(have) * self.block or n < 0:
+                continue
+            if device:
                 raise ValueError(f"place {place} would hold {n + more} tokens, blocks for {len(have) * self.block} are reserved")
+            warnings.warn(f"place {place} counts {n + more} tokens, but blocks for {len(have) * self.block} are reserved: those behind "
+                          "were not stored (reserve() before the step; truncate() to go on)", RuntimeWarning, stacklevel=2)
         self._lengths = [n if n < 0 else n + more for n, more in zip(self._lengths, new)]
         if device:
             self.cached.copy_(torch.tensor(self._lengths, dtype=torch.int32))

@@ -188,3 +188,24 @@ def test_advance_refuses_tokens_without_blocks():
     assert cache.get_seq_length(a) == 0 and cache.cached.tolist() == [0, -1, -1]
     cache.advance(32)
     assert cache.get_seq_length(a) == 32
+
+
+def test_tokens_that_a_captured_step_lost_are_told():
+    import warnings
+
+    cache = make()
+    a, b = cache.add(), cache.add()
+    cache.reserve([16, 16, 0])
+    with warnings.catch_warnings():
+        warnings.simplefilter("error")
+        cache.advance_device(16)
+        cache.advance(16, device=False)   # as many as were reserved
+    cache.advance_device(1)               # a step that nothing was reserved for
+    with pytest.warns(RuntimeWarning, match="place 0 counts 17 tokens, but blocks for 16 are reserved"):
+        cache.advance([1, 0, 0], device=False)
+    with pytest.raises(ValueError, match="place 0 counts 17 tokens, its blocks hold 16"):
+        cache.reserve(1)
+    assert cache.free_blocks() == 8 and cache.get_seq_length(a) == 17 and cache.get_seq_length(b) == 16
+    cache.truncate(a, 16)
+    cache.reserve(1)
+    assert cache.free_blocks() == 6
