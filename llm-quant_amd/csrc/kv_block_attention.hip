@@ -805,7 +805,8 @@ extern "C" int llmq_kv_block_attention(const void* query, int64_t q_row_stride, 
                                        int dtype, llmq_stream_t stream) {
   if (int rc = llmq_host::check_block_shape(tokens, sequences, kv_heads, head_dim, block, n_blocks, table_width, table_stride, dtype)) return rc;
   if (q_heads <= 0 || q_heads % kv_heads != 0) return llmq_host::fail_invalid("q_heads %d is not a multiple of kv_heads %d", q_heads, kv_heads);
-  if (!std::isfinite(sm_scale)) return llmq_host::fail_invalid("sm_scale must be finite");
+  const float scale_log2e = sm_scale * 1.4426950408889634f;
+  if (!std::isfinite(scale_log2e)) return llmq_host::fail_invalid("sm_scale must be finite, times log2 e too");
   if (!query_start_or_null && tokens != sequences)
     return llmq_host::fail_invalid("without query_start a sequence has one row: %d rows, %d sequences", tokens, sequences);
   const int v = dtype == LLMQ_F32 ? 4 : 8;
@@ -835,7 +836,7 @@ extern "C" int llmq_kv_block_attention(const void* query, int64_t q_row_stride, 
   const Problem a{query, q_row_stride, static_cast<const int8_t*>(k_codes), static_cast<const int8_t*>(v_codes), k_scale, v_scale,
                   {block_table, table_stride, table_width, n_blocks}, cached, {query_start_or_null, sequences, tokens}, out,
                   static_cast<int32_t*>(workspace),
-                  workspace ? reinterpret_cast<float*>(static_cast<char*>(workspace) + counts_bytes(vectors)) : nullptr, splits, q_heads, kv_heads, group, shift, sm_scale * 1.4426950408889634f,
+                  workspace ? reinterpret_cast<float*>(static_cast<char*>(workspace) + counts_bytes(vectors)) : nullptr, splits, q_heads, kv_heads, group, shift, scale_log2e,
                   {static_cast<uint32_t>(group), static_cast<uint32_t>(((uint64_t{1} << 32) + group - 1) / group)}};
   hipStream_t s = static_cast<hipStream_t>(stream);
   switch (dtype) {

@@ -209,3 +209,24 @@ def test_tokens_that_a_captured_step_lost_are_told():
     cache.truncate(a, 16)
     cache.reserve(1)
     assert cache.free_blocks() == 6
+
+
+@pytest.mark.parametrize("scale", [3e38, -2.5e38])
+def test_attention_refuses_a_scale_that_overflows(lib, scale):
+    """sm_scale is finite in fp32, but the factor of the scores' exponent to base 2 is not."""
+    assert attention(lib, scale=scale) == 1 and "finite" in text(lib)
+    assert attention(lib, scale=scale * 0.7) == 1 and "null tensor pointer" in text(lib)
+
+
+def test_attention_refuses_a_small_workspace(lib):
+    size = lib.llmq_kv_block_attention_workspace_bytes
+    for shape, stride in (((1, 1, 32, 8, 128, 128, 1024), 4096), ((73, 16, 28, 4, 128, 16, 200), 3584), ((3, 3, 4, 2, 64, 64, 16), 256)):
+        tokens, sequences, q_heads, kv_heads, dim, block, width = shape
+        need = size(*shape)   # (long enough to be split)
+        assert need > 0
+        a = dict(tokens=tokens, sequences=sequences, q_heads=q_heads, kv_heads=kv_heads, dim=dim, block=block, width=width, q_stride=stride,
+                 start=16, pointer=16)
+        assert attention(lib, space=need - 1, **a) == 1 and f"{need - 1} bytes" in text(lib) and str(need) in text(lib)
+        assert attention(lib, space=need, workspace=None, **a) == 1 and "workspace" in text(lib)
+        assert attention(lib, space=need, workspace=24, **a) == 1 and "16-byte aligned" in text(lib)
+    assert size(1, 1, 32, 8, 128, 64, 15) == 0 and size(4096, 1, 32, 8, 128, 64, 10000) == 0   # a short walk, rows enough
