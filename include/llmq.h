@@ -575,7 +575,12 @@ int llmq_kv_block_dequant(const void* k_codes, const void* v_codes, const float*
  *   out[row, h, :] = softmax(sm_scale * q[row, h, :] . k[j, h / (q_heads / kv_heads), :]) v
  * q [tokens, q_heads, head_dim] (row stride in elements), out [tokens, q_heads * head_dim]. Tokens without a block are left
  * out; a row that sees nothing (a sequence that takes no part among them) is zero; rows that no sequence has are not
- * written. workspace: llmq_kv_block_attention_workspace_bytes(...) bytes, 16-byte aligned (NULL where that is 0), needs no
+ * written. Scores, softmax sum and output are summed in fp32. For 16-bit queries the softmax weights enter the product with the values
+ * as fp16 (2^-11 off, 2^-25 of the row's largest at the least), queries as fp16 with one exponent a row (exact but for elements below
+ * 2^-14 of the row's largest, 2^-25 of that off); for fp32 both have 22 bits. The scores' products add up codes that are 1152 too
+ * high for 16-bit queries, so that their fp32 roundings are those of a sum about nine times as large. Value scales that append writes, up to
+ * 2^55. The launch goes by table_width, not by what is cached: a table wider than needed costs a second launch. sm_scale and its
+ * product with log2 e are finite. workspace: llmq_kv_block_attention_workspace_bytes(...) bytes, 16-byte aligned (NULL where that is 0), needs no
  * clearing; calls that overlap in time need one each. out shares no memory with the inputs. */
 size_t llmq_kv_block_attention_workspace_bytes(int tokens, int sequences, int q_heads, int kv_heads, int head_dim, int block,
                                                int table_width);

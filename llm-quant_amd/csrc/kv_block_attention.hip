@@ -4,8 +4,9 @@
 //
 // Mathematics. The value scale goes into the exponent: u_j = t_j + log2 s_v(j), w_j = 2^(u_j - max u), so that
 //   out = sum w_j c_j / sum (w_j / s_v(j))
-// and the second product meets bare codes with weights of at most 1, however far the blocks' scales lie apart; the division in
-// the sum of the softmax is one product for 16 scores, all of one block. Codes become fp16 by placing them, sign flipped, in
+// and the second product meets bare codes with weights of at most 1, whatever the blocks' scales; the division in the sum of the
+// softmax is one product for 16 scores, all of one block. The sum is short of weights that underflow, below 2^-126 of the largest, which
+// a scale of the least, 1e-8, brings to 2^-99 / max s_v of the sum at the most: 2^-44 a token with scales up to 2^55 (values of 4e18). Codes become fp16 by placing them, sign flipped, in
 // the mantissa of 1024 (one byte permute for two codes, exact); the 1152 too many are taken from the value codes (one packed
 // add for two), and from the scores through sum q, in fp32. A query row is brought to [1, 2) by a power of two and enters as
 // fp16: exact for 16-bit types but for elements 2^-14 below the row's largest (off by 2^-25 of that), the weights as fp16 (off by
@@ -727,7 +728,9 @@ __global__ __launch_bounds__(kThreads) void merge_kernel(const Problem a) {
   }
 }
 
-// Row tiles of 16 that a wave takes: one where an average sequence has no more (its waves then share tokens), else two.
+// Row tiles of 16 that a wave takes: one where an average sequence has no more (its waves then share tokens), else two. The host does
+// not know how the rows lie: one prompt of 200 rows, groups of 4, takes 13.3 us by itself (two), 11.0 among 96 places that have none (one),
+// 700 rows 27.4, among 256 places 30.5.
 int row_tiles(int64_t rows, int sequences, int group) {
   const int64_t average = rows * group / sequences;
   return average <= 16 ? 1 : 2;
@@ -738,7 +741,10 @@ int64_t row_groups(int64_t rows, int sequences, int group, int tiles) {
   return rows * group / (kWaves * 16 * tiles) + sequences;
 }
 
-// Partial results that a row can have, 1: none. By the table's width, the longest that a sequence can be.
+// Partial results that a row can have, 1: none. By the table's width, the longest that a sequence can be, which the host knows; what
+// is cached it does not: a row on 600 tokens of heads of 64 takes 6.1 us under a table of 640 tokens, 8.2 under one of 1024 to 4096 (a merge
+// that finds nothing, a wave a row), 9.1 under 8192 and more (a workgroup a row). And by all rows of the call: a row on 131000 tokens takes 51 us by
+// itself, but beside 1100 rows of 32 heads on nothing (43 us) 771, since it is not split.
 int most_splits(int64_t vectors, int block, int table_width) {
   const int64_t tiles = (static_cast<int64_t>(table_width) * block + kTile - 1) / kTile;
   if (tiles < 2 * kLeastTiles) return 1;   // (a second launch costs more than half of so short a walk)
@@ -747,9 +753,11 @@ int most_splits(int64_t vectors, int block, int table_width) {
 size_t counts_bytes(int64_t vectors) { return (static_cast<size_t>(vectors) * sizeof(int32_t) + 15) / 16 * 16; }
 
 // Whether codes are read past the caches, by the bytes of the longest that the sequences can be (their table's width), against the
-// 256 MB Infinity Cache; one row tile a wave. Long sequences: 131000 tokens of eight heads of 128 51.8 -> 49.9 us, 400000
-// 143 -> 133, two of 200000 together 78.5 -> 73.8, but one of 65000 30.6 -> 30.9. A batch's lengths differ and it holds about half of its bound: 48 sequences of 308 MB
-// together 65.8 -> 64.0, 614 MB 115 -> 113, but 205 MB 46.8 -> 50.1, 102 MB 31.5 -> 34.2. Heads of 64, whose requests are the
+// 256 MB Infinity Cache; one row tile a wave. Measured under tables as wide as the longest sequence: 131000 tokens of eight heads of 128
+// 51.8 -> 49.9 us, 400000 143 -> 133, two of 200000 together 78.5 -> 73.8; one of 65000, at the border, 30.6 -> 30.9. 48 ragged sequences, which
+// hold about half of such a table, of 308 MB together 65.8 -> 64.0, 614 MB 115 -> 113, but 205 MB 46.8 -> 50.1, 102 MB 31.5 -> 34.2. Under a wider table
+// the rule takes what is cached for more than it is: 48 sequences of 600 tokens (59 MB) 22.1 us under 4096 tokens each, 25.7 under 8192
+// and more, eight of 1000 11.1 and 12.7 (under 32768); heads of 64, 48 of 600, 13.2 and 14.8. Heads of 64, whose requests are the
 // smallest, gain earlier: 64 sequences of 154 MB 37.1 -> 34.2. Heads of 256 do not: 48 sequences of 307 MB 78.6 -> 85.0, 205 MB 61 -> 67.
 // Two row tiles, which other waves may read again: 20.4 -> 22.9.
 bool streams(const Problem& a, int D) {

@@ -124,7 +124,10 @@ class BlockQuantCache:
     block_table  int32 [max_sequences, blocks of max_len]: a place's blocks in order, -1 where there is none
     cached       int32 [max_sequences]: tokens a place holds; -1: nobody is in it, and it takes no part
 
-    A step: reserve() the blocks for its tokens, append() and attend() in every layer, advance(). The rows of a call are one
+    The attention's launches go by the table's width, and so by `max_len`, not by what is cached: no more than is needed.
+
+    A step: reserve() the blocks for its tokens, append() and attend() in every layer, advance() (a copy to the device that waits
+    for its stream, as reserve() where it takes a block; a captured step has advance_device()). The rows of a call are one
     for each place, or, with `query_start` (int32 [max_sequences + 1]), rows query_start[b] .. query_start[b + 1] - 1 for
     place b: drafted tokens, prompts, a prompt's next chunk, single tokens, mixed as they come.
     """
@@ -178,7 +181,8 @@ class BlockQuantCache:
 
     def truncate(self, place: int, length: int) -> None:
         """Take back what was cached behind the first `length` tokens (drafted tokens that were not accepted). Blocks stay
-        reserved; a partly kept block keeps its scale."""
+        reserved. A partly kept block keeps the scale and the codes that the tokens taken back left: where one of them was larger than
+        all before, the kept ones have that step, and where one was not finite they are lost."""
         self._taken(place)
         if not 0 <= length <= self._lengths[place]:
             raise ValueError(f"place {place} holds {self._lengths[place]} tokens, cannot be cut to {length}")

@@ -907,3 +907,17 @@ def test_out_may_not_share_memory_with_rows_that_stand_apart(ext, dtype):
     for codes in cache[:2]:
         with pytest.raises(RuntimeError, match="out must not share memory"):
             ext.kv_block_attention(q, *cache, table, cached, 1.0, None, codes.view(-1)[:4 * size].view(torch.float32).view(tokens, row))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=TAGS.get)
+def test_attention_of_value_scales_far_apart(ext, dtype):
+    """Blocks of the least value scale beside one of 2^50: the least one's tokens count in the softmax's sum."""
+    def far(q, cache, table):
+        q[:] *= 0.1                            # (scores near each other)
+        cache[3][:] = 1e-8
+        cache[3][table[0, 1]] = 2.0 ** 50
+        cache[3][table[1, 0]] = 2.0 ** 50
+
+    check_attention(ext, dtype, 16, 64, 1, 4, [90, 40], None, adjust=far)
+    check_attention(ext, dtype, 16, 64, 1, 2, [1500, 1100], [1, 3], adjust=far)
+    check_attention(ext, dtype, 16, 128, 1, 4, [60, 20], [40, 33], adjust=far)
