@@ -590,6 +590,39 @@ int llmq_kv_block_attention(const void* query, int64_t q_row_stride, const void*
                             size_t workspace_bytes, float sm_scale, int tokens, int sequences, int q_heads, int kv_heads,
                             int head_dim, int block, int n_blocks, int table_width, int dtype, llmq_stream_t stream);
 
+/* The gradient of a quantized Linear by its input: grad_x[t, k] = sum_n grad[t, n] W[n, k] with W = (dtype)(code * scale), the
+ * matrix of the reference's many-rows branch (llmquant/quantizers/kernel.py:68-79; its autograd is PyTorch's). grad: [rows, N], row
+ * stride in elements; qweight, wscale, keep_per_group (a multiple of 8) and out_group as for llmq_dequant_weight; grad_x: [rows, G *
+ * keep_per_group], contiguous. N a multiple of 8, rows up to 2^20. fp32 sums; fp32 operands as three bfloat16 planes (2^-24 of a
+ * product). Tensors 16-byte aligned. workspace: llmq_wq_linear_grad_workspace_bytes(...) bytes, 16-byte aligned, needs no
+ * clearing; calls that overlap in time need one each. */
+size_t llmq_wq_linear_grad_workspace_bytes(int rows, int N, int G, int keep_per_group, int dtype);
+int llmq_wq_linear_grad(const void* grad, int64_t grad_stride, const void* qweight, const float* wscale, void* grad_x,
+                        void* workspace, size_t workspace_bytes, int rows, int N, int G, int gs, int keep_per_group,
+                        int out_group, int wformat, int dtype, llmq_stream_t stream);
+
+/* Softmax cross entropy over a vocabulary without the logits, and its gradient (no counterpart among the reference's kernels):
+ *   l[t, v] = hidden[t] . weight[v]    lse[t] = log sum_v exp l[t, v]    losses[t] = lse[t] - l[t, targets[t]]
+ *   P[t, v] = (exp(l[t, v] - lse[t]) - [v = targets[t]]) grad[t]    grad_hidden = P weight    grad_weight = P^T hidden
+ * hidden: [rows, hidden_size] `dtype`, row stride in elements. weight: [vocab, hidden_size] `dtype` (wformat 0), or codes [vocab,
+ * hidden_size / group_size, group_size] with wscale (wformat 8 or 4, out_group, as for llmq_wq_gemv), which stand for
+ * (dtype)(code * scale) and have no gradient. losses, lse, grad: fp32 [rows]. A row whose target is ignore_index has loss 0 and
+ * no part in a gradient, whatever it holds; any other target outside [0, vocab) makes the row's loss NaN, its
+ * gradient NaN and grad_weight NaN. lse: as llmq_vocab_loss gave it. Logits and sums in fp32; P is rounded to `dtype` (to three bfloat16
+ * planes for fp32), with grad scaled by a power of two to at most 2. Gradients are rounded once. hidden_size a multiple of 8, up
+ * to 65536; rows up to 2^20, vocab up to 2^24; tensors 16-byte aligned. No rows: nothing is written (grad_weight neither). workspace:
+ * ..._workspace_bytes(...) bytes, 16-byte aligned, needs no clearing; calls that overlap in time need one each. */
+size_t llmq_vocab_loss_workspace_bytes(int rows, int vocab, int hidden_size, int wformat, int dtype);
+int llmq_vocab_loss(const void* hidden, int64_t hidden_stride, const void* weight, const float* wscale_or_null,
+                    const int64_t* targets, int64_t ignore_index, float* losses, float* lse, void* workspace,
+                    size_t workspace_bytes, int rows, int vocab, int hidden_size, int group_size, int out_group,
+                    int wformat, int dtype, llmq_stream_t stream);
+size_t llmq_vocab_loss_grad_workspace_bytes(int rows, int vocab, int hidden_size, int wformat, int dtype, int want_weight);
+int llmq_vocab_loss_grad(const void* hidden, int64_t hidden_stride, const void* weight, const float* wscale_or_null,
+                         const int64_t* targets, int64_t ignore_index, const float* lse, const float* grad, void* grad_hidden,
+                         void* grad_weight_or_null, void* workspace, size_t workspace_bytes, int rows, int vocab,
+                         int hidden_size, int group_size, int out_group, int wformat, int dtype, llmq_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,233 @@
+// Matrices brought into the form that the tiles of dense_tile.h take (rows of a multiple of 64, one plane of 16-bit values or
+// three of an fp32 matrix), as they lie and / or transposed: activations, dense weights, and quantized weights as the
+// values (dtype)(code * scale) they stand for, which is the matrix that the reference multiplies by when many rows come
+// (`_dequantized_weight`, llmquant/quantizers/kernel.py:68-79).
+//
+// 64 x 64 values a workgroup, 16 bytes of every row at a time; the transposed form goes through LDS. Bound: HBM (or the
+// caches: a piece that was just written is read back by the product behind).
+#pragma once
+
+#include "dense_tile.h"
+
+namespace llmq {
+
+struct StageSource {
+  const void* base;        // values [rows, stride], or codes [rows, groups, group_size] (BITS 4: two a byte)
+  const float* scale;      // [scale rows, groups] of codes
+  const float* keep_rows;  // or null: rows whose entry is 0 are zeros in the transposed form
+  int64_t stride;          // elements between rows (values)
+  int rows, cols;          // cols: a multiple of 8
+  int first_row;           // of the piece
+  int piece_rows;          // rows of the piece; those at or past `rows` are zeros
+  int groups, group_size, keep, out_group;   // codes: `keep` values of a group are columns
+  int first_col = 0;       // codes: the first column taken
+};
+struct StageTarget {
+  void* rows;              // or null: [piece_rows, ld] a plane
+  void* transposed;        // or null: [cols, ld_t] a plane, columns up to a multiple of 64 written
+  int64_t plane, plane_t;  // elements between planes
+  int ld, ld_t;
+};
+
+// BITS: 0 values of T, 8 or 4 codes that stand for values of T
+template <typename T, int BITS>
+__global__ __launch_bounds__(256) void stage_kernel(const StageSource src, const StageTarget to) {
+  using O = typename TileType<T>::type;
+  constexpr int P = TileType<T>::kPlanes, kPad = 72;   // (halfwords a row of LDS: 16-byte reads of neighbouring rows meet other banks)
+  __shared__ __attribute__((aligned(16))) uint16_t s_t[P][64][kPad];
+  const int r0 = blockIdx.y * 64, c0 = blockIdx.x * 64;
+#pragma unroll
+  for (int half = 0; half < 2; ++half) {
+    const int r = r0 + half * 32 + static_cast<int>(threadIdx.x) / 8, c = c0 + static_cast<int>(threadIdx.x) % 8 * 8;
+    const int64_t row = static_cast<int64_t>(src.first_row) + r;
+    float f[8] = {};
+    if (r < src.piece_rows && row < src.rows && c < src.cols) {
+      if constexpr (BITS == 0) {
+        const T* x = static_cast<const T*>(src.base) + row * src.stride + c;
+#pragma unroll
+        for (int i = 0; i < 8; i += Pack<T>::N) Pack<T>::unpack(load16(x + i), f + i);
+      } else {
+        const int g = (src.first_col + c) / src.keep, k = src.first_col + c - g * src.keep;
+        const int64_t group = row * src.groups + g;
+        const float s = src.scale[(src.out_group > 0 ? row / src.out_group : row) * src.groups + g];
+        const uint8_t* q = static_cast<const uint8_t*>(src.base) + (group * src.group_size + k) * BITS / 8;
+        if constexpr (BITS == 8) {
+          const u32x2 w = *reinterpret_cast<const u32x2*>(q);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) f[i] = static_cast<float>(static_cast<int8_t>((i < 4 ? w.x : w.y) >> (8 * (i % 4)))) * s;
+        } else {
+          const uint32_t signs = *reinterpret_cast<const uint32_t*>(q) ^ 0x88888888u;   // (code + 8 with its top bit flipped: the code)
+#pragma unroll
+          for (int i = 0; i < 8; ++i) f[i] = static_cast<float>(static_cast<int32_t>(signs << (28 - 4 * i)) >> 28) * s;
+        }
+      }
+    }
+    uint16_t v[P][8];
+    if constexpr (P == 1) {
+      const u32x4 w = Pack<O>::pack(f);   // (values of T come back as they were)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[0][i] = static_cast<uint16_t>((i < 2 ? w.x : i < 4 ? w.y : i < 6 ? w.z : w.w) >> (16 * (i % 2)));
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        uint16_t p[3];
+        planes_of(f[i], p);
+#pragma unroll
+        for (int j = 0; j < P; ++j) v[j][i] = p[j];
+      }
+    }
+    if (to.rows != nullptr && r < src.piece_rows && c < to.ld) {
+#pragma unroll
+      for (int j = 0; j < P; ++j) {
+        u32x4 w;
+        w.x = v[j][0] | static_cast<uint32_t>(v[j][1]) << 16;
+        w.y = v[j][2] | static_cast<uint32_t>(v[j][3]) << 16;
+        w.z = v[j][4] | static_cast<uint32_t>(v[j][5]) << 16;
+        w.w = v[j][6] | static_cast<uint32_t>(v[j][7]) << 16;
+        store16(static_cast<uint16_t*>(to.rows) + j * to.plane + static_cast<int64_t>(r) * to.ld + c, w);
+      }
+    }
+    if (to.transposed != nullptr) {
+      const bool dropped = src.keep_rows != nullptr && row < src.rows && src.keep_rows[row] == 0.0f;
+#pragma unroll
+      for (int j = 0; j < P; ++j)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) s_t[j][threadIdx.x % 8 * 8 + i][half * 32 + threadIdx.x / 8] = dropped ? uint16_t{0} : v[j][i];
+    }
+  }
+  if (to.transposed == nullptr) return;
+  __syncthreads();
+#pragma unroll
+  for (int half = 0; half < 2; ++half) {
+    const int c = half * 32 + static_cast<int>(threadIdx.x) / 8, r = static_cast<int>(threadIdx.x) % 8 * 8;
+    if (c0 + c < src.cols && r0 + r < to.ld_t) {
+#pragma unroll
+      for (int j = 0; j < P; ++j)
+        store16(static_cast<uint16_t*>(to.transposed) + j * to.plane_t + static_cast<int64_t>(c0 + c) * to.ld_t + r0 + r,
+                load16(&s_t[j][c][r]));
+    }
+  }
+}
+
+// Both forms of a piece: rows up to a multiple of 64 and columns up to `ld` are covered (zeros past the ends).
+template <typename T>
+inline void stage_launch(const StageSource& src, const StageTarget& to, int bits, hipStream_t stream) {
+  const int cols = to.rows != nullptr && to.ld > src.cols ? to.ld : src.cols;
+  const dim3 grid((cols + 63) / 64, (src.piece_rows + 63) / 64);
+  if (bits == 0) hipLaunchKernelGGL((stage_kernel<T, 0>), grid, dim3(256), 0, stream, src, to);
+  else if (bits == 8) hipLaunchKernelGGL((stage_kernel<T, 8>), grid, dim3(256), 0, stream, src, to);
+  else hipLaunchKernelGGL((stage_kernel<T, 4>), grid, dim3(256), 0, stream, src, to);
+}
+
+// ---- products whose result is a tensor ------------------------------------------------------------------------------------
+// out[n, m] = sum_k A[m, k] B[n, k], n < B's rows, m < A's rows. SUMS: fp32 planes, one a split of K (blockIdx.z), added to what is there unless
+// `first`; else the type of the call, times *scale (null: 1).
+struct ProductOut {
+  void* base;
+  int64_t plane, ld;   // elements
+  const float* scale;
+  int first;
+};
+
+template <typename T, int TM, int TN, int WM, int WN, bool SUMS>
+__global__ __launch_bounds__(WM * WN * kWave) void product_kernel(const TileOperand a, const TileOperand b, const int k,
+                                                                       const int m_tiles, const ProductOut out) {
+  using O = typename TileType<T>::type;
+  using Tile = DenseTile<O, TM, TN, WM, WN>;
+  __shared__ __attribute__((aligned(16))) uint8_t s_mem[Tile::kLdsBytes];
+  const int steps = k / Tile::kStep, splits = gridDim.z, per = (steps + splits - 1) / splits;
+  const int k0 = min(static_cast<int>(blockIdx.z) * per, steps) * Tile::kStep, k1 = min((static_cast<int>(blockIdx.z) + 1) * per, steps) * Tile::kStep;
+  const int tile = tile_of_workgroup(blockIdx.x, gridDim.x), m0 = tile % m_tiles * TM, n0 = tile / m_tiles * TN;
+  if (k0 >= k1) {   // nothing of K is this split's: zeros where the sums begin, which they do in the first call
+    if (SUMS && out.first) {
+      for (int i = threadIdx.x; i < TM * TN; i += Tile::kThreads) {
+        const int n = n0 + i / TM, m = m0 + i % TM;
+        if (n < b.rows && m < a.rows) static_cast<float*>(out.base)[blockIdx.z * out.plane + n * out.ld + m] = 0.0f;
+      }
+    }
+    return;
+  }
+  Tile t;
+  t.template multiply<(TileType<T>::kPlanes == 3 ? 6 : 1)>(s_mem, a, m0, b, n0, k0, k1);
+  const float scale = SUMS || out.scale == nullptr ? 1.0f : *out.scale;
+#pragma unroll
+  for (int ni = 0; ni < Tile::NI; ++ni) {
+    const int n = n0 + Tile::col_of(ni);
+    if (n >= b.rows) continue;
+#pragma unroll
+    for (int mi = 0; mi < Tile::MI; ++mi) {
+      const int m = m0 + Tile::row_of(mi, 0);
+      if (m >= a.rows) continue;   // (rows of A are a multiple of 4)
+      if constexpr (SUMS) {
+        float* to = static_cast<float*>(out.base) + blockIdx.z * out.plane + n * out.ld + m;
+        tile_v4f v = t.acc[mi][ni];
+        if (!out.first) v += *reinterpret_cast<const tile_v4f*>(to);
+        *reinterpret_cast<tile_v4f*>(to) = v;
+      } else {
+        T* to = static_cast<T*>(out.base) + n * out.ld + m;
+        const float f[4] = {t.acc[mi][ni][0] * scale, t.acc[mi][ni][1] * scale, t.acc[mi][ni][2] * scale, t.acc[mi][ni][3] * scale};
+        if constexpr (sizeof(T) == 4) {
+          *reinterpret_cast<tile_v4f*>(to) = tile_v4f{f[0], f[1], f[2], f[3]};
+        } else {
+          const T h[4] = {from_float<T>(f[0]), from_float<T>(f[1]), from_float<T>(f[2]), from_float<T>(f[3])};
+          *reinterpret_cast<u32x2*>(to) = __builtin_bit_cast(u32x2, h);
+        }
+      }
+    }
+  }
+}
+
+// out[n, m] = (dtype)(scale * the sum of the planes), eight values a lane
+template <typename T>
+__global__ __launch_bounds__(256) void add_planes_kernel(const float* __restrict__ planes, const int64_t plane, const int splits,
+                                                         const float* __restrict__ scale_or_null, T* __restrict__ out, const int64_t count8) {
+  const float scale = scale_or_null == nullptr ? 1.0f : *scale_or_null;
+  for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < count8; i += static_cast<int64_t>(gridDim.x) * 256) {
+    float f[8] = {};
+    for (int z = 0; z < splits; ++z) {
+      const float* p = planes + z * plane + i * 8;
+      const tile_v4f lo = *reinterpret_cast<const tile_v4f*>(p), hi = *reinterpret_cast<const tile_v4f*>(p + 4);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        f[e] += lo[e];
+        f[4 + e] += hi[e];
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) f[e] *= scale;
+#pragma unroll
+    for (int e = 0; e < 8; e += Pack<T>::N) store16(out + i * 8 + e, Pack<T>::pack(f + e));
+  }
+}
+template <typename T>
+inline void add_planes_launch(const float* planes, int64_t plane, int splits, const float* scale, void* out, int64_t count, hipStream_t stream) {
+  const int64_t count8 = count / 8, blocks = (count8 + 255) / 256;
+  hipLaunchKernelGGL((add_planes_kernel<T>), dim3(static_cast<unsigned>(blocks < 4096 ? blocks : 4096)), dim3(256), 0, stream,
+                     planes, plane, splits, scale, static_cast<T*>(out), count8);
+}
+
+// Rows of B a tile takes: 64 where there are no more, else 256 (a tile of few rows is bound by A's bytes, not by the
+// multiplications that its empty rows waste).
+constexpr int kFewRows = 64;
+constexpr int tile_rows(int rows) { return rows <= kFewRows ? kFewRows : 256; }
+
+// Splits of K so that the tiles fill the chip, of eight steps at least.
+inline int splits_for(int m_rows, int n_rows, int k) {
+  const int tn = tile_rows(n_rows), places = tn == kFewRows ? 512 : 256;
+  const int64_t tiles = static_cast<int64_t>((m_rows + 255) / 256) * ((n_rows + tn - 1) / tn);
+  const int64_t wanted = places / (tiles < 1 ? 1 : tiles), most = k / 64 / 8;
+  const int64_t splits = wanted < most ? wanted : most;
+  return static_cast<int>(splits < 1 ? 1 : splits);
+}
+
+template <typename T, bool SUMS>
+inline void product_launch(const TileOperand& a, const TileOperand& b, int k, const ProductOut& out, int splits, hipStream_t stream) {
+  const int m_tiles = (a.rows + 255) / 256, tn = tile_rows(b.rows), n_tiles = (b.rows + tn - 1) / tn;
+  const dim3 grid(static_cast<unsigned>(m_tiles) * n_tiles, 1, splits);
+  if (tn == kFewRows) hipLaunchKernelGGL((product_kernel<T, 256, 64, 4, 2, SUMS>), grid, dim3(512), 0, stream, a, b, k, m_tiles, out);
+  else hipLaunchKernelGGL((product_kernel<T, 256, 256, 2, 4, SUMS>), grid, dim3(512), 0, stream, a, b, k, m_tiles, out);
+}
+
+inline int64_t round_up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
+
+}  // namespace llmq

@@ -1776,6 +1776,149 @@ at::Tensor argmax_advance(const at::Tensor& x, at::Tensor& token, at::Tensor& st
   return out;
 }
 
+// ---- learning beside frozen codes ------------------------------------------------------------------------------------
+// Rows as they lie where they are whole packets that do not overlap (an expanded row becomes one of its own each).
+at::Tensor own_rows(const at::Tensor& t) {
+  const bool overlap = t.size(0) > 1 && t.stride(0) < t.size(1);
+  return packet_rows(overlap ? t.contiguous() : t);
+}
+// stride of rows that may be none
+int64_t own_stride(const at::Tensor& t) { return t.size(0) <= 1 ? t.size(1) : t.stride(0); }
+
+struct QuantWeight {
+  int64_t rows, groups, group_size;
+  int format;
+};
+QuantWeight quant_weight(const at::Tensor& qweight, const at::Tensor& wscale, int64_t out_group, const at::Tensor& like) {
+  TORCH_CHECK(qweight.device() == like.device() && wscale.device() == like.device(), "the weight must lie on the rows' device");
+  TORCH_CHECK(qweight.dim() == 3 && qweight.is_contiguous(), "qweight must be contiguous [N, groups, group_size]");
+  const bool packed = qweight.scalar_type() == at::kByte;
+  TORCH_CHECK(packed || qweight.scalar_type() == at::kChar, "qweight must be int8, or uint8 for nibble-packed int4");
+  TORCH_CHECK(wscale.scalar_type() == at::kFloat && wscale.dim() == 2 && wscale.is_contiguous(),
+              "wscale must be contiguous float32 [scale_rows, groups]");
+  TORCH_CHECK(out_group >= 0 && out_group <= INT32_MAX, "out_group must be >= 0");
+  QuantWeight w{qweight.size(0), qweight.size(1), packed ? qweight.size(2) * 2 : qweight.size(2), packed ? LLMQ_W_INT4_PACKED : LLMQ_W_INT8};
+  const int64_t scale_rows = out_group > 0 ? (w.rows + out_group - 1) / out_group : w.rows;
+  TORCH_CHECK(wscale.size(0) == scale_rows && wscale.size(1) == w.groups, "wscale must be [", scale_rows, ", ", w.groups, "], got [",
+              wscale.size(0), ", ", wscale.size(1), "]");
+  check_int(w.rows, "the weight's rows");
+  check_int(w.groups * w.group_size, "the weight's width");
+  return w;
+}
+
+// gx [rows, groups * keep] of y = x W^T
+at::Tensor wq_linear_grad(const at::Tensor& grad, const at::Tensor& qweight, const at::Tensor& wscale, int64_t out_group,
+                          int64_t keep_per_group) {
+  TORCH_CHECK(grad.is_cuda(), "grad must be a CUDA tensor");
+  const int dtype = dtype_code(grad, "grad");
+  const QuantWeight w = quant_weight(qweight, wscale, out_group, grad);
+  if (keep_per_group <= 0) keep_per_group = w.group_size;
+  TORCH_CHECK(grad.dim() == 2 && grad.size(1) == w.rows, "grad must be [rows, ", w.rows, "]");
+  TORCH_CHECK(keep_per_group <= w.group_size, "keep_per_group must be at most ", w.group_size);
+  const int64_t rows = grad.size(0);
+  check_int(rows, "the number of rows");
+  auto out = at::empty({rows, w.groups * keep_per_group}, grad.options());
+  if (out.numel() == 0) return out;
+  if (w.rows == 0) return out.zero_();
+  const c10::OptionalDeviceGuard guard(at::device_of(grad));
+  const auto gr = own_rows(grad);
+  const size_t need = llmq_wq_linear_grad_workspace_bytes(static_cast<int>(rows), static_cast<int>(w.rows), static_cast<int>(w.groups),
+                                                          static_cast<int>(keep_per_group), dtype);
+  const auto workspace = at::empty({static_cast<int64_t>(need)}, grad.options().dtype(at::kByte));
+  check_rc(llmq_wq_linear_grad(gr.const_data_ptr(), own_stride(gr), qweight.const_data_ptr(), wscale.const_data_ptr<float>(),
+                               out.mutable_data_ptr(), workspace.mutable_data_ptr(), need, static_cast<int>(rows),
+                               static_cast<int>(w.rows), static_cast<int>(w.groups), static_cast<int>(w.group_size),
+                               static_cast<int>(keep_per_group), static_cast<int>(out_group), w.format, dtype, current_stream(grad)),
+           "wq_linear_grad");
+  return out;
+}
+
+// The weight of a vocabulary: dense [vocab, hidden] of hidden's dtype, or codes with their scales.
+struct Vocabulary {
+  int64_t tokens, group_size;
+  int format;
+  const float* scale;
+};
+Vocabulary vocabulary_of(const at::Tensor& hidden, const at::Tensor& weight, const c10::optional<at::Tensor>& wscale, int64_t out_group) {
+  if (wscale.has_value() && wscale->defined()) {
+    const QuantWeight w = quant_weight(weight, *wscale, out_group, hidden);
+    TORCH_CHECK(w.groups * w.group_size == hidden.size(1), "the weight's rows have ", w.groups * w.group_size, " elements, hidden's ", hidden.size(1));
+    return {w.rows, w.group_size, w.format, wscale->const_data_ptr<float>()};
+  }
+  TORCH_CHECK(out_group == 0, "out_group goes with wscale");
+  TORCH_CHECK(weight.device() == hidden.device() && weight.scalar_type() == hidden.scalar_type() && weight.dim() == 2 &&
+                  weight.size(1) == hidden.size(1) && weight.is_contiguous(),
+              "weight must be contiguous [vocab, ", hidden.size(1), "] of hidden's dtype on its device (or codes with wscale)");
+  check_int(weight.size(0), "the vocabulary");
+  return {weight.size(0), 0, 0, nullptr};
+}
+void check_loss_rows(const at::Tensor& hidden, const at::Tensor& targets) {
+  TORCH_CHECK(hidden.is_cuda(), "hidden must be a CUDA tensor");
+  TORCH_CHECK(hidden.dim() == 2, "hidden must be [rows, hidden]");
+  check_int(hidden.size(0), "the number of rows");
+  check_int(hidden.size(1), "the width of hidden");
+  TORCH_CHECK(targets.device() == hidden.device() && targets.scalar_type() == at::kLong && targets.dim() == 1 && targets.size(0) == hidden.size(0),
+              "targets must be int64 [", hidden.size(0), "] on hidden's device");
+}
+at::Tensor float_rows(const at::Tensor& t, const at::Tensor& hidden, const char* name) {
+  TORCH_CHECK(t.device() == hidden.device() && t.scalar_type() == at::kFloat && t.dim() == 1 && t.size(0) == hidden.size(0), name,
+              " must be float32 [", hidden.size(0), "] on hidden's device");
+  return t.contiguous();
+}
+
+// (losses, lse) float32 [rows]
+std::tuple<at::Tensor, at::Tensor> vocab_loss(const at::Tensor& hidden, const at::Tensor& weight, const at::Tensor& targets,
+                                              int64_t ignore_index, const c10::optional<at::Tensor>& wscale, int64_t out_group) {
+  check_loss_rows(hidden, targets);
+  const int dtype = dtype_code(hidden, "hidden");
+  const Vocabulary v = vocabulary_of(hidden, weight, wscale, out_group);
+  const int64_t rows = hidden.size(0);
+  const auto options = hidden.options().dtype(at::kFloat);
+  auto losses = at::empty({rows}, options), lse = at::empty({rows}, options);
+  const c10::OptionalDeviceGuard guard(at::device_of(hidden));
+  const auto hr = own_rows(hidden);
+  const auto wt = packet_rows(weight.reshape({1, weight.numel()}));
+  const auto tr = targets.contiguous();
+  const size_t need = llmq_vocab_loss_workspace_bytes(static_cast<int>(rows), static_cast<int>(v.tokens), static_cast<int>(hidden.size(1)),
+                                                      v.format, dtype);
+  const auto workspace = at::empty({static_cast<int64_t>(need)}, hidden.options().dtype(at::kByte));
+  check_rc(llmq_vocab_loss(hr.const_data_ptr(), own_stride(hr), wt.const_data_ptr(), v.scale, tr.const_data_ptr<int64_t>(), ignore_index,
+                           losses.mutable_data_ptr<float>(), lse.mutable_data_ptr<float>(), workspace.mutable_data_ptr(), need,
+                           static_cast<int>(rows), static_cast<int>(v.tokens), static_cast<int>(hidden.size(1)),
+                           static_cast<int>(v.group_size), static_cast<int>(out_group), v.format, dtype, current_stream(hidden)),
+           "vocab_loss");
+  return {losses, lse};
+}
+
+// (gradient of hidden, gradient of weight or none), from the gradients of the losses
+std::tuple<at::Tensor, c10::optional<at::Tensor>> vocab_loss_grad(const at::Tensor& hidden, const at::Tensor& weight, const at::Tensor& targets,
+                                                                  const at::Tensor& lse, const at::Tensor& grad, int64_t ignore_index,
+                                                                  const c10::optional<at::Tensor>& wscale, int64_t out_group, bool want_weight) {
+  check_loss_rows(hidden, targets);
+  const int dtype = dtype_code(hidden, "hidden");
+  const Vocabulary v = vocabulary_of(hidden, weight, wscale, out_group);
+  TORCH_CHECK(!want_weight || v.format == 0, "a quantized weight has no gradient");
+  const auto ls = float_rows(lse, hidden, "lse"), gr = float_rows(grad, hidden, "grad");
+  const int64_t rows = hidden.size(0);
+  auto grad_hidden = at::empty({rows, hidden.size(1)}, hidden.options());
+  c10::optional<at::Tensor> grad_weight;
+  const c10::OptionalDeviceGuard guard(at::device_of(hidden));
+  if (want_weight) grad_weight = rows == 0 ? at::zeros_like(weight) : at::empty_like(weight);
+  const auto hr = own_rows(hidden);
+  const auto wt = packet_rows(weight.reshape({1, weight.numel()}));
+  const auto tr = targets.contiguous();
+  const size_t need = llmq_vocab_loss_grad_workspace_bytes(static_cast<int>(rows), static_cast<int>(v.tokens), static_cast<int>(hidden.size(1)),
+                                                           v.format, dtype, want_weight);
+  const auto workspace = at::empty({static_cast<int64_t>(need)}, hidden.options().dtype(at::kByte));
+  check_rc(llmq_vocab_loss_grad(hr.const_data_ptr(), own_stride(hr), wt.const_data_ptr(), v.scale, tr.const_data_ptr<int64_t>(), ignore_index,
+                                ls.const_data_ptr<float>(), gr.const_data_ptr<float>(), grad_hidden.mutable_data_ptr(),
+                                want_weight ? grad_weight->mutable_data_ptr() : nullptr, workspace.mutable_data_ptr(), need,
+                                static_cast<int>(rows), static_cast<int>(v.tokens), static_cast<int>(hidden.size(1)),
+                                static_cast<int>(v.group_size), static_cast<int>(out_group), v.format, dtype, current_stream(hidden)),
+           "vocab_loss_grad");
+  return {grad_hidden, grad_weight};
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -1962,5 +2105,13 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         "elements of the int32 zeros tensor argmax_advance_embed takes as workspace");
   m.def("argmax_advance", &argmax_advance, "argmax_row, then token <- index, step64 += 1, step32 += 1",
         py::arg("x"), py::arg("token"), py::arg("step64"), py::arg("step32"));
+  m.def("wq_linear_grad", &wq_linear_grad, "Gradient of a quantized Linear by its input: grad [rows, N] by the weight that codes and scales stand for",
+        py::arg("grad"), py::arg("qweight"), py::arg("wscale"), py::arg("out_group") = 0, py::arg("keep_per_group") = 0);
+  m.def("vocab_loss", &vocab_loss, "Softmax cross entropy of every row over a vocabulary (dense or quantized weight) without the logits: (losses, lse)",
+        py::arg("hidden"), py::arg("weight"), py::arg("targets"), py::arg("ignore_index") = -100, py::arg("wscale") = py::none(),
+        py::arg("out_group") = 0);
+  m.def("vocab_loss_grad", &vocab_loss_grad, "Gradients of vocab_loss by hidden and, where wanted, a dense weight",
+        py::arg("hidden"), py::arg("weight"), py::arg("targets"), py::arg("lse"), py::arg("grad"), py::arg("ignore_index") = -100,
+        py::arg("wscale") = py::none(), py::arg("out_group") = 0, py::arg("want_weight") = false);
   m.def("abi_version", []() { return llmq_abi_version(); });
 }

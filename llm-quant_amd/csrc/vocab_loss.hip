@@ -1,0 +1,450 @@
+// Softmax cross entropy over a vocabulary and its gradient without the logits, gfx950 (no counterpart among the reference's
+// kernels):
+//
+//   l[t, v] = h[t] . W[v]      lse[t] = log sum_v exp l[t, v]      loss[t] = lse[t] - l[t, target[t]]
+//   P[t, v] = (exp(l[t, v] - lse[t]) - [v = target[t]]) g[t]       dh[t] = sum_v P[t, v] W[v]       dW[v] = sum_t P[t, v] h[t]
+//
+// Logits exist as a tile in registers: 256 tokens of the vocabulary by 256 (or 64) rows on the matrix core (dense_tile.h),
+// summed in fp32, of which the largest and the sum of exponentials per row, and the target's own, go to memory: 8 bytes for 256
+// logits. The loss is the log of the sum plus (largest - target's), so that a token that the model is sure of keeps its digits.
+// The gradient goes over pieces of the vocabulary: the tile is multiplied again, and what is written is P of the piece in the type of the
+// call (fp32: three planes), as the operand of the two products behind it. P is rounded to that type, relative to each value; g is scaled
+// by a power of two first, so that a mean over many rows does not leave fp16's range, and the results are scaled back.
+// A quantized head (the model's lm_head) is brought to the values of its dense form piece by piece.
+#include "dense_stage.h"
+
+namespace {
+
+using namespace llmq;
+
+constexpr float kLog2e = 1.4426950408889634f;
+
+struct LossRows {
+  const int64_t* targets;
+  const float* lse;     // gradient
+  const float* grad;    // gradient, scaled; padded with zeros to whole tiles
+  int rows, vocab;
+};
+
+// ---- the loss ---------------------------------------------------------------------------------------------------------------
+template <typename T, int TN, int WM, int WN>
+__global__ __launch_bounds__(WM * WN * kWave) void logits_kernel(const TileOperand weight, const TileOperand hidden, const int k,
+                                                                      const int n_tiles, const int first_token, const int first_tile,
+                                                                      const LossRows rows, float2* __restrict__ stats, float* __restrict__ chosen) {
+  using O = typename TileType<T>::type;
+  using Tile = DenseTile<O, 256, TN, WM, WN>;
+  __shared__ __attribute__((aligned(16))) uint8_t s_mem[Tile::kLdsBytes];
+  const int tile = tile_of_workgroup(blockIdx.x, gridDim.x), n0 = tile % n_tiles * TN, m0 = tile / n_tiles * 256;
+  Tile t;
+  t.template multiply<(TileType<T>::kPlanes == 3 ? 6 : 1)>(s_mem, weight, m0, hidden, n0, 0, k);
+  if (m0 + 256 > weight.rows) {   // (the last tile of the vocabulary)
+#pragma unroll
+    for (int mi = 0; mi < Tile::MI; ++mi)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (m0 + Tile::row_of(mi, i) >= weight.rows) {
+#pragma unroll
+          for (int ni = 0; ni < Tile::NI; ++ni) t.acc[mi][ni][i] = -INFINITY;
+        }
+  }
+  __syncthreads();   // (the stages are free)
+  float2* s_stat = reinterpret_cast<float2*>(s_mem);   // [WM][TN]
+  const int lane = threadIdx.x & (kWave - 1), wm = static_cast<int>(threadIdx.x) / kWave / WN;
+#pragma unroll
+  for (int ni = 0; ni < Tile::NI; ++ni) {
+    const int col = Tile::col_of(ni), n = n0 + col;
+    float top = -INFINITY;
+#pragma unroll
+    for (int mi = 0; mi < Tile::MI; ++mi)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) top = fmaxf(top, t.acc[mi][ni][i]);
+    top = fmaxf(top, __shfl_xor(top, 16));
+    top = fmaxf(top, __shfl_xor(top, 32));
+    const float from = top == -INFINITY ? 0.0f : top;   // (a wave whose tokens all lie past the vocabulary)
+    float sum = 0.0f;
+#pragma unroll
+    for (int mi = 0; mi < Tile::MI; ++mi)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) sum += __builtin_amdgcn_exp2f((t.acc[mi][ni][i] - from) * kLog2e);
+    sum += __shfl_xor(sum, 16);
+    sum += __shfl_xor(sum, 32);
+    if ((lane >> 4) == 0) s_stat[wm * TN + col] = make_float2(top, sum);
+    if (n < rows.rows) {
+      const int64_t at = rows.targets[n] - (first_token + m0);
+      if (at >= 0 && at < 256 && first_token + m0 + at < rows.vocab) {
+#pragma unroll
+        for (int mi = 0; mi < Tile::MI; ++mi)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (Tile::row_of(mi, i) == at) chosen[n] = t.acc[mi][ni][i];
+      }
+    }
+  }
+  __syncthreads();
+  for (int col = threadIdx.x; col < TN && n0 + col < rows.rows; col += Tile::kThreads) {
+    float top = s_stat[col].x;
+#pragma unroll
+    for (int w = 1; w < WM; ++w) top = fmaxf(top, s_stat[w * TN + col].x);
+    const float from = top == -INFINITY ? 0.0f : top;
+    float sum = 0.0f;
+#pragma unroll
+    for (int w = 0; w < WM; ++w) {
+      const float2 s = s_stat[w * TN + col];
+      sum += s.y * __builtin_amdgcn_exp2f(((s.x == -INFINITY ? from : s.x) - from) * kLog2e);
+    }
+    stats[static_cast<int64_t>(first_tile + m0 / 256) * rows.rows + n0 + col] = make_float2(top, sum);
+  }
+}
+
+// 16 rows a workgroup, the tiles dealt to 16 threads each, merged in a fixed order.
+__global__ __launch_bounds__(256) void loss_kernel(const float2* __restrict__ stats, const float* __restrict__ chosen, const int tiles,
+                                                   const LossRows rows, const int64_t ignore_index, float* __restrict__ losses,
+                                                   float* __restrict__ lse) {
+  __shared__ float2 s_part[16][17];
+  const int at = threadIdx.x % 16, part = threadIdx.x / 16, n = blockIdx.x * 16 + at;
+  const bool active = n < rows.rows;
+  float top = -INFINITY, sum = 0.0f;
+  if (active) {
+    for (int i = part; i < tiles; i += 16) {
+      const float2 s = stats[static_cast<int64_t>(i) * rows.rows + n];
+      const float next = fmaxf(top, s.x), from = next == -INFINITY ? 0.0f : next;
+      sum = sum * __builtin_amdgcn_exp2f(((top == -INFINITY ? from : top) - from) * kLog2e) +
+            s.y * __builtin_amdgcn_exp2f(((s.x == -INFINITY ? from : s.x) - from) * kLog2e);
+      top = next;
+    }
+  }
+  s_part[part][at] = make_float2(top, sum);
+  __syncthreads();
+  if (part != 0 || !active) return;
+  top = -INFINITY;
+  for (int p = 0; p < 16; ++p) top = fmaxf(top, s_part[p][at].x);
+  const float from = top == -INFINITY ? 0.0f : top;
+  sum = 0.0f;
+  for (int p = 0; p < 16; ++p) {
+    const float2 s = s_part[p][at];
+    sum += s.y * __builtin_amdgcn_exp2f(((s.x == -INFINITY ? from : s.x) - from) * kLog2e);
+  }
+  const float rest = logf(sum);
+  lse[n] = top + rest;
+  const int64_t target = rows.targets[n];
+  losses[n] = target == ignore_index ? 0.0f
+              : target < 0 || target >= rows.vocab ? NAN : rest + (top - chosen[n]);
+}
+
+// ---- the gradient -----------------------------------------------------------------------------------------------------------
+// scaled[t] = g[t] 2^-e with e the exponent of the largest finite |g| (0 for rows that do not count, and past the end up to
+// `padded`), back = 2^e. One workgroup.
+__global__ __launch_bounds__(1024) void scale_rows_kernel(const float* __restrict__ grad, const int64_t* __restrict__ targets, const int rows,
+                                                          const int padded, const int vocab, const int64_t ignore_index,
+                                                          float* __restrict__ scaled, float* __restrict__ back) {
+  __shared__ float s_top[16];
+  float top = 0.0f;
+  for (int i = threadIdx.x; i < rows; i += 1024) {
+    const float g = fabsf(grad[i]);
+    if (targets[i] != ignore_index && g < INFINITY) top = fmaxf(top, g);
+  }
+  top = group_max<64>(top);
+  if (threadIdx.x % kWave == 0) s_top[threadIdx.x / kWave] = top;
+  __syncthreads();
+  top = s_top[0];
+  for (int w = 1; w < 16; ++w) top = fmaxf(top, s_top[w]);
+  const int e = top > 0.0f ? min(max(ilogbf(top), -125), 125) : 0;
+  for (int i = threadIdx.x; i < padded; i += 1024) {
+    float g = 0.0f;
+    if (i < rows && targets[i] != ignore_index) g = targets[i] < 0 || targets[i] >= vocab ? NAN : ldexpf(grad[i], -e);
+    scaled[i] = g;
+  }
+  if (threadIdx.x == 0) *back = ldexpf(1.0f, e);
+}
+
+struct PieceOut {
+  void* p;             // [rows, ld] a plane
+  void* p_t;           // or null: [tokens of the piece, ld_t] a plane
+  int64_t plane, plane_t;
+  int ld, ld_t;
+};
+
+template <typename T, int TN, int WM, int WN>
+__global__ __launch_bounds__(WM * WN * kWave) void piece_kernel(const TileOperand weight, const TileOperand hidden, const int k,
+                                                                     const int n_tiles, const int first_token, const LossRows rows, const PieceOut out) {
+  using O = typename TileType<T>::type;
+  constexpr int P = TileType<T>::kPlanes;
+  using Tile = DenseTile<O, 256, TN, WM, WN>;
+  __shared__ __attribute__((aligned(16))) uint8_t s_mem[Tile::kLdsBytes];
+  const int tile = tile_of_workgroup(blockIdx.x, gridDim.x), n0 = tile % n_tiles * TN, m0 = tile / n_tiles * 256;
+  Tile t;
+  t.template multiply<(P == 3 ? 6 : 1)>(s_mem, weight, m0, hidden, n0, 0, k);
+#pragma unroll
+  for (int ni = 0; ni < Tile::NI; ++ni) {
+    const int n = n0 + Tile::col_of(ni);
+    const bool real = n < rows.rows;
+    const float g = real ? rows.grad[n] : 0.0f, lse = real ? rows.lse[n] : 0.0f;
+    const int64_t target = real ? rows.targets[n] - (first_token + m0) : -1;   // within the tile
+#pragma unroll
+    for (int mi = 0; mi < Tile::MI; ++mi) {
+      float f[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int m = Tile::row_of(mi, i);
+        const float e = __builtin_amdgcn_exp2f((t.acc[mi][ni][i] - lse) * kLog2e) - (target == m ? 1.0f : 0.0f);
+        f[i] = g == 0.0f || m0 + m >= weight.rows ? 0.0f : e * g;   // (a row that does not count may hold anything)
+      }
+      uint16_t v[P][4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if constexpr (P == 1) {
+          v[0][i] = __builtin_bit_cast(uint16_t, from_float<O>(f[i]));
+        } else {
+          uint16_t p[3];
+          planes_of(f[i], p);
+#pragma unroll
+          for (int j = 0; j < P; ++j) v[j][i] = p[j];
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < P; ++j) {
+        const u32x2 w{v[j][0] | static_cast<uint32_t>(v[j][1]) << 16, v[j][2] | static_cast<uint32_t>(v[j][3]) << 16};
+        if (real) *reinterpret_cast<u32x2*>(static_cast<uint16_t*>(out.p) + j * out.plane + static_cast<int64_t>(n) * out.ld + m0 + Tile::row_of(mi, 0)) = w;
+        if (out.p_t != nullptr && n < out.ld_t) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            static_cast<uint16_t*>(out.p_t)[j * out.plane_t + static_cast<int64_t>(m0 + Tile::row_of(mi, i)) * out.ld_t + n] = v[j][i];
+        }
+      }
+    }
+  }
+}
+
+// ---- what a call takes --------------------------------------------------------------------------------------------------------
+struct Plan {
+  int rows, vocab, hidden, planes, size;   // size: bytes of an element of the call's type
+  int k;                                   // hidden, in whole steps
+  int padded;                              // rows, in whole tiles
+  bool stage_hidden, stage_weight;         // whether they have to be brought into operand form
+  int piece;                               // tokens of a piece, a multiple of 256
+  int splits;                              // of dh's products
+  // offsets into the workspace
+  int64_t o_stats, o_chosen, o_hidden, o_weight, o_scaled, o_back, o_hidden_t, o_weight_t, o_p, o_p_t, o_sums, bytes;
+};
+
+int64_t take(int64_t& at, int64_t bytes) {
+  const int64_t here = at;
+  at = round_up(at + bytes, 256);
+  return here;
+}
+
+// The piece of the vocabulary: a whole number of rounds of 256 workgroups' tiles where that is no more than what the workspace for pieces
+// (kPieceBytes) holds.
+constexpr int64_t kPieceBytes = int64_t{512} << 20;
+
+Plan plan_for(int rows, int vocab, int hidden, int wformat, int dtype, bool gradient, bool learned) {
+  Plan p{};
+  p.rows = rows;
+  p.vocab = vocab;
+  p.hidden = hidden;
+  p.planes = dtype == LLMQ_F32 ? 3 : 1;
+  p.size = dtype == LLMQ_F32 ? 4 : 2;
+  p.k = static_cast<int>(round_up(hidden, 64));
+  const int tn = tile_rows(rows);
+  p.padded = static_cast<int>(round_up(rows, tn));
+  p.stage_hidden = p.planes > 1 || hidden % 64 != 0;
+  p.stage_weight = p.stage_hidden || wformat != 0;
+  const int64_t row16 = int64_t{2} * p.planes;   // bytes of a value in operand form
+  const int64_t whole = round_up(vocab, 256);
+  int64_t per_token = p.stage_weight ? p.k * row16 : 0;
+  if (gradient) per_token += hidden * row16 + rows * row16 + (learned ? p.padded * row16 : 0);
+  int64_t piece = whole;
+  if (per_token > 0) {
+    const int64_t n_tiles = p.padded / tn, round = n_tiles >= 256 ? 256 : 256 / n_tiles * 256;   // tokens of a round of workgroups
+    piece = kPieceBytes / per_token / 256 * 256;
+    if (piece > round) piece = piece / round * round;
+    if (piece < 256) piece = 256;
+    if (piece > whole) piece = whole;
+  }
+  p.piece = static_cast<int>(piece);
+  int64_t at = 0;
+  if (p.stage_hidden) p.o_hidden = take(at, p.rows * p.k * row16);
+  if (p.stage_weight) p.o_weight = take(at, piece * p.k * row16);
+  if (!gradient) {
+    p.o_stats = take(at, whole / 256 * rows * 8);
+    p.o_chosen = take(at, int64_t{4} * rows);
+  } else {
+    p.splits = splits_for(hidden, rows, static_cast<int>(piece));
+    p.o_scaled = take(at, int64_t{4} * p.padded);
+    p.o_back = take(at, 4);
+    p.o_weight_t = take(at, hidden * piece * row16);
+    p.o_p = take(at, rows * piece * row16);
+    if (learned) {
+      p.o_hidden_t = take(at, hidden * round_up(rows, 64) * row16);
+      p.o_p_t = take(at, piece * round_up(rows, 64) * row16);
+    }
+    p.o_sums = take(at, int64_t{4} * p.splits * rows * hidden);
+  }
+  p.bytes = at;
+  return p;
+}
+
+int check(int rows, int vocab, int hidden, int group_size, int out_group, int wformat, int dtype, int64_t hidden_stride) {
+  if (rows < 0 || vocab < 0 || hidden <= 0) return llmq_host::fail_invalid("bad dimension rows=%d vocab=%d hidden=%d", rows, vocab, hidden);
+  if (dtype != LLMQ_F32 && dtype != LLMQ_F16 && dtype != LLMQ_BF16)
+    return llmq_host::fail_invalid("dtype code %d is not float32, float16 or bfloat16", dtype);
+  if (wformat != 0 && wformat != LLMQ_W_INT8 && wformat != LLMQ_W_INT4_PACKED)
+    return llmq_host::fail_invalid("unsupported weight format %d, expected 0 (dense), 8 or 4", wformat);
+  if (hidden % 8) return llmq_host::fail_invalid("hidden must be a multiple of 8, got %d", hidden);
+  if (hidden > 65536) return llmq_host::fail_invalid("hidden must be at most 65536, got %d", hidden);
+  if (wformat != 0 && (group_size <= 0 || group_size % 8 || hidden % group_size))
+    return llmq_host::fail_invalid("group_size must be a positive multiple of 8 that divides hidden=%d, got %d", hidden, group_size);
+  if (out_group < 0) return llmq_host::fail_invalid("out_group must be >= 0, got %d", out_group);
+  if (hidden_stride < hidden || hidden_stride % 8)
+    return llmq_host::fail_invalid("hidden's row stride must be a multiple of 8 of at least hidden=%d, got %lld", hidden, static_cast<long long>(hidden_stride));
+  if (rows > (1 << 20) || vocab > (1 << 24)) return llmq_host::fail_invalid("at most 2^20 rows and 2^24 tokens, got %d and %d", rows, vocab);
+  return 0;
+}
+
+struct Call {
+  const void* hidden;
+  const void* weight;
+  const float* wscale;
+  int64_t hidden_stride;
+  int group_size, out_group, wformat;
+  uint8_t* workspace;
+  hipStream_t stream;
+};
+
+template <typename T> TileOperand hidden_operand(const Plan& p, const Call& c) {
+  if (!p.stage_hidden) return TileOperand{c.hidden, 0, static_cast<uint32_t>(c.hidden_stride * 2), p.rows};
+  return TileOperand{c.workspace + p.o_hidden, int64_t{2} * p.rows * p.k, static_cast<uint32_t>(p.k) * 2, p.rows};
+}
+StageSource hidden_source(const Plan& p, const Call& c, const float* keep) {
+  return StageSource{c.hidden, nullptr, keep, c.hidden_stride, p.rows, p.hidden, 0, p.rows, 0, 0, 0, 0};
+}
+StageSource weight_source(const Plan& p, const Call& c, int first, int tokens) {
+  const int groups = c.wformat ? p.hidden / c.group_size : 0;
+  return StageSource{c.weight, c.wscale, nullptr, p.hidden, p.vocab, p.hidden, first, tokens, groups, c.group_size, c.group_size, c.out_group};
+}
+TileOperand weight_operand(const Plan& p, const Call& c, int first, int tokens) {
+  if (!p.stage_weight) return TileOperand{static_cast<const uint8_t*>(c.weight) + int64_t{2} * first * p.hidden, 0, static_cast<uint32_t>(p.hidden) * 2, tokens};
+  return TileOperand{c.workspace + p.o_weight, int64_t{2} * p.piece * p.k, static_cast<uint32_t>(p.k) * 2, tokens};
+}
+
+template <typename T> int forward(const Plan& p, const Call& c, const int64_t* targets, int64_t ignore_index, float* losses, float* lse) {
+  if (p.stage_hidden)
+    stage_launch<T>(hidden_source(p, c, nullptr), StageTarget{c.workspace + p.o_hidden, nullptr, int64_t{p.rows} * p.k, 0, p.k, 0}, 0, c.stream);
+  const TileOperand hidden = hidden_operand<T>(p, c);
+  const LossRows rows{targets, nullptr, nullptr, p.rows, p.vocab};
+  float2* stats = reinterpret_cast<float2*>(c.workspace + p.o_stats);
+  float* chosen = reinterpret_cast<float*>(c.workspace + p.o_chosen);
+  const int tn = tile_rows(p.rows), n_tiles = p.padded / tn;
+  for (int first = 0; first < p.vocab; first += p.piece) {
+    const int tokens = p.vocab - first < p.piece ? p.vocab - first : p.piece;
+    if (p.stage_weight)
+      stage_launch<T>(weight_source(p, c, first, tokens), StageTarget{c.workspace + p.o_weight, nullptr, int64_t{p.piece} * p.k, 0, p.k, 0}, c.wformat, c.stream);
+    const TileOperand weight = weight_operand(p, c, first, tokens);
+    const dim3 grid(static_cast<unsigned>((tokens + 255) / 256) * n_tiles);
+    if (tn == kFewRows)
+      hipLaunchKernelGGL((logits_kernel<T, 64, 4, 2>), grid, dim3(512), 0, c.stream, weight, hidden, p.k, n_tiles, first, first / 256, rows, stats, chosen);
+    else
+      hipLaunchKernelGGL((logits_kernel<T, 256, 2, 4>), grid, dim3(512), 0, c.stream, weight, hidden, p.k, n_tiles, first, first / 256, rows, stats, chosen);
+  }
+  hipLaunchKernelGGL(loss_kernel, dim3((p.rows + 15) / 16), dim3(256), 0, c.stream, stats, chosen, (p.vocab + 255) / 256, rows, ignore_index, losses, lse);
+  return llmq_host::check_launch("vocab_loss");
+}
+
+template <typename T>
+int backward(const Plan& p, const Call& c, const int64_t* targets, int64_t ignore_index, const float* lse, const float* grad, void* grad_hidden,
+             void* grad_weight) {
+  float* scaled = reinterpret_cast<float*>(c.workspace + p.o_scaled);
+  float* back = reinterpret_cast<float*>(c.workspace + p.o_back);
+  float* sums = reinterpret_cast<float*>(c.workspace + p.o_sums);
+  const bool learned = grad_weight != nullptr;
+  const int64_t rows64 = round_up(p.rows, 64);
+  hipLaunchKernelGGL(scale_rows_kernel, dim3(1), dim3(1024), 0, c.stream, grad, targets, p.rows, p.padded, p.vocab, ignore_index, scaled, back);
+  if (p.stage_hidden || learned)
+    stage_launch<T>(hidden_source(p, c, scaled),
+                    StageTarget{p.stage_hidden ? c.workspace + p.o_hidden : nullptr, learned ? c.workspace + p.o_hidden_t : nullptr,
+                                int64_t{p.rows} * p.k, p.hidden * rows64, p.k, static_cast<int>(rows64)}, 0, c.stream);
+  const TileOperand hidden = hidden_operand<T>(p, c);
+  const LossRows rows{targets, lse, scaled, p.rows, p.vocab};
+  const int tn = tile_rows(p.rows), n_tiles = p.padded / tn;
+  for (int first = 0; first < p.vocab; first += p.piece) {
+    const int tokens = p.vocab - first < p.piece ? p.vocab - first : p.piece, tokens64 = static_cast<int>(round_up(tokens, 64));
+    stage_launch<T>(weight_source(p, c, first, tokens),
+                    StageTarget{p.stage_weight ? c.workspace + p.o_weight : nullptr, c.workspace + p.o_weight_t, int64_t{p.piece} * p.k,
+                                int64_t{p.hidden} * p.piece, p.k, p.piece}, c.wformat, c.stream);
+    const TileOperand weight = weight_operand(p, c, first, tokens);
+    const PieceOut piece{c.workspace + p.o_p, learned ? c.workspace + p.o_p_t : nullptr, int64_t{p.rows} * p.piece, p.piece * rows64, p.piece,
+                         static_cast<int>(rows64)};
+    const dim3 grid(static_cast<unsigned>((tokens + 255) / 256) * n_tiles);
+    if (tn == kFewRows)
+      hipLaunchKernelGGL((piece_kernel<T, 64, 4, 2>), grid, dim3(512), 0, c.stream, weight, hidden, p.k, n_tiles, first, rows, piece);
+    else
+      hipLaunchKernelGGL((piece_kernel<T, 256, 2, 4>), grid, dim3(512), 0, c.stream, weight, hidden, p.k, n_tiles, first, rows, piece);
+    const TileOperand weight_t{c.workspace + p.o_weight_t, int64_t{2} * p.hidden * p.piece, static_cast<uint32_t>(p.piece) * 2, p.hidden};
+    const TileOperand part{c.workspace + p.o_p, int64_t{2} * p.rows * p.piece, static_cast<uint32_t>(p.piece) * 2, p.rows};
+    product_launch<T, true>(weight_t, part, tokens64, ProductOut{sums, int64_t{p.rows} * p.hidden, p.hidden, nullptr, first == 0}, p.splits, c.stream);
+    if (learned) {
+      const TileOperand hidden_t{c.workspace + p.o_hidden_t, 2 * p.hidden * rows64, static_cast<uint32_t>(rows64) * 2, p.hidden};
+      const TileOperand part_t{c.workspace + p.o_p_t, 2 * p.piece * rows64, static_cast<uint32_t>(rows64) * 2, tokens};
+      product_launch<T, false>(hidden_t, part_t, static_cast<int>(rows64),
+                               ProductOut{static_cast<T*>(grad_weight) + static_cast<int64_t>(first) * p.hidden, 0, p.hidden, back, 0}, 1, c.stream);
+    }
+  }
+  add_planes_launch<T>(sums, int64_t{p.rows} * p.hidden, p.splits, back, grad_hidden, int64_t{p.rows} * p.hidden, c.stream);
+  return llmq_host::check_launch("vocab_loss_grad");
+}
+
+bool misaligned(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) != 0; }
+
+}  // namespace
+
+extern "C" size_t llmq_vocab_loss_workspace_bytes(int rows, int vocab, int hidden, int wformat, int dtype) {
+  if (rows <= 0 || vocab <= 0 || hidden <= 0) return 0;
+  return static_cast<size_t>(plan_for(rows, vocab, hidden, wformat, dtype, false, false).bytes);
+}
+extern "C" size_t llmq_vocab_loss_grad_workspace_bytes(int rows, int vocab, int hidden, int wformat, int dtype, int want_weight) {
+  if (rows <= 0 || vocab <= 0 || hidden <= 0) return 0;
+  return static_cast<size_t>(plan_for(rows, vocab, hidden, wformat, dtype, true, want_weight != 0).bytes);
+}
+
+extern "C" int llmq_vocab_loss(const void* hidden, int64_t hidden_stride, const void* weight, const float* wscale_or_null,
+                               const int64_t* targets, int64_t ignore_index, float* losses, float* lse, void* workspace,
+                               size_t workspace_bytes, int rows, int vocab, int hidden_size, int group_size, int out_group,
+                               int wformat, int dtype, llmq_stream_t stream) {
+  if (int rc = check(rows, vocab, hidden_size, group_size, out_group, wformat, dtype, hidden_stride)) return rc;
+  if (rows == 0) return 0;
+  if (vocab == 0) return llmq_host::fail_invalid("a vocabulary of no tokens");
+  if (!hidden || !weight || !targets || !losses || !lse || (wformat != 0 && !wscale_or_null)) return llmq_host::fail_invalid("null tensor pointer");
+  if (misaligned(hidden) || misaligned(weight)) return llmq_host::fail_invalid("hidden and weight must be 16-byte aligned");
+  const Plan p = plan_for(rows, vocab, hidden_size, wformat, dtype, false, false);
+  if (!workspace || misaligned(workspace) || workspace_bytes < static_cast<size_t>(p.bytes))
+    return llmq_host::fail_invalid("the workspace must be 16-byte aligned and hold %lld bytes, got %zu", static_cast<long long>(p.bytes), workspace_bytes);
+  const Call c{hidden, weight, wscale_or_null, hidden_stride, group_size, out_group, wformat, static_cast<uint8_t*>(workspace), static_cast<hipStream_t>(stream)};
+  switch (dtype) {
+    case LLMQ_F32: return forward<float>(p, c, targets, ignore_index, losses, lse);
+    case LLMQ_F16: return forward<f16_t>(p, c, targets, ignore_index, losses, lse);
+    default: return forward<bf16_t>(p, c, targets, ignore_index, losses, lse);
+  }
+}
+
+extern "C" int llmq_vocab_loss_grad(const void* hidden, int64_t hidden_stride, const void* weight, const float* wscale_or_null,
+                                    const int64_t* targets, int64_t ignore_index, const float* lse, const float* grad, void* grad_hidden,
+                                    void* grad_weight_or_null, void* workspace, size_t workspace_bytes, int rows, int vocab, int hidden_size,
+                                    int group_size, int out_group, int wformat, int dtype, llmq_stream_t stream) {
+  if (int rc = check(rows, vocab, hidden_size, group_size, out_group, wformat, dtype, hidden_stride)) return rc;
+  if (wformat != 0 && grad_weight_or_null) return llmq_host::fail_invalid("a quantized weight has no gradient");
+  if (rows == 0) return 0;   // (nothing is written: a gradient of no rows has no elements but the weight's, which the caller clears)
+  if (vocab == 0) return llmq_host::fail_invalid("a vocabulary of no tokens");
+  if (!hidden || !weight || !targets || !lse || !grad || !grad_hidden || (wformat != 0 && !wscale_or_null))
+    return llmq_host::fail_invalid("null tensor pointer");
+  if (misaligned(hidden) || misaligned(weight) || misaligned(grad_hidden) || misaligned(grad_weight_or_null))
+    return llmq_host::fail_invalid("hidden, weight and their gradients must be 16-byte aligned");
+  const Plan p = plan_for(rows, vocab, hidden_size, wformat, dtype, true, grad_weight_or_null != nullptr);
+  if (!workspace || misaligned(workspace) || workspace_bytes < static_cast<size_t>(p.bytes))
+    return llmq_host::fail_invalid("the workspace must be 16-byte aligned and hold %lld bytes, got %zu", static_cast<long long>(p.bytes), workspace_bytes);
+  const Call c{hidden, weight, wscale_or_null, hidden_stride, group_size, out_group, wformat, static_cast<uint8_t*>(workspace), static_cast<hipStream_t>(stream)};
+  switch (dtype) {
+    case LLMQ_F32: return backward<float>(p, c, targets, ignore_index, lse, grad, grad_hidden, grad_weight_or_null);
+    case LLMQ_F16: return backward<f16_t>(p, c, targets, ignore_index, lse, grad, grad_hidden, grad_weight_or_null);
+    default: return backward<bf16_t>(p, c, targets, ignore_index, lse, grad, grad_hidden, grad_weight_or_null);
+  }
+}

@@ -1,0 +1,105 @@
+// The gradient of a quantized Linear by its input, gfx950:
+//
+//   gx[t, k] = sum_n g[t, n] W[n, k],     W = (dtype)(code * scale): the matrix of the reference's many-rows branch
+//                                         (llmquant/quantizers/kernel.py:68-79), whose autograd this stands for
+//
+// The weight is brought, transposed, into operand form a piece of its columns at a time (dense_stage.h), and multiplied on the
+// matrix core (dense_tile.h). Bound: the matrix core for training batches, the weight's way through memory for few rows.
+#include "dense_stage.h"
+
+namespace {
+
+using namespace llmq;
+
+struct Plan {
+  int64_t n_padded, piece;   // N in whole steps; columns of W a piece
+  int splits;
+  bool stage_grad;
+  int64_t o_weight, o_grad, o_sums, bytes;
+};
+
+constexpr int64_t kPieceBytes = int64_t{256} << 20;
+
+Plan plan_for(int rows, int N, int width, int dtype) {
+  Plan p{};
+  const int64_t row16 = dtype == LLMQ_F32 ? 6 : 2;
+  p.n_padded = round_up(N, 64);
+  p.stage_grad = dtype == LLMQ_F32 || N % 64 != 0;
+  p.piece = kPieceBytes / (p.n_padded * row16) / 256 * 256;
+  if (p.piece < 256) p.piece = 256;
+  if (p.piece > width) p.piece = width;
+  p.splits = splits_for(static_cast<int>(p.piece), rows, static_cast<int>(p.n_padded));
+  int64_t at = round_up(p.piece * p.n_padded * row16, 256);
+  if (p.stage_grad) {
+    p.o_grad = at;
+    at += round_up(rows * p.n_padded * row16, 256);
+  }
+  if (p.splits > 1) {
+    p.o_sums = at;
+    at += round_up(int64_t{4} * p.splits * rows * width, 256);
+  }
+  p.bytes = at;
+  return p;
+}
+
+template <typename T>
+void launch(const Plan& p, const void* grad, int64_t stride, const void* qweight, const float* wscale, void* out, uint8_t* workspace, int rows,
+            int N, int G, int gs, int keep, int out_group, int wformat, hipStream_t stream) {
+  const int width = G * keep, n64 = static_cast<int>(p.n_padded);
+  if (p.stage_grad)
+    stage_launch<T>(StageSource{grad, nullptr, nullptr, stride, rows, N, 0, rows, 0, 0, 0, 0},
+                    StageTarget{workspace + p.o_grad, nullptr, rows * p.n_padded, 0, n64, 0}, 0, stream);
+  const TileOperand b = p.stage_grad ? TileOperand{workspace + p.o_grad, 2 * rows * p.n_padded, static_cast<uint32_t>(n64) * 2, rows}
+                                     : TileOperand{grad, 0, static_cast<uint32_t>(stride) * 2, rows};
+  float* sums = reinterpret_cast<float*>(workspace + p.o_sums);
+  for (int first = 0; first < width; first += static_cast<int>(p.piece)) {
+    const int cols = width - first < p.piece ? width - first : static_cast<int>(p.piece);
+    StageSource src{qweight, wscale, nullptr, 0, N, cols, 0, N, G, gs, keep, out_group};
+    src.first_col = first;
+    stage_launch<T>(src, StageTarget{nullptr, workspace, 0, p.piece * p.n_padded, 0, n64}, wformat, stream);
+    const TileOperand a{workspace, 2 * p.piece * p.n_padded, static_cast<uint32_t>(n64) * 2, cols};
+    if (p.splits > 1) product_launch<T, true>(a, b, n64, ProductOut{sums + first, static_cast<int64_t>(rows) * width, width, nullptr, 1}, p.splits, stream);
+    else product_launch<T, false>(a, b, n64, ProductOut{static_cast<T*>(out) + first, 0, width, nullptr, 1}, 1, stream);
+  }
+  if (p.splits > 1) add_planes_launch<T>(sums, static_cast<int64_t>(rows) * width, p.splits, nullptr, out, static_cast<int64_t>(rows) * width, stream);
+}
+
+}  // namespace
+
+extern "C" size_t llmq_wq_linear_grad_workspace_bytes(int rows, int N, int G, int keep_per_group, int dtype) {
+  if (rows <= 0 || N <= 0 || G <= 0 || keep_per_group <= 0) return 0;
+  return static_cast<size_t>(plan_for(rows, N, G * keep_per_group, dtype).bytes);
+}
+
+extern "C" int llmq_wq_linear_grad(const void* grad, int64_t grad_stride, const void* qweight, const float* wscale, void* grad_x,
+                                   void* workspace, size_t workspace_bytes, int rows, int N, int G, int gs, int keep_per_group,
+                                   int out_group, int wformat, int dtype, llmq_stream_t stream) {
+  if (rows < 0 || N < 0 || G < 0) return llmq_host::fail_invalid("negative dimension rows=%d N=%d G=%d", rows, N, G);
+  if (wformat != LLMQ_W_INT8 && wformat != LLMQ_W_INT4_PACKED) return llmq_host::fail_invalid("unsupported weight format %d, expected 8 or 4", wformat);
+  if (gs <= 0 || gs % 8) return llmq_host::fail_invalid("group_size must be a positive multiple of 8, got %d", gs);
+  if (keep_per_group <= 0 || keep_per_group > gs || keep_per_group % 8)
+    return llmq_host::fail_invalid("keep_per_group must be a multiple of 8 up to %d, got %d", gs, keep_per_group);
+  if (out_group < 0) return llmq_host::fail_invalid("out_group must be >= 0, got %d", out_group);
+  if (dtype != LLMQ_F32 && dtype != LLMQ_F16 && dtype != LLMQ_BF16)
+    return llmq_host::fail_invalid("dtype code %d is not float32, float16 or bfloat16", dtype);
+  if (N % 8) return llmq_host::fail_invalid("the weight's rows must be a multiple of 8, got %d", N);
+  if (rows == 0 || G == 0) return 0;
+  if (N == 0) return llmq_host::fail_invalid("a weight of no rows");
+  if (rows > (1 << 20) || N > (1 << 24) || static_cast<int64_t>(G) * keep_per_group > (1 << 24))
+    return llmq_host::fail_invalid("at most 2^20 rows of 2^24 elements, got %d rows, %d x %lld", rows, N, static_cast<long long>(G) * keep_per_group);
+  if (grad_stride < N || grad_stride % 8 || grad_stride > (1 << 24)) return llmq_host::fail_invalid("grad's row stride must be a multiple of 8 of at least %d, got %lld", N, static_cast<long long>(grad_stride));
+  if (!grad || !qweight || !wscale || !grad_x) return llmq_host::fail_invalid("null tensor pointer");
+  if ((reinterpret_cast<uintptr_t>(grad) | reinterpret_cast<uintptr_t>(qweight) | reinterpret_cast<uintptr_t>(grad_x)) & 15u)
+    return llmq_host::fail_invalid("grad, qweight and grad_x must be 16-byte aligned");
+  const Plan p = plan_for(rows, N, G * keep_per_group, dtype);
+  if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 15u) || workspace_bytes < static_cast<size_t>(p.bytes))
+    return llmq_host::fail_invalid("the workspace must be 16-byte aligned and hold %lld bytes, got %zu", static_cast<long long>(p.bytes), workspace_bytes);
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  switch (dtype) {
+    case LLMQ_F32: launch<float>(p, grad, grad_stride, qweight, wscale, grad_x, ws, rows, N, G, gs, keep_per_group, out_group, wformat, s); break;
+    case LLMQ_F16: launch<f16_t>(p, grad, grad_stride, qweight, wscale, grad_x, ws, rows, N, G, gs, keep_per_group, out_group, wformat, s); break;
+    default: launch<bf16_t>(p, grad, grad_stride, qweight, wscale, grad_x, ws, rows, N, G, gs, keep_per_group, out_group, wformat, s); break;
+  }
+  return llmq_host::check_launch("wq_linear_grad");
+}
