@@ -623,6 +623,35 @@ int llmq_vocab_loss_grad(const void* hidden, int64_t hidden_stride, const void* 
                          void* grad_weight_or_null, void* workspace, size_t workspace_bytes, int rows, int vocab,
                          int hidden_size, int group_size, int out_group, int wformat, int dtype, llmq_stream_t stream);
 
+/* Low-rank adapters of many requests beside a shared projection (no counterpart in the reference). For row t of sequence b with a =
+ * adapter[b] (int32; outside [0, slots): no adapter):
+ *   low[t] = x[t] lora_a[a]^T        out[t] = base[t] + scaling[a] low[t] lora_b[a]^T        out[t] = base[t] without an adapter
+ * x [rows, in], base [rows, out] (row strides in elements), out [rows, out] contiguous, which may be base itself; lora_a [slots, rank, in],
+ * lora_b [slots, out, rank] of `dtype`; scaling fp32 [slots]. The rows of sequence b are query_start[b] .. query_start[b + 1] - 1 (int32
+ * [sequences + 1], not decreasing; NULL: row b, rows == sequences); rows of no sequence are base. low_or_null: fp32 [rows, rank],
+ * zeros without an adapter; the gradient wants it. Sums in fp32, out rounded once; for 16-bit types low enters the second product as
+ * two bfloat16 (16 bits of it). rank a multiple of 8 from 8 to 128 (an adapter of a lower rank has zeros behind it), in and out
+ * multiples of 8; tensors 16-byte aligned. workspace: ..._workspace_bytes(...) bytes (ragged: whether there is a query_start),
+ * 16-byte aligned, needs no clearing; calls that overlap in time need one each.
+ *
+ * llmq_lora_grad: from grad, the gradient of out,
+ *   du[t] = scaling[a] grad[t] lora_b[a]    grad_x[t] = grad_base[t] + du[t] lora_a[a]    (grad_base NULL: zeros)
+ *   grad_a[a] = sum_t du[t]^T x[t]          grad_b[a] = scaling[a] sum_t grad[t]^T low[t]
+ * in full: zeros for slots without rows. x as lora_add had it, or (x_scale) its int8 codes [rows, in] with fp32 scales [rows, in / 128] as
+ * llmq_quant_group_codes writes them: an activation kept in 8 bits for the backward pass. At most 1024 slots. grad_x
+ * contiguous; the outputs share no memory with the inputs. The gradient of base is grad. */
+size_t llmq_lora_add_workspace_bytes(int rows, int sequences, int ragged, int in_features, int rank, int dtype);
+int llmq_lora_add(const void* x, int64_t x_stride, const void* base, int64_t base_stride, const void* lora_a, const void* lora_b,
+                  const float* scaling, const int32_t* adapter, const int32_t* query_start_or_null, void* out, float* low_or_null,
+                  void* workspace, size_t workspace_bytes, int rows, int sequences, int in_features, int out_features, int rank,
+                  int slots, int dtype, llmq_stream_t stream);
+size_t llmq_lora_grad_workspace_bytes(int rows, int sequences, int ragged, int in_features, int out_features, int rank, int slots, int dtype);
+int llmq_lora_grad(const void* grad, int64_t grad_stride, const void* x, int64_t x_stride, const float* x_scale_or_null, const float* low,
+                   const void* lora_a, const void* lora_b, const float* scaling, const int32_t* adapter,
+                   const int32_t* query_start_or_null, const void* grad_base_or_null, int64_t base_stride, void* grad_x, void* grad_a,
+                   void* grad_b, void* workspace, size_t workspace_bytes, int rows, int sequences, int in_features,
+                   int out_features, int rank, int slots, int dtype, llmq_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,852 @@
+// Low-rank adapters of many requests beside a shared projection, and their gradients, gfx950 (no counterpart among the
+// reference's kernels). For row t of request b with adapter a = adapter[b], A[a] [rank, in], B[a] [out, rank], scaling s[a]:
+//
+//   low[t] = x[t] A[a]^T          out[t] = base[t] + s[a] low[t] B[a]^T
+//   du[t] = s[a] g[t] B[a]        gx[t] = gbase[t] + du[t] A[a]     gA[a] = sum_t du[t]^T x[t]     gB[a] = s[a] sum_t g[t]^T low[t]
+//
+// shrink   rows by a bank's rows: the reduction is long (in, or out), the result 8 to 128 wide. A workgroup takes a piece of one
+//          request's rows and a part of the reduction, its waves parts of that; sums of the parts go to memory, one plane a part.
+// expand   adds the planes up and multiplies by the other factor into the projection's output: a wave has 64 columns at a time.
+// outer    gradients of the bank: the reduction is over rows, which are sorted by adapter (plan) in blocks of 32. Both operands lie
+//          with the reduction outermost; a lane loads eight columns of its eight rows and turns them over in registers.
+// All on the matrix core in fp32 sums. The 8 to 128 numbers in between stay fp32 in memory; as operands they are
+// two bfloat16 (16 bits of them), against bfloat16 values as they are, fp16 values as two bfloat16 (exact), fp32 on the fp32
+// matrix instructions. Rounded once, at the end. Every sum has a fixed order.
+//
+// Bound: HBM for prompts and training (x, base and out once each); the chain of a launch for single tokens.
+#include "dense_tile.h"
+#include "kv_blocks.h"
+
+namespace {
+
+using namespace llmq;
+
+typedef tile_v4f v4f;
+
+struct Bank {
+  const void* m;      // [slots, rows of a slot, width]
+  int slots, rank;
+  int width;
+};
+struct Requests {
+  const int32_t* adapter;
+  Ragged rows;
+  // The rows of piece `slot` (of 16 NT rows, or one row a request) and their adapter; no rows: nobody's.
+  template <int SHIFT> __device__ __forceinline__ int piece(int slot, int slots, int& first, int& n) const {
+    int a = -1;
+    if (rows.start == nullptr) {
+      first = slot;
+      n = 1;
+      a = adapter[slot];
+    } else {
+      Span span;
+      const int b = rows.find(SHIFT, adapter, slot, span, a);
+      (void)b;
+      first = span.first + (slot << SHIFT);
+      n = min(span.n - (slot << SHIFT), 1 << SHIFT);
+    }
+    return a >= 0 && a < slots ? a : -1;
+  }
+};
+
+template <int NT> constexpr int kPieceShift = NT == 4 ? 6 : NT == 2 ? 5 : 4;
+
+__device__ __forceinline__ v4f mfma_f32(float a, float b, v4f c) { return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0); }
+template <typename T> __device__ __forceinline__ v4f mfma_packet(u32x4 a, u32x4 b, v4f c) { return mfma_16x16x32<T>(a, b, c); }
+template <> __device__ __forceinline__ v4f mfma_packet<float>(u32x4 a, u32x4 b, v4f c) {
+  c = mfma_f32(__builtin_bit_cast(float, a.x), __builtin_bit_cast(float, b.x), c);
+  c = mfma_f32(__builtin_bit_cast(float, a.y), __builtin_bit_cast(float, b.y), c);
+  c = mfma_f32(__builtin_bit_cast(float, a.z), __builtin_bit_cast(float, b.z), c);
+  return mfma_f32(__builtin_bit_cast(float, a.w), __builtin_bit_cast(float, b.w), c);
+}
+
+// eight floats as two bfloat16 each: f = hi + lo to 2^-16 of f
+struct HiLo {
+  u32x4 hi, lo;
+};
+__device__ __forceinline__ float bf16_low(uint32_t w) { return __builtin_bit_cast(float, w << 16); }
+__device__ __forceinline__ float bf16_high(uint32_t w) { return __builtin_bit_cast(float, w & 0xffff0000u); }
+__device__ __forceinline__ HiLo hi_lo(const float* f) {
+  HiLo r;
+  uint32_t h[4], l[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    h[i] = bf16_pair_rne(f[2 * i], f[2 * i + 1]);
+    l[i] = bf16_pair_rne(f[2 * i] - bf16_low(h[i]), f[2 * i + 1] - bf16_high(h[i]));
+  }
+  r.hi = u32x4{h[0], h[1], h[2], h[3]};
+  r.lo = u32x4{l[0], l[1], l[2], l[3]};
+  return r;
+}
+
+// ---- shrink -----------------------------------------------------------------------------------------------------------------
+constexpr int kShrinkWaves = 4;
+
+// RT: tiles of 16 of the rank, NT: of rows. A step is 128 bytes of a row: lanes 16 g .. hold packets 2 g and 2 g + 1 of it, of both
+// operands (the order of a sum is free).
+template <typename T, int RT, int NT>
+__global__ __launch_bounds__(kShrinkWaves * kWave) void shrink_kernel(const T* __restrict__ x, const int64_t x_stride, const Bank bank,
+                                                                          const Requests req, float* __restrict__ planes, const int64_t plane) {
+  constexpr int V = Pack<T>::N, U = RT + NT <= 4 ? 4 : RT + NT <= 8 ? 2 : 1;
+  __shared__ v4f s_sum[kShrinkWaves - 1][RT * NT][kWave];
+  int first, n;
+  const int a = req.template piece<kPieceShift<NT>>(blockIdx.x, bank.slots, first, n);
+  if (n <= 0 || a < 0) return;
+  const int lane = threadIdx.x & (kWave - 1), wv = threadIdx.x / kWave, lr = lane & 15, g = lane >> 4;
+  const int packets = bank.width / V, steps = (packets + 7) / 8, splits = gridDim.y;
+  const int s0 = static_cast<int>(static_cast<int64_t>(steps) * blockIdx.y / splits), s1 = static_cast<int>(static_cast<int64_t>(steps) * (blockIdx.y + 1) / splits);
+  const T* xr[NT];
+  const T* mr[RT];
+#pragma unroll
+  for (int i = 0; i < NT; ++i) xr[i] = x + static_cast<int64_t>(first + min(i * 16 + lr, n - 1)) * x_stride;
+#pragma unroll
+  for (int i = 0; i < RT; ++i)
+    mr[i] = static_cast<const T*>(bank.m) + (static_cast<int64_t>(a) * bank.rank + min(i * 16 + lr, bank.rank - 1)) * bank.width;
+  v4f acc[RT][NT] = {};
+  for (int s = s0 + wv; s < s1; s += kShrinkWaves * U) {
+    u32x4 xv[U][NT][2], mv[U][RT][2];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int at = min(s + u * kShrinkWaves, s1 - 1);   // (a step past the end is loaded again and not multiplied)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int p = min(at * 8 + 2 * g + h, packets - 1) * V;
+#pragma unroll
+        for (int i = 0; i < NT; ++i) xv[u][i][h] = load16(xr[i] + p);
+#pragma unroll
+        for (int i = 0; i < RT; ++i) mv[u][i][h] = load16(mr[i] + p);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int at = s + u * kShrinkWaves;
+      if (at >= s1) break;
+      if (at * 8 + 8 > packets) {   // the row's last step: packets past its end are zeros
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+          if (at * 8 + 2 * g + h >= packets) {
+#pragma unroll
+            for (int i = 0; i < NT; ++i) xv[u][i][h] = u32x4{0, 0, 0, 0};
+#pragma unroll
+            for (int i = 0; i < RT; ++i) mv[u][i][h] = u32x4{0, 0, 0, 0};
+          }
+      }
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int i = 0; i < RT; ++i)
+#pragma unroll
+          for (int j = 0; j < NT; ++j) acc[i][j] = mfma_packet<T>(mv[u][i][h], xv[u][j][h], acc[i][j]);
+    }
+  }
+  if (wv > 0) {
+#pragma unroll
+    for (int i = 0; i < RT * NT; ++i) s_sum[wv - 1][i][lane] = acc[i / NT][i % NT];
+  }
+  __syncthreads();
+  if (wv > 0) return;
+#pragma unroll
+  for (int i = 0; i < RT; ++i)
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+      v4f v = acc[i][j];
+#pragma unroll
+      for (int w = 0; w < kShrinkWaves - 1; ++w) v += s_sum[w][i * NT + j][lane];
+      const int r = i * 16 + 4 * g, t = j * 16 + lr;   // four of the rank, a row
+      if (t < n && r < bank.rank)
+        *reinterpret_cast<v4f*>(planes + blockIdx.y * plane + static_cast<int64_t>(first + t) * bank.rank + r) = v;
+    }
+}
+
+// ---- expand -----------------------------------------------------------------------------------------------------------------
+constexpr int kExpandWaves = 4;
+
+struct Expand {
+  const float* planes;     // [splits][rows][rank]
+  int64_t plane;
+  int splits;
+  const float* scaling;    // [slots], or null: 1
+  const void* base;        // or null: zeros
+  int64_t base_stride;
+  void* out;               // [rows, width], contiguous
+  float* low;              // or null: the sum of the planes [rows, rank], by the first columns' workgroups
+  int rows, columns;       // columns of out
+  int pieces;              // workgroups from there on in blockIdx.x: rows of no request
+  int units;               // of 64 columns a wave
+};
+
+// The columns of MFMA row r of tile mi are named 16 (r / 4) + 4 mi + r % 4, so that a lane's results are 16 neighbours.
+// The bank here is [slots][columns][rank].
+template <typename T, int RT, int NT>
+__global__ __launch_bounds__(kExpandWaves * kWave) void expand_kernel(const Bank bank, const Requests req, const Expand e) {
+  constexpr int V = Pack<T>::N, KT = (RT * 16 + 4 * V - 1) / (4 * V);   // steps of the rank: 32 (fp32: 16)
+  const int lane = threadIdx.x & (kWave - 1), wv = threadIdx.x / kWave, lr = lane & 15, g = lane >> 4;
+  int first, n, a;
+  if (static_cast<int>(blockIdx.x) < e.pieces) {
+    a = req.template piece<kPieceShift<NT>>(blockIdx.x, bank.slots, first, n);
+    if (n <= 0) return;
+  } else {   // rows in front of the first request and behind the last one: the base as it is
+    a = -1;
+    first = (blockIdx.x - e.pieces) << kPieceShift<NT>;
+    n = min(e.rows - first, 1 << kPieceShift<NT>);
+  }
+  const bool rest = static_cast<int>(blockIdx.x) >= e.pieces;
+  const int begin = rest ? req.rows.first(0) : 0, end = rest ? max(req.rows.first(req.rows.sequences), begin) : 0;
+  const int unit0 = (blockIdx.y * kExpandWaves + wv) * e.units;
+  u32x4 low_hi[NT][KT], low_lo[NT][KT];   // (fp32: low_hi alone)
+  if (a >= 0) {
+    const float s = e.scaling != nullptr ? e.scaling[a] : 1.0f;
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+      const int64_t row = first + min(j * 16 + lr, n - 1);
+#pragma unroll
+      for (int k = 0; k < KT; ++k) {
+        const int r = (k * 4 + g) * V;
+        float f[V] = {};
+        if (r < bank.rank) {
+          for (int p = 0; p < e.splits; ++p) {
+            const float* from = e.planes + p * e.plane + row * bank.rank + r;
+#pragma unroll
+            for (int i = 0; i < V; i += 4) {
+              const v4f v = *reinterpret_cast<const v4f*>(from + i);
+#pragma unroll
+              for (int q = 0; q < 4; ++q) f[i + q] += v[q];
+            }
+          }
+          if (e.low != nullptr && unit0 == 0 && j * 16 + lr < n) {
+#pragma unroll
+            for (int i = 0; i < V; i += 4) *reinterpret_cast<v4f*>(e.low + row * bank.rank + r + i) = v4f{f[i], f[i + 1], f[i + 2], f[i + 3]};
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < V; ++i) f[i] *= s;
+        if constexpr (V == 8) {
+          const HiLo v = hi_lo(f);
+          low_hi[j][k] = v.hi;
+          low_lo[j][k] = v.lo;
+        } else {
+          low_hi[j][k] = Pack<float>::pack(f);
+        }
+      }
+    }
+  } else if (e.low != nullptr && unit0 == 0) {   // (no adapter: zeros)
+    for (int i = lane; i < n * bank.rank; i += kWave) {
+      const int64_t row = first + i / bank.rank;
+      if (!rest || row < begin || row >= end) e.low[row * bank.rank + i % bank.rank] = 0.0f;
+    }
+  }
+  for (int u = 0; u < e.units; ++u) {
+    const int c0 = (unit0 + u) * 64;
+    if (c0 >= e.columns) return;
+    v4f acc[NT][4] = {};
+    if (a >= 0) {
+#pragma unroll
+      for (int k = 0; k < KT; ++k) {
+        const int r = (k * 4 + g) * V;
+        u32x4 m[4];
+#pragma unroll
+        for (int mi = 0; mi < 4; ++mi) {
+          const int c = min(c0 + (lr >> 2) * 16 + mi * 4 + (lr & 3), e.columns - 1);
+          m[mi] = load16(static_cast<const T*>(bank.m) + (static_cast<int64_t>(a) * e.columns + c) * bank.rank + min(r, bank.rank - V));
+        }
+        // (past the rank the operand of `low` is zeros, against weights that are looked at a second time)
+#pragma unroll
+        for (int mi = 0; mi < 4; ++mi) {
+          if constexpr (sizeof(T) == 4) {
+#pragma unroll
+            for (int j = 0; j < NT; ++j) acc[j][mi] = mfma_packet<float>(m[mi], low_hi[j][k], acc[j][mi]);
+          } else if constexpr (__is_same(T, f16_t)) {
+            float f[8];
+            Pack<f16_t>::unpack(m[mi], f);
+            const HiLo w = hi_lo(f);   // (exact: 11 bits in 16)
+#pragma unroll
+            for (int j = 0; j < NT; ++j) {
+              acc[j][mi] = mfma_16x16x32<bf16_t>(w.lo, low_hi[j][k], acc[j][mi]);
+              acc[j][mi] = mfma_16x16x32<bf16_t>(w.hi, low_lo[j][k], acc[j][mi]);
+              acc[j][mi] = mfma_16x16x32<bf16_t>(w.hi, low_hi[j][k], acc[j][mi]);
+            }
+          } else {
+#pragma unroll
+            for (int j = 0; j < NT; ++j) {
+              acc[j][mi] = mfma_16x16x32<bf16_t>(m[mi], low_lo[j][k], acc[j][mi]);
+              acc[j][mi] = mfma_16x16x32<bf16_t>(m[mi], low_hi[j][k], acc[j][mi]);
+            }
+          }
+        }
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+      const int t = j * 16 + lr;
+      const int64_t row = first + t;
+      if (t >= n || (rest && row >= begin && row < end)) continue;
+#pragma unroll
+      for (int h = 0; h < 16 / V; ++h) {   // packets of the lane's 16 columns
+        const int c = c0 + g * 16 + h * V;
+        if (c >= e.columns) continue;
+        float f[V] = {};
+        if (e.base != nullptr) Pack<T>::unpack(load16(static_cast<const T*>(e.base) + row * e.base_stride + c), f);
+        if (a >= 0) {   // (else the base to the bit: -0 + 0 is +0)
+#pragma unroll
+          for (int i = 0; i < V; ++i) f[i] += acc[j][(h * V + i) / 4][i % 4];
+        }
+        store16(static_cast<T*>(e.out) + row * e.columns + c, Pack<T>::pack(f));
+      }
+    }
+  }
+}
+
+// ---- the plan of a gradient: rows sorted by adapter -----------------------------------------------------------------------------
+constexpr int kBlock = 32;          // rows of a block: one step of the matrix core
+constexpr int kPlanThreads = 1024;  // and the most slots
+
+// start [slots + 1]: the first virtual row of each slot, a multiple of 32 (rows up to there: none, -1); order: the row behind each
+// virtual row. Requests of a slot keep their order. One workgroup; seq_start: [sequences] scratch.
+__global__ __launch_bounds__(kPlanThreads) void plan_kernel(const Requests req, const int slots, const int capacity, int32_t* __restrict__ start,
+                                                            int32_t* __restrict__ order, int32_t* __restrict__ seq_start) {
+  __shared__ int s_a[kPlanThreads], s_n[kPlanThreads], s_scan[kPlanThreads];
+  const int t = threadIdx.x, sequences = req.rows.sequences;
+  const auto rows_of = [&](int b) { return max(req.rows.first(b + 1) - req.rows.first(b), 0); };
+  int mine = 0;
+  for (int pass = 0; pass < 2; ++pass) {
+    int at = pass == 0 ? 0 : start[min(t, slots)];
+    for (int b0 = 0; b0 < sequences; b0 += kPlanThreads) {
+      __syncthreads();
+      if (b0 + t < sequences) {
+        s_a[t] = req.adapter[b0 + t];
+        s_n[t] = rows_of(b0 + t);
+      }
+      __syncthreads();
+      const int many = min(sequences - b0, kPlanThreads);
+      if (t < slots) {
+        for (int i = 0; i < many; ++i) {
+          if (s_a[i] != t) continue;
+          if (pass == 1) seq_start[b0 + i] = at;
+          at += s_n[i];
+        }
+      }
+    }
+    if (pass == 1) break;
+    mine = t < slots ? (at + kBlock - 1) / kBlock * kBlock : 0;
+    s_scan[t] = mine;
+    __syncthreads();
+    for (int d = 1; d < kPlanThreads; d *= 2) {
+      const int v = t >= d ? s_scan[t - d] : 0;
+      __syncthreads();
+      s_scan[t] += v;
+      __syncthreads();
+    }
+    if (t < slots) start[t] = s_scan[t] - mine;
+    if (t == slots - 1) start[slots] = s_scan[t];
+    __syncthreads();   // (read back below by the same workgroup)
+  }
+  for (int v = t; v < capacity; v += kPlanThreads) order[v] = -1;
+  __syncthreads();
+  for (int row = t; row < req.rows.rows; row += kPlanThreads) {
+    int lo = 0, hi = sequences;   // the last request that begins at or in front of the row
+    while (lo + 1 < hi) {
+      const int mid = (lo + hi) / 2;
+      if (req.rows.first(mid) <= row) lo = mid; else hi = mid;
+    }
+    const int in_b = row - req.rows.first(lo);
+    if (in_b < 0 || in_b >= rows_of(lo)) continue;
+    const int a = req.adapter[lo];
+    if (a < 0 || a >= slots) continue;
+    const int v = seq_start[lo] + in_b;
+    if (v < capacity) order[v] = row;
+  }
+}
+
+// Sums of shrink's planes, times the scaling, as [rows, rank] (du) and, with the kept `low`, as operands of outer: blocks of 32
+// virtual rows, [tile of the rank][block][lane][8], lane 16 g + r holding entry r of the rank of rows 8 g .. 8 g + 7.
+__global__ __launch_bounds__(kWave) void operands_kernel(const float* __restrict__ planes, const int64_t plane, const int splits,
+                                                         const float* __restrict__ low, const float* __restrict__ scaling, const int rank,
+                                                         const int slots, const int32_t* __restrict__ start, const int32_t* __restrict__ order,
+                                                         float* __restrict__ du, float* __restrict__ op_du, float* __restrict__ op_low) {
+  const int block = blockIdx.x, tile = blockIdx.y, lane = threadIdx.x, g = lane >> 4, r = tile * 16 + (lane & 15);
+  if (block * kBlock >= start[slots]) return;
+  int lo = 0, hi = slots;   // the slot: the last one that begins at or in front of the block (empty ones begin where the next does)
+  while (lo + 1 < hi) {
+    const int mid = (lo + hi) / 2;
+    if (start[mid] <= block * kBlock) lo = mid; else hi = mid;
+  }
+  const float s = scaling[lo];
+  float d[8], l[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int row = order[block * kBlock + 8 * g + i];
+    float sum = 0.0f;
+    l[i] = 0.0f;
+    if (row >= 0 && r < rank) {
+      const int64_t at = static_cast<int64_t>(row) * rank + r;
+      for (int p = 0; p < splits; ++p) sum += planes[p * plane + at];
+      sum *= s;
+      du[at] = sum;
+      l[i] = low[at] * s;
+    }
+    d[i] = sum;
+  }
+  const int64_t to = ((static_cast<int64_t>(tile) * gridDim.x + block) * kWave + lane) * 8;
+#pragma unroll
+  for (int i = 0; i < 8; i += 4) {
+    *reinterpret_cast<v4f*>(op_du + to + i) = v4f{d[i], d[i + 1], d[i + 2], d[i + 3]};
+    *reinterpret_cast<v4f*>(op_low + to + i) = v4f{l[i], l[i + 1], l[i + 2], l[i + 3]};
+  }
+}
+
+// ---- outer ------------------------------------------------------------------------------------------------------------------
+struct OuterSide {
+  const void* x;           // rows of `width` values of T, or int8 codes with x_scale
+  int64_t stride;
+  const float* x_scale;    // [rows, width / 128], or null
+  const float* op;         // operands of the other factor
+  float* records;          // [pieces][rank][width]
+  int width;
+};
+struct Outer {
+  OuterSide a, b;          // gradients of A (x and du) and of B (g and low)
+  const int32_t* start;
+  const int32_t* order;
+  int slots, rank, blocks, capacity, shift;   // blocks: of the operands; 1 << shift rows a piece
+  int a_columns;           // workgroups of side a in blockIdx.x
+};
+constexpr int kColumns = 128;   // of a wave: one group of the codes
+
+// One side's sums over the rows of a piece for 128 columns and 16 RTW of the rank.
+template <typename T, bool CODES, int RTW>
+__device__ __forceinline__ void outer_rows(const OuterSide& side, const Outer& o, int c0, int v0, int v1, v4f (&acc)[RTW][8]) {
+  const int lane = threadIdx.x & (kWave - 1), wv = threadIdx.x / kWave, lr = lane & 15, g = lane >> 4;
+  const int spare = max(o.order[v0], 0);   // (the first row of a block: real)
+  const int tile0 = blockIdx.z * RTW;
+  for (int v = v0 + wv * kBlock; v < v1; v += 4 * kBlock) {
+    int64_t row[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int at = o.order[v + 8 * g + i];
+      row[i] = at >= 0 ? at : spare;   // (its other factor is zero; a row of this slot, so that nothing foreign gets in)
+    }
+    float f[RTW][8];
+#pragma unroll
+    for (int i = 0; i < RTW; ++i) {
+      const int tile = min(tile0 + i, (o.rank + 15) / 16 - 1);
+      const float* from = side.op + ((static_cast<int64_t>(tile) * o.blocks + v / kBlock) * kWave + lane) * 8;
+#pragma unroll
+      for (int q = 0; q < 8; q += 4) {
+        const v4f w = *reinterpret_cast<const v4f*>(from + q);
+        f[i][q] = w[0]; f[i][q + 1] = w[1]; f[i][q + 2] = w[2]; f[i][q + 3] = w[3];
+      }
+    }
+    if constexpr (CODES) {
+      float s[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) s[i] = side.x_scale[row[i] * (side.width / kColumns) + c0 / kColumns];
+#pragma unroll
+      for (int i = 0; i < RTW; ++i)
+#pragma unroll
+        for (int q = 0; q < 8; ++q) f[i][q] *= s[q];
+    }
+    if constexpr (sizeof(T) == 4) {   // rows 8 g + e, four neighbouring columns a load: e-th step takes row e of each lane
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int c = min(c0 + (CODES ? 8 * lr + 4 * h : 64 * h + 4 * lr), side.width - 4);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          float x[4];
+          if constexpr (CODES) {
+            const uint32_t w = *reinterpret_cast<const uint32_t*>(static_cast<const int8_t*>(side.x) + row[e] * side.stride + c);
+#pragma unroll
+            for (int q = 0; q < 4; ++q) x[q] = static_cast<float>(static_cast<int8_t>(w >> (8 * q)));
+          } else {
+            Pack<float>::unpack(load16(static_cast<const float*>(side.x) + row[e] * side.stride + c), x);
+          }
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+#pragma unroll
+            for (int i = 0; i < RTW; ++i) acc[i][h * 4 + q] = mfma_f32(x[q], f[i][e], acc[i][h * 4 + q]);
+        }
+      }
+    } else {
+      HiLo u[RTW];
+#pragma unroll
+      for (int i = 0; i < RTW; ++i) u[i] = hi_lo(f[i]);
+      const int c = min(c0 + 8 * lr, side.width - 8);
+      if constexpr (CODES || __is_same(T, f16_t)) {
+        float x[8][8];   // rows, columns
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          if constexpr (CODES) {
+            const u32x2 w = *reinterpret_cast<const u32x2*>(static_cast<const int8_t*>(side.x) + row[e] * side.stride + c);
+#pragma unroll
+            for (int q = 0; q < 8; ++q) x[e][q] = static_cast<float>(static_cast<int8_t>((q < 4 ? w.x : w.y) >> (8 * (q % 4))));
+          } else {
+            Pack<f16_t>::unpack(load16(static_cast<const f16_t*>(side.x) + row[e] * side.stride + c), x[e]);
+          }
+        }
+#pragma unroll
+        for (int q = 0; q < 8; ++q) {
+          const float column[8] = {x[0][q], x[1][q], x[2][q], x[3][q], x[4][q], x[5][q], x[6][q], x[7][q]};
+          const HiLo w = hi_lo(column);   // (codes: the first alone; fp16: exact)
+#pragma unroll
+          for (int i = 0; i < RTW; ++i) {
+            if constexpr (!CODES) acc[i][q] = mfma_16x16x32<bf16_t>(w.lo, u[i].hi, acc[i][q]);
+            acc[i][q] = mfma_16x16x32<bf16_t>(w.hi, u[i].lo, acc[i][q]);
+            acc[i][q] = mfma_16x16x32<bf16_t>(w.hi, u[i].hi, acc[i][q]);
+          }
+        }
+      } else {
+        u32x4 raw[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) raw[e] = load16(static_cast<const bf16_t*>(side.x) + row[e] * side.stride + c);
+        const auto word = [&](int e, int w) { return w == 0 ? raw[e].x : w == 1 ? raw[e].y : w == 2 ? raw[e].z : raw[e].w; };
+#pragma unroll
+        for (int q = 0; q < 8; ++q) {
+          const uint32_t select = q % 2 ? 0x07060302u : 0x05040100u;   // the halves of two rows' words
+          u32x4 w;
+          w.x = __builtin_amdgcn_perm(word(1, q / 2), word(0, q / 2), select);
+          w.y = __builtin_amdgcn_perm(word(3, q / 2), word(2, q / 2), select);
+          w.z = __builtin_amdgcn_perm(word(5, q / 2), word(4, q / 2), select);
+          w.w = __builtin_amdgcn_perm(word(7, q / 2), word(6, q / 2), select);
+#pragma unroll
+          for (int i = 0; i < RTW; ++i) {
+            acc[i][q] = mfma_16x16x32<bf16_t>(w, u[i].lo, acc[i][q]);
+            acc[i][q] = mfma_16x16x32<bf16_t>(w, u[i].hi, acc[i][q]);
+          }
+        }
+      }
+    }
+  }
+}
+
+template <typename T, bool CODES, int RTW>
+__global__ __launch_bounds__(4 * kWave) void outer_kernel(const Outer o) {
+  __shared__ v4f s_sum[2][RTW * 8][kWave];
+  const Ragged slots{o.start, o.slots, o.capacity};
+  int piece = blockIdx.y, none;
+  Span span;
+  slots.find(o.shift, nullptr, piece, span, none);
+  const int v0 = span.first + (piece << o.shift), v1 = min(v0 + (1 << o.shift), span.first + span.n);
+  if (span.n <= 0 || v0 >= v1) return;
+  const bool side_b = static_cast<int>(blockIdx.x) >= o.a_columns;
+  const int c0 = (blockIdx.x - (side_b ? o.a_columns : 0)) * kColumns;
+  v4f acc[RTW][8] = {};
+  if (side_b) outer_rows<T, false, RTW>(o.b, o, c0, v0, v1, acc);
+  else outer_rows<T, CODES, RTW>(o.a, o, c0, v0, v1, acc);
+  const int lane = threadIdx.x & (kWave - 1), wv = threadIdx.x / kWave, lr = lane & 15, g = lane >> 4;
+  if (wv >= 2) {
+#pragma unroll
+    for (int i = 0; i < RTW * 8; ++i) s_sum[wv - 2][i][lane] = acc[i / 8][i % 8];
+  }
+  __syncthreads();
+  if (wv < 2) {
+#pragma unroll
+    for (int i = 0; i < RTW * 8; ++i) acc[i / 8][i % 8] += s_sum[wv][i][lane];
+  }
+  __syncthreads();
+  if (wv == 1) {
+#pragma unroll
+    for (int i = 0; i < RTW * 8; ++i) s_sum[0][i][lane] = acc[i / 8][i % 8];
+  }
+  __syncthreads();
+  if (wv != 0) return;
+  const OuterSide& side = side_b ? o.b : o.a;
+  float* record = side.records + static_cast<int64_t>(blockIdx.y) * o.rank * side.width;
+  const bool quads = sizeof(T) == 4 && !(CODES && !side_b);   // fp32 values: columns 64 h + 16 g + 4 q + i; else 32 g + 8 q + i
+#pragma unroll
+  for (int i = 0; i < RTW; ++i) {
+    const int r = (blockIdx.z * RTW + i) * 16 + lr;
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        v4f v;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = acc[i][h * 4 + e][q] + s_sum[0][i * 8 + h * 4 + e][lane][q];
+        const int c = c0 + (quads ? 64 * h + 16 * g + 4 * q : 32 * g + 8 * q + 4 * h);
+        if (r < o.rank && c < side.width) *reinterpret_cast<v4f*>(record + static_cast<int64_t>(r) * side.width + c) = v;
+      }
+  }
+}
+
+// The pieces' records of each slot added up in order, rounded: eight of the width a lane for A [slots, rank, width], eight of the rank
+// for B [slots, width, rank]. A slot without rows has a gradient of zero.
+template <typename T>
+__global__ __launch_bounds__(256) void records_kernel(const Outer o, T* __restrict__ grad_a, T* __restrict__ grad_b, const int64_t a_items, const int64_t items) {
+  for (int64_t item = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; item < items; item += static_cast<int64_t>(gridDim.x) * 256) {
+    const bool of_b = item >= a_items;
+    const OuterSide& side = of_b ? o.b : o.a;
+    const int64_t at = of_b ? item - a_items : item, each = static_cast<int64_t>(o.rank) * side.width, per_slot = each / 8;
+    const int slot = static_cast<int>(at / per_slot), rest = static_cast<int>(at - slot * per_slot);
+    int r, c;
+    if (of_b) {
+      r = rest / side.width * 8;
+      c = rest % side.width;
+    } else {
+      r = rest / (side.width / 8);
+      c = rest % (side.width / 8) * 8;
+    }
+    const int n = o.start[slot + 1] - o.start[slot], first = (o.start[slot] >> o.shift) + 2 * slot, pieces = (n + (1 << o.shift) - 1) >> o.shift;
+    float f[8] = {};
+    for (int p = 0; p < pieces; ++p) {
+      const float* from = side.records + (first + p) * each + static_cast<int64_t>(r) * side.width + c;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) f[i] += of_b ? from[static_cast<int64_t>(i) * side.width] : from[i];
+    }
+    T* to = of_b ? grad_b + slot * each + static_cast<int64_t>(c) * o.rank + r : grad_a + slot * each + static_cast<int64_t>(r) * side.width + c;
+#pragma unroll
+    for (int i = 0; i < 8; i += Pack<T>::N) store16(to + i, Pack<T>::pack(f + i));
+  }
+}
+
+// [slots, rows, cols] -> [slots, cols, rows], 32 x 32 a workgroup
+template <typename E>
+__global__ __launch_bounds__(256) void transpose_kernel(const E* __restrict__ from, E* __restrict__ to, const int rows, const int cols) {
+  __shared__ E s_t[32][33];
+  const int64_t slot = static_cast<int64_t>(blockIdx.z) * rows * cols;
+  const int r0 = blockIdx.y * 32, c0 = blockIdx.x * 32, x = threadIdx.x % 32, y = threadIdx.x / 32;
+#pragma unroll
+  for (int i = 0; i < 32; i += 8)
+    if (r0 + y + i < rows && c0 + x < cols) s_t[y + i][x] = from[slot + static_cast<int64_t>(r0 + y + i) * cols + c0 + x];
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < 32; i += 8)
+    if (c0 + y + i < cols && r0 + x < rows) to[slot + static_cast<int64_t>(c0 + y + i) * rows + r0 + x] = s_t[x][y + i];
+}
+
+// ---- what a call takes ------------------------------------------------------------------------------------------------------
+// Row tiles of a piece: one for single rows and short requests, four where requests are long (a bank's rows are read once a piece).
+int row_tiles(int rows, int sequences, bool ragged) {
+  if (!ragged || rows < 24 * sequences) return 1;
+  return rows < 96 * sequences ? 2 : 4;
+}
+int pieces_of(int rows, int sequences, bool ragged, int nt) { return ragged ? rows / (16 * nt) + 2 * sequences : sequences; }
+// Parts of the reduction: as many workgroups of four waves as the chip has places for four times over, no less than a step a wave.
+int splits_of(int rows, int sequences, bool ragged, int width, int dtype) {
+  const int nt = row_tiles(rows, sequences, ragged);
+  const int64_t real = ragged ? (rows + 16 * nt - 1) / (16 * nt) : sequences;
+  const int steps = (width * (dtype == LLMQ_F32 ? 4 : 2) + 127) / 128;
+  int64_t splits = 512 / (real < 1 ? 1 : real);
+  const int most = (steps + kShrinkWaves - 1) / kShrinkWaves;
+  if (splits > most) splits = most;
+  if (splits > 16) splits = 16;
+  return static_cast<int>(splits < 1 ? 1 : splits);
+}
+
+template <typename T, int RT>
+void shrink_nt(const T* x, int64_t stride, const Bank& bank, const Requests& req, float* planes, int64_t plane, int splits, int nt, int pieces, hipStream_t s) {
+  const dim3 grid(pieces, splits), block(kShrinkWaves * kWave);
+  if (nt == 1) hipLaunchKernelGGL((shrink_kernel<T, RT, 1>), grid, block, 0, s, x, stride, bank, req, planes, plane);
+  else if (nt == 2) hipLaunchKernelGGL((shrink_kernel<T, RT, 2>), grid, block, 0, s, x, stride, bank, req, planes, plane);
+  else hipLaunchKernelGGL((shrink_kernel<T, RT, 4>), grid, block, 0, s, x, stride, bank, req, planes, plane);
+}
+template <typename T>
+void shrink(const void* x, int64_t stride, const Bank& bank, const Requests& req, float* planes, int64_t plane, int splits, int nt, int pieces, hipStream_t s) {
+  const T* p = static_cast<const T*>(x);
+  if (bank.rank <= 16) shrink_nt<T, 1>(p, stride, bank, req, planes, plane, splits, nt, pieces, s);
+  else if (bank.rank <= 32) shrink_nt<T, 2>(p, stride, bank, req, planes, plane, splits, nt, pieces, s);
+  else if (bank.rank <= 64) shrink_nt<T, 4>(p, stride, bank, req, planes, plane, splits, nt, pieces, s);
+  else shrink_nt<T, 8>(p, stride, bank, req, planes, plane, splits, nt, pieces, s);
+}
+template <typename T, int RT> void expand_nt(const Bank& bank, const Requests& req, const Expand& e, int nt, const dim3& grid, hipStream_t s) {
+  const dim3 block(kExpandWaves * kWave);
+  if (nt == 1) hipLaunchKernelGGL((expand_kernel<T, RT, 1>), grid, block, 0, s, bank, req, e);
+  else if (nt == 2) hipLaunchKernelGGL((expand_kernel<T, RT, 2>), grid, block, 0, s, bank, req, e);
+  else hipLaunchKernelGGL((expand_kernel<T, RT, 4>), grid, block, 0, s, bank, req, e);
+}
+// bank: [slots][columns][rank]
+template <typename T> void expand(const Bank& bank, const Requests& req, Expand e, int nt, int pieces, hipStream_t s) {
+  const int units = (e.columns + 63) / 64;
+  e.pieces = pieces;
+  // (a piece's sums are read once a wave: several units of columns a wave where there are pieces enough)
+  e.units = pieces * ((units + 15) / 16) >= 1024 ? 4 : pieces * ((units + 7) / 8) >= 1024 ? 2 : 1;
+  const bool rest = req.rows.start != nullptr && (e.out != e.base || e.low != nullptr);
+  const dim3 grid(pieces + (rest ? (e.rows + 16 * nt - 1) / (16 * nt) : 0), (units + kExpandWaves * e.units - 1) / (kExpandWaves * e.units));
+  if (bank.rank <= 16) expand_nt<T, 1>(bank, req, e, nt, grid, s);
+  else if (bank.rank <= 32) expand_nt<T, 2>(bank, req, e, nt, grid, s);
+  else if (bank.rank <= 64) expand_nt<T, 4>(bank, req, e, nt, grid, s);
+  else expand_nt<T, 8>(bank, req, e, nt, grid, s);
+}
+
+int64_t round_up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
+int64_t take(int64_t& at, int64_t bytes) {
+  const int64_t here = at;
+  at = round_up(at + bytes, 256);
+  return here;
+}
+
+struct GradPlan {
+  int nt, pieces, splits;
+  int capacity, blocks, tiles, shift, records;   // virtual rows, blocks of 32 of them, tiles of the rank, pieces of outer
+  int64_t o_start, o_order, o_seq, o_at, o_bt, o_planes, o_du, o_op_du, o_op_low, o_rec_a, o_rec_b, bytes;
+};
+GradPlan grad_plan(int rows, int sequences, bool ragged, int in, int out, int rank, int slots, int dtype) {
+  GradPlan p{};
+  const int64_t size = dtype == LLMQ_F32 ? 4 : 2;
+  p.nt = row_tiles(rows, sequences, ragged);
+  p.pieces = pieces_of(rows, sequences, ragged, p.nt);
+  p.splits = splits_of(rows, sequences, ragged, out, dtype);
+  const int64_t used = slots < sequences ? slots : sequences;   // slots that can have rows
+  p.capacity = static_cast<int>(round_up(rows + 31 * used, kBlock));
+  p.blocks = p.capacity / kBlock;
+  p.tiles = (rank + 15) / 16;
+  // a piece of outer: as long as 512 workgroups allow, 128 to 4096 rows
+  const int64_t columns = (in + kColumns - 1) / kColumns + (out + kColumns - 1) / kColumns;
+  p.shift = 7;
+  while (p.shift < 12 && columns * (rows >> (p.shift + 1)) * ((p.tiles + 3) / 4) >= 512) ++p.shift;
+  p.records = (p.capacity >> p.shift) + 2 * slots;
+  int64_t at = 0;
+  p.o_start = take(at, int64_t{4} * (slots + 1));
+  p.o_order = take(at, int64_t{4} * p.capacity);
+  p.o_seq = take(at, int64_t{4} * sequences);
+  p.o_at = take(at, size * slots * rank * in);
+  p.o_bt = take(at, size * slots * rank * out);
+  p.o_planes = take(at, int64_t{4} * p.splits * rows * rank);
+  p.o_du = take(at, int64_t{4} * rows * rank);
+  p.o_op_du = take(at, int64_t{4} * p.tiles * p.capacity * 16);
+  p.o_op_low = take(at, int64_t{4} * p.tiles * p.capacity * 16);
+  p.o_rec_a = take(at, int64_t{4} * p.records * rank * in);
+  p.o_rec_b = take(at, int64_t{4} * p.records * rank * out);
+  p.bytes = at;
+  return p;
+}
+
+template <typename T>
+void gradients(const GradPlan& p, const void* grad, int64_t grad_stride, const void* x, int64_t x_stride, const float* x_scale, const float* low,
+               const void* lora_a, const void* lora_b, const float* scaling, const Requests& req, const void* grad_base, int64_t base_stride,
+               void* grad_x, void* grad_a, void* grad_b, uint8_t* ws, int in, int out, int rank, int slots, hipStream_t s) {
+  const int rows = req.rows.rows;
+  int32_t* start = reinterpret_cast<int32_t*>(ws + p.o_start);
+  int32_t* order = reinterpret_cast<int32_t*>(ws + p.o_order);
+  float* planes = reinterpret_cast<float*>(ws + p.o_planes);
+  float* du = reinterpret_cast<float*>(ws + p.o_du);
+  const int64_t plane = static_cast<int64_t>(rows) * rank;
+  hipLaunchKernelGGL(plan_kernel, dim3(1), dim3(kPlanThreads), 0, s, req, slots, p.capacity, start, order, reinterpret_cast<int32_t*>(ws + p.o_seq));
+  const auto turn = [&](const void* from, void* to, int r, int c) {
+    const dim3 grid((c + 31) / 32, (r + 31) / 32, slots);
+    if constexpr (sizeof(T) == 4) hipLaunchKernelGGL((transpose_kernel<uint32_t>), grid, dim3(256), 0, s, static_cast<const uint32_t*>(from), static_cast<uint32_t*>(to), r, c);
+    else hipLaunchKernelGGL((transpose_kernel<uint16_t>), grid, dim3(256), 0, s, static_cast<const uint16_t*>(from), static_cast<uint16_t*>(to), r, c);
+  };
+  turn(lora_b, ws + p.o_bt, out, rank);
+  turn(lora_a, ws + p.o_at, rank, in);
+  shrink<T>(grad, grad_stride, Bank{ws + p.o_bt, slots, rank, out}, req, planes, plane, p.splits, p.nt, p.pieces, s);
+  float* op_du = reinterpret_cast<float*>(ws + p.o_op_du);
+  float* op_low = reinterpret_cast<float*>(ws + p.o_op_low);
+  hipLaunchKernelGGL(operands_kernel, dim3(p.blocks, p.tiles), dim3(kWave), 0, s, planes, plane, p.splits, low, scaling, rank, slots, start, order, du, op_du, op_low);
+  expand<T>(Bank{ws + p.o_at, slots, rank, in}, req, Expand{du, plane, 1, nullptr, grad_base, base_stride, grad_x, nullptr, rows, in, 0, 0}, p.nt, p.pieces, s);
+  const Outer o{OuterSide{x, x_stride, x_scale, op_du, reinterpret_cast<float*>(ws + p.o_rec_a), in},
+                OuterSide{grad, grad_stride, nullptr, op_low, reinterpret_cast<float*>(ws + p.o_rec_b), out},
+                start, order, slots, rank, p.blocks, p.capacity, p.shift, (in + kColumns - 1) / kColumns};
+  const int rtw = p.tiles >= 4 ? 4 : p.tiles >= 2 ? 2 : 1;
+  const dim3 grid(o.a_columns + (out + kColumns - 1) / kColumns, p.records, (p.tiles + rtw - 1) / rtw);
+#define LLMQ_OUTER(CODES)                                                                                    \
+  if (rtw == 4) hipLaunchKernelGGL((outer_kernel<T, CODES, 4>), grid, dim3(4 * kWave), 0, s, o);            \
+  else if (rtw == 2) hipLaunchKernelGGL((outer_kernel<T, CODES, 2>), grid, dim3(4 * kWave), 0, s, o);       \
+  else hipLaunchKernelGGL((outer_kernel<T, CODES, 1>), grid, dim3(4 * kWave), 0, s, o)
+  if (x_scale != nullptr) { LLMQ_OUTER(true); } else { LLMQ_OUTER(false); }
+#undef LLMQ_OUTER
+  const int64_t a_items = static_cast<int64_t>(slots) * rank * in / 8, items = a_items + static_cast<int64_t>(slots) * rank * out / 8;
+  const int64_t groups = (items + 255) / 256;
+  hipLaunchKernelGGL((records_kernel<T>), dim3(static_cast<unsigned>(groups < 4096 ? groups : 4096)), dim3(256), 0, s, o, static_cast<T*>(grad_a),
+                     static_cast<T*>(grad_b), a_items, items);
+}
+
+int check(int rows, int sequences, bool ragged, int in, int out, int rank, int slots, int dtype) {
+  if (rows < 0 || sequences < 0 || slots < 0) return llmq_host::fail_invalid("bad dimension rows=%d sequences=%d slots=%d", rows, sequences, slots);
+  if (dtype != LLMQ_F32 && dtype != LLMQ_F16 && dtype != LLMQ_BF16)
+    return llmq_host::fail_invalid("dtype code %d is not float32, float16 or bfloat16", dtype);
+  if (rank < 8 || rank > 128 || rank % 8) return llmq_host::fail_invalid("rank must be a multiple of 8 from 8 to 128, got %d", rank);
+  if (in < 8 || out < 8 || in % 8 || out % 8 || in > (1 << 20) || out > (1 << 20))
+    return llmq_host::fail_invalid("in_features and out_features must be multiples of 8 up to 2^20, got %d and %d", in, out);
+  if (rows > (1 << 20) || sequences > (1 << 20) || slots > (1 << 20)) return llmq_host::fail_invalid("at most 2^20 rows, sequences and slots, got %d, %d, %d", rows, sequences, slots);
+  if (!ragged && rows != sequences) return llmq_host::fail_invalid("without query_start a sequence has one row: %d rows, %d sequences", rows, sequences);
+  return 0;
+}
+bool misaligned(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) != 0; }
+int bad_stride(int64_t stride, int width, int packet, const char* what) {
+  if (stride >= width && stride % packet == 0) return 0;
+  return llmq_host::fail_invalid("%s's row stride must be a multiple of %d of at least %d, got %lld", what, packet, width, static_cast<long long>(stride));
+}
+
+}  // namespace
+
+extern "C" size_t llmq_lora_add_workspace_bytes(int rows, int sequences, int ragged, int in_features, int rank, int dtype) {
+  if (rows <= 0 || sequences <= 0 || in_features <= 0 || rank <= 0) return 0;
+  return static_cast<size_t>(int64_t{4} * splits_of(rows, sequences, ragged != 0, in_features, dtype) * rows * rank);
+}
+
+extern "C" int llmq_lora_add(const void* x, int64_t x_stride, const void* base, int64_t base_stride, const void* lora_a, const void* lora_b,
+                             const float* scaling, const int32_t* adapter, const int32_t* query_start_or_null, void* out, float* low_or_null,
+                             void* workspace, size_t workspace_bytes, int rows, int sequences, int in_features, int out_features, int rank,
+                             int slots, int dtype, llmq_stream_t stream) {
+  const bool ragged = query_start_or_null != nullptr;
+  if (int rc = check(rows, sequences, ragged, in_features, out_features, rank, slots, dtype)) return rc;
+  if (rows == 0 || sequences == 0) return 0;   // (no sequence has a row: nothing is written)
+  if (!x || !base || !out || !adapter || (slots > 0 && (!lora_a || !lora_b || !scaling))) return llmq_host::fail_invalid("null tensor pointer");
+  const int v = dtype == LLMQ_F32 ? 4 : 8;
+  if (int rc = bad_stride(x_stride, in_features, v, "x")) return rc;
+  if (int rc = bad_stride(base_stride, out_features, v, "base")) return rc;
+  if (out == base && base_stride != out_features) return llmq_host::fail_invalid("out in place of base needs contiguous rows");
+  if (misaligned(x) || misaligned(base) || misaligned(out) || misaligned(lora_a) || misaligned(lora_b) || misaligned(low_or_null))
+    return llmq_host::fail_invalid("all tensors must be 16-byte aligned");
+  const size_t need = llmq_lora_add_workspace_bytes(rows, sequences, ragged, in_features, rank, dtype);
+  if (!workspace || misaligned(workspace) || workspace_bytes < need)
+    return llmq_host::fail_invalid("the workspace must be 16-byte aligned and hold %zu bytes, got %zu", need, workspace_bytes);
+  const Requests req{adapter, Ragged{query_start_or_null, sequences, rows}};
+  const int nt = row_tiles(rows, sequences, ragged), pieces = pieces_of(rows, sequences, ragged, nt);
+  const int splits = splits_of(rows, sequences, ragged, in_features, dtype);
+  float* planes = static_cast<float*>(workspace);
+  const int64_t plane = static_cast<int64_t>(rows) * rank;
+  const Expand e{planes, plane, splits, scaling, base, base_stride, out, low_or_null, rows, out_features, 0, 0};
+  hipStream_t s = static_cast<hipStream_t>(stream);
+#define LLMQ_ADD(T)                                                                                                        \
+  shrink<T>(x, x_stride, Bank{lora_a, slots, rank, in_features}, req, planes, plane, splits, nt, pieces, s);               \
+  expand<T>(Bank{lora_b, slots, rank, out_features}, req, e, nt, pieces, s)
+  switch (dtype) {
+    case LLMQ_F32: LLMQ_ADD(float); break;
+    case LLMQ_F16: LLMQ_ADD(f16_t); break;
+    default: LLMQ_ADD(bf16_t); break;
+  }
+#undef LLMQ_ADD
+  return llmq_host::check_launch("lora_add");
+}
+
+extern "C" size_t llmq_lora_grad_workspace_bytes(int rows, int sequences, int ragged, int in_features, int out_features, int rank, int slots, int dtype) {
+  if (rows <= 0 || sequences <= 0 || in_features <= 0 || out_features <= 0 || rank <= 0 || slots <= 0) return 0;
+  return static_cast<size_t>(grad_plan(rows, sequences, ragged != 0, in_features, out_features, rank, slots, dtype).bytes);
+}
+
+extern "C" int llmq_lora_grad(const void* grad, int64_t grad_stride, const void* x, int64_t x_stride, const float* x_scale_or_null,
+                              const float* low, const void* lora_a, const void* lora_b, const float* scaling, const int32_t* adapter,
+                              const int32_t* query_start_or_null, const void* grad_base_or_null, int64_t base_stride, void* grad_x, void* grad_a,
+                              void* grad_b, void* workspace, size_t workspace_bytes, int rows, int sequences, int in_features,
+                              int out_features, int rank, int slots, int dtype, llmq_stream_t stream) {
+  const bool ragged = query_start_or_null != nullptr;
+  if (int rc = check(rows, sequences, ragged, in_features, out_features, rank, slots, dtype)) return rc;
+  if (slots > kPlanThreads) return llmq_host::fail_invalid("at most %d slots have gradients, got %d", kPlanThreads, slots);
+  if (x_scale_or_null && in_features % kColumns) return llmq_host::fail_invalid("codes of x come in groups of 128, in_features is %d", in_features);
+  if (rows == 0 || sequences == 0 || slots == 0) return 0;   // (nothing is written)
+  if (!grad || !x || !low || !lora_a || !lora_b || !scaling || !adapter || !grad_x || !grad_a || !grad_b) return llmq_host::fail_invalid("null tensor pointer");
+  const int v = dtype == LLMQ_F32 ? 4 : 8;
+  if (int rc = bad_stride(grad_stride, out_features, v, "grad")) return rc;
+  if (int rc = bad_stride(x_stride, in_features, x_scale_or_null ? 16 : v, "x")) return rc;
+  if (grad_base_or_null)
+    if (int rc = bad_stride(base_stride, in_features, v, "grad_base")) return rc;
+  for (const void* t : {grad, x, static_cast<const void*>(low), lora_a, lora_b, grad_base_or_null, static_cast<const void*>(grad_x),
+                        static_cast<const void*>(grad_a), static_cast<const void*>(grad_b)})
+    if (misaligned(t)) return llmq_host::fail_invalid("all tensors must be 16-byte aligned");
+  const GradPlan p = grad_plan(rows, sequences, ragged, in_features, out_features, rank, slots, dtype);
+  if (!workspace || misaligned(workspace) || workspace_bytes < static_cast<size_t>(p.bytes))
+    return llmq_host::fail_invalid("the workspace must be 16-byte aligned and hold %lld bytes, got %zu", static_cast<long long>(p.bytes), workspace_bytes);
+  const Requests req{adapter, Ragged{query_start_or_null, sequences, rows}};
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  hipStream_t s = static_cast<hipStream_t>(stream);
+#define LLMQ_GRAD(T)                                                                                                                 \
+  gradients<T>(p, grad, grad_stride, x, x_stride, x_scale_or_null, low, lora_a, lora_b, scaling, req, grad_base_or_null, base_stride, \
+               grad_x, grad_a, grad_b, ws, in_features, out_features, rank, slots, s)
+  switch (dtype) {
+    case LLMQ_F32: LLMQ_GRAD(float); break;
+    case LLMQ_F16: LLMQ_GRAD(f16_t); break;
+    default: LLMQ_GRAD(bf16_t); break;
+  }
+#undef LLMQ_GRAD
+  return llmq_host::check_launch("lora_grad");
+}

@@ -1919,6 +1919,143 @@ std::tuple<at::Tensor, c10::optional<at::Tensor>> vocab_loss_grad(const at::Tens
   return {grad_hidden, grad_weight};
 }
 
+// The adapters of a projection: lora_a [slots, rank, in], lora_b [slots, out, rank], scaling [slots], and who has which.
+struct Adapters {
+  int64_t slots, rank, in, out;
+  int sequences;
+  at::Tensor adapter, start;   // start: undefined for one row a sequence
+  const int32_t* start_or_null() const { return start.defined() ? start.const_data_ptr<int32_t>() : nullptr; }
+};
+Adapters adapters_of(const at::Tensor& like, const at::Tensor& lora_a, const at::Tensor& lora_b, const at::Tensor& scaling,
+                     const at::Tensor& adapter, const c10::optional<at::Tensor>& query_start, int64_t rows) {
+  for (const at::Tensor* t : {&lora_a, &lora_b, &scaling, &adapter})
+    TORCH_CHECK(t->device() == like.device(), "the adapters must lie on the rows' device");
+  TORCH_CHECK(lora_a.scalar_type() == like.scalar_type() && lora_b.scalar_type() == like.scalar_type(), "lora_a and lora_b must have the rows' dtype");
+  TORCH_CHECK(lora_a.dim() == 3 && lora_b.dim() == 3 && lora_a.size(0) == lora_b.size(0) && lora_a.size(1) == lora_b.size(2),
+              "lora_a must be [slots, rank, in] and lora_b [slots, out, rank]");
+  for (const at::Tensor* t : {&lora_a, &lora_b})
+    TORCH_CHECK(t->is_contiguous() && reinterpret_cast<uintptr_t>(t->const_data_ptr()) % 16 == 0, "lora_a and lora_b must be contiguous and 16-byte aligned");
+  TORCH_CHECK(scaling.scalar_type() == at::kFloat && scaling.dim() == 1 && scaling.size(0) == lora_a.size(0) && scaling.is_contiguous(),
+              "scaling must be contiguous float32 [slots]");
+  Adapters r{lora_a.size(0), lora_a.size(1), lora_a.size(2), lora_b.size(1), 0, {}, {}};
+  for (int64_t n : {rows, r.slots, r.rank, r.in, r.out, adapter.numel()}) check_int(n, "a size of the adapters");
+  TORCH_CHECK(adapter.scalar_type() == at::kInt && adapter.dim() == 1, "adapter must be int32 [sequences]");
+  const int64_t sequences = adapter.size(0);
+  r.adapter = adapter.contiguous();
+  if (query_start.has_value() && query_start->defined()) {
+    TORCH_CHECK(query_start->device() == like.device() && query_start->scalar_type() == at::kInt && query_start->dim() == 1 &&
+                    query_start->size(0) == sequences + 1, "query_start must be int32 [", sequences + 1, "] on the rows' device");
+    r.start = query_start->contiguous();
+  } else {
+    TORCH_CHECK(rows == sequences, "without query_start a sequence has one row: ", rows, " rows, ", sequences, " sequences");
+  }
+  r.sequences = static_cast<int>(sequences);
+  return r;
+}
+
+// base + scaling * (x lora_a^T) lora_b^T for every row with the adapter of its sequence; low [rows, rank] float32 (or none): x lora_a^T
+at::Tensor lora_add(const at::Tensor& x, const at::Tensor& base, const at::Tensor& lora_a, const at::Tensor& lora_b, const at::Tensor& scaling,
+                    const at::Tensor& adapter, const c10::optional<at::Tensor>& query_start, const c10::optional<at::Tensor>& out,
+                    const c10::optional<at::Tensor>& low) {
+  TORCH_CHECK(x.is_cuda(), "x must be a CUDA tensor");
+  const int dtype = dtype_code(x, "x");
+  TORCH_CHECK(x.dim() == 2 && base.dim() == 2 && base.size(0) == x.size(0) && base.device() == x.device() && base.scalar_type() == x.scalar_type(),
+              "x must be [rows, in], base [rows, out] of x's dtype on its device");
+  const int64_t rows = x.size(0);
+  const Adapters l = adapters_of(x, lora_a, lora_b, scaling, adapter, query_start, rows);
+  TORCH_CHECK(x.size(1) == l.in && base.size(1) == l.out, "the adapters are ", l.in, " x ", l.out, ", x and base ", x.size(1), " x ", base.size(1));
+  const c10::OptionalDeviceGuard guard(at::device_of(x));
+  const auto xr = own_rows(x), br = own_rows(base);
+  at::Tensor result;
+  if (out.has_value() && out->defined()) {
+    TORCH_CHECK(out->device() == x.device() && out->scalar_type() == x.scalar_type() && out->is_contiguous() && out->dim() == 2 &&
+                    out->size(0) == rows && out->size(1) == l.out && reinterpret_cast<uintptr_t>(out->const_data_ptr()) % 16 == 0,
+                "out must be contiguous [", rows, ", ", l.out, "] of x's dtype, 16-byte aligned");
+    const bool in_place = out->const_data_ptr() == br.const_data_ptr() && br.is_contiguous();
+    for (const at::Tensor* t : {&xr, &lora_a, &lora_b, &scaling, &l.adapter, &l.start})
+      TORCH_CHECK(!t->defined() || !shares_memory(*out, *t), "out must not share memory with x, the adapters, adapter or query_start");
+    TORCH_CHECK(in_place || !shares_memory(*out, br), "out must be base or not share memory with it");
+    result = *out;
+  } else {
+    result = at::empty({rows, l.out}, x.options());
+  }
+  float* low_ptr = nullptr;
+  if (low.has_value() && low->defined()) {
+    TORCH_CHECK(low->device() == x.device() && low->scalar_type() == at::kFloat && low->is_contiguous() && low->dim() == 2 && low->size(0) == rows &&
+                    low->size(1) == l.rank && reinterpret_cast<uintptr_t>(low->const_data_ptr()) % 16 == 0,
+                "low must be contiguous float32 [", rows, ", ", l.rank, "], 16-byte aligned");
+    for (const at::Tensor* t : {&xr, &br, &lora_a, &lora_b, &scaling, &l.adapter, &l.start})
+      TORCH_CHECK(!t->defined() || !shares_memory(*low, *t), "low must not share memory with the inputs");
+    TORCH_CHECK(!shares_memory(*low, result), "low must not share memory with out");
+    low_ptr = low->mutable_data_ptr<float>();
+  }
+  if (rows == 0) return result;
+  if (l.sequences == 0) {
+    if (result.const_data_ptr() != br.const_data_ptr()) result.copy_(br);
+    if (low_ptr) at::Tensor(*low).zero_();
+    return result;
+  }
+  const size_t need = llmq_lora_add_workspace_bytes(static_cast<int>(rows), l.sequences, l.start.defined(), static_cast<int>(l.in),
+                                                    static_cast<int>(l.rank), dtype);
+  const auto workspace = at::empty({static_cast<int64_t>(need)}, x.options().dtype(at::kByte));
+  check_rc(llmq_lora_add(xr.const_data_ptr(), own_stride(xr), br.const_data_ptr(), own_stride(br), lora_a.const_data_ptr(), lora_b.const_data_ptr(),
+                         scaling.const_data_ptr<float>(), l.adapter.const_data_ptr<int32_t>(), l.start_or_null(), result.mutable_data_ptr(),
+                         low_ptr, workspace.mutable_data_ptr(), need, static_cast<int>(rows), l.sequences, static_cast<int>(l.in),
+                         static_cast<int>(l.out), static_cast<int>(l.rank), static_cast<int>(l.slots), dtype, current_stream(x)),
+           "lora_add");
+  return result;
+}
+
+// (gradient of x, of lora_a, of lora_b) from that of lora_add's result; x as it was, or its int8 codes with x_scale
+std::tuple<at::Tensor, at::Tensor, at::Tensor> lora_grad(const at::Tensor& grad, const at::Tensor& x, const at::Tensor& low, const at::Tensor& lora_a,
+                                                         const at::Tensor& lora_b, const at::Tensor& scaling, const at::Tensor& adapter,
+                                                         const c10::optional<at::Tensor>& query_start, const c10::optional<at::Tensor>& grad_base,
+                                                         const c10::optional<at::Tensor>& x_scale) {
+  TORCH_CHECK(grad.is_cuda(), "grad must be a CUDA tensor");
+  const int dtype = dtype_code(grad, "grad");
+  TORCH_CHECK(grad.dim() == 2 && x.dim() == 2 && x.size(0) == grad.size(0) && x.device() == grad.device(),
+              "grad must be [rows, out], x [rows, in] on its device");
+  const int64_t rows = grad.size(0);
+  const Adapters l = adapters_of(grad, lora_a, lora_b, scaling, adapter, query_start, rows);
+  TORCH_CHECK(x.size(1) == l.in && grad.size(1) == l.out, "the adapters are ", l.in, " x ", l.out, ", x and grad ", x.size(1), " x ", grad.size(1));
+  TORCH_CHECK(low.device() == grad.device() && low.scalar_type() == at::kFloat && low.dim() == 2 && low.size(0) == rows && low.size(1) == l.rank,
+              "low must be float32 [", rows, ", ", l.rank, "] on grad's device");
+  at::Tensor scale;
+  if (x_scale.has_value() && x_scale->defined()) {
+    TORCH_CHECK(x.scalar_type() == at::kChar && l.in % 128 == 0, "x with x_scale must be int8 codes in groups of 128");
+    TORCH_CHECK(x_scale->device() == grad.device() && x_scale->scalar_type() == at::kFloat && x_scale->dim() == 2 && x_scale->size(0) == rows &&
+                    x_scale->size(1) == l.in / 128, "x_scale must be float32 [", rows, ", ", l.in / 128, "] on grad's device");
+    scale = x_scale->contiguous();
+  } else {
+    TORCH_CHECK(x.scalar_type() == grad.scalar_type(), "x must have grad's dtype (or be int8 codes with x_scale)");
+  }
+  const c10::OptionalDeviceGuard guard(at::device_of(grad));
+  auto grad_x = at::empty({rows, l.in}, grad.options());
+  at::Tensor base;
+  if (grad_base.has_value() && grad_base->defined()) {
+    TORCH_CHECK(grad_base->device() == grad.device() && grad_base->scalar_type() == grad.scalar_type() && grad_base->dim() == 2 &&
+                    grad_base->size(0) == rows && grad_base->size(1) == l.in, "grad_base must be [", rows, ", ", l.in, "] of grad's dtype on its device");
+    base = own_rows(*grad_base);
+  }
+  if (rows == 0 || l.sequences == 0 || l.slots == 0) {
+    if (base.defined()) grad_x.copy_(base); else grad_x.zero_();
+    return {grad_x, at::zeros_like(lora_a), at::zeros_like(lora_b)};
+  }
+  auto grad_a = at::empty_like(lora_a), grad_b = at::empty_like(lora_b);
+  const auto gr = own_rows(grad), xr = own_rows(x), lr = packet_rows(low.contiguous());
+  const size_t need = llmq_lora_grad_workspace_bytes(static_cast<int>(rows), l.sequences, l.start.defined(), static_cast<int>(l.in),
+                                                     static_cast<int>(l.out), static_cast<int>(l.rank), static_cast<int>(l.slots), dtype);
+  const auto workspace = at::empty({static_cast<int64_t>(need)}, grad.options().dtype(at::kByte));
+  check_rc(llmq_lora_grad(gr.const_data_ptr(), own_stride(gr), xr.const_data_ptr(), own_stride(xr), scale.defined() ? scale.const_data_ptr<float>() : nullptr,
+                          lr.const_data_ptr<float>(), lora_a.const_data_ptr(), lora_b.const_data_ptr(), scaling.const_data_ptr<float>(),
+                          l.adapter.const_data_ptr<int32_t>(), l.start_or_null(), base.defined() ? base.const_data_ptr() : nullptr,
+                          base.defined() ? own_stride(base) : l.in, grad_x.mutable_data_ptr(), grad_a.mutable_data_ptr(), grad_b.mutable_data_ptr(),
+                          workspace.mutable_data_ptr(), need, static_cast<int>(rows), l.sequences, static_cast<int>(l.in), static_cast<int>(l.out),
+                          static_cast<int>(l.rank), static_cast<int>(l.slots), dtype, current_stream(grad)),
+           "lora_grad");
+  return {grad_x, grad_a, grad_b};
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -2113,5 +2250,11 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("vocab_loss_grad", &vocab_loss_grad, "Gradients of vocab_loss by hidden and, where wanted, a dense weight",
         py::arg("hidden"), py::arg("weight"), py::arg("targets"), py::arg("lse"), py::arg("grad"), py::arg("ignore_index") = -100,
         py::arg("wscale") = py::none(), py::arg("out_group") = 0, py::arg("want_weight") = false);
+  m.def("lora_add", &lora_add, "base + scaling * (x lora_a^T) lora_b^T, each row with the adapter of its sequence (a slot that does not exist: none)",
+        py::arg("x"), py::arg("base"), py::arg("lora_a"), py::arg("lora_b"), py::arg("scaling"), py::arg("adapter"),
+        py::arg("query_start") = py::none(), py::arg("out") = py::none(), py::arg("low") = py::none());
+  m.def("lora_grad", &lora_grad, "Gradients of lora_add by x (added to grad_base), lora_a and lora_b; x as it was or its 8-bit codes",
+        py::arg("grad"), py::arg("x"), py::arg("low"), py::arg("lora_a"), py::arg("lora_b"), py::arg("scaling"), py::arg("adapter"),
+        py::arg("query_start") = py::none(), py::arg("grad_base") = py::none(), py::arg("x_scale") = py::none());
   m.def("abi_version", []() { return llmq_abi_version(); });
 }

@@ -214,6 +214,14 @@ def load_capi() -> ctypes.CDLL:
     lib.llmq_vocab_loss_grad_workspace_bytes.restype = c_size
     lib.llmq_vocab_loss_grad.argtypes = [c_p, c_i64] + [c_p] * 3 + [c_i64] + [c_p] * 5 + [c_size] + [c_int] * 7 + [c_p]
     lib.llmq_vocab_loss_grad.restype = c_int
+    lib.llmq_lora_add_workspace_bytes.argtypes = [c_int] * 6
+    lib.llmq_lora_add_workspace_bytes.restype = c_size
+    lib.llmq_lora_add.argtypes = [c_p, c_i64, c_p, c_i64] + [c_p] * 8 + [c_size] + [c_int] * 7 + [c_p]
+    lib.llmq_lora_add.restype = c_int
+    lib.llmq_lora_grad_workspace_bytes.argtypes = [c_int] * 8
+    lib.llmq_lora_grad_workspace_bytes.restype = c_size
+    lib.llmq_lora_grad.argtypes = [c_p, c_i64, c_p, c_i64] + [c_p] * 8 + [c_i64] + [c_p] * 4 + [c_size] + [c_int] * 7 + [c_p]
+    lib.llmq_lora_grad.restype = c_int
     for name in ("llmq_fake_quant_group", "llmq_quant_group_codes", "llmq_wq_gemv", "llmq_kv_append",
                  "llmq_kv_dequant", "llmq_kv_decode_attention"):
         getattr(lib, name).restype = c_int
