@@ -34,6 +34,7 @@ def kv_cache_bytes_per_token(model, num_bits: int | None) -> int:
 
 
 def deployed_cost(model, kv_cache_bits: int | None = None) -> dict:
+    from llmquant.quantizers.adapters import LoraAdapters
     from llmquant.quantizers.experts import _QuantExperts
     from llmquant.quantizers.kernel import KernelQuantLinear
     from llmquant.quantizers.real import RealQuantLinear
@@ -64,6 +65,12 @@ def deployed_cost(model, kv_cache_bits: int | None = None) -> dict:
             bits += nbytes * 8
             elements += real
             owned.update(id(t) for t in list(module.parameters(recurse=False)) + list(module.buffers(recurse=False)))
+        elif isinstance(module, LoraAdapters):   # a token reads one adapter of the bank
+            tensors = list(module.parameters(recurse=False)) + list(module.buffers(recurse=False))
+            nbytes = sum(t.numel() * t.element_size() for t in tensors)
+            disk += nbytes
+            decode += nbytes // module.scaling.numel()
+            owned.update(id(t) for t in tensors)
         elif isinstance(module, _QuantExperts):
             tensors = list(module.buffers(recurse=False))
             nbytes = sum(t.numel() * t.element_size() for t in tensors)

@@ -3,6 +3,7 @@
 from __future__ import annotations
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from llmquant.core.observers import pad_to_group
 from llmquant.core.scheme import QuantizationArgs
@@ -56,3 +57,61 @@ def quantize_activation(x: torch.Tensor, args: QuantizationArgs):
 
 # the reference's name for the same op
 fake_quantize_cuda = fake_quantize_hip
+
+
+class _VocabLoss(torch.autograd.Function):
+    """Losses of rows over a vocabulary; the logits are made again in the backward pass, a piece at a time."""
+
+    @staticmethod
+    def forward(ctx, hidden, weight, wscale, out_group, targets, ignore_index):
+        losses, lse = load_extension().vocab_loss(hidden, weight, targets, ignore_index, wscale, out_group)
+        ctx.save_for_backward(hidden, weight, wscale, targets, lse)
+        ctx.out_group, ctx.ignore_index = out_group, ignore_index
+        return losses
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad):
+        hidden, weight, wscale, targets, lse = ctx.saved_tensors
+        of_hidden, of_weight = load_extension().vocab_loss_grad(hidden, weight, targets, lse, grad, ctx.ignore_index, wscale,
+                                                                ctx.out_group, ctx.needs_input_grad[1])
+        return of_hidden, of_weight, None, None, None, None
+
+
+def _head_weight(head):
+    """(weight or codes, scales or None, out_group) of an lm_head: a tensor, a Linear without bias, a kernel-mode Linear."""
+    if isinstance(head, torch.Tensor):
+        return head, None, 0
+    if getattr(head, "bias", None) is not None:
+        raise ValueError("a head with a bias has no fused loss")
+    if getattr(head, "adapters", None) is not None:
+        raise ValueError("a head with adapters has no fused loss")
+    if hasattr(head, "qdata"):
+        if head._needs_padding or head._int8_act:
+            raise ValueError("a fused loss takes a weight-only head of whole groups")
+        return head.qdata, head.wscale, head.out_group
+    scheme = getattr(head, "scheme", None)
+    weight = getattr(head, "weight", None)
+    if weight is None or weight.dim() != 2 or (scheme is not None and scheme.input_activations is not None):
+        raise TypeError(f"{type(head).__name__} is no head that a fused loss takes")
+    return weight, None, 0
+
+
+def vocab_cross_entropy(hidden, head, targets, ignore_index: int = -100, reduction: str = "mean"):
+    """F.cross_entropy(head(hidden), targets) without the logits, in float32, differentiable by hidden and by a dense weight.
+
+    hidden [..., hidden size]; head: an nn.Linear without bias, a kernel-mode Linear (its codes are frozen), or a weight [vocab, hidden size];
+    targets int64 [...]. reduction "none", "sum", or "mean" over the rows whose target is not ignore_index (NaN if there is none,
+    as F.cross_entropy has it). A target outside the vocabulary makes its loss NaN.
+    """
+    if reduction not in ("none", "sum", "mean"):
+        raise ValueError(f"reduction must be 'none', 'sum' or 'mean', got {reduction!r}")
+    weight, wscale, out_group = _head_weight(head)
+    if targets.shape != hidden.shape[:-1]:
+        raise ValueError(f"targets {tuple(targets.shape)} do not go with hidden {tuple(hidden.shape)}")
+    rows = hidden.reshape(-1, hidden.shape[-1])
+    losses = _VocabLoss.apply(rows, weight, wscale, out_group, targets.reshape(-1), ignore_index)
+    if reduction == "none":
+        return losses.reshape(targets.shape)
+    total = losses.sum()
+    return total if reduction == "sum" else total / (targets != ignore_index).sum()

@@ -11,6 +11,7 @@ from __future__ import annotations
 
 import torch
 import torch.nn as nn
+from torch.autograd.function import once_differentiable
 
 from llmquant.core.observers import group_view, pad_to_group
 from llmquant.core.scheme import QuantizationScheme
@@ -132,11 +133,49 @@ def pad_activation(flat: torch.Tensor, args) -> torch.Tensor:
     return pad_to_group(heads, args.group_size).flatten(-2)
 
 
+class _FrozenCodes(torch.autograd.Function):
+    """A kernel-mode Linear with a gradient by its input and its bias: the codes are frozen. 8-bit activations pass their gradient
+    straight through."""
+
+    @staticmethod
+    def forward(ctx, x, bias, module):
+        ctx.module = module
+        ctx.save_for_backward(module.qdata, module.wscale)   # (changed in place before the backward pass: an error, as for any weight)
+        return module._frozen(x)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad):
+        module, of_x, of_bias = ctx.module, None, None
+        qdata, wscale = ctx.saved_tensors
+        rows = grad.reshape(-1, grad.shape[-1])
+        if ctx.needs_input_grad[0]:
+            groups = qdata.shape[1]
+            group_size = module.padded_in_features // groups
+            keep = module._head_keep or group_size
+            if group_size % 8 == 0 and keep % 8 == 0 and module.out_features % 8 == 0:
+                of_x = module._ext.wq_linear_grad(rows, qdata, wscale, module.out_group, keep)
+            else:
+                of_x = rows @ module._dequantized_weight(rows.dtype, real_width=True)
+            # (zeros behind a row that is no whole number of groups; heads padded to groups otherwise)
+            if of_x.shape[1] != module.in_features:
+                head_dim = module._weight_args.head_dim
+                if head_dim and module.in_features % head_dim == 0 and of_x.shape[1] % (module.in_features // head_dim) == 0:
+                    of_x = of_x.unflatten(1, (module.in_features // head_dim, -1))[..., :head_dim].flatten(1)
+                else:
+                    of_x = of_x[:, :module.in_features]
+            of_x = of_x.reshape(*grad.shape[:-1], module.in_features)
+        if ctx.needs_input_grad[1]:
+            of_bias = rows.sum(0, dtype=torch.float32).to(module.bias.dtype)
+        return of_x, of_bias, None
+
+
 class KernelQuantLinear(nn.Module):
     """Linear over a canonical quantized weight: [N, groups, group_size] codes with padding
     and head splits already applied, plus fp32 scales [scale_rows, groups]."""
 
     _few_elements, _head_rows = -1, 0   # (of a module pickled without them)
+    _adapted = False                    # whether low-rank adapters stand beside it (quantizers/adapters.py: `adapters`)
 
     def __init__(self, qweight, wscale, bias, scheme: QuantizationScheme, in_features: int):
         super().__init__()
@@ -274,6 +313,12 @@ class KernelQuantLinear(nn.Module):
         return rows @ self._dequantized_weight(rows.dtype, real_width).T
 
     def forward(self, x):
+        if self._adapted or (x.requires_grad and torch.is_grad_enabled()):
+            out = _FrozenCodes.apply(x, self.bias, self) if x.requires_grad and torch.is_grad_enabled() else self._frozen(x)
+            return self.adapters(x, out) if self._adapted else out
+        return self._frozen(x)
+
+    def _frozen(self, x):
         # (the buffers through their dict: nn.Module.__getattr__ costs a third of a microsecond a look)
         held, bias = self._buffers, self.bias
         qdata, wscale = held["qdata"], held["wscale"]

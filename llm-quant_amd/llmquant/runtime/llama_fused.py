@@ -34,7 +34,7 @@ PRO_NONE, PRO_RMSNORM, PRO_SILU_MUL, PRO_ATTN_MERGE = 0, 1, 2, 3
 def _fusable(*mods) -> bool:
     first = mods[0]
     for m in mods:
-        if not isinstance(m, KernelQuantLinear) or m.bias is not None or m._int8_act:
+        if not isinstance(m, KernelQuantLinear) or m.bias is not None or m._int8_act or m._adapted:
             return False
         if m.qdata.dtype != first.qdata.dtype or m.out_group != first.out_group:
             return False
@@ -159,7 +159,7 @@ class LlamaFusedRuntime(LlamaKernelRuntime):
             if not (_fusable(attn.q_proj, attn.k_proj, attn.v_proj) and _fusable(mlp.gate_proj, mlp.up_proj)
                     and _fusable(attn.o_proj) and _fusable(mlp.down_proj)):
                 raise ValueError("the fused decode step needs kernel-mode Linears (group 128, a multiple of 4 groups per "
-                                 "row, no bias, weight-only) with q/k/v and gate/up sharing a bit width")
+                                 "row, no bias, no adapters, weight-only) with q/k/v and gate/up sharing a bit width")
             for name in ("q_proj", "k_proj", "v_proj"):
                 proj = getattr(attn, name)
                 if proj.out_group and proj.qdata.shape[0] % proj.out_group:
