@@ -87,7 +87,7 @@ constexpr int kShrinkWaves = 4;
 template <typename T, int RT, int NT>
 __global__ __launch_bounds__(kShrinkWaves * kWave) void shrink_kernel(const T* __restrict__ x, const int64_t x_stride, const Bank bank,
                                                                           const Requests req, float* __restrict__ planes, const int64_t plane) {
-  constexpr int V = Pack<T>::N, U = RT + NT <= 4 ? 4 : RT + NT <= 8 ? 2 : 1;
+  constexpr int V = Pack<T>::N, U = 20 / (RT + NT) > 4 ? 4 : 20 / (RT + NT);
   __shared__ v4f s_sum[kShrinkWaves - 1][RT * NT][kWave];
   int first, n;
   const int a = req.template piece<kPieceShift<NT>>(blockIdx.x, bank.slots, first, n);
@@ -176,50 +176,77 @@ struct Expand {
 };
 
 // The columns of MFMA row r of tile mi are named 16 (r / 4) + 4 mi + r % 4, so that a lane's results are 16 neighbours.
-// The bank here is [slots][columns][rank].
+// The bank here is [slots][columns][rank]. The piece's sums are added up once for the workgroup, eight planes in flight, through LDS; the first
+// 64 columns' weights and base are on their way meanwhile (plane after plane in every wave, and base behind the product, had taken 52 us
+// where this takes 17: 333 rows of 20 requests, rank 64, 14336 columns, fp16; 4099 rows of 4096 columns 55 and 25).
 template <typename T, int RT, int NT>
 __global__ __launch_bounds__(kExpandWaves * kWave) void expand_kernel(const Bank bank, const Requests req, const Expand e) {
   constexpr int V = Pack<T>::N, KT = (RT * 16 + 4 * V - 1) / (4 * V);   // steps of the rank: 32 (fp32: 16)
+  constexpr int kRow = RT * 16 + 4, kAhead = 8;
+  __shared__ __attribute__((aligned(16))) float s_low[NT * 16][kRow];
   const int lane = threadIdx.x & (kWave - 1), wv = threadIdx.x / kWave, lr = lane & 15, g = lane >> 4;
   int first, n, a;
-  if (static_cast<int>(blockIdx.x) < e.pieces) {
+  const bool rest = static_cast<int>(blockIdx.x) >= e.pieces;   // rows in front of the first request and behind the last one: the base as it is
+  if (!rest) {
     a = req.template piece<kPieceShift<NT>>(blockIdx.x, bank.slots, first, n);
     if (n <= 0) return;
-  } else {   // rows in front of the first request and behind the last one: the base as it is
+  } else {
     a = -1;
     first = (blockIdx.x - e.pieces) << kPieceShift<NT>;
     n = min(e.rows - first, 1 << kPieceShift<NT>);
   }
-  const bool rest = static_cast<int>(blockIdx.x) >= e.pieces;
   const int begin = rest ? req.rows.first(0) : 0, end = rest ? max(req.rows.first(req.rows.sequences), begin) : 0;
   const int unit0 = (blockIdx.y * kExpandWaves + wv) * e.units;
+  const bool writes_low = e.low != nullptr && blockIdx.y == 0;
+  u32x4 m[KT][4], base[NT][16 / V];
+  const auto request = [&](int c0) {
+    if (e.base != nullptr) {
+#pragma unroll
+      for (int j = 0; j < NT; ++j) {
+        const T* from = static_cast<const T*>(e.base) + (first + min(j * 16 + lr, n - 1)) * e.base_stride;
+#pragma unroll
+        for (int h = 0; h < 16 / V; ++h) base[j][h] = load16(from + min(c0 + g * 16 + h * V, e.columns - V));
+      }
+    }
+    if (a < 0) return;
+#pragma unroll
+    for (int k = 0; k < KT; ++k)
+#pragma unroll
+      for (int mi = 0; mi < 4; ++mi) {
+        const int c = min(c0 + (lr >> 2) * 16 + mi * 4 + (lr & 3), e.columns - 1);
+        // (past the rank the operand of `low` is zeros, against weights that are looked at a second time)
+        m[k][mi] = load16(static_cast<const T*>(bank.m) + (static_cast<int64_t>(a) * e.columns + c) * bank.rank + min((k * 4 + g) * V, bank.rank - V));
+      }
+  };
+  if (unit0 * 64 < e.columns) request(unit0 * 64);
   u32x4 low_hi[NT][KT], low_lo[NT][KT];   // (fp32: low_hi alone)
   if (a >= 0) {
-    const float s = e.scaling != nullptr ? e.scaling[a] : 1.0f;
+    const int quads = bank.rank / 4;
+    for (int item = threadIdx.x; item < n * quads; item += kExpandWaves * kWave) {
+      const int t = item / quads, r = (item - t * quads) * 4;
+      const float* from = e.planes + static_cast<int64_t>(first + t) * bank.rank + r;
+      v4f sum{0.0f, 0.0f, 0.0f, 0.0f};
+      for (int p0 = 0; p0 < e.splits; p0 += kAhead) {
+        v4f v[kAhead];
 #pragma unroll
-    for (int j = 0; j < NT; ++j) {
-      const int64_t row = first + min(j * 16 + lr, n - 1);
+        for (int p = 0; p < kAhead; ++p) v[p] = *reinterpret_cast<const v4f*>(from + min(p0 + p, e.splits - 1) * e.plane);
+#pragma unroll
+        for (int p = 0; p < kAhead; ++p)
+          if (p0 + p < e.splits) sum += v[p];
+      }
+      *reinterpret_cast<v4f*>(&s_low[t][r]) = sum;
+      if (writes_low) *reinterpret_cast<v4f*>(e.low + static_cast<int64_t>(first + t) * bank.rank + r) = sum;
+    }
+    const float s = e.scaling != nullptr ? e.scaling[a] : 1.0f;
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
 #pragma unroll
       for (int k = 0; k < KT; ++k) {
         const int r = (k * 4 + g) * V;
-        float f[V] = {};
-        if (r < bank.rank) {
-          for (int p = 0; p < e.splits; ++p) {
-            const float* from = e.planes + p * e.plane + row * bank.rank + r;
+        float f[V];
 #pragma unroll
-            for (int i = 0; i < V; i += 4) {
-              const v4f v = *reinterpret_cast<const v4f*>(from + i);
-#pragma unroll
-              for (int q = 0; q < 4; ++q) f[i + q] += v[q];
-            }
-          }
-          if (e.low != nullptr && unit0 == 0 && j * 16 + lr < n) {
-#pragma unroll
-            for (int i = 0; i < V; i += 4) *reinterpret_cast<v4f*>(e.low + row * bank.rank + r + i) = v4f{f[i], f[i + 1], f[i + 2], f[i + 3]};
-          }
-        }
-#pragma unroll
-        for (int i = 0; i < V; ++i) f[i] *= s;
+        for (int i = 0; i < V; ++i) f[i] = r < bank.rank ? s_low[min(j * 16 + lr, n - 1)][r + i] * s : 0.0f;
         if constexpr (V == 8) {
           const HiLo v = hi_lo(f);
           low_hi[j][k] = v.hi;
@@ -228,9 +255,8 @@ __global__ __launch_bounds__(kExpandWaves * kWave) void expand_kernel(const Bank
           low_hi[j][k] = Pack<float>::pack(f);
         }
       }
-    }
-  } else if (e.low != nullptr && unit0 == 0) {   // (no adapter: zeros)
-    for (int i = lane; i < n * bank.rank; i += kWave) {
+  } else if (writes_low) {   // (no adapter: zeros)
+    for (int i = threadIdx.x; i < n * bank.rank; i += kExpandWaves * kWave) {
       const int64_t row = first + i / bank.rank;
       if (!rest || row < begin || row >= end) e.low[row * bank.rank + i % bank.rank] = 0.0f;
     }
@@ -238,26 +264,19 @@ __global__ __launch_bounds__(kExpandWaves * kWave) void expand_kernel(const Bank
   for (int u = 0; u < e.units; ++u) {
     const int c0 = (unit0 + u) * 64;
     if (c0 >= e.columns) return;
+    if (u > 0) request(c0);
     v4f acc[NT][4] = {};
     if (a >= 0) {
 #pragma unroll
-      for (int k = 0; k < KT; ++k) {
-        const int r = (k * 4 + g) * V;
-        u32x4 m[4];
-#pragma unroll
-        for (int mi = 0; mi < 4; ++mi) {
-          const int c = min(c0 + (lr >> 2) * 16 + mi * 4 + (lr & 3), e.columns - 1);
-          m[mi] = load16(static_cast<const T*>(bank.m) + (static_cast<int64_t>(a) * e.columns + c) * bank.rank + min(r, bank.rank - V));
-        }
-        // (past the rank the operand of `low` is zeros, against weights that are looked at a second time)
+      for (int k = 0; k < KT; ++k)
 #pragma unroll
         for (int mi = 0; mi < 4; ++mi) {
           if constexpr (sizeof(T) == 4) {
 #pragma unroll
-            for (int j = 0; j < NT; ++j) acc[j][mi] = mfma_packet<float>(m[mi], low_hi[j][k], acc[j][mi]);
+            for (int j = 0; j < NT; ++j) acc[j][mi] = mfma_packet<float>(m[k][mi], low_hi[j][k], acc[j][mi]);
           } else if constexpr (__is_same(T, f16_t)) {
             float f[8];
-            Pack<f16_t>::unpack(m[mi], f);
+            Pack<f16_t>::unpack(m[k][mi], f);
             const HiLo w = hi_lo(f);   // (exact: 11 bits in 16)
 #pragma unroll
             for (int j = 0; j < NT; ++j) {
@@ -268,12 +287,11 @@ __global__ __launch_bounds__(kExpandWaves * kWave) void expand_kernel(const Bank
           } else {
 #pragma unroll
             for (int j = 0; j < NT; ++j) {
-              acc[j][mi] = mfma_16x16x32<bf16_t>(m[mi], low_lo[j][k], acc[j][mi]);
-              acc[j][mi] = mfma_16x16x32<bf16_t>(m[mi], low_hi[j][k], acc[j][mi]);
+              acc[j][mi] = mfma_16x16x32<bf16_t>(m[k][mi], low_lo[j][k], acc[j][mi]);
+              acc[j][mi] = mfma_16x16x32<bf16_t>(m[k][mi], low_hi[j][k], acc[j][mi]);
             }
           }
         }
-      }
     }
 #pragma unroll
     for (int j = 0; j < NT; ++j) {
@@ -285,7 +303,7 @@ __global__ __launch_bounds__(kExpandWaves * kWave) void expand_kernel(const Bank
         const int c = c0 + g * 16 + h * V;
         if (c >= e.columns) continue;
         float f[V] = {};
-        if (e.base != nullptr) Pack<T>::unpack(load16(static_cast<const T*>(e.base) + row * e.base_stride + c), f);
+        if (e.base != nullptr) Pack<T>::unpack(base[j][h], f);
         if (a >= 0) {   // (else the base to the bit: -0 + 0 is +0)
 #pragma unroll
           for (int i = 0; i < V; ++i) f[i] += acc[j][(h * V + i) / 4][i % 4];
@@ -301,96 +319,167 @@ constexpr int kBlock = 32;          // rows of a block: one step of the matrix c
 constexpr int kPlanThreads = 1024;  // and the most slots
 
 // start [slots + 1]: the first virtual row of each slot, a multiple of 32 (rows up to there: none, -1); order: the row behind each
-// virtual row. Requests of a slot keep their order. One workgroup; seq_start: [sequences] scratch.
-__global__ __launch_bounds__(kPlanThreads) void plan_kernel(const Requests req, const int slots, const int capacity, int32_t* __restrict__ start,
-                                                            int32_t* __restrict__ order, int32_t* __restrict__ seq_start) {
-  __shared__ int s_a[kPlanThreads], s_n[kPlanThreads], s_scan[kPlanThreads];
+// virtual row; slot_of: the slot of each block. Requests of a slot keep their order. One workgroup; seq_start: [sequences] scratch.
+struct Plan {
+  int slots, capacity;   // virtual rows at the most
+  int32_t* start;
+  int32_t* order;
+  int32_t* slot_of;
+  int32_t* seq_start;
+};
+struct PlanLds {
+  int a[kPlanThreads], n[kPlanThreads], at[kPlanThreads], seq[kPlanThreads], scan[kPlanThreads];
+};
+__device__ __forceinline__ void make_plan(PlanLds& s, const Requests& req, const Plan& p) {
   const int t = threadIdx.x, sequences = req.rows.sequences;
-  const auto rows_of = [&](int b) { return max(req.rows.first(b + 1) - req.rows.first(b), 0); };
+  const bool few = sequences <= kPlanThreads;   // all requests in LDS
   int mine = 0;
+  for (int v = t * 4; v < p.capacity; v += kPlanThreads * 4) *reinterpret_cast<int4*>(p.order + v) = make_int4(-1, -1, -1, -1);
   for (int pass = 0; pass < 2; ++pass) {
-    int at = pass == 0 ? 0 : start[min(t, slots)];
+    int at = pass == 0 ? 0 : s.scan[t] - mine;
     for (int b0 = 0; b0 < sequences; b0 += kPlanThreads) {
-      __syncthreads();
-      if (b0 + t < sequences) {
-        s_a[t] = req.adapter[b0 + t];
-        s_n[t] = rows_of(b0 + t);
+      if (!few || pass == 0) {
+        __syncthreads();
+        if (b0 + t < sequences) {
+          s.a[t] = req.adapter[b0 + t];
+          s.at[t] = req.rows.first(b0 + t);
+          s.n[t] = max(req.rows.first(b0 + t + 1) - s.at[t], 0);
+        }
+        __syncthreads();
       }
-      __syncthreads();
       const int many = min(sequences - b0, kPlanThreads);
-      if (t < slots) {
+      if (t < p.slots) {
         for (int i = 0; i < many; ++i) {
-          if (s_a[i] != t) continue;
-          if (pass == 1) seq_start[b0 + i] = at;
-          at += s_n[i];
+          if (s.a[i] != t) continue;
+          if (pass == 1) {
+            if (few) s.seq[i] = at;
+            else p.seq_start[b0 + i] = at;
+          }
+          at += s.n[i];
         }
       }
     }
     if (pass == 1) break;
-    mine = t < slots ? (at + kBlock - 1) / kBlock * kBlock : 0;
-    s_scan[t] = mine;
+    mine = t < p.slots ? (at + kBlock - 1) / kBlock * kBlock : 0;
     __syncthreads();
-    for (int d = 1; d < kPlanThreads; d *= 2) {
-      const int v = t >= d ? s_scan[t - d] : 0;
+    s.scan[t] = mine;
+    __syncthreads();
+    for (int d = 1; d < p.slots; d *= 2) {
+      const int v = t >= d ? s.scan[t - d] : 0;
       __syncthreads();
-      s_scan[t] += v;
+      s.scan[t] += v;
       __syncthreads();
     }
-    if (t < slots) start[t] = s_scan[t] - mine;
-    if (t == slots - 1) start[slots] = s_scan[t];
-    __syncthreads();   // (read back below by the same workgroup)
+    if (t < p.slots) p.start[t] = s.scan[t] - mine;
+    if (t == p.slots - 1) p.start[p.slots] = s.scan[t];
   }
-  for (int v = t; v < capacity; v += kPlanThreads) order[v] = -1;
   __syncthreads();
+  for (int block = t; block < p.capacity / kBlock; block += kPlanThreads) {
+    int lo = 0, hi = p.slots - 1;   // the first slot that ends behind the block's begin (none: the last)
+    while (lo < hi) {
+      const int mid = (lo + hi) / 2;
+      if (s.scan[mid] > block * kBlock) hi = mid; else lo = mid + 1;
+    }
+    p.slot_of[block] = lo;
+  }
   for (int row = t; row < req.rows.rows; row += kPlanThreads) {
     int lo = 0, hi = sequences;   // the last request that begins at or in front of the row
     while (lo + 1 < hi) {
       const int mid = (lo + hi) / 2;
-      if (req.rows.first(mid) <= row) lo = mid; else hi = mid;
+      if ((few ? s.at[mid] : req.rows.first(mid)) <= row) lo = mid; else hi = mid;
     }
-    const int in_b = row - req.rows.first(lo);
-    if (in_b < 0 || in_b >= rows_of(lo)) continue;
-    const int a = req.adapter[lo];
-    if (a < 0 || a >= slots) continue;
-    const int v = seq_start[lo] + in_b;
-    if (v < capacity) order[v] = row;
+    const int from = few ? s.at[lo] : req.rows.first(lo), n = few ? s.n[lo] : max(req.rows.first(lo + 1) - from, 0);
+    const int a = few ? s.a[lo] : req.adapter[lo];
+    if (row < from || row - from >= n || a < 0 || a >= p.slots) continue;
+    const int v = (few ? s.seq[lo] : p.seq_start[lo]) + row - from;
+    if (v < p.capacity) p.order[v] = row;
+  }
+}
+
+// The first workgroup makes the plan, the others turn the banks over: lora_a [slots, rank, in] and lora_b [slots, out, rank], 64 x 64 each.
+struct Turn {
+  const void* from;
+  void* to;
+  int rows, cols;   // of a slot
+};
+template <typename E>
+__global__ __launch_bounds__(kPlanThreads) void prepare_kernel(const Requests req, const Plan plan, const Turn a, const Turn b) {
+  union Lds {
+    PlanLds plan;
+    E tile[64][68];
+  };
+  __shared__ __attribute__((aligned(16))) unsigned char s_mem[sizeof(Lds)];
+  Lds& s = *reinterpret_cast<Lds*>(s_mem);
+  if (blockIdx.x == 0) {
+    make_plan(s.plan, req, plan);
+    return;
+  }
+  struct alignas(4 * sizeof(E)) Four { E v[4]; };
+  const int a_cols = (a.cols + 63) / 64, a_tiles = a_cols * ((a.rows + 63) / 64), b_cols = (b.cols + 63) / 64, b_tiles = b_cols * ((b.rows + 63) / 64);
+  const int id = blockIdx.x - 1, of_a = a_tiles * plan.slots;
+  const Turn& turn = id < of_a ? a : b;
+  const int at = id < of_a ? id : id - of_a, tiles = id < of_a ? a_tiles : b_tiles, slot = at / tiles, tile = at - slot * tiles, cols = id < of_a ? a_cols : b_cols;
+  const int r0 = tile / cols * 64, c0 = tile % cols * 64, y = threadIdx.x / 16, x = threadIdx.x % 16 * 4;
+  const int64_t base = static_cast<int64_t>(slot) * turn.rows * turn.cols;
+  if (r0 + y < turn.rows && c0 + x < turn.cols)   // (both are multiples of 8)
+    *reinterpret_cast<Four*>(&s.tile[y][x]) = *reinterpret_cast<const Four*>(static_cast<const E*>(turn.from) + base + static_cast<int64_t>(r0 + y) * turn.cols + c0 + x);
+  __syncthreads();
+  if (c0 + y < turn.cols && r0 + x < turn.rows) {
+    const Four f{{s.tile[x][y], s.tile[x + 1][y], s.tile[x + 2][y], s.tile[x + 3][y]}};
+    *reinterpret_cast<Four*>(static_cast<E*>(turn.to) + base + static_cast<int64_t>(c0 + y) * turn.rows + r0 + x) = f;
   }
 }
 
 // Sums of shrink's planes, times the scaling, as [rows, rank] (du) and, with the kept `low`, as operands of outer: blocks of 32
-// virtual rows, [tile of the rank][block][lane][8], lane 16 g + r holding entry r of the rank of rows 8 g .. 8 g + 7.
-__global__ __launch_bounds__(kWave) void operands_kernel(const float* __restrict__ planes, const int64_t plane, const int splits,
-                                                         const float* __restrict__ low, const float* __restrict__ scaling, const int rank,
-                                                         const int slots, const int32_t* __restrict__ start, const int32_t* __restrict__ order,
-                                                         float* __restrict__ du, float* __restrict__ op_du, float* __restrict__ op_low) {
-  const int block = blockIdx.x, tile = blockIdx.y, lane = threadIdx.x, g = lane >> 4, r = tile * 16 + (lane & 15);
-  if (block * kBlock >= start[slots]) return;
-  int lo = 0, hi = slots;   // the slot: the last one that begins at or in front of the block (empty ones begin where the next does)
-  while (lo + 1 < hi) {
-    const int mid = (lo + hi) / 2;
-    if (start[mid] <= block * kBlock) lo = mid; else hi = mid;
-  }
-  const float s = scaling[lo];
-  float d[8], l[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const int row = order[block * kBlock + 8 * g + i];
-    float sum = 0.0f;
-    l[i] = 0.0f;
-    if (row >= 0 && r < rank) {
+// virtual rows, [tile of the rank][block][lane][8], lane 16 g + r holding entry r of the rank of rows 8 g .. 8 g + 7. A workgroup a block.
+constexpr int kOperandThreads = 256;
+__global__ __launch_bounds__(kOperandThreads) void operands_kernel(const float* __restrict__ planes, const int64_t plane, const int splits,
+                                                                   const float* __restrict__ low, const float* __restrict__ scaling, const int rank,
+                                                                   const Plan plan, float* __restrict__ du, float* __restrict__ op_du,
+                                                                   float* __restrict__ op_low) {
+  constexpr int kAhead = 8, kRow = 132;
+  __shared__ __attribute__((aligned(16))) float s_du[kBlock][kRow], s_lo[kBlock][kRow];
+  const int block = blockIdx.x, quads = rank / 4;
+  if (block * kBlock >= plan.start[plan.slots]) return;
+  const float s = scaling[plan.slot_of[block]];
+  for (int item = threadIdx.x; item < kBlock * quads; item += kOperandThreads) {
+    const int t = item / quads, r = (item - t * quads) * 4, row = plan.order[block * kBlock + t];
+    v4f d{0.0f, 0.0f, 0.0f, 0.0f}, l = d;
+    if (row >= 0) {
       const int64_t at = static_cast<int64_t>(row) * rank + r;
-      for (int p = 0; p < splits; ++p) sum += planes[p * plane + at];
-      sum *= s;
-      du[at] = sum;
-      l[i] = low[at] * s;
-    }
-    d[i] = sum;
-  }
-  const int64_t to = ((static_cast<int64_t>(tile) * gridDim.x + block) * kWave + lane) * 8;
+      l = *reinterpret_cast<const v4f*>(low + at) * s;
+      for (int p0 = 0; p0 < splits; p0 += kAhead) {
+        v4f v[kAhead];
 #pragma unroll
-  for (int i = 0; i < 8; i += 4) {
-    *reinterpret_cast<v4f*>(op_du + to + i) = v4f{d[i], d[i + 1], d[i + 2], d[i + 3]};
-    *reinterpret_cast<v4f*>(op_low + to + i) = v4f{l[i], l[i + 1], l[i + 2], l[i + 3]};
+        for (int p = 0; p < kAhead; ++p) v[p] = *reinterpret_cast<const v4f*>(planes + min(p0 + p, splits - 1) * plane + at);
+#pragma unroll
+        for (int p = 0; p < kAhead; ++p)
+          if (p0 + p < splits) d += v[p];
+      }
+      d *= s;
+      *reinterpret_cast<v4f*>(du + at) = d;
+    }
+    *reinterpret_cast<v4f*>(&s_du[t][r]) = d;
+    *reinterpret_cast<v4f*>(&s_lo[t][r]) = l;
+  }
+  __syncthreads();
+  const int tiles = (rank + 15) / 16;
+  for (int item = threadIdx.x; item < tiles * kWave; item += kOperandThreads) {
+    const int tile = item / kWave, lane = item % kWave, r = tile * 16 + (lane & 15), t = (lane >> 4) * 8;
+    const int64_t to = ((static_cast<int64_t>(tile) * gridDim.x + block) * kWave + lane) * 8;
+#pragma unroll
+    for (int i = 0; i < 8; i += 4) {
+      v4f d{0.0f, 0.0f, 0.0f, 0.0f}, l = d;
+      if (r < rank) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          d[q] = s_du[t + i + q][r];
+          l[q] = s_lo[t + i + q][r];
+        }
+      }
+      *reinterpret_cast<v4f*>(op_du + to + i) = d;
+      *reinterpret_cast<v4f*>(op_low + to + i) = l;
+    }
   }
 }
 
@@ -412,105 +501,110 @@ struct Outer {
 };
 constexpr int kColumns = 128;   // of a wave: one group of the codes
 
-// One side's sums over the rows of a piece for 128 columns and 16 RTW of the rank.
+// One side's sums over the rows of a piece for 128 columns and 16 RTW of the rank. A step's rows and operands are asked for a step ahead, their
+// numbers two.
+template <typename T, bool CODES> struct OuterRows {   // eight columns of eight rows (fp32 values: four of eight, twice)
+  static constexpr int kWords = CODES ? 2 : sizeof(T) == 4 ? 8 : 4;
+  uint32_t w[8][kWords];
+};
 template <typename T, bool CODES, int RTW>
 __device__ __forceinline__ void outer_rows(const OuterSide& side, const Outer& o, int c0, int v0, int v1, v4f (&acc)[RTW][8]) {
   const int lane = threadIdx.x & (kWave - 1), wv = threadIdx.x / kWave, lr = lane & 15, g = lane >> 4;
+  const int tile0 = blockIdx.z * RTW, step = 4 * kBlock;
+  const int begin = v0 + wv * kBlock;
+  if (begin >= v1) return;
   const int spare = max(o.order[v0], 0);   // (the first row of a block: real)
-  const int tile0 = blockIdx.z * RTW;
-  for (int v = v0 + wv * kBlock; v < v1; v += 4 * kBlock) {
-    int64_t row[8];
+  const auto rows_at = [&](int v, int (&row)[8]) {
+    const int at = min(v, v1 - kBlock) + 8 * g;
+    const int4 lo = *reinterpret_cast<const int4*>(o.order + at), hi = *reinterpret_cast<const int4*>(o.order + at + 4);
+    const int got[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+#pragma unroll
+    for (int i = 0; i < 8; ++i) row[i] = got[i] >= 0 ? got[i] : spare;   // (its other factor is zero; a row of this slot, so that nothing foreign gets in)
+  };
+  const auto ask = [&](int v, const int (&row)[8], OuterRows<T, CODES>& x, float (&f)[RTW][8], float (&s)[8]) {
+    const int block = min(v, v1 - kBlock) / kBlock;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const int at = o.order[v + 8 * g + i];
-      row[i] = at >= 0 ? at : spare;   // (its other factor is zero; a row of this slot, so that nothing foreign gets in)
+      if constexpr (CODES) {
+        const u32x2 w = *reinterpret_cast<const u32x2*>(static_cast<const int8_t*>(side.x) + row[i] * side.stride + min(c0 + 8 * lr, side.width - 8));
+        x.w[i][0] = w.x;
+        x.w[i][1] = w.y;
+        s[i] = side.x_scale[static_cast<int64_t>(row[i]) * (side.width / kColumns) + c0 / kColumns];
+      } else if constexpr (sizeof(T) == 4) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const u32x4 w = load16(static_cast<const float*>(side.x) + row[i] * side.stride + min(c0 + 64 * h + 4 * lr, side.width - 4));
+          x.w[i][4 * h] = w.x; x.w[i][4 * h + 1] = w.y; x.w[i][4 * h + 2] = w.z; x.w[i][4 * h + 3] = w.w;
+        }
+      } else {
+        const u32x4 w = load16(static_cast<const T*>(side.x) + row[i] * side.stride + min(c0 + 8 * lr, side.width - 8));
+        x.w[i][0] = w.x; x.w[i][1] = w.y; x.w[i][2] = w.z; x.w[i][3] = w.w;
+      }
     }
-    float f[RTW][8];
 #pragma unroll
     for (int i = 0; i < RTW; ++i) {
       const int tile = min(tile0 + i, (o.rank + 15) / 16 - 1);
-      const float* from = side.op + ((static_cast<int64_t>(tile) * o.blocks + v / kBlock) * kWave + lane) * 8;
+      const float* from = side.op + ((static_cast<int64_t>(tile) * o.blocks + block) * kWave + lane) * 8;
 #pragma unroll
       for (int q = 0; q < 8; q += 4) {
         const v4f w = *reinterpret_cast<const v4f*>(from + q);
         f[i][q] = w[0]; f[i][q + 1] = w[1]; f[i][q + 2] = w[2]; f[i][q + 3] = w[3];
       }
     }
-    if constexpr (CODES) {
-      float s[8];
+  };
+  int row[8];
+  OuterRows<T, CODES> x;
+  float f[RTW][8], s[8];
+  rows_at(begin, row);
+  ask(begin, row, x, f, s);
+  rows_at(begin + step, row);
+  for (int v = begin; v < v1; v += step) {
+    OuterRows<T, CODES> now = x;
+    float u[RTW][8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) s[i] = side.x_scale[row[i] * (side.width / kColumns) + c0 / kColumns];
+    for (int i = 0; i < RTW; ++i)
 #pragma unroll
-      for (int i = 0; i < RTW; ++i)
+      for (int q = 0; q < 8; ++q) u[i][q] = CODES ? f[i][q] * s[q] : f[i][q];
+    ask(v + step, row, x, f, s);   // (behind the last step: that one again)
+    rows_at(v + 2 * step, row);
+    if constexpr (sizeof(T) == 4) {   // e-th product: row 8 g + e of each lane
 #pragma unroll
-        for (int q = 0; q < 8; ++q) f[i][q] *= s[q];
-    }
-    if constexpr (sizeof(T) == 4) {   // rows 8 g + e, four neighbouring columns a load: e-th step takes row e of each lane
+      for (int e = 0; e < 8; ++e)
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int c = min(c0 + (CODES ? 8 * lr + 4 * h : 64 * h + 4 * lr), side.width - 4);
+        for (int q = 0; q < 8; ++q) {
+          float value;
+          if constexpr (CODES) value = static_cast<float>(static_cast<int8_t>(now.w[e][q / 4] >> (8 * (q % 4))));
+          else value = __builtin_bit_cast(float, now.w[e][q]);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          float x[4];
-          if constexpr (CODES) {
-            const uint32_t w = *reinterpret_cast<const uint32_t*>(static_cast<const int8_t*>(side.x) + row[e] * side.stride + c);
-#pragma unroll
-            for (int q = 0; q < 4; ++q) x[q] = static_cast<float>(static_cast<int8_t>(w >> (8 * q)));
-          } else {
-            Pack<float>::unpack(load16(static_cast<const float*>(side.x) + row[e] * side.stride + c), x);
-          }
-#pragma unroll
-          for (int q = 0; q < 4; ++q)
-#pragma unroll
-            for (int i = 0; i < RTW; ++i) acc[i][h * 4 + q] = mfma_f32(x[q], f[i][e], acc[i][h * 4 + q]);
+          for (int i = 0; i < RTW; ++i) acc[i][q] = mfma_f32(value, u[i][e], acc[i][q]);
         }
-      }
     } else {
-      HiLo u[RTW];
+      HiLo other[RTW];
 #pragma unroll
-      for (int i = 0; i < RTW; ++i) u[i] = hi_lo(f[i]);
-      const int c = min(c0 + 8 * lr, side.width - 8);
-      if constexpr (CODES || __is_same(T, f16_t)) {
-        float x[8][8];   // rows, columns
+      for (int i = 0; i < RTW; ++i) other[i] = hi_lo(u[i]);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          if constexpr (CODES) {
-            const u32x2 w = *reinterpret_cast<const u32x2*>(static_cast<const int8_t*>(side.x) + row[e] * side.stride + c);
+      for (int q = 0; q < 8; ++q) {   // column q of the lane's eight
+        HiLo w;
+        if constexpr (CODES || __is_same(T, f16_t)) {
+          float column[8];
 #pragma unroll
-            for (int q = 0; q < 8; ++q) x[e][q] = static_cast<float>(static_cast<int8_t>((q < 4 ? w.x : w.y) >> (8 * (q % 4))));
-          } else {
-            Pack<f16_t>::unpack(load16(static_cast<const f16_t*>(side.x) + row[e] * side.stride + c), x[e]);
+          for (int e = 0; e < 8; ++e) {
+            if constexpr (CODES) column[e] = static_cast<float>(static_cast<int8_t>(now.w[e][q / 4] >> (8 * (q % 4))));
+            else column[e] = static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(now.w[e][q / 2] >> (16 * (q % 2)))));
           }
-        }
-#pragma unroll
-        for (int q = 0; q < 8; ++q) {
-          const float column[8] = {x[0][q], x[1][q], x[2][q], x[3][q], x[4][q], x[5][q], x[6][q], x[7][q]};
-          const HiLo w = hi_lo(column);   // (codes: the first alone; fp16: exact)
-#pragma unroll
-          for (int i = 0; i < RTW; ++i) {
-            if constexpr (!CODES) acc[i][q] = mfma_16x16x32<bf16_t>(w.lo, u[i].hi, acc[i][q]);
-            acc[i][q] = mfma_16x16x32<bf16_t>(w.hi, u[i].lo, acc[i][q]);
-            acc[i][q] = mfma_16x16x32<bf16_t>(w.hi, u[i].hi, acc[i][q]);
-          }
-        }
-      } else {
-        u32x4 raw[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) raw[e] = load16(static_cast<const bf16_t*>(side.x) + row[e] * side.stride + c);
-        const auto word = [&](int e, int w) { return w == 0 ? raw[e].x : w == 1 ? raw[e].y : w == 2 ? raw[e].z : raw[e].w; };
-#pragma unroll
-        for (int q = 0; q < 8; ++q) {
+          w = hi_lo(column);   // (codes: the first alone; fp16: exact)
+        } else {
           const uint32_t select = q % 2 ? 0x07060302u : 0x05040100u;   // the halves of two rows' words
-          u32x4 w;
-          w.x = __builtin_amdgcn_perm(word(1, q / 2), word(0, q / 2), select);
-          w.y = __builtin_amdgcn_perm(word(3, q / 2), word(2, q / 2), select);
-          w.z = __builtin_amdgcn_perm(word(5, q / 2), word(4, q / 2), select);
-          w.w = __builtin_amdgcn_perm(word(7, q / 2), word(6, q / 2), select);
+          w.hi.x = __builtin_amdgcn_perm(now.w[1][q / 2], now.w[0][q / 2], select);
+          w.hi.y = __builtin_amdgcn_perm(now.w[3][q / 2], now.w[2][q / 2], select);
+          w.hi.z = __builtin_amdgcn_perm(now.w[5][q / 2], now.w[4][q / 2], select);
+          w.hi.w = __builtin_amdgcn_perm(now.w[7][q / 2], now.w[6][q / 2], select);
+        }
 #pragma unroll
-          for (int i = 0; i < RTW; ++i) {
-            acc[i][q] = mfma_16x16x32<bf16_t>(w, u[i].lo, acc[i][q]);
-            acc[i][q] = mfma_16x16x32<bf16_t>(w, u[i].hi, acc[i][q]);
-          }
+        for (int i = 0; i < RTW; ++i) {
+          if constexpr (!CODES && __is_same(T, f16_t)) acc[i][q] = mfma_16x16x32<bf16_t>(w.lo, other[i].hi, acc[i][q]);
+          acc[i][q] = mfma_16x16x32<bf16_t>(w.hi, other[i].lo, acc[i][q]);
+          acc[i][q] = mfma_16x16x32<bf16_t>(w.hi, other[i].hi, acc[i][q]);
         }
       }
     }
@@ -571,6 +665,7 @@ __global__ __launch_bounds__(4 * kWave) void outer_kernel(const Outer o) {
 // for B [slots, width, rank]. A slot without rows has a gradient of zero.
 template <typename T>
 __global__ __launch_bounds__(256) void records_kernel(const Outer o, T* __restrict__ grad_a, T* __restrict__ grad_b, const int64_t a_items, const int64_t items) {
+  constexpr int kAhead = 4;
   for (int64_t item = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; item < items; item += static_cast<int64_t>(gridDim.x) * 256) {
     const bool of_b = item >= a_items;
     const OuterSide& side = of_b ? o.b : o.a;
@@ -586,30 +681,25 @@ __global__ __launch_bounds__(256) void records_kernel(const Outer o, T* __restri
     }
     const int n = o.start[slot + 1] - o.start[slot], first = (o.start[slot] >> o.shift) + 2 * slot, pieces = (n + (1 << o.shift) - 1) >> o.shift;
     float f[8] = {};
-    for (int p = 0; p < pieces; ++p) {
-      const float* from = side.records + (first + p) * each + static_cast<int64_t>(r) * side.width + c;
+    const int64_t next = of_b ? side.width : 1;
+    for (int p0 = 0; p0 < pieces; p0 += kAhead) {
+      float v[kAhead][8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) f[i] += of_b ? from[static_cast<int64_t>(i) * side.width] : from[i];
+      for (int p = 0; p < kAhead; ++p) {
+        const float* from = side.records + (first + min(p0 + p, pieces - 1)) * each + static_cast<int64_t>(r) * side.width + c;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[p][i] = from[i * next];
+      }
+#pragma unroll
+      for (int p = 0; p < kAhead; ++p)
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (p0 + p < pieces) f[i] += v[p][i];
     }
     T* to = of_b ? grad_b + slot * each + static_cast<int64_t>(c) * o.rank + r : grad_a + slot * each + static_cast<int64_t>(r) * side.width + c;
 #pragma unroll
     for (int i = 0; i < 8; i += Pack<T>::N) store16(to + i, Pack<T>::pack(f + i));
   }
-}
-
-// [slots, rows, cols] -> [slots, cols, rows], 32 x 32 a workgroup
-template <typename E>
-__global__ __launch_bounds__(256) void transpose_kernel(const E* __restrict__ from, E* __restrict__ to, const int rows, const int cols) {
-  __shared__ E s_t[32][33];
-  const int64_t slot = static_cast<int64_t>(blockIdx.z) * rows * cols;
-  const int r0 = blockIdx.y * 32, c0 = blockIdx.x * 32, x = threadIdx.x % 32, y = threadIdx.x / 32;
-#pragma unroll
-  for (int i = 0; i < 32; i += 8)
-    if (r0 + y + i < rows && c0 + x < cols) s_t[y + i][x] = from[slot + static_cast<int64_t>(r0 + y + i) * cols + c0 + x];
-  __syncthreads();
-#pragma unroll
-  for (int i = 0; i < 32; i += 8)
-    if (c0 + y + i < cols && r0 + x < rows) to[slot + static_cast<int64_t>(c0 + y + i) * rows + r0 + x] = s_t[x][y + i];
 }
 
 // ---- what a call takes ------------------------------------------------------------------------------------------------------
@@ -656,8 +746,9 @@ template <typename T, int RT> void expand_nt(const Bank& bank, const Requests& r
 template <typename T> void expand(const Bank& bank, const Requests& req, Expand e, int nt, int pieces, hipStream_t s) {
   const int units = (e.columns + 63) / 64;
   e.pieces = pieces;
-  // (a piece's sums are read once a wave: several units of columns a wave where there are pieces enough)
-  e.units = pieces * ((units + 15) / 16) >= 1024 ? 4 : pieces * ((units + 7) / 8) >= 1024 ? 2 : 1;
+  // (a workgroup adds up its piece's sums once: several units of columns a wave where there are workgroups enough without)
+  const int real = req.rows.start != nullptr ? (req.rows.rows + 16 * nt - 1) / (16 * nt) : pieces;
+  e.units = real * ((units + 15) / 16) >= 512 ? 4 : real * ((units + 7) / 8) >= 512 ? 2 : 1;
   const bool rest = req.rows.start != nullptr && (e.out != e.base || e.low != nullptr);
   const dim3 grid(pieces + (rest ? (e.rows + 16 * nt - 1) / (16 * nt) : 0), (units + kExpandWaves * e.units - 1) / (kExpandWaves * e.units));
   if (bank.rank <= 16) expand_nt<T, 1>(bank, req, e, nt, grid, s);
@@ -676,7 +767,7 @@ int64_t take(int64_t& at, int64_t bytes) {
 struct GradPlan {
   int nt, pieces, splits;
   int capacity, blocks, tiles, shift, records;   // virtual rows, blocks of 32 of them, tiles of the rank, pieces of outer
-  int64_t o_start, o_order, o_seq, o_at, o_bt, o_planes, o_du, o_op_du, o_op_low, o_rec_a, o_rec_b, bytes;
+  int64_t o_start, o_order, o_slot_of, o_seq, o_at, o_bt, o_planes, o_du, o_op_du, o_op_low, o_rec_a, o_rec_b, bytes;
 };
 GradPlan grad_plan(int rows, int sequences, bool ragged, int in, int out, int rank, int slots, int dtype) {
   GradPlan p{};
@@ -696,6 +787,7 @@ GradPlan grad_plan(int rows, int sequences, bool ragged, int in, int out, int ra
   int64_t at = 0;
   p.o_start = take(at, int64_t{4} * (slots + 1));
   p.o_order = take(at, int64_t{4} * p.capacity);
+  p.o_slot_of = take(at, int64_t{4} * p.blocks);
   p.o_seq = take(at, int64_t{4} * sequences);
   p.o_at = take(at, size * slots * rank * in);
   p.o_bt = take(at, size * slots * rank * out);
@@ -714,27 +806,23 @@ void gradients(const GradPlan& p, const void* grad, int64_t grad_stride, const v
                const void* lora_a, const void* lora_b, const float* scaling, const Requests& req, const void* grad_base, int64_t base_stride,
                void* grad_x, void* grad_a, void* grad_b, uint8_t* ws, int in, int out, int rank, int slots, hipStream_t s) {
   const int rows = req.rows.rows;
-  int32_t* start = reinterpret_cast<int32_t*>(ws + p.o_start);
-  int32_t* order = reinterpret_cast<int32_t*>(ws + p.o_order);
   float* planes = reinterpret_cast<float*>(ws + p.o_planes);
   float* du = reinterpret_cast<float*>(ws + p.o_du);
   const int64_t plane = static_cast<int64_t>(rows) * rank;
-  hipLaunchKernelGGL(plan_kernel, dim3(1), dim3(kPlanThreads), 0, s, req, slots, p.capacity, start, order, reinterpret_cast<int32_t*>(ws + p.o_seq));
-  const auto turn = [&](const void* from, void* to, int r, int c) {
-    const dim3 grid((c + 31) / 32, (r + 31) / 32, slots);
-    if constexpr (sizeof(T) == 4) hipLaunchKernelGGL((transpose_kernel<uint32_t>), grid, dim3(256), 0, s, static_cast<const uint32_t*>(from), static_cast<uint32_t*>(to), r, c);
-    else hipLaunchKernelGGL((transpose_kernel<uint16_t>), grid, dim3(256), 0, s, static_cast<const uint16_t*>(from), static_cast<uint16_t*>(to), r, c);
-  };
-  turn(lora_b, ws + p.o_bt, out, rank);
-  turn(lora_a, ws + p.o_at, rank, in);
+  const Plan plan{slots, p.capacity, reinterpret_cast<int32_t*>(ws + p.o_start), reinterpret_cast<int32_t*>(ws + p.o_order),
+                  reinterpret_cast<int32_t*>(ws + p.o_slot_of), reinterpret_cast<int32_t*>(ws + p.o_seq)};
+  const Turn turn_a{lora_a, ws + p.o_at, rank, in}, turn_b{lora_b, ws + p.o_bt, out, rank};
+  const unsigned tiles = static_cast<unsigned>(slots) * (((in + 63) / 64 + (out + 63) / 64) * ((rank + 63) / 64));
+  if constexpr (sizeof(T) == 4) hipLaunchKernelGGL((prepare_kernel<uint32_t>), dim3(1 + tiles), dim3(kPlanThreads), 0, s, req, plan, turn_a, turn_b);
+  else hipLaunchKernelGGL((prepare_kernel<uint16_t>), dim3(1 + tiles), dim3(kPlanThreads), 0, s, req, plan, turn_a, turn_b);
   shrink<T>(grad, grad_stride, Bank{ws + p.o_bt, slots, rank, out}, req, planes, plane, p.splits, p.nt, p.pieces, s);
   float* op_du = reinterpret_cast<float*>(ws + p.o_op_du);
   float* op_low = reinterpret_cast<float*>(ws + p.o_op_low);
-  hipLaunchKernelGGL(operands_kernel, dim3(p.blocks, p.tiles), dim3(kWave), 0, s, planes, plane, p.splits, low, scaling, rank, slots, start, order, du, op_du, op_low);
+  hipLaunchKernelGGL(operands_kernel, dim3(p.blocks), dim3(kOperandThreads), 0, s, planes, plane, p.splits, low, scaling, rank, plan, du, op_du, op_low);
   expand<T>(Bank{ws + p.o_at, slots, rank, in}, req, Expand{du, plane, 1, nullptr, grad_base, base_stride, grad_x, nullptr, rows, in, 0, 0}, p.nt, p.pieces, s);
   const Outer o{OuterSide{x, x_stride, x_scale, op_du, reinterpret_cast<float*>(ws + p.o_rec_a), in},
                 OuterSide{grad, grad_stride, nullptr, op_low, reinterpret_cast<float*>(ws + p.o_rec_b), out},
-                start, order, slots, rank, p.blocks, p.capacity, p.shift, (in + kColumns - 1) / kColumns};
+                plan.start, plan.order, slots, rank, p.blocks, p.capacity, p.shift, (in + kColumns - 1) / kColumns};
   const int rtw = p.tiles >= 4 ? 4 : p.tiles >= 2 ? 2 : 1;
   const dim3 grid(o.a_columns + (out + kColumns - 1) / kColumns, p.records, (p.tiles + rtw - 1) / rtw);
 #define LLMQ_OUTER(CODES)                                                                                    \
