@@ -5,8 +5,8 @@
 //   du[t] = s[a] g[t] B[a]        gx[t] = gbase[t] + du[t] A[a]     gA[a] = sum_t du[t]^T x[t]     gB[a] = s[a] sum_t g[t]^T low[t]
 //
 // shrink   rows by a bank's rows: the reduction is long (in, or out), the result 8 to 128 wide. A workgroup takes a piece of one
-//          request's rows and a part of the reduction, its waves parts of that; sums of the parts go to memory, one plane a part.
-// expand   adds the planes up and multiplies by the other factor into the projection's output: a wave has 64 columns at a time.
+//          request's rows, its waves parts of the reduction.
+// expand   multiplies that by the other factor into the projection's output: a wave has 128 columns.
 // outer    gradients of the bank: the reduction is over rows, which are sorted by adapter (plan) in blocks of 32. Both operands lie
 //          with the reduction outermost; a lane loads eight columns of its eight rows and turns them over in registers.
 // All on the matrix core in fp32 sums. The 8 to 128 numbers in between stay fp32 in memory; as operands they are
@@ -49,7 +49,7 @@ struct Requests {
   }
 };
 
-template <int NT> constexpr int kPieceShift = NT == 4 ? 6 : NT == 2 ? 5 : 4;
+template <int NT> constexpr int kPieceShift = NT == 2 ? 5 : 4;
 
 __device__ __forceinline__ v4f mfma_f32(float a, float b, v4f c) { return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0); }
 template <typename T> __device__ __forceinline__ v4f mfma_packet(u32x4 a, u32x4 b, v4f c) { return mfma_16x16x32<T>(a, b, c); }
@@ -80,81 +80,99 @@ __device__ __forceinline__ HiLo hi_lo(const float* f) {
 }
 
 // ---- shrink -----------------------------------------------------------------------------------------------------------------
-constexpr int kShrinkWaves = 4;
-
-// RT: tiles of 16 of the rank, NT: of rows. A step is 128 bytes of a row: lanes 16 g .. hold packets 2 g and 2 g + 1 of it, of both
-// operands (the order of a sum is free).
+// RT: tiles of 16 of the rank, NT: of rows. A step is 128 bytes of a row. A workgroup of eight waves (four for ranks above 32) takes 16 or 32 rows, each wave every
+// eighth step of the reduction, through LDS of its own: transfers of eight whole rows' 128 bytes (read as operands, 16 bytes of 16 rows, an instruction meets
+// 64 pieces of lines: 4099 rows of 4096 24.7 us where this takes 12), chunks swizzled by the row, no barrier but the one meeting at the end. Where
+// rows are few the reduction is cut for several workgroups (splits_of).
+constexpr int shrink_waves(int rank) { return rank > 32 ? 4 : 8; }   // (two workgroups a CU at least, for their LDS)
+template <int RT> constexpr int kShrinkWaves = RT >= 4 ? 4 : 8;
+template <int RT, int NT> constexpr int kShrinkAhead = RT + NT <= 2 ? 2 : 1;   // steps of a wave in flight
 template <typename T, int RT, int NT>
-__global__ __launch_bounds__(kShrinkWaves * kWave) void shrink_kernel(const T* __restrict__ x, const int64_t x_stride, const Bank bank,
-                                                                          const Requests req, float* __restrict__ planes, const int64_t plane) {
-  constexpr int V = Pack<T>::N, U = 20 / (RT + NT) > 4 ? 4 : 20 / (RT + NT);
-  __shared__ v4f s_sum[kShrinkWaves - 1][RT * NT][kWave];
+__global__ __launch_bounds__((kShrinkWaves<RT> * kWave)) void shrink_kernel(const T* __restrict__ x, const int64_t x_stride, const Bank bank,
+                                                                            const Requests req, float* __restrict__ planes, const int64_t plane) {
+  constexpr int V = Pack<T>::N, kWaves = kShrinkWaves<RT>, U = kShrinkAhead<RT, NT>, kTile = 2048, kStepBytes = (RT + NT) * kTile;
+  constexpr int kStages = kWaves * U * kStepBytes, kSums = kWaves / 2 * RT * NT * 1024;
+  __shared__ __attribute__((aligned(16))) uint8_t s_mem[kStages > kSums ? kStages : kSums];
   int first, n;
   const int a = req.template piece<kPieceShift<NT>>(blockIdx.x, bank.slots, first, n);
   if (n <= 0 || a < 0) return;
-  const int lane = threadIdx.x & (kWave - 1), wv = threadIdx.x / kWave, lr = lane & 15, g = lane >> 4;
+  const int lane = threadIdx.x & (kWave - 1), wv = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) / kWave), lr = lane & 15, g = lane >> 4;
   const int packets = bank.width / V, steps = (packets + 7) / 8, splits = gridDim.y;
   const int s0 = static_cast<int>(static_cast<int64_t>(steps) * blockIdx.y / splits), s1 = static_cast<int>(static_cast<int64_t>(steps) * (blockIdx.y + 1) / splits);
-  const T* xr[NT];
-  const T* mr[RT];
+  // transfers: eight rows each, lane = (row, slot); slot p of row r holds chunk p ^ (r & 7)
+  const BufferBase xb = buffer_base(x + static_cast<int64_t>(first) * x_stride),
+                   mb = buffer_base(static_cast<const T*>(bank.m) + static_cast<int64_t>(a) * bank.rank * bank.width);
+  const int tr = lane >> 3, chunk = (lane & 7) ^ tr;
+  uint32_t xo[2 * NT], mo[2 * RT];
 #pragma unroll
-  for (int i = 0; i < NT; ++i) xr[i] = x + static_cast<int64_t>(first + min(i * 16 + lr, n - 1)) * x_stride;
+  for (int i = 0; i < 2 * NT; ++i) xo[i] = static_cast<uint32_t>(min(i * 8 + tr, n - 1) * x_stride * static_cast<int64_t>(sizeof(T)));
 #pragma unroll
-  for (int i = 0; i < RT; ++i)
-    mr[i] = static_cast<const T*>(bank.m) + (static_cast<int64_t>(a) * bank.rank + min(i * 16 + lr, bank.rank - 1)) * bank.width;
+  for (int i = 0; i < 2 * RT; ++i) mo[i] = static_cast<uint32_t>(min(i * 8 + tr, bank.rank - 1)) * static_cast<uint32_t>(bank.width * sizeof(T));
+  uint8_t* const mine = s_mem + wv * U * kStepBytes;
+  const uint32_t at0 = lr * 128 + ((g ^ (lr & 7)) << 4);   // chunk g of row lr; chunk g + 4: ^ 64
   v4f acc[RT][NT] = {};
-  for (int s = s0 + wv; s < s1; s += kShrinkWaves * U) {
-    u32x4 xv[U][NT][2], mv[U][RT][2];
+  for (int s = s0 + wv; s < s1; s += kWaves * U) {
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int at = min(s + u * kShrinkWaves, s1 - 1);   // (a step past the end is loaded again and not multiplied)
+      const int at = s + u * kWaves;
+      if (at >= s1) break;   // (the wave's)
+      const uint32_t byte = static_cast<uint32_t>(min(at * 8 + chunk, packets - 1)) * 16u;   // (past the row's end: its last packet, zeros below)
+      uint8_t* stage = mine + u * kStepBytes;
+#pragma unroll
+      for (int i = 0; i < 2 * NT; ++i) buffer_to_lds<16>(xb, stage + i * 1024, xo[i] + byte, 0);
+#pragma unroll
+      for (int i = 0; i < 2 * RT; ++i) buffer_to_lds<16>(mb, stage + NT * kTile + i * 1024, mo[i] + byte, 0);
+    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int at = s + u * kWaves;
+      if (at >= s1) break;
+      const uint8_t* stage = mine + u * kStepBytes;
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const int p = min(at * 8 + 2 * g + h, packets - 1) * V;
+        u32x4 xv[NT], mv[RT];
 #pragma unroll
-        for (int i = 0; i < NT; ++i) xv[u][i][h] = load16(xr[i] + p);
+        for (int i = 0; i < NT; ++i) xv[i] = load16(stage + i * kTile + (at0 ^ (h << 6)));
 #pragma unroll
-        for (int i = 0; i < RT; ++i) mv[u][i][h] = load16(mr[i] + p);
-      }
-    }
+        for (int i = 0; i < RT; ++i) mv[i] = load16(stage + (NT + i) * kTile + (at0 ^ (h << 6)));
+        if (at * 8 + 8 > packets && at * 8 + 4 * h + g >= packets) {   // the row's last step
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int at = s + u * kShrinkWaves;
-      if (at >= s1) break;
-      if (at * 8 + 8 > packets) {   // the row's last step: packets past its end are zeros
+          for (int i = 0; i < NT; ++i) xv[i] = u32x4{0, 0, 0, 0};
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
-          if (at * 8 + 2 * g + h >= packets) {
-#pragma unroll
-            for (int i = 0; i < NT; ++i) xv[u][i][h] = u32x4{0, 0, 0, 0};
-#pragma unroll
-            for (int i = 0; i < RT; ++i) mv[u][i][h] = u32x4{0, 0, 0, 0};
-          }
-      }
-#pragma unroll
-      for (int h = 0; h < 2; ++h)
+          for (int i = 0; i < RT; ++i) mv[i] = u32x4{0, 0, 0, 0};
+        }
 #pragma unroll
         for (int i = 0; i < RT; ++i)
 #pragma unroll
-          for (int j = 0; j < NT; ++j) acc[i][j] = mfma_packet<T>(mv[u][i][h], xv[u][j][h], acc[i][j]);
+          for (int j = 0; j < NT; ++j) acc[i][j] = mfma_packet<T>(mv[i], xv[j], acc[i][j]);
+      }
     }
-  }
-  if (wv > 0) {
-#pragma unroll
-    for (int i = 0; i < RT * NT; ++i) s_sum[wv - 1][i][lane] = acc[i / NT][i % NT];
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // (the stages are asked for again)
   }
   __syncthreads();
+  v4f* const s_sum = reinterpret_cast<v4f*>(s_mem);
+#pragma unroll
+  for (int half = kWaves / 2; half > 0; half /= 2) {   // a tree over the waves
+    if (wv >= half && wv < 2 * half) {
+#pragma unroll
+      for (int i = 0; i < RT * NT; ++i) s_sum[((wv - half) * RT * NT + i) * kWave + lane] = acc[i / NT][i % NT];
+    }
+    __syncthreads();
+    if (wv < half) {
+#pragma unroll
+      for (int i = 0; i < RT * NT; ++i) acc[i / NT][i % NT] += s_sum[(wv * RT * NT + i) * kWave + lane];
+    }
+    __syncthreads();
+  }
   if (wv > 0) return;
 #pragma unroll
   for (int i = 0; i < RT; ++i)
 #pragma unroll
     for (int j = 0; j < NT; ++j) {
-      v4f v = acc[i][j];
-#pragma unroll
-      for (int w = 0; w < kShrinkWaves - 1; ++w) v += s_sum[w][i * NT + j][lane];
       const int r = i * 16 + 4 * g, t = j * 16 + lr;   // four of the rank, a row
       if (t < n && r < bank.rank)
-        *reinterpret_cast<v4f*>(planes + blockIdx.y * plane + static_cast<int64_t>(first + t) * bank.rank + r) = v;
+        *reinterpret_cast<v4f*>(planes + blockIdx.y * plane + static_cast<int64_t>(first + t) * bank.rank + r) = acc[i][j];
     }
 }
 
@@ -165,25 +183,21 @@ struct Expand {
   const float* planes;     // [splits][rows][rank]
   int64_t plane;
   int splits;
-  const float* scaling;    // [slots], or null: 1
+  const float* scaling;    // [slots]
   const void* base;        // or null: zeros
   int64_t base_stride;
   void* out;               // [rows, width], contiguous
-  float* low;              // or null: the sum of the planes [rows, rank], by the first columns' workgroups
+  float* low;              // or null: [rows, rank], the sum of the planes (where there are several) and zeros without an adapter
   int rows, columns;       // columns of out
   int pieces;              // workgroups from there on in blockIdx.x: rows of no request
-  int units;               // of 64 columns a wave
 };
 
-// The columns of MFMA row r of tile mi are named 16 (r / 4) + 4 mi + r % 4, so that a lane's results are 16 neighbours.
-// The bank here is [slots][columns][rank]. The piece's sums are added up once for the workgroup, eight planes in flight, through LDS; the first
-// 64 columns' weights and base are on their way meanwhile (plane after plane in every wave, and base behind the product, had taken 52 us
-// where this takes 17: 333 rows of 20 requests, rank 64, 14336 columns, fp16; 4099 rows of 4096 columns 55 and 25).
+// 128 columns a wave: lane 16 g + r has columns 8 r .. 8 r + 7, one of each of eight tiles, of rows 4 g .. 4 g + 3, so that 16 lanes read and
+// write 256 neighbouring bytes of a row (with rows over the lanes, 64 bytes of each of 16: 4099 rows of 4096 23 us). What does not depend on the
+// rows' sums, the weights and the base, is asked for first. The bank here is [slots][columns][rank].
 template <typename T, int RT, int NT>
 __global__ __launch_bounds__(kExpandWaves * kWave) void expand_kernel(const Bank bank, const Requests req, const Expand e) {
   constexpr int V = Pack<T>::N, KT = (RT * 16 + 4 * V - 1) / (4 * V);   // steps of the rank: 32 (fp32: 16)
-  constexpr int kRow = RT * 16 + 4, kAhead = 8;
-  __shared__ __attribute__((aligned(16))) float s_low[NT * 16][kRow];
   const int lane = threadIdx.x & (kWave - 1), wv = threadIdx.x / kWave, lr = lane & 15, g = lane >> 4;
   int first, n, a;
   const bool rest = static_cast<int>(blockIdx.x) >= e.pieces;   // rows in front of the first request and behind the last one: the base as it is
@@ -196,122 +210,123 @@ __global__ __launch_bounds__(kExpandWaves * kWave) void expand_kernel(const Bank
     n = min(e.rows - first, 1 << kPieceShift<NT>);
   }
   const int begin = rest ? req.rows.first(0) : 0, end = rest ? max(req.rows.first(req.rows.sequences), begin) : 0;
-  const int unit0 = (blockIdx.y * kExpandWaves + wv) * e.units;
-  const bool writes_low = e.low != nullptr && blockIdx.y == 0;
-  u32x4 m[KT][4], base[NT][16 / V];
-  const auto request = [&](int c0) {
-    if (e.base != nullptr) {
-#pragma unroll
-      for (int j = 0; j < NT; ++j) {
-        const T* from = static_cast<const T*>(e.base) + (first + min(j * 16 + lr, n - 1)) * e.base_stride;
-#pragma unroll
-        for (int h = 0; h < 16 / V; ++h) base[j][h] = load16(from + min(c0 + g * 16 + h * V, e.columns - V));
-      }
-    }
-    if (a < 0) return;
-#pragma unroll
-    for (int k = 0; k < KT; ++k)
-#pragma unroll
-      for (int mi = 0; mi < 4; ++mi) {
-        const int c = min(c0 + (lr >> 2) * 16 + mi * 4 + (lr & 3), e.columns - 1);
-        // (past the rank the operand of `low` is zeros, against weights that are looked at a second time)
-        m[k][mi] = load16(static_cast<const T*>(bank.m) + (static_cast<int64_t>(a) * e.columns + c) * bank.rank + min((k * 4 + g) * V, bank.rank - V));
-      }
-  };
-  if (unit0 * 64 < e.columns) request(unit0 * 64);
-  u32x4 low_hi[NT][KT], low_lo[NT][KT];   // (fp32: low_hi alone)
-  if (a >= 0) {
-    const int quads = bank.rank / 4;
-    for (int item = threadIdx.x; item < n * quads; item += kExpandWaves * kWave) {
-      const int t = item / quads, r = (item - t * quads) * 4;
-      const float* from = e.planes + static_cast<int64_t>(first + t) * bank.rank + r;
-      v4f sum{0.0f, 0.0f, 0.0f, 0.0f};
-      for (int p0 = 0; p0 < e.splits; p0 += kAhead) {
-        v4f v[kAhead];
-#pragma unroll
-        for (int p = 0; p < kAhead; ++p) v[p] = *reinterpret_cast<const v4f*>(from + min(p0 + p, e.splits - 1) * e.plane);
-#pragma unroll
-        for (int p = 0; p < kAhead; ++p)
-          if (p0 + p < e.splits) sum += v[p];
-      }
-      *reinterpret_cast<v4f*>(&s_low[t][r]) = sum;
-      if (writes_low) *reinterpret_cast<v4f*>(e.low + static_cast<int64_t>(first + t) * bank.rank + r) = sum;
-    }
-    const float s = e.scaling != nullptr ? e.scaling[a] : 1.0f;
-    __syncthreads();
-#pragma unroll
-    for (int j = 0; j < NT; ++j)
-#pragma unroll
-      for (int k = 0; k < KT; ++k) {
-        const int r = (k * 4 + g) * V;
-        float f[V];
-#pragma unroll
-        for (int i = 0; i < V; ++i) f[i] = r < bank.rank ? s_low[min(j * 16 + lr, n - 1)][r + i] * s : 0.0f;
-        if constexpr (V == 8) {
-          const HiLo v = hi_lo(f);
-          low_hi[j][k] = v.hi;
-          low_lo[j][k] = v.lo;
-        } else {
-          low_hi[j][k] = Pack<float>::pack(f);
-        }
-      }
-  } else if (writes_low) {   // (no adapter: zeros)
-    for (int i = threadIdx.x; i < n * bank.rank; i += kExpandWaves * kWave) {
+  if (rest && first >= begin && first + n <= end) return;   // (the usual: the requests have all rows)
+  const int c0 = (blockIdx.y * kExpandWaves + wv) * 128;
+  const bool writes_low = e.low != nullptr && c0 == 0;
+  if (a < 0 && writes_low) {   // (no adapter: zeros)
+    for (int i = lane; i < n * bank.rank; i += kWave) {
       const int64_t row = first + i / bank.rank;
       if (!rest || row < begin || row >= end) e.low[row * bank.rank + i % bank.rank] = 0.0f;
     }
   }
-  for (int u = 0; u < e.units; ++u) {
-    const int c0 = (unit0 + u) * 64;
-    if (c0 >= e.columns) return;
-    if (u > 0) request(c0);
-    v4f acc[NT][4] = {};
-    if (a >= 0) {
+  if (c0 >= e.columns) return;
+  const int c = c0 + 8 * lr;   // (columns are a multiple of 8)
+  const bool here = c < e.columns;
+  u32x4 m[KT][8], base[NT][4][8 / V];
+  if (a >= 0) {
 #pragma unroll
-      for (int k = 0; k < KT; ++k)
+    for (int k = 0; k < KT; ++k)
 #pragma unroll
-        for (int mi = 0; mi < 4; ++mi) {
-          if constexpr (sizeof(T) == 4) {
+      for (int mi = 0; mi < 8; ++mi)   // (past the rank the operand of `low` is zeros, against weights that are looked at a second time)
+        m[k][mi] = load16(static_cast<const T*>(bank.m) + (static_cast<int64_t>(a) * e.columns + min(c + mi, e.columns - 1)) * bank.rank + min((k * 4 + g) * V, bank.rank - V));
+  }
+  if (e.base != nullptr) {
 #pragma unroll
-            for (int j = 0; j < NT; ++j) acc[j][mi] = mfma_packet<float>(m[k][mi], low_hi[j][k], acc[j][mi]);
-          } else if constexpr (__is_same(T, f16_t)) {
-            float f[8];
-            Pack<f16_t>::unpack(m[k][mi], f);
-            const HiLo w = hi_lo(f);   // (exact: 11 bits in 16)
+    for (int j = 0; j < NT; ++j)
 #pragma unroll
-            for (int j = 0; j < NT; ++j) {
-              acc[j][mi] = mfma_16x16x32<bf16_t>(w.lo, low_hi[j][k], acc[j][mi]);
-              acc[j][mi] = mfma_16x16x32<bf16_t>(w.hi, low_lo[j][k], acc[j][mi]);
-              acc[j][mi] = mfma_16x16x32<bf16_t>(w.hi, low_hi[j][k], acc[j][mi]);
-            }
-          } else {
+      for (int i = 0; i < 4; ++i) {
+        const T* from = static_cast<const T*>(e.base) + (first + min(j * 16 + 4 * g + i, n - 1)) * e.base_stride + min(c, e.columns - 8);
 #pragma unroll
-            for (int j = 0; j < NT; ++j) {
-              acc[j][mi] = mfma_16x16x32<bf16_t>(m[k][mi], low_lo[j][k], acc[j][mi]);
-              acc[j][mi] = mfma_16x16x32<bf16_t>(m[k][mi], low_hi[j][k], acc[j][mi]);
-            }
+        for (int h = 0; h < 8 / V; ++h) base[j][i][h] = load16(from + h * V);
+      }
+  }
+  v4f acc[NT][8] = {};
+  if (a >= 0) {
+    const float s = e.scaling[a];
+#pragma unroll
+    for (int k = 0; k < KT; ++k) {
+      u32x4 low_hi[NT], low_lo[NT];   // (fp32: low_hi alone)
+#pragma unroll
+      for (int j = 0; j < NT; ++j) {
+        const int r = (k * 4 + g) * V;
+        const int64_t at = static_cast<int64_t>(first + min(j * 16 + lr, n - 1)) * bank.rank + min(r, bank.rank - V);
+        v4f sum[V / 4];
+#pragma unroll
+        for (int i = 0; i < V / 4; ++i) sum[i] = *reinterpret_cast<const v4f*>(e.planes + at + 4 * i);
+        if (e.splits > 1) {
+          constexpr int kAhead = 4;
+          for (int p0 = 1; p0 < e.splits; p0 += kAhead) {
+            v4f v[kAhead][V / 4];
+#pragma unroll
+            for (int p = 0; p < kAhead; ++p)
+#pragma unroll
+              for (int i = 0; i < V / 4; ++i) v[p][i] = *reinterpret_cast<const v4f*>(e.planes + min(p0 + p, e.splits - 1) * e.plane + at + 4 * i);
+#pragma unroll
+            for (int p = 0; p < kAhead; ++p)
+#pragma unroll
+              for (int i = 0; i < V / 4; ++i)
+                if (p0 + p < e.splits) sum[i] += v[p][i];
+          }
+          if (writes_low && j * 16 + lr < n && r < bank.rank) {
+#pragma unroll
+            for (int i = 0; i < V / 4; ++i) *reinterpret_cast<v4f*>(e.low + at + 4 * i) = sum[i];
           }
         }
-    }
+        float f[V];
 #pragma unroll
-    for (int j = 0; j < NT; ++j) {
-      const int t = j * 16 + lr;
-      const int64_t row = first + t;
-      if (t >= n || (rest && row >= begin && row < end)) continue;
-#pragma unroll
-      for (int h = 0; h < 16 / V; ++h) {   // packets of the lane's 16 columns
-        const int c = c0 + g * 16 + h * V;
-        if (c >= e.columns) continue;
-        float f[V] = {};
-        if (e.base != nullptr) Pack<T>::unpack(base[j][h], f);
-        if (a >= 0) {   // (else the base to the bit: -0 + 0 is +0)
-#pragma unroll
-          for (int i = 0; i < V; ++i) f[i] += acc[j][(h * V + i) / 4][i % 4];
+        for (int i = 0; i < V; ++i) f[i] = r < bank.rank ? sum[i / 4][i % 4] * s : 0.0f;
+        if constexpr (sizeof(T) == 4) {
+          low_hi[j] = Pack<float>::pack(f);
+        } else {
+          const HiLo low = hi_lo(f);
+          low_hi[j] = low.hi;
+          low_lo[j] = low.lo;
         }
-        store16(static_cast<T*>(e.out) + row * e.columns + c, Pack<T>::pack(f));
+      }
+#pragma unroll
+      for (int mi = 0; mi < 8; ++mi) {
+        if constexpr (sizeof(T) == 4) {
+#pragma unroll
+          for (int j = 0; j < NT; ++j) acc[j][mi] = mfma_packet<float>(low_hi[j], m[k][mi], acc[j][mi]);
+        } else if constexpr (__is_same(T, f16_t)) {
+          float w[8];
+          Pack<f16_t>::unpack(m[k][mi], w);
+          const HiLo v = hi_lo(w);   // (exact: 11 bits in 16)
+#pragma unroll
+          for (int j = 0; j < NT; ++j) {
+            acc[j][mi] = mfma_16x16x32<bf16_t>(low_hi[j], v.lo, acc[j][mi]);
+            acc[j][mi] = mfma_16x16x32<bf16_t>(low_lo[j], v.hi, acc[j][mi]);
+            acc[j][mi] = mfma_16x16x32<bf16_t>(low_hi[j], v.hi, acc[j][mi]);
+          }
+        } else {
+#pragma unroll
+          for (int j = 0; j < NT; ++j) {
+            acc[j][mi] = mfma_16x16x32<bf16_t>(low_lo[j], m[k][mi], acc[j][mi]);
+            acc[j][mi] = mfma_16x16x32<bf16_t>(low_hi[j], m[k][mi], acc[j][mi]);
+          }
+        }
       }
     }
   }
+  if (!here) return;
+#pragma unroll
+  for (int j = 0; j < NT; ++j)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int t = j * 16 + 4 * g + i;
+      const int64_t row = first + t;
+      if (t >= n || (rest && row >= begin && row < end)) continue;
+#pragma unroll
+      for (int h = 0; h < 8 / V; ++h) {
+        float f[V] = {};
+        if (e.base != nullptr) Pack<T>::unpack(base[j][i][h], f);
+        if (a >= 0) {   // (else the base to the bit: -0 + 0 is +0)
+#pragma unroll
+          for (int q = 0; q < V; ++q) f[q] += acc[j][h * V + q][i];
+        }
+        store16(static_cast<T*>(e.out) + row * e.columns + c + h * V, Pack<T>::pack(f));
+      }
+    }
 }
 
 // ---- the plan of a gradient: rows sorted by adapter -----------------------------------------------------------------------------
@@ -319,12 +334,11 @@ constexpr int kBlock = 32;          // rows of a block: one step of the matrix c
 constexpr int kPlanThreads = 1024;  // and the most slots
 
 // start [slots + 1]: the first virtual row of each slot, a multiple of 32 (rows up to there: none, -1); order: the row behind each
-// virtual row; slot_of: the slot of each block. Requests of a slot keep their order. One workgroup; seq_start: [sequences] scratch.
+// virtual row. Requests of a slot keep their order. One workgroup; seq_start: [sequences] scratch.
 struct Plan {
   int slots, capacity;   // virtual rows at the most
   int32_t* start;
   int32_t* order;
-  int32_t* slot_of;
   int32_t* seq_start;
 };
 struct PlanLds {
@@ -374,14 +388,6 @@ __device__ __forceinline__ void make_plan(PlanLds& s, const Requests& req, const
     if (t == p.slots - 1) p.start[p.slots] = s.scan[t];
   }
   __syncthreads();
-  for (int block = t; block < p.capacity / kBlock; block += kPlanThreads) {
-    int lo = 0, hi = p.slots - 1;   // the first slot that ends behind the block's begin (none: the last)
-    while (lo < hi) {
-      const int mid = (lo + hi) / 2;
-      if (s.scan[mid] > block * kBlock) hi = mid; else lo = mid + 1;
-    }
-    p.slot_of[block] = lo;
-  }
   for (int row = t; row < req.rows.rows; row += kPlanThreads) {
     int lo = 0, hi = sequences;   // the last request that begins at or in front of the row
     while (lo + 1 < hi) {
@@ -430,65 +436,12 @@ __global__ __launch_bounds__(kPlanThreads) void prepare_kernel(const Requests re
   }
 }
 
-// Sums of shrink's planes, times the scaling, as [rows, rank] (du) and, with the kept `low`, as operands of outer: blocks of 32
-// virtual rows, [tile of the rank][block][lane][8], lane 16 g + r holding entry r of the rank of rows 8 g .. 8 g + 7. A workgroup a block.
-constexpr int kOperandThreads = 256;
-__global__ __launch_bounds__(kOperandThreads) void operands_kernel(const float* __restrict__ planes, const int64_t plane, const int splits,
-                                                                   const float* __restrict__ low, const float* __restrict__ scaling, const int rank,
-                                                                   const Plan plan, float* __restrict__ du, float* __restrict__ op_du,
-                                                                   float* __restrict__ op_low) {
-  constexpr int kAhead = 8, kRow = 132;
-  __shared__ __attribute__((aligned(16))) float s_du[kBlock][kRow], s_lo[kBlock][kRow];
-  const int block = blockIdx.x, quads = rank / 4;
-  if (block * kBlock >= plan.start[plan.slots]) return;
-  const float s = scaling[plan.slot_of[block]];
-  for (int item = threadIdx.x; item < kBlock * quads; item += kOperandThreads) {
-    const int t = item / quads, r = (item - t * quads) * 4, row = plan.order[block * kBlock + t];
-    v4f d{0.0f, 0.0f, 0.0f, 0.0f}, l = d;
-    if (row >= 0) {
-      const int64_t at = static_cast<int64_t>(row) * rank + r;
-      l = *reinterpret_cast<const v4f*>(low + at) * s;
-      for (int p0 = 0; p0 < splits; p0 += kAhead) {
-        v4f v[kAhead];
-#pragma unroll
-        for (int p = 0; p < kAhead; ++p) v[p] = *reinterpret_cast<const v4f*>(planes + min(p0 + p, splits - 1) * plane + at);
-#pragma unroll
-        for (int p = 0; p < kAhead; ++p)
-          if (p0 + p < splits) d += v[p];
-      }
-      d *= s;
-      *reinterpret_cast<v4f*>(du + at) = d;
-    }
-    *reinterpret_cast<v4f*>(&s_du[t][r]) = d;
-    *reinterpret_cast<v4f*>(&s_lo[t][r]) = l;
-  }
-  __syncthreads();
-  const int tiles = (rank + 15) / 16;
-  for (int item = threadIdx.x; item < tiles * kWave; item += kOperandThreads) {
-    const int tile = item / kWave, lane = item % kWave, r = tile * 16 + (lane & 15), t = (lane >> 4) * 8;
-    const int64_t to = ((static_cast<int64_t>(tile) * gridDim.x + block) * kWave + lane) * 8;
-#pragma unroll
-    for (int i = 0; i < 8; i += 4) {
-      v4f d{0.0f, 0.0f, 0.0f, 0.0f}, l = d;
-      if (r < rank) {
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          d[q] = s_du[t + i + q][r];
-          l[q] = s_lo[t + i + q][r];
-        }
-      }
-      *reinterpret_cast<v4f*>(op_du + to + i) = d;
-      *reinterpret_cast<v4f*>(op_low + to + i) = l;
-    }
-  }
-}
-
 // ---- outer ------------------------------------------------------------------------------------------------------------------
 struct OuterSide {
   const void* x;           // rows of `width` values of T, or int8 codes with x_scale
   int64_t stride;
   const float* x_scale;    // [rows, width / 128], or null
-  const float* op;         // operands of the other factor
+  const float* u;          // the other factor [rows, rank]: g lora_b, or x lora_a^T (the scaling comes at the end)
   float* records;          // [pieces][rank][width]
   int width;
 };
@@ -496,12 +449,13 @@ struct Outer {
   OuterSide a, b;          // gradients of A (x and du) and of B (g and low)
   const int32_t* start;
   const int32_t* order;
-  int slots, rank, blocks, capacity, shift;   // blocks: of the operands; 1 << shift rows a piece
+  const float* scaling;
+  int slots, rank, capacity, shift;   // 1 << shift rows a piece
   int a_columns;           // workgroups of side a in blockIdx.x
 };
 constexpr int kColumns = 128;   // of a wave: one group of the codes
 
-// One side's sums over the rows of a piece for 128 columns and 16 RTW of the rank. A step's rows and operands are asked for a step ahead, their
+// One side's sums over the rows of a piece for 128 columns and 16 RTW of the rank. A step's rows are asked for a step ahead, their
 // numbers two.
 template <typename T, bool CODES> struct OuterRows {   // eight columns of eight rows (fp32 values: four of eight, twice)
   static constexpr int kWords = CODES ? 2 : sizeof(T) == 4 ? 8 : 4;
@@ -519,44 +473,51 @@ __device__ __forceinline__ void outer_rows(const OuterSide& side, const Outer& o
     const int4 lo = *reinterpret_cast<const int4*>(o.order + at), hi = *reinterpret_cast<const int4*>(o.order + at + 4);
     const int got[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
 #pragma unroll
-    for (int i = 0; i < 8; ++i) row[i] = got[i] >= 0 ? got[i] : spare;   // (its other factor is zero; a row of this slot, so that nothing foreign gets in)
+    for (int i = 0; i < 8; ++i) row[i] = got[i];
   };
-  const auto ask = [&](int v, const int (&row)[8], OuterRows<T, CODES>& x, float (&f)[RTW][8], float (&s)[8]) {
-    const int block = min(v, v1 - kBlock) / kBlock;
+  const auto ask = [&](const int (&row)[8], OuterRows<T, CODES>& x, float (&f)[RTW][8], float (&s)[8], uint32_t& real) {
+    real = 0;   // (applied where the values are used: nothing here waits for them)
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
+      real |= row[i] >= 0 ? 1u << i : 0u;
+      const int64_t at = row[i] >= 0 ? row[i] : spare;   // (no row: its other factor is zero; a row of this slot, so that nothing foreign gets in)
       if constexpr (CODES) {
-        const u32x2 w = *reinterpret_cast<const u32x2*>(static_cast<const int8_t*>(side.x) + row[i] * side.stride + min(c0 + 8 * lr, side.width - 8));
+        const u32x2 w = *reinterpret_cast<const u32x2*>(static_cast<const int8_t*>(side.x) + at * side.stride + min(c0 + 8 * lr, side.width - 8));
         x.w[i][0] = w.x;
         x.w[i][1] = w.y;
-        s[i] = side.x_scale[static_cast<int64_t>(row[i]) * (side.width / kColumns) + c0 / kColumns];
+        s[i] = side.x_scale[at * (side.width / kColumns) + c0 / kColumns];
       } else if constexpr (sizeof(T) == 4) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          const u32x4 w = load16(static_cast<const float*>(side.x) + row[i] * side.stride + min(c0 + 64 * h + 4 * lr, side.width - 4));
+          const u32x4 w = load16(static_cast<const float*>(side.x) + at * side.stride + min(c0 + 64 * h + 4 * lr, side.width - 4));
           x.w[i][4 * h] = w.x; x.w[i][4 * h + 1] = w.y; x.w[i][4 * h + 2] = w.z; x.w[i][4 * h + 3] = w.w;
         }
       } else {
-        const u32x4 w = load16(static_cast<const T*>(side.x) + row[i] * side.stride + min(c0 + 8 * lr, side.width - 8));
+        const u32x4 w = load16(static_cast<const T*>(side.x) + at * side.stride + min(c0 + 8 * lr, side.width - 8));
         x.w[i][0] = w.x; x.w[i][1] = w.y; x.w[i][2] = w.z; x.w[i][3] = w.w;
       }
-    }
-#pragma unroll
-    for (int i = 0; i < RTW; ++i) {
-      const int tile = min(tile0 + i, (o.rank + 15) / 16 - 1);
-      const float* from = side.op + ((static_cast<int64_t>(tile) * o.blocks + block) * kWave + lane) * 8;
-#pragma unroll
-      for (int q = 0; q < 8; q += 4) {
-        const v4f w = *reinterpret_cast<const v4f*>(from + q);
-        f[i][q] = w[0]; f[i][q + 1] = w[1]; f[i][q + 2] = w[2]; f[i][q + 3] = w[3];
+      // (entries RTW lr .. of the rank: one of each tile)
+      const float* from = side.u + at * o.rank + min((tile0 * 16) + RTW * lr, o.rank - RTW);
+      float value[RTW];
+      if constexpr (RTW == 4) {
+        const v4f v = *reinterpret_cast<const v4f*>(from);
+        value[0] = v[0]; value[1] = v[1]; value[2] = v[2]; value[3] = v[3];
+      } else if constexpr (RTW == 2) {
+        const float2 v = *reinterpret_cast<const float2*>(from);
+        value[0] = v.x; value[1] = v.y;
+      } else {
+        value[0] = *from;
       }
+#pragma unroll
+      for (int r = 0; r < RTW; ++r) f[r][i] = value[r];
     }
   };
   int row[8];
   OuterRows<T, CODES> x;
   float f[RTW][8], s[8];
+  uint32_t real;
   rows_at(begin, row);
-  ask(begin, row, x, f, s);
+  ask(row, x, f, s, real);
   rows_at(begin + step, row);
   for (int v = begin; v < v1; v += step) {
     OuterRows<T, CODES> now = x;
@@ -564,8 +525,8 @@ __device__ __forceinline__ void outer_rows(const OuterSide& side, const Outer& o
 #pragma unroll
     for (int i = 0; i < RTW; ++i)
 #pragma unroll
-      for (int q = 0; q < 8; ++q) u[i][q] = CODES ? f[i][q] * s[q] : f[i][q];
-    ask(v + step, row, x, f, s);   // (behind the last step: that one again)
+      for (int q = 0; q < 8; ++q) u[i][q] = real >> q & 1 ? (CODES ? f[i][q] * s[q] : f[i][q]) : 0.0f;
+    ask(row, x, f, s, real);   // (behind the last step: that one again)
     rows_at(v + 2 * step, row);
     if constexpr (sizeof(T) == 4) {   // e-th product: row 8 g + e of each lane
 #pragma unroll
@@ -576,7 +537,7 @@ __device__ __forceinline__ void outer_rows(const OuterSide& side, const Outer& o
           if constexpr (CODES) value = static_cast<float>(static_cast<int8_t>(now.w[e][q / 4] >> (8 * (q % 4))));
           else value = __builtin_bit_cast(float, now.w[e][q]);
 #pragma unroll
-          for (int i = 0; i < RTW; ++i) acc[i][q] = mfma_f32(value, u[i][e], acc[i][q]);
+          for (int i = 0; i < RTW; ++i) acc[i][q] = mfma_f32(u[i][e], value, acc[i][q]);
         }
     } else {
       HiLo other[RTW];
@@ -602,9 +563,9 @@ __device__ __forceinline__ void outer_rows(const OuterSide& side, const Outer& o
         }
 #pragma unroll
         for (int i = 0; i < RTW; ++i) {
-          if constexpr (!CODES && __is_same(T, f16_t)) acc[i][q] = mfma_16x16x32<bf16_t>(w.lo, other[i].hi, acc[i][q]);
-          acc[i][q] = mfma_16x16x32<bf16_t>(w.hi, other[i].lo, acc[i][q]);
-          acc[i][q] = mfma_16x16x32<bf16_t>(w.hi, other[i].hi, acc[i][q]);
+          if constexpr (!CODES && __is_same(T, f16_t)) acc[i][q] = mfma_16x16x32<bf16_t>(other[i].hi, w.lo, acc[i][q]);
+          acc[i][q] = mfma_16x16x32<bf16_t>(other[i].lo, w.hi, acc[i][q]);
+          acc[i][q] = mfma_16x16x32<bf16_t>(other[i].hi, w.hi, acc[i][q]);
         }
       }
     }
@@ -644,24 +605,25 @@ __global__ __launch_bounds__(4 * kWave) void outer_kernel(const Outer o) {
   if (wv != 0) return;
   const OuterSide& side = side_b ? o.b : o.a;
   float* record = side.records + static_cast<int64_t>(blockIdx.y) * o.rank * side.width;
-  const bool quads = sizeof(T) == 4 && !(CODES && !side_b);   // fp32 values: columns 64 h + 16 g + 4 q + i; else 32 g + 8 q + i
+  // (lane: entries RTW (4 g + q) + i of the rank's 16 RTW, and of the columns 8 lr .. 8 lr + 7, or of fp32 values 64 h + 4 lr .., h = 0, 1)
+  const bool halves = sizeof(T) == 4 && !(CODES && !side_b);
 #pragma unroll
-  for (int i = 0; i < RTW; ++i) {
-    const int r = (blockIdx.z * RTW + i) * 16 + lr;
+  for (int i = 0; i < RTW; ++i)
 #pragma unroll
-    for (int h = 0; h < 2; ++h)
+    for (int q = 0; q < 4; ++q) {
+      const int r = blockIdx.z * RTW * 16 + RTW * (4 * g + q) + i;
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
+      for (int h = 0; h < 2; ++h) {
         v4f v;
 #pragma unroll
         for (int e = 0; e < 4; ++e) v[e] = acc[i][h * 4 + e][q] + s_sum[0][i * 8 + h * 4 + e][lane][q];
-        const int c = c0 + (quads ? 64 * h + 16 * g + 4 * q : 32 * g + 8 * q + 4 * h);
+        const int c = c0 + (halves ? 64 * h + 4 * lr : 8 * lr + 4 * h);
         if (r < o.rank && c < side.width) *reinterpret_cast<v4f*>(record + static_cast<int64_t>(r) * side.width + c) = v;
       }
-  }
+    }
 }
 
-// The pieces' records of each slot added up in order, rounded: eight of the width a lane for A [slots, rank, width], eight of the rank
+// The pieces' records of each slot added up in order, scaled, rounded: eight of the width a lane for A [slots, rank, width], eight of the rank
 // for B [slots, width, rank]. A slot without rows has a gradient of zero.
 template <typename T>
 __global__ __launch_bounds__(256) void records_kernel(const Outer o, T* __restrict__ grad_a, T* __restrict__ grad_b, const int64_t a_items, const int64_t items) {
@@ -681,6 +643,7 @@ __global__ __launch_bounds__(256) void records_kernel(const Outer o, T* __restri
     }
     const int n = o.start[slot + 1] - o.start[slot], first = (o.start[slot] >> o.shift) + 2 * slot, pieces = (n + (1 << o.shift) - 1) >> o.shift;
     float f[8] = {};
+    const float scale = o.scaling[slot];
     const int64_t next = of_b ? side.width : 1;
     for (int p0 = 0; p0 < pieces; p0 += kAhead) {
       float v[kAhead][8];
@@ -696,6 +659,8 @@ __global__ __launch_bounds__(256) void records_kernel(const Outer o, T* __restri
         for (int i = 0; i < 8; ++i)
           if (p0 + p < pieces) f[i] += v[p][i];
     }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) f[i] = pieces > 0 ? f[i] * scale : 0.0f;
     T* to = of_b ? grad_b + slot * each + static_cast<int64_t>(c) * o.rank + r : grad_a + slot * each + static_cast<int64_t>(r) * side.width + c;
 #pragma unroll
     for (int i = 0; i < 8; i += Pack<T>::N) store16(to + i, Pack<T>::pack(f + i));
@@ -703,54 +668,50 @@ __global__ __launch_bounds__(256) void records_kernel(const Outer o, T* __restri
 }
 
 // ---- what a call takes ------------------------------------------------------------------------------------------------------
-// Row tiles of a piece: one for single rows and short requests, four where requests are long (a bank's rows are read once a piece).
-int row_tiles(int rows, int sequences, bool ragged) {
-  if (!ragged || rows < 24 * sequences) return 1;
-  return rows < 96 * sequences ? 2 : 4;
-}
+// Row tiles of a piece. expand: one for single rows and short requests, two where requests are longer (a bank's rows are read once a piece).
+int row_tiles(int rows, int sequences, bool ragged) { return !ragged || rows < 24 * sequences ? 1 : 2; }
+// shrink: one (many workgroups), two where the bank's rows weigh more than twice the activation's
+int shrink_tiles(int rows, int sequences, bool ragged, int rank) { return rank > 32 && row_tiles(rows, sequences, ragged) > 1 ? 2 : 1; }
 int pieces_of(int rows, int sequences, bool ragged, int nt) { return ragged ? rows / (16 * nt) + 2 * sequences : sequences; }
-// Parts of the reduction: as many workgroups of four waves as the chip has places for four times over, no less than a step a wave.
-int splits_of(int rows, int sequences, bool ragged, int width, int dtype) {
-  const int nt = row_tiles(rows, sequences, ragged);
+// Parts of the reduction: for 768 workgroups, of a step a wave at least; up to eight for single rows, two for
+// few pieces of rows (expand adds them up in every wave: with two parts of 257 pieces it takes 26.5 us instead of 18.9, shrink 11.0 instead of 14.7).
+int splits_of(int rows, int sequences, bool ragged, int width, int rank, int dtype) {
+  const int nt = shrink_tiles(rows, sequences, ragged, rank);
   const int64_t real = ragged ? (rows + 16 * nt - 1) / (16 * nt) : sequences;
-  const int steps = (width * (dtype == LLMQ_F32 ? 4 : 2) + 127) / 128;
-  int64_t splits = 512 / (real < 1 ? 1 : real);
-  const int most = (steps + kShrinkWaves - 1) / kShrinkWaves;
+  const int steps = (width * (dtype == LLMQ_F32 ? 4 : 2) + 127) / 128, most = !ragged ? 8 : real < 96 ? 2 : 1;
+  int64_t splits = 768 / (real < 1 ? 1 : real);
+  if (splits > steps / shrink_waves(rank)) splits = steps / shrink_waves(rank);
   if (splits > most) splits = most;
-  if (splits > 16) splits = 16;
   return static_cast<int>(splits < 1 ? 1 : splits);
 }
 
 template <typename T, int RT>
-void shrink_nt(const T* x, int64_t stride, const Bank& bank, const Requests& req, float* planes, int64_t plane, int splits, int nt, int pieces, hipStream_t s) {
-  const dim3 grid(pieces, splits), block(kShrinkWaves * kWave);
-  if (nt == 1) hipLaunchKernelGGL((shrink_kernel<T, RT, 1>), grid, block, 0, s, x, stride, bank, req, planes, plane);
-  else if (nt == 2) hipLaunchKernelGGL((shrink_kernel<T, RT, 2>), grid, block, 0, s, x, stride, bank, req, planes, plane);
-  else hipLaunchKernelGGL((shrink_kernel<T, RT, 4>), grid, block, 0, s, x, stride, bank, req, planes, plane);
+void shrink_nt(const T* x, int64_t stride, const Bank& bank, const Requests& req, float* planes, int64_t plane, const dim3& grid, int nt, hipStream_t s) {
+  if (nt == 1) hipLaunchKernelGGL((shrink_kernel<T, RT, 1>), grid, dim3(kShrinkWaves<RT> * kWave), 0, s, x, stride, bank, req, planes, plane);
+  else if constexpr (RT >= 4) hipLaunchKernelGGL((shrink_kernel<T, RT, 2>), grid, dim3(kShrinkWaves<RT> * kWave), 0, s, x, stride, bank, req, planes, plane);
 }
 template <typename T>
-void shrink(const void* x, int64_t stride, const Bank& bank, const Requests& req, float* planes, int64_t plane, int splits, int nt, int pieces, hipStream_t s) {
+void shrink(const void* x, int64_t stride, const Bank& bank, const Requests& req, float* planes, int64_t plane, int splits, bool ragged, hipStream_t s) {
   const T* p = static_cast<const T*>(x);
-  if (bank.rank <= 16) shrink_nt<T, 1>(p, stride, bank, req, planes, plane, splits, nt, pieces, s);
-  else if (bank.rank <= 32) shrink_nt<T, 2>(p, stride, bank, req, planes, plane, splits, nt, pieces, s);
-  else if (bank.rank <= 64) shrink_nt<T, 4>(p, stride, bank, req, planes, plane, splits, nt, pieces, s);
-  else shrink_nt<T, 8>(p, stride, bank, req, planes, plane, splits, nt, pieces, s);
+  const int nt = shrink_tiles(req.rows.rows, req.rows.sequences, ragged, bank.rank);
+  const dim3 grid(pieces_of(req.rows.rows, req.rows.sequences, ragged, nt), splits);
+  if (bank.rank <= 16) shrink_nt<T, 1>(p, stride, bank, req, planes, plane, grid, nt, s);
+  else if (bank.rank <= 32) shrink_nt<T, 2>(p, stride, bank, req, planes, plane, grid, nt, s);
+  else if (bank.rank <= 64) shrink_nt<T, 4>(p, stride, bank, req, planes, plane, grid, nt, s);
+  else shrink_nt<T, 8>(p, stride, bank, req, planes, plane, grid, nt, s);
 }
 template <typename T, int RT> void expand_nt(const Bank& bank, const Requests& req, const Expand& e, int nt, const dim3& grid, hipStream_t s) {
   const dim3 block(kExpandWaves * kWave);
   if (nt == 1) hipLaunchKernelGGL((expand_kernel<T, RT, 1>), grid, block, 0, s, bank, req, e);
-  else if (nt == 2) hipLaunchKernelGGL((expand_kernel<T, RT, 2>), grid, block, 0, s, bank, req, e);
-  else hipLaunchKernelGGL((expand_kernel<T, RT, 4>), grid, block, 0, s, bank, req, e);
+  else hipLaunchKernelGGL((expand_kernel<T, RT, 2>), grid, block, 0, s, bank, req, e);
 }
 // bank: [slots][columns][rank]
-template <typename T> void expand(const Bank& bank, const Requests& req, Expand e, int nt, int pieces, hipStream_t s) {
-  const int units = (e.columns + 63) / 64;
-  e.pieces = pieces;
-  // (a workgroup adds up its piece's sums once: several units of columns a wave where there are workgroups enough without)
-  const int real = req.rows.start != nullptr ? (req.rows.rows + 16 * nt - 1) / (16 * nt) : pieces;
-  e.units = real * ((units + 15) / 16) >= 512 ? 4 : real * ((units + 7) / 8) >= 512 ? 2 : 1;
-  const bool rest = req.rows.start != nullptr && (e.out != e.base || e.low != nullptr);
-  const dim3 grid(pieces + (rest ? (e.rows + 16 * nt - 1) / (16 * nt) : 0), (units + kExpandWaves * e.units - 1) / (kExpandWaves * e.units));
+template <typename T> void expand(const Bank& bank, const Requests& req, Expand e, hipStream_t s) {
+  const bool ragged = req.rows.start != nullptr;
+  const int nt = row_tiles(e.rows, req.rows.sequences, ragged);
+  e.pieces = pieces_of(e.rows, req.rows.sequences, ragged, nt);
+  const bool rest = ragged && (e.out != e.base || e.low != nullptr);
+  const dim3 grid(e.pieces + (rest ? (e.rows + 16 * nt - 1) / (16 * nt) : 0), (e.columns + kExpandWaves * 128 - 1) / (kExpandWaves * 128));
   if (bank.rank <= 16) expand_nt<T, 1>(bank, req, e, nt, grid, s);
   else if (bank.rank <= 32) expand_nt<T, 2>(bank, req, e, nt, grid, s);
   else if (bank.rank <= 64) expand_nt<T, 4>(bank, req, e, nt, grid, s);
@@ -765,36 +726,30 @@ int64_t take(int64_t& at, int64_t bytes) {
 }
 
 struct GradPlan {
-  int nt, pieces, splits;
-  int capacity, blocks, tiles, shift, records;   // virtual rows, blocks of 32 of them, tiles of the rank, pieces of outer
-  int64_t o_start, o_order, o_slot_of, o_seq, o_at, o_bt, o_planes, o_du, o_op_du, o_op_low, o_rec_a, o_rec_b, bytes;
+  int splits, capacity, tiles, shift, records;   // parts of shrink, virtual rows, tiles of the rank, pieces of outer
+  int64_t o_start, o_order, o_seq, o_at, o_bt, o_planes, o_du, o_rec_a, o_rec_b, bytes;
 };
 GradPlan grad_plan(int rows, int sequences, bool ragged, int in, int out, int rank, int slots, int dtype) {
   GradPlan p{};
   const int64_t size = dtype == LLMQ_F32 ? 4 : 2;
-  p.nt = row_tiles(rows, sequences, ragged);
-  p.pieces = pieces_of(rows, sequences, ragged, p.nt);
-  p.splits = splits_of(rows, sequences, ragged, out, dtype);
+  p.splits = splits_of(rows, sequences, ragged, out, rank, dtype);
   const int64_t used = slots < sequences ? slots : sequences;   // slots that can have rows
   p.capacity = static_cast<int>(round_up(rows + 31 * used, kBlock));
-  p.blocks = p.capacity / kBlock;
   p.tiles = (rank + 15) / 16;
-  // a piece of outer: as long as 512 workgroups allow, 128 to 4096 rows
-  const int64_t columns = (in + kColumns - 1) / kColumns + (out + kColumns - 1) / kColumns;
+  // a piece of outer: 128 to 4096 rows, as long as it takes for the workgroups to be on the chip at once or nearly (with 64 entries of the rank
+  // one a CU, for their registers: 4099 rows by 8192 columns, pieces of 512 rows 33 us and 11.6 to add them up, 1024 28.4 + 7.4, 2048 34.8 + 7.3)
+  const int64_t columns = (in + kColumns - 1) / kColumns + (out + kColumns - 1) / kColumns, places = p.tiles >= 4 ? 400 : p.tiles >= 2 ? 512 : 1024;
   p.shift = 7;
-  while (p.shift < 12 && columns * (rows >> (p.shift + 1)) * ((p.tiles + 3) / 4) >= 512) ++p.shift;
+  while (p.shift < 12 && columns * ((rows >> p.shift) + used) * ((p.tiles + 3) / 4) > places) ++p.shift;
   p.records = (p.capacity >> p.shift) + 2 * slots;
   int64_t at = 0;
   p.o_start = take(at, int64_t{4} * (slots + 1));
   p.o_order = take(at, int64_t{4} * p.capacity);
-  p.o_slot_of = take(at, int64_t{4} * p.blocks);
   p.o_seq = take(at, int64_t{4} * sequences);
   p.o_at = take(at, size * slots * rank * in);
   p.o_bt = take(at, size * slots * rank * out);
   p.o_planes = take(at, int64_t{4} * p.splits * rows * rank);
-  p.o_du = take(at, int64_t{4} * rows * rank);
-  p.o_op_du = take(at, int64_t{4} * p.tiles * p.capacity * 16);
-  p.o_op_low = take(at, int64_t{4} * p.tiles * p.capacity * 16);
+  p.o_du = p.splits > 1 ? take(at, int64_t{4} * rows * rank) : p.o_planes;
   p.o_rec_a = take(at, int64_t{4} * p.records * rank * in);
   p.o_rec_b = take(at, int64_t{4} * p.records * rank * out);
   p.bytes = at;
@@ -807,22 +762,19 @@ void gradients(const GradPlan& p, const void* grad, int64_t grad_stride, const v
                void* grad_x, void* grad_a, void* grad_b, uint8_t* ws, int in, int out, int rank, int slots, hipStream_t s) {
   const int rows = req.rows.rows;
   float* planes = reinterpret_cast<float*>(ws + p.o_planes);
-  float* du = reinterpret_cast<float*>(ws + p.o_du);
+  float* du = reinterpret_cast<float*>(ws + p.o_du);   // g lora_b
   const int64_t plane = static_cast<int64_t>(rows) * rank;
   const Plan plan{slots, p.capacity, reinterpret_cast<int32_t*>(ws + p.o_start), reinterpret_cast<int32_t*>(ws + p.o_order),
-                  reinterpret_cast<int32_t*>(ws + p.o_slot_of), reinterpret_cast<int32_t*>(ws + p.o_seq)};
+                  reinterpret_cast<int32_t*>(ws + p.o_seq)};
   const Turn turn_a{lora_a, ws + p.o_at, rank, in}, turn_b{lora_b, ws + p.o_bt, out, rank};
   const unsigned tiles = static_cast<unsigned>(slots) * (((in + 63) / 64 + (out + 63) / 64) * ((rank + 63) / 64));
   if constexpr (sizeof(T) == 4) hipLaunchKernelGGL((prepare_kernel<uint32_t>), dim3(1 + tiles), dim3(kPlanThreads), 0, s, req, plan, turn_a, turn_b);
   else hipLaunchKernelGGL((prepare_kernel<uint16_t>), dim3(1 + tiles), dim3(kPlanThreads), 0, s, req, plan, turn_a, turn_b);
-  shrink<T>(grad, grad_stride, Bank{ws + p.o_bt, slots, rank, out}, req, planes, plane, p.splits, p.nt, p.pieces, s);
-  float* op_du = reinterpret_cast<float*>(ws + p.o_op_du);
-  float* op_low = reinterpret_cast<float*>(ws + p.o_op_low);
-  hipLaunchKernelGGL(operands_kernel, dim3(p.blocks), dim3(kOperandThreads), 0, s, planes, plane, p.splits, low, scaling, rank, plan, du, op_du, op_low);
-  expand<T>(Bank{ws + p.o_at, slots, rank, in}, req, Expand{du, plane, 1, nullptr, grad_base, base_stride, grad_x, nullptr, rows, in, 0, 0}, p.nt, p.pieces, s);
-  const Outer o{OuterSide{x, x_stride, x_scale, op_du, reinterpret_cast<float*>(ws + p.o_rec_a), in},
-                OuterSide{grad, grad_stride, nullptr, op_low, reinterpret_cast<float*>(ws + p.o_rec_b), out},
-                plan.start, plan.order, slots, rank, p.blocks, p.capacity, p.shift, (in + kColumns - 1) / kColumns};
+  shrink<T>(grad, grad_stride, Bank{ws + p.o_bt, slots, rank, out}, req, planes, plane, p.splits, req.rows.start != nullptr, s);
+  expand<T>(Bank{ws + p.o_at, slots, rank, in}, req, Expand{planes, plane, p.splits, scaling, grad_base, base_stride, grad_x, p.splits > 1 ? du : nullptr, rows, in, 0}, s);
+  const Outer o{OuterSide{x, x_stride, x_scale, du, reinterpret_cast<float*>(ws + p.o_rec_a), in},
+                OuterSide{grad, grad_stride, nullptr, low, reinterpret_cast<float*>(ws + p.o_rec_b), out},
+                plan.start, plan.order, scaling, slots, rank, p.capacity, p.shift, (in + kColumns - 1) / kColumns};
   const int rtw = p.tiles >= 4 ? 4 : p.tiles >= 2 ? 2 : 1;
   const dim3 grid(o.a_columns + (out + kColumns - 1) / kColumns, p.records, (p.tiles + rtw - 1) / rtw);
 #define LLMQ_OUTER(CODES)                                                                                    \
@@ -858,7 +810,7 @@ int bad_stride(int64_t stride, int width, int packet, const char* what) {
 
 extern "C" size_t llmq_lora_add_workspace_bytes(int rows, int sequences, int ragged, int in_features, int rank, int dtype) {
   if (rows <= 0 || sequences <= 0 || in_features <= 0 || rank <= 0) return 0;
-  return static_cast<size_t>(int64_t{4} * splits_of(rows, sequences, ragged != 0, in_features, dtype) * rows * rank);
+  return static_cast<size_t>(int64_t{4} * splits_of(rows, sequences, ragged != 0, in_features, rank, dtype) * rows * rank);
 }
 
 extern "C" int llmq_lora_add(const void* x, int64_t x_stride, const void* base, int64_t base_stride, const void* lora_a, const void* lora_b,
@@ -879,15 +831,14 @@ extern "C" int llmq_lora_add(const void* x, int64_t x_stride, const void* base, 
   if (!workspace || misaligned(workspace) || workspace_bytes < need)
     return llmq_host::fail_invalid("the workspace must be 16-byte aligned and hold %zu bytes, got %zu", need, workspace_bytes);
   const Requests req{adapter, Ragged{query_start_or_null, sequences, rows}};
-  const int nt = row_tiles(rows, sequences, ragged), pieces = pieces_of(rows, sequences, ragged, nt);
-  const int splits = splits_of(rows, sequences, ragged, in_features, dtype);
-  float* planes = static_cast<float*>(workspace);
+  const int splits = splits_of(rows, sequences, ragged, in_features, rank, dtype);
+  float* planes = splits == 1 && low_or_null ? low_or_null : static_cast<float*>(workspace);   // (one plane is the sum)
   const int64_t plane = static_cast<int64_t>(rows) * rank;
-  const Expand e{planes, plane, splits, scaling, base, base_stride, out, low_or_null, rows, out_features, 0, 0};
+  const Expand e{planes, plane, splits, scaling, base, base_stride, out, low_or_null, rows, out_features, 0};
   hipStream_t s = static_cast<hipStream_t>(stream);
 #define LLMQ_ADD(T)                                                                                                        \
-  shrink<T>(x, x_stride, Bank{lora_a, slots, rank, in_features}, req, planes, plane, splits, nt, pieces, s);               \
-  expand<T>(Bank{lora_b, slots, rank, out_features}, req, e, nt, pieces, s)
+  shrink<T>(x, x_stride, Bank{lora_a, slots, rank, in_features}, req, planes, plane, splits, ragged, s);                   \
+  expand<T>(Bank{lora_b, slots, rank, out_features}, req, e, s)
   switch (dtype) {
     case LLMQ_F32: LLMQ_ADD(float); break;
     case LLMQ_F16: LLMQ_ADD(f16_t); break;
