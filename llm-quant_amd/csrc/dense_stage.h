@@ -1,10 +1,7 @@
-// Matrices brought into the form that the tiles of dense_tile.h take (rows of a multiple of 64, one plane of 16-bit values or
-// three of an fp32 matrix), as they lie and / or transposed: activations, dense weights, and quantized weights as the
-// values (dtype)(code * scale) they stand for, which is the matrix that the reference multiplies by when many rows come
-// (`_dequantized_weight`, llmquant/quantizers/kernel.py:68-79).
-//
-// 64 x 64 values a workgroup, 16 bytes of every row at a time; the transposed form goes through LDS. Bound: HBM (or the
-// caches: a piece that was just written is read back by the product behind).
+// Matrices brought into the form that the tiles of dense_tile.h take where they are not in it (rows of a multiple of 64, one plane of
+// 16-bit values or three of an fp32 matrix): activations, dense weights, and quantized weights as the values (dtype)(code * scale) they
+// stand for, which is the matrix that the reference multiplies by when many rows come (`_dequantized_weight`,
+// llmquant/quantizers/kernel.py:68-79). And products whose result is a tensor.
 #pragma once
 
 #include "dense_tile.h"
@@ -14,113 +11,115 @@ namespace llmq {
 struct StageSource {
   const void* base;        // values [rows, stride], or codes [rows, groups, group_size] (BITS 4: two a byte)
   const float* scale;      // [scale rows, groups] of codes
-  const float* keep_rows;  // or null: rows whose entry is 0 are zeros in the transposed form
+  const float* keep_rows;  // or null: rows whose entry is 0 are zeros
   int64_t stride;          // elements between rows (values)
   int rows, cols;          // cols: a multiple of 8
-  int first_row;           // of the piece
-  int piece_rows;          // rows of the piece; those at or past `rows` are zeros
+  int first_row, piece_rows;   // of the piece; rows at or past `rows` are zeros
   int groups, group_size, keep, out_group;   // codes: `keep` values of a group are columns
-  int first_col = 0;       // codes: the first column taken
 };
+// [piece_rows, ld] a plane, zeros behind `cols`
 struct StageTarget {
-  void* rows;              // or null: [piece_rows, ld] a plane
-  void* transposed;        // or null: [cols, ld_t] a plane, columns up to a multiple of 64 written
-  int64_t plane, plane_t;  // elements between planes
-  int ld, ld_t;
+  void* rows;
+  int64_t plane;   // elements
+  int ld;          // a multiple of 8
 };
 
-// BITS: 0 values of T, 8 or 4 codes that stand for values of T
+constexpr int kStageAhead = 4;   // packets of a lane in flight
+// BITS: 0 values of T, 8 or 4 codes that stand for values of T. Eight values a lane and packet.
 template <typename T, int BITS>
-__global__ __launch_bounds__(256) void stage_kernel(const StageSource src, const StageTarget to) {
+__global__ __launch_bounds__(256) void stage_kernel(const StageSource src, const StageTarget to, const int64_t packets) {
   using O = typename TileType<T>::type;
-  constexpr int P = TileType<T>::kPlanes, kPad = 72;   // (halfwords a row of LDS: 16-byte reads of neighbouring rows meet other banks)
-  __shared__ __attribute__((aligned(16))) uint16_t s_t[P][64][kPad];
-  const int r0 = blockIdx.y * 64, c0 = blockIdx.x * 64;
+  constexpr int P = TileType<T>::kPlanes;
+  const int per_row = to.ld / 8;
+  const int64_t threads = static_cast<int64_t>(gridDim.x) * 256;
+  for (int64_t p0 = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; p0 < packets; p0 += kStageAhead * threads) {
+    u32x4 raw[kStageAhead][sizeof(T) == 4 && BITS == 0 ? 2 : 1];
+    float scale[kStageAhead];
+    bool real[kStageAhead];
 #pragma unroll
-  for (int half = 0; half < 2; ++half) {
-    const int r = r0 + half * 32 + static_cast<int>(threadIdx.x) / 8, c = c0 + static_cast<int>(threadIdx.x) % 8 * 8;
-    const int64_t row = static_cast<int64_t>(src.first_row) + r;
-    float f[8] = {};
-    if (r < src.piece_rows && row < src.rows && c < src.cols) {
+    for (int u = 0; u < kStageAhead; ++u) {
+      const int64_t p = p0 + u * threads < packets ? p0 + u * threads : packets - 1;
+      const int64_t r = p / per_row, row = src.first_row + r;
+      const int c = static_cast<int>(p - r * per_row) * 8;
+      real[u] = row < src.rows && c < src.cols && (src.keep_rows == nullptr || src.keep_rows[row] != 0.0f);
+      const int64_t from = row < src.rows ? row : src.rows - 1;
+      const int col = c < src.cols ? c : src.cols - 8;
+      scale[u] = 1.0f;
       if constexpr (BITS == 0) {
-        const T* x = static_cast<const T*>(src.base) + row * src.stride + c;
-#pragma unroll
-        for (int i = 0; i < 8; i += Pack<T>::N) Pack<T>::unpack(load16(x + i), f + i);
+        const T* x = static_cast<const T*>(src.base) + from * src.stride + col;
+        raw[u][0] = load16(x);
+        if constexpr (sizeof(T) == 4) raw[u][1] = load16(x + 4);
       } else {
-        const int g = (src.first_col + c) / src.keep, k = src.first_col + c - g * src.keep;
-        const int64_t group = row * src.groups + g;
-        const float s = src.scale[(src.out_group > 0 ? row / src.out_group : row) * src.groups + g];
+        const int g = col / src.keep, k = col - g * src.keep;
+        const int64_t group = from * src.groups + g;
+        scale[u] = src.scale[(src.out_group > 0 ? from / src.out_group : from) * src.groups + g];
         const uint8_t* q = static_cast<const uint8_t*>(src.base) + (group * src.group_size + k) * BITS / 8;
         if constexpr (BITS == 8) {
           const u32x2 w = *reinterpret_cast<const u32x2*>(q);
-#pragma unroll
-          for (int i = 0; i < 8; ++i) f[i] = static_cast<float>(static_cast<int8_t>((i < 4 ? w.x : w.y) >> (8 * (i % 4)))) * s;
+          raw[u][0] = u32x4{w.x, w.y, 0, 0};
         } else {
-          const uint32_t signs = *reinterpret_cast<const uint32_t*>(q) ^ 0x88888888u;   // (code + 8 with its top bit flipped: the code)
-#pragma unroll
-          for (int i = 0; i < 8; ++i) f[i] = static_cast<float>(static_cast<int32_t>(signs << (28 - 4 * i)) >> 28) * s;
+          raw[u][0] = u32x4{*reinterpret_cast<const uint32_t*>(q), 0, 0, 0};
         }
       }
     }
-    uint16_t v[P][8];
-    if constexpr (P == 1) {
-      const u32x4 w = Pack<O>::pack(f);   // (values of T come back as they were)
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[0][i] = static_cast<uint16_t>((i < 2 ? w.x : i < 4 ? w.y : i < 6 ? w.z : w.w) >> (16 * (i % 2)));
-    } else {
+    for (int u = 0; u < kStageAhead; ++u) {
+      const int64_t p = p0 + u * threads;
+      if (p >= packets) break;
+      float f[8];
+      if constexpr (BITS == 0) {
+        if constexpr (sizeof(T) == 4) {
+          Pack<float>::unpack(raw[u][0], f);
+          Pack<float>::unpack(raw[u][1], f + 4);
+        } else {
+          Pack<T>::unpack(raw[u][0], f);
+        }
+      } else if constexpr (BITS == 8) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        uint16_t p[3];
-        planes_of(f[i], p);
+        for (int i = 0; i < 8; ++i) f[i] = static_cast<float>(static_cast<int8_t>((i < 4 ? raw[u][0].x : raw[u][0].y) >> (8 * (i % 4)))) * scale[u];
+      } else {
+        const uint32_t signs = raw[u][0].x ^ 0x88888888u;   // (code + 8 with its top bit flipped: the code)
 #pragma unroll
-        for (int j = 0; j < P; ++j) v[j][i] = p[j];
+        for (int i = 0; i < 8; ++i) f[i] = static_cast<float>(static_cast<int32_t>(signs << (28 - 4 * i)) >> 28) * scale[u];
       }
-    }
-    if (to.rows != nullptr && r < src.piece_rows && c < to.ld) {
 #pragma unroll
-      for (int j = 0; j < P; ++j) {
-        u32x4 w;
-        w.x = v[j][0] | static_cast<uint32_t>(v[j][1]) << 16;
-        w.y = v[j][2] | static_cast<uint32_t>(v[j][3]) << 16;
-        w.z = v[j][4] | static_cast<uint32_t>(v[j][5]) << 16;
-        w.w = v[j][6] | static_cast<uint32_t>(v[j][7]) << 16;
-        store16(static_cast<uint16_t*>(to.rows) + j * to.plane + static_cast<int64_t>(r) * to.ld + c, w);
+      for (int i = 0; i < 8; ++i) f[i] = real[u] ? f[i] : 0.0f;
+      if constexpr (P == 1) {
+        store16(static_cast<uint16_t*>(to.rows) + p * 8, Pack<O>::pack(f));   // (values of T come back as they were)
+      } else {
+        uint16_t v[3][8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          uint16_t s[3];
+          planes_of(f[i], s);
+#pragma unroll
+          for (int j = 0; j < 3; ++j) v[j][i] = s[j];
+        }
+#pragma unroll
+        for (int j = 0; j < 3; ++j) {
+          u32x4 w;
+          w.x = v[j][0] | static_cast<uint32_t>(v[j][1]) << 16;
+          w.y = v[j][2] | static_cast<uint32_t>(v[j][3]) << 16;
+          w.z = v[j][4] | static_cast<uint32_t>(v[j][5]) << 16;
+          w.w = v[j][6] | static_cast<uint32_t>(v[j][7]) << 16;
+          store16(static_cast<uint16_t*>(to.rows) + j * to.plane + p * 8, w);
+        }
       }
-    }
-    if (to.transposed != nullptr) {
-      const bool dropped = src.keep_rows != nullptr && row < src.rows && src.keep_rows[row] == 0.0f;
-#pragma unroll
-      for (int j = 0; j < P; ++j)
-#pragma unroll
-        for (int i = 0; i < 8; ++i) s_t[j][threadIdx.x % 8 * 8 + i][half * 32 + threadIdx.x / 8] = dropped ? uint16_t{0} : v[j][i];
-    }
-  }
-  if (to.transposed == nullptr) return;
-  __syncthreads();
-#pragma unroll
-  for (int half = 0; half < 2; ++half) {
-    const int c = half * 32 + static_cast<int>(threadIdx.x) / 8, r = static_cast<int>(threadIdx.x) % 8 * 8;
-    if (c0 + c < src.cols && r0 + r < to.ld_t) {
-#pragma unroll
-      for (int j = 0; j < P; ++j)
-        store16(static_cast<uint16_t*>(to.transposed) + j * to.plane_t + static_cast<int64_t>(c0 + c) * to.ld_t + r0 + r,
-                load16(&s_t[j][c][r]));
     }
   }
 }
 
-// Both forms of a piece: rows up to a multiple of 64 and columns up to `ld` are covered (zeros past the ends).
 template <typename T>
 inline void stage_launch(const StageSource& src, const StageTarget& to, int bits, hipStream_t stream) {
-  const int cols = to.rows != nullptr && to.ld > src.cols ? to.ld : src.cols;
-  const dim3 grid((cols + 63) / 64, (src.piece_rows + 63) / 64);
-  if (bits == 0) hipLaunchKernelGGL((stage_kernel<T, 0>), grid, dim3(256), 0, stream, src, to);
-  else if (bits == 8) hipLaunchKernelGGL((stage_kernel<T, 8>), grid, dim3(256), 0, stream, src, to);
-  else hipLaunchKernelGGL((stage_kernel<T, 4>), grid, dim3(256), 0, stream, src, to);
+  const int64_t packets = static_cast<int64_t>(src.piece_rows) * (to.ld / 8), blocks = (packets + 256 * kStageAhead - 1) / (256 * kStageAhead);
+  const dim3 grid(static_cast<unsigned>(blocks < 256 * 32 ? blocks : 256 * 32));
+  if (bits == 0) hipLaunchKernelGGL((stage_kernel<T, 0>), grid, dim3(256), 0, stream, src, to, packets);
+  else if (bits == 8) hipLaunchKernelGGL((stage_kernel<T, 8>), grid, dim3(256), 0, stream, src, to, packets);
+  else hipLaunchKernelGGL((stage_kernel<T, 4>), grid, dim3(256), 0, stream, src, to, packets);
 }
 
 // ---- products whose result is a tensor ------------------------------------------------------------------------------------
-// out[n, m] = sum_k A[m, k] B[n, k], n < B's rows, m < A's rows. SUMS: fp32 planes, one a split of K (blockIdx.z), added to what is there unless
+// out[n, m] = sum_k A[m, k] B[n, k], n < B's rows, m < A's rows, A with K outermost, B (B_K) too or not. SUMS: fp32 planes, one a split of K (blockIdx.z), added to what is there unless
 // `first`; else the type of the call, times *scale (null: 1).
 struct ProductOut {
   void* base;
@@ -129,11 +128,11 @@ struct ProductOut {
   int first;
 };
 
-template <typename T, int TM, int TN, int WM, int WN, bool SUMS>
+template <typename T, int TM, int TN, int WM, int WN, bool SUMS, bool B_K>
 __global__ __launch_bounds__(WM * WN * kWave) void product_kernel(const TileOperand a, const TileOperand b, const int k,
                                                                        const int m_tiles, const ProductOut out) {
   using O = typename TileType<T>::type;
-  using Tile = DenseTile<O, TM, TN, WM, WN>;
+  using Tile = DenseTile<O, TM, TN, WM, WN, true, B_K>;
   __shared__ __attribute__((aligned(16))) uint8_t s_mem[Tile::kLdsBytes];
   const int steps = k / Tile::kStep, splits = gridDim.z, per = (steps + splits - 1) / splits;
   const int k0 = min(static_cast<int>(blockIdx.z) * per, steps) * Tile::kStep, k1 = min((static_cast<int>(blockIdx.z) + 1) * per, steps) * Tile::kStep;
@@ -220,12 +219,12 @@ inline int splits_for(int m_rows, int n_rows, int k) {
   return static_cast<int>(splits < 1 ? 1 : splits);
 }
 
-template <typename T, bool SUMS>
+template <typename T, bool SUMS, bool B_K>
 inline void product_launch(const TileOperand& a, const TileOperand& b, int k, const ProductOut& out, int splits, hipStream_t stream) {
   const int m_tiles = (a.rows + 255) / 256, tn = tile_rows(b.rows), n_tiles = (b.rows + tn - 1) / tn;
   const dim3 grid(static_cast<unsigned>(m_tiles) * n_tiles, 1, splits);
-  if (tn == kFewRows) hipLaunchKernelGGL((product_kernel<T, 256, 64, 4, 2, SUMS>), grid, dim3(512), 0, stream, a, b, k, m_tiles, out);
-  else hipLaunchKernelGGL((product_kernel<T, 256, 256, 2, 4, SUMS>), grid, dim3(512), 0, stream, a, b, k, m_tiles, out);
+  if (tn == kFewRows) hipLaunchKernelGGL((product_kernel<T, 256, 64, 4, 2, SUMS, B_K>), grid, dim3(512), 0, stream, a, b, k, m_tiles, out);
+  else hipLaunchKernelGGL((product_kernel<T, 256, 256, 2, 4, SUMS, B_K>), grid, dim3(512), 0, stream, a, b, k, m_tiles, out);
 }
 
 inline int64_t round_up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }

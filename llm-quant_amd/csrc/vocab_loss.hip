@@ -158,10 +158,9 @@ __global__ __launch_bounds__(1024) void scale_rows_kernel(const float* __restric
 }
 
 struct PieceOut {
-  void* p;             // [rows, ld] a plane
-  void* p_t;           // or null: [tokens of the piece, ld_t] a plane
-  int64_t plane, plane_t;
-  int ld, ld_t;
+  void* p;        // [padded rows, ld] a plane: zeros for rows past the end and tokens past the vocabulary
+  int64_t plane;
+  int ld, padded;
 };
 
 template <typename T, int TN, int WM, int WN>
@@ -169,7 +168,7 @@ __global__ __launch_bounds__(WM * WN * kWave) void piece_kernel(const TileOperan
                                                                      const int n_tiles, const int first_token, const LossRows rows, const PieceOut out) {
   using O = typename TileType<T>::type;
   constexpr int P = TileType<T>::kPlanes;
-  using Tile = DenseTile<O, 256, TN, WM, WN>;
+  using Tile = DenseTile<O, 256, TN, WM, WN, false, false, 2>;
   __shared__ __attribute__((aligned(16))) uint8_t s_mem[Tile::kLdsBytes];
   const int tile = tile_of_workgroup(blockIdx.x, gridDim.x), n0 = tile % n_tiles * TN, m0 = tile / n_tiles * 256;
   Tile t;
@@ -180,36 +179,32 @@ __global__ __launch_bounds__(WM * WN * kWave) void piece_kernel(const TileOperan
     const bool real = n < rows.rows;
     const float g = real ? rows.grad[n] : 0.0f, lse = real ? rows.lse[n] : 0.0f;
     const int64_t target = real ? rows.targets[n] - (first_token + m0) : -1;   // within the tile
+    if (n >= out.padded) continue;
 #pragma unroll
-    for (int mi = 0; mi < Tile::MI; ++mi) {
-      float f[4];
+    for (int mi = 0; mi < Tile::MI; mi += 2) {   // eight neighbouring tokens
+      uint16_t v[P][8];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int m = Tile::row_of(mi, i);
-        const float e = __builtin_amdgcn_exp2f((t.acc[mi][ni][i] - lse) * kLog2e) - (target == m ? 1.0f : 0.0f);
-        f[i] = g == 0.0f || m0 + m >= weight.rows ? 0.0f : e * g;   // (a row that does not count may hold anything)
-      }
-      uint16_t v[P][4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
+      for (int i = 0; i < 8; ++i) {
+        const int m = Tile::row_of(mi, 0) + i;
+        const float e = __builtin_amdgcn_exp2f((t.acc[mi + i / 4][ni][i % 4] - lse) * kLog2e) - (target == m ? 1.0f : 0.0f);
+        const float f = g == 0.0f || m0 + m >= weight.rows ? 0.0f : e * g;   // (a row that does not count may hold anything)
         if constexpr (P == 1) {
-          v[0][i] = __builtin_bit_cast(uint16_t, from_float<O>(f[i]));
+          v[0][i] = __builtin_bit_cast(uint16_t, from_float<O>(f));
         } else {
           uint16_t p[3];
-          planes_of(f[i], p);
+          planes_of(f, p);
 #pragma unroll
           for (int j = 0; j < P; ++j) v[j][i] = p[j];
         }
       }
 #pragma unroll
       for (int j = 0; j < P; ++j) {
-        const u32x2 w{v[j][0] | static_cast<uint32_t>(v[j][1]) << 16, v[j][2] | static_cast<uint32_t>(v[j][3]) << 16};
-        if (real) *reinterpret_cast<u32x2*>(static_cast<uint16_t*>(out.p) + j * out.plane + static_cast<int64_t>(n) * out.ld + m0 + Tile::row_of(mi, 0)) = w;
-        if (out.p_t != nullptr && n < out.ld_t) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            static_cast<uint16_t*>(out.p_t)[j * out.plane_t + static_cast<int64_t>(m0 + Tile::row_of(mi, i)) * out.ld_t + n] = v[j][i];
-        }
+        u32x4 w;
+        w.x = v[j][0] | static_cast<uint32_t>(v[j][1]) << 16;
+        w.y = v[j][2] | static_cast<uint32_t>(v[j][3]) << 16;
+        w.z = v[j][4] | static_cast<uint32_t>(v[j][5]) << 16;
+        w.w = v[j][6] | static_cast<uint32_t>(v[j][7]) << 16;
+        store16(static_cast<uint16_t*>(out.p) + j * out.plane + static_cast<int64_t>(n) * out.ld + m0 + Tile::row_of(mi, 0), w);
       }
     }
   }
@@ -224,7 +219,7 @@ struct Plan {
   int piece;                               // tokens of a piece, a multiple of 256
   int splits;                              // of dh's products
   // offsets into the workspace
-  int64_t o_stats, o_chosen, o_hidden, o_weight, o_scaled, o_back, o_hidden_t, o_weight_t, o_p, o_p_t, o_sums, bytes;
+  int64_t o_stats, o_chosen, o_hidden, o_weight, o_scaled, o_back, o_p, o_sums, bytes;
 };
 
 int64_t take(int64_t& at, int64_t bytes) {
@@ -234,8 +229,8 @@ int64_t take(int64_t& at, int64_t bytes) {
 }
 
 // The piece of the vocabulary: a whole number of rounds of 256 workgroups' tiles where that is no more than what the workspace for pieces
-// (kPieceBytes) holds.
-constexpr int64_t kPieceBytes = int64_t{512} << 20;
+// (kPieceBytes, which the caches hold) has room for.
+constexpr int64_t kPieceBytes = int64_t{192} << 20;
 
 Plan plan_for(int rows, int vocab, int hidden, int wformat, int dtype, bool gradient, bool learned) {
   Plan p{};
@@ -247,12 +242,13 @@ Plan plan_for(int rows, int vocab, int hidden, int wformat, int dtype, bool grad
   p.k = static_cast<int>(round_up(hidden, 64));
   const int tn = tile_rows(rows);
   p.padded = static_cast<int>(round_up(rows, tn));
-  p.stage_hidden = p.planes > 1 || hidden % 64 != 0;
-  p.stage_weight = p.stage_hidden || wformat != 0;
+  const bool whole_steps = p.planes == 1 && hidden % 64 == 0;
+  p.stage_hidden = !whole_steps || learned;   // (a head that learns: rows that do not count are zeros, whatever they hold)
+  p.stage_weight = !whole_steps || wformat != 0;
   const int64_t row16 = int64_t{2} * p.planes;   // bytes of a value in operand form
-  const int64_t whole = round_up(vocab, 256);
+  const int64_t whole = round_up(vocab, 256), rows64 = round_up(rows, 64);
   int64_t per_token = p.stage_weight ? p.k * row16 : 0;
-  if (gradient) per_token += hidden * row16 + rows * row16 + (learned ? p.padded * row16 : 0);
+  if (gradient) per_token += rows64 * row16;
   int64_t piece = whole;
   if (per_token > 0) {
     const int64_t n_tiles = p.padded / tn, round = n_tiles >= 256 ? 256 : 256 / n_tiles * 256;   // tokens of a round of workgroups
@@ -263,7 +259,7 @@ Plan plan_for(int rows, int vocab, int hidden, int wformat, int dtype, bool grad
   }
   p.piece = static_cast<int>(piece);
   int64_t at = 0;
-  if (p.stage_hidden) p.o_hidden = take(at, p.rows * p.k * row16);
+  if (p.stage_hidden) p.o_hidden = take(at, rows64 * p.k * row16);
   if (p.stage_weight) p.o_weight = take(at, piece * p.k * row16);
   if (!gradient) {
     p.o_stats = take(at, whole / 256 * rows * 8);
@@ -272,12 +268,7 @@ Plan plan_for(int rows, int vocab, int hidden, int wformat, int dtype, bool grad
     p.splits = splits_for(hidden, rows, static_cast<int>(piece));
     p.o_scaled = take(at, int64_t{4} * p.padded);
     p.o_back = take(at, 4);
-    p.o_weight_t = take(at, hidden * piece * row16);
-    p.o_p = take(at, rows * piece * row16);
-    if (learned) {
-      p.o_hidden_t = take(at, hidden * round_up(rows, 64) * row16);
-      p.o_p_t = take(at, piece * round_up(rows, 64) * row16);
-    }
+    p.o_p = take(at, rows64 * piece * row16);
     p.o_sums = take(at, int64_t{4} * p.splits * rows * hidden);
   }
   p.bytes = at;
@@ -311,35 +302,41 @@ struct Call {
   hipStream_t stream;
 };
 
-template <typename T> TileOperand hidden_operand(const Plan& p, const Call& c) {
-  if (!p.stage_hidden) return TileOperand{c.hidden, 0, static_cast<uint32_t>(c.hidden_stride * 2), p.rows};
-  return TileOperand{c.workspace + p.o_hidden, int64_t{2} * p.rows * p.k, static_cast<uint32_t>(p.k) * 2, p.rows};
+template <typename T> void stage_hidden(const Plan& p, const Call& c, const float* keep) {
+  const int rows64 = static_cast<int>(round_up(p.rows, 64));
+  stage_launch<T>(StageSource{c.hidden, nullptr, keep, c.hidden_stride, p.rows, p.hidden, 0, rows64, 0, 0, 0, 0},
+                  StageTarget{c.workspace + p.o_hidden, int64_t{rows64} * p.k, p.k}, 0, c.stream);
 }
-StageSource hidden_source(const Plan& p, const Call& c, const float* keep) {
-  return StageSource{c.hidden, nullptr, keep, c.hidden_stride, p.rows, p.hidden, 0, p.rows, 0, 0, 0, 0};
+TileOperand hidden_operand(const Plan& p, const Call& c) {
+  if (!p.stage_hidden) return TileOperand{c.hidden, 0, c.hidden_stride * 2, p.rows, 0};
+  return TileOperand{c.workspace + p.o_hidden, 2 * round_up(p.rows, 64) * p.k, int64_t{2} * p.k, p.rows, 0};
 }
-StageSource weight_source(const Plan& p, const Call& c, int first, int tokens) {
+// tokens first .. of the weight, brought into operand form where it is not
+template <typename T> int weight_piece(const Plan& p, const Call& c, int first, int tokens, int dtype, TileOperand& weight) {
+  weight = TileOperand{static_cast<const uint8_t*>(c.weight) + int64_t{2} * first * p.hidden, 0, int64_t{2} * p.hidden, tokens, tokens};
+  if (!p.stage_weight) return 0;
+  weight = TileOperand{c.workspace + p.o_weight, int64_t{2} * p.piece * p.k, int64_t{2} * p.k, tokens, tokens};
   const int groups = c.wformat ? p.hidden / c.group_size : 0;
-  return StageSource{c.weight, c.wscale, nullptr, p.hidden, p.vocab, p.hidden, first, tokens, groups, c.group_size, c.group_size, c.out_group};
-}
-TileOperand weight_operand(const Plan& p, const Call& c, int first, int tokens) {
-  if (!p.stage_weight) return TileOperand{static_cast<const uint8_t*>(c.weight) + int64_t{2} * first * p.hidden, 0, static_cast<uint32_t>(p.hidden) * 2, tokens};
-  return TileOperand{c.workspace + p.o_weight, int64_t{2} * p.piece * p.k, static_cast<uint32_t>(p.k) * 2, tokens};
+  if (c.wformat && p.planes == 1 && p.k == p.hidden && (c.out_group == 0 || first % c.out_group == 0))
+    return llmq_dequant_weight(static_cast<const uint8_t*>(c.weight) + static_cast<int64_t>(first) * p.hidden * c.wformat / 8,
+                               c.wscale + static_cast<int64_t>(c.out_group > 0 ? first / c.out_group : first) * groups, c.workspace + p.o_weight, tokens,
+                               groups, c.group_size, c.group_size, c.out_group, c.wformat, dtype, c.stream);
+  stage_launch<T>(StageSource{c.weight, c.wscale, nullptr, p.hidden, p.vocab, p.hidden, first, tokens, groups, c.group_size, c.group_size, c.out_group},
+                  StageTarget{c.workspace + p.o_weight, int64_t{p.piece} * p.k, p.k}, c.wformat, c.stream);
+  return 0;
 }
 
-template <typename T> int forward(const Plan& p, const Call& c, const int64_t* targets, int64_t ignore_index, float* losses, float* lse) {
-  if (p.stage_hidden)
-    stage_launch<T>(hidden_source(p, c, nullptr), StageTarget{c.workspace + p.o_hidden, nullptr, int64_t{p.rows} * p.k, 0, p.k, 0}, 0, c.stream);
-  const TileOperand hidden = hidden_operand<T>(p, c);
+template <typename T> int forward(const Plan& p, const Call& c, const int64_t* targets, int64_t ignore_index, float* losses, float* lse, int dtype) {
+  if (p.stage_hidden) stage_hidden<T>(p, c, nullptr);
+  const TileOperand hidden = hidden_operand(p, c);
   const LossRows rows{targets, nullptr, nullptr, p.rows, p.vocab};
   float2* stats = reinterpret_cast<float2*>(c.workspace + p.o_stats);
   float* chosen = reinterpret_cast<float*>(c.workspace + p.o_chosen);
   const int tn = tile_rows(p.rows), n_tiles = p.padded / tn;
   for (int first = 0; first < p.vocab; first += p.piece) {
     const int tokens = p.vocab - first < p.piece ? p.vocab - first : p.piece;
-    if (p.stage_weight)
-      stage_launch<T>(weight_source(p, c, first, tokens), StageTarget{c.workspace + p.o_weight, nullptr, int64_t{p.piece} * p.k, 0, p.k, 0}, c.wformat, c.stream);
-    const TileOperand weight = weight_operand(p, c, first, tokens);
+    TileOperand weight;
+    if (int rc = weight_piece<T>(p, c, first, tokens, dtype, weight)) return rc;
     const dim3 grid(static_cast<unsigned>((tokens + 255) / 256) * n_tiles);
     if (tn == kFewRows)
       hipLaunchKernelGGL((logits_kernel<T, 64, 4, 2>), grid, dim3(512), 0, c.stream, weight, hidden, p.k, n_tiles, first, first / 256, rows, stats, chosen);
@@ -352,41 +349,40 @@ template <typename T> int forward(const Plan& p, const Call& c, const int64_t* t
 
 template <typename T>
 int backward(const Plan& p, const Call& c, const int64_t* targets, int64_t ignore_index, const float* lse, const float* grad, void* grad_hidden,
-             void* grad_weight) {
+             void* grad_weight, int dtype) {
   float* scaled = reinterpret_cast<float*>(c.workspace + p.o_scaled);
   float* back = reinterpret_cast<float*>(c.workspace + p.o_back);
   float* sums = reinterpret_cast<float*>(c.workspace + p.o_sums);
   const bool learned = grad_weight != nullptr;
-  const int64_t rows64 = round_up(p.rows, 64);
+  const int rows64 = static_cast<int>(round_up(p.rows, 64));
   hipLaunchKernelGGL(scale_rows_kernel, dim3(1), dim3(1024), 0, c.stream, grad, targets, p.rows, p.padded, p.vocab, ignore_index, scaled, back);
-  if (p.stage_hidden || learned)
-    stage_launch<T>(hidden_source(p, c, scaled),
-                    StageTarget{p.stage_hidden ? c.workspace + p.o_hidden : nullptr, learned ? c.workspace + p.o_hidden_t : nullptr,
-                                int64_t{p.rows} * p.k, p.hidden * rows64, p.k, static_cast<int>(rows64)}, 0, c.stream);
-  const TileOperand hidden = hidden_operand<T>(p, c);
+  if (p.stage_hidden) stage_hidden<T>(p, c, learned ? scaled : nullptr);
+  const TileOperand hidden = hidden_operand(p, c);
   const LossRows rows{targets, lse, scaled, p.rows, p.vocab};
   const int tn = tile_rows(p.rows), n_tiles = p.padded / tn;
   for (int first = 0; first < p.vocab; first += p.piece) {
-    const int tokens = p.vocab - first < p.piece ? p.vocab - first : p.piece, tokens64 = static_cast<int>(round_up(tokens, 64));
-    stage_launch<T>(weight_source(p, c, first, tokens),
-                    StageTarget{p.stage_weight ? c.workspace + p.o_weight : nullptr, c.workspace + p.o_weight_t, int64_t{p.piece} * p.k,
-                                int64_t{p.hidden} * p.piece, p.k, p.piece}, c.wformat, c.stream);
-    const TileOperand weight = weight_operand(p, c, first, tokens);
-    const PieceOut piece{c.workspace + p.o_p, learned ? c.workspace + p.o_p_t : nullptr, int64_t{p.rows} * p.piece, p.piece * rows64, p.piece,
-                         static_cast<int>(rows64)};
+    const int tokens = p.vocab - first < p.piece ? p.vocab - first : p.piece;
+    TileOperand weight;
+    if (int rc = weight_piece<T>(p, c, first, tokens, dtype, weight)) return rc;
+    const PieceOut piece{c.workspace + p.o_p, int64_t{rows64} * p.piece, p.piece, rows64};
     const dim3 grid(static_cast<unsigned>((tokens + 255) / 256) * n_tiles);
     if (tn == kFewRows)
       hipLaunchKernelGGL((piece_kernel<T, 64, 4, 2>), grid, dim3(512), 0, c.stream, weight, hidden, p.k, n_tiles, first, rows, piece);
     else
       hipLaunchKernelGGL((piece_kernel<T, 256, 2, 4>), grid, dim3(512), 0, c.stream, weight, hidden, p.k, n_tiles, first, rows, piece);
-    const TileOperand weight_t{c.workspace + p.o_weight_t, int64_t{2} * p.hidden * p.piece, static_cast<uint32_t>(p.piece) * 2, p.hidden};
-    const TileOperand part{c.workspace + p.o_p, int64_t{2} * p.rows * p.piece, static_cast<uint32_t>(p.piece) * 2, p.rows};
-    product_launch<T, true>(weight_t, part, tokens64, ProductOut{sums, int64_t{p.rows} * p.hidden, p.hidden, nullptr, first == 0}, p.splits, c.stream);
-    if (learned) {
-      const TileOperand hidden_t{c.workspace + p.o_hidden_t, 2 * p.hidden * rows64, static_cast<uint32_t>(rows64) * 2, p.hidden};
-      const TileOperand part_t{c.workspace + p.o_p_t, 2 * p.piece * rows64, static_cast<uint32_t>(rows64) * 2, tokens};
-      product_launch<T, false>(hidden_t, part_t, static_cast<int>(rows64),
-                               ProductOut{static_cast<T*>(grad_weight) + static_cast<int64_t>(first) * p.hidden, 0, p.hidden, back, 0}, 1, c.stream);
+    // dh: over the piece's tokens, both as they lie (the weight's last row again behind its end, against zeros)
+    TileOperand weight_k = weight;
+    weight_k.rows = p.hidden;
+    const TileOperand part{c.workspace + p.o_p, int64_t{2} * rows64 * p.piece, int64_t{2} * p.piece, p.rows, 0};
+    product_launch<T, true, false>(weight_k, part, static_cast<int>(round_up(tokens, 64)),
+                                   ProductOut{sums, int64_t{p.rows} * p.hidden, p.hidden, nullptr, first == 0}, p.splits, c.stream);
+    if (learned) {   // dW: over the rows, both with them outermost
+      TileOperand hidden_k = hidden, part_k = part;
+      hidden_k.rows = p.hidden;
+      hidden_k.k_rows = part_k.k_rows = rows64;
+      part_k.rows = tokens;
+      product_launch<T, false, true>(hidden_k, part_k, rows64,
+                                     ProductOut{static_cast<T*>(grad_weight) + static_cast<int64_t>(first) * p.hidden, 0, p.hidden, back, 0}, 1, c.stream);
     }
   }
   add_planes_launch<T>(sums, int64_t{p.rows} * p.hidden, p.splits, back, grad_hidden, int64_t{p.rows} * p.hidden, c.stream);
@@ -420,9 +416,9 @@ extern "C" int llmq_vocab_loss(const void* hidden, int64_t hidden_stride, const 
     return llmq_host::fail_invalid("the workspace must be 16-byte aligned and hold %lld bytes, got %zu", static_cast<long long>(p.bytes), workspace_bytes);
   const Call c{hidden, weight, wscale_or_null, hidden_stride, group_size, out_group, wformat, static_cast<uint8_t*>(workspace), static_cast<hipStream_t>(stream)};
   switch (dtype) {
-    case LLMQ_F32: return forward<float>(p, c, targets, ignore_index, losses, lse);
-    case LLMQ_F16: return forward<f16_t>(p, c, targets, ignore_index, losses, lse);
-    default: return forward<bf16_t>(p, c, targets, ignore_index, losses, lse);
+    case LLMQ_F32: return forward<float>(p, c, targets, ignore_index, losses, lse, dtype);
+    case LLMQ_F16: return forward<f16_t>(p, c, targets, ignore_index, losses, lse, dtype);
+    default: return forward<bf16_t>(p, c, targets, ignore_index, losses, lse, dtype);
   }
 }
 
@@ -443,8 +439,8 @@ extern "C" int llmq_vocab_loss_grad(const void* hidden, int64_t hidden_stride, c
     return llmq_host::fail_invalid("the workspace must be 16-byte aligned and hold %lld bytes, got %zu", static_cast<long long>(p.bytes), workspace_bytes);
   const Call c{hidden, weight, wscale_or_null, hidden_stride, group_size, out_group, wformat, static_cast<uint8_t*>(workspace), static_cast<hipStream_t>(stream)};
   switch (dtype) {
-    case LLMQ_F32: return backward<float>(p, c, targets, ignore_index, lse, grad, grad_hidden, grad_weight_or_null);
-    case LLMQ_F16: return backward<f16_t>(p, c, targets, ignore_index, lse, grad, grad_hidden, grad_weight_or_null);
-    default: return backward<bf16_t>(p, c, targets, ignore_index, lse, grad, grad_hidden, grad_weight_or_null);
+    case LLMQ_F32: return backward<float>(p, c, targets, ignore_index, lse, grad, grad_hidden, grad_weight_or_null, dtype);
+    case LLMQ_F16: return backward<f16_t>(p, c, targets, ignore_index, lse, grad, grad_hidden, grad_weight_or_null, dtype);
+    default: return backward<bf16_t>(p, c, targets, ignore_index, lse, grad, grad_hidden, grad_weight_or_null, dtype);
   }
 }

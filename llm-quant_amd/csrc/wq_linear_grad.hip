@@ -3,8 +3,9 @@
 //   gx[t, k] = sum_n g[t, n] W[n, k],     W = (dtype)(code * scale): the matrix of the reference's many-rows branch
 //                                         (llmquant/quantizers/kernel.py:68-79), whose autograd this stands for
 //
-// The weight is brought, transposed, into operand form a piece of its columns at a time (dense_stage.h), and multiplied on the
-// matrix core (dense_tile.h). Bound: the matrix core for training batches, the weight's way through memory for few rows.
+// The weight is brought to its values a piece of its rows at a time (dense_stage.h: a piece that the caches hold), and multiplied on the
+// matrix core with the reduction outermost, as it lies (dense_tile.h); sums over the pieces and over the splits of one go through fp32 planes. Bound: the
+// matrix core for training batches, the weight's way through memory for few rows.
 #include "dense_stage.h"
 
 namespace {
@@ -12,29 +13,30 @@ namespace {
 using namespace llmq;
 
 struct Plan {
-  int64_t n_padded, piece;   // N in whole steps; columns of W a piece
+  int64_t n_padded, piece, ld;   // N in whole steps; rows of W a piece; its columns
   int splits;
   bool stage_grad;
   int64_t o_weight, o_grad, o_sums, bytes;
 };
 
-constexpr int64_t kPieceBytes = int64_t{256} << 20;
+constexpr int64_t kPieceBytes = int64_t{128} << 20;
 
 Plan plan_for(int rows, int N, int width, int dtype) {
   Plan p{};
   const int64_t row16 = dtype == LLMQ_F32 ? 6 : 2;
   p.n_padded = round_up(N, 64);
+  p.ld = width;
   p.stage_grad = dtype == LLMQ_F32 || N % 64 != 0;
-  p.piece = kPieceBytes / (p.n_padded * row16) / 256 * 256;
-  if (p.piece < 256) p.piece = 256;
-  if (p.piece > width) p.piece = width;
-  p.splits = splits_for(static_cast<int>(p.piece), rows, static_cast<int>(p.n_padded));
-  int64_t at = round_up(p.piece * p.n_padded * row16, 256);
+  p.piece = kPieceBytes / (width * row16) / 64 * 64;
+  if (p.piece < 64) p.piece = 64;
+  if (p.piece > p.n_padded) p.piece = p.n_padded;
+  p.splits = splits_for(width, rows, static_cast<int>(p.piece));
+  int64_t at = round_up(p.piece * width * row16, 256);
   if (p.stage_grad) {
     p.o_grad = at;
     at += round_up(rows * p.n_padded * row16, 256);
   }
-  if (p.splits > 1) {
+  if (p.splits > 1 || p.piece < p.n_padded) {
     p.o_sums = at;
     at += round_up(int64_t{4} * p.splits * rows * width, 256);
   }
@@ -43,25 +45,33 @@ Plan plan_for(int rows, int N, int width, int dtype) {
 }
 
 template <typename T>
-void launch(const Plan& p, const void* grad, int64_t stride, const void* qweight, const float* wscale, void* out, uint8_t* workspace, int rows,
-            int N, int G, int gs, int keep, int out_group, int wformat, hipStream_t stream) {
+int launch(const Plan& p, const void* grad, int64_t stride, const void* qweight, const float* wscale, void* out, uint8_t* workspace, int rows,
+           int N, int G, int gs, int keep, int out_group, int wformat, int dtype, hipStream_t stream) {
+  constexpr int P = TileType<T>::kPlanes;
   const int width = G * keep, n64 = static_cast<int>(p.n_padded);
-  if (p.stage_grad)
-    stage_launch<T>(StageSource{grad, nullptr, nullptr, stride, rows, N, 0, rows, 0, 0, 0, 0},
-                    StageTarget{workspace + p.o_grad, nullptr, rows * p.n_padded, 0, n64, 0}, 0, stream);
-  const TileOperand b = p.stage_grad ? TileOperand{workspace + p.o_grad, 2 * rows * p.n_padded, static_cast<uint32_t>(n64) * 2, rows}
-                                     : TileOperand{grad, 0, static_cast<uint32_t>(stride) * 2, rows};
+  if (p.stage_grad)   // (zeros up to a whole step, against rows of W that are looked at again)
+    stage_launch<T>(StageSource{grad, nullptr, nullptr, stride, rows, N, 0, rows, 0, 0, 0, 0}, StageTarget{workspace + p.o_grad, rows * p.n_padded, n64}, 0, stream);
+  const uint8_t* b_base = p.stage_grad ? workspace + p.o_grad : static_cast<const uint8_t*>(grad);
+  const int64_t b_plane = p.stage_grad ? 2 * rows * p.n_padded : 0, b_row = p.stage_grad ? int64_t{2} * n64 : stride * 2;
   float* sums = reinterpret_cast<float*>(workspace + p.o_sums);
-  for (int first = 0; first < width; first += static_cast<int>(p.piece)) {
-    const int cols = width - first < p.piece ? width - first : static_cast<int>(p.piece);
-    StageSource src{qweight, wscale, nullptr, 0, N, cols, 0, N, G, gs, keep, out_group};
-    src.first_col = first;
-    stage_launch<T>(src, StageTarget{nullptr, workspace, 0, p.piece * p.n_padded, 0, n64}, wformat, stream);
-    const TileOperand a{workspace, 2 * p.piece * p.n_padded, static_cast<uint32_t>(n64) * 2, cols};
-    if (p.splits > 1) product_launch<T, true>(a, b, n64, ProductOut{sums + first, static_cast<int64_t>(rows) * width, width, nullptr, 1}, p.splits, stream);
-    else product_launch<T, false>(a, b, n64, ProductOut{static_cast<T*>(out) + first, 0, width, nullptr, 1}, 1, stream);
+  const bool summed = p.o_sums != 0;
+  for (int first = 0; first < N; first += static_cast<int>(p.piece)) {
+    const int n = N - first < p.piece ? N - first : static_cast<int>(p.piece);
+    if (P == 1 && (out_group == 0 || first % out_group == 0)) {
+      const int64_t scale_row = out_group > 0 ? first / out_group : first;
+      if (int rc = llmq_dequant_weight(static_cast<const uint8_t*>(qweight) + static_cast<int64_t>(first) * G * gs * wformat / 8, wscale + scale_row * G,
+                                       workspace, n, G, gs, keep, out_group, wformat, dtype, stream)) return rc;
+    } else {
+      stage_launch<T>(StageSource{qweight, wscale, nullptr, 0, N, width, first, n, G, gs, keep, out_group}, StageTarget{workspace, p.piece * width, width}, wformat, stream);
+    }
+    const TileOperand a{workspace, 2 * p.piece * width, int64_t{2} * width, width, n};
+    const TileOperand b{b_base + int64_t{2} * first, b_plane, b_row, rows, 0};
+    const int k = static_cast<int>(round_up(n, 64));
+    if (summed) product_launch<T, true, false>(a, b, k, ProductOut{sums, static_cast<int64_t>(rows) * width, width, nullptr, first == 0}, p.splits, stream);
+    else product_launch<T, false, false>(a, b, k, ProductOut{out, 0, width, nullptr, 1}, 1, stream);
   }
-  if (p.splits > 1) add_planes_launch<T>(sums, static_cast<int64_t>(rows) * width, p.splits, nullptr, out, static_cast<int64_t>(rows) * width, stream);
+  if (summed) add_planes_launch<T>(sums, static_cast<int64_t>(rows) * width, p.splits, nullptr, out, static_cast<int64_t>(rows) * width, stream);
+  return llmq_host::check_launch("wq_linear_grad");
 }
 
 }  // namespace
@@ -97,9 +107,8 @@ extern "C" int llmq_wq_linear_grad(const void* grad, int64_t grad_stride, const 
   hipStream_t s = static_cast<hipStream_t>(stream);
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   switch (dtype) {
-    case LLMQ_F32: launch<float>(p, grad, grad_stride, qweight, wscale, grad_x, ws, rows, N, G, gs, keep_per_group, out_group, wformat, s); break;
-    case LLMQ_F16: launch<f16_t>(p, grad, grad_stride, qweight, wscale, grad_x, ws, rows, N, G, gs, keep_per_group, out_group, wformat, s); break;
-    default: launch<bf16_t>(p, grad, grad_stride, qweight, wscale, grad_x, ws, rows, N, G, gs, keep_per_group, out_group, wformat, s); break;
+    case LLMQ_F32: return launch<float>(p, grad, grad_stride, qweight, wscale, grad_x, ws, rows, N, G, gs, keep_per_group, out_group, wformat, dtype, s);
+    case LLMQ_F16: return launch<f16_t>(p, grad, grad_stride, qweight, wscale, grad_x, ws, rows, N, G, gs, keep_per_group, out_group, wformat, dtype, s);
+    default: return launch<bf16_t>(p, grad, grad_stride, qweight, wscale, grad_x, ws, rows, N, G, gs, keep_per_group, out_group, wformat, dtype, s);
   }
-  return llmq_host::check_launch("wq_linear_grad");
 }
