@@ -11,7 +11,7 @@ namespace llmq {
 struct StageSource {
   const void* base;        // values [rows, stride], or codes [rows, groups, group_size] (BITS 4: two a byte)
   const float* scale;      // [scale rows, groups] of codes
-  const float* keep_rows;  // or null: rows whose entry is 0 are zeros
+  const int32_t* gather;   // or null: the row behind each row of the piece; negative: zeros
   int64_t stride;          // elements between rows (values)
   int rows, cols;          // cols: a multiple of 8
   int first_row, piece_rows;   // of the piece; rows at or past `rows` are zeros
@@ -39,10 +39,10 @@ __global__ __launch_bounds__(256) void stage_kernel(const StageSource src, const
 #pragma unroll
     for (int u = 0; u < kStageAhead; ++u) {
       const int64_t p = p0 + u * threads < packets ? p0 + u * threads : packets - 1;
-      const int64_t r = p / per_row, row = src.first_row + r;
+      const int64_t r = p / per_row, row = src.gather != nullptr ? src.gather[r] : src.first_row + r;
       const int c = static_cast<int>(p - r * per_row) * 8;
-      real[u] = row < src.rows && c < src.cols && (src.keep_rows == nullptr || src.keep_rows[row] != 0.0f);
-      const int64_t from = row < src.rows ? row : src.rows - 1;
+      real[u] = row >= 0 && row < src.rows && c < src.cols;
+      const int64_t from = row < 0 ? 0 : row < src.rows ? row : src.rows - 1;
       const int col = c < src.cols ? c : src.cols - 8;
       scale[u] = 1.0f;
       if constexpr (BITS == 0) {
@@ -126,6 +126,7 @@ struct ProductOut {
   int64_t plane, ld;   // elements
   const float* scale;
   int first;
+  const int32_t* count = nullptr;   // or null: how many rows (of B, or with B_K of K) there are; tiles and steps past them are left out
 };
 
 template <typename T, int TM, int TN, int WM, int WN, bool SUMS, bool B_K>
@@ -134,20 +135,15 @@ __global__ __launch_bounds__(WM * WN * kWave) void product_kernel(const TileOper
   using O = typename TileType<T>::type;
   using Tile = DenseTile<O, TM, TN, WM, WN, true, B_K>;
   __shared__ __attribute__((aligned(16))) uint8_t s_mem[Tile::kLdsBytes];
-  const int steps = k / Tile::kStep, splits = gridDim.z, per = (steps + splits - 1) / splits;
+  const int rows = out.count != nullptr ? *out.count : INT32_MAX;
+  const int steps = ((B_K ? min(k, rows) : k) + Tile::kStep - 1) / Tile::kStep, splits = gridDim.z, per = (steps + splits - 1) / splits;
   const int k0 = min(static_cast<int>(blockIdx.z) * per, steps) * Tile::kStep, k1 = min((static_cast<int>(blockIdx.z) + 1) * per, steps) * Tile::kStep;
   const int tile = tile_of_workgroup(blockIdx.x, gridDim.x), m0 = tile % m_tiles * TM, n0 = tile / m_tiles * TN;
-  if (k0 >= k1) {   // nothing of K is this split's: zeros where the sums begin, which they do in the first call
-    if (SUMS && out.first) {
-      for (int i = threadIdx.x; i < TM * TN; i += Tile::kThreads) {
-        const int n = n0 + i / TM, m = m0 + i % TM;
-        if (n < b.rows && m < a.rows) static_cast<float*>(out.base)[blockIdx.z * out.plane + n * out.ld + m] = 0.0f;
-      }
-    }
-    return;
-  }
+  if (!B_K && n0 >= rows) return;
+  if (SUMS && k0 >= k1 && !out.first) return;   // nothing of K is this split's; where the sums begin they are zeros
   Tile t;
-  t.template multiply<(TileType<T>::kPlanes == 3 ? 6 : 1)>(s_mem, a, m0, b, n0, k0, k1);
+  if (k0 < k1) t.template multiply<(TileType<T>::kPlanes == 3 ? 6 : 1)>(s_mem, a, m0, b, n0, k0, k1);
+  else t.clear();
   const float scale = SUMS || out.scale == nullptr ? 1.0f : *out.scale;
 #pragma unroll
   for (int ni = 0; ni < Tile::NI; ++ni) {
@@ -176,20 +172,38 @@ __global__ __launch_bounds__(WM * WN * kWave) void product_kernel(const TileOper
   }
 }
 
-// out[n, m] = (dtype)(scale * the sum of the planes), eight values a lane
+// out[n, m] = (dtype)(scale * the sum of the planes), eight values a lane. from: the planes' row behind each row (negative: zeros), or null.
 template <typename T>
 __global__ __launch_bounds__(256) void add_planes_kernel(const float* __restrict__ planes, const int64_t plane, const int splits,
-                                                         const float* __restrict__ scale_or_null, T* __restrict__ out, const int64_t count8) {
+                                                         const float* __restrict__ scale_or_null, const int32_t* __restrict__ from_or_null,
+                                                         T* __restrict__ out, const int64_t packets, const int per_row) {
+  constexpr int kAhead = 4;
   const float scale = scale_or_null == nullptr ? 1.0f : *scale_or_null;
-  for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < count8; i += static_cast<int64_t>(gridDim.x) * 256) {
+  for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < packets; i += static_cast<int64_t>(gridDim.x) * 256) {
     float f[8] = {};
-    for (int z = 0; z < splits; ++z) {
-      const float* p = planes + z * plane + i * 8;
-      const tile_v4f lo = *reinterpret_cast<const tile_v4f*>(p), hi = *reinterpret_cast<const tile_v4f*>(p + 4);
+    int64_t at = i;
+    if (from_or_null != nullptr) {
+      const int64_t row = i / per_row;
+      const int from = from_or_null[row];
+      at = from < 0 ? -1 : from * static_cast<int64_t>(per_row) + (i - row * per_row);
+    }
+    if (at >= 0) {
+      for (int z0 = 0; z0 < splits; z0 += kAhead) {
+        tile_v4f lo[kAhead], hi[kAhead];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        f[e] += lo[e];
-        f[4 + e] += hi[e];
+        for (int z = 0; z < kAhead; ++z) {
+          const float* p = planes + min(z0 + z, splits - 1) * plane + at * 8;
+          lo[z] = *reinterpret_cast<const tile_v4f*>(p);
+          hi[z] = *reinterpret_cast<const tile_v4f*>(p + 4);
+        }
+#pragma unroll
+        for (int z = 0; z < kAhead; ++z)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (z0 + z < splits) {
+              f[e] += lo[z][e];
+              f[4 + e] += hi[z][e];
+            }
       }
     }
 #pragma unroll
@@ -199,10 +213,11 @@ __global__ __launch_bounds__(256) void add_planes_kernel(const float* __restrict
   }
 }
 template <typename T>
-inline void add_planes_launch(const float* planes, int64_t plane, int splits, const float* scale, void* out, int64_t count, hipStream_t stream) {
-  const int64_t count8 = count / 8, blocks = (count8 + 255) / 256;
-  hipLaunchKernelGGL((add_planes_kernel<T>), dim3(static_cast<unsigned>(blocks < 4096 ? blocks : 4096)), dim3(256), 0, stream,
-                     planes, plane, splits, scale, static_cast<T*>(out), count8);
+inline void add_planes_launch(const float* planes, int64_t plane, int splits, const float* scale, const int32_t* from, void* out, int64_t rows, int width,
+                              hipStream_t stream) {
+  const int64_t packets = rows * (width / 8), blocks = (packets + 255) / 256;
+  hipLaunchKernelGGL((add_planes_kernel<T>), dim3(static_cast<unsigned>(blocks < 8192 ? blocks : 8192)), dim3(256), 0, stream,
+                     planes, plane, splits, scale, from, static_cast<T*>(out), packets, width / 8);
 }
 
 // Rows of B a tile takes: 64 where there are no more, else 256 (a tile of few rows is bound by A's bytes, not by the
@@ -223,8 +238,9 @@ template <typename T, bool SUMS, bool B_K>
 inline void product_launch(const TileOperand& a, const TileOperand& b, int k, const ProductOut& out, int splits, hipStream_t stream) {
   const int m_tiles = (a.rows + 255) / 256, tn = tile_rows(b.rows), n_tiles = (b.rows + tn - 1) / tn;
   const dim3 grid(static_cast<unsigned>(m_tiles) * n_tiles, 1, splits);
+  // (64 x 128 a wave: the transposing reads bring half as much an instruction, so that fewer of A's are better where B has none)
   if (tn == kFewRows) hipLaunchKernelGGL((product_kernel<T, 256, 64, 4, 2, SUMS, B_K>), grid, dim3(512), 0, stream, a, b, k, m_tiles, out);
-  else hipLaunchKernelGGL((product_kernel<T, 256, 256, 2, 4, SUMS, B_K>), grid, dim3(512), 0, stream, a, b, k, m_tiles, out);
+  else hipLaunchKernelGGL((product_kernel<T, 256, 256, 4, 2, SUMS, B_K>), grid, dim3(512), 0, stream, a, b, k, m_tiles, out);
 }
 
 inline int64_t round_up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }

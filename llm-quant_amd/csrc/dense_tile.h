@@ -165,14 +165,17 @@ template <typename T, int TM, int TN, int WM, int WN, bool A_K = false, bool B_K
   }
 
  public:
-  // PAIRS: products of planes (1, or 6 of fp32). k0, k1: the part of K, multiples of 64, k0 < k1.
-  template <int PAIRS>
-  __device__ __forceinline__ void multiply(uint8_t* lds, const TileOperand& a, int m0, const TileOperand& b, int n0, int k0, int k1) {
-    const int wv = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) / kWave), wm = wv / WN, wn = wv % WN;
+  __device__ __forceinline__ void clear() {
 #pragma unroll
     for (int mi = 0; mi < MI; ++mi)
 #pragma unroll
       for (int ni = 0; ni < NI; ++ni) acc[mi][ni] = tile_v4f{0.0f, 0.0f, 0.0f, 0.0f};
+  }
+  // PAIRS: products of planes (1, or 6 of fp32). k0, k1: the part of K, multiples of 64, k0 < k1.
+  template <int PAIRS>
+  __device__ __forceinline__ void multiply(uint8_t* lds, const TileOperand& a, int m0, const TileOperand& b, int n0, int k0, int k1) {
+    const int wv = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) / kWave), wm = wv / WN, wn = wv % WN;
+    clear();
     const Side<TM, MI, kALoads, A_K, MG> as(a, m0, wv, wm, 0);
     const Side<TN, NI, kBLoads, B_K, 1> bs(b, n0, wv, wn, 2 * kStep * TM);
     const int steps = (k1 - k0) / kStep, all = steps * PAIRS;

@@ -21,8 +21,6 @@ constexpr float kLog2e = 1.4426950408889634f;
 
 struct LossRows {
   const int64_t* targets;
-  const float* lse;     // gradient
-  const float* grad;    // gradient, scaled; padded with zeros to whole tiles
   int rows, vocab;
 };
 
@@ -132,54 +130,97 @@ __global__ __launch_bounds__(256) void loss_kernel(const float2* __restrict__ st
 }
 
 // ---- the gradient -----------------------------------------------------------------------------------------------------------
-// scaled[t] = g[t] 2^-e with e the exponent of the largest finite |g| (0 for rows that do not count, and past the end up to
-// `padded`), back = 2^e. One workgroup.
-__global__ __launch_bounds__(1024) void scale_rows_kernel(const float* __restrict__ grad, const int64_t* __restrict__ targets, const int rows,
-                                                          const int padded, const int vocab, const int64_t ignore_index,
-                                                          float* __restrict__ scaled, float* __restrict__ back) {
+// The rows that have a part in the gradient (their target is not ignore_index and their g not zero), in front and in order; the others, a
+// prompt's tokens for instance, cost nothing from here on.
+struct Counted {
+  int32_t* row;        // [padded]: the row of each; -1 behind the last
+  int32_t* place;      // [rows]: where a row went, or -1
+  int64_t* target;     // [padded]
+  float* lse;          // [padded]
+  float* grad;         // [padded]: g 2^-e with e the exponent of the largest finite |g|; 0 behind the last
+  float* back;         // 2^e
+  int32_t* count;
+};
+// One workgroup.
+__global__ __launch_bounds__(1024) void count_rows_kernel(const float* __restrict__ grad, const int64_t* __restrict__ targets, const float* __restrict__ lse,
+                                                          const int rows, const int padded, const int vocab, const int64_t ignore_index, const Counted c) {
   __shared__ float s_top[16];
+  __shared__ int s_n[2][16];
+  const int wv = threadIdx.x / kWave, lane = threadIdx.x % kWave;
   float top = 0.0f;
   for (int i = threadIdx.x; i < rows; i += 1024) {
     const float g = fabsf(grad[i]);
     if (targets[i] != ignore_index && g < INFINITY) top = fmaxf(top, g);
   }
   top = group_max<64>(top);
-  if (threadIdx.x % kWave == 0) s_top[threadIdx.x / kWave] = top;
+  if (lane == 0) s_top[wv] = top;
   __syncthreads();
   top = s_top[0];
   for (int w = 1; w < 16; ++w) top = fmaxf(top, s_top[w]);
   const int e = top > 0.0f ? min(max(ilogbf(top), -125), 125) : 0;
-  for (int i = threadIdx.x; i < padded; i += 1024) {
+  int begin = 0;
+  for (int i0 = 0, turn = 0; i0 < rows; i0 += 1024, turn ^= 1) {
+    const int i = i0 + threadIdx.x;
+    int64_t target = ignore_index;
     float g = 0.0f;
-    if (i < rows && targets[i] != ignore_index) g = targets[i] < 0 || targets[i] >= vocab ? NAN : ldexpf(grad[i], -e);
-    scaled[i] = g;
+    if (i < rows) {
+      target = targets[i];
+      g = target == ignore_index ? 0.0f : grad[i];
+    }
+    const bool counts = g != 0.0f;   // (NaN counts)
+    const uint64_t mask = __ballot(counts);
+    if (lane == 0) s_n[turn][wv] = __popcll(mask);
+    __syncthreads();
+    int at = begin, all = 0;
+    for (int w = 0; w < 16; ++w) {
+      if (w < wv) at += s_n[turn][w];
+      all += s_n[turn][w];
+    }
+    at += __popcll(mask & ((uint64_t{1} << lane) - 1));
+    if (i < rows) c.place[i] = counts ? at : -1;
+    if (counts) {
+      c.row[at] = i;
+      c.target[at] = target;
+      c.lse[at] = lse[i];
+      c.grad[at] = target < 0 || target >= vocab ? NAN : ldexpf(g, -e);
+    }
+    begin += all;
   }
-  if (threadIdx.x == 0) *back = ldexpf(1.0f, e);
+  for (int i = begin + threadIdx.x; i < padded; i += 1024) {
+    c.row[i] = -1;
+    c.target[i] = -1;
+    c.lse[i] = 0.0f;
+    c.grad[i] = 0.0f;
+  }
+  if (threadIdx.x == 0) {
+    *c.back = ldexpf(1.0f, e);
+    *c.count = begin;
+  }
 }
 
 struct PieceOut {
-  void* p;        // [padded rows, ld] a plane: zeros for rows past the end and tokens past the vocabulary
+  void* p;        // [padded rows, ld] a plane: zeros for rows behind the last of a step of 64, and tokens past the vocabulary
   int64_t plane;
   int ld, padded;
 };
 
 template <typename T, int TN, int WM, int WN>
 __global__ __launch_bounds__(WM * WN * kWave) void piece_kernel(const TileOperand weight, const TileOperand hidden, const int k,
-                                                                     const int n_tiles, const int first_token, const LossRows rows, const PieceOut out) {
+                                                                     const int n_tiles, const int first_token, const Counted rows, const PieceOut out) {
   using O = typename TileType<T>::type;
   constexpr int P = TileType<T>::kPlanes;
   using Tile = DenseTile<O, 256, TN, WM, WN, false, false, 2>;
   __shared__ __attribute__((aligned(16))) uint8_t s_mem[Tile::kLdsBytes];
-  const int tile = tile_of_workgroup(blockIdx.x, gridDim.x), n0 = tile % n_tiles * TN, m0 = tile / n_tiles * 256;
+  const int tile = tile_of_workgroup(blockIdx.x, gridDim.x), n0 = tile % n_tiles * TN, m0 = tile / n_tiles * 256, count = *rows.count;
+  if (n0 >= count) return;
   Tile t;
   t.template multiply<(P == 3 ? 6 : 1)>(s_mem, weight, m0, hidden, n0, 0, k);
 #pragma unroll
   for (int ni = 0; ni < Tile::NI; ++ni) {
     const int n = n0 + Tile::col_of(ni);
-    const bool real = n < rows.rows;
-    const float g = real ? rows.grad[n] : 0.0f, lse = real ? rows.lse[n] : 0.0f;
-    const int64_t target = real ? rows.targets[n] - (first_token + m0) : -1;   // within the tile
     if (n >= out.padded) continue;
+    const float g = rows.grad[n], lse = rows.lse[n];   // (0 behind the last)
+    const int64_t target = rows.target[n] - (first_token + m0);   // within the tile
 #pragma unroll
     for (int mi = 0; mi < Tile::MI; mi += 2) {   // eight neighbouring tokens
       uint16_t v[P][8];
@@ -187,7 +228,7 @@ __global__ __launch_bounds__(WM * WN * kWave) void piece_kernel(const TileOperan
       for (int i = 0; i < 8; ++i) {
         const int m = Tile::row_of(mi, 0) + i;
         const float e = __builtin_amdgcn_exp2f((t.acc[mi + i / 4][ni][i % 4] - lse) * kLog2e) - (target == m ? 1.0f : 0.0f);
-        const float f = g == 0.0f || m0 + m >= weight.rows ? 0.0f : e * g;   // (a row that does not count may hold anything)
+        const float f = g == 0.0f || m0 + m >= weight.rows ? 0.0f : e * g;
         if constexpr (P == 1) {
           v[0][i] = __builtin_bit_cast(uint16_t, from_float<O>(f));
         } else {
@@ -219,7 +260,7 @@ struct Plan {
   int piece;                               // tokens of a piece, a multiple of 256
   int splits;                              // of dh's products
   // offsets into the workspace
-  int64_t o_stats, o_chosen, o_hidden, o_weight, o_scaled, o_back, o_p, o_sums, bytes;
+  int64_t o_stats, o_chosen, o_hidden, o_weight, o_row, o_place, o_target, o_lse, o_grad, o_back, o_p, o_sums, bytes;
 };
 
 int64_t take(int64_t& at, int64_t bytes) {
@@ -243,7 +284,7 @@ Plan plan_for(int rows, int vocab, int hidden, int wformat, int dtype, bool grad
   const int tn = tile_rows(rows);
   p.padded = static_cast<int>(round_up(rows, tn));
   const bool whole_steps = p.planes == 1 && hidden % 64 == 0;
-  p.stage_hidden = !whole_steps || learned;   // (a head that learns: rows that do not count are zeros, whatever they hold)
+  p.stage_hidden = !whole_steps || gradient;   // (gradient: the rows that count)
   p.stage_weight = !whole_steps || wformat != 0;
   const int64_t row16 = int64_t{2} * p.planes;   // bytes of a value in operand form
   const int64_t whole = round_up(vocab, 256), rows64 = round_up(rows, 64);
@@ -266,8 +307,12 @@ Plan plan_for(int rows, int vocab, int hidden, int wformat, int dtype, bool grad
     p.o_chosen = take(at, int64_t{4} * rows);
   } else {
     p.splits = splits_for(hidden, rows, static_cast<int>(piece));
-    p.o_scaled = take(at, int64_t{4} * p.padded);
-    p.o_back = take(at, 4);
+    p.o_row = take(at, int64_t{4} * p.padded);
+    p.o_place = take(at, int64_t{4} * rows);
+    p.o_target = take(at, int64_t{8} * p.padded);
+    p.o_lse = take(at, int64_t{4} * p.padded);
+    p.o_grad = take(at, int64_t{4} * p.padded);
+    p.o_back = take(at, 8);
     p.o_p = take(at, rows64 * piece * row16);
     p.o_sums = take(at, int64_t{4} * p.splits * rows * hidden);
   }
@@ -302,9 +347,9 @@ struct Call {
   hipStream_t stream;
 };
 
-template <typename T> void stage_hidden(const Plan& p, const Call& c, const float* keep) {
+template <typename T> void stage_hidden(const Plan& p, const Call& c, const int32_t* gather) {
   const int rows64 = static_cast<int>(round_up(p.rows, 64));
-  stage_launch<T>(StageSource{c.hidden, nullptr, keep, c.hidden_stride, p.rows, p.hidden, 0, rows64, 0, 0, 0, 0},
+  stage_launch<T>(StageSource{c.hidden, nullptr, gather, c.hidden_stride, p.rows, p.hidden, 0, rows64, 0, 0, 0, 0},
                   StageTarget{c.workspace + p.o_hidden, int64_t{rows64} * p.k, p.k}, 0, c.stream);
 }
 TileOperand hidden_operand(const Plan& p, const Call& c) {
@@ -329,7 +374,7 @@ template <typename T> int weight_piece(const Plan& p, const Call& c, int first, 
 template <typename T> int forward(const Plan& p, const Call& c, const int64_t* targets, int64_t ignore_index, float* losses, float* lse, int dtype) {
   if (p.stage_hidden) stage_hidden<T>(p, c, nullptr);
   const TileOperand hidden = hidden_operand(p, c);
-  const LossRows rows{targets, nullptr, nullptr, p.rows, p.vocab};
+  const LossRows rows{targets, p.rows, p.vocab};
   float2* stats = reinterpret_cast<float2*>(c.workspace + p.o_stats);
   float* chosen = reinterpret_cast<float*>(c.workspace + p.o_chosen);
   const int tn = tile_rows(p.rows), n_tiles = p.padded / tn;
@@ -350,15 +395,16 @@ template <typename T> int forward(const Plan& p, const Call& c, const int64_t* t
 template <typename T>
 int backward(const Plan& p, const Call& c, const int64_t* targets, int64_t ignore_index, const float* lse, const float* grad, void* grad_hidden,
              void* grad_weight, int dtype) {
-  float* scaled = reinterpret_cast<float*>(c.workspace + p.o_scaled);
   float* back = reinterpret_cast<float*>(c.workspace + p.o_back);
+  const Counted rows{reinterpret_cast<int32_t*>(c.workspace + p.o_row), reinterpret_cast<int32_t*>(c.workspace + p.o_place),
+                     reinterpret_cast<int64_t*>(c.workspace + p.o_target), reinterpret_cast<float*>(c.workspace + p.o_lse),
+                     reinterpret_cast<float*>(c.workspace + p.o_grad), back, reinterpret_cast<int32_t*>(c.workspace + p.o_back + 4)};
   float* sums = reinterpret_cast<float*>(c.workspace + p.o_sums);
   const bool learned = grad_weight != nullptr;
   const int rows64 = static_cast<int>(round_up(p.rows, 64));
-  hipLaunchKernelGGL(scale_rows_kernel, dim3(1), dim3(1024), 0, c.stream, grad, targets, p.rows, p.padded, p.vocab, ignore_index, scaled, back);
-  if (p.stage_hidden) stage_hidden<T>(p, c, learned ? scaled : nullptr);
+  hipLaunchKernelGGL(count_rows_kernel, dim3(1), dim3(1024), 0, c.stream, grad, targets, lse, p.rows, p.padded, p.vocab, ignore_index, rows);
+  stage_hidden<T>(p, c, rows.row);
   const TileOperand hidden = hidden_operand(p, c);
-  const LossRows rows{targets, lse, scaled, p.rows, p.vocab};
   const int tn = tile_rows(p.rows), n_tiles = p.padded / tn;
   for (int first = 0; first < p.vocab; first += p.piece) {
     const int tokens = p.vocab - first < p.piece ? p.vocab - first : p.piece;
@@ -375,17 +421,17 @@ int backward(const Plan& p, const Call& c, const int64_t* targets, int64_t ignor
     weight_k.rows = p.hidden;
     const TileOperand part{c.workspace + p.o_p, int64_t{2} * rows64 * p.piece, int64_t{2} * p.piece, p.rows, 0};
     product_launch<T, true, false>(weight_k, part, static_cast<int>(round_up(tokens, 64)),
-                                   ProductOut{sums, int64_t{p.rows} * p.hidden, p.hidden, nullptr, first == 0}, p.splits, c.stream);
+                                   ProductOut{sums, int64_t{p.rows} * p.hidden, p.hidden, nullptr, first == 0, rows.count}, p.splits, c.stream);
     if (learned) {   // dW: over the rows, both with them outermost
       TileOperand hidden_k = hidden, part_k = part;
       hidden_k.rows = p.hidden;
       hidden_k.k_rows = part_k.k_rows = rows64;
       part_k.rows = tokens;
       product_launch<T, false, true>(hidden_k, part_k, rows64,
-                                     ProductOut{static_cast<T*>(grad_weight) + static_cast<int64_t>(first) * p.hidden, 0, p.hidden, back, 0}, 1, c.stream);
+                                     ProductOut{static_cast<T*>(grad_weight) + static_cast<int64_t>(first) * p.hidden, 0, p.hidden, back, 0, rows.count}, 1, c.stream);
     }
   }
-  add_planes_launch<T>(sums, int64_t{p.rows} * p.hidden, p.splits, back, grad_hidden, int64_t{p.rows} * p.hidden, c.stream);
+  add_planes_launch<T>(sums, int64_t{p.rows} * p.hidden, p.splits, back, rows.place, grad_hidden, p.rows, p.hidden, c.stream);
   return llmq_host::check_launch("vocab_loss_grad");
 }
 

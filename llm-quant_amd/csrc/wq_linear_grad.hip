@@ -70,7 +70,7 @@ int launch(const Plan& p, const void* grad, int64_t stride, const void* qweight,
     if (summed) product_launch<T, true, false>(a, b, k, ProductOut{sums, static_cast<int64_t>(rows) * width, width, nullptr, first == 0}, p.splits, stream);
     else product_launch<T, false, false>(a, b, k, ProductOut{out, 0, width, nullptr, 1}, 1, stream);
   }
-  if (summed) add_planes_launch<T>(sums, static_cast<int64_t>(rows) * width, p.splits, nullptr, out, static_cast<int64_t>(rows) * width, stream);
+  if (summed) add_planes_launch<T>(sums, static_cast<int64_t>(rows) * width, p.splits, nullptr, nullptr, out, rows, width, stream);
   return llmq_host::check_launch("wq_linear_grad");
 }
 
