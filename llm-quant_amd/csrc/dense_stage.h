@@ -119,13 +119,49 @@ inline void stage_launch(const StageSource& src, const StageTarget& to, int bits
 }
 
 // ---- products whose result is a tensor ------------------------------------------------------------------------------------
-// out[n, m] = sum_k A[m, k] B[n, k], n < B's rows, m < A's rows, A with K outermost, B (B_K) too or not. SUMS: fp32 planes, one a split of K (blockIdx.z), added to what is there unless
-// `first`; else the type of the call, times *scale (null: 1).
+// Rows of B a tile takes: 64 where there are no more, else 256 (a tile of few rows is bound by A's bytes, not by the
+// multiplications that its empty rows waste).
+constexpr int kFewRows = 64;
+constexpr int tile_rows(int rows) { return rows <= kFewRows ? kFewRows : 256; }
+
+// How a sum over K is dealt out: the tiles of the rows there are, and as many splits of K as the chip has places for, `most` at the most.
+struct Splits {
+  int n_tiles, splits;
+  int64_t plane;   // elements of a split's fp32 sums: whole tiles of rows
+};
+__host__ __device__ inline Splits splits_of_rows(int rows, int tn, int m_tiles, int64_t ld, int most) {
+  Splits s;
+  s.n_tiles = (rows + tn - 1) / tn;
+  const int places = tn == kFewRows ? 512 : 256, tiles = s.n_tiles * m_tiles;
+  s.splits = tiles > 0 && places / tiles > 1 ? places / tiles : 1;
+  if (s.splits > most) s.splits = most;
+  s.plane = static_cast<int64_t>(s.n_tiles) * tn * ld;
+  return s;
+}
+// splits of eight steps at least, sixteen at the most
+inline int most_splits(int m_rows, int n_rows, int k) {
+  const Splits s = splits_of_rows(n_rows < 256 ? n_rows : 256, tile_rows(n_rows), (m_rows + 255) / 256, m_rows, 16);   // (a tile of rows alone)
+  const int most = k / 64 / 8;
+  return s.splits < most ? s.splits : most < 1 ? 1 : most;
+}
+// bytes of the sums, however many of the rows there turn out to be
+inline int64_t sums_bytes(int m_rows, int n_rows, int most) {
+  const int tn = tile_rows(n_rows), m_tiles = (m_rows + 255) / 256;
+  int64_t largest = 0;
+  for (int n = tn; n < n_rows + tn; n += tn) {
+    const Splits s = splits_of_rows(n, tn, m_tiles, m_rows, most);
+    if (s.plane * s.splits > largest) largest = s.plane * s.splits;
+  }
+  return largest * 4;
+}
+
+// out[n, m] = sum_k A[m, k] B[n, k], n < B's rows, m < A's rows, A with K outermost, B (B_K) too or not. SUMS: fp32 planes, one a split of K, added
+// to what is there unless `first`; else the type of the call, times *scale (null: 1).
 struct ProductOut {
   void* base;
-  int64_t plane, ld;   // elements
+  int64_t ld;          // elements
   const float* scale;
-  int first;
+  int first, most;     // most: splits
   const int32_t* count = nullptr;   // or null: how many rows (of B, or with B_K of K) there are; tiles and steps past them are left out
 };
 
@@ -134,12 +170,19 @@ __global__ __launch_bounds__(WM * WN * kWave) void product_kernel(const TileOper
                                                                        const int m_tiles, const ProductOut out) {
   using O = typename TileType<T>::type;
   using Tile = DenseTile<O, TM, TN, WM, WN, true, B_K>;
+  constexpr int kBlockN = 4;
   __shared__ __attribute__((aligned(16))) uint8_t s_mem[Tile::kLdsBytes];
   const int rows = out.count != nullptr ? *out.count : INT32_MAX;
-  const int steps = ((B_K ? min(k, rows) : k) + Tile::kStep - 1) / Tile::kStep, splits = gridDim.z, per = (steps + splits - 1) / splits;
-  const int k0 = min(static_cast<int>(blockIdx.z) * per, steps) * Tile::kStep, k1 = min((static_cast<int>(blockIdx.z) + 1) * per, steps) * Tile::kStep;
-  const int tile = tile_of_workgroup(blockIdx.x, gridDim.x), m0 = tile % m_tiles * TM, n0 = tile / m_tiles * TN;
-  if (!B_K && n0 >= rows) return;
+  const int steps = ((B_K ? min(k, rows) : k) + Tile::kStep - 1) / Tile::kStep;
+  const Splits s = splits_of_rows(B_K ? b.rows : min(b.rows, rows), TN, m_tiles, out.ld, out.most);
+  const int tiles = m_tiles * s.n_tiles, id = blockIdx.x;
+  if (id >= tiles * s.splits) return;
+  // Workgroups that run together on an XCD are 32 neighbours of this order: a split's tiles in blocks of four of n, by m, by n: eight tiles of A by four
+  // of B. (By m alone, the splits side by side, an XCD's step read 36 tiles of operands where these are 12: 2048 x 4096 over 14336 259 us.)
+  const int at = tile_of_workgroup(id, tiles * s.splits), z = at / tiles, tile = at - z * tiles;
+  const int block = tile / (m_tiles * kBlockN), in_block = tile - block * m_tiles * kBlockN, wide = min(kBlockN, s.n_tiles - block * kBlockN);
+  const int m0 = in_block / wide * TM, n0 = (block * kBlockN + in_block % wide) * TN;
+  const int per = (steps + s.splits - 1) / s.splits, k0 = min(z * per, steps) * Tile::kStep, k1 = min((z + 1) * per, steps) * Tile::kStep;
   if (SUMS && k0 >= k1 && !out.first) return;   // nothing of K is this split's; where the sums begin they are zeros
   Tile t;
   if (k0 < k1) t.template multiply<(TileType<T>::kPlanes == 3 ? 6 : 1)>(s_mem, a, m0, b, n0, k0, k1);
@@ -154,7 +197,7 @@ __global__ __launch_bounds__(WM * WN * kWave) void product_kernel(const TileOper
       const int m = m0 + Tile::row_of(mi, 0);
       if (m >= a.rows) continue;   // (rows of A are a multiple of 4)
       if constexpr (SUMS) {
-        float* to = static_cast<float*>(out.base) + blockIdx.z * out.plane + n * out.ld + m;
+        float* to = static_cast<float*>(out.base) + z * s.plane + n * out.ld + m;
         tile_v4f v = t.acc[mi][ni];
         if (!out.first) v += *reinterpret_cast<const tile_v4f*>(to);
         *reinterpret_cast<tile_v4f*>(to) = v;
@@ -172,12 +215,28 @@ __global__ __launch_bounds__(WM * WN * kWave) void product_kernel(const TileOper
   }
 }
 
+template <typename T, bool SUMS, bool B_K>
+inline void product_launch(const TileOperand& a, const TileOperand& b, int k, const ProductOut& out, hipStream_t stream) {
+  const int m_tiles = (a.rows + 255) / 256, tn = tile_rows(b.rows);
+  unsigned groups = 0;   // (the most that there can be, however many rows count)
+  for (int n = out.count != nullptr && !B_K ? tn : (b.rows + tn - 1) / tn * tn; n < b.rows + tn; n += tn) {
+    const Splits s = splits_of_rows(n, tn, m_tiles, out.ld, out.most);
+    if (static_cast<unsigned>(m_tiles) * s.n_tiles * s.splits > groups) groups = static_cast<unsigned>(m_tiles) * s.n_tiles * s.splits;
+  }
+  // (64 x 128 a wave: the transposing reads bring half as much an instruction, so that fewer of A's are better where B has none)
+  if (tn == kFewRows) hipLaunchKernelGGL((product_kernel<T, 256, 64, 4, 2, SUMS, B_K>), dim3(groups), dim3(512), 0, stream, a, b, k, m_tiles, out);
+  else hipLaunchKernelGGL((product_kernel<T, 256, 256, 4, 2, SUMS, B_K>), dim3(groups), dim3(512), 0, stream, a, b, k, m_tiles, out);
+}
+
 // out[n, m] = (dtype)(scale * the sum of the planes), eight values a lane. from: the planes' row behind each row (negative: zeros), or null.
 template <typename T>
-__global__ __launch_bounds__(256) void add_planes_kernel(const float* __restrict__ planes, const int64_t plane, const int splits,
-                                                         const float* __restrict__ scale_or_null, const int32_t* __restrict__ from_or_null,
-                                                         T* __restrict__ out, const int64_t packets, const int per_row) {
+__global__ __launch_bounds__(256) void add_planes_kernel(const float* __restrict__ planes, const int rows, const int tn, const int m_tiles, const int most,
+                                                         const int32_t* __restrict__ count_or_null, const float* __restrict__ scale_or_null,
+                                                         const int32_t* __restrict__ from_or_null, T* __restrict__ out, const int64_t packets, const int per_row) {
   constexpr int kAhead = 4;
+  const Splits s = splits_of_rows(count_or_null == nullptr ? rows : min(rows, *count_or_null), tn, m_tiles, per_row * int64_t{8}, most);
+  const int64_t plane = s.plane;
+  const int splits = s.splits;
   const float scale = scale_or_null == nullptr ? 1.0f : *scale_or_null;
   for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < packets; i += static_cast<int64_t>(gridDim.x) * 256) {
     float f[8] = {};
@@ -212,35 +271,13 @@ __global__ __launch_bounds__(256) void add_planes_kernel(const float* __restrict
     for (int e = 0; e < 8; e += Pack<T>::N) store16(out + i * 8 + e, Pack<T>::pack(f + e));
   }
 }
+// (rows and most as the products had them)
 template <typename T>
-inline void add_planes_launch(const float* planes, int64_t plane, int splits, const float* scale, const int32_t* from, void* out, int64_t rows, int width,
+inline void add_planes_launch(const float* planes, int rows, int width, int most, const int32_t* count, const float* scale, const int32_t* from, void* out,
                               hipStream_t stream) {
-  const int64_t packets = rows * (width / 8), blocks = (packets + 255) / 256;
+  const int64_t packets = static_cast<int64_t>(rows) * (width / 8), blocks = (packets + 255) / 256;
   hipLaunchKernelGGL((add_planes_kernel<T>), dim3(static_cast<unsigned>(blocks < 8192 ? blocks : 8192)), dim3(256), 0, stream,
-                     planes, plane, splits, scale, from, static_cast<T*>(out), packets, width / 8);
-}
-
-// Rows of B a tile takes: 64 where there are no more, else 256 (a tile of few rows is bound by A's bytes, not by the
-// multiplications that its empty rows waste).
-constexpr int kFewRows = 64;
-constexpr int tile_rows(int rows) { return rows <= kFewRows ? kFewRows : 256; }
-
-// Splits of K so that the tiles fill the chip, of eight steps at least.
-inline int splits_for(int m_rows, int n_rows, int k) {
-  const int tn = tile_rows(n_rows), places = tn == kFewRows ? 512 : 256;
-  const int64_t tiles = static_cast<int64_t>((m_rows + 255) / 256) * ((n_rows + tn - 1) / tn);
-  const int64_t wanted = places / (tiles < 1 ? 1 : tiles), most = k / 64 / 8;
-  const int64_t splits = wanted < most ? wanted : most;
-  return static_cast<int>(splits < 1 ? 1 : splits);
-}
-
-template <typename T, bool SUMS, bool B_K>
-inline void product_launch(const TileOperand& a, const TileOperand& b, int k, const ProductOut& out, int splits, hipStream_t stream) {
-  const int m_tiles = (a.rows + 255) / 256, tn = tile_rows(b.rows), n_tiles = (b.rows + tn - 1) / tn;
-  const dim3 grid(static_cast<unsigned>(m_tiles) * n_tiles, 1, splits);
-  // (64 x 128 a wave: the transposing reads bring half as much an instruction, so that fewer of A's are better where B has none)
-  if (tn == kFewRows) hipLaunchKernelGGL((product_kernel<T, 256, 64, 4, 2, SUMS, B_K>), grid, dim3(512), 0, stream, a, b, k, m_tiles, out);
-  else hipLaunchKernelGGL((product_kernel<T, 256, 256, 4, 2, SUMS, B_K>), grid, dim3(512), 0, stream, a, b, k, m_tiles, out);
+                     planes, rows, tile_rows(rows), (width + 255) / 256, most, count, scale, from, static_cast<T*>(out), packets, width / 8);
 }
 
 inline int64_t round_up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }

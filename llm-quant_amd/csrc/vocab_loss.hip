@@ -211,8 +211,9 @@ __global__ __launch_bounds__(WM * WN * kWave) void piece_kernel(const TileOperan
   constexpr int P = TileType<T>::kPlanes;
   using Tile = DenseTile<O, 256, TN, WM, WN, false, false, 2>;
   __shared__ __attribute__((aligned(16))) uint8_t s_mem[Tile::kLdsBytes];
-  const int tile = tile_of_workgroup(blockIdx.x, gridDim.x), n0 = tile % n_tiles * TN, m0 = tile / n_tiles * 256, count = *rows.count;
-  if (n0 >= count) return;
+  const int counted = (*rows.count + TN - 1) / TN, tiles = static_cast<int>(gridDim.x) / n_tiles * counted;   // tiles of the rows that count
+  if (static_cast<int>(blockIdx.x) >= tiles) return;
+  const int tile = tile_of_workgroup(blockIdx.x, tiles), n0 = tile % counted * TN, m0 = tile / counted * 256;
   Tile t;
   t.template multiply<(P == 3 ? 6 : 1)>(s_mem, weight, m0, hidden, n0, 0, k);
 #pragma unroll
@@ -269,9 +270,9 @@ int64_t take(int64_t& at, int64_t bytes) {
   return here;
 }
 
-// The piece of the vocabulary: a whole number of rounds of 256 workgroups' tiles where that is no more than what the workspace for pieces
-// (kPieceBytes, which the caches hold) has room for.
-constexpr int64_t kPieceBytes = int64_t{192} << 20;
+// The piece of the vocabulary: a whole number of rounds of 256 workgroups' tiles, as many as the workspace for pieces has room for: how many
+// rows count is not known when a call is made, and in several rounds the tiles of those that do not leave room for others.
+constexpr int64_t kPieceBytes = int64_t{768} << 20;
 
 Plan plan_for(int rows, int vocab, int hidden, int wformat, int dtype, bool gradient, bool learned) {
   Plan p{};
@@ -306,7 +307,7 @@ Plan plan_for(int rows, int vocab, int hidden, int wformat, int dtype, bool grad
     p.o_stats = take(at, whole / 256 * rows * 8);
     p.o_chosen = take(at, int64_t{4} * rows);
   } else {
-    p.splits = splits_for(hidden, rows, static_cast<int>(piece));
+    p.splits = most_splits(hidden, rows, static_cast<int>(piece));
     p.o_row = take(at, int64_t{4} * p.padded);
     p.o_place = take(at, int64_t{4} * rows);
     p.o_target = take(at, int64_t{8} * p.padded);
@@ -314,7 +315,7 @@ Plan plan_for(int rows, int vocab, int hidden, int wformat, int dtype, bool grad
     p.o_grad = take(at, int64_t{4} * p.padded);
     p.o_back = take(at, 8);
     p.o_p = take(at, rows64 * piece * row16);
-    p.o_sums = take(at, int64_t{4} * p.splits * rows * hidden);
+    p.o_sums = take(at, sums_bytes(hidden, rows, p.splits));
   }
   p.bytes = at;
   return p;
@@ -421,17 +422,17 @@ int backward(const Plan& p, const Call& c, const int64_t* targets, int64_t ignor
     weight_k.rows = p.hidden;
     const TileOperand part{c.workspace + p.o_p, int64_t{2} * rows64 * p.piece, int64_t{2} * p.piece, p.rows, 0};
     product_launch<T, true, false>(weight_k, part, static_cast<int>(round_up(tokens, 64)),
-                                   ProductOut{sums, int64_t{p.rows} * p.hidden, p.hidden, nullptr, first == 0, rows.count}, p.splits, c.stream);
+                                   ProductOut{sums, p.hidden, nullptr, first == 0, p.splits, rows.count}, c.stream);
     if (learned) {   // dW: over the rows, both with them outermost
       TileOperand hidden_k = hidden, part_k = part;
       hidden_k.rows = p.hidden;
       hidden_k.k_rows = part_k.k_rows = rows64;
       part_k.rows = tokens;
       product_launch<T, false, true>(hidden_k, part_k, rows64,
-                                     ProductOut{static_cast<T*>(grad_weight) + static_cast<int64_t>(first) * p.hidden, 0, p.hidden, back, 0, rows.count}, 1, c.stream);
+                                     ProductOut{static_cast<T*>(grad_weight) + static_cast<int64_t>(first) * p.hidden, p.hidden, back, 0, 1, rows.count}, c.stream);
     }
   }
-  add_planes_launch<T>(sums, int64_t{p.rows} * p.hidden, p.splits, back, rows.place, grad_hidden, p.rows, p.hidden, c.stream);
+  add_planes_launch<T>(sums, p.rows, p.hidden, p.splits, rows.count, back, rows.place, grad_hidden, c.stream);
   return llmq_host::check_launch("vocab_loss_grad");
 }
 

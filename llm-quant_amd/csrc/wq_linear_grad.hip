@@ -30,15 +30,15 @@ Plan plan_for(int rows, int N, int width, int dtype) {
   p.piece = kPieceBytes / (width * row16) / 64 * 64;
   if (p.piece < 64) p.piece = 64;
   if (p.piece > p.n_padded) p.piece = p.n_padded;
-  p.splits = splits_for(width, rows, static_cast<int>(p.piece));
+  p.splits = most_splits(width, rows, static_cast<int>(p.piece));
   int64_t at = round_up(p.piece * width * row16, 256);
   if (p.stage_grad) {
     p.o_grad = at;
     at += round_up(rows * p.n_padded * row16, 256);
   }
-  if (p.splits > 1 || p.piece < p.n_padded) {
+  if (splits_of_rows(rows, tile_rows(rows), (width + 255) / 256, width, p.splits).splits > 1 || p.piece < p.n_padded) {
     p.o_sums = at;
-    at += round_up(int64_t{4} * p.splits * rows * width, 256);
+    at += round_up(sums_bytes(width, rows, p.splits), 256);
   }
   p.bytes = at;
   return p;
@@ -67,10 +67,10 @@ int launch(const Plan& p, const void* grad, int64_t stride, const void* qweight,
     const TileOperand a{workspace, 2 * p.piece * width, int64_t{2} * width, width, n};
     const TileOperand b{b_base + int64_t{2} * first, b_plane, b_row, rows, 0};
     const int k = static_cast<int>(round_up(n, 64));
-    if (summed) product_launch<T, true, false>(a, b, k, ProductOut{sums, static_cast<int64_t>(rows) * width, width, nullptr, first == 0}, p.splits, stream);
-    else product_launch<T, false, false>(a, b, k, ProductOut{out, 0, width, nullptr, 1}, 1, stream);
+    if (summed) product_launch<T, true, false>(a, b, k, ProductOut{sums, width, nullptr, first == 0, p.splits}, stream);
+    else product_launch<T, false, false>(a, b, k, ProductOut{out, width, nullptr, 1, 1}, stream);
   }
-  if (summed) add_planes_launch<T>(sums, static_cast<int64_t>(rows) * width, p.splits, nullptr, nullptr, out, rows, width, stream);
+  if (summed) add_planes_launch<T>(sums, rows, width, p.splits, nullptr, nullptr, nullptr, out, stream);
   return llmq_host::check_launch("wq_linear_grad");
 }
 
