@@ -596,7 +596,7 @@ int llmq_kv_block_attention(const void* query, int64_t q_row_stride, const void*
  * keep_per_group], contiguous. N a multiple of 8, rows up to 2^20. fp32 sums; fp32 operands as three bfloat16 planes (2^-24 of a
  * product). Tensors 16-byte aligned. workspace: llmq_wq_linear_grad_workspace_bytes(...) bytes, 16-byte aligned, needs no
  * clearing; calls that overlap in time need one each. */
-size_t llmq_wq_linear_grad_workspace_bytes(int rows, int N, int G, int keep_per_group, int dtype);
+size_t llmq_wq_linear_grad_workspace_bytes(int rows, int N, int G, int keep_per_group, int wformat, int dtype);
 int llmq_wq_linear_grad(const void* grad, int64_t grad_stride, const void* qweight, const float* wscale, void* grad_x,
                         void* workspace, size_t workspace_bytes, int rows, int N, int G, int gs, int keep_per_group,
                         int out_group, int wformat, int dtype, llmq_stream_t stream);
@@ -612,12 +612,12 @@ int llmq_wq_linear_grad(const void* grad, int64_t grad_stride, const void* qweig
  * planes for fp32), with grad scaled by a power of two to at most 2. Gradients are rounded once. hidden_size a multiple of 8, up
  * to 65536; rows up to 2^20, vocab up to 2^24; tensors 16-byte aligned. No rows: nothing is written (grad_weight neither). workspace:
  * ..._workspace_bytes(...) bytes, 16-byte aligned, needs no clearing; calls that overlap in time need one each. */
-size_t llmq_vocab_loss_workspace_bytes(int rows, int vocab, int hidden_size, int wformat, int dtype);
+size_t llmq_vocab_loss_workspace_bytes(int rows, int vocab, int hidden_size, int group_size, int wformat, int dtype);
 int llmq_vocab_loss(const void* hidden, int64_t hidden_stride, const void* weight, const float* wscale_or_null,
                     const int64_t* targets, int64_t ignore_index, float* losses, float* lse, void* workspace,
                     size_t workspace_bytes, int rows, int vocab, int hidden_size, int group_size, int out_group,
                     int wformat, int dtype, llmq_stream_t stream);
-size_t llmq_vocab_loss_grad_workspace_bytes(int rows, int vocab, int hidden_size, int wformat, int dtype, int want_weight);
+size_t llmq_vocab_loss_grad_workspace_bytes(int rows, int vocab, int hidden_size, int group_size, int wformat, int dtype, int want_weight);
 int llmq_vocab_loss_grad(const void* hidden, int64_t hidden_stride, const void* weight, const float* wscale_or_null,
                          const int64_t* targets, int64_t ignore_index, const float* lse, const float* grad, void* grad_hidden,
                          void* grad_weight_or_null, void* workspace, size_t workspace_bytes, int rows, int vocab,

@@ -1,0 +1,377 @@
+// Products of a large weight with few rows, for the vocabulary loss and the gradient of a quantized Linear: the weight, dense or codes, is read
+// once as it lies and is the only thing that counts (bound: HBM). Codes become the values (dtype)(code * scale) in registers, the
+// same ones that dequant_weight writes.
+//
+//   FewRows          D[v, t] = sum_k W[v, k] x[t, k]     the reduction runs along the weight's rows
+//   columns_kernel   D[t, k] = sum_v g[t, v] W[v, k]     the reduction runs over the weight's rows
+//
+// float16 and bfloat16; up to 64 rows a pass over the weight.
+#pragma once
+
+#include "dense_tile.h"
+
+namespace llmq {
+
+struct FewWeight {
+  const uint8_t* base;   // rows of `row_bytes`
+  const float* scale;    // of codes: [scale rows, groups]
+  int64_t row_bytes;
+  int rows, width;       // width: columns, `keep` of each group
+  int groups, group_size, keep, out_group;
+  __device__ __forceinline__ int64_t scale_row(int row) const { return static_cast<int64_t>(out_group > 0 ? row / out_group : row) * groups; }
+};
+
+// eight codes with their scale, as two halves of words: word i of the result holds values 2 i and 2 i + 1
+template <typename T> __device__ __forceinline__ uint32_t pair_of(float lo, float hi);
+template <> __device__ __forceinline__ uint32_t pair_of<bf16_t>(float lo, float hi) { return bf16_pair_rne(lo, hi); }
+template <> __device__ __forceinline__ uint32_t pair_of<f16_t>(float lo, float hi) {
+  return static_cast<uint32_t>(__builtin_bit_cast(uint16_t, f16_rne(lo))) | static_cast<uint32_t>(__builtin_bit_cast(uint16_t, f16_rne(hi))) << 16;
+}
+// Eight codes, times the scale as 32 bits, as pairs. BITS 8: two words; 4: one word of code + 8, each brought to the upper half of a byte as
+// 16 code, against a sixteenth of the scale (exact down to 2^-122). float(int8) of a byte is one instruction.
+template <int BITS> struct Codes {
+  uint32_t w[2];
+  __device__ __forceinline__ explicit Codes(const uint32_t* v) {
+    if constexpr (BITS == 8) {
+      w[0] = v[0];
+      w[1] = v[1];
+    } else {
+      const uint32_t c = v[0] ^ 0x88888888u;
+      w[0] = c << 4 & 0xf0f0f0f0u;
+      w[1] = c & 0xf0f0f0f0u;
+    }
+  }
+  static __device__ __forceinline__ float scale_of(float scale) { return BITS == 8 ? scale : scale * 0.0625f; }
+  static __device__ __forceinline__ float at(const uint32_t* w, int i) {
+    return static_cast<float>(static_cast<int8_t>(BITS == 8 ? w[i / 4] >> (8 * (i % 4)) : w[i % 2] >> (8 * (i / 2))));
+  }
+};
+
+// ---- x in operand order -------------------------------------------------------------------------------------------------------
+// [k / 32][tile of 16 rows][lane][8 values]: lane 16 g + r holds values 32 k + 8 g .. of row 16 tile + r; zeros past the rows and past `gather`.
+template <typename T>
+__global__ __launch_bounds__(256) void few_operand_kernel(const T* __restrict__ x, const int64_t stride, const int32_t* __restrict__ gather,
+                                                          const int rows, const int k, const int tiles, T* __restrict__ out) {
+  const int64_t items = static_cast<int64_t>(k / 32) * tiles * kWave, item = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  if (item >= items) return;
+  const int lane = item % kWave, tile = static_cast<int>(item / kWave % tiles), at = static_cast<int>(item / kWave / tiles);
+  const int t = tile * 16 + (lane & 15);
+  const int row = t >= rows ? -1 : gather != nullptr ? gather[t] : t;
+  u32x4 v{0, 0, 0, 0};
+  if (row >= 0) v = load16(x + row * stride + at * 32 + 8 * (lane >> 4));
+  store16(out + item * 8, v);
+}
+
+// ---- the reduction along the weight's rows ----------------------------------------------------------------------------------------
+constexpr int kFewTokens = 64, kFewWaves = 4;   // rows of the weight a workgroup; waves
+
+// The waves of a workgroup take steps of its 64 rows by turns: 128 bytes of each row (int4: 64) through LDS of the wave's own, in whole lines, two
+// steps in flight, no barrier until the sums meet. RowsStep::operand: eight values of a row, from LDS.
+template <typename T, int BITS> struct RowsStep {
+  static constexpr int kK = BITS == 0 ? 64 : 128, kRowBytes = BITS == 4 ? 64 : 128, kSlots = kRowBytes / 16, kRowsPerLoad = 64 / kSlots;
+  static constexpr int kBytes = kFewTokens * kRowBytes, kLoads = kBytes / 1024;
+  // the chunk of 16 bytes that slot p of row r holds (its own inverse): reads of 16 rows meet every bank as often
+  static __device__ __forceinline__ int chunk(int r, int p) {
+    if constexpr (BITS == 0) return p ^ (r & 7);
+    else if constexpr (BITS == 8) return p ^ ((r >> 1 & 3) << 1);
+    else return p ^ (r >> 2 & 3);
+  }
+  // values 32 c + 8 g .. of row r
+  static __device__ __forceinline__ u32x4 operand(const uint8_t* stage, int r, int c, int g, float scale) {
+    if constexpr (BITS == 0) {
+      return load16(stage + r * kRowBytes + (chunk(r, 4 * c + g) << 4));
+    } else {
+      uint32_t w[2];
+      if constexpr (BITS == 8) {
+        const u32x2 v = *reinterpret_cast<const u32x2*>(stage + r * kRowBytes + (chunk(r, 2 * c + (g >> 1)) << 4) + (g & 1) * 8);
+        w[0] = v.x;
+        w[1] = v.y;
+      } else {
+        w[0] = *reinterpret_cast<const uint32_t*>(stage + r * kRowBytes + (chunk(r, c) << 4) + g * 4);
+      }
+      const Codes<BITS> codes(w);
+      const float by = Codes<BITS>::scale_of(scale);
+      float f[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) f[i] = Codes<BITS>::at(codes.w, i) * by;
+      return u32x4{pair_of<T>(f[0], f[1]), pair_of<T>(f[2], f[3]), pair_of<T>(f[4], f[5]), pair_of<T>(f[6], f[7])};
+    }
+  }
+};
+
+// acc[i]: rows 16 i + 4 g .. + 3 of the workgroup's, of row 16 j + r of x, where the wave is j's (j = wave, while there are so many)
+template <typename T, int BITS, int NT> struct FewRows {
+  using Step = RowsStep<T, BITS>;
+  static constexpr int kTiles = kFewTokens / 16, kSums = kFewWaves * kTiles * NT * 1024, kStages = kFewWaves * 2 * Step::kBytes;
+  static constexpr int kLdsBytes = kSums > kStages ? kSums : kStages;
+  tile_v4f acc[kTiles];
+
+  struct Asked {
+    u32x4 x[Step::kK / 32][NT];
+    float scale[BITS ? kTiles : 1];
+  };
+  __device__ __forceinline__ void multiply(uint8_t* lds, const FewWeight& w, int m0, const T* x) {
+    const int lane = threadIdx.x & (kWave - 1), wv = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) / kWave), lr = lane & 15, g = lane >> 4;
+    const int steps = w.width / Step::kK;
+    uint8_t* const mine = lds + wv * 2 * Step::kBytes;
+    const BufferBase base = buffer_base(w.base + m0 * w.row_bytes);
+    uint32_t off[Step::kLoads];
+#pragma unroll
+    for (int i = 0; i < Step::kLoads; ++i) {
+      const int r = i * Step::kRowsPerLoad + lane / Step::kSlots;
+      off[i] = static_cast<uint32_t>((min(m0 + r, w.rows - 1) - m0) * w.row_bytes) + (Step::chunk(r, lane % Step::kSlots) << 4);
+    }
+    const float* scale[kTiles];
+    if constexpr (BITS != 0) {
+#pragma unroll
+      for (int i = 0; i < kTiles; ++i) scale[i] = w.scale + w.scale_row(min(m0 + i * 16 + lr, w.rows - 1));
+    }
+    tile_v4f sum[kTiles][NT] = {};
+    const auto ask = [&](int at, int buf, Asked& a) {   // (the transfers last: what is waited for below leaves them in flight)
+#pragma unroll
+      for (int c = 0; c < Step::kK / 32; ++c)
+#pragma unroll
+        for (int j = 0; j < NT; ++j) a.x[c][j] = load16(x + ((static_cast<int64_t>(at) * (Step::kK / 32) + c) * NT + j) * kWave * 8 + lane * 8);
+      if constexpr (BITS != 0) {
+#pragma unroll
+        for (int i = 0; i < kTiles; ++i) a.scale[i] = scale[i][at * Step::kK / w.group_size];
+      }
+#pragma unroll
+      for (int i = 0; i < Step::kLoads; ++i) buffer_to_lds<16>(base, mine + buf * Step::kBytes + i * 1024, off[i], at * Step::kRowBytes);
+    };
+    // the transfers of all steps but the newest have arrived
+    const auto arrived = [&](bool newer) {
+      if (newer) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(Step::kLoads) : "memory");
+      else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    };
+    const auto use = [&](int buf, const Asked& a) {
+      const uint8_t* stage = mine + buf * Step::kBytes;
+#pragma unroll
+      for (int c = 0; c < Step::kK / 32; ++c)
+#pragma unroll
+        for (int i = 0; i < kTiles; ++i) {
+          const u32x4 v = Step::operand(stage, i * 16 + lr, c, g, a.scale[BITS ? i : 0]);
+#pragma unroll
+          for (int j = 0; j < NT; ++j) sum[i][j] = mfma_16x16x32<T>(v, a.x[c][j], sum[i][j]);
+        }
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // (the stage is asked for again)
+    };
+    Asked a, b;
+    a.scale[0] = b.scale[0] = 1.0f;
+    if (wv < steps) {
+      ask(wv, 0, a);
+      for (int s = wv; s < steps; s += 2 * kFewWaves) {
+        const bool second = s + kFewWaves < steps, third = s + 2 * kFewWaves < steps;
+        if (second) ask(s + kFewWaves, 1, b);
+        arrived(second);
+        use(0, a);
+        if (!second) break;
+        if (third) ask(s + 2 * kFewWaves, 0, a);
+        arrived(third);
+        use(1, b);
+      }
+    }
+    __syncthreads();
+    tile_v4f* const s_sum = reinterpret_cast<tile_v4f*>(lds);   // [wave][tile][row tile][lane]
+#pragma unroll
+    for (int i = 0; i < kTiles; ++i)
+#pragma unroll
+      for (int j = 0; j < NT; ++j) s_sum[((wv * kTiles + i) * NT + j) * kWave + lane] = sum[i][j];
+    __syncthreads();
+    const int j = min(wv, NT - 1);
+#pragma unroll
+    for (int i = 0; i < kTiles; ++i) {
+      acc[i] = s_sum[(i * NT + j) * kWave + lane];
+#pragma unroll
+      for (int v = 1; v < kFewWaves; ++v) acc[i] += s_sum[((v * kTiles + i) * NT + j) * kWave + lane];
+    }
+  }
+};
+
+// ---- the reduction over the weight's rows -----------------------------------------------------------------------------------------
+constexpr int kFewColumns = 128;   // of a wave
+
+struct FewColumns {
+  const void* g;         // [rows, stride] of T: values of the weight's rows, in whole packets
+  int64_t stride;
+  const int32_t* count;  // or null: how many of the rows there are
+  int rows;
+  float* planes;         // [splits][rows][width]
+  int splits;
+};
+
+// A workgroup: 128 columns, 16 NT rows of g (blockIdx.y), a part of the weight's rows, which its waves take 32 at a time; each lane
+// eight columns of eight rows, turned over in registers, a step ahead. The waves' sums meet in LDS.
+template <typename T, int BITS, int NT>
+__global__ __launch_bounds__(kFewWaves * kWave) void columns_kernel(const FewWeight w, const FewColumns c) {
+  constexpr int kWords = BITS == 0 ? 4 : BITS / 4;   // of eight values
+  __shared__ tile_v4f s_sum[2][NT * 8][kWave];
+  const int t0 = blockIdx.y * 16 * NT, rows = c.count != nullptr ? min(*c.count, c.rows) : c.rows;
+  if (t0 >= rows) return;
+  const int lane = threadIdx.x & (kWave - 1), wv = threadIdx.x / kWave, lr = lane & 15, g = lane >> 4;
+  const int steps = (w.rows + 31) / 32, per = (steps + c.splits - 1) / c.splits;
+  const int parts = (w.width + kFewColumns - 1) / kFewColumns, item = tile_of_workgroup(blockIdx.x, gridDim.x), split = item / parts;
+  const int v0 = min(split * per, steps) * 32, v1 = min((split + 1) * per, steps) * 32;
+  const int col = item % parts * kFewColumns + 8 * lr, at = min(col, w.width - 8);
+  const int group = BITS ? at / w.keep : 0;
+  const int64_t byte = BITS == 0 ? at * 2 : (static_cast<int64_t>(group) * w.group_size + (at - group * w.keep)) * BITS / 8;
+  const T* gr[NT];
+#pragma unroll
+  for (int j = 0; j < NT; ++j) gr[j] = static_cast<const T*>(c.g) + min(t0 + j * 16 + lr, rows - 1) * c.stride;
+  struct Asked {
+    uint32_t w[8][kWords];
+    float scale[BITS ? 8 : 1];
+    u32x4 g[NT];
+  };
+  const auto ask = [&](int v, Asked& a) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const int row = min(v + 8 * g + e, w.rows - 1);
+      const uint8_t* from = w.base + row * w.row_bytes + byte;
+      if constexpr (BITS == 0) {
+        const u32x4 q = load16(from);
+        a.w[e][0] = q.x; a.w[e][1] = q.y; a.w[e][2] = q.z; a.w[e][3] = q.w;
+      } else if constexpr (BITS == 8) {
+        const u32x2 q = *reinterpret_cast<const u32x2*>(from);
+        a.w[e][0] = q.x; a.w[e][1] = q.y;
+      } else {
+        a.w[e][0] = *reinterpret_cast<const uint32_t*>(from);
+      }
+      if constexpr (BITS != 0) a.scale[e] = w.scale[w.scale_row(row) + group];
+    }
+#pragma unroll
+    for (int j = 0; j < NT; ++j) a.g[j] = load16(gr[j] + min(v + 8 * g, (w.rows - 1) / 8 * 8));
+  };
+  tile_v4f acc[NT][8] = {};
+  const int begin = v0 + wv * 32, step = 32 * kFewWaves;
+  const auto use = [&](int v, Asked& now) {
+    if (v + 8 * g >= w.rows) {   // the weight's last row again, against zeros
+#pragma unroll
+      for (int j = 0; j < NT; ++j) now.g[j] = u32x4{0, 0, 0, 0};
+    }
+    float by[BITS ? 8 : 1];
+    uint32_t bytes[8][BITS ? 2 : 4];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      if constexpr (BITS != 0) {
+        const Codes<BITS> codes(now.w[e]);
+        bytes[e][0] = codes.w[0];
+        bytes[e][1] = codes.w[1];
+        by[e] = Codes<BITS>::scale_of(now.scale[e]);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) bytes[e][i] = now.w[e][i];
+      }
+    }
+#pragma unroll
+    for (int q = 0; q < 8; ++q) {   // column q of the lane's eight
+      uint32_t word[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const uint32_t *lo = bytes[2 * e], *hi = bytes[2 * e + 1];
+        if constexpr (BITS == 0) word[e] = __builtin_amdgcn_perm(hi[q / 2], lo[q / 2], q % 2 ? 0x07060302u : 0x05040100u);
+        else word[e] = pair_of<T>(Codes<BITS>::at(lo, q) * by[2 * e], Codes<BITS>::at(hi, q) * by[2 * e + 1]);
+      }
+      const u32x4 operand{word[0], word[1], word[2], word[3]};
+#pragma unroll
+      for (int j = 0; j < NT; ++j) acc[j][q] = mfma_16x16x32<T>(now.g[j], operand, acc[j][q]);
+    }
+  };
+  if (begin < v1) {
+    Asked next;
+    ask(begin, next);
+    for (int v = begin; v < v1; v += step) {
+      Asked now = next;
+      ask(min(v + step, v1 - 32), next);   // (behind the last step: the part's last again)
+      use(v, now);
+    }
+  }
+  if (wv >= 2) {
+#pragma unroll
+    for (int i = 0; i < NT * 8; ++i) s_sum[wv - 2][i][lane] = acc[i / 8][i % 8];
+  }
+  __syncthreads();
+  if (wv < 2) {
+#pragma unroll
+    for (int i = 0; i < NT * 8; ++i) acc[i / 8][i % 8] += s_sum[wv][i][lane];
+  }
+  __syncthreads();
+  if (wv == 1) {
+#pragma unroll
+    for (int i = 0; i < NT * 8; ++i) s_sum[0][i][lane] = acc[i / 8][i % 8];
+  }
+  __syncthreads();
+  if (wv != 0 || col >= w.width) return;
+#pragma unroll
+  for (int j = 0; j < NT; ++j)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {   // row 4 g + i, eight neighbouring columns
+      const int t = t0 + j * 16 + 4 * g + i;
+      if (t >= rows) continue;
+      float* to = c.planes + (static_cast<int64_t>(split) * c.rows + t) * w.width + col;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        tile_v4f v;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = acc[j][h * 4 + e][i] + s_sum[0][j * 8 + h * 4 + e][lane][i];
+        *reinterpret_cast<tile_v4f*>(to + 4 * h) = v;
+      }
+    }
+}
+// Splits of the weight's rows, 64 at the most. For 256 workgroups: more are only more planes (4096 x 4096 int8, 64 rows: 17 us with 256, 26 with 512, 39
+// with 1024; 16 rows: 9, 11 and 13), but for 512 where conversion binds and a wave still has 32 steps (128256 x 2048, 16 rows: int8 66 -> 56, int4 58 -> 48; as
+// they are 88 -> 93).
+inline int few_splits(int weight_rows, int width, int rows, int bits) {
+  const int64_t groups = static_cast<int64_t>((width + kFewColumns - 1) / kFewColumns) * ((rows + 63) / 64), step = 32 * kFewWaves;
+  const int64_t most = (weight_rows + step - 1) / step;
+  int64_t splits = 256 / groups;
+  if (bits != 0 && rows <= 32 && most >= 512 / groups * 32) splits = 512 / groups;
+  if (splits > most) splits = most;
+  return static_cast<int>(splits < 1 ? 1 : splits > 64 ? 64 : splits);
+}
+template <typename T, int BITS> inline void columns_launch_bits(const FewWeight& w, const FewColumns& c, hipStream_t stream) {
+  const unsigned x = (w.width + kFewColumns - 1) / kFewColumns * c.splits;
+  if (c.rows <= 16) hipLaunchKernelGGL((columns_kernel<T, BITS, 1>), dim3(x), dim3(kFewWaves * kWave), 0, stream, w, c);
+  else if (c.rows <= 32) hipLaunchKernelGGL((columns_kernel<T, BITS, 2>), dim3(x), dim3(kFewWaves * kWave), 0, stream, w, c);
+  else hipLaunchKernelGGL((columns_kernel<T, BITS, 4>), dim3(x, (c.rows + 63) / 64), dim3(kFewWaves * kWave), 0, stream, w, c);
+}
+template <typename T> inline void columns_launch(const FewWeight& w, const FewColumns& c, int bits, hipStream_t stream) {
+  if (bits == 0) columns_launch_bits<T, 0>(w, c, stream);
+  else if (bits == 8) columns_launch_bits<T, 8>(w, c, stream);
+  else columns_launch_bits<T, 4>(w, c, stream);
+}
+
+// out[row] = (dtype)(scale * the sum of the planes' row `from[row]`); no such row (negative): zeros
+template <typename T>
+__global__ __launch_bounds__(256) void add_few_kernel(const float* __restrict__ planes, const int splits, const int rows, const int width,
+                                                      const float* __restrict__ scale_or_null, const int32_t* __restrict__ from_or_null, T* __restrict__ out) {
+  constexpr int kAhead = 8;
+  const int64_t item = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x, items = static_cast<int64_t>(rows) * (width / 4);
+  if (item >= items) return;
+  const int row = static_cast<int>(item / (width / 4)), c = static_cast<int>(item % (width / 4)) * 4;
+  const int from = from_or_null != nullptr ? from_or_null[row] : row;
+  tile_v4f sum{0.0f, 0.0f, 0.0f, 0.0f};
+  if (from >= 0) {
+    const float* at = planes + static_cast<int64_t>(from) * width + c;
+    const int64_t plane = static_cast<int64_t>(rows) * width;
+    for (int z0 = 0; z0 < splits; z0 += kAhead) {
+      tile_v4f v[kAhead];
+#pragma unroll
+      for (int z = 0; z < kAhead; ++z) v[z] = *reinterpret_cast<const tile_v4f*>(at + min(z0 + z, splits - 1) * plane);
+#pragma unroll
+      for (int z = 0; z < kAhead; ++z)
+        if (z0 + z < splits) sum += v[z];
+    }
+  }
+  const float scale = scale_or_null != nullptr ? *scale_or_null : 1.0f;
+  const u32x2 v{pair_of<T>(sum[0] * scale, sum[1] * scale), pair_of<T>(sum[2] * scale, sum[3] * scale)};
+  *reinterpret_cast<u32x2*>(out + static_cast<int64_t>(row) * width + c) = v;
+}
+template <typename T>
+inline void add_few_launch(const float* planes, int splits, int rows, int width, const float* scale, const int32_t* from, void* out, hipStream_t stream) {
+  const int64_t items = static_cast<int64_t>(rows) * (width / 4);
+  hipLaunchKernelGGL((add_few_kernel<T>), dim3(static_cast<unsigned>((items + 255) / 256)), dim3(256), 0, stream, planes, splits, rows, width, scale, from,
+                     static_cast<T*>(out));
+}
+
+}  // namespace llmq

@@ -1823,7 +1823,7 @@ at::Tensor wq_linear_grad(const at::Tensor& grad, const at::Tensor& qweight, con
   const c10::OptionalDeviceGuard guard(at::device_of(grad));
   const auto gr = own_rows(grad);
   const size_t need = llmq_wq_linear_grad_workspace_bytes(static_cast<int>(rows), static_cast<int>(w.rows), static_cast<int>(w.groups),
-                                                          static_cast<int>(keep_per_group), dtype);
+                                                          static_cast<int>(keep_per_group), w.format, dtype);
   const auto workspace = at::empty({static_cast<int64_t>(need)}, grad.options().dtype(at::kByte));
   check_rc(llmq_wq_linear_grad(gr.const_data_ptr(), own_stride(gr), qweight.const_data_ptr(), wscale.const_data_ptr<float>(),
                                out.mutable_data_ptr(), workspace.mutable_data_ptr(), need, static_cast<int>(rows),
@@ -1880,7 +1880,7 @@ std::tuple<at::Tensor, at::Tensor> vocab_loss(const at::Tensor& hidden, const at
   const auto wt = packet_rows(weight.reshape({1, weight.numel()}));
   const auto tr = targets.contiguous();
   const size_t need = llmq_vocab_loss_workspace_bytes(static_cast<int>(rows), static_cast<int>(v.tokens), static_cast<int>(hidden.size(1)),
-                                                      v.format, dtype);
+                                                      static_cast<int>(v.group_size), v.format, dtype);
   const auto workspace = at::empty({static_cast<int64_t>(need)}, hidden.options().dtype(at::kByte));
   check_rc(llmq_vocab_loss(hr.const_data_ptr(), own_stride(hr), wt.const_data_ptr(), v.scale, tr.const_data_ptr<int64_t>(), ignore_index,
                            losses.mutable_data_ptr<float>(), lse.mutable_data_ptr<float>(), workspace.mutable_data_ptr(), need,
@@ -1908,7 +1908,7 @@ std::tuple<at::Tensor, c10::optional<at::Tensor>> vocab_loss_grad(const at::Tens
   const auto wt = packet_rows(weight.reshape({1, weight.numel()}));
   const auto tr = targets.contiguous();
   const size_t need = llmq_vocab_loss_grad_workspace_bytes(static_cast<int>(rows), static_cast<int>(v.tokens), static_cast<int>(hidden.size(1)),
-                                                           v.format, dtype, want_weight);
+                                                           static_cast<int>(v.group_size), v.format, dtype, want_weight);
   const auto workspace = at::empty({static_cast<int64_t>(need)}, hidden.options().dtype(at::kByte));
   check_rc(llmq_vocab_loss_grad(hr.const_data_ptr(), own_stride(hr), wt.const_data_ptr(), v.scale, tr.const_data_ptr<int64_t>(), ignore_index,
                                 ls.const_data_ptr<float>(), gr.const_data_ptr<float>(), grad_hidden.mutable_data_ptr(),

@@ -10,7 +10,9 @@
 // The gradient goes over pieces of the vocabulary: the tile is multiplied again, and what is written is P of the piece in the type of the
 // call (fp32: three planes), as the operand of the two products behind it. P is rounded to that type, relative to each value; g is scaled
 // by a power of two first, so that a mean over many rows does not leave fp16's range, and the results are scaled back.
-// A quantized head (the model's lm_head) is brought to the values of its dense form piece by piece.
+// A quantized head (the model's lm_head) is brought to the values of its dense form piece by piece. Up to 64 rows of 16 bits go past the weight
+// as it lies instead, dense or codes (dense_few.h; 16 rows of 128256 x 2048, bf16: the tiles' kernel 115 us, this one 87, 6.0 TB/s).
+#include "dense_few.h"
 #include "dense_stage.h"
 
 namespace {
@@ -94,39 +96,84 @@ __global__ __launch_bounds__(WM * WN * kWave) void logits_kernel(const TileOpera
   }
 }
 
-// 16 rows a workgroup, the tiles dealt to 16 threads each, merged in a fixed order.
-__global__ __launch_bounds__(256) void loss_kernel(const float2* __restrict__ stats, const float* __restrict__ chosen, const int tiles,
-                                                   const LossRows rows, const int64_t ignore_index, float* __restrict__ losses,
-                                                   float* __restrict__ lse) {
-  __shared__ float2 s_part[16][17];
-  const int at = threadIdx.x % 16, part = threadIdx.x / 16, n = blockIdx.x * 16 + at;
-  const bool active = n < rows.rows;
-  float top = -INFINITY, sum = 0.0f;
-  if (active) {
-    for (int i = part; i < tiles; i += 16) {
-      const float2 s = stats[static_cast<int64_t>(i) * rows.rows + n];
-      const float next = fmaxf(top, s.x), from = next == -INFINITY ? 0.0f : next;
-      sum = sum * __builtin_amdgcn_exp2f(((top == -INFINITY ? from : top) - from) * kLog2e) +
-            s.y * __builtin_amdgcn_exp2f(((s.x == -INFINITY ? from : s.x) - from) * kLog2e);
-      top = next;
-    }
+__device__ __forceinline__ float2 merged(float2 a, float2 b) {   // (largest, sum of exponentials over it)
+  const float top = fmaxf(a.x, b.x), from = top == -INFINITY ? 0.0f : top;
+  return make_float2(top, a.y * __builtin_amdgcn_exp2f(((a.x == -INFINITY ? from : a.x) - from) * kLog2e) +
+                              b.y * __builtin_amdgcn_exp2f(((b.x == -INFINITY ? from : b.x) - from) * kLog2e));
+}
+// R rows a workgroup, the tiles dealt to 1024 / R threads each, eight in flight, merged in a fixed order. R = 4 where 16 would leave a workgroup or
+// a few on the way (16 rows, 2004 tiles: 9.4 us with 16).
+template <int R>
+__global__ __launch_bounds__(1024) void loss_kernel(const float2* __restrict__ stats, const float* __restrict__ chosen, const int tiles,
+                                                               const LossRows rows, const int64_t ignore_index, float* __restrict__ losses,
+                                                               float* __restrict__ lse) {
+  constexpr int kAhead = 8, kLossParts = 1024 / R;
+  __shared__ float2 s_part[kLossParts][R + 1];
+  const int at = threadIdx.x % R, part = threadIdx.x / R, n = blockIdx.x * R + at;
+  const int row = min(n, rows.rows - 1);
+  float2 all = make_float2(-INFINITY, 0.0f);
+  for (int i0 = part; i0 < tiles; i0 += kAhead * kLossParts) {
+    float2 v[kAhead];
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) v[i] = stats[static_cast<int64_t>(min(i0 + i * kLossParts, tiles - 1)) * rows.rows + row];
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i)
+      if (i0 + i * kLossParts < tiles) all = merged(all, v[i]);
   }
-  s_part[part][at] = make_float2(top, sum);
+  s_part[part][at] = all;
   __syncthreads();
-  if (part != 0 || !active) return;
-  top = -INFINITY;
-  for (int p = 0; p < 16; ++p) top = fmaxf(top, s_part[p][at].x);
-  const float from = top == -INFINITY ? 0.0f : top;
-  sum = 0.0f;
-  for (int p = 0; p < 16; ++p) {
-    const float2 s = s_part[p][at];
-    sum += s.y * __builtin_amdgcn_exp2f(((s.x == -INFINITY ? from : s.x) - from) * kLog2e);
+  for (int half = kLossParts / 2; half > 0; half /= 2) {
+    if (part < half) s_part[part][at] = merged(s_part[part][at], s_part[part + half][at]);
+    __syncthreads();
   }
-  const float rest = logf(sum);
-  lse[n] = top + rest;
+  if (part != 0 || n >= rows.rows) return;
+  all = s_part[0][at];
+  const float rest = logf(all.y);
+  lse[n] = all.x + rest;
   const int64_t target = rows.targets[n];
   losses[n] = target == ignore_index ? 0.0f
-              : target < 0 || target >= rows.vocab ? NAN : rest + (top - chosen[n]);
+              : target < 0 || target >= rows.vocab ? NAN : rest + (all.x - chosen[n]);
+}
+
+// A few rows: 64 tokens a workgroup, a row tile of the sums a wave.
+template <typename T, int BITS, int NT>
+__global__ __launch_bounds__(kFewWaves * kWave) void few_logits_kernel(const FewWeight weight, const T* __restrict__ x, const LossRows rows,
+                                                                       float2* __restrict__ stats, float* __restrict__ chosen) {
+  using Few = FewRows<T, BITS, NT>;
+  __shared__ __attribute__((aligned(16))) uint8_t s_mem[Few::kLdsBytes];
+  const int m0 = blockIdx.x * kFewTokens;
+  Few f;
+  f.multiply(s_mem, weight, m0, x);
+  const int lane = threadIdx.x & (kWave - 1), wv = threadIdx.x / kWave, n = wv * 16 + (lane & 15), v0 = 4 * (lane >> 4);
+  if (wv >= NT) return;
+  float top = -INFINITY;
+#pragma unroll
+  for (int i = 0; i < Few::kTiles; ++i)
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      if (m0 + i * 16 + v0 + q >= weight.rows) f.acc[i][q] = -INFINITY;
+      top = fmaxf(top, f.acc[i][q]);
+    }
+  top = fmaxf(top, __shfl_xor(top, 16));
+  top = fmaxf(top, __shfl_xor(top, 32));
+  const float from = top == -INFINITY ? 0.0f : top;
+  float sum = 0.0f;
+#pragma unroll
+  for (int i = 0; i < Few::kTiles; ++i)
+#pragma unroll
+    for (int q = 0; q < 4; ++q) sum += __builtin_amdgcn_exp2f((f.acc[i][q] - from) * kLog2e);
+  sum += __shfl_xor(sum, 16);
+  sum += __shfl_xor(sum, 32);
+  if (n >= rows.rows) return;
+  if ((lane >> 4) == 0) stats[static_cast<int64_t>(blockIdx.x) * rows.rows + n] = make_float2(top, sum);
+  const int64_t at = rows.targets[n] - m0;
+  if (at >= 0 && at < kFewTokens && m0 + at < rows.vocab) {
+#pragma unroll
+    for (int i = 0; i < Few::kTiles; ++i)
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        if (i * 16 + v0 + q == at) chosen[n] = f.acc[i][q];
+  }
 }
 
 // ---- the gradient -----------------------------------------------------------------------------------------------------------
@@ -252,6 +299,32 @@ __global__ __launch_bounds__(WM * WN * kWave) void piece_kernel(const TileOperan
   }
 }
 
+// P of a few rows: [16 NT, ld], zeros for tokens past the vocabulary up to a multiple of 64
+template <typename T, int BITS, int NT>
+__global__ __launch_bounds__(kFewWaves * kWave) void few_piece_kernel(const FewWeight weight, const T* __restrict__ x, const Counted rows,
+                                                                      T* __restrict__ p, const int64_t ld) {
+  using Few = FewRows<T, BITS, NT>;
+  __shared__ __attribute__((aligned(16))) uint8_t s_mem[Few::kLdsBytes];
+  const int m0 = blockIdx.x * kFewTokens;
+  Few f;
+  f.multiply(s_mem, weight, m0, x);
+  const int lane = threadIdx.x & (kWave - 1), wv = threadIdx.x / kWave, n = wv * 16 + (lane & 15), v0 = 4 * (lane >> 4);
+  if (wv >= NT) return;
+  const float g = rows.grad[n], lse = rows.lse[n];
+  const int64_t target = rows.target[n] - m0;
+#pragma unroll
+  for (int i = 0; i < Few::kTiles; ++i) {
+    float e[4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const int m = i * 16 + v0 + q;
+      const float value = __builtin_amdgcn_exp2f((f.acc[i][q] - lse) * kLog2e) - (target == m ? 1.0f : 0.0f);
+      e[q] = g == 0.0f || m0 + m >= weight.rows ? 0.0f : value * g;
+    }
+    *reinterpret_cast<u32x2*>(p + n * ld + m0 + i * 16 + v0) = u32x2{pair_of<T>(e[0], e[1]), pair_of<T>(e[2], e[3])};
+  }
+}
+
 // ---- what a call takes --------------------------------------------------------------------------------------------------------
 struct Plan {
   int rows, vocab, hidden, planes, size;   // size: bytes of an element of the call's type
@@ -260,8 +333,10 @@ struct Plan {
   bool stage_hidden, stage_weight;         // whether they have to be brought into operand form
   int piece;                               // tokens of a piece, a multiple of 256
   int splits;                              // of dh's products
+  bool few;                                // rows that go past the weight once, as it lies
+  int row_tiles;                           // of 16, for these: 1, 2 or 4
   // offsets into the workspace
-  int64_t o_stats, o_chosen, o_hidden, o_weight, o_row, o_place, o_target, o_lse, o_grad, o_back, o_p, o_sums, bytes;
+  int64_t o_stats, o_chosen, o_hidden, o_weight, o_row, o_place, o_target, o_lse, o_grad, o_back, o_x, o_p, o_sums, bytes;
 };
 
 int64_t take(int64_t& at, int64_t bytes) {
@@ -270,11 +345,15 @@ int64_t take(int64_t& at, int64_t bytes) {
   return here;
 }
 
-// The piece of the vocabulary: a whole number of rounds of 256 workgroups' tiles, as many as the workspace for pieces has room for: how many
-// rows count is not known when a call is made, and in several rounds the tiles of those that do not leave room for others.
-constexpr int64_t kPieceBytes = int64_t{768} << 20;
+// The piece of the vocabulary: a whole number of rounds of 256 workgroups' tiles, in as much workspace. The loss's pieces stay in the caches (whole: 2047
+// rows of a 128256 x 2048 int8 head 1022 us for the tiles, in pieces of up to 192 MB 963, of 68 MB 960 and the codes' pass 168 instead of 133; 1024
+// rows of x 4096 967 and 812). The gradient's are several rounds: how many rows count is not known when a call is made, and there the tiles of those
+// that do not leave room for others (724 of 1024: 1726 us for all products with 768 MB, 1916 with 500, 1932 with 136).
+constexpr int64_t kLossPieceBytes = int64_t{192} << 20, kGradPieceBytes = int64_t{768} << 20;
+// few rows: the whole vocabulary at once, where their P takes no more than 128 MB
+constexpr int kFewVocab = 1 << 20;
 
-Plan plan_for(int rows, int vocab, int hidden, int wformat, int dtype, bool gradient, bool learned) {
+Plan plan_for(int rows, int vocab, int hidden, int group_size, int wformat, int dtype, bool gradient, bool learned) {
   Plan p{};
   p.rows = rows;
   p.vocab = vocab;
@@ -294,13 +373,42 @@ Plan plan_for(int rows, int vocab, int hidden, int wformat, int dtype, bool grad
   int64_t piece = whole;
   if (per_token > 0) {
     const int64_t n_tiles = p.padded / tn, round = n_tiles >= 256 ? 256 : 256 / n_tiles * 256;   // tokens of a round of workgroups
-    piece = kPieceBytes / per_token / 256 * 256;
+    piece = (gradient ? kGradPieceBytes : kLossPieceBytes) / per_token / 256 * 256;
     if (piece > round) piece = piece / round * round;
     if (piece < 256) piece = 256;
     if (piece > whole) piece = whole;
   }
   p.piece = static_cast<int>(piece);
   int64_t at = 0;
+  p.few = rows <= kFewRows && vocab <= kFewVocab && p.planes == 1 && hidden % (wformat ? 128 : 64) == 0 && (wformat == 0 || group_size % 128 == 0);
+  if (p.few) {
+    p.row_tiles = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
+    p.stage_hidden = learned;
+    p.stage_weight = false;
+    p.piece = static_cast<int>(round_up(vocab, kFewTokens));
+    p.o_x = take(at, int64_t{2} * hidden * 16 * p.row_tiles);
+    if (p.stage_hidden) p.o_hidden = take(at, rows64 * p.k * row16);
+    if (!gradient) {
+      p.o_stats = take(at, round_up(vocab, kFewTokens) / kFewTokens * rows * 8);
+      p.o_chosen = take(at, int64_t{4} * rows);
+    } else {
+      p.splits = few_splits(vocab, hidden, rows, wformat);
+      p.o_p = take(at, int64_t{2} * 16 * p.row_tiles * p.piece);
+      p.o_sums = take(at, int64_t{4} * p.splits * rows * hidden);
+    }
+  }
+  if (gradient) {
+    p.o_row = take(at, int64_t{4} * p.padded);
+    p.o_place = take(at, int64_t{4} * rows);
+    p.o_target = take(at, int64_t{8} * p.padded);
+    p.o_lse = take(at, int64_t{4} * p.padded);
+    p.o_grad = take(at, int64_t{4} * p.padded);
+    p.o_back = take(at, 8);
+  }
+  if (p.few) {
+    p.bytes = at;
+    return p;
+  }
   if (p.stage_hidden) p.o_hidden = take(at, rows64 * p.k * row16);
   if (p.stage_weight) p.o_weight = take(at, piece * p.k * row16);
   if (!gradient) {
@@ -308,12 +416,6 @@ Plan plan_for(int rows, int vocab, int hidden, int wformat, int dtype, bool grad
     p.o_chosen = take(at, int64_t{4} * rows);
   } else {
     p.splits = most_splits(hidden, rows, static_cast<int>(piece));
-    p.o_row = take(at, int64_t{4} * p.padded);
-    p.o_place = take(at, int64_t{4} * rows);
-    p.o_target = take(at, int64_t{8} * p.padded);
-    p.o_lse = take(at, int64_t{4} * p.padded);
-    p.o_grad = take(at, int64_t{4} * p.padded);
-    p.o_back = take(at, 8);
     p.o_p = take(at, rows64 * piece * row16);
     p.o_sums = take(at, sums_bytes(hidden, rows, p.splits));
   }
@@ -372,7 +474,79 @@ template <typename T> int weight_piece(const Plan& p, const Call& c, int first, 
   return 0;
 }
 
+void loss_launch(const Plan& p, const Call& c, const float2* stats, const float* chosen, int tiles, const LossRows& rows, int64_t ignore_index,
+                 float* losses, float* lse) {
+  if (p.rows <= kFewRows)
+    hipLaunchKernelGGL((loss_kernel<4>), dim3((p.rows + 3) / 4), dim3(1024), 0, c.stream, stats, chosen, tiles, rows, ignore_index, losses, lse);
+  else
+    hipLaunchKernelGGL((loss_kernel<16>), dim3((p.rows + 15) / 16), dim3(1024), 0, c.stream, stats, chosen, tiles, rows, ignore_index, losses, lse);
+}
+
+FewWeight few_weight(const Plan& p, const Call& c) {
+  const int64_t row_bytes = int64_t{p.hidden} * (c.wformat ? c.wformat : 16) / 8;
+  return FewWeight{static_cast<const uint8_t*>(c.weight), c.wscale, row_bytes, p.vocab, p.hidden, c.wformat ? p.hidden / c.group_size : 0,
+                   c.group_size, c.group_size, c.out_group};
+}
+template <typename T> void few_operand(const Plan& p, const Call& c, const int32_t* gather) {
+  const int64_t items = int64_t{p.hidden} / 32 * p.row_tiles * kWave;
+  hipLaunchKernelGGL((few_operand_kernel<T>), dim3(static_cast<unsigned>((items + 255) / 256)), dim3(256), 0, c.stream, static_cast<const T*>(c.hidden),
+                     c.hidden_stride, gather, p.rows, p.hidden, p.row_tiles, reinterpret_cast<T*>(c.workspace + p.o_x));
+}
+#define LLMQ_FEW_NT(KERNEL, BITS, ...)                                                                                        \
+  if (p.row_tiles == 1) hipLaunchKernelGGL((KERNEL<T, BITS, 1>), grid, dim3(kFewWaves * kWave), 0, c.stream, __VA_ARGS__);    \
+  else if (p.row_tiles == 2) hipLaunchKernelGGL((KERNEL<T, BITS, 2>), grid, dim3(kFewWaves * kWave), 0, c.stream, __VA_ARGS__); \
+  else hipLaunchKernelGGL((KERNEL<T, BITS, 4>), grid, dim3(kFewWaves * kWave), 0, c.stream, __VA_ARGS__)
+#define LLMQ_FEW(KERNEL, ...)                                     \
+  if (c.wformat == 0) { LLMQ_FEW_NT(KERNEL, 0, __VA_ARGS__); }    \
+  else if (c.wformat == 8) { LLMQ_FEW_NT(KERNEL, 8, __VA_ARGS__); } \
+  else { LLMQ_FEW_NT(KERNEL, 4, __VA_ARGS__); }
+
+template <typename T> int few_forward(const Plan& p, const Call& c, const int64_t* targets, int64_t ignore_index, float* losses, float* lse) {
+  few_operand<T>(p, c, nullptr);
+  const LossRows rows{targets, p.rows, p.vocab};
+  float2* stats = reinterpret_cast<float2*>(c.workspace + p.o_stats);
+  float* chosen = reinterpret_cast<float*>(c.workspace + p.o_chosen);
+  const T* x = reinterpret_cast<const T*>(c.workspace + p.o_x);
+  const FewWeight weight = few_weight(p, c);
+  const dim3 grid((p.vocab + kFewTokens - 1) / kFewTokens);
+  LLMQ_FEW(few_logits_kernel, weight, x, rows, stats, chosen)
+  loss_launch(p, c, stats, chosen, static_cast<int>(grid.x), rows, ignore_index, losses, lse);
+  return llmq_host::check_launch("vocab_loss");
+}
+
+// dW of tokens first ..: over the rows, both with them outermost
+template <typename T>
+void weight_gradient(const Plan& p, const Call& c, const TileOperand& part, int first, int tokens, const float* back, const int32_t* count, void* grad_weight) {
+  const int rows64 = static_cast<int>(round_up(p.rows, 64));
+  TileOperand hidden_k = hidden_operand(p, c), part_k = part;
+  hidden_k.rows = p.hidden;
+  hidden_k.k_rows = rows64;
+  part_k.rows = tokens;
+  product_launch<T, false, true>(hidden_k, part_k, rows64,
+                                 ProductOut{static_cast<T*>(grad_weight) + static_cast<int64_t>(first) * p.hidden, p.hidden, back, 0, 1, count}, c.stream);
+}
+
+template <typename T>
+int few_backward(const Plan& p, const Call& c, const Counted& rows, void* grad_hidden, void* grad_weight) {
+  few_operand<T>(p, c, rows.row);
+  if (p.stage_hidden) stage_hidden<T>(p, c, rows.row);
+  const T* x = reinterpret_cast<const T*>(c.workspace + p.o_x);
+  T* part = reinterpret_cast<T*>(c.workspace + p.o_p);
+  float* sums = reinterpret_cast<float*>(c.workspace + p.o_sums);
+  const FewWeight weight = few_weight(p, c);
+  const dim3 grid((p.vocab + kFewTokens - 1) / kFewTokens);
+  LLMQ_FEW(few_piece_kernel, weight, x, rows, part, int64_t{p.piece})
+  columns_launch<T>(weight, FewColumns{part, p.piece, rows.count, p.rows, sums, p.splits}, c.wformat, c.stream);
+  if (grad_weight != nullptr)   // (rows of P behind its last: that one again, against zeros of the hidden rows)
+    weight_gradient<T>(p, c, TileOperand{part, 0, int64_t{2} * p.piece, 0, 16 * p.row_tiles}, 0, p.vocab, rows.back, rows.count, grad_weight);
+  add_few_launch<T>(sums, p.splits, p.rows, p.hidden, rows.back, rows.place, grad_hidden, c.stream);
+  return llmq_host::check_launch("vocab_loss_grad");
+}
+
 template <typename T> int forward(const Plan& p, const Call& c, const int64_t* targets, int64_t ignore_index, float* losses, float* lse, int dtype) {
+  if constexpr (sizeof(T) == 2) {
+    if (p.few) return few_forward<T>(p, c, targets, ignore_index, losses, lse);
+  }
   if (p.stage_hidden) stage_hidden<T>(p, c, nullptr);
   const TileOperand hidden = hidden_operand(p, c);
   const LossRows rows{targets, p.rows, p.vocab};
@@ -389,7 +563,7 @@ template <typename T> int forward(const Plan& p, const Call& c, const int64_t* t
     else
       hipLaunchKernelGGL((logits_kernel<T, 256, 2, 4>), grid, dim3(512), 0, c.stream, weight, hidden, p.k, n_tiles, first, first / 256, rows, stats, chosen);
   }
-  hipLaunchKernelGGL(loss_kernel, dim3((p.rows + 15) / 16), dim3(256), 0, c.stream, stats, chosen, (p.vocab + 255) / 256, rows, ignore_index, losses, lse);
+  loss_launch(p, c, stats, chosen, (p.vocab + 255) / 256, rows, ignore_index, losses, lse);
   return llmq_host::check_launch("vocab_loss");
 }
 
@@ -404,6 +578,9 @@ int backward(const Plan& p, const Call& c, const int64_t* targets, int64_t ignor
   const bool learned = grad_weight != nullptr;
   const int rows64 = static_cast<int>(round_up(p.rows, 64));
   hipLaunchKernelGGL(count_rows_kernel, dim3(1), dim3(1024), 0, c.stream, grad, targets, lse, p.rows, p.padded, p.vocab, ignore_index, rows);
+  if constexpr (sizeof(T) == 2) {
+    if (p.few) return few_backward<T>(p, c, rows, grad_hidden, grad_weight);
+  }
   stage_hidden<T>(p, c, rows.row);
   const TileOperand hidden = hidden_operand(p, c);
   const int tn = tile_rows(p.rows), n_tiles = p.padded / tn;
@@ -423,13 +600,10 @@ int backward(const Plan& p, const Call& c, const int64_t* targets, int64_t ignor
     const TileOperand part{c.workspace + p.o_p, int64_t{2} * rows64 * p.piece, int64_t{2} * p.piece, p.rows, 0};
     product_launch<T, true, false>(weight_k, part, static_cast<int>(round_up(tokens, 64)),
                                    ProductOut{sums, p.hidden, nullptr, first == 0, p.splits, rows.count}, c.stream);
-    if (learned) {   // dW: over the rows, both with them outermost
-      TileOperand hidden_k = hidden, part_k = part;
-      hidden_k.rows = p.hidden;
-      hidden_k.k_rows = part_k.k_rows = rows64;
-      part_k.rows = tokens;
-      product_launch<T, false, true>(hidden_k, part_k, rows64,
-                                     ProductOut{static_cast<T*>(grad_weight) + static_cast<int64_t>(first) * p.hidden, p.hidden, back, 0, 1, rows.count}, c.stream);
+    if (learned) {
+      TileOperand part_k = part;
+      part_k.k_rows = rows64;
+      weight_gradient<T>(p, c, part_k, first, tokens, back, rows.count, grad_weight);
     }
   }
   add_planes_launch<T>(sums, p.rows, p.hidden, p.splits, rows.count, back, rows.place, grad_hidden, c.stream);
@@ -440,13 +614,13 @@ bool misaligned(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) !
 
 }  // namespace
 
-extern "C" size_t llmq_vocab_loss_workspace_bytes(int rows, int vocab, int hidden, int wformat, int dtype) {
+extern "C" size_t llmq_vocab_loss_workspace_bytes(int rows, int vocab, int hidden, int group_size, int wformat, int dtype) {
   if (rows <= 0 || vocab <= 0 || hidden <= 0) return 0;
-  return static_cast<size_t>(plan_for(rows, vocab, hidden, wformat, dtype, false, false).bytes);
+  return static_cast<size_t>(plan_for(rows, vocab, hidden, group_size, wformat, dtype, false, false).bytes);
 }
-extern "C" size_t llmq_vocab_loss_grad_workspace_bytes(int rows, int vocab, int hidden, int wformat, int dtype, int want_weight) {
+extern "C" size_t llmq_vocab_loss_grad_workspace_bytes(int rows, int vocab, int hidden, int group_size, int wformat, int dtype, int want_weight) {
   if (rows <= 0 || vocab <= 0 || hidden <= 0) return 0;
-  return static_cast<size_t>(plan_for(rows, vocab, hidden, wformat, dtype, true, want_weight != 0).bytes);
+  return static_cast<size_t>(plan_for(rows, vocab, hidden, group_size, wformat, dtype, true, want_weight != 0).bytes);
 }
 
 extern "C" int llmq_vocab_loss(const void* hidden, int64_t hidden_stride, const void* weight, const float* wscale_or_null,
@@ -458,7 +632,7 @@ extern "C" int llmq_vocab_loss(const void* hidden, int64_t hidden_stride, const 
   if (vocab == 0) return llmq_host::fail_invalid("a vocabulary of no tokens");
   if (!hidden || !weight || !targets || !losses || !lse || (wformat != 0 && !wscale_or_null)) return llmq_host::fail_invalid("null tensor pointer");
   if (misaligned(hidden) || misaligned(weight)) return llmq_host::fail_invalid("hidden and weight must be 16-byte aligned");
-  const Plan p = plan_for(rows, vocab, hidden_size, wformat, dtype, false, false);
+  const Plan p = plan_for(rows, vocab, hidden_size, group_size, wformat, dtype, false, false);
   if (!workspace || misaligned(workspace) || workspace_bytes < static_cast<size_t>(p.bytes))
     return llmq_host::fail_invalid("the workspace must be 16-byte aligned and hold %lld bytes, got %zu", static_cast<long long>(p.bytes), workspace_bytes);
   const Call c{hidden, weight, wscale_or_null, hidden_stride, group_size, out_group, wformat, static_cast<uint8_t*>(workspace), static_cast<hipStream_t>(stream)};
@@ -481,7 +655,7 @@ extern "C" int llmq_vocab_loss_grad(const void* hidden, int64_t hidden_stride, c
     return llmq_host::fail_invalid("null tensor pointer");
   if (misaligned(hidden) || misaligned(weight) || misaligned(grad_hidden) || misaligned(grad_weight_or_null))
     return llmq_host::fail_invalid("hidden, weight and their gradients must be 16-byte aligned");
-  const Plan p = plan_for(rows, vocab, hidden_size, wformat, dtype, true, grad_weight_or_null != nullptr);
+  const Plan p = plan_for(rows, vocab, hidden_size, group_size, wformat, dtype, true, grad_weight_or_null != nullptr);
   if (!workspace || misaligned(workspace) || workspace_bytes < static_cast<size_t>(p.bytes))
     return llmq_host::fail_invalid("the workspace must be 16-byte aligned and hold %lld bytes, got %zu", static_cast<long long>(p.bytes), workspace_bytes);
   const Call c{hidden, weight, wscale_or_null, hidden_stride, group_size, out_group, wformat, static_cast<uint8_t*>(workspace), static_cast<hipStream_t>(stream)};

@@ -3,9 +3,10 @@
 //   gx[t, k] = sum_n g[t, n] W[n, k],     W = (dtype)(code * scale): the matrix of the reference's many-rows branch
 //                                         (llmquant/quantizers/kernel.py:68-79), whose autograd this stands for
 //
-// The weight is brought to its values a piece of its rows at a time (dense_stage.h: a piece that the caches hold), and multiplied on the
+// Few rows: past the weight as it lies (dense_few.h). Otherwise the weight is brought to its values a piece of its rows at a time (dense_stage.h: a piece that the caches hold), and multiplied on the
 // matrix core with the reduction outermost, as it lies (dense_tile.h); sums over the pieces and over the splits of one go through fp32 planes. Bound: the
-// matrix core for training batches, the weight's way through memory for few rows.
+// matrix core for training batches, the weight's way through memory and the conversion of its codes for few rows.
+#include "dense_few.h"
 #include "dense_stage.h"
 
 namespace {
@@ -15,15 +16,24 @@ using namespace llmq;
 struct Plan {
   int64_t n_padded, piece, ld;   // N in whole steps; rows of W a piece; its columns
   int splits;
-  bool stage_grad;
+  bool stage_grad, few;          // few: rows that go past the weight as it lies
   int64_t o_weight, o_grad, o_sums, bytes;
 };
 
 constexpr int64_t kPieceBytes = int64_t{128} << 20;
+// Up to so many rows the weight is read as it lies, once for each 64 (float16, bfloat16; whole calls, N x K int8: 4096 x 4096, 1 row 16 us for 33,
+// 256 rows 36 for 54; 14336 x 4096, 256 rows 85 for 112, 320 rows 145 for 125).
+constexpr int kFewMost = 256;
 
-Plan plan_for(int rows, int N, int width, int dtype) {
+Plan plan_for(int rows, int N, int width, int wformat, int dtype) {
   Plan p{};
   const int64_t row16 = dtype == LLMQ_F32 ? 6 : 2;
+  p.few = dtype != LLMQ_F32 && rows <= kFewMost;
+  if (p.few) {
+    p.splits = few_splits(N, width, rows, wformat);
+    p.bytes = int64_t{4} * p.splits * rows * width;
+    return p;
+  }
   p.n_padded = round_up(N, 64);
   p.ld = width;
   p.stage_grad = dtype == LLMQ_F32 || N % 64 != 0;
@@ -48,6 +58,15 @@ template <typename T>
 int launch(const Plan& p, const void* grad, int64_t stride, const void* qweight, const float* wscale, void* out, uint8_t* workspace, int rows,
            int N, int G, int gs, int keep, int out_group, int wformat, int dtype, hipStream_t stream) {
   constexpr int P = TileType<T>::kPlanes;
+  if constexpr (P == 1) {
+    if (p.few) {
+      float* sums = reinterpret_cast<float*>(workspace);
+      columns_launch<T>(FewWeight{static_cast<const uint8_t*>(qweight), wscale, static_cast<int64_t>(G) * gs * wformat / 8, N, G * keep, G, gs, keep, out_group},
+                        FewColumns{grad, stride, nullptr, rows, sums, p.splits}, wformat, stream);
+      add_few_launch<T>(sums, p.splits, rows, G * keep, nullptr, nullptr, out, stream);
+      return llmq_host::check_launch("wq_linear_grad");
+    }
+  }
   const int width = G * keep, n64 = static_cast<int>(p.n_padded);
   if (p.stage_grad)   // (zeros up to a whole step, against rows of W that are looked at again)
     stage_launch<T>(StageSource{grad, nullptr, nullptr, stride, rows, N, 0, rows, 0, 0, 0, 0}, StageTarget{workspace + p.o_grad, rows * p.n_padded, n64}, 0, stream);
@@ -76,9 +95,9 @@ int launch(const Plan& p, const void* grad, int64_t stride, const void* qweight,
 
 }  // namespace
 
-extern "C" size_t llmq_wq_linear_grad_workspace_bytes(int rows, int N, int G, int keep_per_group, int dtype) {
+extern "C" size_t llmq_wq_linear_grad_workspace_bytes(int rows, int N, int G, int keep_per_group, int wformat, int dtype) {
   if (rows <= 0 || N <= 0 || G <= 0 || keep_per_group <= 0) return 0;
-  return static_cast<size_t>(plan_for(rows, N, G * keep_per_group, dtype).bytes);
+  return static_cast<size_t>(plan_for(rows, N, G * keep_per_group, wformat, dtype).bytes);
 }
 
 extern "C" int llmq_wq_linear_grad(const void* grad, int64_t grad_stride, const void* qweight, const float* wscale, void* grad_x,
@@ -101,7 +120,7 @@ extern "C" int llmq_wq_linear_grad(const void* grad, int64_t grad_stride, const 
   if (!grad || !qweight || !wscale || !grad_x) return llmq_host::fail_invalid("null tensor pointer");
   if ((reinterpret_cast<uintptr_t>(grad) | reinterpret_cast<uintptr_t>(qweight) | reinterpret_cast<uintptr_t>(grad_x)) & 15u)
     return llmq_host::fail_invalid("grad, qweight and grad_x must be 16-byte aligned");
-  const Plan p = plan_for(rows, N, G * keep_per_group, dtype);
+  const Plan p = plan_for(rows, N, G * keep_per_group, wformat, dtype);
   if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 15u) || workspace_bytes < static_cast<size_t>(p.bytes))
     return llmq_host::fail_invalid("the workspace must be 16-byte aligned and hold %lld bytes, got %zu", static_cast<long long>(p.bytes), workspace_bytes);
   hipStream_t s = static_cast<hipStream_t>(stream);

@@ -202,15 +202,15 @@ def load_capi() -> ctypes.CDLL:
                                             + [c_int] * 9 + [c_p])
     lib.llmq_kv_block_attention.restype = c_int
     c_size = ctypes.c_size_t
-    lib.llmq_wq_linear_grad_workspace_bytes.argtypes = [c_int] * 5
+    lib.llmq_wq_linear_grad_workspace_bytes.argtypes = [c_int] * 6
     lib.llmq_wq_linear_grad_workspace_bytes.restype = c_size
     lib.llmq_wq_linear_grad.argtypes = [c_p, c_i64] + [c_p] * 4 + [c_size] + [c_int] * 8 + [c_p]
     lib.llmq_wq_linear_grad.restype = c_int
-    lib.llmq_vocab_loss_workspace_bytes.argtypes = [c_int] * 5
+    lib.llmq_vocab_loss_workspace_bytes.argtypes = [c_int] * 6
     lib.llmq_vocab_loss_workspace_bytes.restype = c_size
     lib.llmq_vocab_loss.argtypes = [c_p, c_i64] + [c_p] * 3 + [c_i64] + [c_p] * 3 + [c_size] + [c_int] * 7 + [c_p]
     lib.llmq_vocab_loss.restype = c_int
-    lib.llmq_vocab_loss_grad_workspace_bytes.argtypes = [c_int] * 6
+    lib.llmq_vocab_loss_grad_workspace_bytes.argtypes = [c_int] * 7
     lib.llmq_vocab_loss_grad_workspace_bytes.restype = c_size
     lib.llmq_vocab_loss_grad.argtypes = [c_p, c_i64] + [c_p] * 3 + [c_i64] + [c_p] * 5 + [c_size] + [c_int] * 7 + [c_p]
     lib.llmq_vocab_loss_grad.restype = c_int
