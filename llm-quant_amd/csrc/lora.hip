@@ -369,7 +369,7 @@ __device__ __forceinline__ void make_plan(PlanLds& s, const Requests& req, const
             if (few) s.seq[i] = at;
             else p.seq_start[b0 + i] = at;
           }
-          at += s.n[i];
+          at = min(at + s.n[i], p.capacity);   // (more than that only where query_start decreases)
         }
       }
     }
@@ -384,8 +384,8 @@ __device__ __forceinline__ void make_plan(PlanLds& s, const Requests& req, const
       s.scan[t] += v;
       __syncthreads();
     }
-    if (t < p.slots) p.start[t] = s.scan[t] - mine;
-    if (t == p.slots - 1) p.start[p.slots] = s.scan[t];
+    if (t < p.slots) p.start[t] = min(s.scan[t] - mine, p.capacity);
+    if (t == p.slots - 1) p.start[p.slots] = min(s.scan[t], p.capacity);
   }
   __syncthreads();
   for (int row = t; row < req.rows.rows; row += kPlanThreads) {
