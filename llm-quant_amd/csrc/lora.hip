@@ -189,8 +189,25 @@ struct Expand {
   void* out;               // [rows, width], contiguous
   float* low;              // or null: [rows, rank], the sum of the planes (where there are several) and zeros without an adapter
   int rows, columns;       // columns of out
-  int pieces;              // workgroups from there on in blockIdx.x: rows of no request
+  int pieces, rest;        // pieces of requests for each 512 columns; workgroups behind all of them, for rows of no request
 };
+
+// Rows in front of the first request and behind the last one: the base as it is, no sums.
+template <typename T> __device__ __forceinline__ void rows_of_nobody(const int rank, const Ragged& rows, const Expand& e, const int id) {
+  constexpr int V = Pack<T>::N;
+  const int begin = rows.first(0), end = max(rows.first(rows.sequences), begin), packets = e.columns / V;
+  const int64_t n = begin + e.rows - end, step = int64_t{kExpandWaves} * kWave * e.rest;
+  for (int64_t i = static_cast<int64_t>(id) * kExpandWaves * kWave + threadIdx.x; i < n * packets; i += step) {
+    const int64_t at = i / packets, row = at < begin ? at : at - begin + end, c = (i - at * packets) * V;
+    const u32x4 v = e.base == nullptr ? u32x4{0, 0, 0, 0} : load16(static_cast<const T*>(e.base) + row * e.base_stride + c);
+    store16(static_cast<T*>(e.out) + row * e.columns + c, v);
+  }
+  if (e.low == nullptr) return;
+  for (int64_t i = static_cast<int64_t>(id) * kExpandWaves * kWave + threadIdx.x; i < n * rank; i += step) {
+    const int64_t at = i / rank, row = at < begin ? at : at - begin + end;
+    e.low[row * rank + (i - at * rank)] = 0.0f;
+  }
+}
 
 // 128 columns a wave: lane 16 g + r has columns 8 r .. 8 r + 7, one of each of eight tiles, of rows 4 g .. 4 g + 3, so that 16 lanes read and
 // write 256 neighbouring bytes of a row (with rows over the lanes, 64 bytes of each of 16: 4099 rows of 4096 23 us). What does not depend on the
@@ -198,28 +215,23 @@ struct Expand {
 template <typename T, int RT, int NT>
 __global__ __launch_bounds__(kExpandWaves * kWave) void expand_kernel(const Bank bank, const Requests req, const Expand e) {
   constexpr int V = Pack<T>::N, KT = (RT * 16 + 4 * V - 1) / (4 * V);   // steps of the rank: 32 (fp32: 16)
+  constexpr int kBlocks = KT * NT, kParts = kBlocks == 1 ? 4 : kBlocks == 2 ? 2 : 1;   // operands of `low`; threads for each packet of one
+  __shared__ u32x4 s_low[sizeof(T) == 4 ? 1 : 2][kBlocks][kWave];
   const int lane = threadIdx.x & (kWave - 1), wv = threadIdx.x / kWave, lr = lane & 15, g = lane >> 4;
-  int first, n, a;
-  const bool rest = static_cast<int>(blockIdx.x) >= e.pieces;   // rows in front of the first request and behind the last one: the base as it is
-  if (!rest) {
-    a = req.template piece<kPieceShift<NT>>(blockIdx.x, bank.slots, first, n);
-    if (n <= 0) return;
-  } else {
-    a = -1;
-    first = (blockIdx.x - e.pieces) << kPieceShift<NT>;
-    n = min(e.rows - first, 1 << kPieceShift<NT>);
+  const int pieces = static_cast<int>(gridDim.x) - e.rest;
+  if (static_cast<int>(blockIdx.x) >= pieces) {
+    rows_of_nobody<T>(bank.rank, req.rows, e, blockIdx.x - pieces);
+    return;
   }
-  const int begin = rest ? req.rows.first(0) : 0, end = rest ? max(req.rows.first(req.rows.sequences), begin) : 0;
-  if (rest && first >= begin && first + n <= end) return;   // (the usual: the requests have all rows)
-  const int c0 = (blockIdx.y * kExpandWaves + wv) * 128;
-  const bool writes_low = e.low != nullptr && c0 == 0;
-  if (a < 0 && writes_low) {   // (no adapter: zeros)
-    for (int i = lane; i < n * bank.rank; i += kWave) {
-      const int64_t row = first + i / bank.rank;
-      if (!rest || row < begin || row >= end) e.low[row * bank.rank + i % bank.rank] = 0.0f;
-    }
+  // the pieces of the same columns to one XCD, whose cache has the bank's rows for them
+  const int item = tile_of_workgroup(blockIdx.x, pieces), group = item / e.pieces;
+  int first, n;
+  const int a = req.template piece<kPieceShift<NT>>(item - group * e.pieces, bank.slots, first, n);
+  if (n <= 0) return;
+  const int c0 = (group * kExpandWaves + wv) * 128;
+  if (a < 0 && e.low != nullptr && c0 == 0) {   // (no adapter: zeros)
+    for (int i = lane; i < n * bank.rank; i += kWave) e.low[static_cast<int64_t>(first) * bank.rank + i] = 0.0f;
   }
-  if (c0 >= e.columns) return;
   const int c = c0 + 8 * lr;   // (columns are a multiple of 8)
   const bool here = c < e.columns;
   u32x4 m[KT][8], base[NT][4][8 / V];
@@ -241,47 +253,65 @@ __global__ __launch_bounds__(kExpandWaves * kWave) void expand_kernel(const Bank
       }
   }
   v4f acc[NT][8] = {};
-  if (a >= 0) {
+  if (a >= 0) {   // (the workgroup's)
+    // `low` of the piece as operands, made once: packet (row 16 j + lr, values (4 k + g) V ..) by kParts threads, a part of the planes each
+    constexpr int kEach = kWave / kParts;
     const float s = e.scaling[a];
+#pragma unroll
+    for (int i0 = 0; i0 < kBlocks * kParts; i0 += kExpandWaves) {
+      const int packet = (i0 + wv) * kEach + lane % kEach, part = lane / kEach, block = packet / kWave, pl = packet % kWave;
+      if (block >= kBlocks) break;
+      const int j = block % NT, r = (block / NT * 4 + (pl >> 4)) * V, t = j * 16 + (pl & 15);
+      const float* at = e.planes + static_cast<int64_t>(first + min(t, n - 1)) * bank.rank + min(r, bank.rank - V);
+      v4f sum[V / 4] = {};
+      constexpr int kAhead = 4;
+      for (int p0 = part; p0 < e.splits; p0 += kAhead * kParts) {
+        v4f v[kAhead][V / 4];
+#pragma unroll
+        for (int p = 0; p < kAhead; ++p)
+#pragma unroll
+          for (int i = 0; i < V / 4; ++i) v[p][i] = *reinterpret_cast<const v4f*>(at + min(p0 + p * kParts, e.splits - 1) * e.plane + 4 * i);
+#pragma unroll
+        for (int p = 0; p < kAhead; ++p)
+#pragma unroll
+          for (int i = 0; i < V / 4; ++i)
+            if (p0 + p * kParts < e.splits) sum[i] += v[p][i];
+      }
+      float f[V];
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        float v = sum[i / 4][i % 4];
+        if constexpr (kParts > 1) {
+#pragma unroll
+          for (int d = kEach; d < kWave; d *= 2) v += __shfl_xor(v, d);
+        }
+        f[i] = v;
+      }
+      if (part != 0) continue;
+      if (e.splits > 1 && e.low != nullptr && group == 0 && t < n && r < bank.rank) {
+        float* to = e.low + static_cast<int64_t>(first + t) * bank.rank + r;
+#pragma unroll
+        for (int i = 0; i < V; i += 4) *reinterpret_cast<v4f*>(to + i) = v4f{f[i], f[i + 1], f[i + 2], f[i + 3]};
+      }
+#pragma unroll
+      for (int i = 0; i < V; ++i) f[i] = r < bank.rank ? f[i] * s : 0.0f;
+      if constexpr (sizeof(T) == 4) {
+        s_low[0][block][pl] = Pack<float>::pack(f);
+      } else {
+        const HiLo low = hi_lo(f);
+        s_low[0][block][pl] = low.hi;
+        s_low[1][block][pl] = low.lo;
+      }
+    }
+    __syncthreads();
+    if (c0 >= e.columns) return;
 #pragma unroll
     for (int k = 0; k < KT; ++k) {
       u32x4 low_hi[NT], low_lo[NT];   // (fp32: low_hi alone)
 #pragma unroll
       for (int j = 0; j < NT; ++j) {
-        const int r = (k * 4 + g) * V;
-        const int64_t at = static_cast<int64_t>(first + min(j * 16 + lr, n - 1)) * bank.rank + min(r, bank.rank - V);
-        v4f sum[V / 4];
-#pragma unroll
-        for (int i = 0; i < V / 4; ++i) sum[i] = *reinterpret_cast<const v4f*>(e.planes + at + 4 * i);
-        if (e.splits > 1) {
-          constexpr int kAhead = 4;
-          for (int p0 = 1; p0 < e.splits; p0 += kAhead) {
-            v4f v[kAhead][V / 4];
-#pragma unroll
-            for (int p = 0; p < kAhead; ++p)
-#pragma unroll
-              for (int i = 0; i < V / 4; ++i) v[p][i] = *reinterpret_cast<const v4f*>(e.planes + min(p0 + p, e.splits - 1) * e.plane + at + 4 * i);
-#pragma unroll
-            for (int p = 0; p < kAhead; ++p)
-#pragma unroll
-              for (int i = 0; i < V / 4; ++i)
-                if (p0 + p < e.splits) sum[i] += v[p][i];
-          }
-          if (writes_low && j * 16 + lr < n && r < bank.rank) {
-#pragma unroll
-            for (int i = 0; i < V / 4; ++i) *reinterpret_cast<v4f*>(e.low + at + 4 * i) = sum[i];
-          }
-        }
-        float f[V];
-#pragma unroll
-        for (int i = 0; i < V; ++i) f[i] = r < bank.rank ? sum[i / 4][i % 4] * s : 0.0f;
-        if constexpr (sizeof(T) == 4) {
-          low_hi[j] = Pack<float>::pack(f);
-        } else {
-          const HiLo low = hi_lo(f);
-          low_hi[j] = low.hi;
-          low_lo[j] = low.lo;
-        }
+        low_hi[j] = s_low[0][k * NT + j][lane];
+        if constexpr (sizeof(T) == 2) low_lo[j] = s_low[1][k * NT + j][lane];
       }
 #pragma unroll
       for (int mi = 0; mi < 8; ++mi) {
@@ -315,7 +345,7 @@ __global__ __launch_bounds__(kExpandWaves * kWave) void expand_kernel(const Bank
     for (int i = 0; i < 4; ++i) {
       const int t = j * 16 + 4 * g + i;
       const int64_t row = first + t;
-      if (t >= n || (rest && row >= begin && row < end)) continue;
+      if (t >= n) continue;
 #pragma unroll
       for (int h = 0; h < 8 / V; ++h) {
         float f[V] = {};
@@ -710,8 +740,8 @@ template <typename T> void expand(const Bank& bank, const Requests& req, Expand 
   const bool ragged = req.rows.start != nullptr;
   const int nt = row_tiles(e.rows, req.rows.sequences, ragged);
   e.pieces = pieces_of(e.rows, req.rows.sequences, ragged, nt);
-  const bool rest = ragged && (e.out != e.base || e.low != nullptr);
-  const dim3 grid(e.pieces + (rest ? (e.rows + 16 * nt - 1) / (16 * nt) : 0), (e.columns + kExpandWaves * 128 - 1) / (kExpandWaves * 128));
+  e.rest = ragged && (e.out != e.base || e.low != nullptr) ? 32 : 0;   // (usually without a row: the requests have them all)
+  const dim3 grid(e.pieces * ((e.columns + kExpandWaves * 128 - 1) / (kExpandWaves * 128)) + e.rest);
   if (bank.rank <= 16) expand_nt<T, 1>(bank, req, e, nt, grid, s);
   else if (bank.rank <= 32) expand_nt<T, 2>(bank, req, e, nt, grid, s);
   else if (bank.rank <= 64) expand_nt<T, 4>(bank, req, e, nt, grid, s);
@@ -771,7 +801,7 @@ void gradients(const GradPlan& p, const void* grad, int64_t grad_stride, const v
   if constexpr (sizeof(T) == 4) hipLaunchKernelGGL((prepare_kernel<uint32_t>), dim3(1 + tiles), dim3(kPlanThreads), 0, s, req, plan, turn_a, turn_b);
   else hipLaunchKernelGGL((prepare_kernel<uint16_t>), dim3(1 + tiles), dim3(kPlanThreads), 0, s, req, plan, turn_a, turn_b);
   shrink<T>(grad, grad_stride, Bank{ws + p.o_bt, slots, rank, out}, req, planes, plane, p.splits, req.rows.start != nullptr, s);
-  expand<T>(Bank{ws + p.o_at, slots, rank, in}, req, Expand{planes, plane, p.splits, scaling, grad_base, base_stride, grad_x, p.splits > 1 ? du : nullptr, rows, in, 0}, s);
+  expand<T>(Bank{ws + p.o_at, slots, rank, in}, req, Expand{planes, plane, p.splits, scaling, grad_base, base_stride, grad_x, p.splits > 1 ? du : nullptr, rows, in, 0, 0}, s);
   const Outer o{OuterSide{x, x_stride, x_scale, du, reinterpret_cast<float*>(ws + p.o_rec_a), in},
                 OuterSide{grad, grad_stride, nullptr, low, reinterpret_cast<float*>(ws + p.o_rec_b), out},
                 plan.start, plan.order, scaling, slots, rank, p.capacity, p.shift, (in + kColumns - 1) / kColumns};
@@ -834,7 +864,7 @@ extern "C" int llmq_lora_add(const void* x, int64_t x_stride, const void* base, 
   const int splits = splits_of(rows, sequences, ragged, in_features, rank, dtype);
   float* planes = splits == 1 && low_or_null ? low_or_null : static_cast<float*>(workspace);   // (one plane is the sum)
   const int64_t plane = static_cast<int64_t>(rows) * rank;
-  const Expand e{planes, plane, splits, scaling, base, base_stride, out, low_or_null, rows, out_features, 0};
+  const Expand e{planes, plane, splits, scaling, base, base_stride, out, low_or_null, rows, out_features, 0, 0};
   hipStream_t s = static_cast<hipStream_t>(stream);
 #define LLMQ_ADD(T)                                                                                                        \
   shrink<T>(x, x_stride, Bank{lora_a, slots, rank, in_features}, req, planes, plane, splits, ragged, s);                   \
