@@ -216,7 +216,9 @@ template <typename T, int RT, int NT>
 __global__ __launch_bounds__(kExpandWaves * kWave) void expand_kernel(const Bank bank, const Requests req, const Expand e) {
   constexpr int V = Pack<T>::N, KT = (RT * 16 + 4 * V - 1) / (4 * V);   // steps of the rank: 32 (fp32: 16)
   constexpr int kBlocks = KT * NT, kParts = kBlocks == 1 ? 4 : kBlocks == 2 ? 2 : 1;   // operands of `low`; threads for each packet of one
+  constexpr bool kStaged = sizeof(T) == 2 && RT <= 4;   // the bank's rows of a wave's columns through LDS
   __shared__ u32x4 s_low[sizeof(T) == 4 ? 1 : 2][kBlocks][kWave];
+  __shared__ __attribute__((aligned(16))) uint8_t s_bank[kStaged ? kExpandWaves * 4096 * RT : 16];
   const int lane = threadIdx.x & (kWave - 1), wv = threadIdx.x / kWave, lr = lane & 15, g = lane >> 4;
   const int pieces = static_cast<int>(gridDim.x) - e.rest;
   if (static_cast<int>(blockIdx.x) >= pieces) {
@@ -234,8 +236,22 @@ __global__ __launch_bounds__(kExpandWaves * kWave) void expand_kernel(const Bank
   }
   const int c = c0 + 8 * lr;   // (columns are a multiple of 8)
   const bool here = c < e.columns;
-  u32x4 m[KT][8], base[NT][4][8 / V];
-  if (a >= 0) {
+  u32x4 m[kStaged ? 1 : KT][8], base[NT][4][8 / V];
+  uint8_t* const mine = s_bank + __builtin_amdgcn_readfirstlane(wv) * (kStaged ? 4096 * RT : 0);
+  const int per = bank.rank / V;   // packets of a column
+  if constexpr (kStaged) {
+    if (a >= 0 && c0 < e.columns) {   // (past the columns: the last packet again)
+      const BufferBase mb = buffer_base(static_cast<const T*>(bank.m) + (static_cast<int64_t>(a) * e.columns + c0) * bank.rank);
+      const uint32_t eight = 0xffffffffu / static_cast<uint32_t>(8 * per) + 1;   // (a division by the packets of eight columns)
+      const int most = min(e.columns - c0, 128) * per - 1;
+#pragma unroll
+      for (int i = 0; i < 4 * RT; ++i) {
+        if (i >= 2 * per) break;
+        const int at = i * kWave + lane, packet = at ^ (static_cast<int>(__umulhi(at, eight)) & 7);
+        buffer_to_lds<16>(mb, mine + i * 1024, static_cast<uint32_t>(min(packet, most)) * 16u, 0);
+      }
+    }
+  } else if (a >= 0) {
 #pragma unroll
     for (int k = 0; k < KT; ++k)
 #pragma unroll
@@ -303,6 +319,7 @@ __global__ __launch_bounds__(kExpandWaves * kWave) void expand_kernel(const Bank
         s_low[1][block][pl] = low.lo;
       }
     }
+    if constexpr (kStaged) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
     if (c0 >= e.columns) return;
 #pragma unroll
@@ -315,24 +332,31 @@ __global__ __launch_bounds__(kExpandWaves * kWave) void expand_kernel(const Bank
       }
 #pragma unroll
       for (int mi = 0; mi < 8; ++mi) {
+        u32x4 v;
+        if constexpr (kStaged) {   // (past the rank: zeros of `low` against its last packet)
+          const int packet = (8 * lr + mi) * per + min(k * 4 + g, per - 1);
+          v = load16(mine + ((packet ^ (lr & 7)) << 4));
+        } else {
+          v = m[k][mi];
+        }
         if constexpr (sizeof(T) == 4) {
 #pragma unroll
-          for (int j = 0; j < NT; ++j) acc[j][mi] = mfma_packet<float>(low_hi[j], m[k][mi], acc[j][mi]);
+          for (int j = 0; j < NT; ++j) acc[j][mi] = mfma_packet<float>(low_hi[j], v, acc[j][mi]);
         } else if constexpr (__is_same(T, f16_t)) {
           float w[8];
-          Pack<f16_t>::unpack(m[k][mi], w);
-          const HiLo v = hi_lo(w);   // (exact: 11 bits in 16)
+          Pack<f16_t>::unpack(v, w);
+          const HiLo two = hi_lo(w);   // (exact: 11 bits in 16)
 #pragma unroll
           for (int j = 0; j < NT; ++j) {
-            acc[j][mi] = mfma_16x16x32<bf16_t>(low_hi[j], v.lo, acc[j][mi]);
-            acc[j][mi] = mfma_16x16x32<bf16_t>(low_lo[j], v.hi, acc[j][mi]);
-            acc[j][mi] = mfma_16x16x32<bf16_t>(low_hi[j], v.hi, acc[j][mi]);
+            acc[j][mi] = mfma_16x16x32<bf16_t>(low_hi[j], two.lo, acc[j][mi]);
+            acc[j][mi] = mfma_16x16x32<bf16_t>(low_lo[j], two.hi, acc[j][mi]);
+            acc[j][mi] = mfma_16x16x32<bf16_t>(low_hi[j], two.hi, acc[j][mi]);
           }
         } else {
 #pragma unroll
           for (int j = 0; j < NT; ++j) {
-            acc[j][mi] = mfma_16x16x32<bf16_t>(low_lo[j], m[k][mi], acc[j][mi]);
-            acc[j][mi] = mfma_16x16x32<bf16_t>(low_hi[j], m[k][mi], acc[j][mi]);
+            acc[j][mi] = mfma_16x16x32<bf16_t>(low_lo[j], v, acc[j][mi]);
+            acc[j][mi] = mfma_16x16x32<bf16_t>(low_hi[j], v, acc[j][mi]);
           }
         }
       }
@@ -703,12 +727,12 @@ int row_tiles(int rows, int sequences, bool ragged) { return !ragged || rows < 2
 // shrink: one (many workgroups), two where the bank's rows weigh more than twice the activation's
 int shrink_tiles(int rows, int sequences, bool ragged, int rank) { return rank > 32 && row_tiles(rows, sequences, ragged) > 1 ? 2 : 1; }
 int pieces_of(int rows, int sequences, bool ragged, int nt) { return ragged ? rows / (16 * nt) + 2 * sequences : sequences; }
-// Parts of the reduction: for 768 workgroups, of a step a wave at least; up to eight for single rows, two for
-// few pieces of rows (expand adds them up in every wave: with two parts of 257 pieces it takes 26.5 us instead of 18.9, shrink 11.0 instead of 14.7).
+// Parts of the reduction: for 768 workgroups, of a step a wave at least; up to eight for single rows, four for few pieces of rows, two for many
+// (4099 rows of 4096 by 64, one part: shrink 17.0 us, expand 24.4; two: 14.6 and 25.0; four: 13.8 and 26.5).
 int splits_of(int rows, int sequences, bool ragged, int width, int rank, int dtype) {
   const int nt = shrink_tiles(rows, sequences, ragged, rank);
   const int64_t real = ragged ? (rows + 16 * nt - 1) / (16 * nt) : sequences;
-  const int steps = (width * (dtype == LLMQ_F32 ? 4 : 2) + 127) / 128, most = !ragged ? 8 : real < 96 ? 2 : 1;
+  const int steps = (width * (dtype == LLMQ_F32 ? 4 : 2) + 127) / 128, most = !ragged ? 8 : real < 96 ? 4 : 2;
   int64_t splits = 768 / (real < 1 ? 1 : real);
   if (splits > steps / shrink_waves(rank)) splits = steps / shrink_waves(rank);
   if (splits > most) splits = most;
