@@ -383,6 +383,92 @@ __global__ __launch_bounds__(kExpandWaves * kWave) void expand_kernel(const Bank
     }
 }
 
+// ---- a row each, both factors at once ---------------------------------------------------------------------------------------------
+// The next token of a few chats: a workgroup has 512 columns of a row, a column a thread, and makes the row's `low` itself, as every other of the row
+// does: banks this small come out of the XCD's cache sooner than another launch starts. The rank's rows go over the waves, two at a time, their
+// packets over the lanes. All in fp32.
+constexpr int kStepThreads = 512;
+template <typename T>
+__global__ __launch_bounds__(kStepThreads) void step_kernel(const T* __restrict__ x, const int64_t x_stride, const Bank bank, const T* __restrict__ lora_b,
+                                                            const int32_t* __restrict__ adapter, const Expand e, const int groups) {
+  constexpr int V = Pack<T>::N, kWaves = kStepThreads / kWave, kAhead = 4;
+  __shared__ float s_low[128];
+  const int item = tile_of_workgroup(blockIdx.x, gridDim.x), row = item / groups, group = item - row * groups;
+  const int lane = threadIdx.x & (kWave - 1), wv = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) / kWave);
+  const int id = adapter[row], a = id >= 0 && id < bank.slots ? id : -1;
+  const int c = group * kStepThreads + threadIdx.x, at = min(c, e.columns - 1);
+  T* const out = static_cast<T*>(e.out) + static_cast<int64_t>(row) * e.columns + c;
+  const T base = static_cast<const T*>(e.base)[row * e.base_stride + at];
+  float* const low = e.low != nullptr && group == 0 && static_cast<int>(threadIdx.x) < bank.rank ? e.low + static_cast<int64_t>(row) * bank.rank + threadIdx.x : nullptr;
+  if (a < 0) {
+    if (c < e.columns) *out = base;
+    if (low != nullptr) *low = 0.0f;
+    return;
+  }
+  const T* const column = lora_b + (static_cast<int64_t>(a) * e.columns + at) * bank.rank;
+  const int per = bank.rank / V, packets = bank.width / V;
+  u32x4 b[kAhead];
+#pragma unroll
+  for (int i = 0; i < kAhead; ++i) b[i] = load16(column + min(i, per - 1) * V);
+  const float scaling = e.scaling[a];
+  const T* const from = x + row * x_stride;
+  const T* const m = static_cast<const T*>(bank.m) + static_cast<int64_t>(a) * bank.rank * bank.width;
+  for (int r = 2 * wv; r < bank.rank; r += 2 * kWaves) {   // (the rank is even)
+    float sum[2] = {0.0f, 0.0f};
+#pragma unroll 2
+    for (int p0 = 0; p0 < packets; p0 += kAhead * kWave) {
+      u32x4 v[kAhead], w[2][kAhead];
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) {
+        const int p = min(p0 + i * kWave + lane, packets - 1) * V;
+        v[i] = load16(from + p);
+#pragma unroll
+        for (int q = 0; q < 2; ++q) w[q][i] = load16(m + static_cast<int64_t>(r + q) * bank.width + p);
+      }
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) {
+        float f[V], h[V];
+        Pack<T>::unpack(v[i], f);
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+          Pack<T>::unpack(w[q][i], h);
+          float part = 0.0f;
+#pragma unroll
+          for (int k = 0; k < V; ++k) part = __builtin_fmaf(f[k], h[k], part);
+          sum[q] += p0 + i * kWave + lane < packets ? part : 0.0f;
+        }
+      }
+    }
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+#pragma unroll
+      for (int d = 1; d < kWave; d *= 2) sum[q] += __shfl_xor(sum[q], d);
+    }
+    if (lane == 0) {
+      s_low[r] = sum[0];
+      s_low[r + 1] = sum[1];
+    }
+  }
+  __syncthreads();
+  if (low != nullptr) *low = s_low[threadIdx.x];
+  float sum = 0.0f;
+  for (int i0 = 0; i0 < per; i0 += kAhead) {
+    if (i0 > 0) {
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) b[i] = load16(column + min(i0 + i, per - 1) * V);
+    }
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      if (i0 + i >= per) break;
+      float f[V];
+      Pack<T>::unpack(b[i], f);
+#pragma unroll
+      for (int k = 0; k < V; ++k) sum = __builtin_fmaf(s_low[(i0 + i) * V + k], f[k], sum);
+    }
+  }
+  if (c < e.columns) *out = from_float<T>(__builtin_fmaf(scaling, sum, to_float(base)));
+}
+
 // ---- the plan of a gradient: rows sorted by adapter -----------------------------------------------------------------------------
 constexpr int kBlock = 32;          // rows of a block: one step of the matrix core
 constexpr int kPlanThreads = 1024;  // and the most slots
@@ -772,6 +858,15 @@ template <typename T> void expand(const Bank& bank, const Requests& req, Expand 
   else expand_nt<T, 8>(bank, req, e, nt, grid, s);
 }
 
+// Single rows in one launch (step_kernel): workgroups of a row, or 0. For banks of up to 128 KB and up to two workgroups a CU (bf16, calls among others, us,
+// one launch for two: rank 16, 2048 x 2048: 1 row 5.0 for 7.5, 128 rows 5.8 for 8.8; 4096 x 4096: 64 rows 7.3 for 8.7, 128 rows 11.6 for 11.1; rank 64, 4096 x 4096: 1 row
+// 11.0 for 8.8).
+int step_groups(int rows, int slots, bool ragged, int in, int out, int rank, int dtype) {
+  const int groups = (out + kStepThreads - 1) / kStepThreads;
+  const int64_t bank = static_cast<int64_t>(rank) * in * (dtype == LLMQ_F32 ? 4 : 2);
+  return !ragged && slots > 0 && bank <= (128 << 10) && static_cast<int64_t>(rows) * groups <= 512 ? groups : 0;
+}
+
 int64_t round_up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
 int64_t take(int64_t& at, int64_t bytes) {
   const int64_t here = at;
@@ -890,6 +985,18 @@ extern "C" int llmq_lora_add(const void* x, int64_t x_stride, const void* base, 
   const int64_t plane = static_cast<int64_t>(rows) * rank;
   const Expand e{planes, plane, splits, scaling, base, base_stride, out, low_or_null, rows, out_features, 0, 0};
   hipStream_t s = static_cast<hipStream_t>(stream);
+  if (int groups = step_groups(rows, slots, ragged, in_features, out_features, rank, dtype)) {
+    const Expand step{nullptr, 0, 0, scaling, base, base_stride, out, low_or_null, rows, out_features, 0, 0};
+    const Bank bank{lora_a, slots, rank, in_features};
+#define LLMQ_STEP(T)                                                                                                                \
+  hipLaunchKernelGGL((step_kernel<T>), dim3(rows * groups), dim3(kStepThreads), 0, s, static_cast<const T*>(x), x_stride, bank,     \
+                     static_cast<const T*>(lora_b), adapter, step, groups)
+    if (dtype == LLMQ_F32) LLMQ_STEP(float);
+    else if (dtype == LLMQ_F16) LLMQ_STEP(f16_t);
+    else LLMQ_STEP(bf16_t);
+#undef LLMQ_STEP
+    return llmq_host::check_launch("lora_add");
+  }
 #define LLMQ_ADD(T)                                                                                                        \
   shrink<T>(x, x_stride, Bank{lora_a, slots, rank, in_features}, req, planes, plane, splits, ragged, s);                   \
   expand<T>(Bank{lora_b, slots, rank, out_features}, req, e, s)

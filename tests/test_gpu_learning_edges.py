@@ -334,6 +334,27 @@ def test_on_another_stream_and_again(ext, rows):
         assert same(work(), want)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("rows, slots, rank, inp, out", [
+    (1, 2, 16, 2048, 2056), (5, 3, 24, 72, 513 * 8), (64, 48, 16, 4096, 4096), (65, 48, 16, 4096, 4096), (600, 2, 8, 64, 8), (3, 2, 128, 512, 1000),
+    (3, 2, 128, 520, 1000), (2, 1, 8, 8, 8), (11, 5, 40, 1032, 264)])
+def test_single_rows_in_one_launch_and_in_two(ext, rows, slots, rank, inp, out, dtype):
+    adapters = [(5 * b) % (slots + 2) - 1 for b in range(rows)]
+    c = make([1] * rows, adapters, slots, rank, inp, out, dtype, seed=rank, step=True)
+    low = torch.full((rows, rank), NAN, device="cuda")
+    got = call(ext, c, low=low)
+    want, want_low = lora_forward(c, dtype)
+    lora_close(low, want_low, "low")
+    lora_close(got, want, "out")
+    nobody = torch.tensor([not 0 <= a < slots for a in adapters], device="cuda")
+    assert torch.equal(got[nobody], c["base"][nobody]) and (low[nobody] == 0).all()
+    in_place = c["base"].clone()
+    call(ext, dict(c, base=in_place), out=in_place)
+    assert torch.equal(in_place, got)
+    c["x"][nobody] = NAN
+    assert torch.equal(call(ext, c), got)
+
+
 # ---- adapters -----------------------------------------------------------------------------------------------------------------------
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
 def test_rows_of_nobody(ext, dtype):
