@@ -143,8 +143,8 @@ __global__ __launch_bounds__(kFewWaves * kWave) void few_logits_kernel(const Few
   __shared__ __attribute__((aligned(16))) uint8_t s_mem[Few::kLdsBytes];
   const int m0 = blockIdx.x * kFewTokens;
   Few f;
-  f.multiply(s_mem, weight, m0, x);
-  const int lane = threadIdx.x & (kWave - 1), wv = threadIdx.x / kWave, n = wv * 16 + (lane & 15), v0 = 4 * (lane >> 4);
+  f.multiply(s_mem, weight, m0, x + static_cast<int64_t>(blockIdx.y) * 16 * NT * weight.width);
+  const int lane = threadIdx.x & (kWave - 1), wv = threadIdx.x / kWave, n = (blockIdx.y * NT + wv) * 16 + (lane & 15), v0 = 4 * (lane >> 4);
   if (wv >= NT) return;
   float top = -INFINITY;
 #pragma unroll
@@ -299,16 +299,23 @@ __global__ __launch_bounds__(WM * WN * kWave) void piece_kernel(const TileOperan
   }
 }
 
-// P of a few rows: [16 NT, ld], zeros for tokens past the vocabulary up to a multiple of 64
+// P of a few rows: [rows in whole blocks, ld], zeros for tokens past the vocabulary up to a multiple of 64; where the weight learns a second time as
+// [tokens in 64, rows].
+template <typename T> struct FewPiece {
+  T* p;
+  int64_t ld;
+  T* turned;        // or null
+  int turned_ld;
+};
 template <typename T, int BITS, int NT>
-__global__ __launch_bounds__(kFewWaves * kWave) void few_piece_kernel(const FewWeight weight, const T* __restrict__ x, const Counted rows,
-                                                                      T* __restrict__ p, const int64_t ld) {
+__global__ __launch_bounds__(kFewWaves * kWave) void few_piece_kernel(const FewWeight weight, const T* __restrict__ x, const Counted rows, const FewPiece<T> out) {
   using Few = FewRows<T, BITS, NT>;
   __shared__ __attribute__((aligned(16))) uint8_t s_mem[Few::kLdsBytes];
-  const int m0 = blockIdx.x * kFewTokens;
+  const int m0 = blockIdx.x * kFewTokens, t0 = blockIdx.y * 16 * NT;
+  const int lane = threadIdx.x & (kWave - 1), wv = threadIdx.x / kWave, n = t0 + wv * 16 + (lane & 15), v0 = 4 * (lane >> 4);
   Few f;
-  f.multiply(s_mem, weight, m0, x);
-  const int lane = threadIdx.x & (kWave - 1), wv = threadIdx.x / kWave, n = wv * 16 + (lane & 15), v0 = 4 * (lane >> 4);
+  const bool none = t0 >= *rows.count;   // (a block of rows that do not count: zeros)
+  if (!none) f.multiply(s_mem, weight, m0, x + static_cast<int64_t>(blockIdx.y) * 16 * NT * weight.width);
   if (wv >= NT) return;
   const float g = rows.grad[n], lse = rows.lse[n];
   const int64_t target = rows.target[n] - m0;
@@ -318,10 +325,15 @@ __global__ __launch_bounds__(kFewWaves * kWave) void few_piece_kernel(const FewW
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
       const int m = i * 16 + v0 + q;
-      const float value = __builtin_amdgcn_exp2f((f.acc[i][q] - lse) * kLog2e) - (target == m ? 1.0f : 0.0f);
+      const float value = none ? 0.0f : __builtin_amdgcn_exp2f((f.acc[i][q] - lse) * kLog2e) - (target == m ? 1.0f : 0.0f);
       e[q] = g == 0.0f || m0 + m >= weight.rows ? 0.0f : value * g;
+      if (out.turned != nullptr) {
+        T* to = out.turned + static_cast<int64_t>(m0 + m) * out.turned_ld + n;
+        *to = from_float<T>(e[q]);
+        if constexpr (NT == 1 && sizeof(T) == 2) to[16] = from_float<T>(0.0f);   // (a step of 32 rows)
+      }
     }
-    *reinterpret_cast<u32x2*>(p + n * ld + m0 + i * 16 + v0) = u32x2{pair_of<T>(e[0], e[1]), pair_of<T>(e[2], e[3])};
+    store_four(out.p + n * out.ld + m0 + i * 16 + v0, e);
   }
 }
 
@@ -334,9 +346,9 @@ struct Plan {
   int piece;                               // tokens of a piece, a multiple of 256
   int splits;                              // of dh's products
   bool few;                                // rows that go past the weight once, as it lies
-  int row_tiles;                           // of 16, for these: 1, 2 or 4
+  int row_tiles, blocks;                   // of 16, for these: 1, 2 or 4; of 16 row_tiles rows
   // offsets into the workspace
-  int64_t o_stats, o_chosen, o_hidden, o_weight, o_row, o_place, o_target, o_lse, o_grad, o_back, o_x, o_p, o_sums, bytes;
+  int64_t o_stats, o_chosen, o_hidden, o_weight, o_row, o_place, o_target, o_lse, o_grad, o_back, o_x, o_p, o_turned, o_p_turned, o_sums, bytes;
 };
 
 int64_t take(int64_t& at, int64_t bytes) {
@@ -350,8 +362,10 @@ int64_t take(int64_t& at, int64_t bytes) {
 // rows of x 4096 967 and 812). The gradient's are several rounds: how many rows count is not known when a call is made, and there the tiles of those
 // that do not leave room for others (724 of 1024: 1726 us for all products with 768 MB, 1916 with 500, 1932 with 136).
 constexpr int64_t kLossPieceBytes = int64_t{192} << 20, kGradPieceBytes = int64_t{768} << 20;
-// few rows: the whole vocabulary at once, where their P takes no more than 128 MB
+// Few rows: the whole vocabulary at once, up to 2^20 tokens. 64 rows a pass over the weight: one pass where it is as wide as the operands, more where the
+// tiles would have to make operands of it first or take six products.
 constexpr int kFewVocab = 1 << 20;
+constexpr int few_most(int wformat, int dtype) { return dtype == LLMQ_F32 ? 512 : wformat != 0 ? 128 : 64; }
 
 Plan plan_for(int rows, int vocab, int hidden, int group_size, int wformat, int dtype, bool gradient, bool learned) {
   Plan p{};
@@ -380,20 +394,25 @@ Plan plan_for(int rows, int vocab, int hidden, int group_size, int wformat, int 
   }
   p.piece = static_cast<int>(piece);
   int64_t at = 0;
-  p.few = rows <= kFewRows && vocab <= kFewVocab && p.planes == 1 && hidden % (wformat ? 128 : 64) == 0 && (wformat == 0 || group_size % 128 == 0);
+  p.few = rows <= few_most(wformat, dtype) && vocab <= kFewVocab && hidden % (wformat ? 128 : 64) == 0 && (wformat == 0 || group_size % 128 == 0);
   if (p.few) {
     p.row_tiles = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
-    p.stage_hidden = learned;
-    p.stage_weight = false;
+    p.blocks = (rows + 63) / 64;
+    p.stage_hidden = p.stage_weight = false;
     p.piece = static_cast<int>(round_up(vocab, kFewTokens));
-    p.o_x = take(at, int64_t{2} * hidden * 16 * p.row_tiles);
-    if (p.stage_hidden) p.o_hidden = take(at, rows64 * p.k * row16);
+    const int64_t whole_rows = int64_t{16} * p.row_tiles * p.blocks;
+    p.padded = static_cast<int>(round_up(whole_rows, 64));
+    p.o_x = take(at, int64_t{p.size} * hidden * whole_rows);
     if (!gradient) {
       p.o_stats = take(at, round_up(vocab, kFewTokens) / kFewTokens * rows * 8);
       p.o_chosen = take(at, int64_t{4} * rows);
     } else {
       p.splits = few_splits(vocab, hidden, rows, wformat);
-      p.o_p = take(at, int64_t{2} * 16 * p.row_tiles * p.piece);
+      p.o_p = take(at, p.size * whole_rows * p.piece);
+      if (learned) {
+        p.o_turned = take(at, int64_t{p.size} * hidden * p.padded);
+        p.o_p_turned = take(at, int64_t{p.size} * p.padded * p.piece);
+      }
       p.o_sums = take(at, int64_t{4} * p.splits * rows * hidden);
     }
   }
@@ -483,13 +502,13 @@ void loss_launch(const Plan& p, const Call& c, const float2* stats, const float*
 }
 
 FewWeight few_weight(const Plan& p, const Call& c) {
-  const int64_t row_bytes = int64_t{p.hidden} * (c.wformat ? c.wformat : 16) / 8;
+  const int64_t row_bytes = int64_t{p.hidden} * (c.wformat ? c.wformat : 8 * p.size) / 8;
   return FewWeight{static_cast<const uint8_t*>(c.weight), c.wscale, row_bytes, p.vocab, p.hidden, c.wformat ? p.hidden / c.group_size : 0,
                    c.group_size, c.group_size, c.out_group};
 }
 template <typename T> void few_operand(const Plan& p, const Call& c, const int32_t* gather) {
-  const int64_t items = int64_t{p.hidden} / 32 * p.row_tiles * kWave;
-  hipLaunchKernelGGL((few_operand_kernel<T>), dim3(static_cast<unsigned>((items + 255) / 256)), dim3(256), 0, c.stream, static_cast<const T*>(c.hidden),
+  const int64_t items = int64_t{p.hidden} / (4 * kFewPack<T>) * p.row_tiles * kWave;
+  hipLaunchKernelGGL((few_operand_kernel<T>), dim3(static_cast<unsigned>((items + 255) / 256), p.blocks), dim3(256), 0, c.stream, static_cast<const T*>(c.hidden),
                      c.hidden_stride, gather, p.rows, p.hidden, p.row_tiles, reinterpret_cast<T*>(c.workspace + p.o_x));
 }
 #define LLMQ_FEW_NT(KERNEL, BITS, ...)                                                                                        \
@@ -508,7 +527,7 @@ template <typename T> int few_forward(const Plan& p, const Call& c, const int64_
   float* chosen = reinterpret_cast<float*>(c.workspace + p.o_chosen);
   const T* x = reinterpret_cast<const T*>(c.workspace + p.o_x);
   const FewWeight weight = few_weight(p, c);
-  const dim3 grid((p.vocab + kFewTokens - 1) / kFewTokens);
+  const dim3 grid((p.vocab + kFewTokens - 1) / kFewTokens, p.blocks);
   LLMQ_FEW(few_logits_kernel, weight, x, rows, stats, chosen)
   loss_launch(p, c, stats, chosen, static_cast<int>(grid.x), rows, ignore_index, losses, lse);
   return llmq_host::check_launch("vocab_loss");
@@ -529,24 +548,35 @@ void weight_gradient(const Plan& p, const Call& c, const TileOperand& part, int 
 template <typename T>
 int few_backward(const Plan& p, const Call& c, const Counted& rows, void* grad_hidden, void* grad_weight) {
   few_operand<T>(p, c, rows.row);
-  if (p.stage_hidden) stage_hidden<T>(p, c, rows.row);
   const T* x = reinterpret_cast<const T*>(c.workspace + p.o_x);
-  T* part = reinterpret_cast<T*>(c.workspace + p.o_p);
+  const bool learned = grad_weight != nullptr;
+  const FewPiece<T> part{reinterpret_cast<T*>(c.workspace + p.o_p), p.piece, learned ? reinterpret_cast<T*>(c.workspace + p.o_p_turned) : nullptr, p.padded};
   float* sums = reinterpret_cast<float*>(c.workspace + p.o_sums);
   const FewWeight weight = few_weight(p, c);
-  const dim3 grid((p.vocab + kFewTokens - 1) / kFewTokens);
-  LLMQ_FEW(few_piece_kernel, weight, x, rows, part, int64_t{p.piece})
-  columns_launch<T>(weight, FewColumns{part, p.piece, rows.count, p.rows, sums, p.splits}, c.wformat, c.stream);
-  if (grad_weight != nullptr)   // (rows of P behind its last: that one again, against zeros of the hidden rows)
-    weight_gradient<T>(p, c, TileOperand{part, 0, int64_t{2} * p.piece, 0, 16 * p.row_tiles}, 0, p.vocab, rows.back, rows.count, grad_weight);
+  const unsigned tokens = (p.vocab + kFewTokens - 1) / kFewTokens;
+  const dim3 grid(tokens, p.blocks);
+  LLMQ_FEW(few_piece_kernel, weight, x, rows, part)
+  columns_launch<T, true>(weight, FewColumns{part.p, part.ld, rows.count, p.rows, sums, p.splits}, c.wformat, c.stream);
+  if (learned) {
+    T* turned = reinterpret_cast<T*>(c.workspace + p.o_turned);
+    const int steps = (p.rows + 4 * kFewPack<T> - 1) / (4 * kFewPack<T>);
+    const int64_t items = int64_t{p.hidden} / 16 * steps * kWave;
+    hipLaunchKernelGGL((few_turned_kernel<T>), dim3(static_cast<unsigned>((items + 255) / 256)), dim3(256), 0, c.stream, static_cast<const T*>(c.hidden),
+                       c.hidden_stride, rows.row, p.rows, p.hidden, steps, turned);
+    const dim3 outer(tokens, 1);
+    if (p.blocks == 1)
+      hipLaunchKernelGGL((few_outer_kernel<T, true>), outer, dim3(kFewWaves * kWave), 0, c.stream, part.turned, int64_t{p.padded}, turned, steps, rows.back, p.vocab,
+                         p.hidden, static_cast<T*>(grad_weight));
+    else
+      hipLaunchKernelGGL((few_outer_kernel<T, false>), outer, dim3(kFewWaves * kWave), 0, c.stream, part.turned, int64_t{p.padded}, turned, steps, rows.back, p.vocab,
+                         p.hidden, static_cast<T*>(grad_weight));
+  }
   add_few_launch<T>(sums, p.splits, p.rows, p.hidden, rows.back, rows.place, grad_hidden, c.stream);
   return llmq_host::check_launch("vocab_loss_grad");
 }
 
 template <typename T> int forward(const Plan& p, const Call& c, const int64_t* targets, int64_t ignore_index, float* losses, float* lse, int dtype) {
-  if constexpr (sizeof(T) == 2) {
-    if (p.few) return few_forward<T>(p, c, targets, ignore_index, losses, lse);
-  }
+  if (p.few) return few_forward<T>(p, c, targets, ignore_index, losses, lse);
   if (p.stage_hidden) stage_hidden<T>(p, c, nullptr);
   const TileOperand hidden = hidden_operand(p, c);
   const LossRows rows{targets, p.rows, p.vocab};
@@ -578,9 +608,7 @@ int backward(const Plan& p, const Call& c, const int64_t* targets, int64_t ignor
   const bool learned = grad_weight != nullptr;
   const int rows64 = static_cast<int>(round_up(p.rows, 64));
   hipLaunchKernelGGL(count_rows_kernel, dim3(1), dim3(1024), 0, c.stream, grad, targets, lse, p.rows, p.padded, p.vocab, ignore_index, rows);
-  if constexpr (sizeof(T) == 2) {
-    if (p.few) return few_backward<T>(p, c, rows, grad_hidden, grad_weight);
-  }
+  if (p.few) return few_backward<T>(p, c, rows, grad_hidden, grad_weight);
   stage_hidden<T>(p, c, rows.row);
   const TileOperand hidden = hidden_operand(p, c);
   const int tn = tile_rows(p.rows), n_tiles = p.padded / tn;

@@ -28,7 +28,7 @@ constexpr int kFewMost = 256;
 Plan plan_for(int rows, int N, int width, int wformat, int dtype) {
   Plan p{};
   const int64_t row16 = dtype == LLMQ_F32 ? 6 : 2;
-  p.few = dtype != LLMQ_F32 && rows <= kFewMost;
+  p.few = rows <= kFewMost;
   if (p.few) {
     p.splits = few_splits(N, width, rows, wformat);
     p.bytes = int64_t{4} * p.splits * rows * width;
@@ -58,14 +58,12 @@ template <typename T>
 int launch(const Plan& p, const void* grad, int64_t stride, const void* qweight, const float* wscale, void* out, uint8_t* workspace, int rows,
            int N, int G, int gs, int keep, int out_group, int wformat, int dtype, hipStream_t stream) {
   constexpr int P = TileType<T>::kPlanes;
-  if constexpr (P == 1) {
-    if (p.few) {
-      float* sums = reinterpret_cast<float*>(workspace);
-      columns_launch<T>(FewWeight{static_cast<const uint8_t*>(qweight), wscale, static_cast<int64_t>(G) * gs * wformat / 8, N, G * keep, G, gs, keep, out_group},
-                        FewColumns{grad, stride, nullptr, rows, sums, p.splits}, wformat, stream);
-      add_few_launch<T>(sums, p.splits, rows, G * keep, nullptr, nullptr, out, stream);
-      return llmq_host::check_launch("wq_linear_grad");
-    }
+  if (p.few) {
+    float* sums = reinterpret_cast<float*>(workspace);
+    columns_launch<T, false>(FewWeight{static_cast<const uint8_t*>(qweight), wscale, static_cast<int64_t>(G) * gs * wformat / 8, N, G * keep, G, gs, keep, out_group},
+                      FewColumns{grad, stride, nullptr, rows, sums, p.splits}, wformat, stream);
+    add_few_launch<T>(sums, p.splits, rows, G * keep, nullptr, nullptr, out, stream);
+    return llmq_host::check_launch("wq_linear_grad");
   }
   const int width = G * keep, n64 = static_cast<int>(p.n_padded);
   if (p.stage_grad)   // (zeros up to a whole step, against rows of W that are looked at again)

@@ -9,10 +9,9 @@ from test_gpu_lora import backward as lora_backward
 from test_gpu_lora import call, call_grad, make
 from test_gpu_lora import close as lora_close
 from test_gpu_lora import forward as lora_forward
-from test_gpu_vocab_loss import U, case, close, dense_of, expected, quantized, sum_error
+from test_gpu_vocab_loss import DTYPES, U, case, close, dense_of, expected, quantized, sum_error
 
 pytestmark = pytest.mark.gpu
-HALVES = [torch.bfloat16, torch.float16]
 NAN = float("nan")
 
 
@@ -54,11 +53,13 @@ def replays(work, change, outputs_of, times=3):
 
 
 # ---- few rows -------------------------------------------------------------------------------------------------------------------
-@pytest.mark.parametrize("dtype", HALVES)
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("bits", [0, 8, 4])
 @pytest.mark.parametrize("rows, vocab, width, group, out_group", [
     (1, 1, 128, 128, 0), (1, 63, 256, 128, 0), (16, 64, 128, 128, 0), (17, 1000, 384, 384, 0), (33, 2049, 256, 128, 0), (64, 5003, 512, 256, 0),
-    (48, 129, 1024, 128, 64), (31, 8191, 256, 128, 100), (2, 70001, 128, 128, 0)])
+    (48, 129, 1024, 128, 64), (31, 8191, 256, 128, 100), (2, 70001, 128, 128, 0),
+    (65, 700, 192, 64, 0), (100, 3001, 256, 256, 0), (128, 515, 384, 128, 7), (129, 515, 384, 128, 0), (300, 130, 128, 128, 0), (512, 333, 256, 128, 0),
+    (513, 333, 256, 128, 0)])
 def test_few_rows(ext, rows, vocab, width, group, out_group, bits, dtype):
     c = case(rows, vocab, width, dtype, bits, rows * vocab, group, out_group if bits else 0)
     hidden, weight, scale, dense, targets, grad = c
@@ -72,7 +73,7 @@ def test_few_rows(ext, rows, vocab, width, group, out_group, bits, dtype):
     assert (dh[targets == -100] == 0).all() and (losses[targets == -100] == 0).all()
 
 
-@pytest.mark.parametrize("dtype", HALVES)
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("rows, out, width, bits, group, keep, out_group", [
     (1, 4104, 256, 8, 128, 128, 0), (16, 24, 128, 4, 8, 8, 0), (17, 136, 384, 8, 128, 72, 0), (33, 1032, 128, 4, 128, 128, 100), (48, 8, 2048, 8, 64, 64, 0),
     (128, 2056, 256, 4, 256, 256, 0), (129, 520, 136, 8, 8, 8, 3), (256, 264, 1024, 8, 128, 128, 0), (257, 264, 1024, 8, 128, 128, 0)])
