@@ -247,7 +247,7 @@ struct FewColumns {
 // A workgroup: 128 columns, 16 NT rows of g (blockIdx.y), a part of the weight's rows, which its waves take 32 (fp32: 16) at a time; each lane
 // eight columns of eight (four) rows, turned over in registers, a step ahead. The waves' sums meet in LDS.
 template <typename T, int BITS, int NT>
-__global__ __launch_bounds__(kFewWaves * kWave) void columns_kernel(const FewWeight w, const FewColumns c) {
+__global__ __launch_bounds__(kFewWaves * kWave, 2) void columns_kernel(const FewWeight w, const FewColumns c) {
   constexpr int V = kFewPack<T>, kWords = BITS == 0 ? 2 * sizeof(T) : BITS / 4, kRows = 4 * V;   // words of eight values; rows of a step
   constexpr bool kHalves = sizeof(T) == 4 && BITS == 0;   // a lane's columns: 4 lr .. and 64 + 4 lr .., whole lines of 16 lanes
   __shared__ tile_v4f s_sum[2][NT * 8][kWave];
@@ -331,13 +331,15 @@ __global__ __launch_bounds__(kFewWaves * kWave) void columns_kernel(const FewWei
       for (int j = 0; j < NT; ++j) acc[j][q] = few_mfma<T>(now.g[j], operand, acc[j][q]);
     }
   };
-  if (begin < v1) {
-    Asked next;
-    ask(begin, next);
-    for (int v = begin; v < v1; v += step) {
-      Asked now = next;
-      ask(min(v + step, v1 - kRows), next);   // (behind the last step: the part's last again)
-      use(v, now);
+  if (begin < v1) {   // (behind the last step: the part's last again)
+    Asked a, b;
+    ask(begin, a);
+    for (int v = begin; v < v1; v += 2 * step) {
+      ask(min(v + step, v1 - kRows), b);
+      use(v, a);
+      if (v + step >= v1) break;
+      ask(min(v + 2 * step, v1 - kRows), a);
+      use(v + step, b);
     }
   }
   if (wv >= 2) {
@@ -374,14 +376,14 @@ __global__ __launch_bounds__(kFewWaves * kWave) void columns_kernel(const FewWei
     }
 }
 // Splits of the weight's rows, 64 at the most. For 256 workgroups: more are only more planes (4096 x 4096 int8, 64 rows: 17 us with 256, 26 with 512, 39
-// with 1024; 16 rows: 9, 11 and 13), but for 512 where conversion binds and a wave still has 32 steps (128256 x 2048, 16 rows: int8 66 -> 56, int4 58 -> 48; as
-// they are 88 -> 93).
-inline int few_splits(int weight_rows, int width, int rows, int bits) {
+// with 1024; 16 rows: 9, 11 and 13). More where conversion or the fp32 matrix core binds and a wave still has 32 steps (128256 x 2048, 16 rows: int8 256 66 us, 512 56;
+// int4 58 and 48; bf16 88 and 93; fp32, 8 rows: 256 396, 512 252, 1024 190; 64 rows: 447, 423, 416).
+inline int few_splits(int weight_rows, int width, int rows, int bits, bool fp32) {
   const int64_t groups = static_cast<int64_t>((width + kFewColumns - 1) / kFewColumns) * ((rows + 63) / 64), step = 32 * kFewWaves;
   const int64_t most = (weight_rows + step - 1) / step;
-  int64_t splits = 256 / groups;
-  if (bits != 0 && rows <= 32 && most >= 512 / groups * 32) splits = 512 / groups;
-  if (splits > most) splits = most;
+  int64_t places = fp32 ? (rows <= 32 ? 1024 : 512) : bits != 0 && rows <= 32 ? 512 : 256;
+  while (places > 256 && most < places / groups * 32) places /= 2;
+  const int64_t splits = places / groups < most ? places / groups : most;
   return static_cast<int>(splits < 1 ? 1 : splits > 64 ? 64 : splits);
 }
 template <typename T, int BITS> inline void columns_launch_bits(const FewWeight& w, const FewColumns& c, hipStream_t stream) {

@@ -137,7 +137,7 @@ __global__ __launch_bounds__(1024) void loss_kernel(const float2* __restrict__ s
 
 // A few rows: 64 tokens a workgroup, a row tile of the sums a wave.
 template <typename T, int BITS, int NT>
-__global__ __launch_bounds__(kFewWaves * kWave) void few_logits_kernel(const FewWeight weight, const T* __restrict__ x, const LossRows rows,
+__global__ __launch_bounds__(kFewWaves * kWave, BITS != 0 && NT == 4 ? 1 : 2) void few_logits_kernel(const FewWeight weight, const T* __restrict__ x, const LossRows rows,
                                                                        float2* __restrict__ stats, float* __restrict__ chosen) {
   using Few = FewRows<T, BITS, NT>;
   __shared__ __attribute__((aligned(16))) uint8_t s_mem[Few::kLdsBytes];
@@ -308,7 +308,7 @@ template <typename T> struct FewPiece {
   int turned_ld;
 };
 template <typename T, int BITS, int NT>
-__global__ __launch_bounds__(kFewWaves * kWave) void few_piece_kernel(const FewWeight weight, const T* __restrict__ x, const Counted rows, const FewPiece<T> out) {
+__global__ __launch_bounds__(kFewWaves * kWave, BITS != 0 && NT == 4 ? 1 : 2) void few_piece_kernel(const FewWeight weight, const T* __restrict__ x, const Counted rows, const FewPiece<T> out) {
   using Few = FewRows<T, BITS, NT>;
   __shared__ __attribute__((aligned(16))) uint8_t s_mem[Few::kLdsBytes];
   const int m0 = blockIdx.x * kFewTokens, t0 = blockIdx.y * 16 * NT;
@@ -363,9 +363,10 @@ int64_t take(int64_t& at, int64_t bytes) {
 // that do not leave room for others (724 of 1024: 1726 us for all products with 768 MB, 1916 with 500, 1932 with 136).
 constexpr int64_t kLossPieceBytes = int64_t{192} << 20, kGradPieceBytes = int64_t{768} << 20;
 // Few rows: the whole vocabulary at once, up to 2^20 tokens. 64 rows a pass over the weight: one pass where it is as wide as the operands, more where the
-// tiles would have to make operands of it first or take six products.
+// tiles would have to make operands of it first or take six products (128256 x 2048: int8 in bf16, 128 rows 209 us for 337, 192 rows 353 for 350; fp32, 512 rows 2657
+// for 2777, with both gradients 256 rows 6355 for 6950, 512 rows 12600 for 7989).
 constexpr int kFewVocab = 1 << 20;
-constexpr int few_most(int wformat, int dtype) { return dtype == LLMQ_F32 ? 512 : wformat != 0 ? 128 : 64; }
+constexpr int few_most(int wformat, int dtype, bool gradient) { return dtype == LLMQ_F32 ? (gradient ? 256 : 512) : wformat != 0 ? 128 : 64; }
 
 Plan plan_for(int rows, int vocab, int hidden, int group_size, int wformat, int dtype, bool gradient, bool learned) {
   Plan p{};
@@ -394,7 +395,7 @@ Plan plan_for(int rows, int vocab, int hidden, int group_size, int wformat, int 
   }
   p.piece = static_cast<int>(piece);
   int64_t at = 0;
-  p.few = rows <= few_most(wformat, dtype) && vocab <= kFewVocab && hidden % (wformat ? 128 : 64) == 0 && (wformat == 0 || group_size % 128 == 0);
+  p.few = rows <= few_most(wformat, dtype, gradient) && vocab <= kFewVocab && hidden % (wformat ? 128 : 64) == 0 && (wformat == 0 || group_size % 128 == 0);
   if (p.few) {
     p.row_tiles = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
     p.blocks = (rows + 63) / 64;
@@ -407,7 +408,7 @@ Plan plan_for(int rows, int vocab, int hidden, int group_size, int wformat, int 
       p.o_stats = take(at, round_up(vocab, kFewTokens) / kFewTokens * rows * 8);
       p.o_chosen = take(at, int64_t{4} * rows);
     } else {
-      p.splits = few_splits(vocab, hidden, rows, wformat);
+      p.splits = few_splits(vocab, hidden, rows, wformat, dtype == LLMQ_F32);
       p.o_p = take(at, p.size * whole_rows * p.piece);
       if (learned) {
         p.o_turned = take(at, int64_t{p.size} * hidden * p.padded);

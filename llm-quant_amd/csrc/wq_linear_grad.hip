@@ -30,7 +30,7 @@ Plan plan_for(int rows, int N, int width, int wformat, int dtype) {
   const int64_t row16 = dtype == LLMQ_F32 ? 6 : 2;
   p.few = rows <= kFewMost;
   if (p.few) {
-    p.splits = few_splits(N, width, rows, wformat);
+    p.splits = few_splits(N, width, rows, wformat, dtype == LLMQ_F32);
     p.bytes = int64_t{4} * p.splits * rows * width;
     return p;
   }
