@@ -60,6 +60,42 @@ template <int BITS> struct Codes {
   }
 };
 
+// Four values of a row of the weight from column c on (a multiple of four), as the products have them.
+template <typename T> __device__ __forceinline__ void weight_four(const FewWeight& w, const int bits, const int row, const int c, float* f) {
+  const uint8_t* from = w.base + row * w.row_bytes;
+  if (bits == 0) {
+    const T* at = reinterpret_cast<const T*>(from) + c;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) f[i] = to_float(at[i]);
+    return;
+  }
+  const float scale = w.scale[w.scale_row(row) + c / w.group_size];
+  if (bits == 8) {
+    const uint32_t codes = *reinterpret_cast<const uint32_t*>(from + c);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) f[i] = to_float(from_float<T>(static_cast<float>(static_cast<int8_t>(codes >> (8 * i))) * scale));
+  } else {
+    const int codes = *reinterpret_cast<const uint16_t*>(from + c / 2);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) f[i] = to_float(from_float<T>(static_cast<float>((codes >> (4 * i) & 15) - 8) * scale));
+  }
+}
+// What rounding took from the entry of a row's own target, by far the largest of its row of P as a rule: added to the results in fp32.
+struct TargetTerm {
+  const float* rest;        // [rows], or null: nothing
+  const int64_t* target;    // [rows], in the vocabulary where `rest` is not zero
+  FewWeight weight;
+  int bits;
+  template <typename T> __device__ __forceinline__ void add(const int row, const int c, float* f) const {
+    const float by = rest[row];
+    if (by == 0.0f) return;
+    float v[4];
+    weight_four<T>(weight, bits, static_cast<int>(target[row]), c, v);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) f[i] = __builtin_fmaf(by, v[i], f[i]);
+  }
+};
+
 // ---- x in operand order -------------------------------------------------------------------------------------------------------
 // [block of 16 `tiles` rows][k / 4 V][tile of 16 rows][lane][V values]: lane 16 g + r holds values 4 V k + V g .. of row 16 tile + r; zeros past the rows and
 // where `gather` has none. V: a packet's.
@@ -403,7 +439,8 @@ template <typename T, bool DENSE> inline void columns_launch(const FewWeight& w,
 // out[row] = (dtype)(scale * the sum of the planes' row `from[row]`); no such row (negative): zeros
 template <typename T>
 __global__ __launch_bounds__(256) void add_few_kernel(const float* __restrict__ planes, const int splits, const int rows, const int width,
-                                                      const float* __restrict__ scale_or_null, const int32_t* __restrict__ from_or_null, T* __restrict__ out) {
+                                                      const float* __restrict__ scale_or_null, const int32_t* __restrict__ from_or_null, const TargetTerm term,
+                                                      T* __restrict__ out) {
   constexpr int kAhead = 8;
   const int64_t item = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x, items = static_cast<int64_t>(rows) * (width / 4);
   if (item >= items) return;
@@ -423,22 +460,34 @@ __global__ __launch_bounds__(256) void add_few_kernel(const float* __restrict__ 
     }
   }
   const float scale = scale_or_null != nullptr ? *scale_or_null : 1.0f;
-  const float f[4] = {sum[0] * scale, sum[1] * scale, sum[2] * scale, sum[3] * scale};
+  float f[4] = {sum[0], sum[1], sum[2], sum[3]};
+  if (from >= 0 && term.rest != nullptr) term.add<T>(from, c, f);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) f[i] *= scale;
   store_four(out + static_cast<int64_t>(row) * width + c, f);
 }
 template <typename T>
-inline void add_few_launch(const float* planes, int splits, int rows, int width, const float* scale, const int32_t* from, void* out, hipStream_t stream) {
+inline void add_few_launch(const float* planes, int splits, int rows, int width, const float* scale, const int32_t* from, const TargetTerm& term, void* out,
+                           hipStream_t stream) {
   const int64_t items = static_cast<int64_t>(rows) * (width / 4);
-  hipLaunchKernelGGL((add_few_kernel<T>), dim3(static_cast<unsigned>((items + 255) / 256)), dim3(256), 0, stream, planes, splits, rows, width, scale, from,
+  hipLaunchKernelGGL((add_few_kernel<T>), dim3(static_cast<unsigned>((items + 255) / 256)), dim3(256), 0, stream, planes, splits, rows, width, scale, from, term,
                      static_cast<T*>(out));
 }
 
 // ---- the reduction over the few rows ----------------------------------------------------------------------------------------------
 // out[v, k] = scale * sum_t P[v, t] x[t, k] for 64 rows of the result a workgroup, 64 columns a wave at a time. p: [rows in 64, ld], zeros for rows of x that are
-// none; turned: few_turned_kernel's. ONE: all of P's packets stay in registers (up to 64 rows of x).
+// none; turned: few_turned_kernel's. ONE: all of P's packets stay in registers (up to 64 rows of x). 16 bits: up to 64 rows, whose targets' rests are added.
+struct FewRests {
+  const float* rest;
+  const int64_t* target;
+  const int32_t *row, *count;   // of x
+  const void* x;
+  int64_t stride;
+};
 template <typename T, bool ONE>
 __global__ __launch_bounds__(kFewWaves * kWave) void few_outer_kernel(const T* __restrict__ p, const int64_t ld, const T* __restrict__ turned, const int steps,
-                                                                      const float* __restrict__ scale, const int rows, const int width, T* __restrict__ out) {
+                                                                      const float* __restrict__ scale, const int rows, const int width, const FewRests rests,
+                                                                      T* __restrict__ out) {
   constexpr int V = kFewPack<T>, kSteps = 64 / (4 * V);
   const int lane = threadIdx.x & (kWave - 1), wv = threadIdx.x / kWave, lr = lane & 15, g = lane >> 4;
   const int v0 = blockIdx.x * kFewTokens;
@@ -450,6 +499,17 @@ __global__ __launch_bounds__(kFewWaves * kWave) void few_outer_kernel(const T* _
     for (int k = 0; k < kSteps; ++k)
 #pragma unroll
       for (int n = 0; n < 4; ++n) held[k][n] = load16(from + n * 16 * ld + min(k, steps - 1) * 4 * V);
+  }
+  uint64_t here = 0;   // rows whose target is among the workgroup's
+  int target = 0;
+  if constexpr (sizeof(T) == 2) {
+    if (lane < *rests.count) {
+      const int64_t at = rests.target[lane] - v0;
+      target = at >= 0 && at < kFewTokens && rests.rest[lane] != 0.0f ? static_cast<int>(at) : -1;
+    } else {
+      target = -1;
+    }
+    here = __ballot(target >= 0);
   }
   for (int c0 = (blockIdx.y * kFewWaves + wv) * 64; c0 < width; c0 += gridDim.y * kFewWaves * 64) {
     tile_v4f acc[4][4] = {};
@@ -474,6 +534,20 @@ __global__ __launch_bounds__(kFewWaves * kWave) void few_outer_kernel(const T* _
         for (int n = 0; n < 4; ++n) b[n] = load16(from + n * 16 * ld + k * 4 * V);
         multiply(k, b);
       }
+    }
+    for (uint64_t left = here; left != 0; left &= left - 1) {
+      const int t = __builtin_ctzll(left), at = __builtin_amdgcn_readlane(target, t);
+      const T* from = static_cast<const T*>(rests.x) + rests.row[t] * rests.stride + c0;
+      const float by = lr == (at & 15) ? rests.rest[t] : 0.0f;
+#pragma unroll
+      for (int m = 0; m < 4; ++m)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float add = by * to_float(from[(m >> 1) * 32 + 8 * g + 4 * (m & 1) + i]);
+#pragma unroll
+          for (int n = 0; n < 4; ++n)
+            if (n == at >> 4) acc[m][n][i] += lr == (at & 15) ? add : 0.0f;
+        }
     }
 #pragma unroll
     for (int n = 0; n < 4; ++n) {

@@ -4,7 +4,7 @@
 // llmquant/quantizers/kernel.py:68-79). And products whose result is a tensor.
 #pragma once
 
-#include "dense_tile.h"
+#include "dense_few.h"
 
 namespace llmq {
 
@@ -163,6 +163,12 @@ struct ProductOut {
   const float* scale;
   int first, most;     // most: splits
   const int32_t* count = nullptr;   // or null: how many rows (of B, or with B_K of K) there are; tiles and steps past them are left out
+  // B_K, 16 bits: what is added for row t of K to the result's row target[t] - first_token, rest[t] times row `row[t]` of x; null: nothing
+  const float* rest = nullptr;
+  const int64_t* target = nullptr;
+  const int32_t* row = nullptr;
+  const void* x = nullptr;
+  int64_t x_stride = 0, first_token = 0;
 };
 
 template <typename T, int TM, int TN, int WM, int WN, bool SUMS, bool B_K>
@@ -187,6 +193,71 @@ __global__ __launch_bounds__(WM * WN * kWave) void product_kernel(const TileOper
   Tile t;
   if (k0 < k1) t.template multiply<(TileType<T>::kPlanes == 3 ? 6 : 1)>(s_mem, a, m0, b, n0, k0, k1);
   else t.clear();
+  if constexpr (!SUMS && B_K && sizeof(T) == 2) {
+    // the rows of K whose target is one of the tile's, in their order, 2048 rows a time, and of those 32 a product
+    constexpr int kEach = 4, kThreads = WM * WN * kWave;
+    struct Rest {
+      int row, n;
+      float by;
+    };
+    Rest* const list = reinterpret_cast<Rest*>(s_mem);
+    int* const found = reinterpret_cast<int*>(list + kEach * kThreads);   // [kEach][waves]
+    const int lane = threadIdx.x & (kWave - 1), wv = threadIdx.x / kWave, lr = lane & 15, g = lane >> 4;
+    const int last = min(k, rows) - 1;
+    for (int i0 = 0; out.rest != nullptr && i0 <= last; i0 += kEach * kThreads) {
+      uint64_t hit[kEach];
+      Rest mine[kEach];
+      __syncthreads();
+#pragma unroll
+      for (int j = 0; j < kEach; ++j) {
+        const int i = i0 + j * kThreads + threadIdx.x, at = min(i, last);
+        const int64_t n = out.target[at] - out.first_token - n0;
+        mine[j] = Rest{out.row[at], static_cast<int>(n), out.rest[at]};
+        hit[j] = __ballot(i == at && n >= 0 && n < TN && mine[j].by != 0.0f);
+        if (lane == 0) found[j * WM * WN + wv] = __popcll(hit[j]);
+      }
+      __syncthreads();
+      int all = 0;
+#pragma unroll
+      for (int j = 0; j < kEach; ++j) {
+        int first = all;
+        for (int w = 0; w < WM * WN; ++w) {
+          if (w < wv) first += found[j * WM * WN + w];
+          all += found[j * WM * WN + w];
+        }
+        if (hit[j] >> lane & 1) list[first + __popcll(hit[j] & ((uint64_t{1} << lane) - 1))] = mine[j];
+      }
+      __syncthreads();
+      for (int e0 = 0; e0 < all; e0 += 32) {   // lane 16 g + r: rows 8 g .. of the 32, of A's and B's r
+        Rest of[8];
+        uint32_t word[4];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          of[e] = list[min(e0 + 8 * g + e, all - 1)];
+          if (e0 + 8 * g + e >= all) of[e].n = -1;
+        }
+        u32x4 x[Tile::MI];
+#pragma unroll
+        for (int mi = 0; mi < Tile::MI; ++mi) {
+          const T* from = static_cast<const T*>(out.x) + min(m0 + wv / WN * (TM / WM) + mi * 16 + lr, a.rows - 1);
+          uint16_t v[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) v[e] = __builtin_bit_cast(uint16_t, from[of[e].row * out.x_stride]);
+          x[mi] = u32x4{v[0] | static_cast<uint32_t>(v[1]) << 16, v[2] | static_cast<uint32_t>(v[3]) << 16, v[4] | static_cast<uint32_t>(v[5]) << 16,
+                        v[6] | static_cast<uint32_t>(v[7]) << 16};
+        }
+#pragma unroll
+        for (int ni = 0; ni < Tile::NI; ++ni) {
+          const int n = wv % WN * (TN / WN) + ni * 16 + lr;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) word[e] = pair_of<T>(of[2 * e].n == n ? of[2 * e].by : 0.0f, of[2 * e + 1].n == n ? of[2 * e + 1].by : 0.0f);
+          const u32x4 by{word[0], word[1], word[2], word[3]};
+#pragma unroll
+          for (int mi = 0; mi < Tile::MI; ++mi) t.acc[mi][ni] = mfma_16x16x32<T>(x[mi], by, t.acc[mi][ni]);
+        }
+      }
+    }
+  }
   const float scale = SUMS || out.scale == nullptr ? 1.0f : *out.scale;
 #pragma unroll
   for (int ni = 0; ni < Tile::NI; ++ni) {
@@ -232,7 +303,8 @@ inline void product_launch(const TileOperand& a, const TileOperand& b, int k, co
 template <typename T>
 __global__ __launch_bounds__(256) void add_planes_kernel(const float* __restrict__ planes, const int rows, const int tn, const int m_tiles, const int most,
                                                          const int32_t* __restrict__ count_or_null, const float* __restrict__ scale_or_null,
-                                                         const int32_t* __restrict__ from_or_null, T* __restrict__ out, const int64_t packets, const int per_row) {
+                                                         const int32_t* __restrict__ from_or_null, const TargetTerm term, T* __restrict__ out,
+                                                         const int64_t packets, const int per_row) {
   constexpr int kAhead = 4;
   const Splits s = splits_of_rows(count_or_null == nullptr ? rows : min(rows, *count_or_null), tn, m_tiles, per_row * int64_t{8}, most);
   const int64_t plane = s.plane;
@@ -241,9 +313,10 @@ __global__ __launch_bounds__(256) void add_planes_kernel(const float* __restrict
   for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < packets; i += static_cast<int64_t>(gridDim.x) * 256) {
     float f[8] = {};
     int64_t at = i;
+    int from = -1;
     if (from_or_null != nullptr) {
       const int64_t row = i / per_row;
-      const int from = from_or_null[row];
+      from = from_or_null[row];
       at = from < 0 ? -1 : from * static_cast<int64_t>(per_row) + (i - row * per_row);
     }
     if (at >= 0) {
@@ -265,6 +338,11 @@ __global__ __launch_bounds__(256) void add_planes_kernel(const float* __restrict
             }
       }
     }
+    if (term.rest != nullptr && from >= 0) {   // (with `from` alone)
+      const int c = static_cast<int>(i % per_row) * 8;
+      term.add<T>(from, c, f);
+      term.add<T>(from, c + 4, f + 4);
+    }
 #pragma unroll
     for (int e = 0; e < 8; ++e) f[e] *= scale;
 #pragma unroll
@@ -273,11 +351,11 @@ __global__ __launch_bounds__(256) void add_planes_kernel(const float* __restrict
 }
 // (rows and most as the products had them)
 template <typename T>
-inline void add_planes_launch(const float* planes, int rows, int width, int most, const int32_t* count, const float* scale, const int32_t* from, void* out,
-                              hipStream_t stream) {
+inline void add_planes_launch(const float* planes, int rows, int width, int most, const int32_t* count, const float* scale, const int32_t* from,
+                              const TargetTerm& term, void* out, hipStream_t stream) {
   const int64_t packets = static_cast<int64_t>(rows) * (width / 8), blocks = (packets + 255) / 256;
   hipLaunchKernelGGL((add_planes_kernel<T>), dim3(static_cast<unsigned>(blocks < 8192 ? blocks : 8192)), dim3(256), 0, stream,
-                     planes, rows, tile_rows(rows), (width + 255) / 256, most, count, scale, from, static_cast<T*>(out), packets, width / 8);
+                     planes, rows, tile_rows(rows), (width + 255) / 256, most, count, scale, from, term, static_cast<T*>(out), packets, width / 8);
 }
 
 inline int64_t round_up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }

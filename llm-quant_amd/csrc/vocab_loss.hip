@@ -8,11 +8,12 @@
 // summed in fp32, of which the largest and the sum of exponentials per row, and the target's own, go to memory: 8 bytes for 256
 // logits. The loss is the log of the sum plus (largest - target's), so that a token that the model is sure of keeps its digits.
 // The gradient goes over pieces of the vocabulary: the tile is multiplied again, and what is written is P of the piece in the type of the
-// call (fp32: three planes), as the operand of the two products behind it. P is rounded to that type, relative to each value; g is scaled
-// by a power of two first, so that a mean over many rows does not leave fp16's range, and the results are scaled back.
-// A quantized head (the model's lm_head) is brought to the values of its dense form piece by piece. Up to 64 rows of 16 bits go past the weight
-// as it lies instead, dense or codes (dense_few.h; 16 rows of 128256 x 2048, bf16: the tiles' kernel 115 us, this one 87, 6.0 TB/s).
-#include "dense_few.h"
+// call (fp32: three planes), as the operand of the two products behind it. P is rounded to that type, relative to each value; what that takes from the
+// entry of the row's target, nearly all of a row where the others share what is left, is kept in fp32 and added to the results (with it rounded away
+// gradients are 2^-8 off where their own rounding is 2^-9; 2000 rows of 32000 x 2048, the weight's gradient 329 -> 352 us); g is scaled by a power of two
+// first, so that a mean over many rows does not leave fp16's range, and the results are scaled back.
+// A quantized head (the model's lm_head) is brought to the values of its dense form piece by piece. Few rows (few_most) go past the weight as it lies
+// instead, dense or codes (dense_few.h; 16 rows of 128256 x 2048, bf16: the tiles' kernel 115 us, this one 87, 6.0 TB/s).
 #include "dense_stage.h"
 
 namespace {
@@ -185,6 +186,7 @@ struct Counted {
   int64_t* target;     // [padded]
   float* lse;          // [padded]
   float* grad;         // [padded]: g 2^-e with e the exponent of the largest finite |g|; 0 behind the last
+  float* rest;         // [padded], 16 bits: what P's rounding took from the target's entry
   float* back;         // 2^e
   int32_t* count;
 };
@@ -229,6 +231,7 @@ __global__ __launch_bounds__(1024) void count_rows_kernel(const float* __restric
       c.row[at] = i;
       c.target[at] = target;
       c.lse[at] = lse[i];
+      c.rest[at] = 0.0f;
       c.grad[at] = target < 0 || target >= vocab ? NAN : ldexpf(g, -e);
     }
     begin += all;
@@ -238,6 +241,7 @@ __global__ __launch_bounds__(1024) void count_rows_kernel(const float* __restric
     c.target[i] = -1;
     c.lse[i] = 0.0f;
     c.grad[i] = 0.0f;
+    c.rest[i] = 0.0f;
   }
   if (threadIdx.x == 0) {
     *c.back = ldexpf(1.0f, e);
@@ -269,6 +273,7 @@ __global__ __launch_bounds__(WM * WN * kWave) void piece_kernel(const TileOperan
     if (n >= out.padded) continue;
     const float g = rows.grad[n], lse = rows.lse[n];   // (0 behind the last)
     const int64_t target = rows.target[n] - (first_token + m0);   // within the tile
+    float at_target = 0.0f;
 #pragma unroll
     for (int mi = 0; mi < Tile::MI; mi += 2) {   // eight neighbouring tokens
       uint16_t v[P][8];
@@ -279,6 +284,7 @@ __global__ __launch_bounds__(WM * WN * kWave) void piece_kernel(const TileOperan
         const float f = g == 0.0f || m0 + m >= weight.rows ? 0.0f : e * g;
         if constexpr (P == 1) {
           v[0][i] = __builtin_bit_cast(uint16_t, from_float<O>(f));
+          at_target = target == m ? f : at_target;
         } else {
           uint16_t p[3];
           planes_of(f, p);
@@ -295,6 +301,10 @@ __global__ __launch_bounds__(WM * WN * kWave) void piece_kernel(const TileOperan
         w.w = v[j][6] | static_cast<uint32_t>(v[j][7]) << 16;
         store16(static_cast<uint16_t*>(out.p) + j * out.plane + static_cast<int64_t>(n) * out.ld + m0 + Tile::row_of(mi, 0), w);
       }
+    }
+    if constexpr (P == 1) {   // (zero where the target is not the lane's)
+      const float rest = at_target - to_float(from_float<O>(at_target));
+      if (rest != 0.0f) rows.rest[n] = rest;
     }
   }
 }
@@ -327,6 +337,7 @@ __global__ __launch_bounds__(kFewWaves * kWave, BITS != 0 && NT == 4 ? 1 : 2) vo
       const int m = i * 16 + v0 + q;
       const float value = none ? 0.0f : __builtin_amdgcn_exp2f((f.acc[i][q] - lse) * kLog2e) - (target == m ? 1.0f : 0.0f);
       e[q] = g == 0.0f || m0 + m >= weight.rows ? 0.0f : value * g;
+      if (sizeof(T) == 2 && target == m) rows.rest[n] = e[q] - to_float(from_float<T>(e[q]));
       if (out.turned != nullptr) {
         T* to = out.turned + static_cast<int64_t>(m0 + m) * out.turned_ld + n;
         *to = from_float<T>(e[q]);
@@ -348,7 +359,7 @@ struct Plan {
   bool few;                                // rows that go past the weight once, as it lies
   int row_tiles, blocks;                   // of 16, for these: 1, 2 or 4; of 16 row_tiles rows
   // offsets into the workspace
-  int64_t o_stats, o_chosen, o_hidden, o_weight, o_row, o_place, o_target, o_lse, o_grad, o_back, o_x, o_p, o_turned, o_p_turned, o_sums, bytes;
+  int64_t o_stats, o_chosen, o_hidden, o_weight, o_row, o_place, o_target, o_lse, o_grad, o_rest, o_back, o_x, o_p, o_turned, o_p_turned, o_sums, bytes;
 };
 
 int64_t take(int64_t& at, int64_t bytes) {
@@ -423,6 +434,7 @@ Plan plan_for(int rows, int vocab, int hidden, int group_size, int wformat, int 
     p.o_target = take(at, int64_t{8} * p.padded);
     p.o_lse = take(at, int64_t{4} * p.padded);
     p.o_grad = take(at, int64_t{4} * p.padded);
+    p.o_rest = take(at, int64_t{4} * p.padded);
     p.o_back = take(at, 8);
   }
   if (p.few) {
@@ -507,6 +519,9 @@ FewWeight few_weight(const Plan& p, const Call& c) {
   return FewWeight{static_cast<const uint8_t*>(c.weight), c.wscale, row_bytes, p.vocab, p.hidden, c.wformat ? p.hidden / c.group_size : 0,
                    c.group_size, c.group_size, c.out_group};
 }
+TargetTerm target_term(const Plan& p, const Call& c, const Counted& rows) {   // (fp32: nothing is rounded away)
+  return TargetTerm{p.planes == 1 ? rows.rest : nullptr, rows.target, few_weight(p, c), c.wformat};
+}
 template <typename T> void few_operand(const Plan& p, const Call& c, const int32_t* gather) {
   const int64_t items = int64_t{p.hidden} / (4 * kFewPack<T>) * p.row_tiles * kWave;
   hipLaunchKernelGGL((few_operand_kernel<T>), dim3(static_cast<unsigned>((items + 255) / 256), p.blocks), dim3(256), 0, c.stream, static_cast<const T*>(c.hidden),
@@ -536,14 +551,22 @@ template <typename T> int few_forward(const Plan& p, const Call& c, const int64_
 
 // dW of tokens first ..: over the rows, both with them outermost
 template <typename T>
-void weight_gradient(const Plan& p, const Call& c, const TileOperand& part, int first, int tokens, const float* back, const int32_t* count, void* grad_weight) {
+void weight_gradient(const Plan& p, const Call& c, const TileOperand& part, int first, int tokens, const Counted& rows, void* grad_weight) {
   const int rows64 = static_cast<int>(round_up(p.rows, 64));
   TileOperand hidden_k = hidden_operand(p, c), part_k = part;
   hidden_k.rows = p.hidden;
   hidden_k.k_rows = rows64;
   part_k.rows = tokens;
-  product_launch<T, false, true>(hidden_k, part_k, rows64,
-                                 ProductOut{static_cast<T*>(grad_weight) + static_cast<int64_t>(first) * p.hidden, p.hidden, back, 0, 1, count}, c.stream);
+  ProductOut out{static_cast<T*>(grad_weight) + static_cast<int64_t>(first) * p.hidden, p.hidden, rows.back, 0, 1, rows.count};
+  if (p.planes == 1) {
+    out.rest = rows.rest;
+    out.target = rows.target;
+    out.row = rows.row;
+    out.x = c.hidden;
+    out.x_stride = c.hidden_stride;
+    out.first_token = first;
+  }
+  product_launch<T, false, true>(hidden_k, part_k, rows64, out, c.stream);
 }
 
 template <typename T>
@@ -565,14 +588,15 @@ int few_backward(const Plan& p, const Call& c, const Counted& rows, void* grad_h
     hipLaunchKernelGGL((few_turned_kernel<T>), dim3(static_cast<unsigned>((items + 255) / 256)), dim3(256), 0, c.stream, static_cast<const T*>(c.hidden),
                        c.hidden_stride, rows.row, p.rows, p.hidden, steps, turned);
     const dim3 outer(tokens, 1);
-    if (p.blocks == 1)
-      hipLaunchKernelGGL((few_outer_kernel<T, true>), outer, dim3(kFewWaves * kWave), 0, c.stream, part.turned, int64_t{p.padded}, turned, steps, rows.back, p.vocab,
-                         p.hidden, static_cast<T*>(grad_weight));
-    else
-      hipLaunchKernelGGL((few_outer_kernel<T, false>), outer, dim3(kFewWaves * kWave), 0, c.stream, part.turned, int64_t{p.padded}, turned, steps, rows.back, p.vocab,
-                         p.hidden, static_cast<T*>(grad_weight));
+    const FewRests rests{rows.rest, rows.target, rows.row, rows.count, c.hidden, c.hidden_stride};
+#define LLMQ_OUTER(ONE)                                                                                                                             \
+  hipLaunchKernelGGL((few_outer_kernel<T, ONE>), outer, dim3(kFewWaves * kWave), 0, c.stream, part.turned, int64_t{p.padded}, turned, steps, rows.back, \
+                     p.vocab, p.hidden, rests, static_cast<T*>(grad_weight))
+    if (sizeof(T) == 2 || p.blocks == 1) LLMQ_OUTER(true);
+    else if constexpr (sizeof(T) == 4) LLMQ_OUTER(false);
+#undef LLMQ_OUTER
   }
-  add_few_launch<T>(sums, p.splits, p.rows, p.hidden, rows.back, rows.place, grad_hidden, c.stream);
+  add_few_launch<T>(sums, p.splits, p.rows, p.hidden, rows.back, rows.place, target_term(p, c, rows), grad_hidden, c.stream);
   return llmq_host::check_launch("vocab_loss_grad");
 }
 
@@ -604,7 +628,7 @@ int backward(const Plan& p, const Call& c, const int64_t* targets, int64_t ignor
   float* back = reinterpret_cast<float*>(c.workspace + p.o_back);
   const Counted rows{reinterpret_cast<int32_t*>(c.workspace + p.o_row), reinterpret_cast<int32_t*>(c.workspace + p.o_place),
                      reinterpret_cast<int64_t*>(c.workspace + p.o_target), reinterpret_cast<float*>(c.workspace + p.o_lse),
-                     reinterpret_cast<float*>(c.workspace + p.o_grad), back, reinterpret_cast<int32_t*>(c.workspace + p.o_back + 4)};
+                     reinterpret_cast<float*>(c.workspace + p.o_grad), reinterpret_cast<float*>(c.workspace + p.o_rest), back, reinterpret_cast<int32_t*>(c.workspace + p.o_back + 4)};
   float* sums = reinterpret_cast<float*>(c.workspace + p.o_sums);
   const bool learned = grad_weight != nullptr;
   const int rows64 = static_cast<int>(round_up(p.rows, 64));
@@ -632,10 +656,10 @@ int backward(const Plan& p, const Call& c, const int64_t* targets, int64_t ignor
     if (learned) {
       TileOperand part_k = part;
       part_k.k_rows = rows64;
-      weight_gradient<T>(p, c, part_k, first, tokens, back, rows.count, grad_weight);
+      weight_gradient<T>(p, c, part_k, first, tokens, rows, grad_weight);
     }
   }
-  add_planes_launch<T>(sums, p.rows, p.hidden, p.splits, rows.count, back, rows.place, grad_hidden, c.stream);
+  add_planes_launch<T>(sums, p.rows, p.hidden, p.splits, rows.count, back, rows.place, target_term(p, c, rows), grad_hidden, c.stream);
   return llmq_host::check_launch("vocab_loss_grad");
 }
 

@@ -6,7 +6,6 @@
 // Few rows: past the weight as it lies (dense_few.h). Otherwise the weight is brought to its values a piece of its rows at a time (dense_stage.h: a piece that the caches hold), and multiplied on the
 // matrix core with the reduction outermost, as it lies (dense_tile.h); sums over the pieces and over the splits of one go through fp32 planes. Bound: the
 // matrix core for training batches, the weight's way through memory and the conversion of its codes for few rows.
-#include "dense_few.h"
 #include "dense_stage.h"
 
 namespace {
@@ -62,7 +61,7 @@ int launch(const Plan& p, const void* grad, int64_t stride, const void* qweight,
     float* sums = reinterpret_cast<float*>(workspace);
     columns_launch<T, false>(FewWeight{static_cast<const uint8_t*>(qweight), wscale, static_cast<int64_t>(G) * gs * wformat / 8, N, G * keep, G, gs, keep, out_group},
                       FewColumns{grad, stride, nullptr, rows, sums, p.splits}, wformat, stream);
-    add_few_launch<T>(sums, p.splits, rows, G * keep, nullptr, nullptr, out, stream);
+    add_few_launch<T>(sums, p.splits, rows, G * keep, nullptr, nullptr, TargetTerm{}, out, stream);
     return llmq_host::check_launch("wq_linear_grad");
   }
   const int width = G * keep, n64 = static_cast<int>(p.n_padded);
@@ -87,7 +86,7 @@ int launch(const Plan& p, const void* grad, int64_t stride, const void* qweight,
     if (summed) product_launch<T, true, false>(a, b, k, ProductOut{sums, width, nullptr, first == 0, p.splits}, stream);
     else product_launch<T, false, false>(a, b, k, ProductOut{out, width, nullptr, 1, 1}, stream);
   }
-  if (summed) add_planes_launch<T>(sums, rows, width, p.splits, nullptr, nullptr, nullptr, out, stream);
+  if (summed) add_planes_launch<T>(sums, rows, width, p.splits, nullptr, nullptr, nullptr, TargetTerm{}, out, stream);
   return llmq_host::check_launch("wq_linear_grad");
 }
 

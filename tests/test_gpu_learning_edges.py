@@ -94,6 +94,27 @@ def test_few_rows_of_a_linear(ext, rows, out, width, bits, group, keep, out_grou
     assert torch.equal(other[rest], got[rest])
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("bits", [0, 8, 4])
+@pytest.mark.parametrize("rows", [1, 20, 64, 65, 700])
+@pytest.mark.parametrize("same", [False, True])
+def test_a_target_loses_nothing_to_rounding(ext, rows, bits, dtype, same):
+    """Logits near each other: P is (p - [target]) g with p of about 1 / 3000, and the entries of the targets, which rounding to 16 bits would leave u off, are
+    nearly all of it. What is left over the results' own rounding is the others' u p, together below u / 50 (their 3000 independent errors of at most u / 3000 each)."""
+    vocab, width = 3000, 256
+    hidden, weight, scale, dense, targets, grad = case(rows, vocab, width, dtype, bits, rows)
+    hidden = (hidden / 64).to(dtype)
+    if same:
+        targets[:] = 1717   # (all rows on one token: its row of dW has a term from each)
+    grad = torch.full_like(grad, 1 / 1.37)
+    _, _, dh, dw = loss_and_gradients(ext, (hidden, weight, scale, dense, targets, grad))
+    want = expected(hidden, dense, targets, grad, -100, dtype)
+    for got, (value, _) in ((dh, want[2]), (dw, want[3])):
+        if got is not None:
+            own = (value.to(dtype).double() - value).norm()
+            assert (got.double() - value).norm() <= 1.05 * own + 0.02 * U[dtype] * value.norm()
+
+
 # ---- rows that do not count -------------------------------------------------------------------------------------------------------
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("bits", [0, 8])
