@@ -608,8 +608,9 @@ int llmq_wq_linear_grad(const void* grad, int64_t grad_stride, const void* qweig
  * hidden_size / group_size, group_size] with wscale (wformat 8 or 4, out_group, as for llmq_wq_gemv), which stand for
  * (dtype)(code * scale) and have no gradient. losses, lse, grad: fp32 [rows]. A row whose target is ignore_index has loss 0 and
  * no part in a gradient, whatever it holds; any other target outside [0, vocab) makes the row's loss NaN, its
- * gradient NaN and grad_weight NaN. lse: as llmq_vocab_loss gave it. Logits and sums in fp32; P is rounded to `dtype` (to three bfloat16
- * planes for fp32), with grad scaled by a power of two to at most 2. Gradients are rounded once. hidden_size a multiple of 8, up
+ * gradient NaN and grad_weight NaN. lse: as llmq_vocab_loss gave it. Logits and sums in fp32; P is rounded to `dtype` (fp32: three bfloat16
+ * planes, few rows not at all), with grad scaled by a power of two to at most 2; what that takes from a target's own entry is added to the gradients
+ * in fp32 (grad_weight: rounded to `dtype` again). Gradients are rounded once. hidden_size a multiple of 8, up
  * to 65536; rows up to 2^20, vocab up to 2^24; tensors 16-byte aligned. No rows: nothing is written (grad_weight neither). workspace:
  * ..._workspace_bytes(...) bytes, 16-byte aligned, needs no clearing; calls that overlap in time need one each. */
 size_t llmq_vocab_loss_workspace_bytes(int rows, int vocab, int hidden_size, int group_size, int wformat, int dtype);

@@ -7,6 +7,7 @@
 // shrink   rows by a bank's rows: the reduction is long (in, or out), the result 8 to 128 wide. A workgroup takes a piece of one
 //          request's rows, its waves parts of the reduction.
 // expand   multiplies that by the other factor into the projection's output: a wave has 128 columns.
+// step     both at once for single rows beside small banks: every workgroup of a row makes its `low` again.
 // outer    gradients of the bank: the reduction is over rows, which are sorted by adapter (plan) in blocks of 32. Both operands lie
 //          with the reduction outermost; a lane loads eight columns of its eight rows and turns them over in registers.
 // All on the matrix core in fp32 sums. The 8 to 128 numbers in between stay fp32 in memory; as operands they are
@@ -82,7 +83,7 @@ __device__ __forceinline__ HiLo hi_lo(const float* f) {
 // ---- shrink -----------------------------------------------------------------------------------------------------------------
 // RT: tiles of 16 of the rank, NT: of rows. A step is 128 bytes of a row. A workgroup of eight waves (four for ranks above 32) takes 16 or 32 rows, each wave every
 // eighth step of the reduction, through LDS of its own: transfers of eight whole rows' 128 bytes (read as operands, 16 bytes of 16 rows, an instruction meets
-// 64 pieces of lines: 4099 rows of 4096 24.7 us where this takes 12), chunks swizzled by the row, no barrier but the one meeting at the end. Where
+// 64 pieces of lines: 4099 rows of 4096 24.7 us where this takes 11.2), chunks swizzled by the row, no barrier but the one meeting at the end. Where
 // rows are few the reduction is cut for several workgroups (splits_of).
 constexpr int shrink_waves(int rank) { return rank > 32 ? 4 : 8; }   // (two workgroups a CU at least, for their LDS)
 template <int RT> constexpr int kShrinkWaves = RT >= 4 ? 4 : 8;
@@ -210,7 +211,7 @@ template <typename T> __device__ __forceinline__ void rows_of_nobody(const int r
 }
 
 // 128 columns a wave: lane 16 g + r has columns 8 r .. 8 r + 7, one of each of eight tiles, of rows 4 g .. 4 g + 3, so that 16 lanes read and
-// write 256 neighbouring bytes of a row (with rows over the lanes, 64 bytes of each of 16: 4099 rows of 4096 23 us). What does not depend on the
+// write 256 neighbouring bytes of a row (with rows over the lanes, 64 bytes of each of 16: 4099 rows of 4096 23 us where this takes 18.8). What does not depend on the
 // rows' sums, the weights and the base, is asked for first. The bank here is [slots][columns][rank].
 template <typename T, int RT, int NT>
 __global__ __launch_bounds__(kExpandWaves * kWave) void expand_kernel(const Bank bank, const Requests req, const Expand e) {
