@@ -190,7 +190,7 @@ struct Expand {
   void* out;               // [rows, width], contiguous
   float* low;              // or null: [rows, rank], the sum of the planes (where there are several) and zeros without an adapter
   int rows, columns;       // columns of out
-  int pieces, rest;        // pieces of requests for each 512 columns; workgroups behind all of them, for rows of no request
+  int pieces, rest;        // pieces of requests, for each 512 columns (blockIdx.y); workgroups of the last y, for rows of no request (0: there is none)
 };
 
 // Rows in front of the first request and behind the last one: the base as it is, no sums.
@@ -221,13 +221,13 @@ __global__ __launch_bounds__(kExpandWaves * kWave) void expand_kernel(const Bank
   __shared__ u32x4 s_low[sizeof(T) == 4 ? 1 : 2][kBlocks][kWave];
   __shared__ __attribute__((aligned(16))) uint8_t s_bank[kStaged ? kExpandWaves * 4096 * RT : 16];
   const int lane = threadIdx.x & (kWave - 1), wv = threadIdx.x / kWave, lr = lane & 15, g = lane >> 4;
-  const int pieces = static_cast<int>(gridDim.x) - e.rest;
-  if (static_cast<int>(blockIdx.x) >= pieces) {
-    rows_of_nobody<T>(bank.rank, req.rows, e, blockIdx.x - pieces);
+  const int groups = static_cast<int>(gridDim.y) - (e.rest > 0 ? 1 : 0);
+  if (static_cast<int>(blockIdx.y) >= groups) {
+    if (static_cast<int>(blockIdx.x) < e.rest) rows_of_nobody<T>(bank.rank, req.rows, e, blockIdx.x);
     return;
   }
   // the pieces of the same columns to one XCD, whose cache has the bank's rows for them
-  const int item = tile_of_workgroup(blockIdx.x, pieces), group = item / e.pieces;
+  const int item = tile_of_workgroup(blockIdx.x + blockIdx.y * gridDim.x, groups * gridDim.x), group = item / e.pieces;
   int first, n;
   const int a = req.template piece<kPieceShift<NT>>(item - group * e.pieces, bank.slots, first, n);
   if (n <= 0) return;
@@ -851,8 +851,8 @@ template <typename T> void expand(const Bank& bank, const Requests& req, Expand 
   const bool ragged = req.rows.start != nullptr;
   const int nt = row_tiles(e.rows, req.rows.sequences, ragged);
   e.pieces = pieces_of(e.rows, req.rows.sequences, ragged, nt);
-  e.rest = ragged && (e.out != e.base || e.low != nullptr) ? 32 : 0;   // (usually without a row: the requests have them all)
-  const dim3 grid(e.pieces * ((e.columns + kExpandWaves * 128 - 1) / (kExpandWaves * 128)) + e.rest);
+  e.rest = !ragged || (e.out == e.base && e.low == nullptr) ? 0 : e.pieces < 32 ? e.pieces : 32;   // (usually without a row: the requests have them all)
+  const dim3 grid(e.pieces, (e.columns + kExpandWaves * 128 - 1) / (kExpandWaves * 128) + (e.rest > 0 ? 1 : 0));
   if (bank.rank <= 16) expand_nt<T, 1>(bank, req, e, nt, grid, s);
   else if (bank.rank <= 32) expand_nt<T, 2>(bank, req, e, nt, grid, s);
   else if (bank.rank <= 64) expand_nt<T, 4>(bank, req, e, nt, grid, s);
@@ -947,6 +947,8 @@ int check(int rows, int sequences, bool ragged, int in, int out, int rank, int s
   if (in < 8 || out < 8 || in % 8 || out % 8 || in > (1 << 20) || out > (1 << 20))
     return llmq_host::fail_invalid("in_features and out_features must be multiples of 8 up to 2^20, got %d and %d", in, out);
   if (rows > (1 << 20) || sequences > (1 << 20) || slots > (1 << 20)) return llmq_host::fail_invalid("at most 2^20 rows, sequences and slots, got %d, %d, %d", rows, sequences, slots);
+  if ((rows / 16 + int64_t{2} * sequences) * ((in > out ? in : out) / 512 + 1) > (1 << 30))
+    return llmq_host::fail_invalid("too many pieces: %d rows of %d sequences by %d x %d", rows, sequences, in, out);
   if (!ragged && rows != sequences) return llmq_host::fail_invalid("without query_start a sequence has one row: %d rows, %d sequences", rows, sequences);
   return 0;
 }

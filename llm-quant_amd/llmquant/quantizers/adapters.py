@@ -32,11 +32,12 @@ class AdapterBatch:
         self._starts: dict[tuple[int, int], torch.Tensor] = {}
         self._query_start: torch.Tensor | None = None
         self._requests = 1
+        self._captured: list[torch.Tensor] = []   # what captured steps read
 
     def select(self, adapter, query_start=None) -> None:
         """adapter: a slot for each request (a list, or a tensor on any device; negative: none). query_start: int32 [requests + 1] on the device,
         for calls whose requests have unlike numbers of rows (None: as many rows each). It is kept, not copied: a captured
-        step reads the tensor it was captured with."""
+        step reads the tensor it was captured with, which lives as long as the batch."""
         adapter = torch.as_tensor(adapter, dtype=torch.int32).reshape(-1)
         if adapter.numel() == 0:
             raise ValueError("adapters for no request")
@@ -72,6 +73,8 @@ class AdapterBatch:
                     start = torch.zeros(requests + 1, dtype=torch.int32, device=self.device)
                 if not (start.is_cuda and torch.cuda.is_current_stream_capturing()):   # (else it lives in the graph's memory)
                     self._starts[count, requests] = start
+        elif start is not None and start.is_cuda and torch.cuda.is_current_stream_capturing() and not any(t is start for t in self._captured):
+            self._captured.append(start)
         return self._held(requests), start
 
     # (a copy of the model has a batch of its own; captured steps do not come along)

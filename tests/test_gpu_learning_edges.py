@@ -524,6 +524,30 @@ def test_copied_and_saved_banks():
         assert torch.equal(other(ids).logits, want)
 
 
+def test_a_captured_step_keeps_the_starts_it_reads():
+    from llmquant.quantizers.adapters import AdapterBatch, LoraAdapters
+
+    batch = AdapterBatch("cuda")
+    bank = LoraAdapters(64, 64, 8, 2, 16.0, torch.bfloat16, "cuda", batch).requires_grad_(False)
+    gen = torch.Generator(device="cuda").manual_seed(0)
+    bank.lora_b.copy_(torch.randn(bank.lora_b.shape, generator=gen, device="cuda"))
+    x, base = (torch.randn(12, 64, generator=gen, device="cuda").bfloat16() for _ in range(2))
+    batch.select([0, 1], torch.tensor([0, 5, 12], dtype=torch.int32, device="cuda"))
+    want = bank(x, base.clone())
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = bank(x, base.clone())
+    batch.select([1, 0])   # (the tensor of starts is nobody's else)
+    noise = [torch.full((3,), 7, dtype=torch.int32, device="cuda") for _ in range(64)]
+    batch.select([0, 1])
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(got, want)
+    del noise
+
+
 # ---- refusals of the bindings ---------------------------------------------------------------------------------------------------------
 def test_refusals(ext):
     hidden, weight, _, _, targets, grad = case(4, 40, 64, torch.bfloat16, 0, 0)

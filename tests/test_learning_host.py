@@ -131,7 +131,8 @@ ADAPTERS = DTYPE + [
     (dict(rows=-1), "bad dimension"), (dict(sequences=-1), "bad dimension"), (dict(slots=-1), "bad dimension"), (dict(rank=0), "rank must be"),
     (dict(rank=12), "rank must be"), (dict(rank=136), "rank must be"), (dict(inp=252, x_stride=256), "multiples of 8"), (dict(out=0), "multiples of 8"),
     (dict(out=(1 << 20) + 8, base_stride=(1 << 20) + 8), "multiples of 8"), (dict(rows=(1 << 20) + 1), "at most 2^20"),
-    (dict(sequences=(1 << 20) + 1), "at most 2^20"), (dict(start=None), "one row"), (dict(pointer=None), "null tensor pointer"),
+    (dict(sequences=(1 << 20) + 1), "at most 2^20"), (dict(start=None), "one row"),
+    (dict(sequences=1 << 20, inp=1 << 20, out=1 << 20, x_stride=1 << 20, base_stride=1 << 20), "too many pieces"), (dict(pointer=None), "null tensor pointer"),
     (dict(x_stride=248), "row stride"), (dict(x_stride=260), "row stride"), (dict(base_stride=504), "row stride"), (dict(x=24), "16-byte aligned"),
     (dict(to=40), "16-byte aligned"), (dict(bank=20), "16-byte aligned"), (dict(workspace=None), "workspace"), (dict(workspace=24, bytes=GIB), "workspace"),
     (dict(bytes=16), "workspace")]
