@@ -80,6 +80,15 @@ __device__ __forceinline__ HiLo hi_lo(const float* f) {
   return r;
 }
 
+template <typename T> __device__ __forceinline__ void store_four(T* to, const float* f) {   // four neighbouring values
+  if constexpr (sizeof(T) == 4) {
+    *reinterpret_cast<v4f*>(to) = v4f{f[0], f[1], f[2], f[3]};
+  } else {
+    const T h[4] = {from_float<T>(f[0]), from_float<T>(f[1]), from_float<T>(f[2]), from_float<T>(f[3])};
+    *reinterpret_cast<u32x2*>(to) = __builtin_bit_cast(u32x2, h);
+  }
+}
+
 // ---- shrink -----------------------------------------------------------------------------------------------------------------
 // RT: tiles of 16 of the rank, NT: of rows. A step is 128 bytes of a row. A workgroup of eight waves (four for ranks above 32) takes 16 or 32 rows, each wave every
 // eighth step of the reduction, through LDS of its own: transfers of eight whole rows' 128 bytes (read as operands, 16 bytes of 16 rows, an instruction meets
@@ -593,6 +602,7 @@ struct Outer {
   const float* scaling;
   int slots, rank, capacity, shift;   // 1 << shift rows a piece
   int a_columns;           // workgroups of side a in blockIdx.x
+  void *grad_a, *grad_b;   // or null: records. Where a slot's rows are one piece: the results, blockIdx.y is the slot
 };
 constexpr int kColumns = 128;   // of a wave: one group of the codes
 
@@ -716,16 +726,24 @@ __device__ __forceinline__ void outer_rows(const OuterSide& side, const Outer& o
 template <typename T, bool CODES, int RTW>
 __global__ __launch_bounds__(4 * kWave) void outer_kernel(const Outer o) {
   __shared__ v4f s_sum[2][RTW * 8][kWave];
-  const Ragged slots{o.start, o.slots, o.capacity};
-  int piece = blockIdx.y, none;
-  Span span;
-  slots.find(o.shift, nullptr, piece, span, none);
-  const int v0 = span.first + (piece << o.shift), v1 = min(v0 + (1 << o.shift), span.first + span.n);
-  if (span.n <= 0 || v0 >= v1) return;
+  int v0, v1;
+  if (o.grad_a != nullptr) {   // a slot's rows at once
+    v0 = o.start[blockIdx.y];
+    v1 = o.start[blockIdx.y + 1];
+  } else {
+    const Ragged slots{o.start, o.slots, o.capacity};
+    int piece = blockIdx.y, none;
+    Span span;
+    slots.find(o.shift, nullptr, piece, span, none);
+    v0 = span.first + (piece << o.shift);
+    v1 = min(v0 + (1 << o.shift), span.first + span.n);
+    if (span.n <= 0 || v0 >= v1) return;
+  }
   const bool side_b = static_cast<int>(blockIdx.x) >= o.a_columns;
   const int c0 = (blockIdx.x - (side_b ? o.a_columns : 0)) * kColumns;
   v4f acc[RTW][8] = {};
-  if (side_b) outer_rows<T, false, RTW>(o.b, o, c0, v0, v1, acc);
+  if (v0 >= v1) {}   // (a slot without rows: zeros)
+  else if (side_b) outer_rows<T, false, RTW>(o.b, o, c0, v0, v1, acc);
   else outer_rows<T, CODES, RTW>(o.a, o, c0, v0, v1, acc);
   const int lane = threadIdx.x & (kWave - 1), wv = threadIdx.x / kWave, lr = lane & 15, g = lane >> 4;
   if (wv >= 2) {
@@ -745,6 +763,38 @@ __global__ __launch_bounds__(4 * kWave) void outer_kernel(const Outer o) {
   __syncthreads();
   if (wv != 0) return;
   const OuterSide& side = side_b ? o.b : o.a;
+  if (o.grad_a != nullptr) {
+    const float scale = o.scaling[blockIdx.y];
+    const bool halved = sizeof(T) == 4 && !(CODES && !side_b), none = v0 >= v1;
+    const auto value = [&](int i, int q, int c) { return none ? 0.0f : (acc[i][c][q] + s_sum[0][i * 8 + c][lane][q]) * scale; };
+    const int64_t slot = static_cast<int64_t>(blockIdx.y) * o.rank * side.width;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int c = c0 + (halved ? 64 * h + 4 * lr : 8 * lr + 4 * h);
+      if (c >= side.width) continue;   // (a multiple of 8)
+      if (!side_b) {
+#pragma unroll
+        for (int i = 0; i < RTW; ++i)
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const int r = blockIdx.z * RTW * 16 + RTW * (4 * g + q) + i;
+            const float f[4] = {value(i, q, 4 * h), value(i, q, 4 * h + 1), value(i, q, 4 * h + 2), value(i, q, 4 * h + 3)};
+            if (r < o.rank) store_four(static_cast<T*>(o.grad_a) + slot + static_cast<int64_t>(r) * side.width + c, f);
+          }
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+#pragma unroll
+          for (int k = 0; k < 4 * RTW; k += 4) {   // four of the rank
+            const int r = blockIdx.z * RTW * 16 + RTW * 4 * g + k;
+            const float f[4] = {value(k % RTW, k / RTW, 4 * h + e), value((k + 1) % RTW, (k + 1) / RTW, 4 * h + e), value((k + 2) % RTW, (k + 2) / RTW, 4 * h + e),
+                                value((k + 3) % RTW, (k + 3) / RTW, 4 * h + e)};
+            if (r < o.rank) store_four(static_cast<T*>(o.grad_b) + slot + static_cast<int64_t>(c + e) * o.rank + r, f);
+          }
+      }
+    }
+    return;
+  }
   float* record = side.records + static_cast<int64_t>(blockIdx.y) * o.rank * side.width;
   // (lane: entries RTW (4 g + q) + i of the rank's 16 RTW, and of the columns 8 lr .. 8 lr + 7, or of fp32 values 64 h + 4 lr .., h = 0, 1)
   const bool halves = sizeof(T) == 4 && !(CODES && !side_b);
@@ -876,7 +926,8 @@ int64_t take(int64_t& at, int64_t bytes) {
 }
 
 struct GradPlan {
-  int splits, capacity, tiles, shift, records;   // parts of shrink, virtual rows, tiles of the rank, pieces of outer
+  bool direct;   // no records: a workgroup has all of a slot's rows
+  int splits, capacity, tiles, rtw, shift, records;   // parts of shrink, virtual rows, tiles of the rank, pieces of outer
   int64_t o_start, o_order, o_seq, o_at, o_bt, o_planes, o_du, o_rec_a, o_rec_b, bytes;
 };
 GradPlan grad_plan(int rows, int sequences, bool ragged, int in, int out, int rank, int slots, int dtype) {
@@ -886,12 +937,18 @@ GradPlan grad_plan(int rows, int sequences, bool ragged, int in, int out, int ra
   const int64_t used = slots < sequences ? slots : sequences;   // slots that can have rows
   p.capacity = static_cast<int>(round_up(rows + 31 * used, kBlock));
   p.tiles = (rank + 15) / 16;
-  // a piece of outer: 128 to 4096 rows, as long as it takes for the workgroups to be on the chip at once or nearly (with 64 entries of the rank
+  // outer takes one, two or four tiles of the rank a workgroup: fewer read the rows more often, and are smaller programs of fewer registers (bf16, whole calls, us,
+  // by four / two / one: 4096 x 14336 by 64, 32 rows 47 / 35 / 32, 1024 rows 62 / 53 / 52, 2048 77 / 70 / 79, 4096 113 / 118 / 151).
+  p.rtw = p.tiles >= 4 && rows > 2048 ? 4 : p.tiles >= 2 && rows > 1024 ? 2 : 1;
+  // All of a slot's rows in a workgroup, which leaves the records and their launch out, while slots have up to 1024 on average (rank 16, 4096 x 4096, four slots: 64 rows
+  // 24.7 -> 18.7 us, 4096 rows 49.9 -> 45.4; 2048 x 2048, one slot: 1024 rows 29.2 -> 26.9, 4096 rows 46.5 -> 60.5).
+  p.direct = rows <= 1024 * used;
+  // Otherwise a piece of 128 to 4096 rows, as long as it takes for the workgroups to be on the chip at once or nearly (with 64 entries of the rank
   // one a CU, for their registers: 4099 rows by 8192 columns, pieces of 512 rows 33 us and 11.6 to add them up, 1024 28.4 + 7.4, 2048 34.8 + 7.3)
-  const int64_t columns = (in + kColumns - 1) / kColumns + (out + kColumns - 1) / kColumns, places = p.tiles >= 4 ? 400 : p.tiles >= 2 ? 512 : 1024;
+  const int64_t columns = (in + kColumns - 1) / kColumns + (out + kColumns - 1) / kColumns, places = p.rtw == 4 ? 400 : p.rtw == 2 ? 512 : 1024;
   p.shift = 7;
-  while (p.shift < 12 && columns * ((rows >> p.shift) + used) * ((p.tiles + 3) / 4) > places) ++p.shift;
-  p.records = (p.capacity >> p.shift) + 2 * slots;
+  while (p.shift < 12 && columns * ((rows >> p.shift) + used) * ((p.tiles + p.rtw - 1) / p.rtw) > places) ++p.shift;
+  p.records = p.direct ? 0 : (p.capacity >> p.shift) + 2 * slots;
   int64_t at = 0;
   p.o_start = take(at, int64_t{4} * (slots + 1));
   p.o_order = take(at, int64_t{4} * p.capacity);
@@ -924,15 +981,16 @@ void gradients(const GradPlan& p, const void* grad, int64_t grad_stride, const v
   expand<T>(Bank{ws + p.o_at, slots, rank, in}, req, Expand{planes, plane, p.splits, scaling, grad_base, base_stride, grad_x, p.splits > 1 ? du : nullptr, rows, in, 0, 0}, s);
   const Outer o{OuterSide{x, x_stride, x_scale, du, reinterpret_cast<float*>(ws + p.o_rec_a), in},
                 OuterSide{grad, grad_stride, nullptr, low, reinterpret_cast<float*>(ws + p.o_rec_b), out},
-                plan.start, plan.order, scaling, slots, rank, p.capacity, p.shift, (in + kColumns - 1) / kColumns};
-  const int rtw = p.tiles >= 4 ? 4 : p.tiles >= 2 ? 2 : 1;
-  const dim3 grid(o.a_columns + (out + kColumns - 1) / kColumns, p.records, (p.tiles + rtw - 1) / rtw);
+                plan.start, plan.order, scaling, slots, rank, p.capacity, p.shift, (in + kColumns - 1) / kColumns, p.direct ? grad_a : nullptr,
+                p.direct ? grad_b : nullptr};
+  const dim3 grid(o.a_columns + (out + kColumns - 1) / kColumns, p.direct ? slots : p.records, (p.tiles + p.rtw - 1) / p.rtw);
 #define LLMQ_OUTER(CODES)                                                                                    \
-  if (rtw == 4) hipLaunchKernelGGL((outer_kernel<T, CODES, 4>), grid, dim3(4 * kWave), 0, s, o);            \
-  else if (rtw == 2) hipLaunchKernelGGL((outer_kernel<T, CODES, 2>), grid, dim3(4 * kWave), 0, s, o);       \
+  if (p.rtw == 4) hipLaunchKernelGGL((outer_kernel<T, CODES, 4>), grid, dim3(4 * kWave), 0, s, o);            \
+  else if (p.rtw == 2) hipLaunchKernelGGL((outer_kernel<T, CODES, 2>), grid, dim3(4 * kWave), 0, s, o);       \
   else hipLaunchKernelGGL((outer_kernel<T, CODES, 1>), grid, dim3(4 * kWave), 0, s, o)
   if (x_scale != nullptr) { LLMQ_OUTER(true); } else { LLMQ_OUTER(false); }
 #undef LLMQ_OUTER
+  if (p.direct) return;
   const int64_t a_items = static_cast<int64_t>(slots) * rank * in / 8, items = a_items + static_cast<int64_t>(slots) * rank * out / 8;
   const int64_t groups = (items + 255) / 256;
   hipLaunchKernelGGL((records_kernel<T>), dim3(static_cast<unsigned>(groups < 4096 ? groups : 4096)), dim3(256), 0, s, o, static_cast<T*>(grad_a),

@@ -410,6 +410,28 @@ def test_rows_of_nobody(ext, dtype):
     assert (ga[2] == 0).all() and (gb[2] == 0).all()
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("codes", [False, True])
+@pytest.mark.parametrize("lengths, adapters, slots, rank", [
+    ([1030], [0], 1, 24), ([1000, 20], [1, 0], 2, 40), ([700, 700, 700], [0, 2, 0], 4, 72), ([1500, 1300], [0, 1], 2, 128), ([2500], [2], 3, 64), ([2100, 1, 3], [1, 1, 0], 2, 16),
+    ([5, 900], [3, 1], 5, 8)])
+def test_gradients_of_banks_in_one_piece_and_in_several(ext, lengths, adapters, slots, rank, codes, dtype):
+    """Around 1024 rows a slot and 1024 and 2048 rows together, where the sums over rows are cut otherwise; slots without rows are zero."""
+    c = make(lengths, adapters, slots, rank, 256, 136, dtype, seed=rank)
+    low = torch.empty(sum(lengths), rank, device="cuda")
+    call(ext, c, low=low)
+    values, more = c["x"].double(), {}
+    if codes:
+        stored, scale = ext.quant_group_codes(c["x"], 8, 128)
+        values, more = (stored.double().unflatten(1, (-1, 128)) * scale.double()[..., None]).flatten(1), dict(x=stored, x_scale=scale)
+    grads = call_grad(ext, c, low, grad_base=c["grad_base"], **more)
+    for got, pair, what in zip(grads, lora_backward(c, values, low, dtype), ("gx", "gA", "gB")):
+        lora_close(got, pair, what)
+    for slot in set(range(slots)) - set(adapters):
+        assert (grads[1][slot] == 0).all() and (grads[2][slot] == 0).all()
+    assert same(call_grad(ext, c, low, grad_base=c["grad_base"], **more), grads)
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 def test_no_slots_no_rows_no_requests(ext, dtype):
     c = make([3, 2], [0, 1], 0, 8, 64, 72, dtype)
