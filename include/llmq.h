@@ -631,7 +631,7 @@ int llmq_vocab_loss_grad(const void* hidden, int64_t hidden_stride, const void* 
  * lora_b [slots, out, rank] of `dtype`; scaling fp32 [slots]. The rows of sequence b are query_start[b] .. query_start[b + 1] - 1 (int32
  * [sequences + 1], not decreasing; NULL: row b, rows == sequences); rows of no sequence are base. low_or_null: fp32 [rows, rank],
  * zeros without an adapter; the gradient wants it. Sums in fp32, out rounded once; for 16-bit types low enters the second product as
- * two bfloat16 (16 bits of it). rank a multiple of 8 from 8 to 128 (an adapter of a lower rank has zeros behind it), in and out
+ * two bfloat16 (16 bits of it; fp16: two fp16 with an exponent a row, 22 bits; one row a sequence beside small banks: as it is). rank a multiple of 8 from 8 to 128 (an adapter of a lower rank has zeros behind it), in and out
  * multiples of 8; tensors 16-byte aligned. workspace: ..._workspace_bytes(...) bytes (ragged: whether there is a query_start),
  * 16-byte aligned, needs no clearing; calls that overlap in time need one each.
  *

@@ -10,9 +10,10 @@
 // step     both at once for single rows beside small banks: every workgroup of a row makes its `low` again.
 // outer    gradients of the bank: the reduction is over rows, which are sorted by adapter (plan) in blocks of 32. Both operands lie
 //          with the reduction outermost; a lane loads eight columns of its eight rows and turns them over in registers.
-// All on the matrix core in fp32 sums. The 8 to 128 numbers in between stay fp32 in memory; as operands they are
-// two bfloat16 (16 bits of them), against bfloat16 values as they are, fp16 values as two bfloat16 (exact), fp32 on the fp32
-// matrix instructions. Rounded once, at the end. Every sum has a fixed order.
+// All on the matrix core in fp32 sums (step: fp32 arithmetic). The 8 to 128 numbers in between stay fp32 in memory; as operands they are two bfloat16 (16 bits of
+// them), against bfloat16 values as they are. For fp16: two fp16 with one exponent a row in expand (22 bits; 333 rows of 20 requests by 14336 with the bank as two
+// bfloat16 instead 21.1 us, so 19.3), two bfloat16 against values as two bfloat16 (exact) in outer, whose rows are the reduction. fp32 on the fp32 matrix
+// instructions. Rounded once, at the end. Every sum has a fixed order.
 //
 // Bound: HBM for prompts and training (x, base and out once each); the chain of a launch for single tokens.
 #include "dense_tile.h"
@@ -219,6 +220,12 @@ template <typename T> __device__ __forceinline__ void rows_of_nobody(const int r
   }
 }
 
+// the power of two that brings a row of largest magnitude `most` (its bits) to [2^13, 2^14); 0 for nothing, an infinity or NaN
+__device__ __forceinline__ int row_exponent(uint32_t most) {
+  const int e = static_cast<int>(most >> 23);
+  return e == 0 || e == 255 ? 0 : 127 + 13 - e;
+}
+
 // 128 columns a wave: lane 16 g + r has columns 8 r .. 8 r + 7, one of each of eight tiles, of rows 4 g .. 4 g + 3, so that 16 lanes read and
 // write 256 neighbouring bytes of a row (with rows over the lanes, 64 bytes of each of 16: 4099 rows of 4096 23 us where this takes 18.8). What does not depend on the
 // rows' sums, the weights and the base, is asked for first. The bank here is [slots][columns][rank].
@@ -228,6 +235,8 @@ __global__ __launch_bounds__(kExpandWaves * kWave) void expand_kernel(const Bank
   constexpr int kBlocks = KT * NT, kParts = kBlocks == 1 ? 4 : kBlocks == 2 ? 2 : 1;   // operands of `low`; threads for each packet of one
   constexpr bool kStaged = sizeof(T) == 2 && RT <= 4;   // the bank's rows of a wave's columns through LDS
   __shared__ u32x4 s_low[sizeof(T) == 4 ? 1 : 2][kBlocks][kWave];
+  constexpr bool kHalf = __is_same(T, f16_t);
+  __shared__ uint32_t s_most[kHalf ? 16 * NT : 1];        // fp16: the largest magnitude of each row of `low`, as bits
   __shared__ __attribute__((aligned(16))) uint8_t s_bank[kStaged ? kExpandWaves * 4096 * RT : 16];
   const int lane = threadIdx.x & (kWave - 1), wv = threadIdx.x / kWave, lr = lane & 15, g = lane >> 4;
   const int groups = static_cast<int>(gridDim.y) - (e.rest > 0 ? 1 : 0);
@@ -281,8 +290,13 @@ __global__ __launch_bounds__(kExpandWaves * kWave) void expand_kernel(const Bank
   v4f acc[NT][8] = {};
   if (a >= 0) {   // (the workgroup's)
     // `low` of the piece as operands, made once: packet (row 16 j + lr, values (4 k + g) V ..) by kParts threads, a part of the planes each
-    constexpr int kEach = kWave / kParts;
+    constexpr int kEach = kWave / kParts, kTurns = (kBlocks * kParts + kExpandWaves - 1) / kExpandWaves;
     const float s = e.scaling[a];
+    float sums[kHalf ? kTurns : 1][V];
+    if constexpr (kHalf) {
+      if (threadIdx.x < 16 * NT) s_most[threadIdx.x] = 0;
+      __syncthreads();
+    }
 #pragma unroll
     for (int i0 = 0; i0 < kBlocks * kParts; i0 += kExpandWaves) {
       const int packet = (i0 + wv) * kEach + lane % kEach, part = lane / kEach, block = packet / kWave, pl = packet % kWave;
@@ -323,10 +337,37 @@ __global__ __launch_bounds__(kExpandWaves * kWave) void expand_kernel(const Bank
       for (int i = 0; i < V; ++i) f[i] = r < bank.rank ? f[i] * s : 0.0f;
       if constexpr (sizeof(T) == 4) {
         s_low[0][block][pl] = Pack<float>::pack(f);
+      } else if constexpr (kHalf) {
+        uint32_t most = 0;
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          sums[i0 / kExpandWaves][i] = f[i];
+          most = max(most, __builtin_bit_cast(uint32_t, f[i]) & 0x7fffffffu);
+        }
+        atomicMax(&s_most[t], most);   // (of positive floats the order of their bits, NaN above all)
       } else {
         const HiLo low = hi_lo(f);
         s_low[0][block][pl] = low.hi;
         s_low[1][block][pl] = low.lo;
+      }
+    }
+    if constexpr (kHalf) {   // rows scaled to at most 2^14, as two fp16: 22 bits, and 2^-38 of the row's largest at the least
+      __syncthreads();
+#pragma unroll
+      for (int i0 = 0; i0 < kBlocks * kParts; i0 += kExpandWaves) {
+        const int packet = (i0 + wv) * kEach + lane % kEach, block = packet / kWave, pl = packet % kWave;
+        if (block >= kBlocks) break;
+        if (lane / kEach != 0) continue;
+        const int to = row_exponent(s_most[block % NT * 16 + (pl & 15)]);
+        float f[V], rest[V];
+#pragma unroll
+        for (int i = 0; i < V; ++i) f[i] = __builtin_ldexpf(sums[i0 / kExpandWaves][i], to);
+        const u32x4 hi = Pack<f16_t>::pack(f);
+        Pack<f16_t>::unpack(hi, rest);
+#pragma unroll
+        for (int i = 0; i < V; ++i) rest[i] = f[i] - rest[i];
+        s_low[0][block][pl] = hi;
+        s_low[1][block][pl] = Pack<f16_t>::pack(rest);
       }
     }
     if constexpr (kStaged) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -352,21 +393,11 @@ __global__ __launch_bounds__(kExpandWaves * kWave) void expand_kernel(const Bank
         if constexpr (sizeof(T) == 4) {
 #pragma unroll
           for (int j = 0; j < NT; ++j) acc[j][mi] = mfma_packet<float>(low_hi[j], v, acc[j][mi]);
-        } else if constexpr (__is_same(T, f16_t)) {
-          float w[8];
-          Pack<f16_t>::unpack(v, w);
-          const HiLo two = hi_lo(w);   // (exact: 11 bits in 16)
-#pragma unroll
-          for (int j = 0; j < NT; ++j) {
-            acc[j][mi] = mfma_16x16x32<bf16_t>(low_hi[j], two.lo, acc[j][mi]);
-            acc[j][mi] = mfma_16x16x32<bf16_t>(low_lo[j], two.hi, acc[j][mi]);
-            acc[j][mi] = mfma_16x16x32<bf16_t>(low_hi[j], two.hi, acc[j][mi]);
-          }
         } else {
 #pragma unroll
           for (int j = 0; j < NT; ++j) {
-            acc[j][mi] = mfma_16x16x32<bf16_t>(low_lo[j], v, acc[j][mi]);
-            acc[j][mi] = mfma_16x16x32<bf16_t>(low_hi[j], v, acc[j][mi]);
+            acc[j][mi] = mfma_16x16x32<T>(low_lo[j], v, acc[j][mi]);
+            acc[j][mi] = mfma_16x16x32<T>(low_hi[j], v, acc[j][mi]);
           }
         }
       }
@@ -380,13 +411,14 @@ __global__ __launch_bounds__(kExpandWaves * kWave) void expand_kernel(const Bank
       const int t = j * 16 + 4 * g + i;
       const int64_t row = first + t;
       if (t >= n) continue;
+      const int back = kHalf && a >= 0 ? -row_exponent(s_most[t]) : 0;
 #pragma unroll
       for (int h = 0; h < 8 / V; ++h) {
         float f[V] = {};
         if (e.base != nullptr) Pack<T>::unpack(base[j][i][h], f);
         if (a >= 0) {   // (else the base to the bit: -0 + 0 is +0)
 #pragma unroll
-          for (int q = 0; q < V; ++q) f[q] += acc[j][h * V + q][i];
+          for (int q = 0; q < V; ++q) f[q] += kHalf ? __builtin_ldexpf(acc[j][h * V + q][i], back) : acc[j][h * V + q][i];
         }
         store16(static_cast<T*>(e.out) + row * e.columns + c + h * V, Pack<T>::pack(f));
       }
@@ -940,9 +972,9 @@ GradPlan grad_plan(int rows, int sequences, bool ragged, int in, int out, int ra
   // outer takes one, two or four tiles of the rank a workgroup: fewer read the rows more often, and are smaller programs of fewer registers (bf16, whole calls, us,
   // by four / two / one: 4096 x 14336 by 64, 32 rows 47 / 35 / 32, 1024 rows 62 / 53 / 52, 2048 77 / 70 / 79, 4096 113 / 118 / 151).
   p.rtw = p.tiles >= 4 && rows > 2048 ? 4 : p.tiles >= 2 && rows > 1024 ? 2 : 1;
-  // All of a slot's rows in a workgroup, which leaves the records and their launch out, while slots have up to 1024 on average (rank 16, 4096 x 4096, four slots: 64 rows
-  // 24.7 -> 18.7 us, 4096 rows 49.9 -> 45.4; 2048 x 2048, one slot: 1024 rows 29.2 -> 26.9, 4096 rows 46.5 -> 60.5).
-  p.direct = rows <= 1024 * used;
+  // All of a slot's rows in a workgroup, which leaves the records and their launch out, while slots have up to 1536 on average, or 1024 of ranks above 32 (rank 16,
+  // 4096 x 4096, four slots: 64 rows 24.7 -> 18.7 us, 4096 rows 49.9 -> 45.4; 2048 x 2048, one slot: 1024 rows 29.2 -> 26.9; rank 32, 1500 rows 38.2 -> 36.1, 2048 37.2 -> 42.5).
+  p.direct = rows <= (p.tiles <= 2 ? 1536 : 1024) * used;
   // Otherwise a piece of 128 to 4096 rows, as long as it takes for the workgroups to be on the chip at once or nearly (with 64 entries of the rank
   // one a CU, for their registers: 4099 rows by 8192 columns, pieces of 512 rows 33 us and 11.6 to add them up, 1024 28.4 + 7.4, 2048 34.8 + 7.3)
   const int64_t columns = (in + kColumns - 1) / kColumns + (out + kColumns - 1) / kColumns, places = p.rtw == 4 ? 400 : p.rtw == 2 ? 512 : 1024;

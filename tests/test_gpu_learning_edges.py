@@ -410,6 +410,30 @@ def test_rows_of_nobody(ext, dtype):
     assert (ga[2] == 0).all() and (gb[2] == 0).all()
 
 
+@pytest.mark.parametrize("rank", [8, 32, 64, 128])
+@pytest.mark.parametrize("lengths", [[1, 20, 3], [200]])
+@pytest.mark.parametrize("tiny", [False, True])
+def test_rows_of_unlike_magnitude_in_half(ext, lengths, rank, tiny):
+    """fp16 rows from 2^-20 to 2^12 and banks down to its subnormal numbers: what lies between the two products has an exponent of its own for each row."""
+    dtype = torch.float16
+    c = make(lengths, list(range(len(lengths))), len(lengths), rank, 256, 264, dtype, seed=rank)
+    rows = sum(lengths)
+    gen = torch.Generator(device="cuda").manual_seed(rank)
+    size = 2.0 ** torch.randint(-20, 10, (rows, 1), generator=gen, device="cuda")
+    c["x"] = (c["x"].float() * size).to(dtype)
+    c["base"].zero_()
+    c["lora_b"] = (c["lora_b"].float() * (1e-6 if tiny else 1e-2)).to(dtype)
+    c["scaling"] = c["scaling"] * (300.0 if tiny else 0.01)
+    low = torch.empty(rows, rank, device="cuda")
+    out = call(ext, c, low=low)
+    want, want_low = lora_forward(c, dtype)
+    lora_close(low, want_low, "low")
+    lora_close(out, want, "out")
+    c["x"][0, 0] = float("inf")
+    bad = call(ext, c)
+    assert bad[0].isnan().any() and torch.equal(bad[1:], out[1:])
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
 @pytest.mark.parametrize("codes", [False, True])
 @pytest.mark.parametrize("lengths, adapters, slots, rank", [
