@@ -896,12 +896,13 @@ int row_tiles(int rows, int sequences, bool ragged) { return !ragged || rows < 2
 // shrink: one (many workgroups), two where the bank's rows weigh more than twice the activation's
 int shrink_tiles(int rows, int sequences, bool ragged, int rank) { return rank > 32 && row_tiles(rows, sequences, ragged) > 1 ? 2 : 1; }
 int pieces_of(int rows, int sequences, bool ragged, int nt) { return ragged ? rows / (16 * nt) + 2 * sequences : sequences; }
-// Parts of the reduction: for 768 workgroups, of a step a wave at least; up to eight for single rows, four for few pieces of rows, two for many
+// Parts of the reduction: for 768 workgroups, of a step a wave at least; up to eight for single rows and few pieces of rows, four for more, two for many
+// (14336 by 64, 2 to 340 rows: 13.2 to 21.9 us with four, 11.0 to 18.3 with eight, 10.4 to 19.4 with sixteen; 4096 by 128 13.4 to 19.5, 12.7 to 20.0, 13.0 to 24.6)
 // (4099 rows of 4096 by 64, one part: shrink 17.0 us, expand 24.4; two: 14.6 and 25.0; four: 13.8 and 26.5).
 int splits_of(int rows, int sequences, bool ragged, int width, int rank, int dtype) {
   const int nt = shrink_tiles(rows, sequences, ragged, rank);
   const int64_t real = ragged ? (rows + 16 * nt - 1) / (16 * nt) : sequences;
-  const int steps = (width * (dtype == LLMQ_F32 ? 4 : 2) + 127) / 128, most = !ragged ? 8 : real < 96 ? 4 : 2;
+  const int steps = (width * (dtype == LLMQ_F32 ? 4 : 2) + 127) / 128, most = !ragged ? 8 : real < 24 ? 8 : real < 96 ? 4 : 2;
   int64_t splits = 768 / (real < 1 ? 1 : real);
   if (splits > steps / shrink_waves(rank)) splits = steps / shrink_waves(rank);
   if (splits > most) splits = most;
