@@ -511,7 +511,7 @@ __global__ __launch_bounds__(kFewWaves * kWave) void few_outer_kernel(const T* _
     }
     here = __ballot(target >= 0);
   }
-  for (int c0 = (blockIdx.y * kFewWaves + wv) * 64; c0 < width; c0 += gridDim.y * kFewWaves * 64) {
+  for (int c0 = wv * 64; c0 < width; c0 += kFewWaves * 64) {
     tile_v4f acc[4][4] = {};
     const T* x = turned + (static_cast<int64_t>(c0 / 16) * steps * kWave + lane) * V;
     const auto multiply = [&](int step, const u32x4 (&b)[4]) {

@@ -275,7 +275,8 @@ __global__ __launch_bounds__(kExpandWaves * kWave) void expand_kernel(const Bank
     for (int k = 0; k < KT; ++k)
 #pragma unroll
       for (int mi = 0; mi < 8; ++mi)   // (past the rank the operand of `low` is zeros, against weights that are looked at a second time)
-        m[k][mi] = load16(static_cast<const T*>(bank.m) + (static_cast<int64_t>(a) * e.columns + min(c + mi, e.columns - 1)) * bank.rank + min((k * 4 + g) * V, bank.rank - V));
+        m[k][mi] = load16(static_cast<const T*>(bank.m) + (static_cast<int64_t>(a) * e.columns + min(c + mi, e.columns - 1)) * bank.rank +
+                          min((k * 4 + g) * V, bank.rank - V));
   }
   if (e.base != nullptr) {
 #pragma unroll
@@ -974,7 +975,8 @@ GradPlan grad_plan(int rows, int sequences, bool ragged, int in, int out, int ra
   // by four / two / one: 4096 x 14336 by 64, 32 rows 47 / 35 / 32, 1024 rows 62 / 53 / 52, 2048 77 / 70 / 79, 4096 113 / 118 / 151).
   p.rtw = p.tiles >= 4 && rows > 2048 ? 4 : p.tiles >= 2 && rows > 1024 ? 2 : 1;
   // All of a slot's rows in a workgroup, which leaves the records and their launch out, while slots have up to 1536 on average, or 1024 of ranks above 32 (rank 16,
-  // 4096 x 4096, four slots: 64 rows 24.7 -> 18.7 us, 4096 rows 49.9 -> 45.4; 2048 x 2048, one slot: 1024 rows 29.2 -> 26.9; rank 32, 1500 rows 38.2 -> 36.1, 2048 37.2 -> 42.5).
+  // 4096 x 4096, four slots: 64 rows 24.7 -> 18.7 us, 4096 rows 49.9 -> 45.4; 2048 x 2048, one slot: 1024 rows 29.2 -> 26.9; rank 32, 1500 rows 38.2 -> 36.1,
+  // 2048 37.2 -> 42.5).
   p.direct = rows <= (p.tiles <= 2 ? 1536 : 1024) * used;
   // Otherwise a piece of 128 to 4096 rows, as long as it takes for the workgroups to be on the chip at once or nearly (with 64 entries of the rank
   // one a CU, for their registers: 4099 rows by 8192 columns, pieces of 512 rows 33 us and 11.6 to add them up, 1024 28.4 + 7.4, 2048 34.8 + 7.3)
@@ -1037,7 +1039,8 @@ int check(int rows, int sequences, bool ragged, int in, int out, int rank, int s
   if (rank < 8 || rank > 128 || rank % 8) return llmq_host::fail_invalid("rank must be a multiple of 8 from 8 to 128, got %d", rank);
   if (in < 8 || out < 8 || in % 8 || out % 8 || in > (1 << 20) || out > (1 << 20))
     return llmq_host::fail_invalid("in_features and out_features must be multiples of 8 up to 2^20, got %d and %d", in, out);
-  if (rows > (1 << 20) || sequences > (1 << 20) || slots > (1 << 20)) return llmq_host::fail_invalid("at most 2^20 rows, sequences and slots, got %d, %d, %d", rows, sequences, slots);
+  if (rows > (1 << 20) || sequences > (1 << 20) || slots > (1 << 20))
+    return llmq_host::fail_invalid("at most 2^20 rows, sequences and slots, got %d, %d, %d", rows, sequences, slots);
   if ((rows / 16 + int64_t{2} * sequences) * ((in > out ? in : out) / 512 + 1) > (1 << 30))
     return llmq_host::fail_invalid("too many pieces: %d rows of %d sequences by %d x %d", rows, sequences, in, out);
   if (!ragged && rows != sequences) return llmq_host::fail_invalid("without query_start a sequence has one row: %d rows, %d sequences", rows, sequences);

@@ -318,7 +318,8 @@ template <typename T> struct FewPiece {
   int turned_ld;
 };
 template <typename T, int BITS, int NT>
-__global__ __launch_bounds__(kFewWaves * kWave, BITS != 0 && NT == 4 ? 1 : 2) void few_piece_kernel(const FewWeight weight, const T* __restrict__ x, const Counted rows, const FewPiece<T> out) {
+__global__ __launch_bounds__(kFewWaves * kWave, BITS != 0 && NT == 4 ? 1 : 2) void few_piece_kernel(const FewWeight weight, const T* __restrict__ x,
+                                                                                                    const Counted rows, const FewPiece<T> out) {
   using Few = FewRows<T, BITS, NT>;
   __shared__ __attribute__((aligned(16))) uint8_t s_mem[Few::kLdsBytes];
   const int m0 = blockIdx.x * kFewTokens, t0 = blockIdx.y * 16 * NT;
@@ -587,10 +588,9 @@ int few_backward(const Plan& p, const Call& c, const Counted& rows, void* grad_h
     const int64_t items = int64_t{p.hidden} / 16 * steps * kWave;
     hipLaunchKernelGGL((few_turned_kernel<T>), dim3(static_cast<unsigned>((items + 255) / 256)), dim3(256), 0, c.stream, static_cast<const T*>(c.hidden),
                        c.hidden_stride, rows.row, p.rows, p.hidden, steps, turned);
-    const dim3 outer(tokens, 1);
     const FewRests rests{rows.rest, rows.target, rows.row, rows.count, c.hidden, c.hidden_stride};
 #define LLMQ_OUTER(ONE)                                                                                                                             \
-  hipLaunchKernelGGL((few_outer_kernel<T, ONE>), outer, dim3(kFewWaves * kWave), 0, c.stream, part.turned, int64_t{p.padded}, turned, steps, rows.back, \
+  hipLaunchKernelGGL((few_outer_kernel<T, ONE>), dim3(tokens), dim3(kFewWaves * kWave), 0, c.stream, part.turned, int64_t{p.padded}, turned, steps, rows.back, \
                      p.vocab, p.hidden, rests, static_cast<T*>(grad_weight))
     if (sizeof(T) == 2 || p.blocks == 1) LLMQ_OUTER(true);
     else if constexpr (sizeof(T) == 4) LLMQ_OUTER(false);
@@ -628,7 +628,8 @@ int backward(const Plan& p, const Call& c, const int64_t* targets, int64_t ignor
   float* back = reinterpret_cast<float*>(c.workspace + p.o_back);
   const Counted rows{reinterpret_cast<int32_t*>(c.workspace + p.o_row), reinterpret_cast<int32_t*>(c.workspace + p.o_place),
                      reinterpret_cast<int64_t*>(c.workspace + p.o_target), reinterpret_cast<float*>(c.workspace + p.o_lse),
-                     reinterpret_cast<float*>(c.workspace + p.o_grad), reinterpret_cast<float*>(c.workspace + p.o_rest), back, reinterpret_cast<int32_t*>(c.workspace + p.o_back + 4)};
+                     reinterpret_cast<float*>(c.workspace + p.o_grad), reinterpret_cast<float*>(c.workspace + p.o_rest), back,
+                      reinterpret_cast<int32_t*>(c.workspace + p.o_back + 4)};
   float* sums = reinterpret_cast<float*>(c.workspace + p.o_sums);
   const bool learned = grad_weight != nullptr;
   const int rows64 = static_cast<int>(round_up(p.rows, 64));

@@ -3,9 +3,9 @@
 //   gx[t, k] = sum_n g[t, n] W[n, k],     W = (dtype)(code * scale): the matrix of the reference's many-rows branch
 //                                         (llmquant/quantizers/kernel.py:68-79), whose autograd this stands for
 //
-// Few rows: past the weight as it lies (dense_few.h). Otherwise the weight is brought to its values a piece of its rows at a time (dense_stage.h: a piece that the caches hold), and multiplied on the
-// matrix core with the reduction outermost, as it lies (dense_tile.h); sums over the pieces and over the splits of one go through fp32 planes. Bound: the
-// matrix core for training batches, the weight's way through memory and the conversion of its codes for few rows.
+// Few rows: past the weight as it lies (dense_few.h). Otherwise the weight is brought to its values a piece of its rows at a time (dense_stage.h: a piece that the
+// caches hold), and multiplied on the matrix core with the reduction outermost, as it lies (dense_tile.h); sums over the pieces and over the splits of one go
+// through fp32 planes. Bound: the matrix core for training batches, the weight's way through memory and the conversion of its codes for few rows.
 #include "dense_stage.h"
 
 namespace {
@@ -113,7 +113,8 @@ extern "C" int llmq_wq_linear_grad(const void* grad, int64_t grad_stride, const 
   if (N == 0) return llmq_host::fail_invalid("a weight of no rows");
   if (rows > (1 << 20) || N > (1 << 24) || static_cast<int64_t>(G) * keep_per_group > (1 << 24))
     return llmq_host::fail_invalid("at most 2^20 rows of 2^24 elements, got %d rows, %d x %lld", rows, N, static_cast<long long>(G) * keep_per_group);
-  if (grad_stride < N || grad_stride % 8 || grad_stride > (1 << 24)) return llmq_host::fail_invalid("grad's row stride must be a multiple of 8 of at least %d, got %lld", N, static_cast<long long>(grad_stride));
+  if (grad_stride < N || grad_stride % 8 || grad_stride > (1 << 24))
+    return llmq_host::fail_invalid("grad's row stride must be a multiple of 8 of at least %d, got %lld", N, static_cast<long long>(grad_stride));
   if (!grad || !qweight || !wscale || !grad_x) return llmq_host::fail_invalid("null tensor pointer");
   if ((reinterpret_cast<uintptr_t>(grad) | reinterpret_cast<uintptr_t>(qweight) | reinterpret_cast<uintptr_t>(grad_x)) & 15u)
     return llmq_host::fail_invalid("grad, qweight and grad_x must be 16-byte aligned");
