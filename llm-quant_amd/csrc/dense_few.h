@@ -190,7 +190,8 @@ template <typename T, int BITS, int NT> struct FewRows {
     u32x4 x[Step::kPackets][NT];
     float scale[BITS ? kTiles : 1];
   };
-  __device__ __forceinline__ void multiply(uint8_t* lds, const FewWeight& w, int m0, const T* x) {
+  // live: tiles of x that have rows (fp32, where the multiplications bind: the others are left out)
+  __device__ __forceinline__ void multiply(uint8_t* lds, const FewWeight& w, int m0, const T* x, int live) {
     const int lane = threadIdx.x & (kWave - 1), wv = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) / kWave), lr = lane & 15, g = lane >> 4;
     const int steps = w.width / Step::kK;
     uint8_t* const mine = lds + wv * 2 * Step::kBytes;
@@ -232,7 +233,8 @@ template <typename T, int BITS, int NT> struct FewRows {
         for (int i = 0; i < kTiles; ++i) {
           const u32x4 v = Step::operand(stage, i * 16 + lr, c, g, a.scale[BITS ? i : 0]);
 #pragma unroll
-          for (int j = 0; j < NT; ++j) sum[i][j] = few_mfma<T>(v, a.x[c][j], sum[i][j]);
+          for (int j = 0; j < NT; ++j)
+            if (sizeof(T) == 2 || j < live) sum[i][j] = few_mfma<T>(v, a.x[c][j], sum[i][j]);
         }
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // (the stage is asked for again)
     };
@@ -364,7 +366,8 @@ __global__ __launch_bounds__(kFewWaves * kWave, 2) void columns_kernel(const Few
       }
       const u32x4 operand{word[0], word[1], word[2], word[3]};
 #pragma unroll
-      for (int j = 0; j < NT; ++j) acc[j][q] = few_mfma<T>(now.g[j], operand, acc[j][q]);
+      for (int j = 0; j < NT; ++j)
+        if (sizeof(T) == 2 || t0 + j * 16 < rows) acc[j][q] = few_mfma<T>(now.g[j], operand, acc[j][q]);
     }
   };
   if (begin < v1) {   // (behind the last step: the part's last again)

@@ -136,6 +136,9 @@ __global__ __launch_bounds__(1024) void loss_kernel(const float2* __restrict__ s
               : target < 0 || target >= rows.vocab ? NAN : rest + (all.x - chosen[n]);
 }
 
+// tiles of 16 that have rows, of the block's NT
+template <int NT> __device__ __forceinline__ int live_tiles(int rows) { return min((rows - static_cast<int>(blockIdx.y) * 16 * NT + 15) / 16, NT); }
+
 // A few rows: 64 tokens a workgroup, a row tile of the sums a wave.
 template <typename T, int BITS, int NT>
 __global__ __launch_bounds__(kFewWaves * kWave, BITS != 0 && NT == 4 ? 1 : 2) void few_logits_kernel(const FewWeight weight, const T* __restrict__ x, const LossRows rows,
@@ -144,7 +147,7 @@ __global__ __launch_bounds__(kFewWaves * kWave, BITS != 0 && NT == 4 ? 1 : 2) vo
   __shared__ __attribute__((aligned(16))) uint8_t s_mem[Few::kLdsBytes];
   const int m0 = blockIdx.x * kFewTokens;
   Few f;
-  f.multiply(s_mem, weight, m0, x + static_cast<int64_t>(blockIdx.y) * 16 * NT * weight.width);
+  f.multiply(s_mem, weight, m0, x + static_cast<int64_t>(blockIdx.y) * 16 * NT * weight.width, live_tiles<NT>(rows.rows));
   const int lane = threadIdx.x & (kWave - 1), wv = threadIdx.x / kWave, n = (blockIdx.y * NT + wv) * 16 + (lane & 15), v0 = 4 * (lane >> 4);
   if (wv >= NT) return;
   float top = -INFINITY;
@@ -326,7 +329,7 @@ __global__ __launch_bounds__(kFewWaves * kWave, BITS != 0 && NT == 4 ? 1 : 2) vo
   const int lane = threadIdx.x & (kWave - 1), wv = threadIdx.x / kWave, n = t0 + wv * 16 + (lane & 15), v0 = 4 * (lane >> 4);
   Few f;
   const bool none = t0 >= *rows.count;   // (a block of rows that do not count: zeros)
-  if (!none) f.multiply(s_mem, weight, m0, x + static_cast<int64_t>(blockIdx.y) * 16 * NT * weight.width);
+  if (!none) f.multiply(s_mem, weight, m0, x + static_cast<int64_t>(blockIdx.y) * 16 * NT * weight.width, live_tiles<NT>(*rows.count));
   if (wv >= NT) return;
   const float g = rows.grad[n], lse = rows.lse[n];
   const int64_t target = rows.target[n] - m0;
