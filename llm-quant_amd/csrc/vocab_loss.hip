@@ -378,10 +378,11 @@ int64_t take(int64_t& at, int64_t bytes) {
 // that do not leave room for others (724 of 1024: 1726 us for all products with 768 MB, 1916 with 500, 1932 with 136).
 constexpr int64_t kLossPieceBytes = int64_t{192} << 20, kGradPieceBytes = int64_t{768} << 20;
 // Few rows: the whole vocabulary at once, up to 2^20 tokens. 64 rows a pass over the weight: one pass where it is as wide as the operands, more where the
-// tiles would have to make operands of it first or take six products (128256 x 2048: int8 in bf16, 128 rows 209 us for 337, 192 rows 353 for 350; fp32, 512 rows 2657
-// for 2777, with both gradients 256 rows 6355 for 6950, 512 rows 12600 for 7989).
+// tiles would have to make operands of it first or take six products (128256 x 2048: int8 in bf16, 128 rows 209 us for 337, 192 rows 353 for 350; fp32, 512 rows 2248
+// for 2777, 700 rows 3150 for 2713; with gradients 300 rows 6190 for 5847, over int8 4112 for 4616, of 50257 x 768 974 for 1289, 384 rows 7727, 5008 and 1171 for 6377,
+// 5018 and 1389).
 constexpr int kFewVocab = 1 << 20;
-constexpr int few_most(int wformat, int dtype, bool gradient) { return dtype == LLMQ_F32 ? (gradient ? 256 : 512) : wformat != 0 ? 128 : 64; }
+constexpr int few_most(int wformat, int dtype, bool gradient) { return dtype == LLMQ_F32 ? (gradient ? 320 : 512) : wformat != 0 ? 128 : 64; }
 
 Plan plan_for(int rows, int vocab, int hidden, int group_size, int wformat, int dtype, bool gradient, bool learned) {
   Plan p{};

@@ -20,14 +20,14 @@ struct Plan {
 };
 
 constexpr int64_t kPieceBytes = int64_t{128} << 20;
-// Up to so many rows the weight is read as it lies, once for each 64 (float16, bfloat16; whole calls, N x K int8: 4096 x 4096, 1 row 16 us for 33,
-// 256 rows 36 for 54; 14336 x 4096, 256 rows 85 for 112, 320 rows 145 for 125).
-constexpr int kFewMost = 256;
+// Up to so many rows the weight is read as it lies, once for each 64 (whole calls, N x K int8, bf16: 4096 x 4096, 1 row 16 us for 33, 256 rows 36 for 54; 14336 x 4096,
+// 256 rows 85 for 112, 320 rows 145 for 125; fp32, 2048 x 2048, 256 rows 36 for 100, 64 rows more 11 us, of 4096 x 4096 22, for 126).
+constexpr int few_most(int dtype) { return dtype == LLMQ_F32 ? 320 : 256; }
 
 Plan plan_for(int rows, int N, int width, int wformat, int dtype) {
   Plan p{};
   const int64_t row16 = dtype == LLMQ_F32 ? 6 : 2;
-  p.few = rows <= kFewMost;
+  p.few = rows <= few_most(dtype);
   if (p.few) {
     p.splits = few_splits(N, width, rows, wformat, dtype == LLMQ_F32);
     p.bytes = int64_t{4} * p.splits * rows * width;
