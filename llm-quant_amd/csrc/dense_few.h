@@ -415,14 +415,12 @@ __global__ __launch_bounds__(kFewWaves * kWave, 2) void columns_kernel(const Few
     }
 }
 // Splits of the weight's rows, 64 at the most. For 256 workgroups: more are only more planes (4096 x 4096 int8, 64 rows: 17 us with 256, 26 with 512, 39
-// with 1024; 16 rows: 9, 11 and 13). More where conversion or the fp32 matrix core binds and a wave still has 32 steps (128256 x 2048, 16 rows: int8 256 66 us, 512 56;
-// int4 58 and 48; bf16 88 and 93; fp32, 8 rows: 256 396, 512 252, 1024 190; 64 rows: 447, 423, 416).
-inline int few_splits(int weight_rows, int width, int rows, int bits, bool fp32) {
+// with 1024; 128256 x 2048, 16 rows: bf16 87, 92 and 95, int8 56, 55 and 59, fp32, 8 rows, 166, 169 and 179), but for 512 where int4's conversion binds and a wave
+// still has 16 steps (57, 46 and 43 with more planes to add; 64 rows 71, 61 and 66).
+inline int few_splits(int weight_rows, int width, int rows, int bits) {
   const int64_t groups = static_cast<int64_t>((width + kFewColumns - 1) / kFewColumns) * ((rows + 63) / 64), step = 32 * kFewWaves;
-  const int64_t most = (weight_rows + step - 1) / step;
-  int64_t places = fp32 ? (rows <= 32 ? 1024 : 512) : bits != 0 && rows <= 32 ? 512 : 256;
-  while (places > 256 && most < places / groups * 32) places /= 2;
-  const int64_t splits = places / groups < most ? places / groups : most;
+  const int64_t most = (weight_rows + step - 1) / step, places = bits == 4 && most >= 512 / groups * 16 ? 512 : 256;
+  const int64_t near = (places + groups / 2) / groups, splits = near < most ? near : most;
   return static_cast<int>(splits < 1 ? 1 : splits > 64 ? 64 : splits);
 }
 template <typename T, int BITS> inline void columns_launch_bits(const FewWeight& w, const FewColumns& c, hipStream_t stream) {

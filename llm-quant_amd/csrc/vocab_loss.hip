@@ -424,7 +424,7 @@ Plan plan_for(int rows, int vocab, int hidden, int group_size, int wformat, int 
       p.o_stats = take(at, round_up(vocab, kFewTokens) / kFewTokens * rows * 8);
       p.o_chosen = take(at, int64_t{4} * rows);
     } else {
-      p.splits = few_splits(vocab, hidden, rows, wformat, dtype == LLMQ_F32);
+      p.splits = few_splits(vocab, hidden, rows, wformat);
       p.o_p = take(at, p.size * whole_rows * p.piece);
       if (learned) {
         p.o_turned = take(at, int64_t{p.size} * hidden * p.padded);

@@ -29,7 +29,7 @@ Plan plan_for(int rows, int N, int width, int wformat, int dtype) {
   const int64_t row16 = dtype == LLMQ_F32 ? 6 : 2;
   p.few = rows <= few_most(dtype);
   if (p.few) {
-    p.splits = few_splits(N, width, rows, wformat, dtype == LLMQ_F32);
+    p.splits = few_splits(N, width, rows, wformat);
     p.bytes = int64_t{4} * p.splits * rows * width;
     return p;
   }
