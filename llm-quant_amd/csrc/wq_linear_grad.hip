@@ -20,14 +20,15 @@ struct Plan {
 };
 
 constexpr int64_t kPieceBytes = int64_t{128} << 20;
-// Up to so many rows the weight is read as it lies, once for each 64 (whole calls, N x K int8, bf16: 4096 x 4096, 1 row 16 us for 33, 256 rows 36 for 54; 14336 x 4096,
-// 256 rows 85 for 112, 320 rows 145 for 125; fp32, 2048 x 2048, 256 rows 36 for 100, 64 rows more 11 us, of 4096 x 4096 22, for 126).
-constexpr int few_most(int dtype) { return dtype == LLMQ_F32 ? 320 : 256; }
+// Up to so many rows the weight is read as it lies, once for each 64 (whole calls, us, this way for the other; bf16: 4096 x 4096 int8, 1 row 12 for 33, 320 rows 43 for
+// 46, 512 46 for 50; 14336 x 4096 int4, 320 rows 75 for 91, 384 rows 106 for 93; fp32, 2048 x 2048 int8, 320 rows 41 for 100; 14336 x 4096 int4, 320 rows 339 for 430,
+// 512 500 for 475; 4096 x 4096 int8, 320 rows 170 for 127).
+constexpr int kFewMost = 320;
 
 Plan plan_for(int rows, int N, int width, int wformat, int dtype) {
   Plan p{};
   const int64_t row16 = dtype == LLMQ_F32 ? 6 : 2;
-  p.few = rows <= few_most(dtype);
+  p.few = rows <= kFewMost;
   if (p.few) {
     p.splits = few_splits(N, width, rows, wformat);
     p.bytes = int64_t{4} * p.splits * rows * width;

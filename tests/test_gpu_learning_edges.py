@@ -76,7 +76,8 @@ def test_few_rows(ext, rows, vocab, width, group, out_group, bits, dtype):
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("rows, out, width, bits, group, keep, out_group", [
     (1, 4104, 256, 8, 128, 128, 0), (16, 24, 128, 4, 8, 8, 0), (17, 136, 384, 8, 128, 72, 0), (33, 1032, 128, 4, 128, 128, 100), (48, 8, 2048, 8, 64, 64, 0),
-    (128, 2056, 256, 4, 256, 256, 0), (129, 520, 136, 8, 8, 8, 3), (256, 264, 1024, 8, 128, 128, 0), (257, 264, 1024, 8, 128, 128, 0)])
+    (128, 2056, 256, 4, 256, 256, 0), (129, 520, 136, 8, 8, 8, 3), (256, 264, 1024, 8, 128, 128, 0), (257, 264, 1024, 8, 128, 128, 0), (320, 2056, 256, 4, 128, 128, 0),
+    (321, 264, 256, 8, 128, 128, 0)])
 def test_few_rows_of_a_linear(ext, rows, out, width, bits, group, keep, out_group, dtype):
     gen = torch.Generator(device="cuda").manual_seed(rows + out)
     stored, scale, codes = quantized(gen, out, width, bits, group, out_group)
