@@ -593,8 +593,8 @@ int llmq_kv_block_attention(const void* query, int64_t q_row_stride, const void*
 /* The gradient of a quantized Linear by its input: grad_x[t, k] = sum_n grad[t, n] W[n, k] with W = (dtype)(code * scale), the
  * matrix of the reference's many-rows branch (llmquant/quantizers/kernel.py:68-79; its autograd is PyTorch's). grad: [rows, N], row
  * stride in elements; qweight, wscale, keep_per_group (a multiple of 8) and out_group as for llmq_dequant_weight; grad_x: [rows, G *
- * keep_per_group], contiguous. N a multiple of 8, rows up to 2^20. fp32 sums; fp32 operands as three bfloat16 planes (2^-24 of a
- * product). Tensors 16-byte aligned. workspace: llmq_wq_linear_grad_workspace_bytes(...) bytes, 16-byte aligned, needs no
+ * keep_per_group], contiguous. N a multiple of 8, rows up to 2^20, 256 neighbouring rows of grad within 4 GiB. fp32 sums; fp32 operands as three
+ * bfloat16 planes (2^-24 of a product). Tensors 16-byte aligned. workspace: llmq_wq_linear_grad_workspace_bytes(...) bytes, 16-byte aligned, needs no
  * clearing; calls that overlap in time need one each. */
 size_t llmq_wq_linear_grad_workspace_bytes(int rows, int N, int G, int keep_per_group, int wformat, int dtype);
 int llmq_wq_linear_grad(const void* grad, int64_t grad_stride, const void* qweight, const float* wscale, void* grad_x,
@@ -611,7 +611,7 @@ int llmq_wq_linear_grad(const void* grad, int64_t grad_stride, const void* qweig
  * gradient NaN and grad_weight NaN. lse: as llmq_vocab_loss gave it. Logits and sums in fp32; P is rounded to `dtype` (fp32: three bfloat16
  * planes, few rows not at all), with grad scaled by a power of two to at most 2; what that takes from a target's own entry is added to the gradients
  * in fp32 (grad_weight: rounded to `dtype` again). Gradients are rounded once. hidden_size a multiple of 8, up
- * to 65536; rows up to 2^20, vocab up to 2^24; tensors 16-byte aligned. No rows: nothing is written (grad_weight neither). workspace:
+ * to 65536; rows up to 2^20 (256 neighbouring ones of hidden within 4 GiB, for the loss), vocab up to 2^24; tensors 16-byte aligned. No rows: nothing is written (grad_weight neither). workspace:
  * ..._workspace_bytes(...) bytes, 16-byte aligned, needs no clearing; calls that overlap in time need one each. */
 size_t llmq_vocab_loss_workspace_bytes(int rows, int vocab, int hidden_size, int group_size, int wformat, int dtype);
 int llmq_vocab_loss(const void* hidden, int64_t hidden_stride, const void* weight, const float* wscale_or_null,
@@ -632,7 +632,7 @@ int llmq_vocab_loss_grad(const void* hidden, int64_t hidden_stride, const void* 
  * [sequences + 1], not decreasing; NULL: row b, rows == sequences); rows of no sequence are base. low_or_null: fp32 [rows, rank],
  * zeros without an adapter; the gradient wants it. Sums in fp32, out rounded once; for 16-bit types low enters the second product as
  * two bfloat16 (16 bits of it; fp16: two fp16 with an exponent a row, 22 bits; one row a sequence beside small banks: as it is). rank a multiple of 8 from 8 to 128 (an adapter of a lower rank has zeros behind it), in and out
- * multiples of 8; tensors 16-byte aligned. workspace: ..._workspace_bytes(...) bytes (ragged: whether there is a query_start),
+ * multiples of 8; 32 neighbouring rows of x (of grad, backwards) within 4 GiB; tensors 16-byte aligned. workspace: ..._workspace_bytes(...) bytes (ragged: whether there is a query_start),
  * 16-byte aligned, needs no clearing; calls that overlap in time need one each.
  *
  * llmq_lora_grad: from grad, the gradient of out,

@@ -49,10 +49,15 @@ template <> struct TileType<float> { using type = bf16_t; static constexpr int k
 struct TileOperand {
   const void* base;
   int64_t plane_bytes;   // between the planes of an fp32 matrix
-  int64_t row_bytes;     // below 2^25
+  int64_t row_bytes;     // a lane's offset into a tile has 32 bits: tile_spans
   int rows;
   int k_rows;
 };
+
+// Whether the rows of a tile lie close enough for that: the first to the last of `tile` rows, each `row_bytes` behind the one before, and a step of a row.
+inline bool tile_spans(int rows, int tile, int64_t row_bytes, int64_t step_bytes) {
+  return ((rows < tile ? rows : tile) - 1) * row_bytes + step_bytes <= int64_t{0xffffffff};
+}
 
 // tile of a launch for a workgroup: workgroups go to the eight XCDs in turn, and an XCD takes a contiguous run of tiles, so
 // that tiles that share an operand share its L2

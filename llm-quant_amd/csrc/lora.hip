@@ -1051,6 +1051,13 @@ int bad_stride(int64_t stride, int width, int packet, const char* what) {
   if (stride >= width && stride % packet == 0) return 0;
   return llmq_host::fail_invalid("%s's row stride must be a multiple of %d of at least %d, got %lld", what, packet, width, static_cast<long long>(stride));
 }
+// (a piece's rows are offsets of 32 bits from its first)
+int wide_stride(int64_t stride, int width, int rows, int sequences, bool ragged, int rank, int dtype, const char* what) {
+  const int size = dtype == LLMQ_F32 ? 4 : 2, piece = ragged ? 16 * shrink_tiles(rows, sequences, ragged, rank) : 1;
+  if (tile_spans(rows, piece, stride * size, int64_t{width} * size)) return 0;
+  return llmq_host::fail_invalid("%s's row stride is too wide: %d neighbouring rows must lie within 4 GiB, got a stride of %lld elements", what, piece,
+                                 static_cast<long long>(stride));
+}
 
 }  // namespace
 
@@ -1070,6 +1077,7 @@ extern "C" int llmq_lora_add(const void* x, int64_t x_stride, const void* base, 
   const int v = dtype == LLMQ_F32 ? 4 : 8;
   if (int rc = bad_stride(x_stride, in_features, v, "x")) return rc;
   if (int rc = bad_stride(base_stride, out_features, v, "base")) return rc;
+  if (int rc = wide_stride(x_stride, in_features, rows, sequences, ragged, rank, dtype, "x")) return rc;
   if (out == base && base_stride != out_features) return llmq_host::fail_invalid("out in place of base needs contiguous rows");
   if (misaligned(x) || misaligned(base) || misaligned(out) || misaligned(lora_a) || misaligned(lora_b) || misaligned(low_or_null))
     return llmq_host::fail_invalid("all tensors must be 16-byte aligned");
@@ -1124,6 +1132,7 @@ extern "C" int llmq_lora_grad(const void* grad, int64_t grad_stride, const void*
   if (!grad || !x || !low || !lora_a || !lora_b || !scaling || !adapter || !grad_x || !grad_a || !grad_b) return llmq_host::fail_invalid("null tensor pointer");
   const int v = dtype == LLMQ_F32 ? 4 : 8;
   if (int rc = bad_stride(grad_stride, out_features, v, "grad")) return rc;
+  if (int rc = wide_stride(grad_stride, out_features, rows, sequences, ragged, rank, dtype, "grad")) return rc;
   if (int rc = bad_stride(x_stride, in_features, x_scale_or_null ? 16 : v, "x")) return rc;
   if (grad_base_or_null)
     if (int rc = bad_stride(base_stride, in_features, v, "grad_base")) return rc;

@@ -1782,6 +1782,12 @@ at::Tensor own_rows(const at::Tensor& t) {
   const bool overlap = t.size(0) > 1 && t.stride(0) < t.size(1);
   return packet_rows(overlap ? t.contiguous() : t);
 }
+// ... and `near` neighbouring rows within 4 GiB, which is as far as the kernels' offsets into a tile go
+at::Tensor near_rows(const at::Tensor& t, int64_t near) {
+  const auto rows = own_rows(t);
+  const int64_t last = std::min(rows.size(0), near) - 1;
+  return last > 0 && (last * rows.stride(0) + rows.size(1)) * rows.element_size() > int64_t{0xffffffff} ? rows.contiguous() : rows;
+}
 // stride of rows that may be none
 int64_t own_stride(const at::Tensor& t) { return t.size(0) <= 1 ? t.size(1) : t.stride(0); }
 
@@ -1821,7 +1827,7 @@ at::Tensor wq_linear_grad(const at::Tensor& grad, const at::Tensor& qweight, con
   if (out.numel() == 0) return out;
   if (w.rows == 0) return out.zero_();
   const c10::OptionalDeviceGuard guard(at::device_of(grad));
-  const auto gr = own_rows(grad);
+  const auto gr = near_rows(grad, 256);
   const size_t need = llmq_wq_linear_grad_workspace_bytes(static_cast<int>(rows), static_cast<int>(w.rows), static_cast<int>(w.groups),
                                                           static_cast<int>(keep_per_group), w.format, dtype);
   const auto workspace = at::empty({static_cast<int64_t>(need)}, grad.options().dtype(at::kByte));
@@ -1876,7 +1882,7 @@ std::tuple<at::Tensor, at::Tensor> vocab_loss(const at::Tensor& hidden, const at
   const auto options = hidden.options().dtype(at::kFloat);
   auto losses = at::empty({rows}, options), lse = at::empty({rows}, options);
   const c10::OptionalDeviceGuard guard(at::device_of(hidden));
-  const auto hr = own_rows(hidden);
+  const auto hr = near_rows(hidden, 256);
   const auto wt = packet_rows(weight.reshape({1, weight.numel()}));
   const auto tr = targets.contiguous();
   const size_t need = llmq_vocab_loss_workspace_bytes(static_cast<int>(rows), static_cast<int>(v.tokens), static_cast<int>(hidden.size(1)),
@@ -1965,7 +1971,7 @@ at::Tensor lora_add(const at::Tensor& x, const at::Tensor& base, const at::Tenso
   const Adapters l = adapters_of(x, lora_a, lora_b, scaling, adapter, query_start, rows);
   TORCH_CHECK(x.size(1) == l.in && base.size(1) == l.out, "the adapters are ", l.in, " x ", l.out, ", x and base ", x.size(1), " x ", base.size(1));
   const c10::OptionalDeviceGuard guard(at::device_of(x));
-  const auto xr = own_rows(x), br = own_rows(base);
+  const auto xr = near_rows(x, 32), br = own_rows(base);
   at::Tensor result;
   if (out.has_value() && out->defined()) {
     TORCH_CHECK(out->device() == x.device() && out->scalar_type() == x.scalar_type() && out->is_contiguous() && out->dim() == 2 &&
@@ -2042,7 +2048,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> lora_grad(const at::Tensor& grad,
     return {grad_x, at::zeros_like(lora_a), at::zeros_like(lora_b)};
   }
   auto grad_a = at::empty_like(lora_a), grad_b = at::empty_like(lora_b);
-  const auto gr = own_rows(grad), xr = own_rows(x), lr = packet_rows(low.contiguous());
+  const auto gr = near_rows(grad, 32), xr = own_rows(x), lr = packet_rows(low.contiguous());
   const size_t need = llmq_lora_grad_workspace_bytes(static_cast<int>(rows), l.sequences, l.start.defined(), static_cast<int>(l.in),
                                                      static_cast<int>(l.out), static_cast<int>(l.rank), static_cast<int>(l.slots), dtype);
   const auto workspace = at::empty({static_cast<int64_t>(need)}, grad.options().dtype(at::kByte));

@@ -691,6 +691,9 @@ extern "C" int llmq_vocab_loss(const void* hidden, int64_t hidden_stride, const 
   if (!hidden || !weight || !targets || !losses || !lse || (wformat != 0 && !wscale_or_null)) return llmq_host::fail_invalid("null tensor pointer");
   if (misaligned(hidden) || misaligned(weight)) return llmq_host::fail_invalid("hidden and weight must be 16-byte aligned");
   const Plan p = plan_for(rows, vocab, hidden_size, group_size, wformat, dtype, false, false);
+  if (!p.few && !p.stage_hidden && !tile_spans(rows, tile_rows(rows), 2 * hidden_stride, 128))
+    return llmq_host::fail_invalid("hidden's row stride is too wide: %d neighbouring rows must lie within 4 GiB, got a stride of %lld elements", tile_rows(rows),
+                                   static_cast<long long>(hidden_stride));
   if (!workspace || misaligned(workspace) || workspace_bytes < static_cast<size_t>(p.bytes))
     return llmq_host::fail_invalid("the workspace must be 16-byte aligned and hold %lld bytes, got %zu", static_cast<long long>(p.bytes), workspace_bytes);
   const Call c{hidden, weight, wscale_or_null, hidden_stride, group_size, out_group, wformat, static_cast<uint8_t*>(workspace), static_cast<hipStream_t>(stream)};

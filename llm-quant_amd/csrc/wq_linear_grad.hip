@@ -120,6 +120,9 @@ extern "C" int llmq_wq_linear_grad(const void* grad, int64_t grad_stride, const 
   if ((reinterpret_cast<uintptr_t>(grad) | reinterpret_cast<uintptr_t>(qweight) | reinterpret_cast<uintptr_t>(grad_x)) & 15u)
     return llmq_host::fail_invalid("grad, qweight and grad_x must be 16-byte aligned");
   const Plan p = plan_for(rows, N, G * keep_per_group, wformat, dtype);
+  if (!p.few && !tile_spans(rows, tile_rows(rows), 2 * (p.stage_grad ? p.n_padded : grad_stride), 128))
+    return llmq_host::fail_invalid("grad's row stride is too wide: %d neighbouring rows must lie within 4 GiB, got a stride of %lld elements", tile_rows(rows),
+                                   static_cast<long long>(grad_stride));
   if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 15u) || workspace_bytes < static_cast<size_t>(p.bytes))
     return llmq_host::fail_invalid("the workspace must be 16-byte aligned and hold %lld bytes, got %zu", static_cast<long long>(p.bytes), workspace_bytes);
   hipStream_t s = static_cast<hipStream_t>(stream);
