@@ -609,7 +609,8 @@ int llmq_wq_linear_grad(const void* grad, int64_t grad_stride, const void* qweig
  * (dtype)(code * scale) and have no gradient. losses, lse, grad: fp32 [rows]. A row whose target is ignore_index has loss 0 and
  * no part in a gradient, whatever it holds; any other target outside [0, vocab) makes the row's loss NaN, its
  * gradient NaN and grad_weight NaN. lse: as llmq_vocab_loss gave it. Logits and sums in fp32; P is rounded to `dtype` (fp32: three bfloat16
- * planes, few rows not at all), with grad scaled by a power of two to at most 2; what that takes from a target's own entry is added to the gradients
+ * planes, few rows not at all), with grad scaled by a power of two, a row's own, or with grad_weight that of the largest |grad| (in fp16 entries keep their
+ * bits down to 2^-28 of it, and a step of 2^-38 below); what that takes from a target's own entry is added to the gradients
  * in fp32 (grad_weight: rounded to `dtype` again). Gradients are rounded once. hidden_size a multiple of 8, up
  * to 65536; rows up to 2^20 (256 neighbouring ones of hidden within 4 GiB, for the loss), vocab up to 2^24; tensors 16-byte aligned. No rows: nothing is written (grad_weight neither). workspace:
  * ..._workspace_bytes(...) bytes, 16-byte aligned, needs no clearing; calls that overlap in time need one each. */

@@ -437,7 +437,7 @@ template <typename T, bool DENSE> inline void columns_launch(const FewWeight& w,
   else columns_launch_bits<T, 4>(w, c, stream);
 }
 
-// out[row] = (dtype)(scale * the sum of the planes' row `from[row]`); no such row (negative): zeros
+// out[row] = (dtype)(scale[from] * the sum of the planes' row from = `from[row]`); no such row (negative): zeros
 template <typename T>
 __global__ __launch_bounds__(256) void add_few_kernel(const float* __restrict__ planes, const int splits, const int rows, const int width,
                                                       const float* __restrict__ scale_or_null, const int32_t* __restrict__ from_or_null, const TargetTerm term,
@@ -460,7 +460,7 @@ __global__ __launch_bounds__(256) void add_few_kernel(const float* __restrict__ 
         if (z0 + z < splits) sum += v[z];
     }
   }
-  const float scale = scale_or_null != nullptr ? *scale_or_null : 1.0f;
+  const float scale = scale_or_null != nullptr && from >= 0 ? scale_or_null[from] : 1.0f;
   float f[4] = {sum[0], sum[1], sum[2], sum[3]};
   if (from >= 0 && term.rest != nullptr) term.add<T>(from, c, f);
 #pragma unroll

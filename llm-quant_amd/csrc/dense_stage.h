@@ -299,7 +299,8 @@ inline void product_launch(const TileOperand& a, const TileOperand& b, int k, co
   else hipLaunchKernelGGL((product_kernel<T, 256, 256, 4, 2, SUMS, B_K>), dim3(groups), dim3(512), 0, stream, a, b, k, m_tiles, out);
 }
 
-// out[n, m] = (dtype)(scale * the sum of the planes), eight values a lane. from: the planes' row behind each row (negative: zeros), or null.
+// out[n, m] = (dtype)(scale * the sum of the planes), eight values a lane. from: the planes' row behind each row (negative: zeros), and with it scale: a value for
+// each of the planes' rows; or null.
 template <typename T>
 __global__ __launch_bounds__(256) void add_planes_kernel(const float* __restrict__ planes, const int rows, const int tn, const int m_tiles, const int most,
                                                          const int32_t* __restrict__ count_or_null, const float* __restrict__ scale_or_null,
@@ -309,7 +310,6 @@ __global__ __launch_bounds__(256) void add_planes_kernel(const float* __restrict
   const Splits s = splits_of_rows(count_or_null == nullptr ? rows : min(rows, *count_or_null), tn, m_tiles, per_row * int64_t{8}, most);
   const int64_t plane = s.plane;
   const int splits = s.splits;
-  const float scale = scale_or_null == nullptr ? 1.0f : *scale_or_null;
   for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < packets; i += static_cast<int64_t>(gridDim.x) * 256) {
     float f[8] = {};
     int64_t at = i;
@@ -343,6 +343,7 @@ __global__ __launch_bounds__(256) void add_planes_kernel(const float* __restrict
       term.add<T>(from, c, f);
       term.add<T>(from, c + 4, f + 4);
     }
+    const float scale = scale_or_null == nullptr || from < 0 ? 1.0f : scale_or_null[from];
 #pragma unroll
     for (int e = 0; e < 8; ++e) f[e] *= scale;
 #pragma unroll

@@ -11,7 +11,9 @@
 // call (fp32: three planes), as the operand of the two products behind it. P is rounded to that type, relative to each value; what that takes from the
 // entry of the row's target, nearly all of a row where the others share what is left, is kept in fp32 and added to the results (with it rounded away
 // gradients are 2^-8 off where their own rounding is 2^-9; 2000 rows of 32000 x 2048, the weight's gradient 329 -> 352 us); g is scaled by a power of two
-// first, so that a mean over many rows does not leave fp16's range, and the results are scaled back.
+// first, a row's own where the weight does not learn and the largest row's where it does, so that a mean over many rows does not leave the type's range,
+// and the results are scaled back. |P| is at most the scaled g: to [1, 2), for fp16 to [2^14, 2^15), so that its small entries keep their bits
+// down to 2^-28 of that and a step of 2^-38 below (at [1, 2), a row of a thousandth of the largest g lost most of a softmax over 128256 tokens).
 // A quantized head (the model's lm_head) is brought to the values of its dense form piece by piece. Few rows (few_most) go past the weight as it lies
 // instead, dense or codes (dense_few.h; 16 rows of 128256 x 2048, bf16: the tiles' kernel 115 us, this one 87, 6.0 TB/s).
 #include "dense_stage.h"
@@ -188,14 +190,17 @@ struct Counted {
   int32_t* place;      // [rows]: where a row went, or -1
   int64_t* target;     // [padded]
   float* lse;          // [padded]
-  float* grad;         // [padded]: g 2^-e with e the exponent of the largest finite |g|; 0 behind the last
+  float* grad;         // [padded]: g 2^(lift - e) with e its own exponent, or (together) that of the largest finite |g|; 0 behind the last
   float* rest;         // [padded], 16 bits: what P's rounding took from the target's entry
-  float* back;         // 2^e
+  float* back;         // [padded]: 2^(e - lift)
   int32_t* count;
 };
+// (2^(e - lift) stays a normal number)
+__device__ __forceinline__ int exponent_of(float g, int lift) { return g > 0.0f && g < INFINITY ? max(ilogbf(g), lift - 125) : lift; }
 // One workgroup.
 __global__ __launch_bounds__(1024) void count_rows_kernel(const float* __restrict__ grad, const int64_t* __restrict__ targets, const float* __restrict__ lse,
-                                                          const int rows, const int padded, const int vocab, const int64_t ignore_index, const Counted c) {
+                                                          const int rows, const int padded, const int vocab, const int64_t ignore_index, const bool together,
+                                                          const int lift, const Counted c) {
   __shared__ float s_top[16];
   __shared__ int s_n[2][16];
   const int wv = threadIdx.x / kWave, lane = threadIdx.x % kWave;
@@ -209,7 +214,7 @@ __global__ __launch_bounds__(1024) void count_rows_kernel(const float* __restric
   __syncthreads();
   top = s_top[0];
   for (int w = 1; w < 16; ++w) top = fmaxf(top, s_top[w]);
-  const int e = top > 0.0f ? min(max(ilogbf(top), -125), 125) : 0;
+  const int largest = exponent_of(top, lift);
   int begin = 0;
   for (int i0 = 0, turn = 0; i0 < rows; i0 += 1024, turn ^= 1) {
     const int i = i0 + threadIdx.x;
@@ -235,7 +240,9 @@ __global__ __launch_bounds__(1024) void count_rows_kernel(const float* __restric
       c.target[at] = target;
       c.lse[at] = lse[i];
       c.rest[at] = 0.0f;
-      c.grad[at] = target < 0 || target >= vocab ? NAN : ldexpf(g, -e);
+      const int e = together ? largest : exponent_of(fabsf(g), lift);
+      c.grad[at] = target < 0 || target >= vocab ? NAN : ldexpf(g, lift - e);
+      c.back[at] = ldexpf(1.0f, e - lift);
     }
     begin += all;
   }
@@ -244,12 +251,10 @@ __global__ __launch_bounds__(1024) void count_rows_kernel(const float* __restric
     c.target[i] = -1;
     c.lse[i] = 0.0f;
     c.grad[i] = 0.0f;
+    c.back[i] = ldexpf(1.0f, largest - lift);
     c.rest[i] = 0.0f;
   }
-  if (threadIdx.x == 0) {
-    *c.back = ldexpf(1.0f, e);
-    *c.count = begin;
-  }
+  if (threadIdx.x == 0) *c.count = begin;
 }
 
 struct PieceOut {
@@ -363,7 +368,7 @@ struct Plan {
   bool few;                                // rows that go past the weight once, as it lies
   int row_tiles, blocks;                   // of 16, for these: 1, 2 or 4; of 16 row_tiles rows
   // offsets into the workspace
-  int64_t o_stats, o_chosen, o_hidden, o_weight, o_row, o_place, o_target, o_lse, o_grad, o_rest, o_back, o_x, o_p, o_turned, o_p_turned, o_sums, bytes;
+  int64_t o_stats, o_chosen, o_hidden, o_weight, o_row, o_place, o_target, o_lse, o_grad, o_rest, o_back, o_count, o_x, o_p, o_turned, o_p_turned, o_sums, bytes;
 };
 
 int64_t take(int64_t& at, int64_t bytes) {
@@ -440,7 +445,8 @@ Plan plan_for(int rows, int vocab, int hidden, int group_size, int wformat, int 
     p.o_lse = take(at, int64_t{4} * p.padded);
     p.o_grad = take(at, int64_t{4} * p.padded);
     p.o_rest = take(at, int64_t{4} * p.padded);
-    p.o_back = take(at, 8);
+    p.o_back = take(at, int64_t{4} * p.padded);
+    p.o_count = take(at, 4);
   }
   if (p.few) {
     p.bytes = at;
@@ -633,11 +639,12 @@ int backward(const Plan& p, const Call& c, const int64_t* targets, int64_t ignor
   const Counted rows{reinterpret_cast<int32_t*>(c.workspace + p.o_row), reinterpret_cast<int32_t*>(c.workspace + p.o_place),
                      reinterpret_cast<int64_t*>(c.workspace + p.o_target), reinterpret_cast<float*>(c.workspace + p.o_lse),
                      reinterpret_cast<float*>(c.workspace + p.o_grad), reinterpret_cast<float*>(c.workspace + p.o_rest), back,
-                      reinterpret_cast<int32_t*>(c.workspace + p.o_back + 4)};
+                     reinterpret_cast<int32_t*>(c.workspace + p.o_count)};
   float* sums = reinterpret_cast<float*>(c.workspace + p.o_sums);
   const bool learned = grad_weight != nullptr;
   const int rows64 = static_cast<int>(round_up(p.rows, 64));
-  hipLaunchKernelGGL(count_rows_kernel, dim3(1), dim3(1024), 0, c.stream, grad, targets, lse, p.rows, p.padded, p.vocab, ignore_index, rows);
+  hipLaunchKernelGGL(count_rows_kernel, dim3(1), dim3(1024), 0, c.stream, grad, targets, lse, p.rows, p.padded, p.vocab, ignore_index, learned,
+                     dtype == LLMQ_F16 ? 14 : 0, rows);
   if (p.few) return few_backward<T>(p, c, rows, grad_hidden, grad_weight);
   stage_hidden<T>(p, c, rows.row);
   const TileOperand hidden = hidden_operand(p, c);

@@ -1,11 +1,13 @@
-"""Learning where sizes, strides and memory end: rows far apart, what a call touches beside its outputs. Bounds as in test_gpu_vocab_loss.py and
-test_gpu_lora.py."""
+"""Learning where sizes, types and memory end: rows far apart, weights of rows far apart, what a call touches beside its outputs. Bounds as in
+test_gpu_vocab_loss.py and test_gpu_lora.py."""
+
+import math
 
 import pytest
 import torch
 from test_gpu_learning_edges import ext, loss_and_gradients, same  # noqa: F401 (ext: a fixture)
 from test_gpu_lora import call, call_grad, make
-from test_gpu_vocab_loss import case, quantized
+from test_gpu_vocab_loss import DTYPES, F32, U, case, close, dense_of, quantized, sum_error
 
 pytestmark = pytest.mark.gpu
 
@@ -55,3 +57,56 @@ def test_rows_of_a_request_far_apart(ext, room):  # noqa: F811
         far = dict(c, x=apart(room, c["x"], stride))
         assert torch.equal(call(ext, far), want[0])
         assert torch.equal(call_grad(ext, dict(c, grad=apart(room, c["grad"], stride)), low)[0], want[1])
+
+
+def bounded(c, learned):
+    """(dh, dW) in 64 bits with their bounds (those of test_gpu_vocab_loss.py), where an entry of P is off by half a step of the type and, in fp16, by at most half
+    a step of 2^-38 of the power of two below |g|, the row's own or, where the weight learns, the largest."""
+    hidden, _, _, dense, targets, grad = c
+    dtype, (h, w, g) = hidden.dtype, (t.double() for t in (hidden, dense, grad))
+    logits, size = h @ w.T, h.abs() @ w.abs().T
+    d = (sum_error(h.shape[1], dtype) * size).amax(-1)
+    lse = torch.logsumexp(logits, -1)
+    lse_tol = d + (128 + len(w) / 256) * F32 + 4 * F32 * (lse.abs() + math.log(len(w)) + 20)
+    p = torch.exp(logits - lse[:, None])
+    part = p.clone()
+    part[torch.arange(len(h), device="cuda"), targets] -= 1.0
+    part *= g[:, None]
+    p_tol = p * g.abs()[:, None] * (2 * (d + lse_tol) + 8 * F32)[:, None] + U[dtype] * 1.01 * part.abs()
+    small = 0.0
+    if dtype == torch.float16:
+        power = torch.exp2(torch.floor(torch.log2(g.abs())))
+        p_tol, small = p_tol + 2.0 ** -39 * (power.max() if learned else power[:, None]), 2.0 ** -25
+    out = []
+    for value, tol in ((part @ w, p_tol @ w.abs() + sum_error(len(w) + 64, dtype) * (part.abs() @ w.abs())),
+                       (part.T @ h, p_tol.T @ h.abs() + sum_error(len(h) + 64, dtype) * (part.abs().T @ h.abs()))):
+        out.append((value, tol + U[dtype] * (value.abs() + tol) + small))
+    return out
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows", [40, 200])
+@pytest.mark.parametrize("bits, spread", [(0, 10), (8, 10), (8, 20)])
+def test_rows_of_unlike_weight(ext, bits, spread, rows, dtype):  # noqa: F811
+    """Gradients of losses that count unlike, over a head with a common part in all its rows: what a row of little weight has of the softmax must not be lost
+    beside the largest (p is about 2^-15 here), nor a token's row of dW that is no row's target."""
+    vocab, width = 20011, 256
+    gen = torch.Generator(device="cuda").manual_seed(rows + spread)
+    common = 0.5 * torch.randn(width, generator=gen, device="cuda")
+    weight, scale = (common + 0.05 * torch.randn(vocab, width, generator=gen, device="cuda")).to(dtype), None
+    dense = weight
+    if bits:
+        codes = (weight.float() * 48).round().clamp(-128, 127).unflatten(1, (-1, 128))
+        scale = (1 + torch.rand(vocab, width // 128, generator=gen, device="cuda")) / 64
+        weight, dense = codes.to(torch.int8), dense_of(codes, scale, dtype)
+    hidden = torch.randn(rows, width, generator=gen, device="cuda").to(dtype)
+    targets = torch.randint(0, vocab, (rows,), generator=gen, device="cuda")
+    grad = 2.0 ** (6 if spread == 10 else 13) * torch.exp2(-spread * torch.rand(rows, generator=gen, device="cuda"))
+    grad *= torch.where(torch.rand(rows, generator=gen, device="cuda") < 0.5, -1.0, 1.0)
+    c = hidden, weight, scale, dense, targets, grad
+    for learned in (False, True)[: 1 if bits else 2]:
+        _, _, dh, dw = loss_and_gradients(ext, c, learned)
+        want = bounded(c, learned)
+        close(dh, want[0], "dh")
+        if learned:
+            close(dw, want[1], "dW")
