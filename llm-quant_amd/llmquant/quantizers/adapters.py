@@ -33,6 +33,7 @@ class AdapterBatch:
         self._query_start: torch.Tensor | None = None
         self._requests = 1
         self._captured: list[torch.Tensor] = []   # what captured steps read
+        self._held(1)   # (so that a step captured before anything was selected has it)
 
     def select(self, adapter, query_start=None) -> None:
         """adapter: a slot for each request (a list, or a tensor on any device; negative: none). query_start: int32 [requests + 1] on the device,
@@ -53,9 +54,15 @@ class AdapterBatch:
             held.fill_(-1)
         self._requests, self._query_start = 1, None
 
+    def _capturing(self) -> bool:
+        return self.device.type == "cuda" and torch.cuda.is_current_stream_capturing()
+
     def _held(self, requests: int) -> torch.Tensor:
         held = self._adapters.get(requests)
         if held is None:
+            # (made in a capture it would lie in the graph's memory, and every replay would set it to nobody again)
+            if self._capturing():
+                raise RuntimeError(f"{requests} requests are selected for the first time while a step is captured: select as many before")
             held = self._adapters[requests] = torch.full((requests,), -1, dtype=torch.int32, device=self.device)
         return held
 
@@ -71,9 +78,9 @@ class AdapterBatch:
                 start = torch.arange(0, count + 1, max(count // requests, 1), dtype=torch.int32, device=self.device)[: requests + 1]
                 if count == 0:
                     start = torch.zeros(requests + 1, dtype=torch.int32, device=self.device)
-                if not (start.is_cuda and torch.cuda.is_current_stream_capturing()):   # (else it lives in the graph's memory)
+                if not self._capturing():   # (else it lives in the graph's memory)
                     self._starts[count, requests] = start
-        elif start is not None and start.is_cuda and torch.cuda.is_current_stream_capturing() and not any(t is start for t in self._captured):
+        elif start is not None and self._capturing() and not any(t is start for t in self._captured):
             self._captured.append(start)
         return self._held(requests), start
 

@@ -1,0 +1,64 @@
+"""Who has which adapter, as captured steps, several streams and calls of unlike sizes read it."""
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+
+def batch_and_bank(slots=3):
+    from llmquant.quantizers.adapters import AdapterBatch, LoraAdapters
+
+    batch = AdapterBatch("cuda")
+    bank = LoraAdapters(64, 64, 8, slots, 16.0, torch.bfloat16, "cuda", batch).requires_grad_(False)
+    gen = torch.Generator(device="cuda").manual_seed(0)
+    bank.lora_b.copy_(torch.randn(bank.lora_b.shape, generator=gen, device="cuda"))
+    x, base = (torch.randn(12, 64, generator=gen, device="cuda").bfloat16() for _ in range(2))
+    return batch, bank, x, base
+
+
+def alone(bank, x, base, adapter, start=None):
+    """The rows with their adapters, by the operator itself (in the form that the batch takes, so that the bits agree: a row each, or starts)."""
+    from llmquant.hip import load_extension
+
+    start = None if start is None else torch.tensor(start, dtype=torch.int32, device="cuda")
+    return load_extension().lora_add(x, base, bank.lora_a, bank.lora_b, bank.scaling, torch.tensor(adapter, dtype=torch.int32, device="cuda"), start)
+
+
+@pytest.mark.parametrize("rows", [1, 12])
+def test_a_step_captured_before_anything_was_selected(rows):
+    """It reads what is selected later; a fill recorded with it would take that back at every replay."""
+    batch, bank, x, base = batch_and_bank()
+    x, base = x[:rows], base[:rows]
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = bank(x, base.clone())
+    for adapter in (1, -1, 2, 0):
+        batch.select([adapter])
+        for _ in range(2):
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(got, bank(x, base.clone())) and torch.equal(got, alone(bank, x, base, [adapter], None if rows == 1 else [0, rows])), adapter
+    batch.clear()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(got, base)
+
+
+def test_requests_are_not_selected_for_the_first_time_in_a_capture():
+    batch, bank, x, base = batch_and_bank()
+    chosen = torch.tensor([2, -1, 0], dtype=torch.int32, device="cuda")
+    with pytest.raises(RuntimeError, match="for the first time"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            batch.select(chosen)
+    torch.cuda.synchronize()
+    batch.select([0, 0, 0])
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):   # (known: from now on a replay selects them)
+        batch.select(chosen)
+    for _ in range(3):
+        batch.select([1, 1, 1])
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(bank(x[:3], base[:3].clone()), alone(bank, x[:3], base[:3], [2, -1, 0]))
