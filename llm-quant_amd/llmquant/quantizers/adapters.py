@@ -19,15 +19,35 @@ from llmquant.hip.build import load_extension
 from llmquant.quantizers.kernel import KernelQuantLinear
 
 
+_copies: dict[torch.device, torch.cuda.Stream] = {}
+
+
+def _settled(host: torch.Tensor, device: torch.device) -> torch.Tensor:
+    """`host` on the device, there when this returns, so that any stream may read it: a copy on a stream of its own, which alone is waited for."""
+    if device.type != "cuda":
+        return host.to(device)
+    stream = _copies.get(device)
+    if stream is None:
+        stream = _copies[device] = torch.cuda.Stream(device)
+    with torch.cuda.stream(stream):
+        return host.to(device)
+
+
 class AdapterBatch:
     """Which adapter each request has; shared by all banks of a model.
 
     What the kernels read lies on the device, one tensor for each number of requests, which keeps its address: a captured step
-    that ran with n requests reads what select() last said for n. Until then, and after clear(), nobody has an adapter.
+    that ran with n requests reads what select() last said for n. Until then, and after clear(), nobody has an adapter. select() and
+    clear() write on the current stream: calls on others come behind them in the way that any other tensor's readers do. A model has one
+    batch: threads that call it by turns select and call under a lock of theirs.
     """
+
+    STARTS = 256   # starts of requests of equal length that are kept for the next calls
 
     def __init__(self, device):
         self.device = torch.device(device)
+        if self.device.type == "cuda" and self.device.index is None:
+            self.device = torch.device("cuda", torch.cuda.current_device())
         self._adapters: dict[int, torch.Tensor] = {}
         self._starts: dict[tuple[int, int], torch.Tensor] = {}
         self._query_start: torch.Tensor | None = None
@@ -63,7 +83,7 @@ class AdapterBatch:
             # (made in a capture it would lie in the graph's memory, and every replay would set it to nobody again)
             if self._capturing():
                 raise RuntimeError(f"{requests} requests are selected for the first time while a step is captured: select as many before")
-            held = self._adapters[requests] = torch.full((requests,), -1, dtype=torch.int32, device=self.device)
+            held = self._adapters[requests] = _settled(torch.full((requests,), -1, dtype=torch.int32), self.device)
         return held
 
     def rows(self, x: torch.Tensor):
@@ -74,13 +94,15 @@ class AdapterBatch:
             if count % requests:
                 raise ValueError(f"{count} rows are no whole number for each of {requests} requests: select(..., query_start)")
             start = self._starts.get((count, requests))
+            if start is None and self._capturing():   # (in the graph's memory)
+                return self._held(requests), torch.arange(requests + 1, dtype=torch.int32, device=self.device) * (count // requests)
             if start is None:
-                start = torch.arange(0, count + 1, max(count // requests, 1), dtype=torch.int32, device=self.device)[: requests + 1]
-                if count == 0:
-                    start = torch.zeros(requests + 1, dtype=torch.int32, device=self.device)
-                if not self._capturing():   # (else it lives in the graph's memory)
-                    self._starts[count, requests] = start
-        elif start is not None and self._capturing() and not any(t is start for t in self._captured):
+                if len(self._starts) >= self.STARTS:   # nobody reads them any more, but for captured steps
+                    if self.device.type == "cuda":
+                        torch.cuda.synchronize(self.device)
+                    self._starts = {k: t for k, t in self._starts.items() if any(t is c for c in self._captured)}
+                start = self._starts[count, requests] = _settled(torch.arange(requests + 1, dtype=torch.int32) * (count // requests), self.device)
+        if start is not None and self._capturing() and not any(t is start for t in self._captured):
             self._captured.append(start)
         return self._held(requests), start
 

@@ -62,3 +62,42 @@ def test_requests_are_not_selected_for_the_first_time_in_a_capture():
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(bank(x[:3], base[:3].clone()), alone(bank, x[:3], base[:3], [2, -1, 0]))
+
+
+def test_starts_made_on_one_stream_are_read_on_another():
+    """The next call with as many rows, on a stream that does not wait for the first one's."""
+    batch, bank, x, base = batch_and_bank()
+    batch.select([2, 0])
+    want = alone(bank, x, base, [2, 0], [0, 6, 12])
+    torch.cuda.synchronize()
+    busy, other = torch.cuda.Stream(), torch.cuda.Stream()
+    with torch.cuda.stream(busy):
+        torch.cuda._sleep(20_000_000)
+        first = bank(x, base.clone())
+    with torch.cuda.stream(other):
+        second = bank(x, base.clone())
+    other.synchronize()
+    assert torch.equal(second, want)
+    torch.cuda.synchronize()
+    assert torch.equal(first, want)
+
+
+def test_many_prompt_lengths_beside_a_captured_step():
+    from llmquant.quantizers import AdapterBatch
+
+    batch, bank, x, base = batch_and_bank()
+    batch.select([2, 0])
+    want = bank(x, base.clone())
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = bank(x, base.clone())
+    longer = torch.empty(2 * AdapterBatch.STARTS + 20, 64, dtype=torch.bfloat16, device="cuda")
+    for n in range(2, longer.shape[0], 2):
+        assert batch.rows(longer[:n])[1].tolist() == [0, n // 2, n] if n != 2 else batch.rows(longer[:n])[1] is None
+    noise = [torch.full((3,), 7, dtype=torch.int32, device="cuda") for _ in range(64)]
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(got, want) and torch.equal(bank(x, base.clone()), want)
+    del noise
