@@ -33,6 +33,11 @@ def _settled(host: torch.Tensor, device: torch.device) -> torch.Tensor:
         return host.to(device)
 
 
+def _version(tensor: torch.Tensor) -> int | None:
+    """How often it was written in place; None: not known."""
+    return None if tensor.is_inference() else tensor._version
+
+
 class AdapterBatch:
     """Which adapter each request has; shared by all banks of a model.
 
@@ -51,6 +56,7 @@ class AdapterBatch:
         self._adapters: dict[int, torch.Tensor] = {}
         self._starts: dict[tuple[int, int], torch.Tensor] = {}
         self._query_start: torch.Tensor | None = None
+        self._selected: tuple[int, int | None] | None = None   # (rows that query_start gave the requests, its version then)
         self._requests = 1
         self._captured: list[torch.Tensor] = []   # what captured steps read
         self._held(1)   # (so that a step captured before anything was selected has it)
@@ -58,21 +64,25 @@ class AdapterBatch:
     def select(self, adapter, query_start=None) -> None:
         """adapter: a slot for each request (a list, or a tensor on any device; negative: none). query_start: int32 [requests + 1] on the device,
         for calls whose requests have unlike numbers of rows (None: as many rows each). It is kept, not copied: a captured
-        step reads the tensor it was captured with, which lives as long as the batch."""
+        step reads the tensor it was captured with, which lives as long as the batch. Calls of fewer rows than it gives the requests are refused
+        (a prompt's starts are no step's), unless adapter lies on the device, where nothing is waited for, or the starts were written since."""
         adapter = torch.as_tensor(adapter, dtype=torch.int32).reshape(-1)
         if adapter.numel() == 0:
             raise ValueError("adapters for no request")
         if query_start is not None and (query_start.dtype != torch.int32 or query_start.shape != (adapter.numel() + 1,)
                                         or query_start.device.type != self.device.type):
             raise ValueError(f"query_start must be int32 [{adapter.numel() + 1}] on the model's device")
+        selected = None
+        if query_start is not None and not adapter.is_cuda and not self._capturing():
+            selected = int(query_start[-1]), _version(query_start)
         self._held(adapter.numel()).copy_(adapter)
-        self._requests, self._query_start = adapter.numel(), query_start
+        self._requests, self._query_start, self._selected = adapter.numel(), query_start, selected
 
     def clear(self) -> None:
         """Nobody has an adapter, whatever the number of requests."""
         for held in self._adapters.values():
             held.fill_(-1)
-        self._requests, self._query_start = 1, None
+        self._requests, self._query_start, self._selected = 1, None, None
 
     def _capturing(self) -> bool:
         return self.device.type == "cuda" and torch.cuda.is_current_stream_capturing()
@@ -89,7 +99,9 @@ class AdapterBatch:
     def rows(self, x: torch.Tensor):
         """(adapter, query_start) for a call on x [..., in]."""
         count = x.numel() // x.shape[-1] if x.shape[-1] else 0
-        requests, start = self._requests, self._query_start
+        requests, start, selected = self._requests, self._query_start, self._selected
+        if selected is not None and count < selected[0] and selected[1] == _version(start):
+            raise ValueError(f"{count} rows are fewer than the {selected[0]} of the requests that were selected: select() for this call")
         if start is None and count != requests:
             if count % requests:
                 raise ValueError(f"{count} rows are no whole number for each of {requests} requests: select(..., query_start)")
@@ -111,6 +123,8 @@ class AdapterBatch:
         new = AdapterBatch(self.device)
         new._adapters = {n: t.clone() for n, t in self._adapters.items()}
         new._query_start = None if self._query_start is None else self._query_start.clone()
+        if self._selected is not None and self._selected[1] == _version(self._query_start):
+            new._selected = self._selected[0], _version(new._query_start)
         new._requests = self._requests
         memo[id(self)] = new
         return new

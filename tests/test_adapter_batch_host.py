@@ -1,5 +1,8 @@
 """The bookkeeping of who has which adapter, on the CPU."""
 
+import copy
+
+import pytest
 import torch
 
 from llmquant.quantizers import AdapterBatch
@@ -34,3 +37,30 @@ def test_what_is_kept_has_an_end(monkeypatch):
         assert batch.rows(torch.empty(n, 8))[1].tolist() == [0, n]
         assert len(batch._starts) <= AdapterBatch.STARTS
     assert batch.rows(torch.empty(2, 8))[1] is first and len(batch._captured) == 1
+
+
+def test_starts_of_a_prompt_are_no_steps():
+    """A call of fewer rows than the selected requests have would lie in the first ones' ranges."""
+    batch = AdapterBatch("cpu")
+    start = torch.tensor([0, 4, 4, 9], dtype=torch.int32)
+    batch.select([0, 1, 2], start)
+    assert rows(batch, 9) == ([0, 1, 2], [0, 4, 4, 9]) and rows(batch, 3, 4) == ([0, 1, 2], [0, 4, 4, 9])   # (rows behind the last request's: nobody's)
+    for lead in ((3,), (1, 3), (8,), (1,)):
+        with pytest.raises(ValueError, match="fewer than the 9"):
+            rows(batch, *lead)
+    twin = copy.deepcopy(batch)
+    with pytest.raises(ValueError, match="fewer than the 9"):
+        rows(twin, 3)
+    start.copy_(torch.tensor([0, 1, 2, 3], dtype=torch.int32))   # (written since: whoever wrote knows what calls come)
+    assert rows(batch, 3) == ([0, 1, 2], [0, 1, 2, 3])
+    with pytest.raises(ValueError, match="fewer than the 9"):
+        rows(twin, 3)
+    batch.select([0, 1, 2])
+    assert rows(batch, 3) == ([0, 1, 2], None)
+    with torch.inference_mode():
+        batch.select([5], torch.tensor([0, 6], dtype=torch.int32))
+        with pytest.raises(ValueError, match="fewer than the 6"):
+            rows(batch, 5)
+        assert rows(batch, 6) == ([5], [0, 6])
+    batch.clear()
+    assert rows(batch, 2) == ([-1], [0, 2])

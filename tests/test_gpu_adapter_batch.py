@@ -101,3 +101,18 @@ def test_many_prompt_lengths_beside_a_captured_step():
         torch.cuda.synchronize()
         assert torch.equal(got, want) and torch.equal(bank(x, base.clone()), want)
     del noise
+
+
+def test_a_step_behind_a_prompt():
+    """One row of each of two requests while a prompt's starts are selected: refused; with adapters that lie on the device nothing is asked of it."""
+    batch, bank, x, base = batch_and_bank()
+    start = torch.tensor([0, 5, 12], dtype=torch.int32, device="cuda")
+    batch.select([2, 0], start)
+    assert torch.equal(bank(x, base.clone()), alone(bank, x, base, [2, 0], [0, 5, 12]))
+    with pytest.raises(ValueError, match="fewer than the 12"):
+        bank(x[:2], base[:2].clone())
+    batch.select([2, 0])
+    assert torch.equal(bank(x[:2], base[:2].clone()), alone(bank, x[:2], base[:2], [2, 0]))
+    batch.select(torch.tensor([2, 0], dtype=torch.int32, device="cuda"), start)
+    assert torch.equal(bank(x, base.clone()), alone(bank, x, base, [2, 0], [0, 5, 12]))
+    assert torch.equal(bank(x[:2], base[:2].clone()), alone(bank, x[:2], base[:2], [2, 0], [0, 5, 12]))
