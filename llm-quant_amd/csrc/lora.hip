@@ -517,15 +517,19 @@ constexpr int kBlock = 32;          // rows of a block: one step of the matrix c
 constexpr int kPlanThreads = 1024;  // and the most slots
 
 // start [slots + 1]: the first virtual row of each slot, a multiple of 32 (rows up to there: none, -1); order: the row behind each
-// virtual row. Requests of a slot keep their order. One workgroup; seq_start: [sequences] scratch.
+// virtual row; used_start [used + 1]: the starts of the slots that have rows alone, and behind them the end; place [slots]: where a slot stands among
+// those. Requests of a slot keep their order. One workgroup; seq_start: [sequences] scratch.
 struct Plan {
   int slots, capacity;   // virtual rows at the most
+  int used;              // slots that can have rows: there are no more of them than requests
   int32_t* start;
+  int32_t* used_start;
+  int32_t* place;
   int32_t* order;
   int32_t* seq_start;
 };
 struct PlanLds {
-  int a[kPlanThreads], n[kPlanThreads], at[kPlanThreads], seq[kPlanThreads], scan[kPlanThreads];
+  int a[kPlanThreads], n[kPlanThreads], at[kPlanThreads], seq[kPlanThreads], scan[kPlanThreads], waves[kPlanThreads / kWave];
 };
 __device__ __forceinline__ void make_plan(PlanLds& s, const Requests& req, const Plan& p) {
   const int t = threadIdx.x, sequences = req.rows.sequences;
@@ -567,8 +571,22 @@ __device__ __forceinline__ void make_plan(PlanLds& s, const Requests& req, const
       s.scan[t] += v;
       __syncthreads();
     }
-    if (t < p.slots) p.start[t] = min(s.scan[t] - mine, p.capacity);
-    if (t == p.slots - 1) p.start[p.slots] = min(s.scan[t], p.capacity);
+    const int begin = min(s.scan[t] - mine, p.capacity), end = min(s.scan[p.slots - 1], p.capacity);
+    const uint64_t have = __ballot(mine > 0);   // (0 past the slots)
+    if (t % kWave == 0) s.waves[t / kWave] = __popcll(have);
+    __syncthreads();
+    int place = __popcll(have & ((uint64_t{1} << t % kWave) - 1)), all = 0;
+    for (int w = 0; w < kPlanThreads / kWave; ++w) {
+      if (w < t / kWave) place += s.waves[w];
+      all += s.waves[w];
+    }
+    if (t < p.slots) {
+      p.start[t] = begin;
+      p.place[t] = place;
+      if (mine > 0 && place < p.used) p.used_start[place] = begin;
+    }
+    for (int i = all + t; i <= p.used; i += kPlanThreads) p.used_start[i] = end;
+    if (t == 0) p.start[p.slots] = end;
   }
   __syncthreads();
   for (int row = t; row < req.rows.rows; row += kPlanThreads) {
@@ -631,9 +649,11 @@ struct OuterSide {
 struct Outer {
   OuterSide a, b;          // gradients of A (x and du) and of B (g and low)
   const int32_t* start;
+  const int32_t* used_start;   // [used + 1] and place [slots]: as the plan has them
+  const int32_t* place;
   const int32_t* order;
   const float* scaling;
-  int slots, rank, capacity, shift;   // 1 << shift rows a piece
+  int slots, used, rank, capacity, shift;   // 1 << shift rows a piece
   int a_columns;           // workgroups of side a in blockIdx.x
   void *grad_a, *grad_b;   // or null: records. Where a slot's rows are one piece: the results, blockIdx.y is the slot
 };
@@ -764,7 +784,7 @@ __global__ __launch_bounds__(4 * kWave) void outer_kernel(const Outer o) {
     v0 = o.start[blockIdx.y];
     v1 = o.start[blockIdx.y + 1];
   } else {
-    const Ragged slots{o.start, o.slots, o.capacity};
+    const Ragged slots{o.used_start, o.used, o.capacity};
     int piece = blockIdx.y, none;
     Span span;
     slots.find(o.shift, nullptr, piece, span, none);
@@ -865,7 +885,7 @@ __global__ __launch_bounds__(256) void records_kernel(const Outer o, T* __restri
       r = rest / (side.width / 8);
       c = rest % (side.width / 8) * 8;
     }
-    const int n = o.start[slot + 1] - o.start[slot], first = (o.start[slot] >> o.shift) + 2 * slot, pieces = (n + (1 << o.shift) - 1) >> o.shift;
+    const int n = o.start[slot + 1] - o.start[slot], first = (o.start[slot] >> o.shift) + 2 * o.place[slot], pieces = (n + (1 << o.shift) - 1) >> o.shift;
     float f[8] = {};
     const float scale = o.scaling[slot];
     const int64_t next = of_b ? side.width : 1;
@@ -961,14 +981,15 @@ int64_t take(int64_t& at, int64_t bytes) {
 
 struct GradPlan {
   bool direct;   // no records: a workgroup has all of a slot's rows
-  int splits, capacity, tiles, rtw, shift, records;   // parts of shrink, virtual rows, tiles of the rank, pieces of outer
-  int64_t o_start, o_order, o_seq, o_at, o_bt, o_planes, o_du, o_rec_a, o_rec_b, bytes;
+  int splits, capacity, used, tiles, rtw, shift, records;   // parts of shrink, virtual rows, slots that can have rows, tiles of the rank, pieces of outer
+  int64_t o_start, o_used, o_place, o_order, o_seq, o_at, o_bt, o_planes, o_du, o_rec_a, o_rec_b, bytes;
 };
 GradPlan grad_plan(int rows, int sequences, bool ragged, int in, int out, int rank, int slots, int dtype) {
   GradPlan p{};
   const int64_t size = dtype == LLMQ_F32 ? 4 : 2;
   p.splits = splits_of(rows, sequences, ragged, out, rank, dtype);
   const int64_t used = slots < sequences ? slots : sequences;   // slots that can have rows
+  p.used = static_cast<int>(used);
   p.capacity = static_cast<int>(round_up(rows + 31 * used, kBlock));
   p.tiles = (rank + 15) / 16;
   // outer takes one, two or four tiles of the rank a workgroup: fewer read the rows more often, and are smaller programs of fewer registers (bf16, whole calls, us,
@@ -983,9 +1004,11 @@ GradPlan grad_plan(int rows, int sequences, bool ragged, int in, int out, int ra
   const int64_t columns = (in + kColumns - 1) / kColumns + (out + kColumns - 1) / kColumns, places = p.rtw == 4 ? 400 : p.rtw == 2 ? 512 : 1024;
   p.shift = 7;
   while (p.shift < 12 && columns * ((rows >> p.shift) + used) * ((p.tiles + p.rtw - 1) / p.rtw) > places) ++p.shift;
-  p.records = p.direct ? 0 : (p.capacity >> p.shift) + 2 * slots;
+  p.records = p.direct ? 0 : (p.capacity >> p.shift) + 2 * p.used;
   int64_t at = 0;
   p.o_start = take(at, int64_t{4} * (slots + 1));
+  p.o_used = take(at, int64_t{4} * (used + 1));
+  p.o_place = take(at, int64_t{4} * slots);
   p.o_order = take(at, int64_t{4} * p.capacity);
   p.o_seq = take(at, int64_t{4} * sequences);
   p.o_at = take(at, size * slots * rank * in);
@@ -1006,8 +1029,8 @@ void gradients(const GradPlan& p, const void* grad, int64_t grad_stride, const v
   float* planes = reinterpret_cast<float*>(ws + p.o_planes);
   float* du = reinterpret_cast<float*>(ws + p.o_du);   // g lora_b
   const int64_t plane = static_cast<int64_t>(rows) * rank;
-  const Plan plan{slots, p.capacity, reinterpret_cast<int32_t*>(ws + p.o_start), reinterpret_cast<int32_t*>(ws + p.o_order),
-                  reinterpret_cast<int32_t*>(ws + p.o_seq)};
+  const Plan plan{slots, p.capacity, p.used, reinterpret_cast<int32_t*>(ws + p.o_start), reinterpret_cast<int32_t*>(ws + p.o_used),
+                  reinterpret_cast<int32_t*>(ws + p.o_place), reinterpret_cast<int32_t*>(ws + p.o_order), reinterpret_cast<int32_t*>(ws + p.o_seq)};
   const Turn turn_a{lora_a, ws + p.o_at, rank, in}, turn_b{lora_b, ws + p.o_bt, out, rank};
   const unsigned tiles = static_cast<unsigned>(slots) * (((in + 63) / 64 + (out + 63) / 64) * ((rank + 63) / 64));
   if constexpr (sizeof(T) == 4) hipLaunchKernelGGL((prepare_kernel<uint32_t>), dim3(1 + tiles), dim3(kPlanThreads), 0, s, req, plan, turn_a, turn_b);
@@ -1016,7 +1039,7 @@ void gradients(const GradPlan& p, const void* grad, int64_t grad_stride, const v
   expand<T>(Bank{ws + p.o_at, slots, rank, in}, req, Expand{planes, plane, p.splits, scaling, grad_base, base_stride, grad_x, p.splits > 1 ? du : nullptr, rows, in, 0, 0}, s);
   const Outer o{OuterSide{x, x_stride, x_scale, du, reinterpret_cast<float*>(ws + p.o_rec_a), in},
                 OuterSide{grad, grad_stride, nullptr, low, reinterpret_cast<float*>(ws + p.o_rec_b), out},
-                plan.start, plan.order, scaling, slots, rank, p.capacity, p.shift, (in + kColumns - 1) / kColumns, p.direct ? grad_a : nullptr,
+                plan.start, plan.used_start, plan.place, plan.order, scaling, slots, p.used, rank, p.capacity, p.shift, (in + kColumns - 1) / kColumns, p.direct ? grad_a : nullptr,
                 p.direct ? grad_b : nullptr};
   const dim3 grid(o.a_columns + (out + kColumns - 1) / kColumns, p.direct ? slots : p.records, (p.tiles + p.rtw - 1) / p.rtw);
 #define LLMQ_OUTER(CODES)                                                                                    \

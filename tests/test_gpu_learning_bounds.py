@@ -6,7 +6,9 @@ import math
 import pytest
 import torch
 from test_gpu_learning_edges import ext, loss_and_gradients, same  # noqa: F401 (ext: a fixture)
+from test_gpu_lora import backward as lora_backward
 from test_gpu_lora import call, call_grad, make
+from test_gpu_lora import close as lora_close
 from test_gpu_vocab_loss import DTYPES, F32, U, case, close, dense_of, quantized, sum_error
 
 pytestmark = pytest.mark.gpu
@@ -110,3 +112,24 @@ def test_rows_of_unlike_weight(ext, bits, spread, rows, dtype):  # noqa: F811
         close(dh, want[0], "dh")
         if learned:
             close(dw, want[1], "dW")
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("rank, lengths, adapters, slots", [
+    (64, [1500], [700], 1024), (64, [1100, 1200], [40, 3], 64), (16, [4000, 0, 7, 4100], [9, 2, -1, 0], 12), (128, [1300, 900], [1, 1], 2), (8, [5000], [5], 6)])
+def test_gradients_of_a_bank_with_idle_slots(ext, rank, lengths, adapters, slots, dtype):  # noqa: F811
+    """Long slots among slots without rows, in pieces; zeros for the others. Where as many slots can have rows, as in a bank of their own."""
+    c = make(lengths, adapters, slots, rank, 136, 128, dtype)
+    low = torch.empty(sum(lengths), rank, device="cuda")
+    call(ext, c, low=low)
+    gx, ga, gb = call_grad(ext, c, low)
+    used = sorted({a for a in adapters if a >= 0})
+    if len(used) == len(adapters):   # (otherwise pieces may be of other lengths)
+        alone = dict(c, lora_a=c["lora_a"][used].contiguous(), lora_b=c["lora_b"][used].contiguous(), scaling=c["scaling"][used].contiguous(),
+                     adapter=torch.tensor([used.index(a) for a in adapters], dtype=torch.int32, device="cuda"))
+        hx, ha, hb = call_grad(ext, alone, low)
+        assert torch.equal(gx, hx) and torch.equal(ga[used], ha) and torch.equal(gb[used], hb)
+    idle = [s for s in range(slots) if s not in used]
+    assert not ga[idle].any() and not gb[idle].any()
+    for got, pair in zip((gx, ga, gb), lora_backward(c, c["x"].double(), low, dtype, False)):
+        lora_close(got, pair)

@@ -42,3 +42,12 @@ def test_rows_of_a_request_lie_within_reach(lib, change, fits):  # noqa: F811
     stride = change.pop("stride")
     for rows in (lora(lib, inp=256, x_stride=stride, **change), lora_grad(lib, out=256, base_stride=stride, **change)):
         assert rows == 1 and (WIDE in text(lib)) != fits and ("workspace" in text(lib)) == fits
+
+
+@pytest.mark.parametrize("rows, sequences, inp, out, rank", [(2000, 1, 4096, 4096, 64), (4096, 2, 4096, 14336, 64), (4099, 3, 4096, 4096, 128), (20000, 5, 2048, 2048, 16)])
+def test_slots_without_rows_take_their_turned_banks_alone(lib, rows, sequences, inp, out, rank):  # noqa: F811
+    """A large bank of which few learn at a time: sums of pieces for the slots that can have rows, not for all."""
+    few = lib.llmq_lora_grad_workspace_bytes(rows, sequences, 1, inp, out, rank, sequences, BF16)
+    for slots in (8, 64, 1024):
+        more = lib.llmq_lora_grad_workspace_bytes(rows, sequences, 1, inp, out, rank, slots, BF16)
+        assert 0 <= more - few <= (slots - sequences) * (2 * rank * (inp + out) + 8) + 5 * 256
