@@ -11,7 +11,6 @@ from __future__ import annotations
 
 import torch
 import torch.nn as nn
-from torch.autograd.function import once_differentiable
 
 from llmquant.core.observers import group_view, pad_to_group
 from llmquant.core.scheme import QuantizationScheme
@@ -144,30 +143,31 @@ class _FrozenCodes(torch.autograd.Function):
         return module._frozen(x)
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, grad):
         module, of_x, of_bias = ctx.module, None, None
-        qdata, wscale = ctx.saved_tensors
+        ctx.saved_tensors   # (what raises that error)
         rows = grad.reshape(-1, grad.shape[-1])
         if ctx.needs_input_grad[0]:
-            groups = qdata.shape[1]
-            group_size = module.padded_in_features // groups
-            keep = module._head_keep or group_size
-            if group_size % 8 == 0 and keep % 8 == 0 and module.out_features % 8 == 0:
-                of_x = module._ext.wq_linear_grad(rows, qdata, wscale, module.out_group, keep)
-            else:
-                of_x = rows @ module._dequantized_weight(rows.dtype, real_width=True)
-            # (zeros behind a row that is no whole number of groups; heads padded to groups otherwise)
-            if of_x.shape[1] != module.in_features:
-                head_dim = module._weight_args.head_dim
-                if head_dim and module.in_features % head_dim == 0 and of_x.shape[1] % (module.in_features // head_dim) == 0:
-                    of_x = of_x.unflatten(1, (module.in_features // head_dim, -1))[..., :head_dim].flatten(1)
-                else:
-                    of_x = of_x[:, :module.in_features]
-            of_x = of_x.reshape(*grad.shape[:-1], module.in_features)
+            # (to be differentiated again, or many gradients at once: torch's own product, which can be)
+            plain = torch.is_grad_enabled() or not _stored(rows)
+            of_x = (rows @ module._real_weight(rows.dtype) if plain else module._input_gradient(rows)).reshape(*grad.shape[:-1], module.in_features)
         if ctx.needs_input_grad[1]:
             of_bias = rows.sum(0, dtype=torch.float32).to(module.bias.dtype)
         return of_x, of_bias, None
+
+
+def _stored(tensor) -> bool:
+    """Whether it has memory of its own that a kernel can read; a batch of gradients that is mapped over has none."""
+    try:
+        tensor.data_ptr()
+    except RuntimeError:
+        return False
+    return True
+
+
+def _transformed() -> bool:
+    """Whether a transform of torch.func is at work (vmap, grad, jvp), whose tensors no kernel takes."""
+    return torch._C._are_functorch_transforms_active()
 
 
 class KernelQuantLinear(nn.Module):
@@ -300,6 +300,9 @@ class KernelQuantLinear(nn.Module):
         group_size = self.padded_in_features // self.qdata.shape[1]
         if group_size % 8 == 0:
             keep = self._head_keep if real_width else 0
+            if _transformed():   # (the weight is none of the transform's tensors)
+                with torch._C._DisableFuncTorch():
+                    return self._ext.dequant_weight(self.qdata, self.wscale, self.out_group, keep, dtype)
             return self._ext.dequant_weight(self.qdata, self.wscale, self.out_group, keep, dtype)
         return (self.qweight * self._broadcast_scale).to(dtype).reshape(self.out_features, -1)
 
@@ -314,9 +317,31 @@ class KernelQuantLinear(nn.Module):
 
     def forward(self, x):
         if self._adapted or (x.requires_grad and torch.is_grad_enabled()):
-            out = _FrozenCodes.apply(x, self.bias, self) if x.requires_grad and torch.is_grad_enabled() else self._frozen(x)
+            learning = x.requires_grad and torch.is_grad_enabled() and not _transformed()
+            out = _FrozenCodes.apply(x, self.bias, self) if learning else self._frozen(x)
             return self.adapters(x, out) if self._adapted else out
         return self._frozen(x)
+
+    def _cut(self, rows):
+        """Rows over the padded weight's columns, or over whole head groups, without what pads them."""
+        if rows.shape[-1] == self.in_features:
+            return rows
+        head_dim = self._weight_args.head_dim
+        if head_dim and self.in_features % head_dim == 0 and rows.shape[-1] % (self.in_features // head_dim) == 0:
+            return rows.unflatten(-1, (self.in_features // head_dim, -1))[..., :head_dim].flatten(-2)
+        return rows[..., :self.in_features]
+
+    def _real_weight(self, dtype):
+        """[out_features, in_features]: what the codes stand for."""
+        return self._cut(self._dequantized_weight(dtype, real_width=True))
+
+    def _input_gradient(self, rows):
+        """rows [rows, out] times that."""
+        group_size = self.padded_in_features // self.qdata.shape[1]
+        keep = self._head_keep or group_size
+        if group_size % 8 == 0 and keep % 8 == 0 and self.out_features % 8 == 0:
+            return self._cut(self._ext.wq_linear_grad(rows, self.qdata, self.wscale, self.out_group, keep))
+        return rows @ self._real_weight(rows.dtype)
 
     def _frozen(self, x):
         # (the buffers through their dict: nn.Module.__getattr__ costs a third of a microsecond a look)
