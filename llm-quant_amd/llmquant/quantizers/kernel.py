@@ -145,12 +145,17 @@ class _FrozenCodes(torch.autograd.Function):
     @staticmethod
     def backward(ctx, grad):
         module, of_x, of_bias = ctx.module, None, None
-        ctx.saved_tensors   # (what raises that error)
+        qdata, wscale = ctx.saved_tensors
         rows = grad.reshape(-1, grad.shape[-1])
         if ctx.needs_input_grad[0]:
+            group_size = module.padded_in_features // qdata.shape[1]
+            keep = module._head_keep or group_size
             # (to be differentiated again, or many gradients at once: torch's own product, which can be)
-            plain = torch.is_grad_enabled() or not _stored(rows)
-            of_x = (rows @ module._real_weight(rows.dtype) if plain else module._input_gradient(rows)).reshape(*grad.shape[:-1], module.in_features)
+            if (group_size % 8 == 0 and keep % 8 == 0 and module.out_features % 8 == 0 and not torch.is_grad_enabled() and _stored(rows)):
+                of_x = module._cut(module._ext.wq_linear_grad(rows, qdata, wscale, module.out_group, keep))
+            else:
+                of_x = rows @ module._real_weight(rows.dtype)
+            of_x = of_x.reshape(*grad.shape[:-1], module.in_features)
         if ctx.needs_input_grad[1]:
             of_bias = rows.sum(0, dtype=torch.float32).to(module.bias.dtype)
         return of_x, of_bias, None
@@ -316,11 +321,28 @@ class KernelQuantLinear(nn.Module):
         return rows @ self._dequantized_weight(rows.dtype, real_width).T
 
     def forward(self, x):
-        if self._adapted or (x.requires_grad and torch.is_grad_enabled()):
-            learning = x.requires_grad and torch.is_grad_enabled() and not _transformed()
+        learning = x.requires_grad and torch.is_grad_enabled()
+        if learning or self._adapted:
+            learning = learning and not self._plain(x) and not _transformed()
             out = _FrozenCodes.apply(x, self.bias, self) if learning else self._frozen(x)
             return self.adapters(x, out) if self._adapted else out
         return self._frozen(x)
+
+    def _plain(self, x):
+        """Whether x goes through torch's own product and its gradient had better, too, which keeps the dense weight until then: float32 rows between those of
+        which the codes' gradient is the faster one (`wq_linear_grad`), and groups that no kernel takes. Forward and backward, us, the codes' gradient for torch's:
+        14336 x 4096 int8 64 rows 201 for 229, 65 rows 289 for 261, 320 rows 835 for 640, 2048 rows 3088 for 3246; 4096 x 14336 16 rows 151 for 151, 32 rows 181
+        for 164, 1024 rows 1658 for 1671; 4096 x 4096 512 rows 272 for 257, 1024 rows 466 for 484; 2048 x 2048 512 rows 140 for 87, 1024 rows 176 for 139, 2048 rows
+        248 for 250; 512 x 2048 2048 rows 130 for 83."""
+        whole = self.scheme.weights.group_size % 8 == 0
+        if whole and x.dtype in (torch.bfloat16, torch.float16):
+            return False
+        count = x.numel() // max(x.shape[-1], 1)
+        if count <= KERNEL_MAX_ROWS or self._int8_act:
+            return False
+        few = count <= (64 if self.in_features <= 4096 else 16)
+        many = count >= 1024 and count * self.out_features * self.in_features >= 1 << 34
+        return not whole or not (few or many)
 
     def _cut(self, rows):
         """Rows over the padded weight's columns, or over whole head groups, without what pads them."""
@@ -334,14 +356,6 @@ class KernelQuantLinear(nn.Module):
     def _real_weight(self, dtype):
         """[out_features, in_features]: what the codes stand for."""
         return self._cut(self._dequantized_weight(dtype, real_width=True))
-
-    def _input_gradient(self, rows):
-        """rows [rows, out] times that."""
-        group_size = self.padded_in_features // self.qdata.shape[1]
-        keep = self._head_keep or group_size
-        if group_size % 8 == 0 and keep % 8 == 0 and self.out_features % 8 == 0:
-            return self._cut(self._ext.wq_linear_grad(rows, self.qdata, self.wscale, self.out_group, keep))
-        return rows @ self._real_weight(rows.dtype)
 
     def _frozen(self, x):
         # (the buffers through their dict: nn.Module.__getattr__ costs a third of a microsecond a look)

@@ -105,3 +105,32 @@ def test_differentiated_twice_on_the_device(inp, heads, rows, dtype):
         want = want @ matrix
         tol = tol * size + sums + u * (want.norm() + tol * size + sums)
     assert (got.double() - want).norm() <= tol
+
+
+@pytest.mark.parametrize("inp, out, rows, dtype, plain", [
+    (2048, 2048, 4, torch.float32, False), (2048, 2048, 64, torch.float32, False), (2048, 2048, 65, torch.float32, True), (2048, 2048, 320, torch.float32, True),
+    (2048, 2048, 4095, torch.float32, True), (2048, 2048, 4096, torch.float32, False), (4096, 4096, 1023, torch.float32, True), (4096, 4096, 1024, torch.float32, False),
+    (8192, 1024, 16, torch.float32, False), (8192, 1024, 17, torch.float32, True), (2048, 2048, 320, torch.bfloat16, False), (2048, 2048, 65, torch.float16, False)])
+def test_where_the_gradient_is_torchs_own(no_kernels, inp, out, rows, dtype, plain):
+    module = KernelQuantLinear(torch.zeros(out, inp // 128, 128, dtype=torch.int8), torch.ones(out, inp // 128), None,
+                               QuantizationScheme(weights=QuantizationArgs(num_bits=8, strategy="group", group_size=128), input_activations=None), inp)
+    assert module._plain(torch.empty(rows, inp, dtype=dtype, device="meta")) == plain
+    assert module._plain(torch.empty(1, rows, inp, dtype=dtype, device="meta")) == plain
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows", [5, 64, 65, 320, 321, 1023, 1030])
+def test_one_gradient_on_both_sides(rows):
+    """float32, the codes' gradient and torch's own against the weight in 64 bits."""
+    module = linear(256, 136, 128, 8, device="cuda")
+    x = torch.randn(rows, 256, generator=torch.Generator().manual_seed(rows)).cuda()
+    way = torch.randn(rows, 136, generator=torch.Generator().manual_seed(1)).cuda()
+    weight = module._real_weight(torch.float32).double()
+    want, size = way.double() @ weight, way.double().abs() @ weight.abs()
+    y = x.clone().requires_grad_()
+    assert module._plain(y) == (rows > 64)
+    for out in (module(y), _FrozenCodes.apply(y, module.bias, module)):
+        with torch.no_grad():
+            assert torch.equal(out, module(x))
+        got, = torch.autograd.grad(out, y, way)
+        assert ((got.double() - want).abs() <= (6 * 136 + 72) * 2.0 ** -24 * size + 2.0 ** -22 * size + 2.0 ** -23 * want.abs()).all()
