@@ -19,6 +19,8 @@ model_io.py:174-189), so nothing wider than the file ever exists on the device.
 
 from __future__ import annotations
 
+import warnings
+
 import torch
 import torch.nn as nn
 
@@ -44,7 +46,11 @@ def _quantized_layers(model):
 
 
 def save_packed_model(model: nn.Module, path, model_id: str, kv_cache_bits=None, extra=None):
-    """Write every weight of a kernel-mode model into one file; returns the path."""
+    """Write every weight of a kernel-mode model into one file; returns the path. Low-rank adapters beside its Linears are no part of the file (their banks are
+    in state_dict()), which a warning says."""
+    adapted = [name for name, module in _quantized_layers(model) if module._adapted]
+    if adapted:
+        warnings.warn(f"the file holds no adapters: those beside {len(adapted)} Linears ({adapted[0]}, ...) are not written", stacklevel=2)
     tensors, layers = {}, {}
     for name, module in _quantized_layers(model):
         args = module.scheme.weights

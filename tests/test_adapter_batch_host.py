@@ -64,3 +64,27 @@ def test_starts_of_a_prompt_are_no_steps():
         assert rows(batch, 6) == ([5], [0, 6])
     batch.clear()
     assert rows(batch, 2) == ([-1], [0, 2])
+
+
+def test_a_packed_file_says_that_it_holds_no_adapters(monkeypatch, tmp_path, recwarn):
+    """What was learned beside the codes does not go with them; it is in the state dict."""
+    import llmquant.quantizers.kernel as kernel
+    from llmquant.core.scheme import QuantizationArgs, QuantizationScheme
+    from llmquant.packing import read_packed, save_packed_model
+    from llmquant.quantizers import KernelQuantLinear, add_adapters, remove_adapters
+
+    monkeypatch.setattr(kernel, "load_extension", lambda: type("None", (), {"wq_gemv": None})())
+    model = torch.nn.Module()
+    scheme = QuantizationScheme(weights=QuantizationArgs(num_bits=8, strategy="group", group_size=128), input_activations=None)
+    model.up_proj = KernelQuantLinear.from_linear(torch.nn.Linear(128, 16, bias=False), scheme)
+    save_packed_model(model, tmp_path / "bare", "test/model")
+    assert not recwarn.list
+    add_adapters(model, rank=8)
+    with pytest.warns(UserWarning, match="no adapters.*up_proj"):
+        save_packed_model(model, tmp_path / "adapted", "test/model")
+    assert (tmp_path / "bare").read_bytes() == (tmp_path / "adapted").read_bytes()
+    assert sum("adapters" in name for name in model.state_dict()) == 3
+    remove_adapters(model)
+    recwarn.clear()
+    save_packed_model(model, tmp_path / "again", "test/model")
+    assert not recwarn.list and not any("adapters" in name for name in read_packed(tmp_path / "again")[0])
