@@ -203,7 +203,8 @@ def _forget_captured(model) -> None:
 def add_adapters(model, rank: int = 16, slots: int = 1, alpha: float | None = None, targets: str | None = None,
                  save_bits: int = 16, dtype=None) -> list[str]:
     """A bank of adapters beside every kernel-mode Linear whose name `targets` (a regular expression) finds; without it, beside all but
-    lm_head. alpha: scaling is alpha / rank (None: 2). Everything else of the model stops learning. Returns the names."""
+    lm_head. alpha: scaling is alpha / rank (None: 2). Everything else of the model stops learning. Steps that a program of its own captured before run on
+    without the adapters: capture them again. Returns the names."""
     chosen = [(name, module) for name, module in _kernel_linears(model, targets)]
     if not chosen:
         raise ValueError("the model has no kernel-mode Linear of that name")

@@ -130,10 +130,12 @@ class _Kept(dict):
 
 
 def _module_tree(model):
-    """Every (parent, name, child) edge of the module tree and every place a tensor hangs in it (the
-    `_parameters` / `_buffers` dict of a module and the name in it)."""
-    edges, slots = [], []
+    """Every (parent, name, child) edge of the module tree, every place a tensor hangs in it (the
+    `_parameters` / `_buffers` dict of a module and the name in it), and the Linears that may have adapters beside them."""
+    edges, slots, linears = [], [], []
     for parent in model.modules():
+        if hasattr(parent, "_adapted"):
+            linears.append(parent)
         for name, child in parent._modules.items():
             if child is not None:
                 edges.append((parent, name, child))
@@ -141,7 +143,7 @@ def _module_tree(model):
             for name, tensor in holder.items():
                 if tensor is not None:
                     slots.append((holder, name))
-    return _Kept(edges=edges, slots=slots)
+    return _Kept(edges=edges, slots=slots, linears=linears)
 
 
 def _weights_key(model):
@@ -157,7 +159,7 @@ def _weights_key(model):
     if not tree or not all(parent._modules.get(name) is child for parent, name, child in tree["edges"]):
         tree = _module_tree(model)
         model.__dict__["_llmq_module_tree"] = tree
-    key = []
+    key = [linear._adapted for linear in tree["linears"]]   # (adapters may be added through a part of the model)
     for holder, name in tree["slots"]:
         tensor = holder.get(name)
         if tensor is None:

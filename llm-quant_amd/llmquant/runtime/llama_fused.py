@@ -113,6 +113,8 @@ def _fused(owner, name, *mods):
 
 
 class LlamaFusedRuntime(LlamaKernelRuntime):
+    _linears = ()
+
     def __init__(self, model, max_len: int, kv_bits: int = 8, exact_prefill: bool = False, attn_splits=None):
         """attn_splits: workgroups per query head in the attention launch. None picks enough to put
         a workgroup on every CU (and more for long caches); 1 keeps each head in one workgroup and
@@ -182,7 +184,13 @@ class LlamaFusedRuntime(LlamaKernelRuntime):
         head = model.lm_head
         if not _fusable(head):
             raise ValueError("the fused decode step needs a kernel-mode lm_head")
+        self._linears = [module for module in model.modules() if isinstance(module, KernelQuantLinear)]
         self._init_token_pick(model, head.qdata.shape[0])
+
+    def prefill(self, input_ids):
+        if any(module._adapted for module in self._linears):
+            raise RuntimeError("adapters stand beside the model's Linears since this runtime was built, whose step has none: build another")
+        return super().prefill(input_ids)
 
     def _init_token_pick(self, model, head_rows: int):
         """The final norm's weight and what the token pick at the end of a step needs."""

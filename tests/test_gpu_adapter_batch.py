@@ -116,3 +116,26 @@ def test_a_step_behind_a_prompt():
     batch.select(torch.tensor([2, 0], dtype=torch.int32, device="cuda"), start)
     assert torch.equal(bank(x, base.clone()), alone(bank, x, base, [2, 0], [0, 5, 12]))
     assert torch.equal(bank(x[:2], base[:2].clone()), alone(bank, x[:2], base[:2], [2, 0], [0, 5, 12]))
+
+
+def test_runtimes_from_before_the_adapters():
+    """What is kept on the whole model gives way to adapters that are added through a part of it; a fused runtime in a program's hands refuses."""
+    from llmquant.quantizers import add_adapters, remove_adapters, use_adapters
+    from llmquant.runtime import graphed_generate, kernel_runtime
+    from test_gpu_adapters import build, stir
+
+    _, kernel = build(torch.float32, hidden=512, inter=1024, heads=8, vocab=512)
+    ids = torch.randint(0, 512, (1, 12), generator=torch.Generator().manual_seed(4)).cuda()
+    held = kernel_runtime(kernel, 32)
+    plain = graphed_generate(kernel, ids, 12, kv_bits=8)
+    assert torch.equal(held.generate(ids, 12), plain)
+    add_adapters(kernel.model, rank=8, slots=2)
+    stir(kernel)
+    use_adapters(kernel, [1])
+    want = kernel_runtime(kernel, 32).generate(ids, 12, use_graph=False)
+    assert not torch.equal(want, plain)
+    assert torch.equal(graphed_generate(kernel, ids, 12, kv_bits=8), want)
+    with pytest.raises(RuntimeError, match="build another"):
+        held.generate(ids, 12)
+    remove_adapters(kernel.model)
+    assert torch.equal(graphed_generate(kernel, ids, 12, kv_bits=8), plain) and torch.equal(held.generate(ids, 12), plain)
