@@ -2,6 +2,7 @@
 test_gpu_vocab_loss.py and test_gpu_lora.py."""
 
 import math
+import random
 
 import pytest
 import torch
@@ -133,3 +134,65 @@ def test_gradients_of_a_bank_with_idle_slots(ext, rank, lengths, adapters, slots
     assert not ga[idle].any() and not gb[idle].any()
     for got, pair in zip((gx, ga, gb), lora_backward(c, c["x"].double(), low, dtype, False)):
         lora_close(got, pair)
+
+
+class Walled:
+    """Memory in which every piece that is handed out has walls of a known pattern before and behind it."""
+
+    WALL = 1 << 16
+
+    def __init__(self, nbytes):
+        self.held = torch.full((nbytes,), 0xA5, dtype=torch.uint8, device="cuda")
+        self.at, self.pieces = 0, []
+
+    def take(self, nbytes):
+        begin = self.at + self.WALL
+        self.at = (begin + nbytes + 255) // 256 * 256
+        assert self.at + self.WALL <= self.held.numel()
+        self.pieces.append((begin, begin + nbytes))
+        return self.held.data_ptr() + begin
+
+    def whole(self):
+        at = 0
+        for begin, end in [*self.pieces, (self.held.numel(), 0)]:
+            if not bool((self.held[at:begin] == 0xA5).all()):
+                return False
+            at = end
+        return True
+
+
+def malformed(rows, sequences, seed):
+    """Starts that decrease, repeat, leave the rows on both sides."""
+    rng = random.Random(seed)
+    edge = [0, rows, -9, rows + 50, -2 ** 31, 2 ** 31 - 1]
+    return [rng.choice([rng.randint(0, rows), rng.randint(-rows, 2 * rows), *edge][: 2 + rng.randint(0, 6)]) for _ in range(sequences + 1)]
+
+
+@pytest.mark.parametrize("rows, sequences, slots, rank", [(256, 8, 2, 8), (300, 70, 5, 64), (5000, 3, 9, 16), (4500, 130, 1, 128), (40, 200, 200, 16), (2500, 1, 3, 64)])
+@pytest.mark.parametrize("seed", range(3))
+def test_malformed_starts_write_within_what_a_call_was_given(rows, sequences, slots, rank, seed):
+    """Nothing is promised of the results, but that no byte beside the outputs and the workspace changes: a wall on both sides of each, every start clamped to the
+    rows, pieces, virtual rows and records counted from sizes alone."""
+    from llmquant.hip.build import load_capi
+
+    lib, bf16, inp, out = load_capi(), 2, 72, 136
+    c = make([rows], [0], slots, rank, inp, out, torch.bfloat16)
+    adapter = torch.tensor([random.Random(seed + 9).randint(-1, slots) for _ in range(sequences)], dtype=torch.int32, device="cuda")
+    start = torch.tensor(malformed(rows, sequences, seed), dtype=torch.int32, device="cuda")
+    stream = torch.cuda.current_stream().cuda_stream
+    add = lib.llmq_lora_add_workspace_bytes(rows, sequences, 1, inp, rank, bf16)
+    back = lib.llmq_lora_grad_workspace_bytes(rows, sequences, 1, inp, out, rank, slots, bf16)
+    sizes = dict(out=2 * rows * out, low=4 * rows * rank, add=add, gx=2 * rows * inp, ga=2 * slots * rank * inp, gb=2 * slots * rank * out, back=back)
+    room = Walled(sum(sizes.values()) + 16 * Walled.WALL)
+    to = {name: room.take(n) for name, n in sizes.items()}
+    weights = [c[k].data_ptr() for k in ("lora_a", "lora_b", "scaling")]
+    assert lib.llmq_lora_add(c["x"].data_ptr(), inp, c["base"].data_ptr(), out, *weights, adapter.data_ptr(), start.data_ptr(), to["out"], to["low"], to["add"], add,
+                             rows, sequences, inp, out, rank, slots, bf16, stream) == 0, lib.llmq_last_error()
+    torch.cuda.synchronize()
+    assert room.whole(), "lora_add"
+    low = torch.randn(rows, rank, device="cuda")
+    assert lib.llmq_lora_grad(c["grad"].data_ptr(), out, c["x"].data_ptr(), inp, None, low.data_ptr(), *weights, adapter.data_ptr(), start.data_ptr(),
+                              c["grad_base"].data_ptr(), inp, to["gx"], to["ga"], to["gb"], to["back"], back, rows, sequences, inp, out, rank, slots, bf16,
+                              stream) == 0, lib.llmq_last_error()
+    torch.cuda.synchronize()
+    assert room.whole(), "lora_grad"
