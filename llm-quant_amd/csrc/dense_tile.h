@@ -5,7 +5,7 @@
 // the core that the vocabulary loss and the gradient of a quantized Linear build on. Each operand lies with the reduction axis innermost
 // ([rows, K]) or outermost ([K, rows]: no matrix is turned over on the way). fp32 matrices take part as three bfloat16 planes
 // each (planes_of: x = x0 + x1 + x2, 8 bits and 8 and 8: exact), of whose nine products the six largest are added: what is left out is
-// at most 2^-23 of a term (x1 y2 and x2 y1, 2^-8 times 2^-16 each).
+// at most 2^-23 of a term (x1 y2 and x2 y1, 2^-8 times 2^-16 each). An infinity has no such planes: what it takes part in is NaN.
 //
 // Shape. TM x TN outputs a workgroup of eight waves, 64 of K a step; both operands reach LDS as they lie in memory (buffer loads into
 // LDS, 16 bytes a lane, nothing in registers), their chunks of 16 bytes swizzled by the row so that the reads of operands spread over
