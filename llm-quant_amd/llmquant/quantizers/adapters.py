@@ -22,15 +22,18 @@ from llmquant.quantizers.kernel import KernelQuantLinear
 _copies: dict[torch.device, torch.cuda.Stream] = {}
 
 
-def _settled(host: torch.Tensor, device: torch.device) -> torch.Tensor:
-    """`host` on the device, there when this returns, so that any stream may read it: a copy on a stream of its own, which alone is waited for."""
-    if device.type != "cuda":
-        return host.to(device)
-    stream = _copies.get(device)
-    if stream is None:
-        stream = _copies[device] = torch.cuda.Stream(device)
-    with torch.cuda.stream(stream):
-        return host.to(device)
+def _settled(values: list[int], device: torch.device) -> torch.Tensor:
+    """int32 values on the device, there when this returns, so that any stream may read them: a copy on a stream of its own, which alone is waited for. An ordinary
+    tensor in inference mode, too: a training step may read it later."""
+    with torch.inference_mode(False):
+        host = torch.tensor(values, dtype=torch.int32)
+        if device.type != "cuda":
+            return host.to(device)
+        stream = _copies.get(device)
+        if stream is None:
+            stream = _copies[device] = torch.cuda.Stream(device)
+        with torch.cuda.stream(stream):
+            return host.to(device)
 
 
 def _version(tensor: torch.Tensor) -> int | None:
@@ -93,7 +96,7 @@ class AdapterBatch:
             # (made in a capture it would lie in the graph's memory, and every replay would set it to nobody again)
             if self._capturing():
                 raise RuntimeError(f"{requests} requests are selected for the first time while a step is captured: select as many before")
-            held = self._adapters[requests] = _settled(torch.full((requests,), -1, dtype=torch.int32), self.device)
+            held = self._adapters[requests] = _settled([-1] * requests, self.device)
         return held
 
     def rows(self, x: torch.Tensor):
@@ -113,7 +116,7 @@ class AdapterBatch:
                     if self.device.type == "cuda":
                         torch.cuda.synchronize(self.device)
                     self._starts = {k: t for k, t in self._starts.items() if any(t is c for c in self._captured)}
-                start = self._starts[count, requests] = _settled(torch.arange(requests + 1, dtype=torch.int32) * (count // requests), self.device)
+                start = self._starts[count, requests] = _settled([b * (count // requests) for b in range(requests + 1)], self.device)
         if start is not None and self._capturing() and not any(t is start for t in self._captured):
             self._captured.append(start)
         return self._held(requests), start

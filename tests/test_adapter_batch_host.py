@@ -88,3 +88,13 @@ def test_a_packed_file_says_that_it_holds_no_adapters(monkeypatch, tmp_path, rec
     recwarn.clear()
     save_packed_model(model, tmp_path / "again", "test/model")
     assert not recwarn.list and not any("adapters" in name for name in read_packed(tmp_path / "again")[0])
+
+
+def test_what_is_kept_from_inference_mode_serves_training():
+    batch = AdapterBatch("cpu")
+    with torch.inference_mode():
+        batch.select([1, 0])
+        kept = batch.rows(torch.empty(6, 8))
+    assert not any(t.is_inference() for t in kept)
+    batch.select([0, 1])
+    assert rows(batch, 6) == ([0, 1], [0, 3, 6])

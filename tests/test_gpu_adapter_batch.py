@@ -139,3 +139,18 @@ def test_runtimes_from_before_the_adapters():
         held.generate(ids, 12)
     remove_adapters(kernel.model)
     assert torch.equal(graphed_generate(kernel, ids, 12, kv_bits=8), plain) and torch.equal(held.generate(ids, 12), plain)
+
+
+def test_a_training_step_behind_an_evaluation():
+    """In inference mode with as many rows before: what was kept from it is read by autograd."""
+    batch, bank, x, base = batch_and_bank()
+    bank.requires_grad_(True)
+    with torch.inference_mode():
+        batch.select([2, 0])
+        want = bank(x, base.clone())
+    out = bank(x, base)
+    assert torch.equal(out, want)
+    out.float().square().sum().backward()
+    assert bank.lora_a.grad[2].any() and bank.lora_b.grad[0].any() and not bank.lora_b.grad[1].any()
+    batch.select([1, 1])
+    assert not torch.equal(bank(x, base), want)
