@@ -59,20 +59,30 @@ def quantize_activation(x: torch.Tensor, args: QuantizationArgs):
 fake_quantize_cuda = fake_quantize_hip
 
 
+def keep(ctx, *tensors) -> None:
+    """Tensors (or None) for the backward pass, where a change in place since then is an error; those of inference mode, which autograd does not save, as they are."""
+    ctx.plain = [t if t is not None and t.is_inference() else None for t in tensors]
+    ctx.save_for_backward(*(t if p is None else None for t, p in zip(tensors, ctx.plain)))
+
+
+def kept(ctx) -> list:
+    return [saved if p is None else p for saved, p in zip(ctx.saved_tensors, ctx.plain)]
+
+
 class _VocabLoss(torch.autograd.Function):
     """Losses of rows over a vocabulary; the logits are made again in the backward pass, a piece at a time."""
 
     @staticmethod
     def forward(ctx, hidden, weight, wscale, out_group, targets, ignore_index):
         losses, lse = load_extension().vocab_loss(hidden, weight, targets, ignore_index, wscale, out_group)
-        ctx.save_for_backward(hidden, weight, wscale, targets, lse)
+        keep(ctx, hidden, weight, wscale, targets, lse)
         ctx.out_group, ctx.ignore_index = out_group, ignore_index
         return losses
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad):
-        hidden, weight, wscale, targets, lse = ctx.saved_tensors
+        hidden, weight, wscale, targets, lse = kept(ctx)
         of_hidden, of_weight = load_extension().vocab_loss_grad(hidden, weight, targets, lse, grad, ctx.ignore_index, wscale,
                                                                 ctx.out_group, ctx.needs_input_grad[1])
         return of_hidden, of_weight, None, None, None, None

@@ -16,6 +16,7 @@ import torch.nn as nn
 from torch.autograd.function import once_differentiable
 
 from llmquant.hip.build import load_extension
+from llmquant.hip.ops import keep, kept
 from llmquant.quantizers.kernel import KernelQuantLinear
 
 
@@ -142,15 +143,15 @@ class _LoraAdd(torch.autograd.Function):
         ext = load_extension()
         low = torch.empty(x.shape[0], lora_a.shape[1], dtype=torch.float32, device=x.device)
         out = ext.lora_add(x, base, lora_a, lora_b, scaling, adapter, query_start, low=low)
-        kept, scale = (x, None) if save_bits == 16 else ext.quant_group_codes(x, 8, 128, False)
+        held, scale = (x, None) if save_bits == 16 else ext.quant_group_codes(x, 8, 128, False)
         # (the rows' adapters as they are now: select() writes the batch's in place)
-        ctx.save_for_backward(kept, scale, low, lora_a, lora_b, scaling, adapter.clone(), query_start)
+        keep(ctx, held, scale, low, lora_a, lora_b, scaling, adapter.clone(), query_start)
         return out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad):
-        x, scale, low, lora_a, lora_b, scaling, adapter, query_start = ctx.saved_tensors
+        x, scale, low, lora_a, lora_b, scaling, adapter, query_start = kept(ctx)
         of_x, of_a, of_b = load_extension().lora_grad(grad, x, low, lora_a, lora_b, scaling, adapter, query_start, x_scale=scale)
         return of_x, grad, of_a, of_b, None, None, None, None
 

@@ -15,6 +15,7 @@ import torch.nn as nn
 from llmquant.core.observers import group_view, pad_to_group
 from llmquant.core.scheme import QuantizationScheme
 from llmquant.hip.build import load_extension
+from llmquant.hip.ops import keep, kept
 from llmquant.packing.packing import pack_int4, unpack_int4
 from llmquant.quantizers.real import quantize_weight
 
@@ -139,13 +140,13 @@ class _FrozenCodes(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, bias, module):
         ctx.module = module
-        ctx.save_for_backward(module.qdata, module.wscale)   # (changed in place before the backward pass: an error, as for any weight)
+        keep(ctx, module.qdata, module.wscale)
         return module._frozen(x)
 
     @staticmethod
     def backward(ctx, grad):
         module, of_x, of_bias = ctx.module, None, None
-        qdata, wscale = ctx.saved_tensors
+        qdata, wscale = kept(ctx)
         rows = grad.reshape(-1, grad.shape[-1])
         if ctx.needs_input_grad[0]:
             group_size = module.padded_in_features // qdata.shape[1]

@@ -154,3 +154,29 @@ def test_a_training_step_behind_an_evaluation():
     assert bank.lora_a.grad[2].any() and bank.lora_b.grad[0].any() and not bank.lora_b.grad[1].any()
     batch.select([1, 1])
     assert not torch.equal(bank(x, base), want)
+
+
+def test_a_model_of_inference_mode_learns():
+    """Codes, scales, targets and starts that were made there have no gradient and are read by one."""
+    from llmquant.hip import vocab_cross_entropy
+    from llmquant.quantizers import KernelQuantLinear, add_adapters, use_adapters
+    from test_kernel_linear_derivatives import linear
+
+    torch.manual_seed(0)
+    plain = torch.nn.Sequential(linear(128, 256, 128, 8, bias=False, device="cuda"), linear(256, 512, 128, 4, bias=False, device="cuda"))
+    with torch.inference_mode():
+        parts = [linear(128, 256, 128, 8, bias=False, device="cuda"), linear(256, 512, 128, 4, bias=False, device="cuda")]
+        start, targets = torch.tensor([0, 5, 12], dtype=torch.int32, device="cuda"), torch.randint(0, 512, (12,), device="cuda")
+    model = torch.nn.Sequential(*parts)
+    assert isinstance(model[0], KernelQuantLinear) and model[0].qdata.is_inference() and targets.is_inference()
+    x = torch.randn(12, 128, device="cuda")
+    grads = []
+    for m, t, s in ((model, targets, start), (plain, targets.clone(), start.clone())):
+        torch.manual_seed(1)
+        add_adapters(m, rank=8, slots=2, targets="0", dtype=torch.float32)
+        torch.nn.init.normal_(m[0].adapters.lora_b)
+        use_adapters(m, [1, 0], s)
+        leaf = x.clone().requires_grad_()
+        vocab_cross_entropy(m[0](leaf), m[1], t).backward()
+        grads.append((leaf.grad, m[0].adapters.lora_a.grad, m[0].adapters.lora_b.grad))
+    assert all(torch.equal(a, b) and a.any() for a, b in zip(*grads))

@@ -134,3 +134,24 @@ def test_one_gradient_on_both_sides(rows):
             assert torch.equal(out, module(x))
         got, = torch.autograd.grad(out, y, way)
         assert ((got.double() - want).abs() <= (6 * 136 + 72) * 2.0 ** -24 * size + 2.0 ** -22 * size + 2.0 ** -23 * want.abs()).all()
+
+
+def test_codes_from_inference_mode(no_kernels):
+    """A model that was quantized in inference mode has gradients by its input."""
+    with torch.inference_mode():
+        module = linear(36, 10, 12, 8, bias=False)
+    assert module.qdata.is_inference()
+    x = torch.randn(6, 36, generator=torch.Generator().manual_seed(1), requires_grad=True)
+    got, = torch.autograd.grad(_FrozenCodes.apply(x, None, module), x, torch.ones(6, 10))
+    with torch.inference_mode():
+        want = torch.ones(6, 10) @ module._real_weight(torch.float32)
+    assert torch.allclose(got, want)
+
+
+def test_codes_written_before_the_backward_pass_are_an_error(no_kernels):
+    module = linear(36, 10, 12, 8)
+    x = torch.randn(6, 36, generator=torch.Generator().manual_seed(1), requires_grad=True)
+    out = _FrozenCodes.apply(x, module.bias, module)
+    module.qdata.zero_()
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        out.sum().backward()
