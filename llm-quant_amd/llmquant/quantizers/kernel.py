@@ -335,7 +335,7 @@ class KernelQuantLinear(nn.Module):
         14336 x 4096 int8 64 rows 201 for 229, 65 rows 289 for 261, 320 rows 835 for 640, 2048 rows 3088 for 3246; 4096 x 14336 16 rows 151 for 151, 32 rows 181
         for 164, 1024 rows 1658 for 1671; 4096 x 4096 512 rows 272 for 257, 1024 rows 466 for 484; 2048 x 2048 512 rows 140 for 87, 1024 rows 176 for 139, 2048 rows
         248 for 250; 512 x 2048 2048 rows 130 for 83."""
-        whole = self.scheme.weights.group_size % 8 == 0
+        whole = self.padded_in_features // self._buffers["qdata"].shape[1] % 8 == 0
         if whole and x.dtype in (torch.bfloat16, torch.float16):
             return False
         count = x.numel() // max(x.shape[-1], 1)

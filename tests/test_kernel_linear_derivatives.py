@@ -116,6 +116,9 @@ def test_where_the_gradient_is_torchs_own(no_kernels, inp, out, rows, dtype, pla
                                QuantizationScheme(weights=QuantizationArgs(num_bits=8, strategy="group", group_size=128), input_activations=None), inp)
     assert module._plain(torch.empty(rows, inp, dtype=dtype, device="meta")) == plain
     assert module._plain(torch.empty(1, rows, inp, dtype=dtype, device="meta")) == plain
+    a_scale_a_row = QuantizationScheme(weights=QuantizationArgs(num_bits=8, strategy="channel"), input_activations=None)
+    module = KernelQuantLinear(torch.zeros(out, 1, inp, dtype=torch.int8), torch.ones(out, 1), None, a_scale_a_row, inp)
+    assert module._plain(torch.empty(rows, inp, dtype=dtype, device="meta")) == plain
 
 
 @pytest.mark.gpu
