@@ -594,8 +594,8 @@ int llmq_kv_block_attention(const void* query, int64_t q_row_stride, const void*
  * matrix of the reference's many-rows branch (llmquant/quantizers/kernel.py:68-79; its autograd is PyTorch's). grad: [rows, N], row
  * stride in elements; qweight, wscale, keep_per_group (a multiple of 8) and out_group as for llmq_dequant_weight; grad_x: [rows, G *
  * keep_per_group], contiguous. N a multiple of 8, rows up to 2^20, 256 neighbouring rows of grad within 4 GiB. fp32 sums; fp32 operands as three
- * bfloat16 planes where rows are many (up to 2^-23 of a product is left out, an infinity becomes NaN). Tensors 16-byte aligned. workspace: llmq_wq_linear_grad_workspace_bytes(...) bytes, 16-byte aligned, needs no
- * clearing; calls that overlap in time need one each. */
+ * bfloat16 planes where rows are many (up to 2^-23 of a product is left out, an infinity becomes NaN). Tensors 16-byte aligned. workspace:
+ * llmq_wq_linear_grad_workspace_bytes(...) bytes, 16-byte aligned, needs no clearing; calls that overlap in time need one each. */
 size_t llmq_wq_linear_grad_workspace_bytes(int rows, int N, int G, int keep_per_group, int wformat, int dtype);
 int llmq_wq_linear_grad(const void* grad, int64_t grad_stride, const void* qweight, const float* wscale, void* grad_x,
                         void* workspace, size_t workspace_bytes, int rows, int N, int G, int gs, int keep_per_group,
@@ -609,8 +609,8 @@ int llmq_wq_linear_grad(const void* grad, int64_t grad_stride, const void* qweig
  * (dtype)(code * scale) and have no gradient. losses, lse, grad: fp32 [rows]. A row whose target is ignore_index has loss 0 and
  * no part in a gradient, whatever it holds; any other target outside [0, vocab) makes the row's loss NaN, its
  * gradient NaN and grad_weight NaN. lse: as llmq_vocab_loss gave it. Logits and sums in fp32; P is rounded to `dtype` (fp32: three bfloat16
- * planes as its other operands, which leave out up to 2^-23 of a product, few rows not at all), with grad scaled by a power of two, a row's own, or with grad_weight that of the largest |grad| (in fp16 entries keep their
- * bits down to 2^-28 of it, and a step of 2^-38 below); what that takes from a target's own entry is added to the gradients
+ * planes as its other operands, which leave out up to 2^-23 of a product, few rows not at all), with grad scaled by a power of two, a row's own, or with
+ * grad_weight that of the largest |grad| (in fp16 entries keep their bits down to 2^-28 of it, and a step of 2^-38 below); what that takes from a target's own entry is added to the gradients
  * in fp32 (grad_weight: rounded to `dtype` again). Gradients are rounded once. hidden_size a multiple of 8, up
  * to 65536; rows up to 2^20 (256 neighbouring ones of hidden within 4 GiB, for the loss), vocab up to 2^24; tensors 16-byte aligned. No rows: nothing is
  * written (grad_weight neither). workspace: ..._workspace_bytes(...) bytes, 16-byte aligned, needs no clearing; calls that overlap in time need one each. */
@@ -633,8 +633,8 @@ int llmq_vocab_loss_grad(const void* hidden, int64_t hidden_stride, const void* 
  * [sequences + 1], not decreasing; NULL: row b, rows == sequences); rows of no sequence are base. low_or_null: fp32 [rows, rank],
  * zeros without an adapter; the gradient wants it. Sums in fp32, out rounded once; for 16-bit types low enters the second product as
  * two bfloat16 (16 bits of it; fp16: two fp16 with an exponent a row, 22 bits; one row a sequence beside small banks: as it is), du and, for grad_b, low
- * likewise (grad_a, grad_b: two bfloat16): results may be NaN where x, low or du has an infinity, whatever the definition makes of it. rank a multiple of 8 from 8 to 128 (an adapter of a lower rank has zeros behind it), in and out
- * multiples of 8; 32 neighbouring rows of x (of grad, backwards) within 4 GiB; tensors 16-byte aligned. workspace: ..._workspace_bytes(...) bytes
+ * likewise (grad_a, grad_b: two bfloat16): results may be NaN where x, low or du has an infinity, whatever the definition makes of it. rank a multiple
+ * of 8 from 8 to 128 (an adapter of a lower rank has zeros behind it), in and out multiples of 8; 32 neighbouring rows of x (of grad, backwards) within 4 GiB; tensors 16-byte aligned. workspace: ..._workspace_bytes(...) bytes
  * (ragged: whether there is a query_start), 16-byte aligned, needs no clearing; calls that overlap in time need one each.
  *
  * llmq_lora_grad: from grad, the gradient of out,

@@ -28,7 +28,10 @@ def _losses(model, input_ids: torch.Tensor, hidden: torch.Tensor) -> torch.Tenso
 
 
 def _decoded(model, input_ids: torch.Tensor) -> torch.Tensor:
-    """The decoder's hidden states [batch, length, hidden size]."""
+    """The decoder's hidden states [batch, length, hidden size], of a model whose logits are its head's product with them (not asked in a capture, which can
+    wait for no answer)."""
+    if input_ids.is_cuda and torch.cuda.is_current_stream_capturing():
+        return model.get_decoder()(input_ids=input_ids, use_cache=False).last_hidden_state
     if "logits_to_keep" not in inspect.signature(model.forward).parameters:   # (all logits or none: a token tells)
         _check_logits(model, model.get_decoder()(input_ids=input_ids[:1, :1], use_cache=False).last_hidden_state,
                       model(input_ids=input_ids[:1, :1], use_cache=False).logits)
